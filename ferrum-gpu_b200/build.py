@@ -1,7 +1,7 @@
 """Build the ferrum-gpu B200 libraries in-tree.
 
 Outputs (next to the Python package so they travel with the source tree):
-  ferrum_gpu/libferrum_fft.so                    C ABI (include/ferrum_fft.h) + sm_100a kernels
+  ferrum_gpu/libferrum_fft.so                    C ABI (include/ferrum_fft.h, ferrum_seq.h) + sm_100a kernels
   ferrum_gpu/_native.<python-ext-suffix>         pybind11 module over the C ABI
 
 Every .cu is compiled with
@@ -42,13 +42,19 @@ NVCC_FLAGS = ["-std=c++17", "-O3", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompil
 
 CU_SOURCES = ["launch_rows.cu", "launch_pass.cu", "launch_misc.cu", "launch_tile.cu", "capi.cu", "host_path.cu", "dist.cu",
               "no_alloc.cu", "substrate.cu"]
+# Sequence operators (include/ferrum_seq.h).
+SEQ_SOURCES = ["seq_common.cu", "conv1d.cu", "scan_fwd.cu", "scan_bwd.cu", "norm.cu",
+               "long_conv.cu"]
 LIB = os.path.join(PKG, "libferrum_fft.so")
 EXT = os.path.join(PKG, "_native" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 
-def _headers() -> list[str]:
-    return (glob.glob(os.path.join(CSRC, "*.h")) + glob.glob(os.path.join(CSRC, "*.cuh"))
-            + glob.glob(os.path.join(INCLUDE, "*.h")))
+def _headers(seq: bool = False) -> list[str]:
+    fft = (glob.glob(os.path.join(CSRC, "*.h")) + glob.glob(os.path.join(CSRC, "*.cuh"))
+           + [os.path.join(INCLUDE, "ferrum_fft.h")])
+    if not seq:
+        return fft
+    return fft + glob.glob(os.path.join(CSRC, "seq", "*.cuh")) + [os.path.join(INCLUDE, "ferrum_seq.h")]
 
 
 def _stale(target: str, deps: list[str]) -> bool:
@@ -67,14 +73,15 @@ def _run(cmd: list[str]) -> None:
 
 def _compile_cu(src: str, force: bool) -> str:
     obj = os.path.join(BUILD, os.path.basename(src).replace(".cu", ".o"))
-    if force or _stale(obj, [src] + _headers()):
+    if force or _stale(obj, [src] + _headers(os.path.dirname(src) != CSRC)):
         _run([NVCC] + NVCC_FLAGS + ["-c", src, "-o", obj])
     return obj
 
 
 def build(jobs: int = 4, force: bool = False) -> None:
     os.makedirs(BUILD, exist_ok=True)
-    srcs = [os.path.join(CSRC, s) for s in CU_SOURCES]
+    srcs = ([os.path.join(CSRC, s) for s in CU_SOURCES]
+            + [os.path.join(CSRC, "seq", s) for s in SEQ_SOURCES])
     with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
         objs = list(ex.map(lambda s: _compile_cu(s, force), srcs))
     if force or _stale(LIB, objs):

@@ -1,0 +1,176 @@
+// Shared pieces of the sequence operators (include/ferrum_seq.h): element
+// types, the activation functions, reductions, and the host-side argument
+// checks, workspaces and error handling of their C entry points.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <exception>
+#include <new>
+#include <string>
+
+#include "../../../include/ferrum_seq.h"
+#include "../launch_common.cuh"
+#include "../runtime.h"
+
+namespace ferrum {
+namespace seq {
+
+using launch_detail::ceil_div;
+
+// ---------------------------------------------------------------- device
+template <class T>
+__device__ __forceinline__ float to_f(T v) { return (float)v; }
+template <>
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+template <>
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+template <class T>
+__device__ __forceinline__ T from_f(float v) { return (T)v; }
+template <>
+__device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// 1 / (1 + e^-x). For x below about -88 e^-x overflows to infinity and the
+// quotient is 0, the limit.
+__device__ __forceinline__ float sigmoid_f(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
+
+// Sum over the 32 lanes, in every lane, in a fixed order.
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// ---------------------------------------------------------------- host
+// A (batch, length, channels) argument with its element type.
+template <class T>
+struct Rows {
+  T* p;
+  int64_t sb, st;
+  __device__ __forceinline__ T* at(int64_t b, int64_t t) const { return p + b * sb + t * st; }
+  __host__ __device__ explicit operator bool() const { return p != nullptr; }
+};
+template <class T>
+Rows<T> rows_of(const ferrum_rows& r) { return Rows<T>{(T*)r.ptr, r.batch_stride, r.row_stride}; }
+
+inline size_t dtype_size(int dtype) { return dtype == FERRUM_F32 ? 4 : 2; }
+
+// Workspace from the device's stream-ordered pool, returned to it on scope
+// exit (in stream order, so after the work enqueued in between).
+class PoolBuffer {
+ public:
+  PoolBuffer(ferrum_device* dev, size_t bytes, cudaStream_t stream) : stream_(stream) {
+    if (bytes > 0) status_ = cudaMallocFromPoolAsync(&p_, bytes, dev->pool, stream);
+  }
+  ~PoolBuffer() {
+    if (p_) (void)cudaFreeAsync(p_, stream_);
+  }
+  PoolBuffer(const PoolBuffer&) = delete;
+  PoolBuffer& operator=(const PoolBuffer&) = delete;
+  cudaError_t status() const { return status_; }
+  template <class T>
+  T* as() const { return (T*)p_; }
+
+ private:
+  void* p_ = nullptr;
+  cudaStream_t stream_;
+  cudaError_t status_ = cudaSuccess;
+};
+
+inline ferrum_status invalid(const char* what, const std::string& msg) {
+  return set_error(FERRUM_ERR_INVALID_ARG, std::string(what) + ": " + msg);
+}
+
+inline bool aligned(const void* p, size_t n) { return ((uintptr_t)p % n) == 0; }
+
+// Common checks of an entry point: handle, argument block, element type.
+template <class Args>
+ferrum_status check_args(const ferrum_device* dev, const Args* a, const char* what) {
+  if (dev == nullptr || dev->tables == nullptr)
+    return set_error(FERRUM_ERR_INVALID_ARG, "device handle is NULL or destroyed");
+  if (a == nullptr) return invalid(what, "args is NULL");
+  if (a->struct_size != sizeof(Args))
+    return invalid(what, "struct_size is " + std::to_string(a->struct_size) + ", expected " +
+                             std::to_string(sizeof(Args)));
+  if (a->dtype != FERRUM_F32 && a->dtype != FERRUM_F16 && a->dtype != FERRUM_BF16)
+    return invalid(what, "dtype must be FERRUM_F32, FERRUM_F16 or FERRUM_BF16, got " +
+                             std::to_string(a->dtype));
+  return FERRUM_OK;
+}
+
+// An array argument: present (unless `optional`) and aligned to its element.
+inline ferrum_status check_ptr(const void* p, size_t align, bool optional, const char* what,
+                               const char* name) {
+  if (p == nullptr) {
+    if (optional) return FERRUM_OK;
+    return invalid(what, std::string(name) + " is NULL");
+  }
+  if (!aligned(p, align))
+    return invalid(what, std::string(name) + " must be " + std::to_string(align) + "-byte aligned");
+  return FERRUM_OK;
+}
+
+// Most values one array of a call may hold, as for the transforms.
+constexpr int64_t kMaxElems = (int64_t)1 << kMaxLogElems;
+
+// product of sizes, or -1 above kMaxElems
+inline int64_t bounded_product(std::initializer_list<size_t> f) {
+  int64_t p = 1;
+  for (size_t v : f) {
+    if (v == 0) return 0;
+    if (v > (size_t)kMaxElems || p > kMaxElems / (int64_t)v) return -1;
+    p *= (int64_t)v;
+  }
+  return p;
+}
+
+// Runs a C entry's body: makes the device current, and turns anything the
+// body throws into a status (nothing may unwind through a C caller).
+template <class F>
+ferrum_status guarded(const char* what, F body) noexcept {
+  try {
+    clear_error();
+    return body();
+  } catch (const std::bad_alloc&) {
+    try {
+      return set_error(FERRUM_ERR_ALLOC, std::string(what) + ": out of host memory");
+    } catch (...) {
+      return FERRUM_ERR_ALLOC;
+    }
+  } catch (const std::exception& e) {
+    try {
+      return set_error(FERRUM_ERR_CUDA, std::string(what) + ": " + e.what());
+    } catch (...) {
+      return FERRUM_ERR_CUDA;
+    }
+  } catch (...) {
+    return FERRUM_ERR_CUDA;
+  }
+}
+
+inline ferrum_status launched(const char* what) {
+  cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? FERRUM_OK : cuda_error(e, what);
+}
+
+// Calls f with a value of the element type `dtype` names.
+template <class F>
+ferrum_status with_dtype(int dtype, F f) {
+  if (dtype == FERRUM_F32) return f(float());
+  if (dtype == FERRUM_F16) return f(__half());
+  return f(__nv_bfloat16());
+}
+
+// out[i] = sum over r < rows of part[r * n + i], in row order (a fixed order,
+// so results do not depend on scheduling).
+cudaError_t launch_sum_rows(const float* part, int64_t rows, int64_t n, float* out,
+                            cudaStream_t stream);
+
+}  // namespace seq
+}  // namespace ferrum
