@@ -1,85 +1,344 @@
 // Selective state space scan over (batch, length, channels), forward:
 //   dt = softplus(delta + bias),  h[n] = exp(dt A[n]) h[n] + dt u B[n],
 //   out = (sum_n h[n] C[n] + D u) * silu(z)
-// One thread owns one channel of one sequence and its N states in registers
-// and walks the steps; lanes span adjacent channels, so u, delta, z and out
-// are read and written in whole segments and B, C are broadcast.
+//
+// A step maps h to a h + b, and such maps compose: (a2, b2) after (a1, b1) is
+// (a2 a1, a2 b1 + b2). So the steps of one channel are split over G lanes, 8
+// consecutive steps each: a lane composes its 8 maps, the G lanes scan the
+// compositions by shuffles (log2 G rounds), and each lane, now knowing the
+// state in front of its steps, walks them again for the outputs, with the
+// same a and b still in registers. Each exponential is computed once, which
+// matters because they bound the kernel: N per value on the special-function
+// unit (16 a clock and SM) against about 6 N FP32 operations (128 a clock).
+// Splitting the axis over blocks instead would need the exponentials twice.
+// A block holds W * 32 / G channels and walks the sequence in pieces of 8 G
+// steps; u and dt are transposed through shared memory (global rows run over
+// channels, a lane needs its channel's steps), B and C rows are shared by all
+// channels of the block. States go in fours: 4 chains in flight, 16-byte
+// reads of B and C, and the two-wide FP32 instructions over pairs of states.
 #include "scan.cuh"
 
 namespace ferrum {
 namespace seq {
 namespace {
 
-constexpr int kThreads = 64;
+constexpr int kLaneSteps = 8;
 
-template <class T, int N>
-__global__ void __launch_bounds__(kThreads)
+template <int G, int W>
+struct FwdCfg {
+  static constexpr int THREADS = W * 32;
+  static constexpr int CH = W * 32 / G;           // channels per block
+  static constexpr int CK = kLaneSteps * G;       // steps per piece
+  static constexpr int LD = CK + 4;               // channel stride of the transposed tiles
+  // B and C tiles: row t at t * NP + (t / 8) * 4, so that the lanes of a
+  // channel, 8 rows apart, read from different banks
+  static constexpr int bc_floats(int np) { return CK * np + (CK / 8) * 4; }
+  static size_t smem_bytes(int np) {
+    return sizeof(float) * (size_t)(2 * CH * LD + 2 * bc_floats(np) + 2 * CH * np);
+  }
+};
+
+template <class T, int G, int W>
+__global__ void __launch_bounds__(W * 32, W == 4 ? 3 : 1)
 scan_fwd_kernel(ScanIn<T> in, Rows<T> out, float* fin, float* __restrict__ saved, ScanSizes s,
-                int64_t col_blocks) {
-  const int64_t b = blockIdx.x / col_blocks;
-  const int64_t d = (blockIdx.x % col_blocks) * kThreads + threadIdx.x;
-  if (d >= s.channels) return;
-  const int64_t len = scan_length(in.lengths, b, s.length), g = d / s.per_group;
-  const int64_t sd = (b * s.channels + d) * s.states;
-  float h[N], a2[N];
-#pragma unroll
-  for (int n = 0; n < N; ++n) {
-    a2[n] = n < s.states ? in.A[d * s.states + n] * kLog2e : 0.f;
-    h[n] = (in.initial && n < s.states) ? in.initial[sd + n] : 0.f;
+                int lnp, int64_t col_blocks) {
+  using C = FwdCfg<G, W>;
+  constexpr int CH = C::CH, CK = C::CK, LD = C::LD;
+  extern __shared__ float4 smem4[];
+  const int NP = 1 << lnp;
+  float* sU = (float*)smem4;
+  float* sDt = sU + CH * LD;
+  float* sB = sDt + CH * LD;
+  float* sC = sB + C::bc_floats(NP);
+  float* sA = sC + C::bc_floats(NP);   // A log2 e
+  float* sH = sA + CH * NP;            // the state in front of the piece
+
+  int64_t q = blockIdx.x;
+  const int64_t cb = q % col_blocks;
+  q /= col_blocks;
+  const int64_t grp = q % s.groups, b = q / s.groups;
+  const int64_t d0 = grp * s.per_group + cb * CH;
+  const int nch = (int)(s.per_group - cb * CH < CH ? s.per_group - cb * CH : CH);
+  const int64_t len = scan_length(in.lengths, b, s.length);
+  const int tid = threadIdx.x, lane = tid & 31, g = lane % G;
+  const int c = (tid >> 5) * (32 / G) + lane / G;
+
+  for (int i = tid; i < CH * NP; i += C::THREADS) {
+    const int cc = i >> lnp, n = i & (NP - 1);
+    const bool ok = cc < nch && n < s.states;
+    const int64_t o = (d0 + cc) * s.states + n;
+    sA[i] = ok ? in.A[o] * kLog2e : 0.f;
+    sH[i] = (ok && in.initial) ? in.initial[b * s.channels * s.states + o] : 0.f;
   }
-  const float skip = in.D ? in.D[d] : 0.f, bias = in.bias ? in.bias[d] : 0.f;
-  for (int64_t t = 0; t < s.length; ++t) {
-    if (saved != nullptr && t % kSaveSteps == 0) {
-      float* o = saved + ((b * s.saves + t / kSaveSteps) * s.channels + d) * s.states;
+  const int tc = tid % CH;             // this thread's channel in the tile copies
+  const bool tok = tc < nch;
+  const float bias = (in.bias && tok) ? in.bias[d0 + tc] : 0.f;
+  const float skip = (in.D && c < nch) ? in.D[d0 + c] : 0.f;
+
+  for (int64_t t0 = 0; t0 < len; t0 += CK) {
 #pragma unroll
-      for (int n = 0; n < N; ++n)
-        if (n < s.states) o[n] = h[n];
-    }
-    if (t >= len) {
-      out.at(b, t)[d] = from_f<T>(0.f);
-      continue;
-    }
-    const float x = to_f(in.u.at(b, t)[d]);
-    float dt = to_f(in.delta.at(b, t)[d]) + bias;
-    if (s.softplus) dt = softplus_f(dt);
-    const float dx = dt * x;
-    const T* Bt = in.B.at(b, t) + g * in.B_group;
-    const T* Ct = in.C.at(b, t) + g * in.C_group;
-    float y = skip * x;
-#pragma unroll
-    for (int n = 0; n < N; ++n)
-      if (n < s.states) {
-        h[n] = fmaf(exp2f(dt * a2[n]), h[n], dx * to_f(Bt[n]));
-        y = fmaf(h[n], to_f(Ct[n]), y);
+    for (int i = 0; i < CK * CH / C::THREADS; ++i) {
+      const int t = i * (C::THREADS / CH) + tid / CH;
+      float x = 0.f, dt = 0.f;         // past the end: a = 1, b = 0
+      if (tok && t0 + t < len) {
+        x = to_f(in.u.at(b, t0 + t)[d0 + tc]);
+        dt = to_f(in.delta.at(b, t0 + t)[d0 + tc]) + bias;
+        if (s.softplus) dt = softplus_f(dt);
       }
-    if (in.z) {
-      const float z = to_f(in.z.at(b, t)[d]);
-      y *= z * sigmoid_f(z);
+      sU[tc * LD + t] = x;
+      sDt[tc * LD + t] = dt;
     }
-    out.at(b, t)[d] = from_f<T>(y);
-  }
-  if (fin != nullptr)
+    for (int i = tid; i < CK * NP; i += C::THREADS) {
+      const int t = i >> lnp, n = i & (NP - 1);
+      float vb = 0.f, vc = 0.f;
+      if (n < s.states && t0 + t < len) {
+        vb = to_f(in.B.at(b, t0 + t)[grp * in.B_group + n]);
+        vc = to_f(in.C.at(b, t0 + t)[grp * in.C_group + n]);
+      }
+      sB[i + (t >> 3) * 4] = vb;
+      sC[i + (t >> 3) * 4] = vc;
+    }
+    __syncthreads();
+
+    float dt[8], du[8];
+    f2 y[8];
+    float* mine = sU + c * LD + g * 8;
+    {
+      const float* pd = sDt + c * LD + g * 8;
 #pragma unroll
-    for (int n = 0; n < N; ++n)
-      if (n < s.states) fin[sd + n] = h[n];
+      for (int i = 0; i < 8; ++i) dt[i] = pd[i], du[i] = dt[i] * mine[i], y[i] = 0;
+    }
+    const bool save = saved != nullptr && ((t0 >> 3) + g) % (kSaveSteps / 8) == 0 && c < nch &&
+                      t0 + g * 8 < s.length;
+    float* so = save ? saved + ((b * s.saves + (t0 + g * 8) / kSaveSteps) * s.channels + d0 + c) *
+                                   s.states
+                     : nullptr;
+    for (int n = 0; n < NP; n += 4) {
+      const float4 A4 = *(const float4*)(sA + c * NP + n);
+      const float* pb = sB + g * (8 * NP + 4) + n;
+      const float* pc = sC + g * (8 * NP + 4) + n;
+      f2 a0[8], a1[8], b0[8], b1[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float4 B4 = *(const float4*)(pb + i * NP);
+        a0[i] = pack(ex2(dt[i] * A4.x), ex2(dt[i] * A4.y));
+        a1[i] = pack(ex2(dt[i] * A4.z), ex2(dt[i] * A4.w));
+        const f2 w = pack(du[i], du[i]);
+        b0[i] = mul2(w, pack(B4.x, B4.y));
+        b1[i] = mul2(w, pack(B4.z, B4.w));
+      }
+      f2 P0 = a0[0], P1 = a1[0], H0 = b0[0], H1 = b1[0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) {
+        H0 = fma2(a0[i], H0, b0[i]), P0 = mul2(a0[i], P0);
+        H1 = fma2(a1[i], H1, b1[i]), P1 = mul2(a1[i], P1);
+      }
+      float4* carry = (float4*)(sH + c * NP + n);
+      const float4 h4 = *carry;
+      f2 h0 = pack(h4.x, h4.y), h1 = pack(h4.z, h4.w);
+      if (g == 0) H0 = fma2(P0, h0, H0), H1 = fma2(P1, h1, H1);
+#pragma unroll
+      for (int o = 1; o < G; o <<= 1) {
+        const f2 u0 = __shfl_up_sync(0xffffffffu, H0, o, G);
+        const f2 u1 = __shfl_up_sync(0xffffffffu, H1, o, G);
+        if (g >= o) H0 = fma2(P0, u0, H0), H1 = fma2(P1, u1, H1);
+        if (2 * o < G) {
+          const f2 v0 = __shfl_up_sync(0xffffffffu, P0, o, G);
+          const f2 v1 = __shfl_up_sync(0xffffffffu, P1, o, G);
+          if (g >= o) P0 = mul2(P0, v0), P1 = mul2(P1, v1);
+        }
+      }
+      // the state in front of this lane's steps; lane 0 gets the piece's last
+      const f2 u0 = __shfl_sync(0xffffffffu, H0, (g + G - 1) % G, G);
+      const f2 u1 = __shfl_sync(0xffffffffu, H1, (g + G - 1) % G, G);
+      if (g == 0) {
+        const float2 p = unpack(u0), r = unpack(u1);
+        *carry = make_float4(p.x, p.y, r.x, r.y);
+      } else {
+        h0 = u0, h1 = u1;
+      }
+      if (save) {
+        const float2 p = unpack(h0), r = unpack(h1);
+        if (n + 0 < s.states) so[n + 0] = p.x;
+        if (n + 1 < s.states) so[n + 1] = p.y;
+        if (n + 2 < s.states) so[n + 2] = r.x;
+        if (n + 3 < s.states) so[n + 3] = r.y;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float4 C4 = *(const float4*)(pc + i * NP);
+        h0 = fma2(a0[i], h0, b0[i]);
+        h1 = fma2(a1[i], h1, b1[i]);
+        y[i] = fma2(h0, pack(C4.x, C4.y), y[i]);
+        y[i] = fma2(h1, pack(C4.z, C4.w), y[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float2 v = unpack(y[i]);
+      mine[i] = fmaf(skip, mine[i], v.x + v.y);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < CK * CH / C::THREADS; ++i) {
+      const int t = i * (C::THREADS / CH) + tid / CH;
+      if (tok && t0 + t < s.length) {
+        float v = 0.f;
+        if (t0 + t < len) {
+          v = sU[tc * LD + t];
+          if (in.z) {
+            const float z = to_f(in.z.at(b, t0 + t)[d0 + tc]);
+            v *= z * sigmoid_f(z);
+          }
+        }
+        out.at(b, t0 + t)[d0 + tc] = from_f<T>(v);
+      }
+    }
+    __syncthreads();
+  }
+  // steps past the sequence's last piece
+  if (tok)
+    for (int64_t t = (len + CK - 1) / CK * CK + tid / CH; t < s.length; t += C::THREADS / CH)
+      out.at(b, t)[d0 + tc] = from_f<T>(0.f);
+  if (fin != nullptr) {
+    __syncthreads();
+    for (int i = tid; i < CH * NP; i += C::THREADS) {
+      const int cc = i >> lnp, n = i & (NP - 1);
+      if (cc < nch && n < s.states)
+        fin[(b * s.channels + d0 + cc) * s.states + n] = sH[i];
+    }
+  }
+}
+
+// One step: every value of the state is read and written once, which is all
+// the traffic that counts. L lanes share a channel, 4 states each (16-byte
+// accesses), and add up the output by shuffles.
+template <class T, int L>
+__global__ void __launch_bounds__(128)
+scan_step_kernel(ScanIn<T> in, Rows<T> out, float* fin, ScanSizes s, bool vec) {
+  const int64_t i = ((int64_t)blockIdx.x * 128 + threadIdx.x) / L;
+  const int n0 = (threadIdx.x % L) * 4;
+  const bool live = i < s.batch * s.channels;
+  const int64_t b = live ? i / s.channels : 0, d = live ? i % s.channels : 0, g = d / s.per_group;
+  const int64_t so = (b * s.channels + d) * s.states + n0;
+  const float *pa = in.A + d * s.states + n0, *ph = in.initial + so;
+  const T *pb = in.B.at(b, 0) + g * in.B_group + n0, *pc = in.C.at(b, 0) + g * in.C_group + n0;
+  float h[4], a[4], Bv[4], Cv[4];
+  if (vec) {
+    const float4 x = *(const float4*)ph, w = *(const float4*)pa;
+    h[0] = x.x, h[1] = x.y, h[2] = x.z, h[3] = x.w;
+    a[0] = w.x, a[1] = w.y, a[2] = w.z, a[3] = w.w;
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const bool ok = n0 + k < s.states;
+    if (!vec) h[k] = ok ? ph[k] : 0.f, a[k] = ok ? pa[k] : 0.f;
+    Bv[k] = ok ? to_f(pb[k]) : 0.f;
+    Cv[k] = ok ? to_f(pc[k]) : 0.f;
+  }
+  const float x = to_f(in.u.at(b, 0)[d]);
+  float dt = to_f(in.delta.at(b, 0)[d]) + (in.bias ? in.bias[d] : 0.f);
+  const float z = in.z ? to_f(in.z.at(b, 0)[d]) : 0.f;
+  const float skip = in.D ? in.D[d] : 0.f;
+  const bool run = in.lengths == nullptr || in.lengths[b] > 0;
+  if (s.softplus) dt = softplus_f(dt);
+  float y = 0.f;
+  if (run) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      h[k] = fmaf(ex2(dt * (a[k] * kLog2e)), h[k], dt * x * Bv[k]);
+      y = fmaf(h[k], Cv[k], y);
+    }
+  }
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o, L);
+  if (!live) return;
+  if (vec) {
+    *(float4*)(fin + so) = make_float4(h[0], h[1], h[2], h[3]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (n0 + k < s.states) fin[so + k] = h[k];
+  }
+  if (n0 == 0) {
+    y = fmaf(skip, x, y);
+    if (in.z) y *= z * sigmoid_f(z);
+    out.at(b, 0)[d] = from_f<T>(run ? y : 0.f);
+  }
+}
+
+template <class T, int G, int W>
+ferrum_status run_fwd(const ferrum_scan_args* a, const ScanSizes& s, int lnp, cudaStream_t stream,
+                      const char* what) {
+  using C = FwdCfg<G, W>;
+  static std::atomic<uint64_t> done{0};
+  const int64_t col_blocks = ceil_div(s.per_group, C::CH);
+  const int64_t blocks = s.batch * s.groups * col_blocks;
+  if (blocks > 0x7fffffff) return invalid(what, "too many blocks for one launch");
+  const size_t smem = C::smem_bytes(1 << lnp);
+  cudaError_t e = launch_detail::ensure_smem(scan_fwd_kernel<T, G, W>, C::smem_bytes(64), done);
+  if (e != cudaSuccess) return cuda_error(e, what);
+  launch_detail::clear_stale_error();
+  scan_fwd_kernel<T, G, W><<<(unsigned)blocks, C::THREADS, smem, stream>>>(
+      scan_in<T>(a), rows_of<T>(a->out), a->final_state, a->saved_states, s, lnp, col_blocks);
+  return launched(what);
+}
+
+int log_states(int states) {   // log2 of the padded number of states, at least 2
+  int l = 2;
+  while ((1 << l) < states) ++l;
+  return l;
 }
 
 ferrum_status scan_fwd(ferrum_device* dev, const ferrum_scan_args* a, cudaStream_t stream,
                        const char* what) {
   if (a->batch == 0 || a->channels == 0) return FERRUM_OK;
   const ScanSizes s = scan_sizes(a);
-  const int64_t col_blocks = ceil_div(s.channels, kThreads), blocks = s.batch * col_blocks;
+  DeviceGuard guard(dev->ordinal);
+  if (guard.status() != cudaSuccess) return cuda_error(guard.status(), "cudaSetDevice");
+  const int lnp = log_states(s.states);
+  // Lanes per channel: few keep the scan short, many give enough warps where
+  // there are few channels. The least of 4..32 that reaches 12 warps an SM,
+  // within the sequence's length and (B, C tiles) shared memory.
+  int G = 4;
+  while (G < 32 && s.batch * s.channels * G / 32 < 148 * 12 && G * kLaneSteps < s.length &&
+         2 * G * kLaneSteps * (1 << lnp) * 8 <= 96 * 1024)
+    G *= 2;
+  return with_dtype(a->dtype, [&](auto tag) {
+    using T = decltype(tag);
+    if (G == 4) return run_fwd<T, 4, 4>(a, s, lnp, stream, what);
+    if (G == 8) return run_fwd<T, 8, 4>(a, s, lnp, stream, what);
+    if (G == 16) return run_fwd<T, 16, 8>(a, s, lnp, stream, what);
+    return run_fwd<T, 32, 8>(a, s, lnp, stream, what);
+  });
+}
+
+ferrum_status scan_step(ferrum_device* dev, const ferrum_scan_args* a, cudaStream_t stream,
+                        const char* what) {
+  if (a->batch == 0 || a->channels == 0) return FERRUM_OK;
+  const ScanSizes s = scan_sizes(a);
+  const int lanes = 1 << (log_states(s.states) - 2);
+  const int64_t blocks = ceil_div(s.batch * s.channels * lanes, 128);
   if (blocks > 0x7fffffff) return invalid(what, "too many blocks for one launch");
+  const bool vec = s.states % 4 == 0 && s.states == 4 * lanes && aligned(a->A, 16) &&
+                   aligned(a->initial_state, 16) && aligned(a->final_state, 16);
   DeviceGuard guard(dev->ordinal);
   if (guard.status() != cudaSuccess) return cuda_error(guard.status(), "cudaSetDevice");
   return with_dtype(a->dtype, [&](auto tag) {
     using T = decltype(tag);
-    return with_states(s.states, [&](auto n) {
+    auto go = [&](auto l) {
       launch_detail::clear_stale_error();
-      scan_fwd_kernel<T, decltype(n)::value><<<(unsigned)blocks, kThreads, 0, stream>>>(
-          scan_in<T>(a), rows_of<T>(a->out), a->final_state, a->saved_states, s, col_blocks);
+      scan_step_kernel<T, decltype(l)::value><<<(unsigned)blocks, 128, 0, stream>>>(
+          scan_in<T>(a), rows_of<T>(a->out), a->final_state, s, vec);
       return launched(what);
-    });
+    };
+    switch (lanes) {
+      case 1: return go(std::integral_constant<int, 1>());
+      case 2: return go(std::integral_constant<int, 2>());
+      case 4: return go(std::integral_constant<int, 4>());
+      case 8: return go(std::integral_constant<int, 8>());
+      default: return go(std::integral_constant<int, 16>());
+    }
   });
 }
 
@@ -151,7 +410,7 @@ ferrum_status ferrum_selective_scan_step(ferrum_device* dev, const ferrum_scan_a
     if (a->batch > 0 && a->channels > 0 &&
         (a->initial_state == nullptr || a->final_state == nullptr))
       return invalid(what, "initial_state and final_state are required");
-    return scan_fwd(dev, a, (cudaStream_t)stream, what);
+    return scan_step(dev, a, (cudaStream_t)stream, what);
   });
 }
 
