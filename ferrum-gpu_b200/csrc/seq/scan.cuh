@@ -79,6 +79,71 @@ __device__ __forceinline__ f2 mul2(f2 a, f2 b) {
   return r;
 }
 
+// Asynchronous copies from global to shared memory, `bytes` of the unit read
+// and the rest zeroed.
+template <int UNIT>
+__device__ __forceinline__ void cp_async(void* dst, const void* src, int bytes) {
+  const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
+  if constexpr (UNIT == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src), "r"(bytes));
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(d), "l"(src), "r"(bytes));
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;"); }
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// A piece of a (steps, columns) array in shared memory, in its own type: row
+// t at t * COLS elements plus 16 bytes for every 8 rows, so that lanes 8 rows
+// apart meet different banks.
+template <class T, int COLS>
+struct Piece {
+  static constexpr int SKEW = 16 / (int)sizeof(T);
+  __host__ __device__ static constexpr int size(int rows) { return rows * COLS + rows / 8 * SKEW; }
+  __device__ static __forceinline__ int at(int t, int c) { return t * COLS + (t >> 3) * SKEW + c; }
+};
+
+// How the rows of a call's arrays can be copied: 16 bytes or 4 bytes at a
+// time, or (0) by single elements where a row starts at an odd element.
+enum { kCopyScalar = 0, kCopy4 = 4, kCopy16 = 16 };
+
+template <class T>
+int copy_unit(const ferrum_rows& r, int64_t extra = 0) {
+  const uintptr_t v = (uintptr_t)r.ptr | (uintptr_t)(r.batch_stride * (int64_t)sizeof(T)) |
+                      (uintptr_t)(r.row_stride * (int64_t)sizeof(T)) |
+                      (uintptr_t)(extra * (int64_t)sizeof(T));
+  return v % 16 == 0 ? kCopy16 : (v % 4 == 0 ? kCopy4 : kCopyScalar);
+}
+
+// Rows [0, ROWS) of columns [0, cols) of an array to a piece, rows from
+// `rows` and columns from `cols` on as zeros. THREADS threads take part; the
+// 16- and 4-byte forms are asynchronous.
+template <class T, int ROWS, int COLS, int THREADS, int UNIT>
+__device__ __forceinline__ void copy_units(T* dst, const T* src, int64_t stride, int rows, int cols,
+                                           int tid) {
+  constexpr int E = UNIT / (int)sizeof(T), PER = COLS / E;
+#pragma unroll 4
+  for (int i = tid; i < ROWS * PER; i += THREADS) {
+    const int t = i / PER, c = (i % PER) * E;
+    int n = t < rows ? cols - c : 0;
+    n = n < 0 ? 0 : (n > E ? E : n);
+    cp_async<UNIT>(dst + Piece<T, COLS>::at(t, c), n > 0 ? src + t * stride + c : src,
+                   n * (int)sizeof(T));
+  }
+}
+template <class T, int ROWS, int COLS, int THREADS>
+__device__ __forceinline__ void copy_piece(T* dst, const T* src, int64_t stride, int rows, int cols,
+                                           int unit, int tid) {
+  if constexpr (COLS * sizeof(T) >= 16) {
+    if (unit == kCopy16) return copy_units<T, ROWS, COLS, THREADS, 16>(dst, src, stride, rows, cols, tid);
+  }
+  if (unit != kCopyScalar)
+    return copy_units<T, ROWS, COLS, THREADS, 4>(dst, src, stride, rows, cols, tid);
+  for (int i = tid; i < ROWS * COLS; i += THREADS) {
+    const int t = i / COLS, c = i % COLS;
+    dst[Piece<T, COLS>::at(t, c)] = (t < rows && c < cols) ? src[t * stride + c] : from_f<T>(0.f);
+  }
+}
+
 template <class T>
 ScanIn<T> scan_in(const ferrum_scan_args* a) {
   return ScanIn<T>{rows_of<T>(a->u), rows_of<T>(a->delta), rows_of<T>(a->z), rows_of<T>(a->B),

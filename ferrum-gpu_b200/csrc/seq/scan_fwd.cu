@@ -11,11 +11,15 @@
 // matters because they bound the kernel: N per value on the special-function
 // unit (16 a clock and SM) against about 6 N FP32 operations (128 a clock).
 // Splitting the axis over blocks instead would need the exponentials twice.
-// A block holds W * 32 / G channels and walks the sequence in pieces of 8 G
-// steps; u and dt are transposed through shared memory (global rows run over
-// channels, a lane needs its channel's steps), B and C rows are shared by all
-// channels of the block. States go in fours: 4 chains in flight, 16-byte
-// reads of B and C, and the two-wide FP32 instructions over pairs of states.
+// A block holds 128 / G channels and walks the sequence in pieces of 8 G
+// steps. The next piece's rows come by asynchronous copies while a piece is
+// computed (global rows run over channels, a lane needs its channel's steps,
+// so they pass through shared memory); B and C, shared by the block's
+// channels, are converted to float32 once per piece. States go in fours: 4
+// chains in flight, 16-byte reads of B and C, and the two-wide FP32
+// instructions over pairs of states.
+#include <algorithm>
+
 #include "scan.cuh"
 
 namespace ferrum {
@@ -23,35 +27,34 @@ namespace seq {
 namespace {
 
 constexpr int kLaneSteps = 8;
+constexpr int kWarps = 4, kThreads = 32 * kWarps;
 
-template <int G, int W>
+template <class T, int G, int NP>
 struct FwdCfg {
-  static constexpr int THREADS = W * 32;
-  static constexpr int CH = W * 32 / G;           // channels per block
+  static constexpr int CH = kThreads / G;         // channels per block
   static constexpr int CK = kLaneSteps * G;       // steps per piece
-  static constexpr int LD = CK + 4;               // channel stride of the transposed tiles
-  // B and C tiles: row t at t * NP + (t / 8) * 4, so that the lanes of a
-  // channel, 8 rows apart, read from different banks
-  static constexpr int bc_floats(int np) { return CK * np + (CK / 8) * 4; }
-  static size_t smem_bytes(int np) {
-    return sizeof(float) * (size_t)(2 * CH * LD + 2 * bc_floats(np) + 2 * CH * np);
-  }
+  static constexpr int XS = Piece<T, CH>::size(CK), RS = Piece<T, NP>::size(CK);
+  static constexpr int FS = Piece<float, NP>::size(CK);
+  static constexpr size_t BYTES = sizeof(T) * (size_t)(6 * XS + 2 * RS) +
+                                  sizeof(float) * (size_t)(2 * FS + 2 * CH * NP);
 };
 
-template <class T, int G, int W>
-__global__ void __launch_bounds__(W * 32, W == 4 ? 3 : 1)
+template <class T, int G, int NP>
+__global__ void __launch_bounds__(kThreads, 4)
 scan_fwd_kernel(ScanIn<T> in, Rows<T> out, float* fin, float* __restrict__ saved, ScanSizes s,
-                int lnp, int64_t col_blocks) {
-  using C = FwdCfg<G, W>;
-  constexpr int CH = C::CH, CK = C::CK, LD = C::LD;
+                int64_t col_blocks, int unit, int bc_unit) {
+  using C = FwdCfg<T, G, NP>;
+  constexpr int CH = C::CH, CK = C::CK;
+  using X = Piece<T, CH>;
+  using F = Piece<float, NP>;
   extern __shared__ float4 smem4[];
-  const int NP = 1 << lnp;
-  float* sU = (float*)smem4;
-  float* sDt = sU + CH * LD;
-  float* sB = sDt + CH * LD;
-  float* sC = sB + C::bc_floats(NP);
-  float* sA = sC + C::bc_floats(NP);   // A log2 e
+  float* sB = (float*)smem4;
+  float* sC = sB + C::FS;
+  float* sA = sC + C::FS;              // A log2 e
   float* sH = sA + CH * NP;            // the state in front of the piece
+  T* raw = (T*)(sH + CH * NP);         // 2 x (u, delta, z), then B and C as they come
+  T* rawB = raw + 6 * C::XS;
+  T* rawC = rawB + C::RS;
 
   int64_t q = blockIdx.x;
   const int64_t cb = q % col_blocks;
@@ -60,72 +63,78 @@ scan_fwd_kernel(ScanIn<T> in, Rows<T> out, float* fin, float* __restrict__ saved
   const int64_t d0 = grp * s.per_group + cb * CH;
   const int nch = (int)(s.per_group - cb * CH < CH ? s.per_group - cb * CH : CH);
   const int64_t len = scan_length(in.lengths, b, s.length);
-  const int tid = threadIdx.x, lane = tid & 31, g = lane % G;
-  const int c = (tid >> 5) * (32 / G) + lane / G;
+  const int tid = threadIdx.x, g = tid % G, c = tid / G;
+  const bool live = c < nch;
 
-  for (int i = tid; i < CH * NP; i += C::THREADS) {
-    const int cc = i >> lnp, n = i & (NP - 1);
+  auto fetch = [&](int64_t t0, int buf) {
+    const int rows = (int)(len - t0 < CK ? len - t0 : CK);
+    T* x = raw + buf * 3 * C::XS;
+    copy_piece<T, CK, CH, kThreads>(x, in.u.at(b, t0) + d0, in.u.st, rows, nch, unit, tid);
+    copy_piece<T, CK, CH, kThreads>(x + C::XS, in.delta.at(b, t0) + d0, in.delta.st, rows, nch,
+                                    unit, tid);
+    if (in.z)
+      copy_piece<T, CK, CH, kThreads>(x + 2 * C::XS, in.z.at(b, t0) + d0, in.z.st, rows, nch, unit,
+                                      tid);
+    copy_piece<T, CK, NP, kThreads>(rawB, in.B.at(b, t0) + grp * in.B_group, in.B.st, rows,
+                                    s.states, bc_unit, tid);
+    copy_piece<T, CK, NP, kThreads>(rawC, in.C.at(b, t0) + grp * in.C_group, in.C.st, rows,
+                                    s.states, bc_unit, tid);
+  };
+  if (len > 0) fetch(0, 0);
+
+  for (int i = tid; i < CH * NP; i += kThreads) {
+    const int cc = i / NP, n = i % NP;
     const bool ok = cc < nch && n < s.states;
     const int64_t o = (d0 + cc) * s.states + n;
     sA[i] = ok ? in.A[o] * kLog2e : 0.f;
     sH[i] = (ok && in.initial) ? in.initial[b * s.channels * s.states + o] : 0.f;
   }
-  const int tc = tid % CH;             // this thread's channel in the tile copies
-  const bool tok = tc < nch;
-  const float bias = (in.bias && tok) ? in.bias[d0 + tc] : 0.f;
-  const float skip = (in.D && c < nch) ? in.D[d0 + c] : 0.f;
+  const float bias = (in.bias && live) ? in.bias[d0 + c] : 0.f;
+  const float skip = (in.D && live) ? in.D[d0 + c] : 0.f;
 
-  for (int64_t t0 = 0; t0 < len; t0 += CK) {
-#pragma unroll
-    for (int i = 0; i < CK * CH / C::THREADS; ++i) {
-      const int t = i * (C::THREADS / CH) + tid / CH;
-      float x = 0.f, dt = 0.f;         // past the end: a = 1, b = 0
-      if (tok && t0 + t < len) {
-        x = to_f(in.u.at(b, t0 + t)[d0 + tc]);
-        dt = to_f(in.delta.at(b, t0 + t)[d0 + tc]) + bias;
-        if (s.softplus) dt = softplus_f(dt);
-      }
-      sU[tc * LD + t] = x;
-      sDt[tc * LD + t] = dt;
-    }
-    for (int i = tid; i < CK * NP; i += C::THREADS) {
-      const int t = i >> lnp, n = i & (NP - 1);
-      float vb = 0.f, vc = 0.f;
-      if (n < s.states && t0 + t < len) {
-        vb = to_f(in.B.at(b, t0 + t)[grp * in.B_group + n]);
-        vc = to_f(in.C.at(b, t0 + t)[grp * in.C_group + n]);
-      }
-      sB[i + (t >> 3) * 4] = vb;
-      sC[i + (t >> 3) * 4] = vc;
+  int buf = 0;
+  for (int64_t t0 = 0; t0 < len; t0 += CK, buf ^= 1) {
+    cp_async_wait();
+    __syncthreads();
+    for (int i = tid; i < CK * NP; i += kThreads) {
+      const int t = i / NP, n = i % NP;
+      sB[F::at(t, n)] = to_f(rawB[Piece<T, NP>::at(t, n)]);
+      sC[F::at(t, n)] = to_f(rawC[Piece<T, NP>::at(t, n)]);
     }
     __syncthreads();
+    if (t0 + CK < len) fetch(t0 + CK, buf ^ 1);
 
+    T* mine = raw + buf * 3 * C::XS + X::at(g * 8, c);
     float dt[8], du[8];
     f2 y[8];
-    float* mine = sU + c * LD + g * 8;
-    {
-      const float* pd = sDt + c * LD + g * 8;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) dt[i] = pd[i], du[i] = dt[i] * mine[i], y[i] = 0;
+    for (int i = 0; i < 8; ++i) {
+      float v = to_f(mine[C::XS + i * CH]) + bias;
+      if (s.softplus) v = softplus_f(v);
+      dt[i] = t0 + g * 8 + i < len ? v : 0.f;     // past the end: a = 1, b = 0
+      du[i] = dt[i] * to_f(mine[i * CH]);
+      y[i] = 0;
     }
-    const bool save = saved != nullptr && ((t0 >> 3) + g) % (kSaveSteps / 8) == 0 && c < nch &&
-                      t0 + g * 8 < s.length;
-    float* so = save ? saved + ((b * s.saves + (t0 + g * 8) / kSaveSteps) * s.channels + d0 + c) *
-                                   s.states
-                     : nullptr;
+    const int64_t ts = t0 + g * 8;
+    float* so = nullptr;
+    if (saved != nullptr && ts % kSaveSteps == 0 && live && ts < s.length)
+      so = saved + ((b * s.saves + ts / kSaveSteps) * s.channels + d0 + c) * s.states;
+#pragma unroll 1
     for (int n = 0; n < NP; n += 4) {
       const float4 A4 = *(const float4*)(sA + c * NP + n);
-      const float* pb = sB + g * (8 * NP + 4) + n;
-      const float* pc = sC + g * (8 * NP + 4) + n;
+      const f2 A01 = pack(A4.x, A4.y), A23 = pack(A4.z, A4.w);
+      const float* pb = sB + F::at(g * 8, n);
+      const float* pc = sC + F::at(g * 8, n);
       f2 a0[8], a1[8], b0[8], b1[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float4 B4 = *(const float4*)(pb + i * NP);
-        a0[i] = pack(ex2(dt[i] * A4.x), ex2(dt[i] * A4.y));
-        a1[i] = pack(ex2(dt[i] * A4.z), ex2(dt[i] * A4.w));
-        const f2 w = pack(du[i], du[i]);
-        b0[i] = mul2(w, pack(B4.x, B4.y));
-        b1[i] = mul2(w, pack(B4.z, B4.w));
+        const f2 w = pack(dt[i], dt[i]), v = pack(du[i], du[i]);
+        const float2 e0 = unpack(mul2(w, A01)), e1 = unpack(mul2(w, A23));
+        a0[i] = pack(ex2(e0.x), ex2(e0.y));
+        a1[i] = pack(ex2(e1.x), ex2(e1.y));
+        b0[i] = mul2(v, pack(B4.x, B4.y));
+        b1[i] = mul2(v, pack(B4.z, B4.w));
       }
       f2 P0 = a0[0], P1 = a1[0], H0 = b0[0], H1 = b1[0];
 #pragma unroll
@@ -157,7 +166,7 @@ scan_fwd_kernel(ScanIn<T> in, Rows<T> out, float* fin, float* __restrict__ saved
       } else {
         h0 = u0, h1 = u1;
       }
-      if (save) {
+      if (so != nullptr) {
         const float2 p = unpack(h0), r = unpack(h1);
         if (n + 0 < s.states) so[n + 0] = p.x;
         if (n + 1 < s.states) so[n + 1] = p.y;
@@ -175,35 +184,30 @@ scan_fwd_kernel(ScanIn<T> in, Rows<T> out, float* fin, float* __restrict__ saved
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float2 v = unpack(y[i]);
-      mine[i] = fmaf(skip, mine[i], v.x + v.y);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < CK * CH / C::THREADS; ++i) {
-      const int t = i * (C::THREADS / CH) + tid / CH;
-      if (tok && t0 + t < s.length) {
-        float v = 0.f;
-        if (t0 + t < len) {
-          v = sU[tc * LD + t];
-          if (in.z) {
-            const float z = to_f(in.z.at(b, t0 + t)[d0 + tc]);
-            v *= z * sigmoid_f(z);
-          }
-        }
-        out.at(b, t0 + t)[d0 + tc] = from_f<T>(v);
+      const float2 p = unpack(y[i]);
+      float v = fmaf(skip, to_f(mine[i * CH]), p.x + p.y);
+      if (in.z) {
+        const float z = to_f(mine[2 * C::XS + i * CH]);
+        v *= z * sigmoid_f(z);
       }
+      mine[i * CH] = from_f<T>(t0 + g * 8 + i < len ? v : 0.f);   // in u's place
     }
     __syncthreads();
+    const T* x = raw + buf * 3 * C::XS;
+#pragma unroll
+    for (int i = 0; i < CK * CH / kThreads; ++i) {
+      const int t = i * (kThreads / CH) + tid / CH, cc = tid % CH;
+      if (cc < nch && t0 + t < s.length) out.at(b, t0 + t)[d0 + cc] = x[X::at(t, cc)];
+    }
   }
   // steps past the sequence's last piece
-  if (tok)
-    for (int64_t t = (len + CK - 1) / CK * CK + tid / CH; t < s.length; t += C::THREADS / CH)
-      out.at(b, t)[d0 + tc] = from_f<T>(0.f);
+  if (tid % CH < nch)
+    for (int64_t t = (len + CK - 1) / CK * CK + tid / CH; t < s.length; t += kThreads / CH)
+      out.at(b, t)[d0 + tid % CH] = from_f<T>(0.f);
   if (fin != nullptr) {
     __syncthreads();
-    for (int i = tid; i < CH * NP; i += C::THREADS) {
-      const int cc = i >> lnp, n = i & (NP - 1);
+    for (int i = tid; i < CH * NP; i += kThreads) {
+      const int cc = i / NP, n = i % NP;
       if (cc < nch && n < s.states)
         fin[(b * s.channels + d0 + cc) * s.states + n] = sH[i];
     }
@@ -267,20 +271,25 @@ scan_step_kernel(ScanIn<T> in, Rows<T> out, float* fin, ScanSizes s, bool vec) {
   }
 }
 
-template <class T, int G, int W>
-ferrum_status run_fwd(const ferrum_scan_args* a, const ScanSizes& s, int lnp, cudaStream_t stream,
+template <class T, int G, int NP>
+ferrum_status run_fwd(const ferrum_scan_args* a, const ScanSizes& s, cudaStream_t stream,
                       const char* what) {
-  using C = FwdCfg<G, W>;
+  using C = FwdCfg<T, G, NP>;
   static std::atomic<uint64_t> done{0};
   const int64_t col_blocks = ceil_div(s.per_group, C::CH);
   const int64_t blocks = s.batch * s.groups * col_blocks;
   if (blocks > 0x7fffffff) return invalid(what, "too many blocks for one launch");
-  const size_t smem = C::smem_bytes(1 << lnp);
-  cudaError_t e = launch_detail::ensure_smem(scan_fwd_kernel<T, G, W>, C::smem_bytes(64), done);
+  cudaError_t e = launch_detail::ensure_smem(scan_fwd_kernel<T, G, NP>, C::BYTES, done);
   if (e != cudaSuccess) return cuda_error(e, what);
+  const bool one_group = s.groups == 1;
+  int unit = std::min(copy_unit<T>(a->u), copy_unit<T>(a->delta, one_group ? 0 : s.per_group));
+  if (a->z.ptr) unit = std::min(unit, copy_unit<T>(a->z));
+  const int bc_unit = std::min(copy_unit<T>(a->B, a->B_group_stride),
+                               copy_unit<T>(a->C, a->C_group_stride));
   launch_detail::clear_stale_error();
-  scan_fwd_kernel<T, G, W><<<(unsigned)blocks, C::THREADS, smem, stream>>>(
-      scan_in<T>(a), rows_of<T>(a->out), a->final_state, a->saved_states, s, lnp, col_blocks);
+  scan_fwd_kernel<T, G, NP><<<(unsigned)blocks, kThreads, C::BYTES, stream>>>(
+      scan_in<T>(a), rows_of<T>(a->out), a->final_state, a->saved_states, s, col_blocks, unit,
+      bc_unit);
   return launched(what);
 }
 
@@ -296,20 +305,24 @@ ferrum_status scan_fwd(ferrum_device* dev, const ferrum_scan_args* a, cudaStream
   const ScanSizes s = scan_sizes(a);
   DeviceGuard guard(dev->ordinal);
   if (guard.status() != cudaSuccess) return cuda_error(guard.status(), "cudaSetDevice");
-  const int lnp = log_states(s.states);
   // Lanes per channel: few keep the scan short, many give enough warps where
-  // there are few channels. The least of 4..32 that reaches 12 warps an SM,
-  // within the sequence's length and (B, C tiles) shared memory.
+  // there are few channels. The least that reaches 12 warps an SM, within the
+  // sequence's length.
   int G = 4;
-  while (G < 32 && s.batch * s.channels * G / 32 < 148 * 12 && G * kLaneSteps < s.length &&
-         2 * G * kLaneSteps * (1 << lnp) * 8 <= 96 * 1024)
-    G *= 2;
+  while (G < 32 && s.batch * s.channels * G / 32 < 148 * 12 && G * kLaneSteps < s.length) G *= 2;
   return with_dtype(a->dtype, [&](auto tag) {
     using T = decltype(tag);
-    if (G == 4) return run_fwd<T, 4, 4>(a, s, lnp, stream, what);
-    if (G == 8) return run_fwd<T, 8, 4>(a, s, lnp, stream, what);
-    if (G == 16) return run_fwd<T, 16, 8>(a, s, lnp, stream, what);
-    return run_fwd<T, 32, 8>(a, s, lnp, stream, what);
+    auto go = [&](auto np) -> ferrum_status {
+      constexpr int NP = decltype(np)::value;
+      if (G == 4) return run_fwd<T, 4, NP>(a, s, stream, what);
+      if (G == 8 || NP == 64) return run_fwd<T, 8, NP>(a, s, stream, what);
+      if constexpr (NP <= 32) {
+        if (G == 16 || NP == 32) return run_fwd<T, 16, NP>(a, s, stream, what);
+        if constexpr (NP <= 16) return run_fwd<T, 32, NP>(a, s, stream, what);
+      }
+      return FERRUM_OK;
+    };
+    return with_states(s.states, go);
   });
 }
 
