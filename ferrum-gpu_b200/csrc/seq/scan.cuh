@@ -1,6 +1,8 @@
 // Argument views and helpers shared by the selective scan's kernels.
 #pragma once
 
+#include <type_traits>
+
 #include "seq_common.cuh"
 
 namespace ferrum {
@@ -116,22 +118,25 @@ int copy_unit(const ferrum_rows& r, int64_t extra = 0) {
 
 // Rows [0, ROWS) of columns [0, cols) of an array to a piece, rows from
 // `rows` and columns from `cols` on as zeros. THREADS threads take part; the
-// 16- and 4-byte forms are asynchronous.
+// 16- and 4-byte forms are asynchronous. Row strides fit 32 bits (checked on
+// the host), so an address is one wide multiply-add.
 template <class T, int ROWS, int COLS, int THREADS, int UNIT>
-__device__ __forceinline__ void copy_units(T* dst, const T* src, int64_t stride, int rows, int cols,
+__device__ __forceinline__ void copy_units(T* dst, const T* src, int stride, int rows, int cols,
                                            int tid) {
   constexpr int E = UNIT / (int)sizeof(T), PER = COLS / E;
-#pragma unroll 4
-  for (int i = tid; i < ROWS * PER; i += THREADS) {
+#pragma unroll
+  for (int i0 = 0; i0 < ROWS * PER; i0 += THREADS) {
+    const int i = i0 + tid;
+    if (ROWS * PER % THREADS != 0 && i >= ROWS * PER) break;
     const int t = i / PER, c = (i % PER) * E;
     int n = t < rows ? cols - c : 0;
     n = n < 0 ? 0 : (n > E ? E : n);
-    cp_async<UNIT>(dst + Piece<T, COLS>::at(t, c), n > 0 ? src + t * stride + c : src,
+    cp_async<UNIT>(dst + Piece<T, COLS>::at(t, c), n > 0 ? src + (int64_t)t * stride + c : src,
                    n * (int)sizeof(T));
   }
 }
 template <class T, int ROWS, int COLS, int THREADS>
-__device__ __forceinline__ void copy_piece(T* dst, const T* src, int64_t stride, int rows, int cols,
+__device__ __forceinline__ void copy_piece(T* dst, const T* src, int stride, int rows, int cols,
                                            int unit, int tid) {
   if constexpr (COLS * sizeof(T) >= 16) {
     if (unit == kCopy16) return copy_units<T, ROWS, COLS, THREADS, 16>(dst, src, stride, rows, cols, tid);
@@ -140,7 +145,50 @@ __device__ __forceinline__ void copy_piece(T* dst, const T* src, int64_t stride,
     return copy_units<T, ROWS, COLS, THREADS, 4>(dst, src, stride, rows, cols, tid);
   for (int i = tid; i < ROWS * COLS; i += THREADS) {
     const int t = i / COLS, c = i % COLS;
-    dst[Piece<T, COLS>::at(t, c)] = (t < rows && c < cols) ? src[t * stride + c] : from_f<T>(0.f);
+    dst[Piece<T, COLS>::at(t, c)] =
+        (t < rows && c < cols) ? src[(int64_t)t * stride + c] : from_f<T>(0.f);
+  }
+}
+
+// A piece in shared memory to rows [0, rows), columns [0, cols) of an array.
+template <class T, int ROWS, int COLS, int THREADS>
+__device__ __forceinline__ void store_piece(T* dst, const T* src, int stride, int rows, int cols,
+                                            int unit, int tid) {
+  if constexpr (COLS * sizeof(T) >= 16) {
+    if (unit == kCopy16 && cols == COLS) {
+      constexpr int E = 16 / (int)sizeof(T), PER = COLS / E;
+#pragma unroll
+      for (int i0 = 0; i0 < ROWS * PER; i0 += THREADS) {
+        const int i = i0 + tid, t = i / PER, c = (i % PER) * E;
+        if (i < ROWS * PER && t < rows)
+          *(uint4*)(dst + (int64_t)t * stride + c) = *(const uint4*)(src + Piece<T, COLS>::at(t, c));
+      }
+      return;
+    }
+  }
+#pragma unroll 4
+  for (int i = tid; i < ROWS * COLS; i += THREADS) {
+    const int t = i / COLS, c = i % COLS;
+    if (t < rows && c < cols) dst[(int64_t)t * stride + c] = src[Piece<T, COLS>::at(t, c)];
+  }
+}
+
+// A piece of rows [0, ROWS) converted to float32, two values at a time.
+template <class T, int ROWS, int COLS, int THREADS>
+__device__ __forceinline__ void widen_piece(float* dst, const T* src, int tid) {
+#pragma unroll
+  for (int i0 = 0; i0 < ROWS * COLS / 2; i0 += THREADS) {
+    const int i = i0 + tid;
+    if (ROWS * COLS / 2 % THREADS != 0 && i >= ROWS * COLS / 2) break;
+    const int t = i / (COLS / 2), c = i % (COLS / 2) * 2;
+    float2 v;
+    if constexpr (std::is_same<T, float>::value)
+      v = *(const float2*)(src + Piece<T, COLS>::at(t, c));
+    else if constexpr (std::is_same<T, __half>::value)
+      v = __half22float2(*(const __half2*)(src + Piece<T, COLS>::at(t, c)));
+    else
+      v = __bfloat1622float2(*(const __nv_bfloat162*)(src + Piece<T, COLS>::at(t, c)));
+    *(float2*)(dst + Piece<float, COLS>::at(t, c)) = v;
   }
 }
 

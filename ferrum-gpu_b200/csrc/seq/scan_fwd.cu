@@ -42,7 +42,7 @@ struct FwdCfg {
 template <class T, int G, int NP>
 __global__ void __launch_bounds__(kThreads, 4)
 scan_fwd_kernel(ScanIn<T> in, Rows<T> out, float* fin, float* __restrict__ saved, ScanSizes s,
-                int64_t col_blocks, int unit, int bc_unit) {
+                int64_t col_blocks, int unit, int bc_unit, int out_unit) {
   using C = FwdCfg<T, G, NP>;
   constexpr int CH = C::CH, CK = C::CK;
   using X = Piece<T, CH>;
@@ -69,15 +69,15 @@ scan_fwd_kernel(ScanIn<T> in, Rows<T> out, float* fin, float* __restrict__ saved
   auto fetch = [&](int64_t t0, int buf) {
     const int rows = (int)(len - t0 < CK ? len - t0 : CK);
     T* x = raw + buf * 3 * C::XS;
-    copy_piece<T, CK, CH, kThreads>(x, in.u.at(b, t0) + d0, in.u.st, rows, nch, unit, tid);
-    copy_piece<T, CK, CH, kThreads>(x + C::XS, in.delta.at(b, t0) + d0, in.delta.st, rows, nch,
-                                    unit, tid);
+    copy_piece<T, CK, CH, kThreads>(x, in.u.at(b, t0) + d0, (int)in.u.st, rows, nch, unit, tid);
+    copy_piece<T, CK, CH, kThreads>(x + C::XS, in.delta.at(b, t0) + d0, (int)in.delta.st, rows,
+                                    nch, unit, tid);
     if (in.z)
-      copy_piece<T, CK, CH, kThreads>(x + 2 * C::XS, in.z.at(b, t0) + d0, in.z.st, rows, nch, unit,
-                                      tid);
-    copy_piece<T, CK, NP, kThreads>(rawB, in.B.at(b, t0) + grp * in.B_group, in.B.st, rows,
+      copy_piece<T, CK, CH, kThreads>(x + 2 * C::XS, in.z.at(b, t0) + d0, (int)in.z.st, rows, nch,
+                                      unit, tid);
+    copy_piece<T, CK, NP, kThreads>(rawB, in.B.at(b, t0) + grp * in.B_group, (int)in.B.st, rows,
                                     s.states, bc_unit, tid);
-    copy_piece<T, CK, NP, kThreads>(rawC, in.C.at(b, t0) + grp * in.C_group, in.C.st, rows,
+    copy_piece<T, CK, NP, kThreads>(rawC, in.C.at(b, t0) + grp * in.C_group, (int)in.C.st, rows,
                                     s.states, bc_unit, tid);
   };
   if (len > 0) fetch(0, 0);
@@ -96,22 +96,21 @@ scan_fwd_kernel(ScanIn<T> in, Rows<T> out, float* fin, float* __restrict__ saved
   for (int64_t t0 = 0; t0 < len; t0 += CK, buf ^= 1) {
     cp_async_wait();
     __syncthreads();
-    for (int i = tid; i < CK * NP; i += kThreads) {
-      const int t = i / NP, n = i % NP;
-      sB[F::at(t, n)] = to_f(rawB[Piece<T, NP>::at(t, n)]);
-      sC[F::at(t, n)] = to_f(rawC[Piece<T, NP>::at(t, n)]);
-    }
+    widen_piece<T, CK, NP, kThreads>(sB, rawB, tid);
+    widen_piece<T, CK, NP, kThreads>(sC, rawC, tid);
     __syncthreads();
     if (t0 + CK < len) fetch(t0 + CK, buf ^ 1);
 
     T* mine = raw + buf * 3 * C::XS + X::at(g * 8, c);
+    const int64_t left = len - t0 - g * 8;          // valid steps from this lane's first on
+    const int steps = left < 0 ? 0 : (left > 8 ? 8 : (int)left);
     float dt[8], du[8];
     f2 y[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       float v = to_f(mine[C::XS + i * CH]) + bias;
       if (s.softplus) v = softplus_f(v);
-      dt[i] = t0 + g * 8 + i < len ? v : 0.f;     // past the end: a = 1, b = 0
+      dt[i] = i < steps ? v : 0.f;                  // past the end: a = 1, b = 0
       du[i] = dt[i] * to_f(mine[i * CH]);
       y[i] = 0;
     }
@@ -122,19 +121,23 @@ scan_fwd_kernel(ScanIn<T> in, Rows<T> out, float* fin, float* __restrict__ saved
 #pragma unroll 1
     for (int n = 0; n < NP; n += 4) {
       const float4 A4 = *(const float4*)(sA + c * NP + n);
-      const f2 A01 = pack(A4.x, A4.y), A23 = pack(A4.z, A4.w);
+      const f2 Ax = pack(A4.x, A4.x), Ay = pack(A4.y, A4.y), Az = pack(A4.z, A4.z),
+               Aw = pack(A4.w, A4.w);
       const float* pb = sB + F::at(g * 8, n);
       const float* pc = sC + F::at(g * 8, n);
       f2 a0[8], a1[8], b0[8], b1[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float4 B4 = *(const float4*)(pb + i * NP);
-        const f2 w = pack(dt[i], dt[i]), v = pack(du[i], du[i]);
-        const float2 e0 = unpack(mul2(w, A01)), e1 = unpack(mul2(w, A23));
-        a0[i] = pack(ex2(e0.x), ex2(e0.y));
-        a1[i] = pack(ex2(e1.x), ex2(e1.y));
-        b0[i] = mul2(v, pack(B4.x, B4.y));
-        b1[i] = mul2(v, pack(B4.z, B4.w));
+        b0[i] = pack(du[i] * B4.x, du[i] * B4.y);
+        b1[i] = pack(du[i] * B4.z, du[i] * B4.w);
+        if (i % 2 == 0) {     // exponents of two steps at a time: A's halves stay put
+          const f2 w = pack(dt[i], dt[i + 1]);
+          const float2 p = unpack(mul2(w, Ax)), q = unpack(mul2(w, Ay));
+          const float2 r = unpack(mul2(w, Az)), v = unpack(mul2(w, Aw));
+          a0[i] = pack(ex2(p.x), ex2(q.x)), a0[i + 1] = pack(ex2(p.y), ex2(q.y));
+          a1[i] = pack(ex2(r.x), ex2(v.x)), a1[i + 1] = pack(ex2(r.y), ex2(v.y));
+        }
       }
       f2 P0 = a0[0], P1 = a1[0], H0 = b0[0], H1 = b1[0];
 #pragma unroll
@@ -190,15 +193,12 @@ scan_fwd_kernel(ScanIn<T> in, Rows<T> out, float* fin, float* __restrict__ saved
         const float z = to_f(mine[2 * C::XS + i * CH]);
         v *= z * sigmoid_f(z);
       }
-      mine[i * CH] = from_f<T>(t0 + g * 8 + i < len ? v : 0.f);   // in u's place
+      mine[i * CH] = from_f<T>(i < steps ? v : 0.f);   // in u's place
     }
     __syncthreads();
-    const T* x = raw + buf * 3 * C::XS;
-#pragma unroll
-    for (int i = 0; i < CK * CH / kThreads; ++i) {
-      const int t = i * (kThreads / CH) + tid / CH, cc = tid % CH;
-      if (cc < nch && t0 + t < s.length) out.at(b, t0 + t)[d0 + cc] = x[X::at(t, cc)];
-    }
+    store_piece<T, CK, CH, kThreads>(out.at(b, t0) + d0, raw + buf * 3 * C::XS, (int)out.st,
+                                     (int)(s.length - t0 < CK ? s.length - t0 : CK), nch, out_unit,
+                                     tid);
   }
   // steps past the sequence's last piece
   if (tid % CH < nch)
@@ -289,7 +289,7 @@ ferrum_status run_fwd(const ferrum_scan_args* a, const ScanSizes& s, cudaStream_
   launch_detail::clear_stale_error();
   scan_fwd_kernel<T, G, NP><<<(unsigned)blocks, kThreads, C::BYTES, stream>>>(
       scan_in<T>(a), rows_of<T>(a->out), a->final_state, a->saved_states, s, col_blocks, unit,
-      bc_unit);
+      bc_unit, copy_unit<T>(a->out, one_group ? 0 : s.per_group));
   return launched(what);
 }
 
@@ -367,6 +367,10 @@ ferrum_status check_scan(const ferrum_device* dev, const ferrum_scan_args* a, co
                              std::to_string(a->channels) + ")");
   if (bounded_product({a->batch, a->length + 1, a->channels, a->states}) < 0)
     return invalid(what, "batch * length * channels * states is too large");
+  for (const ferrum_rows* r : {&a->u, &a->delta, &a->z, &a->out, &a->B, &a->C, &a->dout, &a->du,
+                               &a->ddelta, &a->dz})
+    if (r->row_stride > 0x7fffffff || r->row_stride < -0x7fffffff)
+      return invalid(what, "row strides must fit 32 bits");
   const size_t e = dtype_size(a->dtype);
   const bool none = a->batch == 0 || a->channels == 0, empty = none || a->length == 0;
   if (ferrum_status s = check_ptr(a->A, 4, none, what, "A")) return s;
