@@ -27,24 +27,27 @@ namespace seq {
 namespace {
 
 constexpr int kLaneSteps = 8;
-constexpr int kWarps = 4, kThreads = 32 * kWarps;
 
-template <class T, int G, int NP>
+// G lanes share a channel's steps, S warps its states.
+template <class T, int G, int S, int NP>
 struct FwdCfg {
-  static constexpr int CH = kThreads / G;         // channels per block
+  static constexpr int THREADS = S == 1 ? 128 : 256;
+  static constexpr int CH = THREADS / S / G;      // channels per block
   static constexpr int CK = kLaneSteps * G;       // steps per piece
   static constexpr int XS = Piece<T, CH>::size(CK), RS = Piece<T, NP>::size(CK);
   static constexpr int FS = Piece<float, NP>::size(CK);
-  static constexpr size_t BYTES = sizeof(T) * (size_t)(6 * XS + 2 * RS) +
-                                  sizeof(float) * (size_t)(2 * FS + 2 * CH * NP);
+  static constexpr int YS = CH * (CK + 4);        // a float32 (channel, step) tile
+  static constexpr size_t BYTES =
+      sizeof(T) * (size_t)(6 * XS + 2 * RS) +
+      sizeof(float) * (size_t)(2 * FS + 2 * CH * NP + (S == 1 ? 0 : (S + 1) * YS));
 };
 
-template <class T, int G, int NP>
-__global__ void __launch_bounds__(kThreads, 4)
+template <class T, int G, int S, int NP>
+__global__ void __launch_bounds__(FwdCfg<T, G, S, NP>::THREADS, 512 / FwdCfg<T, G, S, NP>::THREADS)
 scan_fwd_kernel(ScanIn<T> in, Rows<T> out, float* fin, float* __restrict__ saved, ScanSizes s,
                 int64_t col_blocks, int unit, int bc_unit, int out_unit) {
-  using C = FwdCfg<T, G, NP>;
-  constexpr int CH = C::CH, CK = C::CK;
+  using C = FwdCfg<T, G, S, NP>;
+  constexpr int CH = C::CH, CK = C::CK, kThreads = C::THREADS;
   using X = Piece<T, CH>;
   using F = Piece<float, NP>;
   extern __shared__ float4 smem4[];
@@ -52,7 +55,9 @@ scan_fwd_kernel(ScanIn<T> in, Rows<T> out, float* fin, float* __restrict__ saved
   float* sC = sB + C::FS;
   float* sA = sC + C::FS;              // A log2 e
   float* sH = sA + CH * NP;            // the state in front of the piece
-  T* raw = (T*)(sH + CH * NP);         // 2 x (u, delta, z), then B and C as they come
+  float* sDt = sH + CH * NP;           // S > 1: dt, then the warps' parts of y
+  float* sY = sDt + (S == 1 ? 0 : C::YS);
+  T* raw = (T*)(sY + (S == 1 ? 0 : S * C::YS));   // 2 x (u, delta, z), then B, C as they come
   T* rawB = raw + 6 * C::XS;
   T* rawC = rawB + C::RS;
 
@@ -63,7 +68,8 @@ scan_fwd_kernel(ScanIn<T> in, Rows<T> out, float* fin, float* __restrict__ saved
   const int64_t d0 = grp * s.per_group + cb * CH;
   const int nch = (int)(s.per_group - cb * CH < CH ? s.per_group - cb * CH : CH);
   const int64_t len = scan_length(in.lengths, b, s.length);
-  const int tid = threadIdx.x, g = tid % G, c = tid / G;
+  const int tid = threadIdx.x, g = tid % G, sg = tid / (CH * G);   // sg: this warp's states
+  const int c = tid / G % CH, row = c * (CK + 4) + g * 8;
   const bool live = c < nch;
 
   auto fetch = [&](int64_t t0, int buf) {
@@ -106,20 +112,31 @@ scan_fwd_kernel(ScanIn<T> in, Rows<T> out, float* fin, float* __restrict__ saved
     const int steps = left < 0 ? 0 : (left > 8 ? 8 : (int)left);
     float dt[8], du[8];
     f2 y[8];
+    constexpr int PART = 8 / S;                     // steps whose dt and output are this warp's
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int k = 0; k < PART; ++k) {
+      const int i = S == 1 ? k : sg * PART + k;
       float v = to_f(mine[C::XS + i * CH]) + bias;
       if (s.softplus) v = softplus_f(v);
-      dt[i] = i < steps ? v : 0.f;                  // past the end: a = 1, b = 0
-      du[i] = dt[i] * to_f(mine[i * CH]);
-      y[i] = 0;
+      v = i < steps ? v : 0.f;                      // past the end: a = 1, b = 0
+      if constexpr (S == 1)
+        dt[k] = v;
+      else
+        sDt[row + i] = v;
     }
+    if constexpr (S > 1) {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) dt[i] = sDt[row + i];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) du[i] = dt[i] * to_f(mine[i * CH]), y[i] = 0;
     const int64_t ts = t0 + g * 8;
     float* so = nullptr;
     if (saved != nullptr && ts % kSaveSteps == 0 && live && ts < s.length)
       so = saved + ((b * s.saves + ts / kSaveSteps) * s.channels + d0 + c) * s.states;
 #pragma unroll 1
-    for (int n = 0; n < NP; n += 4) {
+    for (int n = sg * (NP / S); n < (sg + 1) * (NP / S); n += 4) {
       const float4 A4 = *(const float4*)(sA + c * NP + n);
       const f2 Ax = pack(A4.x, A4.x), Ay = pack(A4.y, A4.y), Az = pack(A4.z, A4.z),
                Aw = pack(A4.w, A4.w);
@@ -185,10 +202,26 @@ scan_fwd_kernel(ScanIn<T> in, Rows<T> out, float* fin, float* __restrict__ saved
         y[i] = fma2(h1, pack(C4.z, C4.w), y[i]);
       }
     }
+    float sum[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float2 p = unpack(y[i]);
-      float v = fmaf(skip, to_f(mine[i * CH]), p.x + p.y);
+      sum[i] = p.x + p.y;
+    }
+    if constexpr (S > 1) {
+      float4* w = (float4*)(sY + sg * C::YS + row);
+      w[0] = make_float4(sum[0], sum[1], sum[2], sum[3]);
+      w[1] = make_float4(sum[4], sum[5], sum[6], sum[7]);
+      __syncthreads();
+    }
+#pragma unroll
+    for (int k = 0; k < PART; ++k) {
+      const int i = S == 1 ? k : sg * PART + k;
+      float v = S == 1 ? sum[k] : 0.f;
+      if constexpr (S > 1)
+#pragma unroll
+        for (int r = 0; r < S; ++r) v += sY[r * C::YS + row + i];
+      v = fmaf(skip, to_f(mine[i * CH]), v);
       if (in.z) {
         const float z = to_f(mine[2 * C::XS + i * CH]);
         v *= z * sigmoid_f(z);
@@ -271,15 +304,15 @@ scan_step_kernel(ScanIn<T> in, Rows<T> out, float* fin, ScanSizes s, bool vec) {
   }
 }
 
-template <class T, int G, int NP>
+template <class T, int G, int S, int NP>
 ferrum_status run_fwd(const ferrum_scan_args* a, const ScanSizes& s, cudaStream_t stream,
                       const char* what) {
-  using C = FwdCfg<T, G, NP>;
+  using C = FwdCfg<T, G, S, NP>;
   static std::atomic<uint64_t> done{0};
   const int64_t col_blocks = ceil_div(s.per_group, C::CH);
   const int64_t blocks = s.batch * s.groups * col_blocks;
   if (blocks > 0x7fffffff) return invalid(what, "too many blocks for one launch");
-  cudaError_t e = launch_detail::ensure_smem(scan_fwd_kernel<T, G, NP>, C::BYTES, done);
+  cudaError_t e = launch_detail::ensure_smem(scan_fwd_kernel<T, G, S, NP>, C::BYTES, done);
   if (e != cudaSuccess) return cuda_error(e, what);
   const bool one_group = s.groups == 1;
   int unit = std::min(copy_unit<T>(a->u), copy_unit<T>(a->delta, one_group ? 0 : s.per_group));
@@ -287,7 +320,7 @@ ferrum_status run_fwd(const ferrum_scan_args* a, const ScanSizes& s, cudaStream_
   const int bc_unit = std::min(copy_unit<T>(a->B, a->B_group_stride),
                                copy_unit<T>(a->C, a->C_group_stride));
   launch_detail::clear_stale_error();
-  scan_fwd_kernel<T, G, NP><<<(unsigned)blocks, kThreads, C::BYTES, stream>>>(
+  scan_fwd_kernel<T, G, S, NP><<<(unsigned)blocks, C::THREADS, C::BYTES, stream>>>(
       scan_in<T>(a), rows_of<T>(a->out), a->final_state, a->saved_states, s, col_blocks, unit,
       bc_unit, copy_unit<T>(a->out, one_group ? 0 : s.per_group));
   return launched(what);
@@ -305,24 +338,23 @@ ferrum_status scan_fwd(ferrum_device* dev, const ferrum_scan_args* a, cudaStream
   const ScanSizes s = scan_sizes(a);
   DeviceGuard guard(dev->ordinal);
   if (guard.status() != cudaSuccess) return cuda_error(guard.status(), "cudaSetDevice");
-  // Lanes per channel: few keep the scan short, many give enough warps where
-  // there are few channels. The least that reaches 12 warps an SM, within the
-  // sequence's length.
-  int G = 4;
-  while (G < 32 && s.batch * s.channels * G / 32 < 148 * 12 && G * kLaneSteps < s.length) G *= 2;
+  // Lanes per channel: few keep the shuffles short. Where a batch has too few
+  // channels for 12 warps an SM that way, a channel gets more lanes, then
+  // several warps that share its states.
+  const int64_t warps = s.batch * s.channels / 8;   // with 4 lanes
+  constexpr int64_t kEnough = 148 * 12;
+  const int level = warps >= kEnough || s.length <= 32 ? 0
+                    : 2 * warps >= kEnough             ? 1
+                    : 8 * warps >= kEnough || s.length <= 64 ? 2 : 3;
   return with_dtype(a->dtype, [&](auto tag) {
     using T = decltype(tag);
-    auto go = [&](auto np) -> ferrum_status {
-      constexpr int NP = decltype(np)::value;
-      if (G == 4) return run_fwd<T, 4, NP>(a, s, stream, what);
-      if (G == 8 || NP == 64) return run_fwd<T, 8, NP>(a, s, stream, what);
-      if constexpr (NP <= 32) {
-        if (G == 16 || NP == 32) return run_fwd<T, 16, NP>(a, s, stream, what);
-        if constexpr (NP <= 16) return run_fwd<T, 32, NP>(a, s, stream, what);
-      }
-      return FERRUM_OK;
-    };
-    return with_states(s.states, go);
+    return with_states(s.states, [&](auto np) -> ferrum_status {
+      constexpr int NP = decltype(np)::value, S = NP == 8 ? 2 : 4;
+      if (level == 0) return run_fwd<T, 4, 1, NP>(a, s, stream, what);
+      if (level == 1) return run_fwd<T, 8, 1, NP>(a, s, stream, what);
+      if (level == 2) return run_fwd<T, 8, S, NP>(a, s, stream, what);
+      return run_fwd<T, 16, S, NP>(a, s, stream, what);
+    });
   });
 }
 
