@@ -86,6 +86,11 @@ scan_fwd_kernel(ScanIn<T> in, Rows<T> out, float* fin, float* __restrict__ saved
     copy_piece<T, CK, NP, kThreads>(rawC, in.C.at(b, t0) + grp * in.C_group, (int)in.C.st, rows,
                                     s.states, bc_unit, tid);
   };
+  auto put = [&](int64_t t0, int buf) {
+    store_piece<T, CK, CH, kThreads>(out.at(b, t0) + d0, raw + buf * 3 * C::XS, (int)out.st,
+                                     (int)(s.length - t0 < CK ? s.length - t0 : CK), nch, out_unit,
+                                     tid);
+  };
   if (len > 0) fetch(0, 0);
 
   for (int i = tid; i < CH * NP; i += kThreads) {
@@ -102,10 +107,9 @@ scan_fwd_kernel(ScanIn<T> in, Rows<T> out, float* fin, float* __restrict__ saved
   for (int64_t t0 = 0; t0 < len; t0 += CK, buf ^= 1) {
     cp_async_wait();
     __syncthreads();
+    if (t0 > 0) put(t0 - CK, buf ^ 1);
     widen_piece<T, CK, NP, kThreads>(sB, rawB, tid);
     widen_piece<T, CK, NP, kThreads>(sC, rawC, tid);
-    __syncthreads();
-    if (t0 + CK < len) fetch(t0 + CK, buf ^ 1);
 
     T* mine = raw + buf * 3 * C::XS + X::at(g * 8, c);
     const int64_t left = len - t0 - g * 8;          // valid steps from this lane's first on
@@ -124,11 +128,11 @@ scan_fwd_kernel(ScanIn<T> in, Rows<T> out, float* fin, float* __restrict__ saved
       else
         sDt[row + i] = v;
     }
-    if constexpr (S > 1) {
-      __syncthreads();
+    __syncthreads();
+    if (t0 + CK < len) fetch(t0 + CK, buf ^ 1);
+    if constexpr (S > 1)
 #pragma unroll
       for (int i = 0; i < 8; ++i) dt[i] = sDt[row + i];
-    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) du[i] = dt[i] * to_f(mine[i * CH]), y[i] = 0;
     const int64_t ts = t0 + g * 8;
@@ -228,10 +232,10 @@ scan_fwd_kernel(ScanIn<T> in, Rows<T> out, float* fin, float* __restrict__ saved
       }
       mine[i * CH] = from_f<T>(i < steps ? v : 0.f);   // in u's place
     }
+  }
+  if (len > 0) {
     __syncthreads();
-    store_piece<T, CK, CH, kThreads>(out.at(b, t0) + d0, raw + buf * 3 * C::XS, (int)out.st,
-                                     (int)(s.length - t0 < CK ? s.length - t0 : CK), nch, out_unit,
-                                     tid);
+    put((len - 1) / CK * CK, buf ^ 1);
   }
   // steps past the sequence's last piece
   if (tid % CH < nch)
