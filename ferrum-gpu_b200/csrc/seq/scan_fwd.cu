@@ -343,13 +343,15 @@ ferrum_status scan_fwd(ferrum_device* dev, const ferrum_scan_args* a, cudaStream
   DeviceGuard guard(dev->ordinal);
   if (guard.status() != cudaSuccess) return cuda_error(guard.status(), "cudaSetDevice");
   // Lanes per channel: few keep the shuffles short. Where a batch has too few
-  // channels for 12 warps an SM that way, a channel gets more lanes, then
-  // several warps that share its states.
-  const int64_t warps = s.batch * s.channels / 8;   // with 4 lanes
-  constexpr int64_t kEnough = 148 * 12;
-  const int level = warps >= kEnough || s.length <= 32 ? 0
-                    : 2 * warps >= kEnough             ? 1
-                    : 8 * warps >= kEnough || s.length <= 64 ? 2 : 3;
+  // channels to fill the GPU that way, a channel gets more lanes, then several
+  // warps that share its states. Measured (us, 16 states, bf16), levels 0..3:
+  //   8 x 2048 x 2048    385  381  571  759     4 x 4096 x 2048   527  421  588  757
+  //   2 x 8192 x 2048    901  585  649  775     1 x 8192 x 2048   901  516  332  439
+  //   64 x 256 x 2048    341  375  627  837     1 x 4096 x 512    453  262  127   80
+  const int64_t rows = s.batch * s.channels;
+  const int level = rows >= 12288 || s.length <= 32 ? 0
+                    : rows >= 3000                  ? 1
+                    : rows >= 1000 || s.length <= 64 ? 2 : 3;
   return with_dtype(a->dtype, [&](auto tag) {
     using T = decltype(tag);
     return with_states(s.states, [&](auto np) -> ferrum_status {

@@ -44,7 +44,7 @@ from ferrum_gpu.device import _handle
 
 MAX_TAPS = 8
 MAX_STATES = 64
-SAVE_STEPS = 64
+SAVE_STEPS = 16
 
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _KINDS = {"rms": 0, "layer": 1}

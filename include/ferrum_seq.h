@@ -36,7 +36,7 @@ enum { FERRUM_NORM_RMS = 0, FERRUM_NORM_LAYER = 1 };
 /* Largest number of states per channel of the scan. */
 #define FERRUM_SCAN_MAX_STATES 64
 /* Steps between the states the scan saves for its gradient. */
-#define FERRUM_SCAN_SAVE_STEPS 64
+#define FERRUM_SCAN_SAVE_STEPS 16
 /* Longest sequence of the long convolution. */
 #define FERRUM_LONG_CONV_MAX_LENGTH (1 << 25)
 
@@ -81,6 +81,7 @@ ferrum_status ferrum_causal_conv1d_step(ferrum_device *dev, const ferrum_conv1d_
                                         void *stream);
 
 /* ---------------------------------------------------------------------------
+ * Row strides of the scan's arrays must fit 32 bits.
  * Selective state space scan, N states per channel, N in [1, 64]:
  *   s  = delta[b,t,d] + delta_bias[d];  dt = delta_softplus ? log(1 + e^s) : s
  *   h[n] = exp(dt * A[d,n]) * h[n] + dt * u[b,t,d] * B[b,t,g,n]
@@ -99,7 +100,7 @@ typedef struct {
   const float *initial_state;               /* (batch, channels, N), optional (zeros) */
   float *final_state;                       /* (batch, channels, N), optional */
   const int32_t *lengths;
-  /* (batch, ceil(length / 64), channels, N): the state in front of every 64th
+  /* (batch, ceil(length / 16), channels, N): the state in front of every 16th
    * step. Optional output of the scan, needed by its gradient. */
   float *saved_states;
   /* gradients (ferrum_selective_scan_bwd) */
