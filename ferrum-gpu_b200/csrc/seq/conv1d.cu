@@ -1,25 +1,31 @@
 // Short causal depthwise convolution over (batch, length, channels):
 //   p[t] = bias + sum_j w[j] x[t-K+1+j],  y = p or p * sigmoid(p)
-// One thread owns one channel over a run of steps and slides a window of K
-// values through registers, so x is read once (and K-1 values again at the
-// start of each run); lanes span adjacent channels, so rows are read in whole
-// segments. The work is 2K operations per 2 moved values: bound by HBM.
+// The work is 2K operations per 2 moved values: bound by HBM. A thread owns
+// VL adjacent channels (16-byte accesses forward, 8-byte in the gradient,
+// single values where the rows are not aligned) over a run of steps, and
+// slides a window of K values through registers, so x is read once, and K-1
+// rows again at the start of each run. It loads four rows ahead of using
+// them. Runs are long (64 steps) where the batch fills the GPU and shorter
+// where it does not.
 //
 // Gradient, with g[t] = dy[t] * act'(p[t]):
 //   dx[s] = sum_j w[j] g[s+K-1-j],  dw[j] = sum_t g[t] x[t-K+1+j],  db = sum_t g[t]
 // The same run of steps recomputes p; the per-run sums of dw and db go to a
 // workspace and are added in a fixed order.
+#include <algorithm>
+#include <type_traits>
+
 #include "seq_common.cuh"
 
 namespace ferrum {
 namespace seq {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kRun = 64;  // steps per thread
+constexpr int kThreads = 128;
+constexpr int kAhead = 4;   // rows loaded ahead
 
 struct ConvSizes {
-  int64_t batch, length, channels, runs, col_blocks;
+  int64_t batch, length, channels, run, runs, col_blocks;
 };
 
 __device__ __forceinline__ int64_t valid_length(const int32_t* lengths, int64_t b, int64_t length) {
@@ -28,115 +34,180 @@ __device__ __forceinline__ int64_t valid_length(const int32_t* lengths, int64_t 
   return n < 0 ? 0 : (n > length ? length : n);
 }
 
-// x at step t (t >= -(K-1)) of one channel: the state in front of the
-// sequence, zero past its end.
-template <class T, int K>
-__device__ __forceinline__ float conv_in(const Rows<T>& x, const T* st, int64_t b, int64_t t,
-                                         int64_t d, int64_t len, int64_t channels) {
-  if (t >= 0) return t < len ? to_f(x.at(b, t)[d]) : 0.f;
-  return st ? to_f(st[(b * (K - 1) + (t + K - 1)) * channels + d]) : 0.f;
+template <int VL>
+__device__ __forceinline__ void clear(float (&v)[VL]) {
+#pragma unroll
+  for (int e = 0; e < VL; ++e) v[e] = 0.f;
 }
 
-template <class T, int K>
+// x at step t (t >= -(K-1)) of VL channels: the state in front of the
+// sequence, zero past its end.
+template <class T, int K, int VL>
+__device__ __forceinline__ void conv_in(const Rows<T>& x, const T* st, int64_t b, int64_t t,
+                                        int64_t d, int64_t len, int64_t channels, float (&v)[VL]) {
+  clear(v);
+  if (t >= 0) {
+    if (t < len) load_vec<T, VL>(x.at(b, t) + d, v);
+  } else if (st) {
+    load_vec<T, VL>(st + (b * (K - 1) + (t + K - 1)) * channels + d, v);
+  }
+}
+
+// Blocks run over (column block, run, sequence).
+struct ConvPlace {
+  int64_t d, run, b;
+  template <int VL>
+  static __device__ __forceinline__ ConvPlace of(const ConvSizes& s) {
+    int64_t q = blockIdx.x;
+    ConvPlace p;
+    p.d = (q % s.col_blocks * kThreads + threadIdx.x) * VL;
+    q /= s.col_blocks;
+    p.run = q % s.runs, p.b = q / s.runs;
+    return p;
+  }
+};
+
+template <class T, int K, int VL>
 __global__ void __launch_bounds__(kThreads)
 conv1d_fwd_kernel(Rows<T> x, Rows<T> y, const float* __restrict__ weight,
                   const float* __restrict__ bias, const T* st, T* fin,
                   const int32_t* __restrict__ lengths, ConvSizes s, bool silu) {
-  int64_t q = blockIdx.x;
-  const int64_t d = (q % s.col_blocks) * kThreads + threadIdx.x;
-  q /= s.col_blocks;
-  const int64_t t0 = (q % s.runs) * kRun, b = q / s.runs;
+  const ConvPlace at = ConvPlace::of<VL>(s);
+  const int64_t d = at.d, b = at.b, t0 = at.run * s.run;
   if (d >= s.channels) return;
   const int64_t len = valid_length(lengths, b, s.length);
-  float w[K], win[K];
+  float w[K][VL], win[K][VL], bs[VL];
 #pragma unroll
-  for (int j = 0; j < K; ++j) w[j] = weight[d * K + j];
-  const float bs = bias ? bias[d] : 0.f;
+  for (int j = 0; j < K; ++j)
 #pragma unroll
-  for (int j = 1; j < K; ++j) win[j] = conv_in<T, K>(x, st, b, t0 - K + j, d, len, s.channels);
-  const int64_t t1 = t0 + kRun < s.length ? t0 + kRun : s.length;
-  for (int64_t t = t0; t < t1; ++t) {
+    for (int e = 0; e < VL; ++e) w[j][e] = weight[(d + e) * K + j];
 #pragma unroll
-    for (int j = 0; j + 1 < K; ++j) win[j] = win[j + 1];
-    win[K - 1] = t < len ? to_f(x.at(b, t)[d]) : 0.f;
-    float p = bs;
+  for (int e = 0; e < VL; ++e) bs[e] = bias ? bias[d + e] : 0.f;
 #pragma unroll
-    for (int j = 0; j < K; ++j) p = fmaf(w[j], win[j], p);
-    if (silu) p *= sigmoid_f(p);
-    y.at(b, t)[d] = from_f<T>(t < len ? p : 0.f);
+  for (int j = 1; j < K; ++j) conv_in<T, K, VL>(x, st, b, t0 - K + j, d, len, s.channels, win[j]);
+  const int64_t t1 = t0 + s.run < s.length ? t0 + s.run : s.length;
+  for (int64_t t = t0; t < t1; t += kAhead) {
+    float in[kAhead][VL];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      clear(in[i]);
+      if (t + i < len) load_vec<T, VL>(x.at(b, t + i) + d, in[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (t + i >= t1) break;
+      float p[VL];
+#pragma unroll
+      for (int e = 0; e < VL; ++e) {
+#pragma unroll
+        for (int j = 0; j + 1 < K; ++j) win[j][e] = win[j + 1][e];
+        win[K - 1][e] = in[i][e];
+        float v = bs[e];
+#pragma unroll
+        for (int j = 0; j < K; ++j) v = fmaf(w[j][e], win[j][e], v);
+        if (silu) v *= sigmoid_f(v);
+        p[e] = t + i < len ? v : 0.f;
+      }
+      store_vec<T, VL>(y.at(b, t + i) + d, p);
+    }
   }
   if (t0 == 0 && fin != nullptr) {
     // all reads come first: fin may be the initial state's array
-    T keep[K];
+    float keep[K][VL];
 #pragma unroll
     for (int i = 0; i + 1 < K; ++i)
-      keep[i] = from_f<T>(conv_in<T, K>(x, st, b, len - (K - 1) + i, d, len, s.channels));
+      conv_in<T, K, VL>(x, st, b, len - (K - 1) + i, d, len, s.channels, keep[i]);
 #pragma unroll
-    for (int i = 0; i + 1 < K; ++i) fin[(b * (K - 1) + i) * s.channels + d] = keep[i];
+    for (int i = 0; i + 1 < K; ++i)
+      store_vec<T, VL>(fin + (b * (K - 1) + i) * s.channels + d, keep[i]);
   }
 }
 
-template <class T, int K>
+template <class T, int K, int VL>
 __global__ void __launch_bounds__(kThreads)
 conv1d_bwd_kernel(Rows<T> x, Rows<T> dy, Rows<T> dx, const float* __restrict__ weight,
                   const float* __restrict__ bias, const T* st, const T* dfin, T* dst,
                   const int32_t* __restrict__ lengths, float* __restrict__ part, ConvSizes s,
                   bool silu) {
-  int64_t q = blockIdx.x;
-  const int64_t d = (q % s.col_blocks) * kThreads + threadIdx.x;
-  q /= s.col_blocks;
-  const int64_t run = q % s.runs, t0 = run * kRun, b = q / s.runs;
+  const ConvPlace at = ConvPlace::of<VL>(s);
+  const int64_t d = at.d, b = at.b, t0 = at.run * s.run;
   if (d >= s.channels) return;
   const int64_t len = valid_length(lengths, b, s.length);
-  float w[K], win[K], g[K], dw[K], db = 0.f;
+  float w[K][VL], win[K][VL], g[K][VL], dw[K][VL], db[VL], bs[VL];
 #pragma unroll
-  for (int j = 0; j < K; ++j) w[j] = weight[d * K + j], dw[j] = 0.f, g[j] = 0.f;
-  const float bs = bias ? bias[d] : 0.f;
+  for (int e = 0; e < VL; ++e) {
+    bs[e] = bias ? bias[d + e] : 0.f, db[e] = 0.f;
 #pragma unroll
-  for (int j = 1; j < K; ++j) win[j] = conv_in<T, K>(x, st, b, t0 - K + j, d, len, s.channels);
-  const int64_t t1 = t0 + kRun < s.length ? t0 + kRun : s.length;
+    for (int j = 0; j < K; ++j) w[j][e] = weight[(d + e) * K + j], dw[j][e] = 0.f, g[j][e] = 0.f;
+  }
+#pragma unroll
+  for (int j = 1; j < K; ++j) conv_in<T, K, VL>(x, st, b, t0 - K + j, d, len, s.channels, win[j]);
+  const int64_t t1 = t0 + s.run < s.length ? t0 + s.run : s.length;
   // g[j] holds the gradient of p at step t-K+1+j; after it moved on to step t,
   // dx of step t-K+1 is complete.
-  for (int64_t t = t0; t < t1 + K - 1; ++t) {
+  for (int64_t t = t0; t < t1 + K - 1; t += kAhead) {
+    float in[kAhead][VL], gin[kAhead][VL];
 #pragma unroll
-    for (int j = 0; j + 1 < K; ++j) win[j] = win[j + 1], g[j] = g[j + 1];
-    float gt = 0.f;
-    win[K - 1] = 0.f;
-    if (t < len) {
-      win[K - 1] = to_f(x.at(b, t)[d]);
-      gt = to_f(dy.at(b, t)[d]);
-      if (silu) {
-        float p = bs;
-#pragma unroll
-        for (int j = 0; j < K; ++j) p = fmaf(w[j], win[j], p);
-        const float sg = sigmoid_f(p);
-        gt *= sg * (1.f + p * (1.f - sg));
-      }
-      if (t < t1) {
-        db += gt;
-#pragma unroll
-        for (int j = 0; j < K; ++j) dw[j] = fmaf(gt, win[j], dw[j]);
+    for (int i = 0; i < kAhead; ++i) {
+      clear(in[i]), clear(gin[i]);
+      if (t + i < len && t + i < t1 + K - 1) {
+        load_vec<T, VL>(x.at(b, t + i) + d, in[i]);
+        load_vec<T, VL>(dy.at(b, t + i) + d, gin[i]);
       }
     }
-    g[K - 1] = gt;
-    const int64_t r = t - K + 1;
-    if (r < t0 && !(t0 == 0 && dst != nullptr)) continue;
-    float o = 0.f;
 #pragma unroll
-    for (int j = 0; j < K; ++j) o = fmaf(w[j], g[K - 1 - j], o);
-    // a final state is the input's last K-1 values
-    const int64_t i = r - (len - (K - 1));
-    if (dfin != nullptr && i >= 0 && i < K - 1)
-      o += to_f(dfin[(b * (K - 1) + i) * s.channels + d]);
-    if (r >= 0)
-      dx.at(b, r)[d] = from_f<T>(r < len ? o : 0.f);
-    else if (r >= -(K - 1))
-      dst[(b * (K - 1) + (r + K - 1)) * s.channels + d] = from_f<T>(o);
+    for (int i = 0; i < kAhead; ++i) {
+      if (t + i >= t1 + K - 1) break;
+      const int64_t r = t + i - K + 1;
+      float o[VL];
+#pragma unroll
+      for (int e = 0; e < VL; ++e) {
+#pragma unroll
+        for (int j = 0; j + 1 < K; ++j) win[j][e] = win[j + 1][e], g[j][e] = g[j + 1][e];
+        win[K - 1][e] = in[i][e];
+        float gt = gin[i][e];
+        if (silu) {
+          float p = bs[e];
+#pragma unroll
+          for (int j = 0; j < K; ++j) p = fmaf(w[j][e], win[j][e], p);
+          const float sg = sigmoid_f(p);
+          gt *= sg * (1.f + p * (1.f - sg));
+        }
+        if (t + i >= len) gt = 0.f;     // whatever the padding's p
+        g[K - 1][e] = gt;
+        if (t + i < t1) {
+          db[e] += gt;
+#pragma unroll
+          for (int j = 0; j < K; ++j) dw[j][e] = fmaf(gt, win[j][e], dw[j][e]);
+        }
+        o[e] = 0.f;
+#pragma unroll
+        for (int j = 0; j < K; ++j) o[e] = fmaf(w[j][e], g[K - 1 - j][e], o[e]);
+      }
+      if (r < t0 && !(t0 == 0 && dst != nullptr)) continue;
+      // a final state is the input's last K-1 values
+      const int64_t f = r - (len - (K - 1));
+      if (dfin != nullptr && f >= 0 && f < K - 1) {
+        float q[VL];
+        load_vec<T, VL>(dfin + (b * (K - 1) + f) * s.channels + d, q);
+#pragma unroll
+        for (int e = 0; e < VL; ++e) o[e] += q[e];
+      }
+      if (r >= 0) {
+        if (r >= len) clear(o);
+        store_vec<T, VL>(dx.at(b, r) + d, o);
+      } else if (r >= -(K - 1)) {
+        store_vec<T, VL>(dst + (b * (K - 1) + (r + K - 1)) * s.channels + d, o);
+      }
+    }
   }
-  float* o = part + (b * s.runs + run) * (K + 1) * s.channels;
+  float* o = part + (b * s.runs + at.run) * (K + 1) * s.channels;
 #pragma unroll
-  for (int j = 0; j < K; ++j) o[d * K + j] = dw[j];
-  o[K * s.channels + d] = db;
+  for (int e = 0; e < VL; ++e) {
+#pragma unroll
+    for (int j = 0; j < K; ++j) o[(d + e) * K + j] = dw[j][e];
+    o[K * s.channels + d + e] = db[e];
+  }
 }
 
 template <class F>
@@ -179,11 +250,14 @@ ferrum_status check_conv(const ferrum_device* dev, const ferrum_conv1d_args* a, 
   return check_ptr(a->dbias, 4, true, what, "dbias");
 }
 
-ConvSizes conv_sizes(const ferrum_conv1d_args* a) {
+ConvSizes conv_sizes(const ferrum_conv1d_args* a, int vl) {
   ConvSizes s;
   s.batch = (int64_t)a->batch, s.length = (int64_t)a->length, s.channels = (int64_t)a->channels;
-  s.runs = s.length > 0 ? ceil_div(s.length, kRun) : 1;  // an empty prompt still copies its state
-  s.col_blocks = ceil_div(s.channels, kThreads);
+  s.col_blocks = ceil_div(s.channels, kThreads * vl);
+  // at least 1024 threads an SM, if that takes runs of no less than 8 steps
+  s.run = 64;
+  while (s.run > 8 && s.batch * s.col_blocks * ceil_div(s.length, s.run) < 148 * 8) s.run /= 2;
+  s.runs = s.length > 0 ? ceil_div(s.length, s.run) : 1;  // an empty prompt still copies its state
   return s;
 }
 
@@ -191,21 +265,46 @@ ferrum_status grid_ok(int64_t blocks, const char* what) {
   return blocks > 0x7fffffff ? invalid(what, "too many blocks for one launch") : FERRUM_OK;
 }
 
+// Whether all arrays can be accessed `bytes` at a time.
+bool conv_vec(const ferrum_conv1d_args* a, bool bwd, int vl) {
+  const size_t e = dtype_size(a->dtype), bytes = std::min<size_t>(16, vl * e);
+  auto ok = [&](const ferrum_rows& r) {
+    return aligned(r.ptr, bytes) && r.batch_stride * (int64_t)e % (int64_t)bytes == 0 &&
+           r.row_stride * (int64_t)e % (int64_t)bytes == 0;
+  };
+  bool v = a->channels % vl == 0 && ok(a->x) && aligned(a->initial_state, bytes);
+  if (!bwd) return v && ok(a->y) && aligned(a->final_state, bytes);
+  return v && ok(a->dy) && ok(a->dx) && aligned(a->dfinal_state, bytes) &&
+         aligned(a->dinitial_state, bytes);
+}
+
+// f(taps, values per thread): wide accesses for the taps in use (up to 4)
+template <int WIDE, class F>
+ferrum_status with_conv(int taps, bool vec, F f) {
+  return with_taps(taps, [&](auto k) {
+    if constexpr (decltype(k)::value <= 4) {
+      if (vec) return f(k, std::integral_constant<int, WIDE>());
+    }
+    return f(k, std::integral_constant<int, 1>());
+  });
+}
+
 ferrum_status conv_fwd(ferrum_device* dev, const ferrum_conv1d_args* a, cudaStream_t stream,
                        const char* what) {
   if (a->batch == 0 || a->channels == 0) return FERRUM_OK;
-  const ConvSizes s = conv_sizes(a);
-  const int64_t blocks = s.batch * s.runs * s.col_blocks;
-  if (ferrum_status st = grid_ok(blocks, what)) return st;
   DeviceGuard guard(dev->ordinal);
   if (guard.status() != cudaSuccess) return cuda_error(guard.status(), "cudaSetDevice");
   return with_dtype(a->dtype, [&](auto tag) {
     using T = decltype(tag);
-    return with_taps(a->taps, [&](auto k) {
+    return with_conv<8>(a->taps, conv_vec(a, false, 8), [&](auto k, auto vl) -> ferrum_status {
+      const ConvSizes s = conv_sizes(a, decltype(vl)::value);
+      const int64_t blocks = s.batch * s.runs * s.col_blocks;
+      if (ferrum_status st = grid_ok(blocks, what)) return st;
       launch_detail::clear_stale_error();
-      conv1d_fwd_kernel<T, decltype(k)::value><<<(unsigned)blocks, kThreads, 0, stream>>>(
-          rows_of<T>(a->x), rows_of<T>(a->y), a->weight, a->bias, (const T*)a->initial_state,
-          (T*)a->final_state, a->lengths, s, a->silu != 0);
+      conv1d_fwd_kernel<T, decltype(k)::value, decltype(vl)::value>
+          <<<(unsigned)blocks, kThreads, 0, stream>>>(
+              rows_of<T>(a->x), rows_of<T>(a->y), a->weight, a->bias, (const T*)a->initial_state,
+              (T*)a->final_state, a->lengths, s, a->silu != 0);
       return launched(what);
     });
   });
@@ -248,38 +347,33 @@ ferrum_status ferrum_causal_conv1d_bwd(ferrum_device* dev, const ferrum_conv1d_a
     if (ferrum_status s = check_conv(dev, a, what, true)) return s;
     if (a->channels == 0) return FERRUM_OK;
     cudaStream_t st = (cudaStream_t)stream;
-    const ConvSizes z = conv_sizes(a);
-    const int64_t parts = z.batch * z.runs, blocks = parts * z.col_blocks;
-    if (ferrum_status s = grid_ok(blocks, what)) return s;
     DeviceGuard guard(dev->ordinal);
     if (guard.status() != cudaSuccess) return cuda_error(guard.status(), "cudaSetDevice");
-    const int64_t cols = (int64_t)(a->taps + 1) * z.channels;
-    PoolBuffer ws(dev, (size_t)(parts * cols) * 4 + 4, st);
-    PoolBuffer sums(dev, (size_t)cols * 4, st);
-    if (ws.status() != cudaSuccess) return cuda_error(ws.status(), "workspace");
-    if (sums.status() != cudaSuccess) return cuda_error(sums.status(), "workspace");
-    if (parts > 0) {
-      ferrum_status s = with_dtype(a->dtype, [&](auto tag) {
-        using T = decltype(tag);
-        return with_taps(a->taps, [&](auto k) {
+    return with_dtype(a->dtype, [&](auto tag) {
+      using T = decltype(tag);
+      return with_conv<4>(a->taps, conv_vec(a, true, 4), [&](auto k, auto vl) -> ferrum_status {
+        const ConvSizes z = conv_sizes(a, decltype(vl)::value);
+        const int64_t parts = z.batch * z.runs, blocks = parts * z.col_blocks;
+        if (ferrum_status s = grid_ok(blocks, what)) return s;
+        const int64_t cols = (int64_t)(a->taps + 1) * z.channels;
+        PoolBuffer ws(dev, (size_t)(parts * cols) * 4 + 4, st);
+        if (ws.status() != cudaSuccess) return cuda_error(ws.status(), "workspace");
+        float* part = ws.as<float>();
+        if (parts > 0) {
           launch_detail::clear_stale_error();
-          conv1d_bwd_kernel<T, decltype(k)::value><<<(unsigned)blocks, kThreads, 0, st>>>(
-              rows_of<T>(a->x), rows_of<T>(a->dy), rows_of<T>(a->dx), a->weight, a->bias,
-              (const T*)a->initial_state, (const T*)a->dfinal_state, (T*)a->dinitial_state,
-              a->lengths, ws.as<float>(), z, a->silu != 0);
-          return launched(what);
-        });
+          conv1d_bwd_kernel<T, decltype(k)::value, decltype(vl)::value>
+              <<<(unsigned)blocks, kThreads, 0, st>>>(
+                  rows_of<T>(a->x), rows_of<T>(a->dy), rows_of<T>(a->dx), a->weight, a->bias,
+                  (const T*)a->initial_state, (const T*)a->dfinal_state, (T*)a->dinitial_state,
+                  a->lengths, part, z, a->silu != 0);
+          if (ferrum_status s = launched(what)) return s;
+        }
+        cudaError_t e = launch_sum_rows(part, parts, a->taps * z.channels, cols, a->dweight, st);
+        if (e == cudaSuccess && a->dbias)
+          e = launch_sum_rows(part + a->taps * z.channels, parts, z.channels, cols, a->dbias, st);
+        return e == cudaSuccess ? FERRUM_OK : cuda_error(e, what);
       });
-      if (s) return s;
-    }
-    cudaError_t e = launch_sum_rows(ws.as<float>(), parts, cols, sums.as<float>(), st);
-    if (e != cudaSuccess) return cuda_error(e, what);
-    e = cudaMemcpyAsync(a->dweight, sums.as<float>(), (size_t)a->taps * z.channels * 4,
-                        cudaMemcpyDeviceToDevice, st);
-    if (e == cudaSuccess && a->dbias)
-      e = cudaMemcpyAsync(a->dbias, sums.as<float>() + a->taps * z.channels,
-                          (size_t)z.channels * 4, cudaMemcpyDeviceToDevice, st);
-    return e == cudaSuccess ? FERRUM_OK : cuda_error(e, what);
+    });
   });
 }
 

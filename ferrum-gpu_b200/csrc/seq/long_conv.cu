@@ -611,7 +611,8 @@ ferrum_status fused_dkernel(ferrum_device* dev, const Staged<T>& x, const Staged
         x.rows(), dy.rows(), parts > 1 ? ws.as<float>() : dk, tw, s, share, x.vec(), dy.vec());
     if (ferrum_status r = launched(what)) return r;
     if (parts == 1) return FERRUM_OK;
-    cudaError_t e = launch_sum_rows(ws.as<float>(), parts, s.channels * s.taps, dk, st);
+    cudaError_t e = launch_sum_rows(ws.as<float>(), parts, s.channels * s.taps,
+                                    s.channels * s.taps, dk, st);
     return e == cudaSuccess ? FERRUM_OK : cuda_error(e, what);
   });
 }

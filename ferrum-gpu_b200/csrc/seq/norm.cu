@@ -8,28 +8,22 @@
 // gradient, dv = i * (dn - n * mean(dn * n) - [layer] mean(dn)).
 // (A row of one value leaves dn - n * mean(dn * n) = dn (1 - n^2) to a
 // difference of equals; there 1 - n^2 = eps i^2 is used instead.)
-// A few operations per moved value: bound by HBM. One block per row (behind:
-// per group of a row); the parameters' gradients are column sums over the
-// rows, taken by a second kernel from the rows' statistics.
+// A few operations per moved value, so HBM bounds it: every array is read and
+// written once. A row (behind: a group of one) stays in the registers of a
+// warp, or of a block of 128 to 1024 threads for wide rows, in 16-byte
+// accesses where the arrays allow. The gradient kernel also keeps the column
+// sums (dweight, dbias, dscale) of all the rows that a warp or block takes, so
+// no second pass over the arrays is needed; their few hundred partial sums
+// are added in a fixed order.
+#include <algorithm>
+
 #include "seq_common.cuh"
 
 namespace ferrum {
 namespace seq {
 namespace {
 
-constexpr int kThreads = 256;
-
-// Sum over the block, in every thread, in a fixed order.
-__device__ float block_sum(float v, float* sh) {
-  v = warp_sum(v);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float s = 0.f;
-#pragma unroll
-  for (int i = 0; i < kThreads / 32; ++i) s += sh[i];
-  return s;
-}
+constexpr int64_t kMaxWidth = 32768;
 
 struct NormArgs {
   int64_t rows, channels, groups, width;  // width = channels / groups
@@ -37,7 +31,48 @@ struct NormArgs {
   bool layer, inside;
   const float *weight, *bias, *scale;
   int64_t x_st, gate_st, res_st, y_st, r_st, dy_st, dr_st, dx_st, dgate_st, dres_st;
-  float4* stats;  // (rows * groups): mean, 1 / deviation, mean of dn, mean of dn * n
+};
+
+// Sums of N values over the TPR threads of a row, in every thread, in a fixed
+// order. Blocks alternate between two buffers: one barrier per call.
+template <int TPR, int N>
+__device__ __forceinline__ void row_sum(float (&v)[N], float* sh, int& flip) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = warp_sum(v[i]);
+  if constexpr (TPR > 32) {
+    constexpr int W = TPR / 32;
+    float* buf = sh + flip * W * 3;
+    flip ^= 1;
+    const int w = threadIdx.x >> 5;
+    if ((threadIdx.x & 31) == 0)
+#pragma unroll
+      for (int i = 0; i < N; ++i) buf[i * W + w] = v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float s = buf[i * W];
+      for (int k = 1; k < W; ++k) s += buf[i * W + k];
+      v[i] = s;
+    }
+  }
+}
+
+// The rows of one warp or block ("unit"): its group, its lane in the row.
+template <int TPR, int VL, int NC>
+struct Unit {
+  static constexpr int THREADS = TPR == 32 ? 256 : TPR;
+  static constexpr int EPT = NC * VL;
+  int64_t index, count, g, first, step;
+  int lane;
+  __device__ __forceinline__ Unit(int64_t groups) {
+    index = ((int64_t)blockIdx.x * THREADS + threadIdx.x) / TPR;
+    count = (int64_t)gridDim.x * (THREADS / TPR);
+    g = index % groups, first = index / groups, step = count / groups;
+    if (index >= step * groups) first = INT64_MAX;   // units beyond a multiple of the groups
+    lane = threadIdx.x % TPR;
+  }
+  // column of chunk k in the group, and whether it lies in it
+  __device__ __forceinline__ int col(int k) const { return (k * TPR + lane) * VL; }
 };
 
 // Gradient of a value from that of its normalised value n.
@@ -47,138 +82,6 @@ __device__ __forceinline__ float norm_grad(const NormArgs& a, float inv, float d
   return inv * (dn - mean_dn - n * mean_dnn);
 }
 
-// r (a row of the residual stream) in front of a block
-template <class T, class R>
-__device__ __forceinline__ float before_value(const T* x, const R* res, const float* scale,
-                                              int64_t c) {
-  float v = res ? to_f(res[c]) : 0.f;
-  if (x) v = fmaf(scale ? scale[c] : 1.f, to_f(x[c]), v);
-  return v;
-}
-
-template <class T, class R>
-__global__ void __launch_bounds__(kThreads)
-norm_before_kernel(NormArgs a, const T* x, const R* res, T* y, R* r) {
-  __shared__ float sh[kThreads / 32];
-  const int64_t row = blockIdx.x;
-  if (x) x += row * a.x_st;
-  if (res) res += row * a.res_st;
-  y += row * a.y_st;
-  float s = 0.f;
-  for (int64_t c = threadIdx.x; c < a.channels; c += kThreads)
-    s += before_value(x, res, a.scale, c);
-  const float mean = a.layer ? block_sum(s, sh) / (float)a.channels : 0.f;
-  float q = 0.f;
-  for (int64_t c = threadIdx.x; c < a.channels; c += kThreads) {
-    const float v = before_value(x, res, a.scale, c) - mean;
-    q = fmaf(v, v, q);
-  }
-  const float inv = 1.f / sqrtf(block_sum(q, sh) / (float)a.channels + a.eps);
-  for (int64_t c = threadIdx.x; c < a.channels; c += kThreads) {
-    const float v = before_value(x, res, a.scale, c);
-    const float n = (v - mean) * inv;
-    if (r) r[row * a.r_st + c] = from_f<R>(v);
-    y[c] = from_f<T>(fmaf(n, a.weight[c], a.bias ? a.bias[c] : 0.f));
-  }
-}
-
-template <class T, class R>
-__global__ void __launch_bounds__(kThreads)
-norm_before_bwd_kernel(NormArgs a, const R* r, const T* dy, const R* dr, T* dx, R* dres) {
-  __shared__ float sh[kThreads / 32];
-  const int64_t row = blockIdx.x;
-  r += row * a.r_st, dy += row * a.dy_st;
-  const float w = 1.f / (float)a.channels;
-  float s = 0.f;
-  for (int64_t c = threadIdx.x; c < a.channels; c += kThreads) s += to_f(r[c]);
-  const float mean = a.layer ? block_sum(s, sh) * w : 0.f;
-  float q = 0.f, g1 = 0.f, g2 = 0.f;
-  for (int64_t c = threadIdx.x; c < a.channels; c += kThreads) {
-    const float v = to_f(r[c]) - mean, g = to_f(dy[c]) * a.weight[c];
-    q = fmaf(v, v, q), g1 += g, g2 = fmaf(g, v, g2);
-  }
-  const float inv = 1.f / sqrtf(block_sum(q, sh) * w + a.eps);
-  g1 = a.layer ? block_sum(g1, sh) * w : 0.f;
-  g2 = block_sum(g2, sh) * w * inv;
-  if (threadIdx.x == 0) a.stats[row] = make_float4(mean, inv, g1, g2);
-  for (int64_t c = threadIdx.x; c < a.channels; c += kThreads) {
-    const float n = (to_f(r[c]) - mean) * inv;
-    float o = norm_grad(a, inv, to_f(dy[c]) * a.weight[c], n, g1, g2);
-    if (dr) o += to_f(dr[row * a.dr_st + c]);
-    if (dres) dres[row * a.dres_st + c] = from_f<R>(o);
-    if (dx) dx[row * a.dx_st + c] = from_f<T>(a.scale ? o * a.scale[c] : o);
-  }
-}
-
-// Column sums over a block's share of the rows: part[(share * 3 + k) * channels + c]
-// for k = dweight, dbias, dscale.
-template <class T, class R>
-__global__ void __launch_bounds__(kThreads)
-norm_before_cols_kernel(NormArgs a, const T* x, const R* r, const T* dy, const R* dr,
-                        float* part, int64_t col_blocks, int64_t share) {
-  const int64_t c = (blockIdx.x % col_blocks) * kThreads + threadIdx.x, p = blockIdx.x / col_blocks;
-  if (c >= a.channels) return;
-  const int64_t r1 = (p + 1) * share < a.rows ? (p + 1) * share : a.rows;
-  const float w = a.weight[c];
-  float dw = 0.f, db = 0.f, ds = 0.f;
-  for (int64_t i = p * share; i < r1; ++i) {
-    const float4 st = a.stats[i];
-    const float g = to_f(dy[i * a.dy_st + c]), n = (to_f(r[i * a.r_st + c]) - st.x) * st.y;
-    dw = fmaf(g, n, dw);
-    db += g;
-    if (x) {
-      float o = norm_grad(a, st.y, g * w, n, st.z, st.w);
-      if (dr) o += to_f(dr[i * a.dr_st + c]);
-      ds = fmaf(o, to_f(x[i * a.x_st + c]), ds);
-    }
-  }
-  part[(p * 3 + 0) * a.channels + c] = dw;
-  part[(p * 3 + 1) * a.channels + c] = db;
-  part[(p * 3 + 2) * a.channels + c] = ds;
-}
-
-template <class T>
-__device__ __forceinline__ float after_value(const NormArgs& a, const T* x, const T* gate,
-                                             int64_t c) {
-  float v = to_f(x[c]);
-  if (a.inside && gate) {
-    const float g = to_f(gate[c]);
-    v *= g * sigmoid_f(g);
-  }
-  return v;
-}
-
-template <class T, class R>
-__global__ void __launch_bounds__(kThreads)
-norm_after_kernel(NormArgs a, const T* x, const T* gate, const R* res, T* y) {
-  __shared__ float sh[kThreads / 32];
-  const int64_t row = blockIdx.x / a.groups, c0 = (blockIdx.x % a.groups) * a.width,
-                c1 = c0 + a.width;
-  x += row * a.x_st;
-  if (gate) gate += row * a.gate_st;
-  if (res) res += row * a.res_st;
-  y += row * a.y_st;
-  float s = 0.f;
-  for (int64_t c = c0 + threadIdx.x; c < c1; c += kThreads) s += after_value(a, x, gate, c);
-  const float mean = a.layer ? block_sum(s, sh) / (float)a.width : 0.f;
-  float q = 0.f;
-  for (int64_t c = c0 + threadIdx.x; c < c1; c += kThreads) {
-    const float v = after_value(a, x, gate, c) - mean;
-    q = fmaf(v, v, q);
-  }
-  const float inv = 1.f / sqrtf(block_sum(q, sh) / (float)a.width + a.eps);
-  for (int64_t c = c0 + threadIdx.x; c < c1; c += kThreads) {
-    float p = fmaf((after_value(a, x, gate, c) - mean) * inv, a.weight[c],
-                   a.bias ? a.bias[c] : 0.f);
-    if (!a.inside && gate) {
-      const float g = to_f(gate[c]);
-      p *= g * sigmoid_f(g);
-    }
-    const float base = res ? to_f(res[c]) : 0.f;
-    y[c] = from_f<T>(fmaf(a.scale ? a.scale[c] : 1.f, p, base));
-  }
-}
-
 // d silu(g) / dg, and silu(g)
 __device__ __forceinline__ void silu_grad(float g, float& f, float& df) {
   const float sg = sigmoid_f(g);
@@ -186,82 +89,325 @@ __device__ __forceinline__ void silu_grad(float g, float& f, float& df) {
   df = sg * (1.f + g * (1.f - sg));
 }
 
-template <class T>
-__global__ void __launch_bounds__(kThreads)
-norm_after_bwd_kernel(NormArgs a, const T* x, const T* gate, const T* dy, T* dx, T* dgate) {
-  __shared__ float sh[kThreads / 32];
-  const int64_t row = blockIdx.x / a.groups, c0 = (blockIdx.x % a.groups) * a.width,
-                c1 = c0 + a.width;
-  x += row * a.x_st, dy += row * a.dy_st, dx += row * a.dx_st;
-  if (gate) gate += row * a.gate_st, dgate += row * a.dgate_st;
+// mean and 1 / deviation of a row held as v (zeros beyond its end)
+template <int TPR, int VL, int NC>
+__device__ __forceinline__ void row_stats(const NormArgs& a, const Unit<TPR, VL, NC>& u,
+                                          const float (&v)[NC][VL], float& mean, float& inv,
+                                          float* sh, int& flip) {
   const float w = 1.f / (float)a.width;
-  float s = 0.f;
-  for (int64_t c = c0 + threadIdx.x; c < c1; c += kThreads) s += after_value(a, x, gate, c);
-  const float mean = a.layer ? block_sum(s, sh) * w : 0.f;
-  // gradient of the normalised value of column c
-  auto dnorm = [&](int64_t c) {
-    float g = to_f(dy[c]) * (a.scale ? a.scale[c] : 1.f) * a.weight[c];
-    if (!a.inside && gate) {
-      const float z = to_f(gate[c]);
-      g *= z * sigmoid_f(z);
-    }
-    return g;
-  };
-  float q = 0.f, g1 = 0.f, g2 = 0.f;
-  for (int64_t c = c0 + threadIdx.x; c < c1; c += kThreads) {
-    const float v = after_value(a, x, gate, c) - mean, g = dnorm(c);
-    q = fmaf(v, v, q), g1 += g, g2 = fmaf(g, v, g2);
+  float q[1];
+  mean = 0.f;
+  if (a.layer) {
+    q[0] = 0.f;
+#pragma unroll
+    for (int k = 0; k < NC; ++k)
+#pragma unroll
+      for (int e = 0; e < VL; ++e) q[0] += v[k][e];
+    row_sum<TPR>(q, sh, flip);
+    mean = q[0] * w;
   }
-  const float inv = 1.f / sqrtf(block_sum(q, sh) * w + a.eps);
-  g1 = a.layer ? block_sum(g1, sh) * w : 0.f;
-  g2 = block_sum(g2, sh) * w * inv;
-  if (threadIdx.x == 0) a.stats[blockIdx.x] = make_float4(mean, inv, g1, g2);
-  for (int64_t c = c0 + threadIdx.x; c < c1; c += kThreads) {
-    const float n = (after_value(a, x, gate, c) - mean) * inv;
-    const float dv = norm_grad(a, inv, dnorm(c), n, g1, g2);
-    if (!gate) {
-      dx[c] = from_f<T>(dv);
-      continue;
+  q[0] = 0.f;
+#pragma unroll
+  for (int k = 0; k < NC; ++k)
+    if (u.col(k) < a.width)
+#pragma unroll
+      for (int e = 0; e < VL; ++e) q[0] = fmaf(v[k][e] - mean, v[k][e] - mean, q[0]);
+  row_sum<TPR>(q, sh, flip);
+  inv = 1.f / sqrtf(fmaf(q[0], w, a.eps));
+}
+
+// VL floats of a parameter, or a constant where it is absent
+template <int VL>
+__device__ __forceinline__ void load_param(const float* p, int64_t c, float (&v)[VL], float other) {
+  if (p) {
+    load_vec<float, VL>(p + c, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < VL; ++e) v[e] = other;
+  }
+}
+
+template <class T, class R, int TPR, int VL, int NC>
+__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, 1)
+norm_before_kernel(NormArgs a, const T* x, const R* res, T* y, R* r) {
+  __shared__ float sh[2 * 3 * TPR / 32];
+  const Unit<TPR, VL, NC> u(a.groups);
+  int flip = 0;
+  for (int64_t row = u.first; row < a.rows; row += u.step) {
+    float v[NC][VL];
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      const int c = u.col(k);
+#pragma unroll
+      for (int e = 0; e < VL; ++e) v[k][e] = 0.f;
+      if (c >= a.width) continue;
+      if (res) load_vec<R, VL>(res + row * a.res_st + c, v[k]);
+      if (x) {
+        float xv[VL], sc[VL];
+        load_vec<T, VL>(x + row * a.x_st + c, xv);
+        load_param<VL>(a.scale, c, sc, 1.f);
+#pragma unroll
+        for (int e = 0; e < VL; ++e) v[k][e] = fmaf(sc[e], xv[e], v[k][e]);
+      }
+      if (r) store_vec<R, VL>(r + row * a.r_st + c, v[k]);
     }
-    float f, df;
-    silu_grad(to_f(gate[c]), f, df);
-    if (a.inside) {
-      dx[c] = from_f<T>(dv * f);
-      dgate[c] = from_f<T>(dv * to_f(x[c]) * df);
-    } else {
-      dx[c] = from_f<T>(dv);
-      const float p = fmaf(n, a.weight[c], a.bias ? a.bias[c] : 0.f);
-      dgate[c] = from_f<T>(to_f(dy[c]) * (a.scale ? a.scale[c] : 1.f) * p * df);
+    float mean, inv;
+    row_stats(a, u, v, mean, inv, sh, flip);
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      const int c = u.col(k);
+      if (c >= a.width) continue;
+      float w[VL], bs[VL];
+      load_vec<float, VL>(a.weight + c, w);
+      load_param<VL>(a.bias, c, bs, 0.f);
+#pragma unroll
+      for (int e = 0; e < VL; ++e) v[k][e] = fmaf((v[k][e] - mean) * inv, w[e], bs[e]);
+      store_vec<T, VL>(y + row * a.y_st + c, v[k]);
     }
   }
 }
 
-template <class T>
-__global__ void __launch_bounds__(kThreads)
-norm_after_cols_kernel(NormArgs a, const T* x, const T* gate, const T* dy, float* part,
-                       int64_t col_blocks, int64_t share) {
-  const int64_t c = (blockIdx.x % col_blocks) * kThreads + threadIdx.x, p = blockIdx.x / col_blocks;
-  if (c >= a.channels) return;
-  const int64_t r1 = (p + 1) * share < a.rows ? (p + 1) * share : a.rows;
-  const float w = a.weight[c], bs = a.bias ? a.bias[c] : 0.f, sc = a.scale ? a.scale[c] : 1.f;
-  float dw = 0.f, db = 0.f, ds = 0.f;
-  for (int64_t i = p * share; i < r1; ++i) {
-    const float4 st = a.stats[i * a.groups + c / a.width];
-    const T* gr = gate ? gate + i * a.gate_st : nullptr;
-    const float n = (after_value(a, x + i * a.x_st, gr, c) - st.x) * st.y;
-    const float o = to_f(dy[i * a.dy_st + c]);
-    float f = 1.f;
-    if (!a.inside && gate) {
-      const float z = to_f(gr[c]);
-      f = z * sigmoid_f(z);
+// A unit's column sums to part[(unit * 3 + j) * width + column].
+template <int TPR, int VL, int NC>
+__device__ __forceinline__ void store_sums(const NormArgs& a, const Unit<TPR, VL, NC>& u,
+                                           const float (&s)[3][NC][VL], float* part) {
+#pragma unroll
+  for (int j = 0; j < 3; ++j)
+#pragma unroll
+    for (int k = 0; k < NC; ++k)
+      if (u.col(k) < a.width)
+#pragma unroll
+        for (int e = 0; e < VL; ++e) part[(u.index * 3 + j) * a.width + u.col(k) + e] = s[j][k][e];
+}
+
+template <class T, class R, int TPR, int VL, int NC>
+__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, 1)
+norm_before_bwd_kernel(NormArgs a, const T* x, const R* r, const T* dy, const R* dr, T* dx, R* dres,
+                       float* part) {
+  __shared__ float sh[2 * 3 * TPR / 32];
+  const Unit<TPR, VL, NC> u(a.groups);
+  int flip = 0;
+  float sums[3][NC][VL] = {};      // dweight, dbias, dscale
+  const float w1 = 1.f / (float)a.width;
+  for (int64_t row = u.first; row < a.rows; row += u.step) {
+    float v[NC][VL], g[NC][VL];
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      const int c = u.col(k);
+#pragma unroll
+      for (int e = 0; e < VL; ++e) v[k][e] = 0.f, g[k][e] = 0.f;
+      if (c >= a.width) continue;
+      load_vec<R, VL>(r + row * a.r_st + c, v[k]);
+      load_vec<T, VL>(dy + row * a.dy_st + c, g[k]);
     }
-    ds = fmaf(o, fmaf(n, w, bs) * f, ds);
-    dw = fmaf(o * sc * f, n, dw);
-    db = fmaf(o * sc, f, db);
+    float mean, inv;
+    row_stats(a, u, v, mean, inv, sh, flip);
+    float m[2] = {0.f, 0.f};       // means of dn and dn * n
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      const int c = u.col(k);
+      if (c >= a.width) continue;
+      float w[VL];
+      load_vec<float, VL>(a.weight + c, w);
+#pragma unroll
+      for (int e = 0; e < VL; ++e) {
+        const float n = (v[k][e] - mean) * inv;
+        v[k][e] = n;
+        sums[0][k][e] = fmaf(g[k][e], n, sums[0][k][e]);
+        sums[1][k][e] += g[k][e];
+        g[k][e] *= w[e];
+        m[0] += g[k][e], m[1] = fmaf(g[k][e], n, m[1]);
+      }
+    }
+    row_sum<TPR>(m, sh, flip);
+    const float g1 = a.layer ? m[0] * w1 : 0.f, g2 = m[1] * w1;
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      const int c = u.col(k);
+      if (c >= a.width) continue;
+      float o[VL];
+#pragma unroll
+      for (int e = 0; e < VL; ++e) o[e] = norm_grad(a, inv, g[k][e], v[k][e], g1, g2);
+      if (dr) {
+        float q[VL];
+        load_vec<R, VL>(dr + row * a.dr_st + c, q);
+#pragma unroll
+        for (int e = 0; e < VL; ++e) o[e] += q[e];
+      }
+      if (dres) store_vec<R, VL>(dres + row * a.dres_st + c, o);
+      if (x) {                     // dscale is wanted
+        float q[VL];
+        load_vec<T, VL>(x + row * a.x_st + c, q);
+#pragma unroll
+        for (int e = 0; e < VL; ++e) sums[2][k][e] = fmaf(o[e], q[e], sums[2][k][e]);
+      }
+      if (dx) {
+        float sc[VL];
+        load_param<VL>(a.scale, c, sc, 1.f);
+#pragma unroll
+        for (int e = 0; e < VL; ++e) o[e] *= sc[e];
+        store_vec<T, VL>(dx + row * a.dx_st + c, o);
+      }
+    }
   }
-  part[(p * 3 + 0) * a.channels + c] = dw;
-  part[(p * 3 + 1) * a.channels + c] = db;
-  part[(p * 3 + 2) * a.channels + c] = ds;
+  store_sums(a, u, sums, part);
+}
+
+template <class T, class R, int TPR, int VL, int NC>
+__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, 1)
+norm_after_kernel(NormArgs a, const T* x, const T* gate, const R* res, T* y) {
+  __shared__ float sh[2 * 3 * TPR / 32];
+  const Unit<TPR, VL, NC> u(a.groups);
+  int flip = 0;
+  const int64_t off = u.g * a.width;
+  for (int64_t row = u.first; row < a.rows; row += u.step) {
+    float v[NC][VL], f[NC][VL];    // the norm's input; silu(gate) where it comes after
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      const int64_t c = off + u.col(k);
+#pragma unroll
+      for (int e = 0; e < VL; ++e) v[k][e] = 0.f, f[k][e] = 1.f;
+      if (u.col(k) >= a.width) continue;
+      load_vec<T, VL>(x + row * a.x_st + c, v[k]);
+      if (gate) {
+        load_vec<T, VL>(gate + row * a.gate_st + c, f[k]);
+#pragma unroll
+        for (int e = 0; e < VL; ++e) {
+          f[k][e] *= sigmoid_f(f[k][e]);
+          if (a.inside) v[k][e] *= f[k][e], f[k][e] = 1.f;
+        }
+      }
+    }
+    float mean, inv;
+    row_stats(a, u, v, mean, inv, sh, flip);
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      const int64_t c = off + u.col(k);
+      if (u.col(k) >= a.width) continue;
+      float w[VL], bs[VL], sc[VL], base[VL];
+      load_vec<float, VL>(a.weight + c, w);
+      load_param<VL>(a.bias, c, bs, 0.f);
+      load_param<VL>(a.scale, c, sc, 1.f);
+#pragma unroll
+      for (int e = 0; e < VL; ++e) base[e] = 0.f;
+      if (res) load_vec<R, VL>(res + row * a.res_st + c, base);
+#pragma unroll
+      for (int e = 0; e < VL; ++e) {
+        const float p = fmaf((v[k][e] - mean) * inv, w[e], bs[e]) * f[k][e];
+        base[e] = fmaf(sc[e], p, base[e]);
+      }
+      store_vec<T, VL>(y + row * a.y_st + c, base);
+    }
+  }
+}
+
+template <class T, int TPR, int VL, int NC>
+__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, 1)
+norm_after_bwd_kernel(NormArgs a, const T* x, const T* gate, const T* dy, T* dx, T* dgate,
+                      float* part) {
+  __shared__ float sh[2 * 3 * TPR / 32];
+  const Unit<TPR, VL, NC> u(a.groups);
+  int flip = 0;
+  const int64_t off = u.g * a.width;
+  float sums[3][NC][VL] = {};      // dweight, dbias, dscale
+  const float w1 = 1.f / (float)a.width;
+  for (int64_t row = u.first; row < a.rows; row += u.step) {
+    float v[NC][VL], z[NC][VL], o[NC][VL];   // norm input (then n), gate, dy (then dn)
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      const int64_t c = off + u.col(k);
+#pragma unroll
+      for (int e = 0; e < VL; ++e) v[k][e] = 0.f, z[k][e] = 0.f, o[k][e] = 0.f;
+      if (u.col(k) >= a.width) continue;
+      load_vec<T, VL>(x + row * a.x_st + c, v[k]);
+      load_vec<T, VL>(dy + row * a.dy_st + c, o[k]);
+      if (gate) {
+        load_vec<T, VL>(gate + row * a.gate_st + c, z[k]);
+        if (a.inside)
+#pragma unroll
+          for (int e = 0; e < VL; ++e) v[k][e] *= z[k][e] * sigmoid_f(z[k][e]);
+      }
+    }
+    float mean, inv;
+    row_stats(a, u, v, mean, inv, sh, flip);
+    float m[2] = {0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      const int64_t c = off + u.col(k);
+      if (u.col(k) >= a.width) continue;
+      float w[VL], bs[VL], sc[VL], dg[VL];
+      load_vec<float, VL>(a.weight + c, w);
+      load_param<VL>(a.bias, c, bs, 0.f);
+      load_param<VL>(a.scale, c, sc, 1.f);
+#pragma unroll
+      for (int e = 0; e < VL; ++e) {
+        const float n = (v[k][e] - mean) * inv, p = fmaf(n, w[e], bs[e]);
+        float f = 1.f, df = 0.f;
+        if (gate && !a.inside) silu_grad(z[k][e], f, df);
+        sums[2][k][e] = fmaf(o[k][e], p * f, sums[2][k][e]);
+        const float g = o[k][e] * sc[e];
+        dg[e] = g * p * df;
+        sums[0][k][e] = fmaf(g * f, n, sums[0][k][e]);
+        sums[1][k][e] = fmaf(g, f, sums[1][k][e]);
+        v[k][e] = n;
+        o[k][e] = g * f * w[e];
+        m[0] += o[k][e], m[1] = fmaf(o[k][e], n, m[1]);
+      }
+      if (gate && !a.inside) store_vec<T, VL>(dgate + row * a.dgate_st + c, dg);
+    }
+    row_sum<TPR>(m, sh, flip);
+    const float g1 = a.layer ? m[0] * w1 : 0.f, g2 = m[1] * w1;
+#pragma unroll
+    for (int k = 0; k < NC; ++k) {
+      const int64_t c = off + u.col(k);
+      if (u.col(k) >= a.width) continue;
+#pragma unroll
+      for (int e = 0; e < VL; ++e) o[k][e] = norm_grad(a, inv, o[k][e], v[k][e], g1, g2);
+      if (gate && a.inside) {
+        float xv[VL], dg[VL];
+        load_vec<T, VL>(x + row * a.x_st + c, xv);   // again, from the cache
+#pragma unroll
+        for (int e = 0; e < VL; ++e) {
+          float f, df;
+          silu_grad(z[k][e], f, df);
+          dg[e] = o[k][e] * xv[e] * df;
+          o[k][e] *= f;
+        }
+        store_vec<T, VL>(dgate + row * a.dgate_st + c, dg);
+      }
+      store_vec<T, VL>(dx + row * a.dx_st + c, o[k]);
+    }
+  }
+  store_sums(a, u, sums, part);
+}
+
+// The units' column sums, added in order: unit j * groups + g holds group g's.
+__global__ void __launch_bounds__(256)
+norm_sums_kernel(const float* __restrict__ part, int64_t units, int64_t groups, int64_t width,
+                 float* dweight, float* dbias, float* dscale) {
+  __shared__ float sh[8][32];
+  const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+  const int64_t wb = (width + 31) / 32;
+  int64_t q = blockIdx.x;
+  const int64_t i = q % wb * 32 + x;
+  q /= wb;
+  const int64_t g = q % groups;
+  const int k = (int)(q / groups);
+  float* out = k == 0 ? dweight : (k == 1 ? dbias : dscale);
+  if (out == nullptr) return;
+  float s = 0.f;
+  if (i < width) {
+#pragma unroll 4
+    for (int64_t j = y; j < units / groups; j += 8)
+      s += part[((j * groups + g) * 3 + k) * width + i];
+  }
+  sh[y][x] = s;
+  __syncthreads();
+  if (y == 0 && i < width) {
+#pragma unroll
+    for (int j = 1; j < 8; ++j) s += sh[j][x];
+    out[g * width + i] = s;
+  }
 }
 
 NormArgs norm_args(const ferrum_norm_args* a) {
@@ -273,7 +419,6 @@ NormArgs norm_args(const ferrum_norm_args* a) {
   n.x_st = a->x_stride, n.gate_st = a->gate_stride, n.res_st = a->residual_stride;
   n.y_st = a->y_stride, n.r_st = a->r_stride, n.dy_st = a->dy_stride, n.dr_st = a->dr_stride;
   n.dx_st = a->dx_stride, n.dgate_st = a->dgate_stride, n.dres_st = a->dresidual_stride;
-  n.stats = nullptr;
   return n;
 }
 
@@ -290,6 +435,9 @@ ferrum_status check_norm(const ferrum_device* dev, const ferrum_norm_args* a, co
                                       ", " + std::to_string(a->channels) + ")");
   if (bounded_product({a->rows, a->channels, 4}) < 0)
     return invalid(what, "rows * channels is too large");
+  if ((int64_t)(a->channels / a->groups) > kMaxWidth)
+    return invalid(what, "a normalised row may have at most 32768 values, got " +
+                             std::to_string(a->channels / a->groups));
   const size_t e = dtype_size(a->dtype), re = dtype_size(a->residual_dtype);
   const bool empty = a->rows == 0 || a->channels == 0;
   if (ferrum_status s = check_ptr(a->weight, 4, empty, what, "weight")) return s;
@@ -328,25 +476,53 @@ ferrum_status with_residual(int dtype, int residual_dtype, F f) {
   });
 }
 
-// Copies the column sums to the gradients the caller asked for.
-ferrum_status store_sums(const float* sums, const ferrum_norm_args* a, cudaStream_t st,
-                         const char* what) {
-  float* dst[3] = {a->dweight, a->dbias, a->dscale};
-  for (int k = 0; k < 3; ++k)
-    if (dst[k]) {
-      cudaError_t e = cudaMemcpyAsync(dst[k], sums + k * a->channels, a->channels * 4,
-                                      cudaMemcpyDeviceToDevice, st);
-      if (e != cudaSuccess) return cuda_error(e, what);
-    }
-  return FERRUM_OK;
+// Threads per row, values per access and accesses per thread for a row of
+// `width` values: f(TPR, VL, NC) with TPR * VL * NC >= width. 16 values a
+// thread at most where they fit, so the gradient kernel's rows and column sums
+// stay in registers.
+template <int V>
+using Int = std::integral_constant<int, V>;
+template <class F>
+ferrum_status with_shape(int64_t width, bool vec, F f) {
+  if (vec) {
+    if (width <= 256) return f(Int<32>(), Int<8>(), Int<1>());
+    if (width <= 512) return f(Int<32>(), Int<8>(), Int<2>());
+    if (width <= 1024) return f(Int<128>(), Int<8>(), Int<1>());
+    if (width <= 2048) return f(Int<256>(), Int<8>(), Int<1>());
+    if (width <= 4096) return f(Int<256>(), Int<8>(), Int<2>());
+    if (width <= 8192) return f(Int<512>(), Int<8>(), Int<2>());
+    return f(Int<1024>(), Int<8>(), Int<4>());
+  }
+  if (width <= 512) return f(Int<32>(), Int<1>(), Int<16>());
+  if (width <= 4096) return f(Int<256>(), Int<1>(), Int<16>());
+  return f(Int<1024>(), Int<1>(), Int<32>());
 }
 
-// Rows per block of the column sums: enough blocks to fill the GPU, and a
-// workspace far below the arrays themselves.
-int64_t rows_share(int64_t rows, int64_t col_blocks) {
-  int64_t parts = ceil_div(148 * 4, col_blocks);
-  if (parts > rows) parts = rows;
-  return rows > 0 ? ceil_div(rows, parts) : 1;
+// Whether rows can go in 16-byte accesses.
+bool rows_vec(const void* p, int64_t stride, size_t e) {
+  return p == nullptr || (aligned(p, 16) && (stride * (int64_t)e) % 16 == 0);
+}
+bool norm_vec(const ferrum_norm_args* a, bool bwd) {
+  const size_t e = dtype_size(a->dtype), re = dtype_size(a->residual_dtype);
+  const int64_t width = (int64_t)(a->channels / a->groups);
+  bool v = width % 8 == 0 && rows_vec(a->weight, 0, 4) && rows_vec(a->bias, 0, 4) &&
+           rows_vec(a->scale, 0, 4) && rows_vec(a->x, a->x_stride, e) &&
+           rows_vec(a->gate, a->gate_stride, e) && rows_vec(a->r, a->r_stride, re);
+  if (!bwd) return v && rows_vec(a->residual, a->residual_stride, re) && rows_vec(a->y, a->y_stride, e);
+  return v && rows_vec(a->dy, a->dy_stride, e) && rows_vec(a->dr, a->dr_stride, re) &&
+         rows_vec(a->dx, a->dx_stride, e) && rows_vec(a->dgate, a->dgate_stride, e) &&
+         rows_vec(a->dresidual, a->dresidual_stride, re);
+}
+
+// Blocks of a launch: enough units for all rows, at most `per_sm` blocks' worth
+// of threads on every SM, and a number of units that holds every group.
+template <int TPR>
+int64_t unit_blocks(int64_t rows, int64_t groups, int threads_per_sm) {
+  constexpr int threads = TPR == 32 ? 256 : TPR, per = threads / TPR;
+  int64_t blocks = std::min(ceil_div(rows * groups, per),
+                            (int64_t)148 * std::max(1, threads_per_sm / threads));
+  const int64_t need = ceil_div(groups, per);
+  return std::max(blocks, need);
 }
 
 }  // namespace
@@ -356,23 +532,67 @@ int64_t rows_share(int64_t rows, int64_t col_blocks) {
 using namespace ferrum;
 using namespace ferrum::seq;
 
+namespace {
+
+template <class Go>
+ferrum_status norm_fwd(ferrum_device* dev, const ferrum_norm_args* a, bool before,
+                       const char* what, Go go) {
+  if (ferrum_status s = check_norm(dev, a, what, before, false)) return s;
+  if (a->rows == 0 || a->channels == 0) return FERRUM_OK;
+  DeviceGuard guard(dev->ordinal);
+  if (guard.status() != cudaSuccess) return cuda_error(guard.status(), "cudaSetDevice");
+  const NormArgs n = norm_args(a);
+  return with_residual(a->dtype, a->residual_dtype, [&](auto tx, auto tr) {
+    return with_shape(n.width, norm_vec(a, false), [&](auto tpr, auto vl, auto nc) {
+      constexpr int TPR = decltype(tpr)::value;
+      const int64_t blocks = unit_blocks<TPR>(n.rows, n.groups, 2048);
+      launch_detail::clear_stale_error();
+      go(n, tx, tr, tpr, vl, nc, (unsigned)blocks, TPR == 32 ? 256 : TPR);
+      return launched(what);
+    });
+  });
+}
+
+// The gradients' launch and the sums of its units.
+template <class Go>
+ferrum_status norm_bwd(ferrum_device* dev, const ferrum_norm_args* a, bool before,
+                       const char* what, cudaStream_t st, Go go) {
+  if (ferrum_status s = check_norm(dev, a, what, before, true)) return s;
+  if (a->channels == 0) return FERRUM_OK;
+  DeviceGuard guard(dev->ordinal);
+  if (guard.status() != cudaSuccess) return cuda_error(guard.status(), "cudaSetDevice");
+  const NormArgs n = norm_args(a);
+  return with_residual(a->dtype, a->residual_dtype, [&](auto tx, auto tr) {
+    return with_shape(n.width, norm_vec(a, true), [&](auto tpr, auto vl, auto nc) -> ferrum_status {
+      constexpr int TPR = decltype(tpr)::value;
+      constexpr int threads = TPR == 32 ? 256 : TPR;
+      const int64_t blocks = unit_blocks<TPR>(n.rows, n.groups, 512);
+      const int64_t units = blocks * (threads / TPR) / n.groups * n.groups;
+      PoolBuffer part(dev, sizeof(float) * (size_t)(blocks * (threads / TPR) * 3 * n.width), st);
+      if (part.status() != cudaSuccess) return cuda_error(part.status(), "workspace");
+      launch_detail::clear_stale_error();
+      go(n, tx, tr, tpr, vl, nc, (unsigned)blocks, threads, part.as<float>());
+      norm_sums_kernel<<<(unsigned)(ceil_div(n.width, 32) * n.groups * 3), 256, 0, st>>>(
+          part.as<float>(), units, n.groups, n.width, a->dweight, a->dbias, a->dscale);
+      return launched(what);
+    });
+  });
+}
+
+}  // namespace
+
 extern "C" {
 
 ferrum_status ferrum_norm_before(ferrum_device* dev, const ferrum_norm_args* a, void* stream) {
   const char* what = "norm_before";
   return guarded(what, [&]() -> ferrum_status {
-    if (ferrum_status s = check_norm(dev, a, what, true, false)) return s;
-    if (a->rows == 0 || a->channels == 0) return FERRUM_OK;
-    if (a->rows > 0x7fffffff) return invalid(what, "too many rows for one launch");
-    DeviceGuard guard(dev->ordinal);
-    if (guard.status() != cudaSuccess) return cuda_error(guard.status(), "cudaSetDevice");
-    return with_residual(a->dtype, a->residual_dtype, [&](auto tx, auto tr) {
+    return norm_fwd(dev, a, true, what, [&](const NormArgs& n, auto tx, auto tr, auto tpr, auto vl,
+                                            auto nc, unsigned blocks, int threads) {
       using T = decltype(tx);
       using R = decltype(tr);
-      launch_detail::clear_stale_error();
-      norm_before_kernel<T, R><<<(unsigned)a->rows, kThreads, 0, (cudaStream_t)stream>>>(
-          norm_args(a), (const T*)a->x, (const R*)a->residual, (T*)a->y, (R*)a->r);
-      return launched(what);
+      norm_before_kernel<T, R, decltype(tpr)::value, decltype(vl)::value, decltype(nc)::value>
+          <<<blocks, threads, 0, (cudaStream_t)stream>>>(n, (const T*)a->x, (const R*)a->residual,
+                                                         (T*)a->y, (R*)a->r);
     });
   });
 }
@@ -380,58 +600,29 @@ ferrum_status ferrum_norm_before(ferrum_device* dev, const ferrum_norm_args* a, 
 ferrum_status ferrum_norm_before_bwd(ferrum_device* dev, const ferrum_norm_args* a, void* stream) {
   const char* what = "norm_before_bwd";
   return guarded(what, [&]() -> ferrum_status {
-    if (ferrum_status s = check_norm(dev, a, what, true, true)) return s;
-    if (a->channels == 0) return FERRUM_OK;
-    if (a->rows > 0x7fffffff) return invalid(what, "too many rows for one launch");
-    cudaStream_t st = (cudaStream_t)stream;
-    DeviceGuard guard(dev->ordinal);
-    if (guard.status() != cudaSuccess) return cuda_error(guard.status(), "cudaSetDevice");
-    NormArgs n = norm_args(a);
-    const int64_t col_blocks = ceil_div(n.channels, kThreads);
-    const int64_t share = rows_share(n.rows, col_blocks), parts = ceil_div(n.rows, share);
-    PoolBuffer stats(dev, (size_t)(n.rows + 1) * sizeof(float4), st);
-    PoolBuffer part(dev, (size_t)(parts + 1) * 3 * n.channels * 4, st);
-    if (stats.status() != cudaSuccess) return cuda_error(stats.status(), "workspace");
-    if (part.status() != cudaSuccess) return cuda_error(part.status(), "workspace");
-    n.stats = stats.as<float4>();
-    float* sums = part.as<float>() + parts * 3 * n.channels;
-    if (n.rows > 0) {
-      ferrum_status s = with_residual(a->dtype, a->residual_dtype, [&](auto tx, auto tr) {
-        using T = decltype(tx);
-        using R = decltype(tr);
-        launch_detail::clear_stale_error();
-        norm_before_bwd_kernel<T, R><<<(unsigned)n.rows, kThreads, 0, st>>>(
-            n, (const R*)a->r, (const T*)a->dy, (const R*)a->dr, (T*)a->dx, (R*)a->dresidual);
-        norm_before_cols_kernel<T, R><<<(unsigned)(parts * col_blocks), kThreads, 0, st>>>(
-            n, a->dscale ? (const T*)a->x : nullptr, (const R*)a->r, (const T*)a->dy,
-            (const R*)a->dr,
-            part.as<float>(), col_blocks, share);
-        return launched(what);
-      });
-      if (s) return s;
-    }
-    cudaError_t e = launch_sum_rows(part.as<float>(), parts, 3 * n.channels, sums, st);
-    if (e != cudaSuccess) return cuda_error(e, what);
-    return store_sums(sums, a, st, what);
+    return norm_bwd(dev, a, true, what, (cudaStream_t)stream,
+                    [&](const NormArgs& n, auto tx, auto tr, auto tpr, auto vl, auto nc,
+                        unsigned blocks, int threads, float* part) {
+      using T = decltype(tx);
+      using R = decltype(tr);
+      norm_before_bwd_kernel<T, R, decltype(tpr)::value, decltype(vl)::value, decltype(nc)::value>
+          <<<blocks, threads, 0, (cudaStream_t)stream>>>(
+              n, a->dscale ? (const T*)a->x : nullptr, (const R*)a->r, (const T*)a->dy,
+              (const R*)a->dr, (T*)a->dx, (R*)a->dresidual, part);
+    });
   });
 }
 
 ferrum_status ferrum_norm_after(ferrum_device* dev, const ferrum_norm_args* a, void* stream) {
   const char* what = "norm_after";
   return guarded(what, [&]() -> ferrum_status {
-    if (ferrum_status s = check_norm(dev, a, what, false, false)) return s;
-    if (a->rows == 0 || a->channels == 0) return FERRUM_OK;
-    if (a->rows * a->groups > 0x7fffffff) return invalid(what, "too many rows for one launch");
-    DeviceGuard guard(dev->ordinal);
-    if (guard.status() != cudaSuccess) return cuda_error(guard.status(), "cudaSetDevice");
-    return with_residual(a->dtype, a->residual_dtype, [&](auto tx, auto tr) {
+    return norm_fwd(dev, a, false, what, [&](const NormArgs& n, auto tx, auto tr, auto tpr, auto vl,
+                                             auto nc, unsigned blocks, int threads) {
       using T = decltype(tx);
       using R = decltype(tr);
-      launch_detail::clear_stale_error();
-      norm_after_kernel<T, R>
-          <<<(unsigned)(a->rows * a->groups), kThreads, 0, (cudaStream_t)stream>>>(
-              norm_args(a), (const T*)a->x, (const T*)a->gate, (const R*)a->residual, (T*)a->y);
-      return launched(what);
+      norm_after_kernel<T, R, decltype(tpr)::value, decltype(vl)::value, decltype(nc)::value>
+          <<<blocks, threads, 0, (cudaStream_t)stream>>>(n, (const T*)a->x, (const T*)a->gate,
+                                                         (const R*)a->residual, (T*)a->y);
     });
   });
 }
@@ -439,37 +630,15 @@ ferrum_status ferrum_norm_after(ferrum_device* dev, const ferrum_norm_args* a, v
 ferrum_status ferrum_norm_after_bwd(ferrum_device* dev, const ferrum_norm_args* a, void* stream) {
   const char* what = "norm_after_bwd";
   return guarded(what, [&]() -> ferrum_status {
-    if (ferrum_status s = check_norm(dev, a, what, false, true)) return s;
-    if (a->channels == 0) return FERRUM_OK;
-    if (a->rows * a->groups > 0x7fffffff) return invalid(what, "too many rows for one launch");
-    cudaStream_t st = (cudaStream_t)stream;
-    DeviceGuard guard(dev->ordinal);
-    if (guard.status() != cudaSuccess) return cuda_error(guard.status(), "cudaSetDevice");
-    NormArgs n = norm_args(a);
-    const int64_t col_blocks = ceil_div(n.channels, kThreads);
-    const int64_t share = rows_share(n.rows, col_blocks), parts = ceil_div(n.rows, share);
-    PoolBuffer stats(dev, (size_t)(n.rows * n.groups + 1) * sizeof(float4), st);
-    PoolBuffer part(dev, (size_t)(parts + 1) * 3 * n.channels * 4, st);
-    if (stats.status() != cudaSuccess) return cuda_error(stats.status(), "workspace");
-    if (part.status() != cudaSuccess) return cuda_error(part.status(), "workspace");
-    n.stats = stats.as<float4>();
-    float* sums = part.as<float>() + parts * 3 * n.channels;
-    if (n.rows > 0) {
-      ferrum_status s = with_dtype(a->dtype, [&](auto tx) {
-        using T = decltype(tx);
-        launch_detail::clear_stale_error();
-        norm_after_bwd_kernel<T><<<(unsigned)(n.rows * n.groups), kThreads, 0, st>>>(
-            n, (const T*)a->x, (const T*)a->gate, (const T*)a->dy, (T*)a->dx, (T*)a->dgate);
-        norm_after_cols_kernel<T><<<(unsigned)(parts * col_blocks), kThreads, 0, st>>>(
-            n, (const T*)a->x, (const T*)a->gate, (const T*)a->dy, part.as<float>(), col_blocks,
-            share);
-        return launched(what);
-      });
-      if (s) return s;
-    }
-    cudaError_t e = launch_sum_rows(part.as<float>(), parts, 3 * n.channels, sums, st);
-    if (e != cudaSuccess) return cuda_error(e, what);
-    return store_sums(sums, a, st, what);
+    return norm_bwd(dev, a, false, what, (cudaStream_t)stream,
+                    [&](const NormArgs& n, auto tx, auto, auto tpr, auto vl, auto nc,
+                        unsigned blocks, int threads, float* part) {
+      using T = decltype(tx);
+      norm_after_bwd_kernel<T, decltype(tpr)::value, decltype(vl)::value, decltype(nc)::value>
+          <<<blocks, threads, 0, (cudaStream_t)stream>>>(n, (const T*)a->x, (const T*)a->gate,
+                                                         (const T*)a->dy, (T*)a->dx, (T*)a->dgate,
+                                                         part);
+    });
   });
 }
 

@@ -40,6 +40,48 @@ __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return
 // quotient is 0, the limit.
 __device__ __forceinline__ float sigmoid_f(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
 
+// VL consecutive values to and from float32: 16-byte accesses for VL = 8 (the
+// caller has checked the alignment), single values for VL = 1.
+template <class T, int VL>
+__device__ __forceinline__ void load_vec(const T* p, float (&v)[VL]) {
+  if constexpr (VL == 1) {
+    v[0] = to_f(*p);
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < VL; i += 4) {
+      const float4 u = *(const float4*)(p + i);
+      v[i] = u.x, v[i + 1] = u.y, v[i + 2] = u.z, v[i + 3] = u.w;
+    }
+  } else if constexpr (VL == 4) {
+    const uint2 u = *(const uint2*)p;
+    const T* w = (const T*)&u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = to_f(w[i]);
+  } else {
+    const uint4 u = *(const uint4*)p;
+    const T* w = (const T*)&u;
+#pragma unroll
+    for (int i = 0; i < VL; ++i) v[i] = to_f(w[i]);
+  }
+}
+template <class T, int VL>
+__device__ __forceinline__ void store_vec(T* p, const float (&v)[VL]) {
+  if constexpr (VL == 1) {
+    *p = from_f<T>(v[0]);
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < VL; i += 4) *(float4*)(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+  } else {
+    T w[VL];
+#pragma unroll
+    for (int i = 0; i < VL; ++i) w[i] = from_f<T>(v[i]);
+    if constexpr (VL == 4)
+      *(uint2*)p = *(const uint2*)w;
+    else
+      *(uint4*)p = *(const uint4*)w;
+  }
+}
+
 // Sum over the 32 lanes, in every lane, in a fixed order.
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
@@ -167,10 +209,10 @@ ferrum_status with_dtype(int dtype, F f) {
   return f(__nv_bfloat16());
 }
 
-// out[i] = sum over r < rows of part[r * n + i], in row order (a fixed order,
-// so results do not depend on scheduling).
-cudaError_t launch_sum_rows(const float* part, int64_t rows, int64_t n, float* out,
-                            cudaStream_t stream);
+// out[i] = sum over r < rows of part[r * row_stride + i], i < n, in a fixed
+// order (results do not depend on scheduling).
+cudaError_t launch_sum_rows(const float* part, int64_t rows, int64_t n, int64_t row_stride,
+                            float* out, cudaStream_t stream);
 
 }  // namespace seq
 }  // namespace ferrum

@@ -121,7 +121,7 @@ ferrum_status ferrum_selective_scan_step(ferrum_device *dev, const ferrum_scan_a
 
 /* ---------------------------------------------------------------------------
  * Norms around a block, over rows of `channels` values (row stride in
- * elements, values contiguous). N(v) = v / sqrt(mean(v^2) + eps) (RMS) or
+ * elements, values contiguous); a normalised row has at most 32768 values. N(v) = v / sqrt(mean(v^2) + eps) (RMS) or
  * (v - mean) / sqrt(var + eps) (LAYER).
  *
  * In front:  r = residual + scale * x (either part optional);
