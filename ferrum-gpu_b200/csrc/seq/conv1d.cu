@@ -1,8 +1,9 @@
 // Short causal depthwise convolution over (batch, length, channels):
 //   p[t] = bias + sum_j w[j] x[t-K+1+j],  y = p or p * sigmoid(p)
 // The work is 2K operations per 2 moved values: bound by HBM. A thread owns
-// VL adjacent channels (16-byte accesses forward, 8-byte in the gradient,
-// single values where the rows are not aligned) over a run of steps, and
+// VL adjacent channels (4 forward, 2 in the gradient, so that its windows fit
+// 80 registers and 24 warps an SM hide the loads; 1 where the rows are not
+// aligned) over a run of steps, and
 // slides a window of K values through registers, so x is read once, and K-1
 // rows again at the start of each run. It loads four rows ahead of using
 // them. Runs are long (64 steps) where the batch fills the GPU and shorter
@@ -68,7 +69,7 @@ struct ConvPlace {
 };
 
 template <class T, int K, int VL>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, VL == 1 ? 1 : 6)
 conv1d_fwd_kernel(Rows<T> x, Rows<T> y, const float* __restrict__ weight,
                   const float* __restrict__ bias, const T* st, T* fin,
                   const int32_t* __restrict__ lengths, ConvSizes s, bool silu) {
@@ -124,7 +125,7 @@ conv1d_fwd_kernel(Rows<T> x, Rows<T> y, const float* __restrict__ weight,
 }
 
 template <class T, int K, int VL>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, VL == 1 ? 1 : 6)
 conv1d_bwd_kernel(Rows<T> x, Rows<T> dy, Rows<T> dx, const float* __restrict__ weight,
                   const float* __restrict__ bias, const T* st, const T* dfin, T* dst,
                   const int32_t* __restrict__ lengths, float* __restrict__ part, ConvSizes s,
@@ -296,7 +297,7 @@ ferrum_status conv_fwd(ferrum_device* dev, const ferrum_conv1d_args* a, cudaStre
   if (guard.status() != cudaSuccess) return cuda_error(guard.status(), "cudaSetDevice");
   return with_dtype(a->dtype, [&](auto tag) {
     using T = decltype(tag);
-    return with_conv<8>(a->taps, conv_vec(a, false, 8), [&](auto k, auto vl) -> ferrum_status {
+    return with_conv<4>(a->taps, conv_vec(a, false, 4), [&](auto k, auto vl) -> ferrum_status {
       const ConvSizes s = conv_sizes(a, decltype(vl)::value);
       const int64_t blocks = s.batch * s.runs * s.col_blocks;
       if (ferrum_status st = grid_ok(blocks, what)) return st;
@@ -351,7 +352,7 @@ ferrum_status ferrum_causal_conv1d_bwd(ferrum_device* dev, const ferrum_conv1d_a
     if (guard.status() != cudaSuccess) return cuda_error(guard.status(), "cudaSetDevice");
     return with_dtype(a->dtype, [&](auto tag) {
       using T = decltype(tag);
-      return with_conv<4>(a->taps, conv_vec(a, true, 4), [&](auto k, auto vl) -> ferrum_status {
+      return with_conv<2>(a->taps, conv_vec(a, true, 2), [&](auto k, auto vl) -> ferrum_status {
         const ConvSizes z = conv_sizes(a, decltype(vl)::value);
         const int64_t parts = z.batch * z.runs, blocks = parts * z.col_blocks;
         if (ferrum_status s = grid_ok(blocks, what)) return s;

@@ -145,11 +145,10 @@ __device__ __forceinline__ void store_values(T* p, int64_t q, int64_t n, float2 
   const int64_t i = 2 * q;
   if (i >= n) return;
   if (vec && i + 1 < n) {
-    T w[2] = {from_f<T>(v.x), from_f<T>(v.y)};
     if constexpr (sizeof(T) == 4)
       *(float2*)(p + i) = make_float2(v.x, v.y);
     else
-      *(uint32_t*)(p + i) = *(uint32_t*)w;
+      *(uint32_t*)(p + i) = pack_pair<T>(v.x, v.y);
     return;
   }
   p[i] = from_f<T>(v.x);

@@ -28,7 +28,7 @@ constexpr int64_t kMaxWidth = 32768;
 struct NormArgs {
   int64_t rows, channels, groups, width;  // width = channels / groups
   float eps;
-  bool layer, inside;
+  bool layer;
   const float *weight, *bias, *scale;
   int64_t x_st, gate_st, res_st, y_st, r_st, dy_st, dr_st, dx_st, dgate_st, dres_st;
 };
@@ -61,7 +61,6 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float* sh, int& flip) {
 template <int TPR, int VL, int NC>
 struct Unit {
   static constexpr int THREADS = TPR == 32 ? 256 : TPR;
-  static constexpr int EPT = NC * VL;
   int64_t index, count, g, first, step;
   int lane;
   __device__ __forceinline__ Unit(int64_t groups) {
@@ -74,6 +73,16 @@ struct Unit {
   // column of chunk k in the group, and whether it lies in it
   __device__ __forceinline__ int col(int k) const { return (k * TPR + lane) * VL; }
 };
+
+// Warps an SM that the registers must allow for, so that enough loads are in
+// flight: 32 forward; 24 (of blocks up to 256 threads) or 32 in the gradient,
+// whose sums take more.
+constexpr int kFwdWarps = 32;
+template <int TPR, int EPT>
+constexpr int bwd_blocks() {
+  constexpr int threads = TPR == 32 ? 256 : TPR;
+  return EPT > 8 ? 1 : (threads <= 256 ? 768 / threads : 1024 / threads);
+}
 
 // Gradient of a value from that of its normalised value n.
 __device__ __forceinline__ float norm_grad(const NormArgs& a, float inv, float dn, float n,
@@ -128,7 +137,7 @@ __device__ __forceinline__ void load_param(const float* p, int64_t c, float (&v)
 }
 
 template <class T, class R, int TPR, int VL, int NC>
-__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, 1)
+__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, NC * VL <= 8 ? kFwdWarps * 32 / (TPR == 32 ? 256 : TPR) : 1)
 norm_before_kernel(NormArgs a, const T* x, const R* res, T* y, R* r) {
   __shared__ float sh[2 * 3 * TPR / 32];
   const Unit<TPR, VL, NC> u(a.groups);
@@ -181,7 +190,7 @@ __device__ __forceinline__ void store_sums(const NormArgs& a, const Unit<TPR, VL
 }
 
 template <class T, class R, int TPR, int VL, int NC>
-__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, 1)
+__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, bwd_blocks<TPR, VL * NC>())
 norm_before_bwd_kernel(NormArgs a, const T* x, const R* r, const T* dy, const R* dr, T* dx, R* dres,
                        float* part) {
   __shared__ float sh[2 * 3 * TPR / 32];
@@ -253,8 +262,11 @@ norm_before_bwd_kernel(NormArgs a, const T* x, const R* r, const T* dy, const R*
   store_sums(a, u, sums, part);
 }
 
-template <class T, class R, int TPR, int VL, int NC>
-__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, 1)
+// Where the gate enters.
+enum { kNoGate = 0, kInside = 1, kOutside = 2 };
+
+template <class T, class R, int GATE, int TPR, int VL, int NC>
+__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, NC * VL <= 8 ? kFwdWarps * 32 / (TPR == 32 ? 256 : TPR) : 1)
 norm_after_kernel(NormArgs a, const T* x, const T* gate, const R* res, T* y) {
   __shared__ float sh[2 * 3 * TPR / 32];
   const Unit<TPR, VL, NC> u(a.groups);
@@ -269,12 +281,12 @@ norm_after_kernel(NormArgs a, const T* x, const T* gate, const R* res, T* y) {
       for (int e = 0; e < VL; ++e) v[k][e] = 0.f, f[k][e] = 1.f;
       if (u.col(k) >= a.width) continue;
       load_vec<T, VL>(x + row * a.x_st + c, v[k]);
-      if (gate) {
+      if constexpr (GATE != kNoGate) {
         load_vec<T, VL>(gate + row * a.gate_st + c, f[k]);
 #pragma unroll
         for (int e = 0; e < VL; ++e) {
           f[k][e] *= sigmoid_f(f[k][e]);
-          if (a.inside) v[k][e] *= f[k][e], f[k][e] = 1.f;
+          if constexpr (GATE == kInside) v[k][e] *= f[k][e], f[k][e] = 1.f;
         }
       }
     }
@@ -301,8 +313,8 @@ norm_after_kernel(NormArgs a, const T* x, const T* gate, const R* res, T* y) {
   }
 }
 
-template <class T, int TPR, int VL, int NC>
-__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, 1)
+template <class T, int GATE, int TPR, int VL, int NC>
+__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, bwd_blocks<TPR, VL * NC>())
 norm_after_bwd_kernel(NormArgs a, const T* x, const T* gate, const T* dy, T* dx, T* dgate,
                       float* part) {
   __shared__ float sh[2 * 3 * TPR / 32];
@@ -321,9 +333,9 @@ norm_after_bwd_kernel(NormArgs a, const T* x, const T* gate, const T* dy, T* dx,
       if (u.col(k) >= a.width) continue;
       load_vec<T, VL>(x + row * a.x_st + c, v[k]);
       load_vec<T, VL>(dy + row * a.dy_st + c, o[k]);
-      if (gate) {
+      if constexpr (GATE != kNoGate) {
         load_vec<T, VL>(gate + row * a.gate_st + c, z[k]);
-        if (a.inside)
+        if constexpr (GATE == kInside)
 #pragma unroll
           for (int e = 0; e < VL; ++e) v[k][e] *= z[k][e] * sigmoid_f(z[k][e]);
       }
@@ -343,7 +355,7 @@ norm_after_bwd_kernel(NormArgs a, const T* x, const T* gate, const T* dy, T* dx,
       for (int e = 0; e < VL; ++e) {
         const float n = (v[k][e] - mean) * inv, p = fmaf(n, w[e], bs[e]);
         float f = 1.f, df = 0.f;
-        if (gate && !a.inside) silu_grad(z[k][e], f, df);
+        if constexpr (GATE == kOutside) silu_grad(z[k][e], f, df);
         sums[2][k][e] = fmaf(o[k][e], p * f, sums[2][k][e]);
         const float g = o[k][e] * sc[e];
         dg[e] = g * p * df;
@@ -353,7 +365,7 @@ norm_after_bwd_kernel(NormArgs a, const T* x, const T* gate, const T* dy, T* dx,
         o[k][e] = g * f * w[e];
         m[0] += o[k][e], m[1] = fmaf(o[k][e], n, m[1]);
       }
-      if (gate && !a.inside) store_vec<T, VL>(dgate + row * a.dgate_st + c, dg);
+      if constexpr (GATE == kOutside) store_vec<T, VL>(dgate + row * a.dgate_st + c, dg);
     }
     row_sum<TPR>(m, sh, flip);
     const float g1 = a.layer ? m[0] * w1 : 0.f, g2 = m[1] * w1;
@@ -363,7 +375,7 @@ norm_after_bwd_kernel(NormArgs a, const T* x, const T* gate, const T* dy, T* dx,
       if (u.col(k) >= a.width) continue;
 #pragma unroll
       for (int e = 0; e < VL; ++e) o[k][e] = norm_grad(a, inv, o[k][e], v[k][e], g1, g2);
-      if (gate && a.inside) {
+      if constexpr (GATE == kInside) {
         float xv[VL], dg[VL];
         load_vec<T, VL>(x + row * a.x_st + c, xv);   // again, from the cache
 #pragma unroll
@@ -414,7 +426,7 @@ NormArgs norm_args(const ferrum_norm_args* a) {
   NormArgs n;
   n.rows = (int64_t)a->rows, n.channels = (int64_t)a->channels, n.groups = (int64_t)a->groups;
   n.width = n.channels / n.groups;
-  n.eps = a->eps, n.layer = a->kind == FERRUM_NORM_LAYER, n.inside = a->gate_inside != 0;
+  n.eps = a->eps, n.layer = a->kind == FERRUM_NORM_LAYER;
   n.weight = a->weight, n.bias = a->bias, n.scale = a->scale;
   n.x_st = a->x_stride, n.gate_st = a->gate_stride, n.res_st = a->residual_stride;
   n.y_st = a->y_stride, n.r_st = a->r_stride, n.dy_st = a->dy_stride, n.dr_st = a->dr_stride;
@@ -477,25 +489,31 @@ ferrum_status with_residual(int dtype, int residual_dtype, F f) {
 }
 
 // Threads per row, values per access and accesses per thread for a row of
-// `width` values: f(TPR, VL, NC) with TPR * VL * NC >= width. 16 values a
-// thread at most where they fit, so the gradient kernel's rows and column sums
-// stay in registers.
+// `width` values: f(TPR, VL, NC) with TPR * VL * NC >= width. 8 values a
+// thread up to width 8192: few registers, many warps.
 template <int V>
 using Int = std::integral_constant<int, V>;
 template <class F>
 ferrum_status with_shape(int64_t width, bool vec, F f) {
   if (vec) {
     if (width <= 256) return f(Int<32>(), Int<8>(), Int<1>());
-    if (width <= 512) return f(Int<32>(), Int<8>(), Int<2>());
+    if (width <= 512) return f(Int<64>(), Int<8>(), Int<1>());
     if (width <= 1024) return f(Int<128>(), Int<8>(), Int<1>());
     if (width <= 2048) return f(Int<256>(), Int<8>(), Int<1>());
-    if (width <= 4096) return f(Int<256>(), Int<8>(), Int<2>());
-    if (width <= 8192) return f(Int<512>(), Int<8>(), Int<2>());
+    if (width <= 4096) return f(Int<512>(), Int<8>(), Int<1>());
+    if (width <= 8192) return f(Int<1024>(), Int<8>(), Int<1>());
     return f(Int<1024>(), Int<8>(), Int<4>());
   }
-  if (width <= 512) return f(Int<32>(), Int<1>(), Int<16>());
-  if (width <= 4096) return f(Int<256>(), Int<1>(), Int<16>());
+  if (width <= 256) return f(Int<32>(), Int<1>(), Int<8>());
+  if (width <= 2048) return f(Int<256>(), Int<1>(), Int<8>());
+  if (width <= 8192) return f(Int<1024>(), Int<1>(), Int<8>());
   return f(Int<1024>(), Int<1>(), Int<32>());
+}
+template <class F>
+void with_gate(const ferrum_norm_args* a, F f) {
+  if (a->gate == nullptr) return f(Int<kNoGate>());
+  if (a->gate_inside) return f(Int<kInside>());
+  return f(Int<kOutside>());
 }
 
 // Whether rows can go in 16-byte accesses.
@@ -545,7 +563,7 @@ ferrum_status norm_fwd(ferrum_device* dev, const ferrum_norm_args* a, bool befor
   return with_residual(a->dtype, a->residual_dtype, [&](auto tx, auto tr) {
     return with_shape(n.width, norm_vec(a, false), [&](auto tpr, auto vl, auto nc) {
       constexpr int TPR = decltype(tpr)::value;
-      const int64_t blocks = unit_blocks<TPR>(n.rows, n.groups, 2048);
+      const int64_t blocks = unit_blocks<TPR>(n.rows, n.groups, kFwdWarps * 32);
       launch_detail::clear_stale_error();
       go(n, tx, tr, tpr, vl, nc, (unsigned)blocks, TPR == 32 ? 256 : TPR);
       return launched(what);
@@ -566,7 +584,7 @@ ferrum_status norm_bwd(ferrum_device* dev, const ferrum_norm_args* a, bool befor
     return with_shape(n.width, norm_vec(a, true), [&](auto tpr, auto vl, auto nc) -> ferrum_status {
       constexpr int TPR = decltype(tpr)::value;
       constexpr int threads = TPR == 32 ? 256 : TPR;
-      const int64_t blocks = unit_blocks<TPR>(n.rows, n.groups, 512);
+      const int64_t blocks = unit_blocks<TPR>(n.rows, n.groups, TPR <= 256 ? 768 : 1024);
       const int64_t units = blocks * (threads / TPR) / n.groups * n.groups;
       PoolBuffer part(dev, sizeof(float) * (size_t)(blocks * (threads / TPR) * 3 * n.width), st);
       if (part.status() != cudaSuccess) return cuda_error(part.status(), "workspace");
@@ -620,9 +638,11 @@ ferrum_status ferrum_norm_after(ferrum_device* dev, const ferrum_norm_args* a, v
                                              auto nc, unsigned blocks, int threads) {
       using T = decltype(tx);
       using R = decltype(tr);
-      norm_after_kernel<T, R, decltype(tpr)::value, decltype(vl)::value, decltype(nc)::value>
-          <<<blocks, threads, 0, (cudaStream_t)stream>>>(n, (const T*)a->x, (const T*)a->gate,
-                                                         (const R*)a->residual, (T*)a->y);
+      with_gate(a, [&](auto gate) {
+        norm_after_kernel<T, R, decltype(gate)::value, decltype(tpr)::value, decltype(vl)::value,
+                          decltype(nc)::value><<<blocks, threads, 0, (cudaStream_t)stream>>>(
+            n, (const T*)a->x, (const T*)a->gate, (const R*)a->residual, (T*)a->y);
+      });
     });
   });
 }
@@ -634,10 +654,11 @@ ferrum_status ferrum_norm_after_bwd(ferrum_device* dev, const ferrum_norm_args* 
                     [&](const NormArgs& n, auto tx, auto, auto tpr, auto vl, auto nc,
                         unsigned blocks, int threads, float* part) {
       using T = decltype(tx);
-      norm_after_bwd_kernel<T, decltype(tpr)::value, decltype(vl)::value, decltype(nc)::value>
-          <<<blocks, threads, 0, (cudaStream_t)stream>>>(n, (const T*)a->x, (const T*)a->gate,
-                                                         (const T*)a->dy, (T*)a->dx, (T*)a->dgate,
-                                                         part);
+      with_gate(a, [&](auto gate) {
+        norm_after_bwd_kernel<T, decltype(gate)::value, decltype(tpr)::value, decltype(vl)::value,
+                              decltype(nc)::value><<<blocks, threads, 0, (cudaStream_t)stream>>>(
+            n, (const T*)a->x, (const T*)a->gate, (const T*)a->dy, (T*)a->dx, (T*)a->dgate, part);
+      });
     });
   });
 }

@@ -9,7 +9,6 @@ namespace ferrum {
 namespace seq {
 
 constexpr int kSaveSteps = FERRUM_SCAN_SAVE_STEPS;
-constexpr float kLog2e = 1.4426950408889634f;
 
 struct ScanSizes {
   int64_t batch, length, channels, groups, per_group, saves;
@@ -30,13 +29,6 @@ __device__ __forceinline__ int64_t scan_length(const int32_t* lengths, int64_t b
   if (lengths == nullptr) return length;
   const int64_t n = lengths[b];
   return n < 0 ? 0 : (n > length ? length : n);
-}
-
-// 2^x by the special-function unit (2 units in the last place).
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
 }
 
 // log(1 + e^x) = max(x, 0) + log(1 + e), e = e^-|x| in (0, 1]. log(1 + e) / e

@@ -76,8 +76,7 @@ template <class T>
 __device__ __forceinline__ void store_pair(T* p, float2 v, int n, bool vec) {
   if constexpr (sizeof(T) == 2) {
     if (vec && n == 2) {
-      T w[2] = {from_f<T>(v.x), from_f<T>(v.y)};
-      *(uint32_t*)p = *(uint32_t*)w;
+      *(uint32_t*)p = pack_pair<T>(v.x, v.y);
       return;
     }
   }

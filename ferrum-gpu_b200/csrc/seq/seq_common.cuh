@@ -11,6 +11,7 @@
 #include <exception>
 #include <new>
 #include <string>
+#include <type_traits>
 
 #include "../../../include/ferrum_seq.h"
 #include "../launch_common.cuh"
@@ -36,16 +37,50 @@ __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// 1 / (1 + e^-x). For x below about -88 e^-x overflows to infinity and the
-// quotient is 0, the limit.
-__device__ __forceinline__ float sigmoid_f(float x) { return __fdividef(1.f, 1.f + __expf(-x)); }
+constexpr float kLog2e = 1.4426950408889634f;
 
-// VL consecutive values to and from float32: 16-byte accesses for VL = 8 (the
-// caller has checked the alignment), single values for VL = 1.
+// 2^x by the special-function unit (2 units in the last place).
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// 1 / x by the special-function unit (1 unit in the last place).
+__device__ __forceinline__ float rcp(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// 1 / (1 + e^-x). For x below about -88 e^-x overflows to infinity, whose
+// reciprocal is 0, the limit.
+__device__ __forceinline__ float sigmoid_f(float x) { return rcp(1.f + ex2(-x * kLog2e)); }
+
+// Two 16-bit values rounded and packed by one instruction.
+template <class T>
+__device__ __forceinline__ uint32_t pack_pair(float x, float y) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(x, y);
+    return *(const uint32_t*)&h;
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    return *(const uint32_t*)&h;
+  }
+}
+
+// VL consecutive values to and from float32 in accesses of up to 16 bytes (the
+// caller has checked the alignment); single values for VL = 1.
 template <class T, int VL>
 __device__ __forceinline__ void load_vec(const T* p, float (&v)[VL]) {
   if constexpr (VL == 1) {
     v[0] = to_f(*p);
+  } else if constexpr (sizeof(T) == 4 && VL == 2) {
+    const float2 u = *(const float2*)p;
+    v[0] = u.x, v[1] = u.y;
+  } else if constexpr (VL == 2) {
+    const uint32_t u = *(const uint32_t*)p;
+    const T* w = (const T*)&u;
+    v[0] = to_f(w[0]), v[1] = to_f(w[1]);
   } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
     for (int i = 0; i < VL; i += 4) {
@@ -68,13 +103,17 @@ template <class T, int VL>
 __device__ __forceinline__ void store_vec(T* p, const float (&v)[VL]) {
   if constexpr (VL == 1) {
     *p = from_f<T>(v[0]);
+  } else if constexpr (sizeof(T) == 4 && VL == 2) {
+    *(float2*)p = make_float2(v[0], v[1]);
+  } else if constexpr (VL == 2) {
+    *(uint32_t*)p = pack_pair<T>(v[0], v[1]);
   } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
     for (int i = 0; i < VL; i += 4) *(float4*)(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
   } else {
-    T w[VL];
+    uint32_t w[VL / 2];
 #pragma unroll
-    for (int i = 0; i < VL; ++i) w[i] = from_f<T>(v[i]);
+    for (int i = 0; i < VL / 2; ++i) w[i] = pack_pair<T>(v[2 * i], v[2 * i + 1]);
     if constexpr (VL == 4)
       *(uint2*)p = *(const uint2*)w;
     else
