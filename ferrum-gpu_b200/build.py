@@ -3,6 +3,7 @@
 Outputs (next to the Python package so they travel with the source tree):
   ferrum_gpu/libferrum_fft.so                    C ABI (include/ferrum_fft.h, ferrum_seq.h) + sm_100a kernels
   ferrum_gpu/_native.<python-ext-suffix>         pybind11 module over the C ABI
+  ferrum_gpu/_sequence.<python-ext-suffix>       the sequence operators on torch tensors
 
 Every .cu is compiled with
   nvcc -gencode arch=compute_100a,code=sm_100a -lineinfo -O3
@@ -47,6 +48,7 @@ SEQ_SOURCES = ["seq_common.cu", "conv1d.cu", "scan_fwd.cu", "scan_bwd.cu", "norm
                "long_conv.cu"]
 LIB = os.path.join(PKG, "libferrum_fft.so")
 EXT = os.path.join(PKG, "_native" + sysconfig.get_config_var("EXT_SUFFIX"))
+SEQ_EXT = os.path.join(PKG, "_sequence" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 
 def _headers(seq: bool = False) -> list[str]:
@@ -95,6 +97,18 @@ def build(jobs: int = 4, force: bool = False) -> None:
         _run([CXX, "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
               f"-I{pybind11.get_include()}", f"-I{py_inc}", f"-I{INCLUDE}", native_src,
               "-o", EXT, f"-L{PKG}", "-lferrum_fft", "-Wl,-rpath,$ORIGIN"])
+    seq_src = os.path.join(CSRC, "seq", "torch_binding.cpp")
+    if force or _stale(SEQ_EXT, [seq_src, LIB] + _headers(seq=True)):
+        import torch
+
+        torch_dir = os.path.dirname(torch.__file__)
+        py_inc = sysconfig.get_paths()["include"]
+        _run([CXX, "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+              f"-I{torch_dir}/include", f"-I{torch_dir}/include/torch/csrc/api/include",
+              f"-I{CUDA_HOME}/include", f"-I{py_inc}", f"-I{INCLUDE}", seq_src, "-o", SEQ_EXT,
+              f"-L{torch_dir}/lib", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python",
+              f"-L{PKG}", "-lferrum_fft", "-Wl,-rpath,$ORIGIN"])
 
 
 def main() -> None:
@@ -105,6 +119,7 @@ def main() -> None:
     build(a.jobs, a.force)
     print(LIB)
     print(EXT)
+    print(SEQ_EXT)
 
 
 if __name__ == "__main__":

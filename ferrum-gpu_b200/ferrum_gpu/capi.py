@@ -1,4 +1,4 @@
-"""ctypes binding of the C ABI in include/ferrum_fft.h.
+"""ctypes binding of the C ABI in include/ferrum_fft.h and ferrum_seq.h.
 
 This is the binding a caller of the reference would add to reach the B200
 kernels through plain pointers: device-resident buffers (for example
@@ -80,6 +80,70 @@ SIGNATURES = {
 }
 
 
+class Rows(ctypes.Structure):
+    _fields_ = [("ptr", _vp), ("batch_stride", ctypes.c_int64), ("row_stride", ctypes.c_int64)]
+
+
+def _fields(spec: str):
+    """Struct fields from "type name name; type name" text."""
+    kinds = {"size": _sz, "int": _i, "i64": ctypes.c_int64, "ptr": _vp, "rows": Rows, "float": ctypes.c_float}
+    out = []
+    for part in spec.split(";"):
+        words = part.split()
+        out += [(name, kinds[words[0]]) for name in words[1:]]
+    return out
+
+
+# Mirrors of the argument blocks of include/ferrum_seq.h, field by field.
+class ConvArgs(ctypes.Structure):
+    _fields_ = _fields("size struct_size; int dtype taps silu; size batch length channels;"
+                       "ptr weight bias initial_state lengths; rows x y; ptr final_state;"
+                       "rows dy dx; ptr dfinal_state dweight dbias dinitial_state")
+
+
+class ScanArgs(ctypes.Structure):
+    _fields_ = _fields("size struct_size; int dtype delta_softplus;"
+                       "size batch length channels states groups; rows u delta z out B C;"
+                       "i64 B_group_stride C_group_stride;"
+                       "ptr A D delta_bias initial_state final_state lengths saved_states;"
+                       "rows dout du ddelta dz; ptr dfinal_state dB dC dA dD ddelta_bias"
+                       " dinitial_state")
+
+
+class NormArgs(ctypes.Structure):
+    _fields_ = _fields("size struct_size; int dtype residual_dtype kind gate_inside;"
+                       "size rows channels groups; float eps; ptr weight bias scale x gate"
+                       " residual y r; i64 x_stride gate_stride residual_stride y_stride r_stride;"
+                       "ptr dy dr dx dgate dresidual;"
+                       "i64 dy_stride dr_stride dx_stride dgate_stride dresidual_stride;"
+                       "ptr dweight dbias dscale")
+
+
+class LongArgs(ctypes.Structure):
+    _fields_ = _fields("size struct_size; int dtype; size batch channels length kernel_length;"
+                       "ptr kernel skip; rows x y; i64 x_step y_step; rows dy dx;"
+                       "i64 dy_step dx_step; ptr dkernel dskip; rows history; ptr positions")
+
+
+# Sequence operators: entry point -> argument block; each is called with the
+# device handle, a pointer to its block and the stream.
+SEQ_SIGNATURES = {
+    "ferrum_causal_conv1d": ConvArgs,
+    "ferrum_causal_conv1d_bwd": ConvArgs,
+    "ferrum_causal_conv1d_step": ConvArgs,
+    "ferrum_selective_scan": ScanArgs,
+    "ferrum_selective_scan_bwd": ScanArgs,
+    "ferrum_selective_scan_step": ScanArgs,
+    "ferrum_norm_before": NormArgs,
+    "ferrum_norm_before_bwd": NormArgs,
+    "ferrum_norm_after": NormArgs,
+    "ferrum_norm_after_bwd": NormArgs,
+    "ferrum_long_conv": LongArgs,
+    "ferrum_long_conv_bwd": LongArgs,
+    "ferrum_long_conv_step": LongArgs,
+}
+
+
 class FerrumError(RuntimeError):
     def __init__(self, status: int, message: str):
         super().__init__(f"ferrum status {status}: {message}")
@@ -102,6 +166,10 @@ def lib() -> ctypes.CDLL:
             fn = getattr(handle, name)
             fn.restype = res
             fn.argtypes = args
+        for name, block in SEQ_SIGNATURES.items():
+            fn = getattr(handle, name)
+            fn.restype = _i
+            fn.argtypes = [_vp, ctypes.POINTER(block), _vp]
         _lib = handle
     return _lib
 

@@ -767,15 +767,15 @@ def test_refusals():
         sq.long_conv_step(x[:, 0], rnd(7, 2, 8, 5), torch.zeros(2, device="cuda"), rnd(6, 8, 5))
     # the C entries refuse what a C caller can get wrong
     h = capi.DeviceHandle(0)
-    args = sq.ConvArgs(struct_size=1)
-    assert sq._entry("ferrum_causal_conv1d")(h.ptr, args, None) == capi.FERRUM_ERR_INVALID_ARG
+    args = capi.ConvArgs(struct_size=1)
+    assert capi.lib().ferrum_causal_conv1d(h.ptr, args, None) == capi.FERRUM_ERR_INVALID_ARG
     assert "struct_size" in capi.last_error()
-    assert sq._entry("ferrum_causal_conv1d")(h.ptr, None, None) == capi.FERRUM_ERR_INVALID_ARG
+    assert capi.lib().ferrum_causal_conv1d(h.ptr, None, None) == capi.FERRUM_ERR_INVALID_ARG
     import ctypes
-    args = sq.ConvArgs(struct_size=ctypes.sizeof(sq.ConvArgs), taps=4, batch=1 << 40,
+    args = capi.ConvArgs(struct_size=ctypes.sizeof(capi.ConvArgs), taps=4, batch=1 << 40,
                        length=1 << 20, channels=1 << 20)
-    assert sq._entry("ferrum_causal_conv1d")(h.ptr, args, None) == capi.FERRUM_ERR_INVALID_ARG
-    args = sq.ConvArgs(struct_size=ctypes.sizeof(sq.ConvArgs), taps=4, batch=1, length=1, channels=1)
-    assert sq._entry("ferrum_causal_conv1d")(h.ptr, args, None) == capi.FERRUM_ERR_INVALID_ARG
+    assert capi.lib().ferrum_causal_conv1d(h.ptr, args, None) == capi.FERRUM_ERR_INVALID_ARG
+    args = capi.ConvArgs(struct_size=ctypes.sizeof(capi.ConvArgs), taps=4, batch=1, length=1, channels=1)
+    assert capi.lib().ferrum_causal_conv1d(h.ptr, args, None) == capi.FERRUM_ERR_INVALID_ARG
     assert "weight is NULL" in capi.last_error()
     h.close()

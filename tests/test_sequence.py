@@ -20,15 +20,15 @@ HEADER = os.path.join(REPO, "include", "ferrum_seq.h")
 
 def test_header_and_binding_agree():
     text = re.sub(r"/\*.*?\*/", "", open(HEADER).read(), flags=re.S)
-    assert sorted(set(re.findall(r"\b(ferrum_[a-z0-9_]+)\s*\(", text))) == sorted(sq.SIGNATURES)
-    for name in sq.SIGNATURES:
+    assert sorted(set(re.findall(r"\b(ferrum_[a-z0-9_]+)\s*\(", text))) == sorted(capi.SEQ_SIGNATURES)
+    for name in capi.SEQ_SIGNATURES:
         assert hasattr(capi.lib(), name)
 
 
 def test_argument_blocks_match_the_header(tmp_path):
     """Size and every field offset, as the C compiler lays them out."""
-    blocks = {"ferrum_conv1d_args": sq.ConvArgs, "ferrum_scan_args": sq.ScanArgs,
-              "ferrum_norm_args": sq.NormArgs, "ferrum_long_conv_args": sq.LongArgs}
+    blocks = {"ferrum_conv1d_args": capi.ConvArgs, "ferrum_scan_args": capi.ScanArgs,
+              "ferrum_norm_args": capi.NormArgs, "ferrum_long_conv_args": capi.LongArgs}
     lines = []
     for c, py in blocks.items():
         lines.append(f'printf("%zu\\n", sizeof({c}));')
@@ -47,10 +47,10 @@ def test_argument_blocks_match_the_header(tmp_path):
     assert got == want
 
 
-@pytest.mark.parametrize("name", sorted(sq.SIGNATURES))
+@pytest.mark.parametrize("name", sorted(capi.SEQ_SIGNATURES))
 def test_null_device_and_block_are_refused(name):
-    args = sq.SIGNATURES[name]()
-    assert sq._entry(name)(None, ctypes.byref(args), None) == capi.FERRUM_ERR_INVALID_ARG
+    args = capi.SEQ_SIGNATURES[name]()
+    assert getattr(capi.lib(), name)(None, ctypes.byref(args), None) == capi.FERRUM_ERR_INVALID_ARG
     assert "device handle" in capi.last_error()
 
 
@@ -66,5 +66,9 @@ def test_cpu_tensors_are_refused():
         sq.norm_after(x, torch.zeros(4))
     with pytest.raises(ValueError, match="must be a CUDA tensor"):
         sq.long_conv(x, torch.zeros(3, 4))
-    with pytest.raises(ValueError, match="must be a CUDA tensor"):
+    with pytest.raises(ValueError, match="x is required"):
         sq.long_conv(None, torch.zeros(3, 4))
+    with pytest.raises(ValueError, match="CUDA tensor"):
+        sq.long_conv(x.numpy(), torch.zeros(3, 4))
+    with pytest.raises(ValueError, match="CUDA tensor"):
+        sq.long_conv("x", torch.zeros(3, 4))
