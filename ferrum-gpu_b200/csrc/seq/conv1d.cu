@@ -211,6 +211,40 @@ conv1d_bwd_kernel(Rows<T> x, Rows<T> dy, Rows<T> dx, const float* __restrict__ w
   }
 }
 
+// One step of every sequence: K - 1 rows of state and one of x in, the state
+// moved up by one row and y out. Each thread owns VL channels of a sequence
+// and reads before it writes, so the state may be updated in place.
+template <class T, int K, int VL>
+__global__ void __launch_bounds__(kThreads)
+conv1d_step_kernel(Rows<T> x, Rows<T> y, const float* __restrict__ weight,
+                   const float* __restrict__ bias, const T* st, T* fin, int64_t batch,
+                   int64_t channels, bool silu) {
+  const int64_t per = channels / VL, i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (i >= batch * per) return;
+  const int64_t b = i / per, d = i % per * VL;
+  float win[K][VL], w[VL * K], p[VL];
+#pragma unroll
+  for (int j = 0; j + 1 < K; ++j) load_vec<T, VL>(st + (b * (K - 1) + j) * channels + d, win[j]);
+  load_vec<T, VL>(x.at(b, 0) + d, win[K - 1]);
+  if constexpr (VL % 4 == 0) {       // a channel's taps are adjacent, and 16-byte aligned
+    load_vec<float, VL * K>(weight + d * K, w);
+  } else {
+#pragma unroll
+    for (int j = 0; j < VL * K; ++j) w[j] = weight[d * K + j];
+  }
+#pragma unroll
+  for (int e = 0; e < VL; ++e) {
+    float v = bias ? bias[d + e] : 0.f;
+#pragma unroll
+    for (int j = 0; j < K; ++j) v = fmaf(w[e * K + j], win[j][e], v);
+    if (silu) v *= sigmoid_f(v);
+    p[e] = v;
+  }
+  store_vec<T, VL>(y.at(b, 0) + d, p);
+#pragma unroll
+  for (int j = 0; j + 1 < K; ++j) store_vec<T, VL>(fin + (b * (K - 1) + j) * channels + d, win[j + 1]);
+}
+
 template <class F>
 ferrum_status with_taps(int taps, F f) {
   switch (taps) {
@@ -337,7 +371,26 @@ ferrum_status ferrum_causal_conv1d_step(ferrum_device* dev, const ferrum_conv1d_
     if (a->taps > 1 && a->batch > 0 && a->channels > 0 &&
         (a->initial_state == nullptr || a->final_state == nullptr))
       return invalid(what, "initial_state and final_state are required");
-    return conv_fwd(dev, a, (cudaStream_t)stream, what);
+    if (a->lengths != nullptr) return invalid(what, "lengths does not apply to one step");
+    if (a->batch == 0 || a->channels == 0) return FERRUM_OK;
+    DeviceGuard guard(dev->ordinal);
+    if (guard.status() != cudaSuccess) return cuda_error(guard.status(), "cudaSetDevice");
+    return with_dtype(a->dtype, [&](auto tag) {
+      using T = decltype(tag);
+      const bool vec = conv_vec(a, false, 4) && aligned(a->weight, 16);
+      return with_conv<4>(a->taps, vec, [&](auto k, auto vl) -> ferrum_status {
+        constexpr int VL = decltype(vl)::value;
+        const int64_t blocks = ceil_div((int64_t)a->batch * (int64_t)(a->channels / VL), kThreads);
+        if (ferrum_status s = grid_ok(blocks, what)) return s;
+        launch_detail::clear_stale_error();
+        conv1d_step_kernel<T, decltype(k)::value, VL>
+            <<<(unsigned)blocks, kThreads, 0, (cudaStream_t)stream>>>(
+                rows_of<T>(a->x), rows_of<T>(a->y), a->weight, a->bias,
+                (const T*)a->initial_state, (T*)a->final_state, (int64_t)a->batch,
+                (int64_t)a->channels, a->silu != 0);
+        return launched(what);
+      });
+    });
   });
 }
 

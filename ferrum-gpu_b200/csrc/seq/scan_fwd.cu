@@ -253,58 +253,80 @@ scan_fwd_kernel(ScanIn<T> in, Rows<T> out, float* fin, float* __restrict__ saved
 
 // One step: every value of the state is read and written once, which is all
 // the traffic that counts. L lanes share a channel, 4 states each (16-byte
-// accesses), and add up the output by shuffles.
-template <class T, int L>
+// accesses), and add up the output by shuffles. A thread takes its channel in
+// BT sequences, with all their loads issued first: more bytes in flight, and A
+// and the parameters are read once for them.
+template <class T, int L, int BT>
 __global__ void __launch_bounds__(128)
-scan_step_kernel(ScanIn<T> in, Rows<T> out, float* fin, ScanSizes s, bool vec) {
-  const int64_t i = ((int64_t)blockIdx.x * 128 + threadIdx.x) / L;
-  const int n0 = (threadIdx.x % L) * 4;
-  const bool live = i < s.batch * s.channels;
-  const int64_t b = live ? i / s.channels : 0, d = live ? i % s.channels : 0, g = d / s.per_group;
-  const int64_t so = (b * s.channels + d) * s.states + n0;
-  const float *pa = in.A + d * s.states + n0, *ph = in.initial + so;
-  const T *pb = in.B.at(b, 0) + g * in.B_group + n0, *pc = in.C.at(b, 0) + g * in.C_group + n0;
-  float h[4], a[4], Bv[4], Cv[4];
-  if (vec) {
-    const float4 x = *(const float4*)ph, w = *(const float4*)pa;
-    h[0] = x.x, h[1] = x.y, h[2] = x.z, h[3] = x.w;
-    a[0] = w.x, a[1] = w.y, a[2] = w.z, a[3] = w.w;
-  }
+scan_step_kernel(ScanIn<T> in, Rows<T> out, float* fin, ScanSizes s, bool vec, bool bc_vec,
+                 int64_t col_blocks) {
+  const int64_t d0 = blockIdx.x % col_blocks * (128 / L) + threadIdx.x / L;
+  const int64_t b0 = blockIdx.x / col_blocks * BT;
+  const int n0 = threadIdx.x % L * 4;
+  const bool live = d0 < s.channels;
+  const int64_t d = live ? d0 : 0, g = d / s.per_group;
+  float h[BT][4], a[4], Bv[BT][4], Cv[BT][4], x[BT], dt[BT], z[BT];
+  const float* pa = in.A + d * s.states + n0;
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const bool ok = n0 + k < s.states;
-    if (!vec) h[k] = ok ? ph[k] : 0.f, a[k] = ok ? pa[k] : 0.f;
-    Bv[k] = ok ? to_f(pb[k]) : 0.f;
-    Cv[k] = ok ? to_f(pc[k]) : 0.f;
-  }
-  const float x = to_f(in.u.at(b, 0)[d]);
-  float dt = to_f(in.delta.at(b, 0)[d]) + (in.bias ? in.bias[d] : 0.f);
-  const float z = in.z ? to_f(in.z.at(b, 0)[d]) : 0.f;
-  const float skip = in.D ? in.D[d] : 0.f;
-  const bool run = in.lengths == nullptr || in.lengths[b] > 0;
-  if (s.softplus) dt = softplus_f(dt);
-  float y = 0.f;
-  if (run) {
+  for (int k = 0; k < BT; ++k) {
+    const int64_t b = b0 + k < s.batch ? b0 + k : s.batch - 1;
+    const float* ph = in.initial + (b * s.channels + d) * s.states + n0;
+    if (vec) {
+      load_vec<float, 4>(ph, h[k]);
+    } else {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      h[k] = fmaf(ex2(dt * (a[k] * kLog2e)), h[k], dt * x * Bv[k]);
-      y = fmaf(h[k], Cv[k], y);
+      for (int e = 0; e < 4; ++e) h[k][e] = n0 + e < s.states ? ph[e] : 0.f;
     }
-  }
+    const T *pb = in.B.at(b, 0) + g * in.B_group + n0, *pc = in.C.at(b, 0) + g * in.C_group + n0;
+    if (bc_vec) {
+      load_vec<T, 4>(pb, Bv[k]);
+      load_vec<T, 4>(pc, Cv[k]);
+    } else {
 #pragma unroll
-  for (int o = L / 2; o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o, L);
-  if (!live) return;
+      for (int e = 0; e < 4; ++e) {
+        Bv[k][e] = n0 + e < s.states ? to_f(pb[e]) : 0.f;
+        Cv[k][e] = n0 + e < s.states ? to_f(pc[e]) : 0.f;
+      }
+    }
+    x[k] = to_f(in.u.at(b, 0)[d]);
+    dt[k] = to_f(in.delta.at(b, 0)[d]);
+    z[k] = in.z ? to_f(in.z.at(b, 0)[d]) : 0.f;
+  }
   if (vec) {
-    *(float4*)(fin + so) = make_float4(h[0], h[1], h[2], h[3]);
+    load_vec<float, 4>(pa, a);
   } else {
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (n0 + k < s.states) fin[so + k] = h[k];
+    for (int e = 0; e < 4; ++e) a[e] = n0 + e < s.states ? pa[e] : 0.f;
   }
-  if (n0 == 0) {
-    y = fmaf(skip, x, y);
-    if (in.z) y *= z * sigmoid_f(z);
-    out.at(b, 0)[d] = from_f<T>(run ? y : 0.f);
+  const float bias = in.bias ? in.bias[d] : 0.f, skip = in.D ? in.D[d] : 0.f;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) a[e] *= kLog2e;
+#pragma unroll
+  for (int k = 0; k < BT; ++k) {
+    const int64_t b = b0 + k;
+    float v = dt[k] + bias, y = 0.f;
+    if (s.softplus) v = softplus_f(v);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      h[k][e] = fmaf(ex2(v * a[e]), h[k][e], v * x[k] * Bv[k][e]);
+      y = fmaf(h[k][e], Cv[k][e], y);
+    }
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) y += __shfl_xor_sync(0xffffffffu, y, o, L);
+    if (!live || b >= s.batch) continue;
+    float* pf = fin + (b * s.channels + d) * s.states + n0;
+    if (vec) {
+      store_vec<float, 4>(pf, h[k]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (n0 + e < s.states) pf[e] = h[k][e];
+    }
+    if (n0 == 0) {
+      y = fmaf(skip, x[k], y);
+      if (in.z) y *= z[k] * sigmoid_f(z[k]);
+      out.at(b, 0)[d] = from_f<T>(y);
+    }
   }
 }
 
@@ -369,26 +391,41 @@ ferrum_status scan_step(ferrum_device* dev, const ferrum_scan_args* a, cudaStrea
   if (a->batch == 0 || a->channels == 0) return FERRUM_OK;
   const ScanSizes s = scan_sizes(a);
   const int lanes = 1 << (log_states(s.states) - 2);
-  const int64_t blocks = ceil_div(s.batch * s.channels * lanes, 128);
-  if (blocks > 0x7fffffff) return invalid(what, "too many blocks for one launch");
-  const bool vec = s.states % 4 == 0 && s.states == 4 * lanes && aligned(a->A, 16) &&
-                   aligned(a->initial_state, 16) && aligned(a->final_state, 16);
+  const bool vec = s.states == 4 * lanes && aligned(a->A, 16) && aligned(a->initial_state, 16) &&
+                   aligned(a->final_state, 16);
   DeviceGuard guard(dev->ordinal);
   if (guard.status() != cudaSuccess) return cuda_error(guard.status(), "cudaSetDevice");
   return with_dtype(a->dtype, [&](auto tag) {
     using T = decltype(tag);
-    auto go = [&](auto l) {
+    auto quad = [&](const ferrum_rows& r, int64_t group) {   // 4 values of a row at once
+      const int64_t e = sizeof(T);
+      return aligned(r.ptr, 4 * e) && r.batch_stride % 4 == 0 && group % 4 == 0;
+    };
+    const bool bc_vec = s.states == 4 * lanes && quad(a->B, a->B_group_stride) &&
+                        quad(a->C, a->C_group_stride);
+    auto go = [&](auto l, auto bt) -> ferrum_status {
+      constexpr int L = decltype(l)::value, BT = decltype(bt)::value;
+      const int64_t col_blocks = ceil_div(s.channels, 128 / L);
+      const int64_t blocks = col_blocks * ceil_div(s.batch, BT);
+      if (blocks > 0x7fffffff) return invalid(what, "too many blocks for one launch");
       launch_detail::clear_stale_error();
-      scan_step_kernel<T, decltype(l)::value><<<(unsigned)blocks, 128, 0, stream>>>(
-          scan_in<T>(a), rows_of<T>(a->out), a->final_state, s, vec);
+      scan_step_kernel<T, L, BT><<<(unsigned)blocks, 128, 0, stream>>>(
+          scan_in<T>(a), rows_of<T>(a->out), a->final_state, s, vec, bc_vec, col_blocks);
       return launched(what);
     };
+    auto lane = [&](auto l) -> ferrum_status {
+      // sequences a thread: 4 where that still leaves two full waves of blocks
+      constexpr int L = decltype(l)::value;
+      if (ceil_div(s.channels, 128 / L) * (s.batch / 4) >= 148 * 16)
+        return go(l, std::integral_constant<int, 4>());
+      return go(l, std::integral_constant<int, 1>());
+    };
     switch (lanes) {
-      case 1: return go(std::integral_constant<int, 1>());
-      case 2: return go(std::integral_constant<int, 2>());
-      case 4: return go(std::integral_constant<int, 4>());
-      case 8: return go(std::integral_constant<int, 8>());
-      default: return go(std::integral_constant<int, 16>());
+      case 1: return lane(std::integral_constant<int, 1>());
+      case 2: return lane(std::integral_constant<int, 2>());
+      case 4: return lane(std::integral_constant<int, 4>());
+      case 8: return lane(std::integral_constant<int, 8>());
+      default: return lane(std::integral_constant<int, 16>());
     }
   });
 }
@@ -465,6 +502,7 @@ ferrum_status ferrum_selective_scan_step(ferrum_device* dev, const ferrum_scan_a
     if (a->batch > 0 && a->channels > 0 &&
         (a->initial_state == nullptr || a->final_state == nullptr))
       return invalid(what, "initial_state and final_state are required");
+    if (a->lengths != nullptr) return invalid(what, "lengths does not apply to one step");
     return scan_step(dev, a, (cudaStream_t)stream, what);
   });
 }
