@@ -316,6 +316,20 @@ def test_scan_step_continues_a_prompt(dtype, N, G, d):
     check(st, fr, 12 * 20 + 16 * N, "state")
 
 
+@pytest.mark.parametrize("b,d,N,G", [(83, 4104, 16, 2), (41, 8200, 8, 1), (163, 4096, 5, 1)])
+def test_scan_step_of_a_large_batch(b, d, N, G):
+    """Batches whose threads take several sequences, the last one short."""
+    a, k, h0, _, _ = scan_inputs((b, 1, d, N, G, True, False), torch.bfloat16)
+    yr, fr = scan_ref({i: dbl(v) for i, v in a.items()},
+                      {i: dbl(v) if isinstance(v, torch.Tensor) else v for i, v in k.items()},
+                      dbl(h0), None)
+    cut = lambda t: t[:, 0] if isinstance(t, torch.Tensor) and t.dim() > 2 else t
+    o = sq.selective_scan_step(**{i: cut(v) for i, v in a.items()}, state=h0,
+                               **{i: cut(v) for i, v in k.items()})
+    check(o, yr[:, 0], 12 + 16 * N, "out")
+    check(h0, fr, 12 + 16 * N, "state")
+
+
 def test_scan_strides():
     """u and z as halves of one projection, B and C as columns of another; the
     same values give the same bits whatever the strides and alignment."""
