@@ -86,17 +86,24 @@ conv1d_fwd_kernel(Rows<T> x, Rows<T> y, const float* __restrict__ weight,
   for (int e = 0; e < VL; ++e) bs[e] = bias ? bias[d + e] : 0.f;
 #pragma unroll
   for (int j = 1; j < K; ++j) conv_in<T, K, VL>(x, st, b, t0 - K + j, d, len, s.channels, win[j]);
-  const int64_t t1 = t0 + s.run < s.length ? t0 + s.run : s.length;
-  for (int64_t t = t0; t < t1; t += kAhead) {
+  // The run's steps and those of them inside the sequence, from t0 on.
+  const int n = (int)(s.length - t0 < s.run ? s.length - t0 : s.run);
+  const int valid = len - t0 < n ? (len - t0 < 0 ? 0 : (int)(len - t0)) : n;
+  const T* px = x.at(b, t0) + d;
+  T* py = y.at(b, t0) + d;
+  // kAhead steps from t on; EDGE where some lie past the run or the sequence
+  auto block = [&](auto edge, int t) {
+    constexpr bool EDGE = decltype(edge)::value;
     float in[kAhead][VL];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      clear(in[i]);
-      if (t + i < len) load_vec<T, VL>(x.at(b, t + i) + d, in[i]);
+      if (EDGE) clear(in[i]);
+      if (!EDGE || t + i < valid) load_vec<T, VL>(px + i * x.st, in[i]);
     }
+    px += kAhead * x.st;
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      if (t + i >= t1) break;
+      if (EDGE && t + i >= n) return;
       float p[VL];
 #pragma unroll
       for (int e = 0; e < VL; ++e) {
@@ -107,11 +114,15 @@ conv1d_fwd_kernel(Rows<T> x, Rows<T> y, const float* __restrict__ weight,
 #pragma unroll
         for (int j = 0; j < K; ++j) v = fmaf(w[j][e], win[j][e], v);
         if (silu) v *= sigmoid_f(v);
-        p[e] = t + i < len ? v : 0.f;
+        p[e] = !EDGE || t + i < valid ? v : 0.f;
       }
-      store_vec<T, VL>(y.at(b, t + i) + d, p);
+      store_vec<T, VL>(py, p);
+      py += y.st;
     }
-  }
+  };
+  int t = 0;
+  for (; t + kAhead <= valid; t += kAhead) block(std::false_type(), t);
+  for (; t < n; t += kAhead) block(std::true_type(), t);
   if (t0 == 0 && fin != nullptr) {
     // all reads come first: fin may be the initial state's array
     float keep[K][VL];
@@ -143,23 +154,31 @@ conv1d_bwd_kernel(Rows<T> x, Rows<T> dy, Rows<T> dx, const float* __restrict__ w
   }
 #pragma unroll
   for (int j = 1; j < K; ++j) conv_in<T, K, VL>(x, st, b, t0 - K + j, d, len, s.channels, win[j]);
-  const int64_t t1 = t0 + s.run < s.length ? t0 + s.run : s.length;
+  // The run's steps and those of them inside the sequence, from t0 on; the
+  // gradients of the last K-1 need as many steps of the next run.
+  const int n = (int)(s.length - t0 < s.run ? s.length - t0 : s.run);
+  const int64_t left = len - t0 < 0 ? 0 : len - t0;
+  const int valid = (int)(left < n + K - 1 ? left : n + K - 1);
+  const T *px = x.at(b, t0) + d, *pg = dy.at(b, t0) + d;
+  T* po = dx.at(b, t0) + d - (K - 1) * dx.st;    // row t-K+1
   // g[j] holds the gradient of p at step t-K+1+j; after it moved on to step t,
-  // dx of step t-K+1 is complete.
-  for (int64_t t = t0; t < t1 + K - 1; t += kAhead) {
+  // dx of step t-K+1 is complete. EDGE where steps lie past the run or the
+  // sequence, or dx in front of the run, or a final state's gradient joins.
+  auto block = [&](auto edge, int t) {
+    constexpr bool EDGE = decltype(edge)::value;
     float in[kAhead][VL], gin[kAhead][VL];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      clear(in[i]), clear(gin[i]);
-      if (t + i < len && t + i < t1 + K - 1) {
-        load_vec<T, VL>(x.at(b, t + i) + d, in[i]);
-        load_vec<T, VL>(dy.at(b, t + i) + d, gin[i]);
+      if (EDGE) clear(in[i]), clear(gin[i]);
+      if (!EDGE || t + i < valid) {
+        load_vec<T, VL>(px + i * x.st, in[i]);
+        load_vec<T, VL>(pg + i * dy.st, gin[i]);
       }
     }
+    px += kAhead * x.st, pg += kAhead * dy.st;
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      if (t + i >= t1 + K - 1) break;
-      const int64_t r = t + i - K + 1;
+      if (EDGE && t + i >= n + K - 1) return;
       float o[VL];
 #pragma unroll
       for (int e = 0; e < VL; ++e) {
@@ -172,11 +191,11 @@ conv1d_bwd_kernel(Rows<T> x, Rows<T> dy, Rows<T> dx, const float* __restrict__ w
 #pragma unroll
           for (int j = 0; j < K; ++j) p = fmaf(w[j][e], win[j][e], p);
           const float sg = sigmoid_f(p);
-          gt *= sg * (1.f + p * (1.f - sg));
+          gt *= sg * fmaf(p, 1.f - sg, 1.f);
         }
-        if (t + i >= len) gt = 0.f;     // whatever the padding's p
+        if (EDGE && t + i >= valid) gt = 0.f;     // whatever the padding's p
         g[K - 1][e] = gt;
-        if (t + i < t1) {
+        if (!EDGE || t + i < n) {
           db[e] += gt;
 #pragma unroll
           for (int j = 0; j < K; ++j) dw[j][e] = fmaf(gt, win[j][e], dw[j][e]);
@@ -185,23 +204,38 @@ conv1d_bwd_kernel(Rows<T> x, Rows<T> dy, Rows<T> dx, const float* __restrict__ w
 #pragma unroll
         for (int j = 0; j < K; ++j) o[e] = fmaf(w[j][e], g[K - 1 - j][e], o[e]);
       }
-      if (r < t0 && !(t0 == 0 && dst != nullptr)) continue;
-      // a final state is the input's last K-1 values
-      const int64_t f = r - (len - (K - 1));
-      if (dfin != nullptr && f >= 0 && f < K - 1) {
-        float q[VL];
-        load_vec<T, VL>(dfin + (b * (K - 1) + f) * s.channels + d, q);
+      if constexpr (EDGE) {
+        const int64_t r = t0 + t + i - K + 1;
+        if (r >= t0 || (t0 == 0 && dst != nullptr)) {
+          // a final state is the input's last K-1 values
+          const int64_t f = r - (len - (K - 1));
+          if (dfin != nullptr && f >= 0 && f < K - 1) {
+            float q[VL];
+            load_vec<T, VL>(dfin + (b * (K - 1) + f) * s.channels + d, q);
 #pragma unroll
-        for (int e = 0; e < VL; ++e) o[e] += q[e];
+            for (int e = 0; e < VL; ++e) o[e] += q[e];
+          }
+          if (r >= 0) {
+            if (r >= len) clear(o);
+            store_vec<T, VL>(po, o);
+          } else {
+            store_vec<T, VL>(dst + (b * (K - 1) + (r + K - 1)) * s.channels + d, o);
+          }
+        }
+      } else {
+        store_vec<T, VL>(po, o);
       }
-      if (r >= 0) {
-        if (r >= len) clear(o);
-        store_vec<T, VL>(dx.at(b, r) + d, o);
-      } else if (r >= -(K - 1)) {
-        store_vec<T, VL>(dst + (b * (K - 1) + (r + K - 1)) * s.channels + d, o);
-      }
+      po += dx.st;
     }
-  }
+  };
+  // steps whose blocks are whole: inside the run and, where a final state has
+  // a gradient, in front of its rows
+  const int64_t whole64 = dfin != nullptr ? left - (K - 1) : left;
+  const int whole = (int)(whole64 < n ? whole64 : n);
+  int t = 0;
+  for (; t < n + K - 1 && t < K - 1; t += kAhead) block(std::true_type(), t);
+  for (; t + kAhead <= whole; t += kAhead) block(std::false_type(), t);
+  for (; t < n + K - 1; t += kAhead) block(std::true_type(), t);
   float* o = part + (b * s.runs + at.run) * (K + 1) * s.channels;
 #pragma unroll
   for (int e = 0; e < VL; ++e) {
