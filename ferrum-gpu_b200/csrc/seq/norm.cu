@@ -50,9 +50,14 @@ __device__ __forceinline__ void row_sum(float (&v)[N], float* sh, int& flip) {
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      float s = buf[i * W];
-      for (int k = 1; k < W; ++k) s += buf[i * W + k];
-      v[i] = s;
+      if constexpr (W <= 4) {
+        float s = buf[i * W];
+#pragma unroll
+        for (int k = 1; k < W; ++k) s += buf[i * W + k];
+        v[i] = s;
+      } else {
+        v[i] = warp_sum((threadIdx.x & 31) < W ? buf[i * W + (threadIdx.x & 31)] : 0.f);
+      }
     }
   }
 }
@@ -64,7 +69,9 @@ struct Unit {
   int64_t index, count, g, first, step;
   int lane;
   __device__ __forceinline__ Unit(int64_t groups) {
-    index = ((int64_t)blockIdx.x * THREADS + threadIdx.x) / TPR;
+    // for a whole block the row is uniform, and so are its addresses
+    index = TPR == THREADS ? blockIdx.x
+                           : ((int64_t)blockIdx.x * THREADS + threadIdx.x) / TPR;
     count = (int64_t)gridDim.x * (THREADS / TPR);
     g = index % groups, first = index / groups, step = count / groups;
     if (index >= step * groups) first = INT64_MAX;   // units beyond a multiple of the groups
@@ -84,6 +91,13 @@ constexpr int bwd_blocks() {
   return EPT > 8 ? 1 : (threads <= 256 ? 768 / threads : 1024 / threads);
 }
 
+// The next row's line to the L2 cache while this row is worked on: 8 % for
+// norm_before at 8191 x 4096; the other kernels, bound by instructions, lose.
+template <class T>
+__device__ __forceinline__ void prefetch(const T* p) {
+  asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
+}
+
 // Gradient of a value from that of its normalised value n.
 __device__ __forceinline__ float norm_grad(const NormArgs& a, float inv, float dn, float n,
                                            float mean_dn, float mean_dnn) {
@@ -98,23 +112,28 @@ __device__ __forceinline__ void silu_grad(float g, float& f, float& df) {
   df = sg * (1.f + g * (1.f - sg));
 }
 
-// mean and 1 / deviation of a row held as v (zeros beyond its end)
+// The mean of a row held as v (zeros beyond its end): 0 for RMS.
+template <int TPR, int VL, int NC>
+__device__ __forceinline__ float row_mean(const NormArgs& a, const float (&v)[NC][VL], float* sh,
+                                          int& flip) {
+  if (!a.layer) return 0.f;
+  float q[1] = {0.f};
+#pragma unroll
+  for (int k = 0; k < NC; ++k)
+#pragma unroll
+    for (int e = 0; e < VL; ++e) q[0] += v[k][e];
+  row_sum<TPR>(q, sh, flip);
+  return q[0] / (float)a.width;
+}
+
+// mean and 1 / deviation of a row held as v
 template <int TPR, int VL, int NC>
 __device__ __forceinline__ void row_stats(const NormArgs& a, const Unit<TPR, VL, NC>& u,
                                           const float (&v)[NC][VL], float& mean, float& inv,
                                           float* sh, int& flip) {
   const float w = 1.f / (float)a.width;
+  mean = row_mean<TPR>(a, v, sh, flip);
   float q[1];
-  mean = 0.f;
-  if (a.layer) {
-    q[0] = 0.f;
-#pragma unroll
-    for (int k = 0; k < NC; ++k)
-#pragma unroll
-      for (int e = 0; e < VL; ++e) q[0] += v[k][e];
-    row_sum<TPR>(q, sh, flip);
-    mean = q[0] * w;
-  }
   q[0] = 0.f;
 #pragma unroll
   for (int k = 0; k < NC; ++k)
@@ -143,6 +162,13 @@ norm_before_kernel(NormArgs a, const T* x, const R* res, T* y, R* r) {
   const Unit<TPR, VL, NC> u(a.groups);
   int flip = 0;
   for (int64_t row = u.first; row < a.rows; row += u.step) {
+    if (row + u.step < a.rows)
+#pragma unroll
+      for (int k = 0; k < NC; ++k)
+        if (u.col(k) < a.width) {
+          if (x) prefetch(x + (row + u.step) * a.x_st + u.col(k));
+          if (res) prefetch(res + (row + u.step) * a.res_st + u.col(k));
+        }
     float v[NC][VL];
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
@@ -199,7 +225,7 @@ norm_before_bwd_kernel(NormArgs a, const T* x, const R* r, const T* dy, const R*
   float sums[3][NC][VL] = {};      // dweight, dbias, dscale
   const float w1 = 1.f / (float)a.width;
   for (int64_t row = u.first; row < a.rows; row += u.step) {
-    float v[NC][VL], g[NC][VL];
+    float v[NC][VL], g[NC][VL], dn[NC][VL];   // r (then centred), dy, gradient of n
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
       const int c = u.col(k);
@@ -209,9 +235,8 @@ norm_before_bwd_kernel(NormArgs a, const T* x, const R* r, const T* dy, const R*
       load_vec<R, VL>(r + row * a.r_st + c, v[k]);
       load_vec<T, VL>(dy + row * a.dy_st + c, g[k]);
     }
-    float mean, inv;
-    row_stats(a, u, v, mean, inv, sh, flip);
-    float m[2] = {0.f, 0.f};       // means of dn and dn * n
+    const float mean = row_mean<TPR>(a, v, sh, flip);
+    float m[3] = {0.f, 0.f, 0.f};             // sums of v^2, dn and dn * v
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
       const int c = u.col(k);
@@ -220,23 +245,28 @@ norm_before_bwd_kernel(NormArgs a, const T* x, const R* r, const T* dy, const R*
       load_vec<float, VL>(a.weight + c, w);
 #pragma unroll
       for (int e = 0; e < VL; ++e) {
-        const float n = (v[k][e] - mean) * inv;
-        v[k][e] = n;
-        sums[0][k][e] = fmaf(g[k][e], n, sums[0][k][e]);
-        sums[1][k][e] += g[k][e];
-        g[k][e] *= w[e];
-        m[0] += g[k][e], m[1] = fmaf(g[k][e], n, m[1]);
+        v[k][e] -= mean;
+        dn[k][e] = g[k][e] * w[e];
+        m[0] = fmaf(v[k][e], v[k][e], m[0]);
+        m[1] += dn[k][e];
+        m[2] = fmaf(dn[k][e], v[k][e], m[2]);
       }
     }
     row_sum<TPR>(m, sh, flip);
-    const float g1 = a.layer ? m[0] * w1 : 0.f, g2 = m[1] * w1;
+    const float inv = 1.f / sqrtf(fmaf(m[0], w1, a.eps));
+    const float g1 = a.layer ? m[1] * w1 : 0.f, g2 = m[2] * inv * w1;
 #pragma unroll
     for (int k = 0; k < NC; ++k) {
       const int c = u.col(k);
       if (c >= a.width) continue;
       float o[VL];
 #pragma unroll
-      for (int e = 0; e < VL; ++e) o[e] = norm_grad(a, inv, g[k][e], v[k][e], g1, g2);
+      for (int e = 0; e < VL; ++e) {
+        const float n = v[k][e] * inv;
+        sums[0][k][e] = fmaf(g[k][e], n, sums[0][k][e]);
+        sums[1][k][e] += g[k][e];
+        o[e] = norm_grad(a, inv, dn[k][e], n, g1, g2);
+      }
       if (dr) {
         float q[VL];
         load_vec<R, VL>(dr + row * a.dr_st + c, q);
