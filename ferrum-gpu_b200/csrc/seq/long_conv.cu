@@ -163,6 +163,14 @@ struct LongCfg {
   static constexpr int THREADS = FPB * G::T;
   static constexpr int RS = RegionStride<LOGM, LOGP, G::T >= 16 ? 1 : 16 / G::T>::value;
   static constexpr size_t BYTES = (size_t)FPB * RS * sizeof(float2);
+  // Blocks an SM that the registers must allow for. The kernels wait on loads
+  // (the factors, mostly), so warps count more than registers: rows_kernel at
+  // 8 x 1024 x 4096 took 340, 328, 281 and 312 us with 2, 3, 4 and 5 blocks;
+  // with 32 values a thread (M = 8192), 1362 us with 1 and 934 with 2. The
+  // dkernel's sums take 32 or 64 registers more: 2 blocks up to M = 2048, 3 at
+  // 4096 (forward + gradient 722 -> 689 us), 1 at 8192.
+  static constexpr int ROW_BLOCKS = LOGM >= 13 ? 2 : 4;
+  static constexpr int DK_BLOCKS = LOGM >= 13 ? 1 : (LOGM == 12 ? 3 : 2);
 };
 
 // Orders a row's threads: its warp, its warps, or the block.
@@ -210,7 +218,7 @@ struct LongTables {
 
 // A channel's alpha and beta (scaled by 1/M) to ab[d * M + j].
 template <int LOGM>
-__global__ void __launch_bounds__(LongCfg<LOGM>::THREADS, LOGM >= 13 ? 1 : 2)
+__global__ void __launch_bounds__(LongCfg<LOGM>::THREADS, LongCfg<LOGM>::ROW_BLOCKS)
 filter_kernel(const float* __restrict__ k, const float* __restrict__ skip, float4* __restrict__ ab,
               LongTables tw, LongSizes s, bool reversed) {
   using C = LongCfg<LOGM>;
@@ -244,7 +252,7 @@ filter_kernel(const float* __restrict__ k, const float* __restrict__ skip, float
 // Rows through transform, product and inverse. Rows of a channel are
 // neighbours, so its factors come from the L2 cache after the first.
 template <class T, int LOGM>
-__global__ void __launch_bounds__(LongCfg<LOGM>::THREADS, LOGM >= 13 ? 1 : 2)
+__global__ void __launch_bounds__(LongCfg<LOGM>::THREADS, LongCfg<LOGM>::ROW_BLOCKS)
 rows_kernel(Rows<T> x, Rows<T> y, const float4* __restrict__ ab, LongTables tw, LongSizes s,
             bool x_vec, bool y_vec) {
   using C = LongCfg<LOGM>;
@@ -284,7 +292,7 @@ rows_kernel(Rows<T> x, Rows<T> y, const float4* __restrict__ ab, LongTables tw, 
 // dk of a channel over a share of the batch: the spectra of x and dy of each
 // row, their correlation summed in registers, one inverse at the end.
 template <class T, int LOGM>
-__global__ void __launch_bounds__(LongCfg<LOGM>::THREADS, LOGM >= 13 ? 1 : 2)
+__global__ void __launch_bounds__(LongCfg<LOGM>::THREADS, LongCfg<LOGM>::DK_BLOCKS)
 dkernel_kernel(Rows<T> x, Rows<T> dy, float* __restrict__ dk, LongTables tw, LongSizes s,
                int64_t share, bool x_vec, bool dy_vec) {
   using C = LongCfg<LOGM>;
