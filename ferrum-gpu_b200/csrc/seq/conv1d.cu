@@ -456,9 +456,8 @@ ferrum_status ferrum_causal_conv1d_bwd(ferrum_device* dev, const ferrum_conv1d_a
                   a->lengths, part, z, a->silu != 0);
           if (ferrum_status s = launched(what)) return s;
         }
-        cudaError_t e = launch_sum_rows(part, parts, a->taps * z.channels, cols, a->dweight, st);
-        if (e == cudaSuccess && a->dbias)
-          e = launch_sum_rows(part + a->taps * z.channels, parts, z.channels, cols, a->dbias, st);
+        cudaError_t e =
+            launch_sum_rows(part, parts, cols, a->taps * z.channels, a->dweight, a->dbias, st);
         return e == cudaSuccess ? FERRUM_OK : cuda_error(e, what);
       });
     });

@@ -619,7 +619,7 @@ ferrum_status fused_dkernel(ferrum_device* dev, const Staged<T>& x, const Staged
     if (ferrum_status r = launched(what)) return r;
     if (parts == 1) return FERRUM_OK;
     cudaError_t e = launch_sum_rows(ws.as<float>(), parts, s.channels * s.taps,
-                                    s.channels * s.taps, dk, st);
+                                    s.channels * s.taps, dk, nullptr, st);
     return e == cudaSuccess ? FERRUM_OK : cuda_error(e, what);
   });
 }

@@ -248,10 +248,11 @@ ferrum_status with_dtype(int dtype, F f) {
   return f(__nv_bfloat16());
 }
 
-// out[i] = sum over r < rows of part[r * row_stride + i], i < n, in a fixed
-// order (results do not depend on scheduling).
-cudaError_t launch_sum_rows(const float* part, int64_t rows, int64_t n, int64_t row_stride,
-                            float* out, cudaStream_t stream);
+// Sums over r < rows of part[r * n + i], in a fixed order (results do not
+// depend on scheduling): to out[i] for i < split, to rest[i - split] (where
+// rest is given) for the others.
+cudaError_t launch_sum_rows(const float* part, int64_t rows, int64_t n, int64_t split, float* out,
+                            float* rest, cudaStream_t stream);
 
 }  // namespace seq
 }  // namespace ferrum
