@@ -1,13 +1,15 @@
 // Short causal depthwise convolution over (batch, length, channels):
 //   p[t] = bias + sum_j w[j] x[t-K+1+j],  y = p or p * sigmoid(p)
 // The work is 2K operations per 2 moved values: bound by HBM. A thread owns
-// VL adjacent channels (4 forward, 2 in the gradient, so that its windows fit
-// 80 registers and 24 warps an SM hide the loads; 1 where the rows are not
-// aligned) over a run of steps, and
-// slides a window of K values through registers, so x is read once, and K-1
-// rows again at the start of each run. It loads four rows ahead of using
-// them. Runs are long (64 steps) where the batch fills the GPU and shorter
-// where it does not.
+// two adjacent channels (one where the rows are not aligned) over a run of
+// steps and slides a window of K values through registers, so x is read once,
+// and K-1 rows again at the start of each run. It loads 8 rows ahead of using
+// them (4 in the gradient). Bytes in flight decide: 8 x 2048 x 4096, 4 taps,
+// bf16 took 75 us with 4 channels, 4 rows ahead and 24 warps an SM, 92 with 8
+// channels and 16 warps, 70 with 2 channels, 8 rows and 32 warps; the
+// gradient 142 with 24 warps and 129 with 32 (float32, whose windows spill
+// there, 162 and 181). Runs are long (64 steps) where the batch fills the GPU
+// and shorter where it does not.
 //
 // Gradient, with g[t] = dy[t] * act'(p[t]):
 //   dx[s] = sum_j w[j] g[s+K-1-j],  dw[j] = sum_t g[t] x[t-K+1+j],  db = sum_t g[t]
@@ -23,7 +25,7 @@ namespace seq {
 namespace {
 
 constexpr int kThreads = 128;
-constexpr int kAhead = 4;   // rows loaded ahead
+constexpr int kAhead = 8, kAheadBwd = 4;   // rows loaded ahead
 
 struct ConvSizes {
   int64_t batch, length, channels, run, runs, col_blocks;
@@ -69,7 +71,7 @@ struct ConvPlace {
 };
 
 template <class T, int K, int VL>
-__global__ void __launch_bounds__(kThreads, VL == 1 ? 1 : 6)
+__global__ void __launch_bounds__(kThreads, VL == 1 ? 1 : 8)
 conv1d_fwd_kernel(Rows<T> x, Rows<T> y, const float* __restrict__ weight,
                   const float* __restrict__ bias, const T* st, T* fin,
                   const int32_t* __restrict__ lengths, ConvSizes s, bool silu) {
@@ -136,7 +138,7 @@ conv1d_fwd_kernel(Rows<T> x, Rows<T> y, const float* __restrict__ weight,
 }
 
 template <class T, int K, int VL>
-__global__ void __launch_bounds__(kThreads, VL == 1 ? 1 : 6)
+__global__ void __launch_bounds__(kThreads, VL == 1 ? 1 : (sizeof(T) == 2 ? 8 : 6))
 conv1d_bwd_kernel(Rows<T> x, Rows<T> dy, Rows<T> dx, const float* __restrict__ weight,
                   const float* __restrict__ bias, const T* st, const T* dfin, T* dst,
                   const int32_t* __restrict__ lengths, float* __restrict__ part, ConvSizes s,
@@ -166,18 +168,18 @@ conv1d_bwd_kernel(Rows<T> x, Rows<T> dy, Rows<T> dx, const float* __restrict__ w
   // sequence, or dx in front of the run, or a final state's gradient joins.
   auto block = [&](auto edge, int t) {
     constexpr bool EDGE = decltype(edge)::value;
-    float in[kAhead][VL], gin[kAhead][VL];
+    float in[kAheadBwd][VL], gin[kAheadBwd][VL];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
+    for (int i = 0; i < kAheadBwd; ++i) {
       if (EDGE) clear(in[i]), clear(gin[i]);
       if (!EDGE || t + i < valid) {
         load_vec<T, VL>(px + i * x.st, in[i]);
         load_vec<T, VL>(pg + i * dy.st, gin[i]);
       }
     }
-    px += kAhead * x.st, pg += kAhead * dy.st;
+    px += kAheadBwd * x.st, pg += kAheadBwd * dy.st;
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
+    for (int i = 0; i < kAheadBwd; ++i) {
       if (EDGE && t + i >= n + K - 1) return;
       float o[VL];
 #pragma unroll
@@ -233,9 +235,9 @@ conv1d_bwd_kernel(Rows<T> x, Rows<T> dy, Rows<T> dx, const float* __restrict__ w
   const int64_t whole64 = dfin != nullptr ? left - (K - 1) : left;
   const int whole = (int)(whole64 < n ? whole64 : n);
   int t = 0;
-  for (; t < n + K - 1 && t < K - 1; t += kAhead) block(std::true_type(), t);
-  for (; t + kAhead <= whole; t += kAhead) block(std::false_type(), t);
-  for (; t < n + K - 1; t += kAhead) block(std::true_type(), t);
+  for (; t < n + K - 1 && t < K - 1; t += kAheadBwd) block(std::true_type(), t);
+  for (; t + kAheadBwd <= whole; t += kAheadBwd) block(std::false_type(), t);
+  for (; t < n + K - 1; t += kAheadBwd) block(std::true_type(), t);
   float* o = part + (b * s.runs + at.run) * (K + 1) * s.channels;
 #pragma unroll
   for (int e = 0; e < VL; ++e) {
@@ -365,7 +367,7 @@ ferrum_status conv_fwd(ferrum_device* dev, const ferrum_conv1d_args* a, cudaStre
   if (guard.status() != cudaSuccess) return cuda_error(guard.status(), "cudaSetDevice");
   return with_dtype(a->dtype, [&](auto tag) {
     using T = decltype(tag);
-    return with_conv<4>(a->taps, conv_vec(a, false, 4), [&](auto k, auto vl) -> ferrum_status {
+    return with_conv<2>(a->taps, conv_vec(a, false, 2), [&](auto k, auto vl) -> ferrum_status {
       const ConvSizes s = conv_sizes(a, decltype(vl)::value);
       const int64_t blocks = s.batch * s.runs * s.col_blocks;
       if (ferrum_status st = grid_ok(blocks, what)) return st;
