@@ -170,6 +170,13 @@ struct LongCfg {
   // dkernel's sums take 32 or 64 registers more: 2 blocks up to M = 2048, 3 at
   // 4096 (forward + gradient 722 -> 689 us), 1 at 8192.
   static constexpr int ROW_BLOCKS = LOGM >= 13 ? 2 : 4;
+  // rows_kernel's factors (16 bytes a bin, from the L2 cache) cost a quarter of
+  // its time where each is loaded when it is needed (8 x 1024 x 4096 without
+  // any loads: 211 us). What shared memory is left beside ROW_BLOCKS blocks
+  // takes the first STAGED of a thread's P of them, copied while the first
+  // transform runs: 281 -> 271 us, M = 8192 934 -> 840.
+  static constexpr int STAGED = LOGM >= 13 ? 10 : 5;
+  static constexpr size_t ROW_BYTES = BYTES + sizeof(float4) * (size_t)(STAGED * THREADS);
   static constexpr int DK_BLOCKS = LOGM >= 13 ? 1 : (LOGM == 12 ? 3 : 2);
 };
 
@@ -265,6 +272,10 @@ rows_kernel(Rows<T> x, Rows<T> y, const float4* __restrict__ ab, LongTables tw, 
   float2* sm = sm_all + g * C::RS;
   const RowSync<G::T, C::FPB> sync{g};
   const T* xr = x.at(b, d);
+  const float4* f = ab + (d << LOGM);
+  float4* staged = (float4*)(sm_all + C::FPB * C::RS) + threadIdx.x;   // read back by this thread
+#pragma unroll
+  for (int m = 0; m < C::STAGED; ++m) cp_async<16>(staged + m * C::THREADS, f + t + G::T * m, 16);
   float2 v[G::P];
 #pragma unroll
   for (int m = 0; m < G::P; ++m)
@@ -272,10 +283,10 @@ rows_kernel(Rows<T> x, Rows<T> y, const float4* __restrict__ ab, LongTables tw, 
                         : make_float2(0.f, 0.f);
   run_stages<LOGM, C::LOGP, 0>(v, sm, t, tw.stage, sync);
   put_spectrum<LOGM>(v, sm, t, sync);
-  const float4* f = ab + (d << LOGM);
+  cp_async_wait();
 #pragma unroll
   for (int m = 0; m < G::P; ++m) {
-    const float4 c = __ldg(f + t + G::T * m);
+    const float4 c = m < C::STAGED ? staged[m * C::THREADS] : __ldg(f + t + G::T * m);
     const float2 u = c_add(c_mul(v[m], make_float2(c.x, c.y)),
                            c_mul(conj2(mirrored<LOGM>(sm, t, m)), make_float2(c.z, c.w)));
     v[m] = make_float2(u.y, u.x);     // swapped: the inverse by a forward transform
@@ -585,12 +596,12 @@ ferrum_status fused_rows(ferrum_device* dev, const Staged<T>& x, const Staged<T>
     using C = LongCfg<L>;
     static std::atomic<uint64_t> done_f{0}, done_r{0};
     if (ferrum_status r = allow_smem(filter_kernel<L>, C::BYTES, done_f, what)) return r;
-    if (ferrum_status r = allow_smem(rows_kernel<T, L>, C::BYTES, done_r, what)) return r;
+    if (ferrum_status r = allow_smem(rows_kernel<T, L>, C::ROW_BYTES, done_r, what)) return r;
     launch_detail::clear_stale_error();
     filter_kernel<L><<<(unsigned)ceil_div(s.channels, C::FPB), C::THREADS, C::BYTES, st>>>(
         k, skip, ab.as<float4>(), tw, s, reversed);
     rows_kernel<T, L>
-        <<<(unsigned)ceil_div(s.batch * s.channels, C::FPB), C::THREADS, C::BYTES, st>>>(
+        <<<(unsigned)ceil_div(s.batch * s.channels, C::FPB), C::THREADS, C::ROW_BYTES, st>>>(
             x.rows(), y.rows(), ab.as<float4>(), tw, s, x.vec(), y.vec());
     return launched(what);
   });

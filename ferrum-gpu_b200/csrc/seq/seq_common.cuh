@@ -121,6 +121,19 @@ __device__ __forceinline__ void store_vec(T* p, const float (&v)[VL]) {
   }
 }
 
+// Asynchronous copies from global to shared memory, `bytes` of the unit read
+// and the rest zeroed.
+template <int UNIT>
+__device__ __forceinline__ void cp_async(void* dst, const void* src, int bytes) {
+  const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
+  if constexpr (UNIT == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src), "r"(bytes));
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(d), "l"(src), "r"(bytes));
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;"); }
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
 // Sum over the 32 lanes, in every lane, in a fixed order.
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll

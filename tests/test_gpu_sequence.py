@@ -723,6 +723,64 @@ def test_graph_capture_of_a_decode_step():
         assert torch.equal(out, want[i])
 
 
+def test_offsets_beyond_32_bits():
+    """Arrays of more than 2^31 values: their last part equals a call on that
+    part alone. Steps are cut at a multiple of every internal piece length, so
+    the same arithmetic runs and the bits agree."""
+    dt = torch.bfloat16
+    n, d, cut = (1 << 20) + 40, 2056, 1 << 20
+    assert n * d > 2 ** 31
+    x = torch.empty(1, n, d, dtype=dt, device="cuda").normal_()
+    tail = x[:, cut:].contiguous()
+    w = rnd(1, d, 4)
+    y = sq.causal_conv1d(x, w, activation="silu")
+    st = x[:, cut - 3:cut].contiguous()
+    assert torch.equal(y[:, cut:], sq.causal_conv1d(tail, w, activation="silu", initial_state=st))
+    g = sq.causal_conv1d_backward(y, x, w, activation="silu")
+    h = sq.causal_conv1d_backward(y[:, cut:].contiguous(), tail, w, activation="silu",
+                                  initial_state=st)
+    assert torch.equal(g.dx[:, cut:], h.dx)
+    del g, h
+    A, B = -rnd(2, d, 8).abs(), rnd(3, 1, n, 8, dtype=dt)
+    one = sq.selective_scan(x, y, A, B, B, delta_softplus=True, save_states=True)
+    at = one.states[:, cut // sq.SAVE_STEPS].clone()
+    two = sq.selective_scan(tail, y[:, cut:], A, B[:, cut:], B[:, cut:], delta_softplus=True,
+                            initial_state=at, save_states=True)
+    check(one.out[:, cut:], two.out.double(), 12 * 40)
+    check(one.final_state, two.final_state.double(), 12 * 40)
+    g = sq.selective_scan_backward(y, x, y, A, B, B, one.states, delta_softplus=True)
+    h = sq.selective_scan_backward(y[:, cut:], tail, y[:, cut:], A, B[:, cut:], B[:, cut:],
+                                   two.states, delta_softplus=True)
+    check(g.du[:, cut:], h.du.double(), 24 * 40 + d)
+    check(g.dB[:, cut:], h.dB.double(), 24 * 40 + d)
+    del one, two, g, h
+    m, wt = x[0], rnd(4, d)
+    yb, r = sq.norm_before(m, wt, residual=y[0])
+    yt, rt = sq.norm_before(m[cut:], wt, residual=y[0, cut:])
+    assert torch.equal(yb[cut:], yt) and torch.equal(r[cut:], rt)
+    assert torch.equal(sq.norm_before_backward(yb, r, wt).dx[cut:],
+                       sq.norm_before_backward(yt, rt, wt).dx)
+    del yb, r
+    assert torch.equal(sq.norm_after(m, wt, gate=y[0], groups=8)[cut:],
+                       sq.norm_after(m[cut:], wt, gate=y[0, cut:], groups=8))
+    assert torch.equal(sq.norm_after_backward(y[0], m, wt, gate=y[0], groups=8).dgate[cut:],
+                       sq.norm_after_backward(y[0, cut:], m[cut:], wt, gate=y[0, cut:], groups=8).dgate)
+    del x, y, m
+    rows, length = 1 << 16, 1 << 15
+    x = torch.empty(rows + 8, 1, length, dtype=dt, device="cuda").normal_()
+    assert x.numel() > 2 ** 31
+    pos = torch.full((rows + 8,), length - 1, dtype=torch.int32, device="cuda")
+    k = rnd(5, 1, length, std=length ** -0.5)
+    last = x[-8:].clone()
+    v = rnd(6, rows + 8, 1, dtype=dt)
+    y = sq.long_conv_step(v, x, pos, k)
+    assert torch.equal(y[-8:], sq.long_conv_step(v[-8:], last, pos[-8:], k))
+    assert torch.equal(x[-8:], last)
+    x = x.view(-1, 1, 4096)
+    assert torch.equal(sq.long_conv(x, k[:, :4096].contiguous())[-8:],
+                       sq.long_conv(x[-8:], k[:, :4096].contiguous()))
+
+
 def test_refusals():
     x = rnd(1, 2, 6, 8)
     w4 = rnd(2, 8, 4)
