@@ -45,7 +45,7 @@ struct FwdCfg {
 template <class T, int G, int S, int NP>
 __global__ void __launch_bounds__(FwdCfg<T, G, S, NP>::THREADS, 512 / FwdCfg<T, G, S, NP>::THREADS)
 scan_fwd_kernel(ScanIn<T> in, Rows<T> out, float* fin, float* __restrict__ saved, ScanSizes s,
-                int64_t col_blocks, int unit, int bc_unit, int out_unit) {
+                int64_t col_blocks, int unit, int bc_unit, int out_unit, bool save_vec) {
   using C = FwdCfg<T, G, S, NP>;
   constexpr int CH = C::CH, CK = C::CK, kThreads = C::THREADS;
   using X = Piece<T, CH>;
@@ -192,10 +192,14 @@ scan_fwd_kernel(ScanIn<T> in, Rows<T> out, float* fin, float* __restrict__ saved
       }
       if (so != nullptr) {
         const float2 p = unpack(h0), r = unpack(h1);
-        if (n + 0 < s.states) so[n + 0] = p.x;
-        if (n + 1 < s.states) so[n + 1] = p.y;
-        if (n + 2 < s.states) so[n + 2] = r.x;
-        if (n + 3 < s.states) so[n + 3] = r.y;
+        if (save_vec) {
+          *(float4*)(so + n) = make_float4(p.x, p.y, r.x, r.y);
+        } else {
+          if (n + 0 < s.states) so[n + 0] = p.x;
+          if (n + 1 < s.states) so[n + 1] = p.y;
+          if (n + 2 < s.states) so[n + 2] = r.x;
+          if (n + 3 < s.states) so[n + 3] = r.y;
+        }
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -366,7 +370,8 @@ ferrum_status run_fwd(const ferrum_scan_args* a, const ScanSizes& s, cudaStream_
   launch_detail::clear_stale_error();
   scan_fwd_kernel<T, G, S, NP><<<(unsigned)blocks, C::THREADS, C::BYTES, stream>>>(
       scan_in<T>(a), rows_of<T>(a->out), a->final_state, a->saved_states, s, col_blocks, unit,
-      bc_unit, copy_unit<T>(a->out, one_group ? 0 : s.per_group));
+      bc_unit, copy_unit<T>(a->out, one_group ? 0 : s.per_group),
+      s.states == NP && aligned(a->saved_states, 16));
   return launched(what);
 }
 
