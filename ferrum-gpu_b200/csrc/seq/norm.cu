@@ -82,14 +82,13 @@ struct Unit {
 };
 
 // Warps an SM that the registers must allow for, so that enough loads are in
-// flight: 32 forward; 24 (of blocks up to 256 threads) or 32 in the gradient,
-// whose sums take more.
-constexpr int kFwdWarps = 32;
-template <int TPR, int EPT>
-constexpr int bwd_blocks() {
-  constexpr int threads = TPR == 32 ? 256 : TPR;
-  return EPT > 8 ? 1 : (threads <= 256 ? 768 / threads : 1024 / threads);
+// flight: 32; in norm_after's gradient, which spills more than it gains there
+// (16384 x 2048: 111 us against 125), 24 for blocks of up to 256 threads.
+constexpr int kWarps = 32, kAfterBwdWarps = 24;
+constexpr int min_blocks(int tpr, int values, int warps) {
+  return values > 8 ? 1 : (tpr == 32 ? warps / 8 : std::max(1, warps * 32 / tpr));
 }
+constexpr int after_bwd_warps(int tpr) { return tpr <= 256 ? kAfterBwdWarps : kWarps; }
 
 // The next row's line to the L2 cache while this row is worked on: 8 % for
 // norm_before at 8191 x 4096; the other kernels, bound by instructions, lose.
@@ -156,7 +155,7 @@ __device__ __forceinline__ void load_param(const float* p, int64_t c, float (&v)
 }
 
 template <class T, class R, int TPR, int VL, int NC>
-__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, NC * VL <= 8 ? kFwdWarps * 32 / (TPR == 32 ? 256 : TPR) : 1)
+__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, min_blocks(TPR, VL * NC, kWarps))
 norm_before_kernel(NormArgs a, const T* x, const R* res, T* y, R* r) {
   __shared__ float sh[2 * 3 * TPR / 32];
   const Unit<TPR, VL, NC> u(a.groups);
@@ -215,8 +214,8 @@ __device__ __forceinline__ void store_sums(const NormArgs& a, const Unit<TPR, VL
         for (int e = 0; e < VL; ++e) part[(u.index * 3 + j) * a.width + u.col(k) + e] = s[j][k][e];
 }
 
-template <class T, class R, int TPR, int VL, int NC>
-__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, bwd_blocks<TPR, VL * NC>())
+template <class T, class R, bool BIAS, int TPR, int VL, int NC>
+__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, min_blocks(TPR, VL * NC, kWarps))
 norm_before_bwd_kernel(NormArgs a, const T* x, const R* r, const T* dy, const R* dr, T* dx, R* dres,
                        float* part) {
   __shared__ float sh[2 * 3 * TPR / 32];
@@ -264,7 +263,7 @@ norm_before_bwd_kernel(NormArgs a, const T* x, const R* r, const T* dy, const R*
       for (int e = 0; e < VL; ++e) {
         const float n = v[k][e] * inv;
         sums[0][k][e] = fmaf(g[k][e], n, sums[0][k][e]);
-        sums[1][k][e] += g[k][e];
+        if constexpr (BIAS) sums[1][k][e] += g[k][e];
         o[e] = norm_grad(a, inv, dn[k][e], n, g1, g2);
       }
       if (dr) {
@@ -296,7 +295,7 @@ norm_before_bwd_kernel(NormArgs a, const T* x, const R* r, const T* dy, const R*
 enum { kNoGate = 0, kInside = 1, kOutside = 2 };
 
 template <class T, class R, int GATE, int TPR, int VL, int NC>
-__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, NC * VL <= 8 ? kFwdWarps * 32 / (TPR == 32 ? 256 : TPR) : 1)
+__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, min_blocks(TPR, VL * NC, kWarps))
 norm_after_kernel(NormArgs a, const T* x, const T* gate, const R* res, T* y) {
   __shared__ float sh[2 * 3 * TPR / 32];
   const Unit<TPR, VL, NC> u(a.groups);
@@ -344,7 +343,8 @@ norm_after_kernel(NormArgs a, const T* x, const T* gate, const R* res, T* y) {
 }
 
 template <class T, int GATE, int TPR, int VL, int NC>
-__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR, bwd_blocks<TPR, VL * NC>())
+__global__ void __launch_bounds__(TPR == 32 ? 256 : TPR,
+                                  min_blocks(TPR, VL * NC, after_bwd_warps(TPR)))
 norm_after_bwd_kernel(NormArgs a, const T* x, const T* gate, const T* dy, T* dx, T* dgate,
                       float* part) {
   __shared__ float sh[2 * 3 * TPR / 32];
@@ -423,33 +423,31 @@ norm_after_bwd_kernel(NormArgs a, const T* x, const T* gate, const T* dy, T* dx,
   store_sums(a, u, sums, part);
 }
 
-// The units' column sums, added in order: unit j * groups + g holds group g's.
-__global__ void __launch_bounds__(256)
+// The units' column sums, added in a fixed order: unit j * groups + g holds
+// group g's. 32 columns by 32 strands of units.
+__global__ void __launch_bounds__(1024)
 norm_sums_kernel(const float* __restrict__ part, int64_t units, int64_t groups, int64_t width,
                  float* dweight, float* dbias, float* dscale) {
-  __shared__ float sh[8][32];
+  __shared__ float sh[32][33];
   const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
   const int64_t wb = (width + 31) / 32;
   int64_t q = blockIdx.x;
-  const int64_t i = q % wb * 32 + x;
+  const int64_t i0 = q % wb * 32;
   q /= wb;
   const int64_t g = q % groups;
   const int k = (int)(q / groups);
   float* out = k == 0 ? dweight : (k == 1 ? dbias : dscale);
   if (out == nullptr) return;
   float s = 0.f;
-  if (i < width) {
+  if (i0 + x < width) {
 #pragma unroll 4
-    for (int64_t j = y; j < units / groups; j += 8)
-      s += part[((j * groups + g) * 3 + k) * width + i];
+    for (int64_t j = y; j < units / groups; j += 32)
+      s += part[((j * groups + g) * 3 + k) * width + i0 + x];
   }
   sh[y][x] = s;
   __syncthreads();
-  if (y == 0 && i < width) {
-#pragma unroll
-    for (int j = 1; j < 8; ++j) s += sh[j][x];
-    out[g * width + i] = s;
-  }
+  s = warp_sum(sh[x][y]);       // column y of the 32, over the strands
+  if (x == 0 && i0 + y < width) out[g * width + i0 + y] = s;
 }
 
 NormArgs norm_args(const ferrum_norm_args* a) {
@@ -593,7 +591,7 @@ ferrum_status norm_fwd(ferrum_device* dev, const ferrum_norm_args* a, bool befor
   return with_residual(a->dtype, a->residual_dtype, [&](auto tx, auto tr) {
     return with_shape(n.width, norm_vec(a, false), [&](auto tpr, auto vl, auto nc) {
       constexpr int TPR = decltype(tpr)::value;
-      const int64_t blocks = unit_blocks<TPR>(n.rows, n.groups, kFwdWarps * 32);
+      const int64_t blocks = unit_blocks<TPR>(n.rows, n.groups, kWarps * 32);
       launch_detail::clear_stale_error();
       go(n, tx, tr, tpr, vl, nc, (unsigned)blocks, TPR == 32 ? 256 : TPR);
       return launched(what);
@@ -614,13 +612,14 @@ ferrum_status norm_bwd(ferrum_device* dev, const ferrum_norm_args* a, bool befor
     return with_shape(n.width, norm_vec(a, true), [&](auto tpr, auto vl, auto nc) -> ferrum_status {
       constexpr int TPR = decltype(tpr)::value;
       constexpr int threads = TPR == 32 ? 256 : TPR;
-      const int64_t blocks = unit_blocks<TPR>(n.rows, n.groups, TPR <= 256 ? 768 : 1024);
+      const int64_t blocks = unit_blocks<TPR>(
+          n.rows, n.groups, 32 * (before ? kWarps : after_bwd_warps(TPR)));
       const int64_t units = blocks * (threads / TPR) / n.groups * n.groups;
       PoolBuffer part(dev, sizeof(float) * (size_t)(blocks * (threads / TPR) * 3 * n.width), st);
       if (part.status() != cudaSuccess) return cuda_error(part.status(), "workspace");
       launch_detail::clear_stale_error();
       go(n, tx, tr, tpr, vl, nc, (unsigned)blocks, threads, part.as<float>());
-      norm_sums_kernel<<<(unsigned)(ceil_div(n.width, 32) * n.groups * 3), 256, 0, st>>>(
+      norm_sums_kernel<<<(unsigned)(ceil_div(n.width, 32) * n.groups * 3), 1024, 0, st>>>(
           part.as<float>(), units, n.groups, n.width, a->dweight, a->dbias, a->dscale);
       return launched(what);
     });
@@ -653,10 +652,17 @@ ferrum_status ferrum_norm_before_bwd(ferrum_device* dev, const ferrum_norm_args*
                         unsigned blocks, int threads, float* part) {
       using T = decltype(tx);
       using R = decltype(tr);
-      norm_before_bwd_kernel<T, R, decltype(tpr)::value, decltype(vl)::value, decltype(nc)::value>
-          <<<blocks, threads, 0, (cudaStream_t)stream>>>(
-              n, a->dscale ? (const T*)a->x : nullptr, (const R*)a->r, (const T*)a->dy,
-              (const R*)a->dr, (T*)a->dx, (R*)a->dresidual, part);
+      auto go = [&](auto bias) {
+        norm_before_bwd_kernel<T, R, decltype(bias)::value, decltype(tpr)::value,
+                               decltype(vl)::value, decltype(nc)::value>
+            <<<blocks, threads, 0, (cudaStream_t)stream>>>(
+                n, a->dscale ? (const T*)a->x : nullptr, (const R*)a->r, (const T*)a->dy,
+                (const R*)a->dr, (T*)a->dx, (R*)a->dresidual, part);
+      };
+      if (a->dbias)     // its sums take registers that the others can use
+        go(std::true_type());
+      else
+        go(std::false_type());
     });
   });
 }
