@@ -20,6 +20,10 @@
 // and one write of it (the butterflies and exchanges of stockham.cuh, and one
 // more exchange for Z[M-j]); longer rows go through the library's multi-pass
 // transforms. Short rows take the defining sum.
+// Measured, 8 x 1024 x 4096, bf16: 271 us, of which the filter's transform 20;
+// two 4096-point transforms a row alone (no factor loads) 190. Exchanges in
+// shared memory (62 % of its bandwidth), issue slots (51 %) and the waits for
+// the factors bound it; HBM would take 23 us. With dx and dk 677 us.
 #include <algorithm>
 
 #include "../fft_kernels.cuh"

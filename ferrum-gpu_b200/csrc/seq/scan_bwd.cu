@@ -13,8 +13,13 @@
 // memory; sums over channels (dB, dC) likewise, 16 values of 32 lanes at a
 // time (a transposed read costs a third of a reduction by shuffles), and from
 // block to block through a workspace, all in fixed order.
-// About 22 instructions and 1.5 exponentials per (step, channel, state) bound
-// it: issue slots first, the special-function unit next, HBM last.
+// Measured, 8 x 2048 x 2048, 16 states, bf16: 1.16 ms (HBM would take 90 us, the
+// special-function unit about 200). Shared memory bandwidth (75 %: tiles, and
+// the sums over states and channels) and short-scoreboard waits at 14 warps
+// an SM bound it; issue slots are 44 % used. Four states a thread with the
+// sums over states by shuffles inside a warp halves the shared memory
+// traffic but leaves 7 warps an SM at that size: 1.35 ms (0.99 against 1.07 at
+// 64 x 256 x 2048, 6.7 against 3.7 with 64 states).
 #include <algorithm>
 
 #include "scan.cuh"
