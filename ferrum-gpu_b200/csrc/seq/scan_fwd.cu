@@ -20,7 +20,7 @@
 // instructions over pairs of states.
 // Measured, 16 states, bf16: 8 x 2048 x 2048 in 384 us, 1.4e12 exponentials a
 // second (39 % of the special-function unit, issue slots 56 %, shared memory
-// 64 %; HBM would take 41 us); 1 x 8192 x 2048 in 332 us, issue 54 %. What is
+// 64 %; HBM would take 41 us); 1 x 8192 x 2048 in 307 us. What is
 // left is latency at 13 warps an SM: steps are a chain within a channel.
 // Giving each thread a share of a channel's states over all steps instead (no
 // compositions, 30 % fewer instructions) took 350 us at 8 x 2048 x 2048, but
@@ -396,22 +396,30 @@ ferrum_status scan_fwd(ferrum_device* dev, const ferrum_scan_args* a, cudaStream
   if (guard.status() != cudaSuccess) return cuda_error(guard.status(), "cudaSetDevice");
   // Lanes per channel: few keep the shuffles short. Where a batch has too few
   // channels to fill the GPU that way, a channel gets more lanes, then several
-  // warps that share its states. Measured (us, 16 states, bf16), levels 0..3:
-  //   8 x 2048 x 2048    385  381  571  759     4 x 4096 x 2048   527  421  588  757
-  //   2 x 8192 x 2048    901  585  649  775     1 x 8192 x 2048   901  516  332  439
-  //   64 x 256 x 2048    341  375  627  837     1 x 4096 x 512    453  262  127   80
+  // warps that share its states. Measured (us, 16 states, bf16) for lanes x
+  // warps, the choice marked:
+  //                    4 x 1   8 x 1   16 x 1   16 x 2   16 x 4   8 x 4
+  //   8 x 2048 x 2048   382*    377     416      531      754     567
+  //   4 x 4096 x 2048   519     418*    424      547      752     586
+  //   2 x 8192 x 2048   883     574     471*     604      770     649
+  //   1 x 8192 x 2048   883     501     330      307*     436     332
+  //   1 x 4096 x 512    444     254     145      115       80*    125
+  // (13 x 777 x 1000 in float32: 137 and 152 with 4 x 1 and 8 x 1.)
   const int64_t rows = s.batch * s.channels;
-  const int level = rows >= 12288 || s.length <= 32 ? 0
-                    : rows >= 3000                  ? 1
-                    : rows >= 1000 || s.length <= 64 ? 2 : 3;
+  const int level = rows >= 12288 || s.length <= 32  ? 0
+                    : rows >= 6000 || s.length <= 64 ? 1
+                    : rows >= 3000                   ? 2
+                    : rows >= 1000                   ? 3 : 4;
   return with_dtype(a->dtype, [&](auto tag) {
     using T = decltype(tag);
     return with_states(s.states, [&](auto np) -> ferrum_status {
-      constexpr int NP = decltype(np)::value, S = NP == 8 ? 2 : 4;
+      constexpr int NP = decltype(np)::value;
       if (level == 0) return run_fwd<T, 4, 1, NP>(a, s, stream, what);
       if (level == 1) return run_fwd<T, 8, 1, NP>(a, s, stream, what);
-      if (level == 2) return run_fwd<T, 8, S, NP>(a, s, stream, what);
-      return run_fwd<T, 16, S, NP>(a, s, stream, what);
+      if (level == 2) return run_fwd<T, 16, 1, NP>(a, s, stream, what);
+      if (level == 3 || NP == 8) return run_fwd<T, 16, 2, NP>(a, s, stream, what);
+      if constexpr (NP > 8) return run_fwd<T, 16, 4, NP>(a, s, stream, what);
+      return FERRUM_OK;
     });
   });
 }

@@ -218,6 +218,14 @@ SCAN = [  # batch, length, channels, states, groups, full (D, z, bias, softplus,
     (1, 193, 70, 64, 2, False, False),
     (1, 1030, 16, 16, 1, True, False),
     (2, 256, 160, 16, 1, False, True),
+    # more channels: every split of a channel's steps and states over lanes
+    (1, 270, 1100, 16, 1, True, False),
+    (2, 140, 1604, 16, 2, True, True),
+    (4, 100, 1702, 13, 1, True, True),
+    (7, 90, 1800, 16, 1, True, False),
+    (1, 135, 1001, 64, 1, True, False),
+    (3, 131, 1002, 32, 2, False, True),
+    (3, 70, 4100, 8, 1, True, True),
 ]
 
 
