@@ -390,7 +390,8 @@ def ref_norm(v, kind, eps, groups=1):
     return (v / torch.sqrt((v * v).mean(-1, keepdim=True) + eps)).reshape(s)
 
 
-ROWS = [(1, 1), (3, 7), (5, 64), (33, 257), (2, 1000), (130, 768), (17, 4096), (3, 5001), (2, 20000)]
+ROWS = [(1, 1), (3, 7), (5, 64), (33, 257), (2, 1000), (130, 768), (17, 4096), (3, 5001), (2, 20000),
+        (3, 6000), (2, 9001)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -433,7 +434,7 @@ def test_norm_before(dtype, m, d, kind, parts, res32):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("m,d,groups", [(1, 1, 1), (3, 12, 4), (5, 64, 1), (33, 258, 2),
                                         (7, 1000, 8), (130, 768, 1), (9, 4096, 8), (3, 5005, 5),
-                                        (2, 20000, 1)])
+                                        (2, 20000, 1), (3, 6000, 1), (2, 9001, 1)])
 @pytest.mark.parametrize("kind,where,parts", [("rms", "in", "rsb"), ("layer", "out", "rsb"),
                                               ("rms", "out", "r"), ("layer", "none", "s"),
                                               ("layer", "in", "")])
@@ -505,7 +506,7 @@ def ref_long(x, k, skip):
 
 
 LONG = [(1, 1, 1, 1), (2, 3, 2, 2), (3, 5, 17, 17), (2, 4, 64, 30), (1, 3, 100, 100),
-        (3, 7, 129, 129), (2, 5, 255, 200), (1, 2, 256, 256), (2, 3, 513, 513), (3, 4, 1000, 1000),
+        (3, 7, 129, 129), (2, 5, 255, 200), (1, 2, 256, 256), (3, 9, 500, 500), (2, 3, 513, 513), (3, 4, 1000, 1000),
         (2, 2, 2048, 2048), (1, 3, 4095, 1), (2, 2, 4096, 4096), (3, 2, 5000, 4000),
         (1, 2, 8193, 8193), (2, 1, 16384, 16384), (1, 2, 16385, 16385), (1, 1, 40000, 40000)]
 
