@@ -75,19 +75,19 @@ ferrum_status ferrum_causal_conv1d(ferrum_device *dev, const ferrum_conv1d_args 
 /* Uses x, dy, weight, bias, initial_state, lengths, dfinal_state. */
 ferrum_status ferrum_causal_conv1d_bwd(ferrum_device *dev, const ferrum_conv1d_args *args,
                                        void *stream);
-/* One step of every sequence (length 1): initial_state is the state before,
- * final_state the state after (may be the same array). */
+/* One step of every sequence (length 1, no lengths): initial_state is the state
+ * before, final_state the state after (may be the same array). */
 ferrum_status ferrum_causal_conv1d_step(ferrum_device *dev, const ferrum_conv1d_args *args,
                                         void *stream);
 
 /* ---------------------------------------------------------------------------
- * Row strides of the scan's arrays must fit 32 bits.
  * Selective state space scan, N states per channel, N in [1, 64]:
  *   s  = delta[b,t,d] + delta_bias[d];  dt = delta_softplus ? log(1 + e^s) : s
  *   h[n] = exp(dt * A[d,n]) * h[n] + dt * u[b,t,d] * B[b,t,g,n]
  *   y  = sum_n h[n] * C[b,t,g,n] + D[d] * u[b,t,d]
  *   out = z ? y * z * sigmoid(z) : y
- * Channel d belongs to group g = d / (channels / groups).
+ * Channel d belongs to group g = d / (channels / groups). Row strides must fit
+ * 32 bits.
  */
 typedef struct {
   size_t struct_size;
@@ -114,8 +114,8 @@ typedef struct {
 ferrum_status ferrum_selective_scan(ferrum_device *dev, const ferrum_scan_args *args, void *stream);
 ferrum_status ferrum_selective_scan_bwd(ferrum_device *dev, const ferrum_scan_args *args,
                                         void *stream);
-/* One step of every sequence (length 1): initial_state (required) before,
- * final_state (required, may be the same array) after. */
+/* One step of every sequence (length 1, no lengths): initial_state (required)
+ * before, final_state (required, may be the same array) after. */
 ferrum_status ferrum_selective_scan_step(ferrum_device *dev, const ferrum_scan_args *args,
                                          void *stream);
 
