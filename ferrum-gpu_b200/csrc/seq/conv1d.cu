@@ -327,9 +327,12 @@ ConvSizes conv_sizes(const ferrum_conv1d_args* a, int vl) {
   ConvSizes s;
   s.batch = (int64_t)a->batch, s.length = (int64_t)a->length, s.channels = (int64_t)a->channels;
   s.col_blocks = ceil_div(s.channels, kThreads * vl);
-  // at least 1024 threads an SM, if that takes runs of no less than 8 steps
+  // Long runs read few rows twice; short ones give every SM work. 4 blocks an
+  // SM, if that takes runs of no less than 8 steps (us, forward and gradient,
+  // with runs of 64 and 8 steps: 1 x 1000 x 2048 16.4, 28.9 and 10.2, 22.8;
+  // 1 x 8192 x 2048 24.6, 47.4 and 34.8, 82.2).
   s.run = 64;
-  while (s.run > 8 && s.batch * s.col_blocks * ceil_div(s.length, s.run) < 148 * 8) s.run /= 2;
+  while (s.run > 8 && s.batch * s.col_blocks * ceil_div(s.length, s.run) < 148 * 4) s.run /= 2;
   s.runs = s.length > 0 ? ceil_div(s.length, s.run) : 1;  // an empty prompt still copies its state
   return s;
 }
