@@ -73,6 +73,13 @@ __device__ __forceinline__ f2 mul2(f2 a, f2 b) {
   return r;
 }
 
+// The smaller value, or NaN where either is one.
+__device__ __forceinline__ float min_nan(float x, float y) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+  return r;
+}
+
 // A piece of a (steps, columns) array in shared memory, in its own type: row
 // t at t * COLS elements plus 16 bytes for every 8 rows, so that lanes 8 rows
 // apart meet different banks.

@@ -7,7 +7,11 @@
 // consecutive steps each: a lane composes its 8 maps, the G lanes scan the
 // compositions by shuffles (log2 G rounds), and each lane, now knowing the
 // state in front of its steps, walks them again for the outputs, with the
-// same a and b still in registers. Each exponential is computed once, which
+// same a and b still in registers. A range's factor is the product of its
+// steps' while none of them can be above 1. Where A > 0, or dt < 0 for want of
+// the softplus, that product can pass the largest float32 in front of a state
+// that is 0 or small; there a block takes exp(A sum dt), applied as its square
+// root, twice (8 x 2048 x 2048 of 16 states: 406 us against 385). Each exponential is computed once, which
 // matters because they bound the kernel: N per value on the special-function
 // unit (16 a clock and SM) against about 6 N FP32 operations (128 a clock).
 // Splitting the axis over blocks instead would need the exponentials twice.
@@ -41,6 +45,7 @@ struct FwdCfg {
   static constexpr int THREADS = S == 1 ? 128 : 256;
   static constexpr int CH = THREADS / S / G;      // channels per block
   static constexpr int CK = kLaneSteps * G;       // steps per piece
+  static constexpr int ROUNDS = G == 4 ? 2 : (G == 8 ? 3 : 4);   // log2 G
   static constexpr int XS = Piece<T, CH>::size(CK), RS = Piece<T, NP>::size(CK);
   static constexpr int FS = Piece<float, NP>::size(CK);
   static constexpr int YS = CH * (CK + 4);        // a float32 (channel, step) tile
@@ -49,12 +54,20 @@ struct FwdCfg {
       sizeof(float) * (size_t)(2 * FS + 2 * CH * NP + (S == 1 ? 0 : (S + 1) * YS));
 };
 
+// The square roots of two states' factors over steps whose dt add up to 2 w.
+// Clamped below the exponent range's end: a factor that large overflows any
+// state but 0. A NaN stays.
+__device__ __forceinline__ f2 root_factor(float w, float Ax, float Ay) {
+  const float2 e = unpack(mul2(pack(w, w), pack(Ax, Ay)));
+  return pack(ex2(min_nan(e.x, 127.f)), ex2(min_nan(e.y, 127.f)));
+}
+
 template <class T, int G, int S, int NP>
 __global__ void __launch_bounds__(FwdCfg<T, G, S, NP>::THREADS, 512 / FwdCfg<T, G, S, NP>::THREADS)
 scan_fwd_kernel(ScanIn<T> in, Rows<T> out, float* fin, float* __restrict__ saved, ScanSizes s,
                 int64_t col_blocks, int unit, int bc_unit, int out_unit, bool save_vec) {
   using C = FwdCfg<T, G, S, NP>;
-  constexpr int CH = C::CH, CK = C::CK, kThreads = C::THREADS;
+  constexpr int CH = C::CH, CK = C::CK, kThreads = C::THREADS, ROUNDS = C::ROUNDS;
   using X = Piece<T, CH>;
   using F = Piece<float, NP>;
   extern __shared__ float4 smem4[];
@@ -100,150 +113,173 @@ scan_fwd_kernel(ScanIn<T> in, Rows<T> out, float* fin, float* __restrict__ saved
   };
   if (len > 0) fetch(0, 0);
 
+  bool above = !s.softplus;
   for (int i = tid; i < CH * NP; i += kThreads) {
     const int cc = i / NP, n = i % NP;
     const bool ok = cc < nch && n < s.states;
     const int64_t o = (d0 + cc) * s.states + n;
     sA[i] = ok ? in.A[o] * kLog2e : 0.f;
+    above = above || sA[i] > 0.f;
     sH[i] = (ok && in.initial) ? in.initial[b * s.channels * s.states + o] : 0.f;
   }
   const float bias = (in.bias && live) ? in.bias[d0 + c] : 0.f;
   const float skip = (in.D && live) ? in.D[d0 + c] : 0.f;
 
   int buf = 0;
-  for (int64_t t0 = 0; t0 < len; t0 += CK, buf ^= 1) {
-    cp_async_wait();
-    __syncthreads();
-    if (t0 > 0) put(t0 - CK, buf ^ 1);
-    widen_piece<T, CK, NP, kThreads>(sB, rawB, tid);
-    widen_piece<T, CK, NP, kThreads>(sC, rawC, tid);
-
-    T* mine = raw + buf * 3 * C::XS + X::at(g * 8, c);
-    const int64_t left = len - t0 - g * 8;          // valid steps from this lane's first on
-    const int steps = left < 0 ? 0 : (left > 8 ? 8 : (int)left);
-    float dt[8], du[8];
-    f2 y[8];
-    constexpr int PART = 8 / S;                     // steps whose dt and output are this warp's
-#pragma unroll
-    for (int k = 0; k < PART; ++k) {
-      const int i = S == 1 ? k : sg * PART + k;
-      float v = to_f(mine[C::XS + i * CH]) + bias;
-      if (s.softplus) v = softplus_f(v);
-      v = i < steps ? v : 0.f;                      // past the end: a = 1, b = 0
-      if constexpr (S == 1)
-        dt[k] = v;
-      else
-        sDt[row + i] = v;
-    }
-    __syncthreads();
-    if (t0 + CK < len) fetch(t0 + CK, buf ^ 1);
-    if constexpr (S > 1)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) dt[i] = sDt[row + i];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) du[i] = dt[i] * to_f(mine[i * CH]), y[i] = 0;
-    const int64_t ts = t0 + g * 8;
-    float* so = nullptr;
-    if (saved != nullptr && ts % kSaveSteps == 0 && live && ts < s.length)
-      so = saved + ((b * s.saves + ts / kSaveSteps) * s.channels + d0 + c) * s.states;
-#pragma unroll 1
-    for (int n = sg * (NP / S); n < (sg + 1) * (NP / S); n += 4) {
-      const float4 A4 = *(const float4*)(sA + c * NP + n);
-      const f2 Ax = pack(A4.x, A4.x), Ay = pack(A4.y, A4.y), Az = pack(A4.z, A4.z),
-               Aw = pack(A4.w, A4.w);
-      const float* pb = sB + F::at(g * 8, n);
-      const float* pc = sC + F::at(g * 8, n);
-      f2 a0[8], a1[8], b0[8], b1[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float4 B4 = *(const float4*)(pb + i * NP);
-        b0[i] = pack(du[i] * B4.x, du[i] * B4.y);
-        b1[i] = pack(du[i] * B4.z, du[i] * B4.w);
-        if (i % 2 == 0) {     // exponents of two steps at a time: A's halves stay put
-          const f2 w = pack(dt[i], dt[i + 1]);
-          const float2 p = unpack(mul2(w, Ax)), q = unpack(mul2(w, Ay));
-          const float2 r = unpack(mul2(w, Az)), v = unpack(mul2(w, Aw));
-          a0[i] = pack(ex2(p.x), ex2(q.x)), a0[i + 1] = pack(ex2(p.y), ex2(q.y));
-          a1[i] = pack(ex2(r.x), ex2(v.x)), a1[i + 1] = pack(ex2(r.y), ex2(v.y));
-        }
-      }
-      f2 P0 = a0[0], P1 = a1[0], H0 = b0[0], H1 = b1[0];
-#pragma unroll
-      for (int i = 1; i < 8; ++i) {
-        H0 = fma2(a0[i], H0, b0[i]), P0 = mul2(a0[i], P0);
-        H1 = fma2(a1[i], H1, b1[i]), P1 = mul2(a1[i], P1);
-      }
-      float4* carry = (float4*)(sH + c * NP + n);
-      const float4 h4 = *carry;
-      f2 h0 = pack(h4.x, h4.y), h1 = pack(h4.z, h4.w);
-      if (g == 0) H0 = fma2(P0, h0, H0), H1 = fma2(P1, h1, H1);
-#pragma unroll
-      for (int o = 1; o < G; o <<= 1) {
-        const f2 u0 = __shfl_up_sync(0xffffffffu, H0, o, G);
-        const f2 u1 = __shfl_up_sync(0xffffffffu, H1, o, G);
-        if (g >= o) H0 = fma2(P0, u0, H0), H1 = fma2(P1, u1, H1);
-        if (2 * o < G) {
-          const f2 v0 = __shfl_up_sync(0xffffffffu, P0, o, G);
-          const f2 v1 = __shfl_up_sync(0xffffffffu, P1, o, G);
-          if (g >= o) P0 = mul2(P0, v0), P1 = mul2(P1, v1);
-        }
-      }
-      // the state in front of this lane's steps; lane 0 gets the piece's last
-      const f2 u0 = __shfl_sync(0xffffffffu, H0, (g + G - 1) % G, G);
-      const f2 u1 = __shfl_sync(0xffffffffu, H1, (g + G - 1) % G, G);
-      if (g == 0) {
-        const float2 p = unpack(u0), r = unpack(u1);
-        *carry = make_float4(p.x, p.y, r.x, r.y);
-      } else {
-        h0 = u0, h1 = u1;
-      }
-      if (so != nullptr) {
-        const float2 p = unpack(h0), r = unpack(h1);
-        if (save_vec) {
-          *(float4*)(so + n) = make_float4(p.x, p.y, r.x, r.y);
-        } else {
-          if (n + 0 < s.states) so[n + 0] = p.x;
-          if (n + 1 < s.states) so[n + 1] = p.y;
-          if (n + 2 < s.states) so[n + 2] = r.x;
-          if (n + 3 < s.states) so[n + 3] = r.y;
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float4 C4 = *(const float4*)(pc + i * NP);
-        h0 = fma2(a0[i], h0, b0[i]);
-        h1 = fma2(a1[i], h1, b1[i]);
-        y[i] = fma2(h0, pack(C4.x, C4.y), y[i]);
-        y[i] = fma2(h1, pack(C4.z, C4.w), y[i]);
-      }
-    }
-    float sum[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float2 p = unpack(y[i]);
-      sum[i] = p.x + p.y;
-    }
-    if constexpr (S > 1) {
-      float4* w = (float4*)(sY + sg * C::YS + row);
-      w[0] = make_float4(sum[0], sum[1], sum[2], sum[3]);
-      w[1] = make_float4(sum[4], sum[5], sum[6], sum[7]);
+  auto walk = [&](auto flag) {
+    constexpr bool ABOVE = decltype(flag)::value;   // some factor may be above 1
+    for (int64_t t0 = 0; t0 < len; t0 += CK, buf ^= 1) {
+      cp_async_wait();
       __syncthreads();
-    }
+      if (t0 > 0) put(t0 - CK, buf ^ 1);
+      widen_piece<T, CK, NP, kThreads>(sB, rawB, tid);
+      widen_piece<T, CK, NP, kThreads>(sC, rawC, tid);
+
+      T* mine = raw + buf * 3 * C::XS + X::at(g * 8, c);
+      const int64_t left = len - t0 - g * 8;          // valid steps from this lane's first on
+      const int steps = left < 0 ? 0 : (left > 8 ? 8 : (int)left);
+      float dt[8], du[8];
+      f2 y[8];
+      constexpr int PART = 8 / S;                     // steps whose dt and output are this warp's
 #pragma unroll
-    for (int k = 0; k < PART; ++k) {
-      const int i = S == 1 ? k : sg * PART + k;
-      float v = S == 1 ? sum[k] : 0.f;
+      for (int k = 0; k < PART; ++k) {
+        const int i = S == 1 ? k : sg * PART + k;
+        float v = to_f(mine[C::XS + i * CH]) + bias;
+        if (!ABOVE || s.softplus) v = softplus_f(v);
+        v = i < steps ? v : 0.f;                      // past the end: a = 1, b = 0
+        if constexpr (S == 1)
+          dt[k] = v;
+        else
+          sDt[row + i] = v;
+      }
+      __syncthreads();
+      if (t0 + CK < len) fetch(t0 + CK, buf ^ 1);
       if constexpr (S > 1)
 #pragma unroll
-        for (int r = 0; r < S; ++r) v += sY[r * C::YS + row + i];
-      v = fmaf(skip, to_f(mine[i * CH]), v);
-      if (in.z) {
-        const float z = to_f(mine[2 * C::XS + i * CH]);
-        v *= z * sigmoid_f(z);
+        for (int i = 0; i < 8; ++i) dt[i] = sDt[row + i];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) du[i] = dt[i] * to_f(mine[i * CH]), y[i] = 0;
+      float hw[ROUNDS];                               // half the sums of dt over 1, 2, 4.. lanes
+      if constexpr (ABOVE) {
+        hw[0] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) hw[0] = fmaf(0.5f, dt[i], hw[0]);
+#pragma unroll
+        for (int r = 1; r < ROUNDS; ++r)
+          hw[r] = hw[r - 1] + __shfl_up_sync(0xffffffffu, hw[r - 1], 1 << (r - 1), G);
       }
-      mine[i * CH] = from_f<T>(i < steps ? v : 0.f);   // in u's place
+      const int64_t ts = t0 + g * 8;
+      float* so = nullptr;
+      if (saved != nullptr && ts % kSaveSteps == 0 && live && ts < s.length)
+        so = saved + ((b * s.saves + ts / kSaveSteps) * s.channels + d0 + c) * s.states;
+#pragma unroll 1
+      for (int n = sg * (NP / S); n < (sg + 1) * (NP / S); n += 4) {
+        const float4 A4 = *(const float4*)(sA + c * NP + n);
+        const f2 Ax = pack(A4.x, A4.x), Ay = pack(A4.y, A4.y), Az = pack(A4.z, A4.z),
+                 Aw = pack(A4.w, A4.w);
+        const float* pb = sB + F::at(g * 8, n);
+        const float* pc = sC + F::at(g * 8, n);
+        f2 a0[8], a1[8], b0[8], b1[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float4 B4 = *(const float4*)(pb + i * NP);
+          b0[i] = pack(du[i] * B4.x, du[i] * B4.y);
+          b1[i] = pack(du[i] * B4.z, du[i] * B4.w);
+          if (i % 2 == 0) {     // exponents of two steps at a time: A's halves stay put
+            const f2 w = pack(dt[i], dt[i + 1]);
+            const float2 p = unpack(mul2(w, Ax)), q = unpack(mul2(w, Ay));
+            const float2 r = unpack(mul2(w, Az)), v = unpack(mul2(w, Aw));
+            a0[i] = pack(ex2(p.x), ex2(q.x)), a0[i + 1] = pack(ex2(p.y), ex2(q.y));
+            a1[i] = pack(ex2(r.x), ex2(v.x)), a1[i + 1] = pack(ex2(r.y), ex2(v.y));
+          }
+        }
+        float4* carry = (float4*)(sH + c * NP + n);
+        const float4 h4 = *carry;
+        f2 h0 = pack(h4.x, h4.y), h1 = pack(h4.z, h4.w), H0 = b0[0], H1 = b1[0];
+        f2 P0 = a0[0], P1 = a1[0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) {
+          H0 = fma2(a0[i], H0, b0[i]), H1 = fma2(a1[i], H1, b1[i]);
+          if constexpr (!ABOVE) P0 = mul2(a0[i], P0), P1 = mul2(a1[i], P1);
+        }
+        // the range's map at the state h
+        auto after = [&](f2 P, f2 h, f2 H) { return fma2(P, ABOVE ? mul2(P, h) : h, H); };
+#pragma unroll
+        for (int r = 0; r < ROUNDS; ++r) {
+          const int o = 1 << r;
+          if constexpr (ABOVE)
+            P0 = root_factor(hw[r], A4.x, A4.y), P1 = root_factor(hw[r], A4.z, A4.w);
+          if (r == 0 && g == 0) H0 = after(P0, h0, H0), H1 = after(P1, h1, H1);
+          const f2 u0 = __shfl_up_sync(0xffffffffu, H0, o, G);
+          const f2 u1 = __shfl_up_sync(0xffffffffu, H1, o, G);
+          if (g >= o) H0 = after(P0, u0, H0), H1 = after(P1, u1, H1);
+          if (!ABOVE && 2 * o < G) {
+            const f2 v0 = __shfl_up_sync(0xffffffffu, P0, o, G);
+            const f2 v1 = __shfl_up_sync(0xffffffffu, P1, o, G);
+            if (g >= o) P0 = mul2(P0, v0), P1 = mul2(P1, v1);
+          }
+        }
+        // the state in front of this lane's steps; lane 0 gets the piece's last
+        const f2 u0 = __shfl_sync(0xffffffffu, H0, (g + G - 1) % G, G);
+        const f2 u1 = __shfl_sync(0xffffffffu, H1, (g + G - 1) % G, G);
+        if (g == 0) {
+          const float2 p = unpack(u0), r = unpack(u1);
+          *carry = make_float4(p.x, p.y, r.x, r.y);
+        } else {
+          h0 = u0, h1 = u1;
+        }
+        if (so != nullptr) {
+          const float2 p = unpack(h0), r = unpack(h1);
+          if (!ABOVE && save_vec) {     // (vectors there too spill: 1 x 8191 x 2048 327 us against 316)
+            *(float4*)(so + n) = make_float4(p.x, p.y, r.x, r.y);
+          } else {
+            if (n + 0 < s.states) so[n + 0] = p.x;
+            if (n + 1 < s.states) so[n + 1] = p.y;
+            if (n + 2 < s.states) so[n + 2] = r.x;
+            if (n + 3 < s.states) so[n + 3] = r.y;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float4 C4 = *(const float4*)(pc + i * NP);
+          h0 = fma2(a0[i], h0, b0[i]);
+          h1 = fma2(a1[i], h1, b1[i]);
+          y[i] = fma2(h0, pack(C4.x, C4.y), y[i]);
+          y[i] = fma2(h1, pack(C4.z, C4.w), y[i]);
+        }
+      }
+      float sum[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float2 p = unpack(y[i]);
+        sum[i] = p.x + p.y;
+      }
+      if constexpr (S > 1) {
+        float4* w = (float4*)(sY + sg * C::YS + row);
+        w[0] = make_float4(sum[0], sum[1], sum[2], sum[3]);
+        w[1] = make_float4(sum[4], sum[5], sum[6], sum[7]);
+        __syncthreads();
+      }
+#pragma unroll
+      for (int k = 0; k < PART; ++k) {
+        const int i = S == 1 ? k : sg * PART + k;
+        float v = S == 1 ? sum[k] : 0.f;
+        if constexpr (S > 1)
+#pragma unroll
+          for (int r = 0; r < S; ++r) v += sY[r * C::YS + row + i];
+        v = fmaf(skip, to_f(mine[i * CH]), v);
+        if (in.z) {
+          const float z = to_f(mine[2 * C::XS + i * CH]);
+          v *= z * sigmoid_f(z);
+        }
+        mine[i * CH] = from_f<T>(i < steps ? v : 0.f);   // in u's place
+      }
     }
-  }
+  };
+  if (__syncthreads_or(above))
+    walk(std::true_type());
+  else
+    walk(std::false_type());
   if (len > 0) {
     __syncthreads();
     put((len - 1) / CK * CK, buf ^ 1);

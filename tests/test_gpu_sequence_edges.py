@@ -1,0 +1,81 @@
+"""Sequence operators on the GPU at the ends of their domain: growing and
+vanishing states, infinities, small results in relative terms, streams,
+arguments of other libraries and arrays that share memory.
+
+Tolerances are counted in units of 2^-24 (float32 roundings), with the count
+derived at each test.
+"""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from conftest import gpu_available
+
+from ferrum_gpu import sequence as sq
+
+pytestmark = pytest.mark.gpu
+
+F32 = torch.float32
+UNIT = 2.0 ** -24
+
+
+@pytest.fixture(autouse=True, scope="module")
+def _gpu():
+    if not gpu_available():
+        pytest.skip("no B200")
+
+
+def rnd(seed, *shape, dtype=F32, std=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * std).to("cuda").to(dtype)
+
+
+def full(value, *shape, dtype=F32):
+    return torch.full(shape, value, dtype=dtype, device="cuda")
+
+
+# Batches and channels for every split of a channel's steps and states over
+# lanes and warps: 4, 8, 16 lanes, then 2 and 4 warps of 16 (4 take more than
+# 8 states).
+SPLITS = [(3, 4100), (6, 1001), (3, 1002), (1, 1001), (1, 40)]
+
+
+# ---------------------------------------------------------------- growing states
+
+def grown(u, dt, A, B, C, h):
+    """The recurrence in 64 bits, for constant dt and one group."""
+    u, A, B, C, h = (t.double() for t in (u, A, B, C, h))
+    a, ys = torch.exp(dt * A), [torch.zeros_like(u[:, 0])]
+    for t in range(u.shape[1]):
+        h = a * h + (dt * u[:, t])[..., None] * B[:, t, None]
+        ys.append((h * C[:, t, None]).sum(-1))
+    return torch.stack(ys[1:] or ys, 1), h
+
+
+@pytest.mark.parametrize("n,rate", [(112, 1.45), (56, 2.9), (28, 5.8)])
+@pytest.mark.parametrize("N", [16, 8])
+@pytest.mark.parametrize("b,d", SPLITS)
+def test_scan_of_growing_states(b, d, N, n, rate):
+    """Factors above 1, whose product over some lanes' steps (64, 32, 16 of
+    them) passes the largest float32 while the state in front is zero or small:
+    e^162 in all, from 1e-37 to 3e33."""
+    delta, A = full(1.0, b, n, d), full(rate, d, N)
+    B, C = rnd(1, b, n, N).abs(), rnd(2, b, n, N).abs()
+    late = torch.zeros(b, n, d, device="cuda")
+    tail = int(30 / rate)                            # e^30 behind the first input
+    late[:, -tail:] = rnd(3, b, tail, d).abs() + 0.1
+    for u, h0 in ((late, full(0.0, b, d, N)), (late * 0, full(1e-37, b, d, N))):
+        yr, hr = grown(u, 1.0, A, B, C, h0)
+        r = sq.selective_scan(u, delta, A, B, C, initial_state=h0, save_states=True)
+        # Every term is positive, so nothing cancels. Units: 8 for a step's
+        # exponential, product and sum; one for each nat of the exponents
+        # (162) in A log2 e, in a step's product, and twice in a sum of steps.
+        tol = (8 * n + 4 * 162 + N) * UNIT
+        assert bool(torch.isfinite(r.final_state).all())
+        assert ((r.final_state - hr).abs() <= tol * hr).all()
+        assert ((r.out - yr).abs() <= tol * yr).all()
+        at = (n - 1) // 16                           # the last state saved
+        mid = grown(u[:, :16 * at], 1.0, A, B[:, :16 * at], C[:, :16 * at], h0)[1]
+        assert ((r.states[:, at] - mid).abs() <= tol * mid).all()
