@@ -1,6 +1,7 @@
 // Argument views and helpers shared by the selective scan's kernels.
 #pragma once
 
+#include <cfloat>
 #include <type_traits>
 
 #include "seq_common.cuh"
@@ -71,6 +72,15 @@ __device__ __forceinline__ f2 mul2(f2 a, f2 b) {
   f2 r;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
+}
+
+// A state's rate A as the kernels take it, for factors 2^(dt A log2 e). An
+// infinite one becomes the largest float, so that steps of dt = 0, which fill
+// up a sequence's last piece, leave the state as it is (0 * inf would be NaN);
+// any other step still takes the factor to 0.
+__device__ __forceinline__ float scaled_rate(float A) {
+  const float r = A * kLog2e;
+  return isinf(r) ? copysignf(FLT_MAX, r) : r;
 }
 
 // The smaller value, or NaN where either is one.

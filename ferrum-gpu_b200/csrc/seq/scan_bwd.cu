@@ -166,7 +166,7 @@ scan_bwd_kernel(ScanIn<T> in, ScanGrad<T> gr, ScanSizes s, int64_t group_blocks,
     for (int e = 0; e < 2; ++e) {
       const bool ok = e < nc && n0 + k < s.states;
       const int64_t o = (d0 + c + e) * s.states + n0 + k;
-      a[e] = ok ? in.A[o] * kLog2e : 0.f;
+      a[e] = ok ? scaled_rate(in.A[o]) : 0.f;
       g[e] = ok && gr.dfin ? gr.dfin[b * s.channels * s.states + o] : 0.f;
     }
     A[k] = pack(a[0], a[1]), r[k] = pack(g[0], g[1]), dA[k] = 0;

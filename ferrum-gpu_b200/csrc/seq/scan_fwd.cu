@@ -118,7 +118,7 @@ scan_fwd_kernel(ScanIn<T> in, Rows<T> out, float* fin, float* __restrict__ saved
     const int cc = i / NP, n = i % NP;
     const bool ok = cc < nch && n < s.states;
     const int64_t o = (d0 + cc) * s.states + n;
-    sA[i] = ok ? in.A[o] * kLog2e : 0.f;
+    sA[i] = ok ? scaled_rate(in.A[o]) : 0.f;
     above = above || sA[i] > 0.f;
     sH[i] = (ok && in.initial) ? in.initial[b * s.channels * s.states + o] : 0.f;
   }
@@ -357,7 +357,7 @@ scan_step_kernel(ScanIn<T> in, Rows<T> out, float* fin, ScanSizes s, bool vec, b
   }
   const float skip = in.D ? in.D[d] : 0.f;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) a[e] *= kLog2e;
+  for (int e = 0; e < 4; ++e) a[e] = scaled_rate(a[e]);
   if (s.softplus) dt = softplus_f(dt);
   const float dx = dt * x;
   float* pf = fin + so;

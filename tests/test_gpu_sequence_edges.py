@@ -79,3 +79,25 @@ def test_scan_of_growing_states(b, d, N, n, rate):
         at = (n - 1) // 16                           # the last state saved
         mid = grown(u[:, :16 * at], 1.0, A, B[:, :16 * at], C[:, :16 * at], h0)[1]
         assert ((r.states[:, at] - mid).abs() <= tol * mid).all()
+
+
+@pytest.mark.parametrize("n", [5, 64, 150])
+@pytest.mark.parametrize("b,d", SPLITS)
+def test_scan_states_that_forget_at_once(b, d, n):
+    """A = -inf: exp(dt A) = 0 at every step, whatever follows the sequence's
+    end inside the last piece."""
+    N = 16
+    A = -rnd(1, d, N).abs()
+    A[:, ::2] = -float("inf")
+    u, delta = rnd(2, b, n, d), rnd(3, b, n, d).abs() + 0.1
+    B, C = rnd(4, b, n, N), rnd(5, b, n, N)
+    h0 = rnd(6, b, d, N)
+    r = sq.selective_scan(u, delta, A, B, C, initial_state=h0, save_states=True)
+    g = sq.selective_scan_backward(u, u, delta, A, B, C, r.states)
+    for t in (r.out, r.final_state, g.du, g.ddelta, g.dA, g.dB, g.dC, g.dinitial_state):
+        assert bool(torch.isfinite(t).all())
+    last = delta[:, -1].double() * u[:, -1].double()
+    want = last[..., None] * B[:, -1, None, ::2].double()
+    # two products
+    assert not g.dinitial_state[..., ::2].any()
+    assert ((r.final_state[..., ::2] - want).abs() <= 4 * UNIT * want.abs()).all()
