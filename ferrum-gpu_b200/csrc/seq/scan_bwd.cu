@@ -310,19 +310,21 @@ scan_bwd_kernel(ScanIn<T> in, ScanGrad<T> gr, ScanSizes s, int64_t group_blocks,
           gB = add2(gB, *(const f2*)(sG + x * C::SLAB + po));
           dd = add2(dd, *(const f2*)(sT + x * C::SLAB + po));
         }
-        const float2 vy = unpack(y), vg = unpack(gB), vd = unpack(dd);
+        float2 vy = unpack(y);
+        const float2 vg = unpack(gB), vd = unpack(dd);
         const float2 x = *(const float2*)(sX + o), dt = *(const float2*)(sDt + o);
         const float2 dy = *(const float2*)(sDy + o), sl = *(const float2*)(sSl + o);
         const float2 zg = *(const float2*)(sZg + o);
-        const float2 dd2 = make_float2(fmaf(vg.x, x.x, vd.x * kLn2) * sl.x,
-                                       fmaf(vg.y, x.y, vd.y * kLn2) * sl.y);
+        float2 dd2 = make_float2(fmaf(vg.x, x.x, vd.x * kLn2) * sl.x,
+                                 fmaf(vg.y, x.y, vd.y * kLn2) * sl.y);
+        float2 du2 = make_float2(fmaf(vg.x, dt.x, skip.x * dy.x), fmaf(vg.y, dt.y, skip.y * dy.y));
+        if (t >= rows)      // behind the sequence, whatever the states and their gradients hold
+          dd2 = du2 = vy = make_float2(0.f, 0.f);
         dD.x = fmaf(dy.x, x.x, dD.x), dD.y = fmaf(dy.y, x.y, dD.y);
         dbias.x += dd2.x, dbias.y += dd2.y;
         const int64_t tt = t0 + t;
         if (tt < s.length) {
-          store_pair(gr.du.at(b, tt) + d0 + c,
-                     make_float2(fmaf(vg.x, dt.x, skip.x * dy.x), fmaf(vg.y, dt.y, skip.y * dy.y)),
-                     nc, out_vec);
+          store_pair(gr.du.at(b, tt) + d0 + c, du2, nc, out_vec);
           store_pair(gr.ddelta.at(b, tt) + d0 + c, dd2, nc, out_vec);
           if (in.z)
             store_pair(gr.dz.at(b, tt) + d0 + c,

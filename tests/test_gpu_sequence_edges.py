@@ -101,3 +101,19 @@ def test_scan_states_that_forget_at_once(b, d, n):
     # two products
     assert not g.dinitial_state[..., ::2].any()
     assert ((r.final_state[..., ::2] - want).abs() <= 4 * UNIT * want.abs()).all()
+
+
+def test_scan_gradients_are_zero_behind_a_sequence():
+    """Whatever the states and the final state's gradient hold."""
+    b, n, d, N = 3, 40, 33, 16
+    lengths = torch.tensor([5, 0, 21], dtype=torch.int32, device="cuda")
+    u, delta, z, dout = (rnd(i, b, n, d) for i in range(4))
+    B, C, A = rnd(5, b, n, N), rnd(6, b, n, N), -rnd(7, d, N).abs()
+    dfin = h0 = full(float("inf"), b, d, N)
+    r = sq.selective_scan(u, delta, A, B, C, z=z, delta_softplus=True, lengths=lengths,
+                          initial_state=h0, save_states=True)
+    g = sq.selective_scan_backward(dout, u, delta, A, B, C, r.states, z=z, delta_softplus=True,
+                                   lengths=lengths, dfinal_state=dfin)
+    for i, ln in enumerate((5, 0, 21)):
+        for t in (r.out, g.du, g.ddelta, g.dz, g.dB, g.dC):
+            assert not t[i, ln:].any()
