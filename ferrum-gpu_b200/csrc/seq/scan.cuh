@@ -83,6 +83,18 @@ __device__ __forceinline__ float scaled_rate(float A) {
   return isinf(r) ? copysignf(FLT_MAX, r) : r;
 }
 
+// Added to the exponent of a step's factor, in the product's multiply-add. The
+// special-function unit's 2^x errs to one side: measured over -1 < x < -2^-8 by
+// -0.3 to -0.45 units of 2^-24 on average, which adds up where a state keeps
+// its value over many steps. With half a unit more the average is within 0.1 of zero there
+// (0.26 closer to 1), and 2^0 is still 1. Over 400 steps with dt |A| from 0.001
+// to 0.16 the state is 1.6e-7 from its 64-bit value and dA 5e-7 (1.5e-6 and
+// 3.7e-6 without; a plain float32 loop 3.2e-7 and 6.6e-7), in the same time.
+constexpr float kExponentShift = 0x1p-25f;
+__device__ __forceinline__ f2 exponents(f2 dt, f2 A) {
+  return fma2(dt, A, pack(kExponentShift, kExponentShift));
+}
+
 // The smaller value, or NaN where either is one.
 __device__ __forceinline__ float min_nan(float x, float y) {
   float r;

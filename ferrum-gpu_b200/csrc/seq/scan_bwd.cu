@@ -230,7 +230,7 @@ scan_bwd_kernel(ScanIn<T> in, ScanGrad<T> gr, ScanSizes s, int64_t group_blocks,
         const f2 dt = *(const f2*)(sDt + t * CHN + c), du = *(const f2*)(sDu + t * CHN + c);
 #pragma unroll
         for (int k = 0; k < NS; ++k) {
-          const float2 e = unpack(mul2(dt, A[k]));
+          const float2 e = unpack(exponents(dt, A[k]));
           h[k] = fma2(pack(ex2(e.x), ex2(e.y)), h[k],
                       mul2(du, *(const f2*)(sB + (t * NP + n0 + k) * 2)));
         }
@@ -253,7 +253,7 @@ scan_bwd_kernel(ScanIn<T> in, ScanGrad<T> gr, ScanSizes s, int64_t group_blocks,
         f2 y = 0;
 #pragma unroll
         for (int k = 0; k < NS; ++k) {
-          const float2 e = unpack(mul2(dt, A[k]));
+          const float2 e = unpack(exponents(dt, A[k]));
           a[i][k] = pack(ex2(e.x), ex2(e.y));
           h[i + 1][k] = fma2(a[i][k], h[i][k], mul2(du, *(const f2*)(sB + (t * NP + n0 + k) * 2)));
           y = fma2(h[i + 1][k], *(const f2*)(sC + (t * NP + n0 + k) * 2), y);

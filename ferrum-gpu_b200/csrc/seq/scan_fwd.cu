@@ -58,7 +58,7 @@ struct FwdCfg {
 // Clamped below the exponent range's end: a factor that large overflows any
 // state but 0. A NaN stays.
 __device__ __forceinline__ f2 root_factor(float w, float Ax, float Ay) {
-  const float2 e = unpack(mul2(pack(w, w), pack(Ax, Ay)));
+  const float2 e = unpack(exponents(pack(w, w), pack(Ax, Ay)));
   return pack(ex2(min_nan(e.x, 127.f)), ex2(min_nan(e.y, 127.f)));
 }
 
@@ -187,8 +187,8 @@ scan_fwd_kernel(ScanIn<T> in, Rows<T> out, float* fin, float* __restrict__ saved
           b1[i] = pack(du[i] * B4.z, du[i] * B4.w);
           if (i % 2 == 0) {     // exponents of two steps at a time: A's halves stay put
             const f2 w = pack(dt[i], dt[i + 1]);
-            const float2 p = unpack(mul2(w, Ax)), q = unpack(mul2(w, Ay));
-            const float2 r = unpack(mul2(w, Az)), v = unpack(mul2(w, Aw));
+            const float2 p = unpack(exponents(w, Ax)), q = unpack(exponents(w, Ay));
+            const float2 r = unpack(exponents(w, Az)), v = unpack(exponents(w, Aw));
             a0[i] = pack(ex2(p.x), ex2(q.x)), a0[i + 1] = pack(ex2(p.y), ex2(q.y));
             a1[i] = pack(ex2(r.x), ex2(v.x)), a1[i + 1] = pack(ex2(r.y), ex2(v.y));
           }
@@ -370,7 +370,7 @@ scan_step_kernel(ScanIn<T> in, Rows<T> out, float* fin, ScanSizes s, bool vec, b
       float y = 0.f;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        h[k][e] = fmaf(ex2(dtk * a[e]), h[k][e], dxk * Bv[k][e]);
+        h[k][e] = fmaf(ex2(fmaf(dtk, a[e], kExponentShift)), h[k][e], dxk * Bv[k][e]);
         y = fmaf(h[k][e], Cv[k][e], y);
       }
 #pragma unroll

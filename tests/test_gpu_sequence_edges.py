@@ -117,3 +117,44 @@ def test_scan_gradients_are_zero_behind_a_sequence():
     for i, ln in enumerate((5, 0, 21)):
         for t in (r.out, g.du, g.ddelta, g.dz, g.dB, g.dC):
             assert not t[i, ln:].any()
+
+
+# ---------------------------------------------------------------- slow states
+
+@pytest.mark.parametrize("b,d", SPLITS)
+def test_scan_of_slow_states_errs_like_a_float32_loop(b, d):
+    """Factors from 0.85 to 0.999 over 400 steps, where a one-sided error of the
+    exponential would add up. The kernel makes the roundings of a plain float32
+    loop and its exponentials' (2 units against 1): at most twice its distance
+    from 64 bits in the root-mean-square sense."""
+    n, N = 400, 16
+    u, B, C, dout = rnd(1, b, n, d), rnd(2, b, n, N), rnd(3, b, n, N), rnd(4, b, n, d)
+    delta = (rnd(5, b, n, d).abs() * 0.004 + 0.001).clamp(max=0.01)
+    A = -torch.arange(1.0, N + 1, device="cuda").expand(d, N).contiguous()
+
+    def loop(dtype):
+        v = [t.to(dtype).requires_grad_(True) for t in (u, delta, A, B, C)]
+        U, D, a, b_, c = v
+        h, ys = torch.zeros(b, d, N, dtype=dtype, device="cuda"), []
+        for t in range(n):
+            h = torch.exp(D[:, t, :, None] * a) * h + (D[:, t] * U[:, t])[..., None] * b_[:, t, None]
+            ys.append((h * c[:, t, None]).sum(-1))
+        y = torch.stack(ys, 1)
+        return [y.detach(), h.detach(), *torch.autograd.grad((y * dout.to(dtype)).sum(), v)]
+
+    exact, plain = loop(torch.float64), loop(torch.float32)
+    r = sq.selective_scan(u, delta, A, B, C, save_states=True)
+    g = sq.selective_scan_backward(dout, u, delta, A, B, C, r.states)
+    got = [r.out, r.final_state, g.du, g.ddelta, g.dA, g.dB, g.dC]
+    off = lambda x, ref: ((x - ref).norm() / ref.norm()).item()
+    for name, k, p, e in zip(("out", "final_state", "du", "ddelta", "dA", "dB", "dC"), got, plain, exact):
+        assert off(k, e) <= 2 * off(p, e), (name, off(k, e), off(p, e))
+    state = rnd(6, b, d, N)                          # one step at a time
+    ref = [state.to(t).clone() for t in (torch.float64, F32)]
+    for t in range(n):
+        for h in ref:
+            x = h.dtype
+            h.mul_(torch.exp(delta[:, t, :, None].to(x) * A.to(x)))
+            h.add_((delta[:, t].to(x) * u[:, t].to(x))[..., None] * B[:, t, None].to(x))
+        sq.selective_scan_step(u[:, t], delta[:, t], A, B[:, t], C[:, t], state)
+    assert off(state, ref[0]) <= 2 * off(ref[1], ref[0])
