@@ -32,13 +32,30 @@ __device__ __forceinline__ int64_t scan_length(const int32_t* lengths, int64_t b
   return n < 0 ? 0 : (n > length ? length : n);
 }
 
+// The smaller value, or NaN where either is one.
+__device__ __forceinline__ float min_nan(float x, float y) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
+  return r;
+}
+
+// e^-|x|, flushed to 0 below 2^-126 (|x| above 87.3). 2^t takes t with a
+// rounding error of up to |t| 2^-24, 64 units of the result at |x| = 87; what
+// the product |x| log2 e loses, d, is put back as e (1 + d ln 2).
+__device__ __forceinline__ float exp_minus(float x) {
+  const float ax = -min_nan(fabsf(x), 200.f), t = ax * kLog2e;   // (finite: inf - inf is NaN)
+  const float d = fmaf(ax, kLog2e, -t);
+  const float e = ex2(t);
+  return fmaf(e, fmaf(ax, 1.3349758e-8f, d * 0.69314718f), e);   // 1.33e-8 = ln 2 (log2 e - kLog2e)
+}
+
 // log(1 + e^x) = max(x, 0) + log(1 + e), e = e^-|x| in (0, 1]. log(1 + e) / e
 // is a polynomial in e (least squares at Chebyshev nodes of [0, 1], relative
-// error 3.1e-8), so small results keep their relative accuracy; it costs one
-// exponential and ten products and sums, where log1pf takes a few times that
-// and the scan spends it once per value.
-__device__ __forceinline__ float softplus_f(float x) {
-  const float e = ex2(-fabsf(x) * kLog2e);
+// error 6.1e-8), so small results keep their relative accuracy (9 units of
+// 2^-24 in all, down to x = -87); it costs one exponential and a dozen products
+// and sums, where log1pf takes a few times that and the scan spends it once
+// per value.
+__device__ __forceinline__ float softplus_of(float x, float e) {
   float p = 0.00525345793f;
   p = fmaf(p, e, -0.0295885075f);
   p = fmaf(p, e, 0.0783616677f);
@@ -49,6 +66,13 @@ __device__ __forceinline__ float softplus_f(float x) {
   p = fmaf(p, e, -0.499995023f);
   p = fmaf(p, e, 1.f);
   return fmaf(p, e, fmaxf(x, 0.f));
+}
+__device__ __forceinline__ float softplus_f(float x) { return softplus_of(x, exp_minus(x)); }
+// The same, and its slope 1 / (1 + e^-x).
+__device__ __forceinline__ float softplus_f(float x, float& slope) {
+  const float e = exp_minus(x), r = rcp(1.f + e);
+  slope = x < 0.f ? e * r : r;
+  return softplus_of(x, e);
 }
 
 // Pairs of floats for the two-wide FP32 instructions.
@@ -93,13 +117,6 @@ __device__ __forceinline__ float scaled_rate(float A) {
 constexpr float kExponentShift = 0x1p-25f;
 __device__ __forceinline__ f2 exponents(f2 dt, f2 A) {
   return fma2(dt, A, pack(kExponentShift, kExponentShift));
-}
-
-// The smaller value, or NaN where either is one.
-__device__ __forceinline__ float min_nan(float x, float y) {
-  float r;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(y));
-  return r;
 }
 
 // A piece of a (steps, columns) array in shared memory, in its own type: row

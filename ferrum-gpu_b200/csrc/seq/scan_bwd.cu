@@ -193,8 +193,10 @@ scan_bwd_kernel(ScanIn<T> in, ScanGrad<T> gr, ScanSizes s, int64_t group_blocks,
         const float v = to_f(raw[C::XS + o]) + (e ? bias.y : bias.x);
         vx[e] = to_f(raw[o]);
         vdy[e] = to_f(raw[3 * C::XS + o]);
-        vdt[e] = ok ? (s.softplus ? softplus_f(v) : v) : 0.f;
-        vsl[e] = ok ? (s.softplus ? sigmoid_f(v) : 1.f) : 0.f;
+        float dt = v, slope = 1.f;
+        if (s.softplus) dt = softplus_f(v, slope);
+        vdt[e] = ok ? dt : 0.f;
+        vsl[e] = ok ? slope : 0.f;
         vzg[e] = 0.f;
         if (in.z) {
           const float z = to_f(raw[2 * C::XS + o]), sg = sigmoid_f(z);

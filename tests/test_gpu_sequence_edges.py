@@ -119,6 +119,39 @@ def test_scan_gradients_are_zero_behind_a_sequence():
             assert not t[i, ln:].any()
 
 
+# ---------------------------------------------------------------- small results
+
+def test_softplus_keeps_its_relative_accuracy():
+    """out = dt = softplus(delta) for one step of u = B = C = 1 from a zero
+    state. Units: the exponential 4 (2 in its last place), its argument's
+    correction 1, the polynomial 3, its products and the sum 3; 12 in all. In
+    the gradient ddelta = sigmoid(delta): the exponential 5, the quotient 2 and
+    products 3."""
+    x = torch.linspace(-87, 30, 20001, device="cuda")
+    d = x.numel()
+    one, A = full(1.0, 1, 1, d), full(0.0, d, 1)
+    bc = full(1.0, 1, 1, 1)
+    want = torch.nn.functional.softplus(x.double(), threshold=100.0)
+    tol = 12 * UNIT * want
+    r = sq.selective_scan(one, x[None, None], A, bc, bc, delta_softplus=True, save_states=True)
+    assert ((r.out[0, 0] - want).abs() <= tol).all()
+    assert ((r.final_state[0, :, 0] - want).abs() <= tol).all()
+    state = full(0.0, 1, d, 1)
+    out = sq.selective_scan_step(one[0], x[None], A, bc[0], bc[0], state, delta_softplus=True)
+    assert ((out[0] - want).abs() <= tol).all()
+    g = sq.selective_scan_backward(one, one, x[None, None], A, bc, bc, r.states,
+                                   delta_softplus=True)
+    assert ((g.du[0, 0] - want).abs() <= tol).all()
+    slope = torch.sigmoid(x.double())
+    assert ((g.ddelta[0, 0] - slope).abs() <= 10 * UNIT * slope).all()
+    ends = torch.tensor([float("inf"), -float("inf"), float("nan"), -200.0], device="cuda")
+    bc = full(1.0, 1, 1, 8)
+    r = sq.selective_scan(one[..., :4], ends[None, None], full(-1.0, 4, 8), bc, bc,
+                          delta_softplus=True)
+    got = r.out[0, 0].tolist()
+    assert got[0] == float("inf") and got[1] == 0 and got[2] != got[2] and got[3] == 0
+
+
 # ---------------------------------------------------------------- slow states
 
 @pytest.mark.parametrize("b,d", SPLITS)
