@@ -302,7 +302,8 @@ ferrum_status check_conv(const ferrum_device* dev, const ferrum_conv1d_args* a, 
   if (ferrum_status s = check_args(dev, a, what)) return s;
   if (a->taps < 1 || a->taps > FERRUM_CONV1D_MAX_TAPS)
     return invalid(what, "taps must be in [1, 8], got " + std::to_string(a->taps));
-  if (bounded_product({a->batch, a->length + (size_t)a->taps, a->channels}) < 0)
+  if (a->length > (size_t)kMaxElems ||      // (and length + taps would wrap around)
+      bounded_product({a->batch, a->length + (size_t)a->taps, a->channels}) < 0)
     return invalid(what, "batch * length * channels is too large");
   const size_t e = dtype_size(a->dtype);
   const bool none = a->batch == 0 || a->channels == 0, empty = none || a->length == 0;

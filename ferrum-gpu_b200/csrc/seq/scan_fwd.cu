@@ -514,7 +514,8 @@ ferrum_status check_scan(const ferrum_device* dev, const ferrum_scan_args* a, co
   if (a->groups < 1 || a->channels % a->groups != 0)
     return invalid(what, "groups must divide channels (" + std::to_string(a->groups) + ", " +
                              std::to_string(a->channels) + ")");
-  if (bounded_product({a->batch, a->length + 1, a->channels, a->states}) < 0)
+  if (a->length > (size_t)kMaxElems ||      // (and length + 1 would wrap around)
+      bounded_product({a->batch, a->length + 1, a->channels, a->states}) < 0)
     return invalid(what, "batch * length * channels * states is too large");
   for (const ferrum_rows* r : {&a->u, &a->delta, &a->z, &a->out, &a->B, &a->C, &a->dout, &a->du,
                                &a->ddelta, &a->dz})

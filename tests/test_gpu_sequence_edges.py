@@ -8,12 +8,14 @@ derived at each test.
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
 from conftest import gpu_available
 
-from ferrum_gpu import sequence as sq
+from ferrum_gpu import capi, sequence as sq
 
 pytestmark = pytest.mark.gpu
 
@@ -191,3 +193,21 @@ def test_scan_of_slow_states_errs_like_a_float32_loop(b, d):
             h.add_((delta[:, t].to(x) * u[:, t].to(x))[..., None] * B[:, t, None].to(x))
         sq.selective_scan_step(u[:, t], delta[:, t], A, B[:, t], C[:, t], state)
     assert off(state, ref[0]) <= 2 * off(ref[1], ref[0])
+
+
+# ---------------------------------------------------------------- sizes
+
+def test_lengths_that_wrap_around_are_refused():
+    """Checked before any size is computed from them; nothing is launched."""
+    h = capi.DeviceHandle(0)
+    buf = torch.zeros(64, device="cuda").data_ptr()
+    rows = capi.Rows(buf, 0, 0)
+    conv = capi.ConvArgs(struct_size=ctypes.sizeof(capi.ConvArgs), taps=4, batch=1, channels=1,
+                         length=2 ** 64 - 2, weight=buf, x=rows, y=rows)
+    scan = capi.ScanArgs(struct_size=ctypes.sizeof(capi.ScanArgs), batch=1, channels=1, states=1,
+                         groups=1, length=2 ** 64 - 1, u=rows, delta=rows, out=rows, B=rows, C=rows,
+                         A=buf)
+    for call, args in ((capi.lib().ferrum_causal_conv1d, conv), (capi.lib().ferrum_selective_scan, scan)):
+        assert call(h.ptr, args, None) == capi.FERRUM_ERR_INVALID_ARG
+        assert "too large" in capi.last_error()
+    h.close()
