@@ -154,9 +154,10 @@ class Call {
   Tensor zeros(at::IntArrayRef shape, at::ScalarType t) const {
     return at::zeros(shape, ref_.options().dtype(t));
   }
+  // `used`: every tensor of the caller's that the call reads or writes
   template <class Args>
   void run(ferrum_status (*entry)(ferrum_device*, const Args*, void*), Args& a,
-           std::initializer_list<const Opt*> inputs) const {
+           std::initializer_list<const Opt*> used) const {
     a.struct_size = sizeof(Args);
     ferrum_status s;
     {
@@ -165,7 +166,7 @@ class Call {
     }
     if (s != FERRUM_OK) py::module_::import("ferrum_gpu.capi").attr("check")(s);
     if (other_)
-      for (const Opt* x : inputs)   // the caching allocator must not reuse them early
+      for (const Opt* x : used)   // the caching allocator must not reuse them early
         if (given(*x)) (*x)->record_stream(*other_);
   }
 
@@ -223,7 +224,7 @@ py::object causal_conv1d(const Opt& xo, const Opt& weight, const Opt& bias,
   if (want_state) fin = c.empty({x.size(0), a.taps - 1, x.size(2)}, x.scalar_type());
   a.y = rows(y);
   if (want_state) a.final_state = fin.data_ptr();
-  c.run(ferrum_causal_conv1d, a, {&xo, &weight, &bias, &state, &lengths});
+  c.run(ferrum_causal_conv1d, a, {&xo, &weight, &bias, &state, &lengths, &out});
   if (want_state) return py::make_tuple(y, fin);
   return py::cast(y);
 }
@@ -261,7 +262,7 @@ Tensor causal_conv1d_step(const Opt& xo, const Opt& state, const Opt& weight, co
   Call c(x, device, stream);
   Tensor y = given(out) ? writable(like(out, x, x.sizes(), "out"), {&xo, &state}) : c.empty_like(x);
   a.y = rows(y);
-  c.run(ferrum_causal_conv1d_step, a, {&xo, &state, &next, &weight, &bias});
+  c.run(ferrum_causal_conv1d_step, a, {&xo, &state, &next, &weight, &bias, &out});
   return y;
 }
 
@@ -327,7 +328,7 @@ py::tuple selective_scan(const Opt& uo, const Opt& delta, const Opt& A, const Op
   if (save) saved = c.empty({b, saves(a), d, ns}, at::kFloat);
   a.out = rows(y), a.final_state = (float*)fin.data_ptr();
   if (save) a.saved_states = (float*)saved.data_ptr();
-  c.run(ferrum_selective_scan, a, {&uo, &delta, &A, &B, &C, &D, &z, &bias, &state, &lengths});
+  c.run(ferrum_selective_scan, a, {&uo, &delta, &A, &B, &C, &D, &z, &bias, &state, &lengths, &out});
   return py::make_tuple(y, fin, to_py(saved));
 }
 
@@ -375,7 +376,8 @@ Tensor selective_scan_step(const Opt& uo, const Opt& delta, const Opt& A, const 
                  ? writable(like(out, u, u.sizes(), "out"), {&uo, &delta, &z, &B, &C})
                  : c.empty_like(u);
   a.out = rows(y);
-  c.run(ferrum_selective_scan_step, a, {&uo, &delta, &A, &B, &C, &state, &next, &D, &z, &bias});
+  c.run(ferrum_selective_scan_step, a,
+        {&uo, &delta, &A, &B, &C, &state, &next, &D, &z, &bias, &out});
   return y;
 }
 
@@ -509,7 +511,7 @@ Tensor norm_after(const Opt& xo, const Opt& weight, const Opt& bias, const Opt& 
   Tensor y = given(out) ? writable(like(out, x, x.sizes(), "out"), {&xo, &gate, &residual})
                         : c.empty_like(x);
   a.y = y.data_ptr(), a.y_stride = matrix(y, "out").stride;
-  c.run(ferrum_norm_after, a, {&xo, &gate, &residual, &weight, &bias, &scale});
+  c.run(ferrum_norm_after, a, {&xo, &gate, &residual, &weight, &bias, &scale, &out});
   return y;
 }
 
@@ -561,7 +563,7 @@ Tensor long_conv(const Opt& xo, const Opt& kernel, const Opt& skip, const Opt& o
   Call c(x, device, stream);
   Tensor y = given(out) ? writable(like(out, x, x.sizes(), "out", false), {&xo}) : c.empty_like(x);
   a.x = rows(x), a.x_step = x.stride(2), a.y = rows(y), a.y_step = y.stride(2);
-  c.run(ferrum_long_conv, a, {&xo, &kernel, &skip});
+  c.run(ferrum_long_conv, a, {&xo, &kernel, &skip, &out});
   return y;
 }
 
@@ -596,7 +598,7 @@ Tensor long_conv_step(const Opt& xo, const Opt& history, const Opt& positions, c
   Call c(x, device, stream);
   Tensor y = given(out) ? writable(like(out, x, x.sizes(), "out"), {&xo, &history}) : c.empty_like(x);
   a.x = rows(x), a.y = rows(y), a.history = rows(h);
-  c.run(ferrum_long_conv_step, a, {&xo, &history, &positions, &kernel, &skip});
+  c.run(ferrum_long_conv_step, a, {&xo, &history, &positions, &kernel, &skip, &out});
   return y;
 }
 

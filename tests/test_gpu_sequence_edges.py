@@ -211,3 +211,51 @@ def test_lengths_that_wrap_around_are_refused():
         assert call(h.ptr, args, None) == capi.FERRUM_ERR_INVALID_ARG
         assert "too large" in capi.last_error()
     h.close()
+
+
+# ---------------------------------------------------------------- streams and memory
+
+def calls(seed=70):
+    """Every operator that takes `out`: name, shape of out, call(out, stream)."""
+    b, n, d, N = 4, 256, 512, 8
+    x, z, w = rnd(seed, b, n, d), rnd(seed + 1, b, n, d), rnd(seed + 2, d, 4)
+    A, bc = -rnd(seed + 3, d, N).abs(), rnd(seed + 4, b, n, N)
+    cst, sst, nw = rnd(seed + 5, b, 3, d), rnd(seed + 6, b, d, N), rnd(seed + 7, d)
+    xl, k = rnd(seed + 8, b, d, n), rnd(seed + 9, d, n, std=0.05)
+    pos = torch.full((b,), n - 1, dtype=torch.int32, device="cuda")
+    return [
+        ("conv", (b, n, d), lambda o, s: sq.causal_conv1d(x, w, out=o, stream=s)),
+        ("conv step", (b, d), lambda o, s: sq.causal_conv1d_step(x[:, 0], cst, w, out=o, stream=s)),
+        ("scan", (b, n, d), lambda o, s: sq.selective_scan(x, z, A, bc, bc, delta_softplus=True,
+                                                           out=o, stream=s).out),
+        ("scan step", (b, d), lambda o, s: sq.selective_scan_step(
+            x[:, 0], z[:, 0], A, bc[:, 0], bc[:, 0], sst, delta_softplus=True, out=o, stream=s)),
+        ("norm after", (b, n, d), lambda o, s: sq.norm_after(x, nw, gate=z, out=o, stream=s)),
+        ("long conv", (b, d, n), lambda o, s: sq.long_conv(xl, k, out=o, stream=s)),
+        ("long step", (b, d), lambda o, s: sq.long_conv_step(xl[:, :, 0].contiguous(), xl, pos, k,
+                                                             out=o, stream=s)),
+    ]
+
+
+@pytest.mark.parametrize("i", range(7))
+def test_a_given_output_outlives_its_call_on_another_stream(i):
+    """The caller drops `out` while the call still waits: its memory must not go
+    to the next allocation of the caller's stream."""
+    name, shape, call = calls()[i]
+    s = torch.cuda.Stream()
+    call(torch.empty(shape, device="cuda"), s)      # loads the kernels, which may wait
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    torch.zeros(shape, device="cuda")
+    out = torch.empty(shape, device="cuda")
+    at = out.data_ptr()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        torch.cuda._sleep(200_000_000)      # some 0.1 s in which the call waits
+    call(out, s)
+    del out
+    assert not s.query(), "the call ran too early to tell"
+    fresh = torch.zeros(shape, device="cuda")       # the same request as out's
+    assert fresh.data_ptr() != at, name
+    s.synchronize()
+    assert not bool(fresh.any()), name
