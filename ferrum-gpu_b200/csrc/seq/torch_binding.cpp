@@ -11,10 +11,13 @@
 #include <pybind11/stl.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
 #include <initializer_list>
 #include <optional>
 #include <sstream>
 #include <string>
+#include <utility>
+#include <vector>
 
 #include "../../../include/ferrum_seq.h"
 
@@ -107,22 +110,94 @@ P* param(const Opt& x, const Tensor& ref, Shape shape, const char* what,
   return (P*)t.data_ptr();
 }
 
-// An output the caller gave: no two of its elements share memory, and it
-// starts at none of the inputs.
-const Tensor& writable(const Tensor& out, std::initializer_list<const Opt*> inputs) {
+// An array the call writes: no two of its elements share memory.
+const Tensor& writable(const Tensor& t, const char* what) {
   std::vector<std::pair<int64_t, int64_t>> d;
-  for (int64_t i = 0; i < out.dim(); ++i)
-    if (out.size(i) > 1) d.emplace_back(out.stride(i), out.size(i));
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (t.size(i) > 1) d.emplace_back(t.stride(i), t.size(i));
   std::sort(d.begin(), d.end());
   int64_t reach = 1;
   for (auto [st, n] : d) {
-    if (st < reach) bad("out must not overlap itself");
+    if (st < reach) bad(std::string(what) + " must not overlap itself");
     reach += st * (n - 1);
   }
-  if (out.numel())
-    for (const Opt* x : inputs)
-      if (given(*x) && (*x)->data_ptr() == out.data_ptr()) bad("out must not be one of the inputs");
-  return out;
+  return t;
+}
+
+// Whether two tensors have a byte in common: whether the distance of their
+// starts is a sum of their strides' multiples, a's forwards and b's backwards.
+// The largest strides are tried first, each multiple only if the rest can still
+// make up the difference, which leaves few of them where strides nest, as
+// slices of one wider array have them. After kTries the answer is yes.
+class Overlap {
+ public:
+  static bool of(const Tensor& a, const Tensor& b) {
+    if (a.numel() == 0 || b.numel() == 0) return false;
+    const int64_t gap = (const char*)b.data_ptr() - (const char*)a.data_ptr();
+    if (gap >= bytes(a) || -gap >= bytes(b)) return false;
+    Overlap o;
+    o.add(a, 1), o.add(b, -1);
+    std::sort(o.terms_.begin(), o.terms_.end(),
+              [](const Term& x, const Term& y) { return x.stride > y.stride; });
+    return o.makes(0, gap);
+  }
+
+ private:
+  struct Term {
+    int64_t stride, lo, hi;
+  };
+  static constexpr int kTries = 1 << 16;
+  static int64_t bytes(const Tensor& t) {    // from its start to its end
+    int64_t n = 1;
+    for (int64_t i = 0; i < t.dim(); ++i) n += (t.size(i) - 1) * t.stride(i);
+    return n * (int64_t)t.element_size();
+  }
+  void add(const Tensor& t, int sign) {
+    for (int64_t i = 0; i < t.dim(); ++i)
+      add(t.stride(i) * (int64_t)t.element_size(), sign * (t.size(i) - 1));
+    add(1, sign * ((int64_t)t.element_size() - 1));
+  }
+  void add(int64_t stride, int64_t most) {   // multiples from 0 to `most`
+    if (stride == 0 || most == 0) return;
+    auto at = std::find_if(terms_.begin(), terms_.end(),
+                           [&](const Term& x) { return x.stride == stride; });
+    if (at == terms_.end()) at = terms_.insert(at, Term{stride, 0, 0});
+    (most > 0 ? at->hi : at->lo) += most;
+  }
+  bool makes(size_t k, int64_t gap) {
+    if (++tries_ > kTries) return true;
+    if (k == terms_.size()) return gap == 0;
+    int64_t lo = 0, hi = 0;                  // what the smaller strides can add
+    for (size_t i = k + 1; i < terms_.size(); ++i)
+      lo += terms_[i].stride * terms_[i].lo, hi += terms_[i].stride * terms_[i].hi;
+    const Term& t = terms_[k];
+    auto down = [&](int64_t x) { return x >= 0 ? x / t.stride : -((-x + t.stride - 1) / t.stride); };
+    const int64_t last = std::min(t.hi, down(gap - lo));
+    for (int64_t m = std::max(t.lo, -down(hi - gap)); m <= last; ++m)
+      if (makes(k + 1, gap - m * t.stride)) return true;
+    return false;
+  }
+  c10::SmallVector<Term, 10> terms_;
+  int tries_ = 0;
+};
+
+// Other tensors of a call, by name.
+using Named = std::initializer_list<std::pair<const char*, const Opt*>>;
+
+// `t`, which the call writes, shares no memory with the others: blocks run in
+// any order, so one would read what another has already written.
+void apart(const Tensor& t, const char* what, Named others) {
+  for (const auto& [name, x] : others)
+    if (given(*x) && Overlap::of(t, **x))
+      bad(std::string(what) + " must not share memory with one of the inputs (" + name + ")");
+}
+
+// A step's state, or the array that takes the state after it. That may be the
+// state itself: each element is then read and written by one thread.
+void apart_states(const Opt& state, const Opt& next, Named others) {
+  const bool other = given(next) && next->data_ptr() != state->data_ptr();
+  if (other) apart(*next, "next_state", {{"state", &state}});
+  apart(other ? *next : *state, other ? "next_state" : "state", others);
 }
 
 // (batch, rows, values), or (batch, values) for a single step.
@@ -187,6 +262,14 @@ class Call {
   std::optional<c10::cuda::CUDAStreamGuard> guard_;
 };
 
+// The caller's `out`, or a new tensor like x.
+Tensor output(const Call& c, const Opt& out, const Tensor& x, Named inputs, bool contiguous = true) {
+  if (!given(out)) return c.empty_like(x);
+  const Tensor& t = writable(like(out, x, x.sizes(), "out", contiguous), "out");
+  apart(t, "out", inputs);
+  return t;
+}
+
 py::object to_py(const Tensor& t) { return t.defined() ? py::cast(t) : py::none(); }
 
 // ---------------------------------------------------------------- short convolution
@@ -219,7 +302,8 @@ py::object causal_conv1d(const Opt& xo, const Opt& weight, const Opt& bias,
   const Tensor& x = activation(xo, "x", 3);
   auto a = conv_args(x, weight, bias, act, state, lengths, "initial_state");
   Call c(x, device, stream);
-  Tensor y = given(out) ? writable(like(out, x, x.sizes(), "out"), {&xo, &state}) : c.empty_like(x);
+  Tensor y = output(c, out, x, {{"x", &xo}, {"weight", &weight}, {"bias", &bias},
+                                {"initial_state", &state}, {"lengths", &lengths}});
   Tensor fin;
   if (want_state) fin = c.empty({x.size(0), a.taps - 1, x.size(2)}, x.scalar_type());
   a.y = rows(y);
@@ -259,8 +343,10 @@ Tensor causal_conv1d_step(const Opt& xo, const Opt& state, const Opt& weight, co
   a.final_state = given(next) ? param<void>(next, x, {x.size(0), a.taps - 1, x.size(1)},
                                             "next_state", x.scalar_type())
                               : (void*)a.initial_state;
+  apart_states(state, next, {{"x", &xo}, {"weight", &weight}, {"bias", &bias}});
   Call c(x, device, stream);
-  Tensor y = given(out) ? writable(like(out, x, x.sizes(), "out"), {&xo, &state}) : c.empty_like(x);
+  Tensor y = output(c, out, x, {{"x", &xo}, {"weight", &weight}, {"bias", &bias}, {"state", &state},
+                                {"next_state", &next}});
   a.y = rows(y);
   c.run(ferrum_causal_conv1d_step, a, {&xo, &state, &next, &weight, &bias, &out});
   return y;
@@ -320,9 +406,9 @@ py::tuple selective_scan(const Opt& uo, const Opt& delta, const Opt& A, const Op
   const Tensor& u = activation(uo, "u", 3);
   auto a = scan_args({uo, delta, A, B, C, D, z, bias, softplus}, u, state, lengths, "initial_state");
   Call c(u, device, stream);
-  Tensor y = given(out)
-                 ? writable(like(out, u, u.sizes(), "out"), {&uo, &delta, &z, &B, &C})
-                 : c.empty_like(u);
+  Tensor y = output(c, out, u, {{"u", &uo}, {"delta", &delta}, {"z", &z}, {"B", &B}, {"C", &C},
+                                {"A", &A}, {"D", &D}, {"delta_bias", &bias},
+                                {"initial_state", &state}, {"lengths", &lengths}});
   const int64_t b = u.size(0), d = u.size(2), ns = (int64_t)a.states;
   Tensor fin = c.empty({b, d, ns}, at::kFloat), saved;
   if (save) saved = c.empty({b, saves(a), d, ns}, at::kFloat);
@@ -371,10 +457,12 @@ Tensor selective_scan_step(const Opt& uo, const Opt& delta, const Opt& A, const 
   auto a = scan_args({uo, delta, A, B, C, D, z, bias, softplus}, u, state, std::nullopt, "state");
   a.final_state = given(next) ? param(next, u, {u.size(0), u.size(1), (int64_t)a.states}, "next_state")
                               : (float*)a.initial_state;
+  apart_states(state, next, {{"u", &uo}, {"delta", &delta}, {"z", &z}, {"B", &B}, {"C", &C},
+                             {"A", &A}, {"D", &D}, {"delta_bias", &bias}});
   Call c(u, device, stream);
-  Tensor y = given(out)
-                 ? writable(like(out, u, u.sizes(), "out"), {&uo, &delta, &z, &B, &C})
-                 : c.empty_like(u);
+  Tensor y = output(c, out, u, {{"u", &uo}, {"delta", &delta}, {"z", &z}, {"B", &B}, {"C", &C},
+                                {"A", &A}, {"D", &D}, {"delta_bias", &bias}, {"state", &state},
+                                {"next_state", &next}});
   a.out = rows(y);
   c.run(ferrum_selective_scan_step, a,
         {&uo, &delta, &A, &B, &C, &state, &next, &D, &z, &bias, &out});
@@ -508,8 +596,8 @@ Tensor norm_after(const Opt& xo, const Opt& weight, const Opt& bias, const Opt& 
     a.residual_stride = matrix(*residual, "residual").stride;
   }
   Call c(x, device, stream);
-  Tensor y = given(out) ? writable(like(out, x, x.sizes(), "out"), {&xo, &gate, &residual})
-                        : c.empty_like(x);
+  Tensor y = output(c, out, x, {{"x", &xo}, {"gate", &gate}, {"residual", &residual},
+                                {"weight", &weight}, {"bias", &bias}, {"scale", &scale}});
   a.y = y.data_ptr(), a.y_stride = matrix(y, "out").stride;
   c.run(ferrum_norm_after, a, {&xo, &gate, &residual, &weight, &bias, &scale, &out});
   return y;
@@ -561,7 +649,7 @@ Tensor long_conv(const Opt& xo, const Opt& kernel, const Opt& skip, const Opt& o
   const Tensor& x = activation(xo, "x", 3, false);
   auto a = long_args(x, x.sizes(), kernel, skip);
   Call c(x, device, stream);
-  Tensor y = given(out) ? writable(like(out, x, x.sizes(), "out", false), {&xo}) : c.empty_like(x);
+  Tensor y = output(c, out, x, {{"x", &xo}, {"kernel", &kernel}, {"skip", &skip}}, false);
   a.x = rows(x), a.x_step = x.stride(2), a.y = rows(y), a.y_step = y.stride(2);
   c.run(ferrum_long_conv, a, {&xo, &kernel, &skip, &out});
   return y;
@@ -595,8 +683,11 @@ Tensor long_conv_step(const Opt& xo, const Opt& history, const Opt& positions, c
   auto a = long_args(x, shape, kernel, skip);
   required(positions, "positions");
   a.positions = param<int32_t>(positions, x, {x.size(0)}, "positions", at::kInt);
+  apart(writable(h, "history"), "history", {{"x", &xo}, {"kernel", &kernel}, {"skip", &skip},
+                                            {"positions", &positions}});
   Call c(x, device, stream);
-  Tensor y = given(out) ? writable(like(out, x, x.sizes(), "out"), {&xo, &history}) : c.empty_like(x);
+  Tensor y = output(c, out, x, {{"x", &xo}, {"history", &history}, {"kernel", &kernel},
+                                {"skip", &skip}, {"positions", &positions}});
   a.x = rows(x), a.y = rows(y), a.history = rows(h);
   c.run(ferrum_long_conv_step, a, {&xo, &history, &positions, &kernel, &skip, &out});
   return y;
@@ -618,4 +709,5 @@ PYBIND11_MODULE(_sequence, m) {
   m.def("long_conv", &long_conv);
   m.def("long_conv_backward", &long_conv_backward);
   m.def("long_conv_step", &long_conv_step);
+  m.def("_shares_memory", &Overlap::of);
 }

@@ -28,6 +28,10 @@ of the tensors' device; outputs belong to that stream. ``device`` is an
 optional ``ferrum_gpu.cuda.Device``. Other tensors with a ``__dlpack__``
 export on a GPU are taken without a copy.
 
+``out``, ``next_state``, a state updated in place and ``history`` may not share
+memory with a call's other tensors (``next_state`` may be ``state``); columns of
+one wider array are fine.
+
 Errors: ``ValueError`` for arguments, ``ferrum_gpu.capi.FerrumError`` for
 failures of the library.
 """

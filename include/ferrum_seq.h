@@ -13,6 +13,8 @@
  * type `dtype`; parameters, scan states and parameter gradients are float32.
  * Sums, recurrences and statistics run in float32; each output is rounded
  * once to its type. No result depends on the order in which blocks run.
+ * An array that a call writes shares no memory with its other arrays, except
+ * where a block says so; the C entries take the caller's word for it.
  *
  * `lengths` (int32, one per sequence, optional) are the valid lengths of a
  * padded batch. A length is clamped to [0, length]. Steps past it are not

@@ -259,3 +259,60 @@ def test_a_given_output_outlives_its_call_on_another_stream(i):
     assert fresh.data_ptr() != at, name
     s.synchronize()
     assert not bool(fresh.any()), name
+
+
+def test_outputs_that_share_memory_are_refused():
+    b, n, d, N = 2, 40, 16, 4
+    refused = pytest.raises(ValueError, match="share memory")
+    buf, z, w = rnd(1, b, n + 1, d), rnd(2, b, n, d), rnd(3, d, 4)
+    x, shifted = buf[:, 1:], buf[:, :-1]
+    A, bc, nw = -rnd(4, d, N).abs(), rnd(5, b, n, N), rnd(6, d)
+    keep = buf.clone()
+    with refused:
+        sq.causal_conv1d(x, w, out=shifted)
+    with refused:
+        sq.selective_scan(x, z, A, bc, bc, out=shifted)
+    with refused:
+        sq.selective_scan(z, z, A, x[..., :N], bc, out=x)            # B inside out
+    with refused:
+        sq.norm_after(z[0], nw, residual=x[0], out=shifted[0])
+    line = rnd(7, b * d * (n + 8) + 1)
+    with refused:
+        sq.long_conv(line[1:1 + b * d * n].view(b, d, n), rnd(8, d, n), out=line[:b * d * n].view(b, d, n))
+    st = rnd(9, 3 * b * 3 * d)
+    old, nxt = st[:b * 3 * d].view(b, 3, d), st[d:d + b * 3 * d].view(b, 3, d)
+    with refused:
+        sq.causal_conv1d_step(z[:, 0], old, w, next_state=nxt)
+    with refused:
+        sq.causal_conv1d_step(z[:, 0], old, w, out=old[:, 0])
+    with refused:
+        sq.causal_conv1d_step(old[:, 1], old, w)                     # x inside the state
+    st = rnd(10, 2 * b * d * N)
+    old, nxt = st[:b * d * N].view(b, d, N), st[N:N + b * d * N].view(b, d, N)
+    with refused:
+        sq.selective_scan_step(z[:, 0], z[:, 1], A, bc[:, 0], bc[:, 0], old, next_state=nxt)
+    with refused:
+        sq.selective_scan_step(z[:, 0], z[:, 1], A, bc[:, 0], bc[:, 0], old,
+                               out=st[:b * d].view(b, d))
+    hist, pos = rnd(11, b, d, n), torch.zeros(b, dtype=torch.int32, device="cuda")
+    with refused:
+        sq.long_conv_step(z[:, 0], hist, pos, rnd(12, d, n), out=hist.view(-1)[:b * d].view(b, d))
+    with pytest.raises(ValueError, match="overlap itself"):
+        sq.long_conv_step(z[:, 0], hist[:1].expand(b, d, n), pos, rnd(12, d, n))
+    assert torch.equal(buf, keep)
+
+
+def test_outputs_beside_their_inputs_are_taken():
+    """Columns of one array, and a state that is its own successor."""
+    b, n, d = 2, 40, 16
+    wide, w = rnd(1, b, n, 3 * d), rnd(2, d, 4)
+    x = wide[..., d:2 * d]
+    want = sq.causal_conv1d(x, w)
+    sq.causal_conv1d(x, w, out=wide[..., 2 * d:])
+    assert torch.equal(wide[..., 2 * d:], want)
+    sq.norm_after(x, rnd(3, d), gate=wide[..., 2 * d:], out=wide[..., :d])
+    st = rnd(4, b, 3, d)
+    other = torch.empty_like(st)
+    y = sq.causal_conv1d_step(x[:, 0], st, w, next_state=other)
+    assert torch.equal(y, sq.causal_conv1d_step(x[:, 0], st, w, next_state=st))
+    assert torch.equal(st, other)
