@@ -50,23 +50,35 @@ SAVE_STEPS = 16
 
 
 def _call(fn, *args):
-    """``fn(*args)``; tensors of other libraries are taken over DLPack."""
+    """``fn(*args)``, ``args`` ending with the call's stream; tensors of other
+    libraries are taken over DLPack."""
     try:
         return fn(*args)
     except TypeError:
-        taken = [_from_dlpack(a) for a in args]
+        taken = [_from_dlpack(a, args[-1]) for a in args]
         if all(a is b for a, b in zip(taken, args)):
             raise ValueError("tensor arguments must be CUDA tensors") from None
         return fn(*taken)
 
 
-def _from_dlpack(x):
+def _from_dlpack(x, stream):
     place = getattr(x, "__dlpack_device__", None)
     if isinstance(x, torch.Tensor) or place is None:
         return x
-    if place()[0] != 2:   # kDLCUDA
+    kind, ordinal = place()
+    if kind != 2:   # kDLCUDA
         raise ValueError("tensor arguments must be a CUDA tensor (got one on the host)")
-    return torch.from_dlpack(x)
+    # The producer orders its work in front of the stream that is current.
+    with torch.cuda.stream(_torch_stream(stream, ordinal)):
+        return torch.from_dlpack(x)
+
+
+def _torch_stream(stream, ordinal):
+    if stream is None or isinstance(stream, torch.cuda.Stream):
+        return stream
+    handle = int(getattr(stream, "cuda_stream", stream))
+    return (torch.cuda.ExternalStream(handle, device=ordinal) if handle
+            else torch.cuda.default_stream(ordinal))
 
 
 # ---------------------------------------------------------------- short convolution

@@ -316,3 +316,51 @@ def test_outputs_beside_their_inputs_are_taken():
     y = sq.causal_conv1d_step(x[:, 0], st, w, next_state=other)
     assert torch.equal(y, sq.causal_conv1d_step(x[:, 0], st, w, next_state=st))
     assert torch.equal(st, other)
+
+
+class Exported:
+    """An array of another library: only DLPack, and it notes the stream that its
+    producer is asked to be ready for."""
+
+    def __init__(self, t):
+        self.t, self.asked = t, []
+
+    def __dlpack_device__(self):
+        return self.t.__dlpack_device__()
+
+    def __dlpack__(self, *, stream=None, **kw):
+        self.asked.append(stream)
+        return self.t.__dlpack__(stream=stream, **kw)
+
+
+def test_arrays_of_other_libraries():
+    """Taken without a copy, ready for the stream that the call runs on."""
+    b, n, d, N = 2, 40, 16, 4
+    x, z, w, nw = rnd(1, b, n, d), rnd(2, b, n, d), rnd(3, d, 4), rnd(4, d)
+    A, bc, k = -rnd(5, d, N).abs(), rnd(6, b, n, N), rnd(7, n, d)
+    pos = torch.zeros(b, dtype=torch.int32, device="cuda")
+    e = Exported
+    for given, want in (
+            (lambda **s: sq.causal_conv1d(e(x), e(w), e(nw), **s), sq.causal_conv1d(x, w, nw)),
+            (lambda **s: sq.selective_scan(x, e(z), e(A), bc, e(bc), z=e(z), **s).out,
+             sq.selective_scan(x, z, A, bc, bc, z=z).out),
+            (lambda **s: sq.norm_before(e(x), nw, residual=e(z), **s)[0],
+             sq.norm_before(x, nw, residual=z)[0]),
+            (lambda **s: sq.norm_after(x, e(nw), gate=e(z), **s), sq.norm_after(x, nw, gate=z)),
+            (lambda **s: sq.long_conv(e(x), k, **s), sq.long_conv(x, k)),
+            (lambda **s: sq.causal_conv1d_step(e(x[:, 0]), e(z[:, :3].contiguous()), w, **s),
+             sq.causal_conv1d_step(x[:, 0], z[:, :3].contiguous(), w))):
+        assert torch.equal(given(), want)
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        got = given(stream=s)
+        s.synchronize()
+        assert torch.equal(got, want)
+    out = torch.empty_like(x)
+    assert sq.causal_conv1d(e(x), w, out=e(out)).data_ptr() == out.data_ptr()
+    s = torch.cuda.Stream()
+    for stream, asked in ((None, 1), (s, s.cuda_stream), (s.cuda_stream, s.cuda_stream), (0, 1)):
+        x2 = e(x)
+        sq.causal_conv1d(x2, w, stream=stream)
+        assert x2.asked == [asked]         # (1 is DLPack's number of the default stream)
+    torch.cuda.synchronize()
