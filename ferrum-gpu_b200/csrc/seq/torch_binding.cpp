@@ -217,7 +217,12 @@ class Call {
       stream_ = c10::cuda::getCurrentCUDAStream(ordinal_).stream();
     } else {
       const py::object s = py::hasattr(stream, "cuda_stream") ? stream.attr("cuda_stream") : stream;
-      stream_ = (cudaStream_t)s.cast<uintptr_t>();
+      try {
+        stream_ = (cudaStream_t)s.cast<uintptr_t>();
+      } catch (const py::cast_error&) {
+        bad("stream must be a cudaStream_t as int or a torch stream, got " +
+            py::str(py::type::of(s).attr("__name__")).cast<std::string>());
+      }
       other_ = c10::cuda::getStreamFromExternal(stream_, ordinal_);
       guard_.emplace(*other_);
     }

@@ -38,6 +38,7 @@ failures of the library.
 
 from __future__ import annotations
 
+import inspect
 from typing import NamedTuple, Optional
 
 import torch
@@ -54,11 +55,37 @@ def _call(fn, *args):
     libraries are taken over DLPack."""
     try:
         return fn(*args)
-    except TypeError:
+    except TypeError as e:
+        _check_types(fn.__name__, args)
         taken = [_from_dlpack(a, args[-1]) for a in args]
         if all(a is b for a, b in zip(taken, args)):
-            raise ValueError("tensor arguments must be CUDA tensors") from None
+            raise ValueError(str(e).split("\n")[0]) from None
         return fn(*taken)
+
+
+# Arguments that are no tensors: what they must be, and whether one is.
+_OTHERS = {
+    "activation": ("None or a string", lambda v: v is None or isinstance(v, str)),
+    "kind": ("a string", lambda v: isinstance(v, str)),
+    "eps": ("a number", lambda v: hasattr(v, "__float__") and not isinstance(v, str)),
+    "groups": ("an integer", lambda v: hasattr(v, "__index__")),
+    "device": ("a ferrum_gpu.cuda.Device", lambda v: True),      # looked at by the call
+    "stream": ("a stream", lambda v: True),
+    **{name: ("a truth value", lambda v: hasattr(v, "__bool__"))
+       for name in ("return_final_state", "delta_softplus", "save_states", "gate_inside")},
+}
+
+
+def _check_types(name, args):
+    """Names the argument of the public function ``name`` that has a type its
+    binding cannot take (both have their arguments in the same order)."""
+    for arg, v in zip(inspect.signature(globals()[name]).parameters, args):
+        if arg in _OTHERS:
+            what, good = _OTHERS[arg]
+            if not good(v):
+                raise ValueError(f"{arg} must be {what}, got {type(v).__name__}")
+        elif v is not None and not isinstance(v, torch.Tensor) and not hasattr(v, "__dlpack_device__"):
+            raise ValueError(f"{arg} must be a CUDA tensor, got {type(v).__name__}")
 
 
 def _from_dlpack(x, stream):

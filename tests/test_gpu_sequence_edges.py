@@ -364,3 +364,10 @@ def test_arrays_of_other_libraries():
         sq.causal_conv1d(x2, w, stream=stream)
         assert x2.asked == [asked]         # (1 is DLPack's number of the default stream)
     torch.cuda.synchronize()
+
+
+def test_a_stream_of_a_wrong_type_is_refused():
+    x, w = rnd(1, 4, 8), rnd(2, 8)
+    for stream in ("s", -1, 1.5):
+        with pytest.raises(ValueError, match="stream must be"):
+            sq.norm_before(x, w, stream=stream)
