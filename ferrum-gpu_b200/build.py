@@ -3,7 +3,8 @@
 Outputs (next to the Python package so they travel with the source tree):
   ferrum_gpu/libferrum_fft.so                    C ABI (include/ferrum_fft.h, ferrum_seq.h) + sm_100a kernels
   ferrum_gpu/_native.<python-ext-suffix>         pybind11 module over the C ABI
-  ferrum_gpu/_sequence.<python-ext-suffix>       the sequence operators on torch tensors
+  ferrum_gpu/_sequence.<python-ext-suffix>       the sequence operators on torch tensors (where
+                                                 torch is installed, against that version)
 
 Every .cu is compiled with
   nvcc -gencode arch=compute_100a,code=sm_100a -lineinfo -O3
@@ -23,6 +24,7 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+from importlib import metadata
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(HERE)
@@ -97,8 +99,30 @@ def build(jobs: int = 4, force: bool = False) -> None:
         _run([CXX, "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
               f"-I{pybind11.get_include()}", f"-I{py_inc}", f"-I{INCLUDE}", native_src,
               "-o", EXT, f"-L{PKG}", "-lferrum_fft", "-Wl,-rpath,$ORIGIN"])
-    seq_src = os.path.join(CSRC, "seq", "torch_binding.cpp")
-    if force or _stale(SEQ_EXT, [seq_src, LIB] + _headers(seq=True)):
+    if not build_sequence(force):
+        print("torch is not installed: ferrum_gpu.sequence is left out", file=sys.stderr)
+
+
+def _torch_version() -> str | None:
+    try:
+        return metadata.version("torch")
+    except metadata.PackageNotFoundError:
+        return None
+
+
+def build_sequence(force: bool = False) -> bool:
+    """The module on torch tensors; False where torch is not installed. It is
+    rebuilt for another torch, whose C++ interface it is compiled against."""
+    version = _torch_version()
+    if version is None:
+        return False
+    src = os.path.join(CSRC, "seq", "torch_binding.cpp")
+    stamp = os.path.join(BUILD, "torch_version")
+    built = ""
+    if os.path.exists(stamp):
+        with open(stamp) as f:
+            built = f.read()
+    if force or built != version or _stale(SEQ_EXT, [src, LIB] + _headers(seq=True)):
         import torch
 
         torch_dir = os.path.dirname(torch.__file__)
@@ -106,9 +130,12 @@ def build(jobs: int = 4, force: bool = False) -> None:
         _run([CXX, "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
               f"-I{torch_dir}/include", f"-I{torch_dir}/include/torch/csrc/api/include",
-              f"-I{CUDA_HOME}/include", f"-I{py_inc}", f"-I{INCLUDE}", seq_src, "-o", SEQ_EXT,
+              f"-I{CUDA_HOME}/include", f"-I{py_inc}", f"-I{INCLUDE}", src, "-o", SEQ_EXT,
               f"-L{torch_dir}/lib", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python",
               f"-L{PKG}", "-lferrum_fft", "-Wl,-rpath,$ORIGIN"])
+        with open(stamp, "w") as f:
+            f.write(version)
+    return True
 
 
 def main() -> None:
@@ -119,7 +146,8 @@ def main() -> None:
     build(a.jobs, a.force)
     print(LIB)
     print(EXT)
-    print(SEQ_EXT)
+    if _torch_version() is not None:
+        print(SEQ_EXT)
 
 
 if __name__ == "__main__":
