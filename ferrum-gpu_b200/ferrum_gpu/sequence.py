@@ -9,7 +9,10 @@ reference:
 ``norm_before``     residual update and norm in front of a block
 ``norm_after``      gated norm behind a block, scaled onto the residual
 
-Each has a ``*_backward``; the filters have a ``*_step`` for one token of
+The calls are not recorded by autograd: a result does not require a gradient,
+whatever its arguments do. Each operator has a ``*_backward`` instead, to be
+called from a ``torch.autograd.Function`` (``examples/sequence_block.py`` has one
+for each). The filters have a ``*_step`` for one token of
 every sequence on kept state. They call the C ABI of ``include/ferrum_seq.h``
 (``ferrum_gpu.capi`` binds it for callers with raw pointers).
 
