@@ -154,6 +154,53 @@ def test_softplus_keeps_its_relative_accuracy():
     assert got[0] == float("inf") and got[1] == 0 and got[2] != got[2] and got[3] == 0
 
 
+# ---------------------------------------------------------------- long sequences
+# A state's error is made anew by each step and decays with it. Per step: the
+# exponential 4 units (2 in its last place), its argument |dt A log2 e| <= 2
+# twice, product and sum 3: 12 units of the state, so 12 / (1 - a) at most, with
+# a the largest factor exp(dt A). Terms are of the size of the results (random
+# signs); a factor of 4 covers the sums that cancel, and every error is
+# measured against the largest value of its own channel.
+
+LONG = [(1, 1030, 40, 16), (2, 517, 130, 16), (1, 300, 1001, 13), (1, 2049, 33, 32),
+        (3, 260, 4100, 8), (6, 150, 1001, 16), (1, 700, 20, 64)]
+
+
+@pytest.mark.parametrize("b,n,d,N", LONG)
+def test_long_scans_keep_float32_accuracy(b, n, d, N):
+    u, z, dout = rnd(1, b, n, d), rnd(2, b, n, d), rnd(3, b, n, d)
+    delta = rnd(4, b, n, d, std=0.3).abs().clamp(0.05, 1.0)
+    A = -(1 + rnd(5, d, N).abs().clamp(max=1.0))       # 1 <= -A <= 2, a <= e^-0.05
+    B, C, D, h0 = rnd(6, b, n, N), rnd(7, b, n, N), rnd(8, d), rnd(9, b, d, N)
+    leaves = [t.double().requires_grad_(True) for t in (u, delta, A, B, C, D, z, h0)]
+    ud, dd, Ad, Bd, Cd, Dd, zd, h = leaves
+    ys = []
+    for t in range(n):
+        h = torch.exp(dd[:, t, :, None] * Ad) * h + (dd[:, t] * ud[:, t])[..., None] * Bd[:, t, None]
+        ys.append((h * Cd[:, t, None]).sum(-1))
+    out = (torch.stack(ys, 1) + Dd * ud) * zd * torch.sigmoid(zd)
+    c = 12 / (1 - torch.exp(torch.tensor(-0.05)).item()) + N + 16
+
+    def close(got, ref, units, dims, what):
+        top = ref.abs().amax(dims, keepdim=True)
+        worst = ((got - ref).abs() / top).max().item() / UNIT
+        assert worst <= 4 * units, f"{what}: {worst:.0f} units above {4 * units:.0f}"
+
+    k = dict(D=D, z=z)
+    r = sq.selective_scan(u, delta, A, B, C, initial_state=h0, save_states=True, **k)
+    close(r.out, out.detach(), c, 1, "out")
+    close(r.final_state, h.detach(), c, 2, "final_state")
+    ref = torch.autograd.grad((out * dout.double()).sum(), leaves)
+    g = sq.selective_scan_backward(dout, u, delta, A, B, C, r.states, **k)
+    # the gradient's recurrence decays alike, on states with errors of their own
+    for got, want, units, dims, what in (
+            (g.du, ref[0], 2 * c, 1, "du"), (g.ddelta, ref[1], 2 * c + N, 1, "ddelta"),
+            (g.dB, ref[3], 2 * c + d ** 0.5, 1, "dB"), (g.dC, ref[4], c + d ** 0.5, 1, "dC"),
+            (g.dz, ref[6], c, 1, "dz"), (g.dinitial_state, ref[7], 2 * c, 2, "dinitial_state"),
+            (g.dA, ref[2], 2 * c + n ** 0.5, 1, "dA"), (g.dD, ref[5], c + n ** 0.5, 0, "dD")):
+        close(got, want, units, dims, what)
+
+
 # ---------------------------------------------------------------- slow states
 
 @pytest.mark.parametrize("b,d", SPLITS)
@@ -371,3 +418,66 @@ def test_a_stream_of_a_wrong_type_is_refused():
     for stream in ("s", -1, 1.5):
         with pytest.raises(ValueError, match="stream must be"):
             sq.norm_before(x, w, stream=stream)
+
+
+def stream_calls():
+    """Every operator, gradient and step: name, the input that changes, call(stream)."""
+    b, n, d, N = 3, 70, 40, 8
+    r = lambda i, *s, **k: rnd(200 + i, *s, **k)
+    x, z, dy = r(0, b, n, d), r(1, b, n, d), r(2, b, n, d)
+    w, nw, cs = r(3, d, 4), r(4, d), r(5, b, 3, d)
+    A, B, C, h = -r(6, d, N).abs(), r(7, b, n, N), r(8, b, n, N), r(9, b, d, N)
+    st = sq.selective_scan(x, z, A, B, C, delta_softplus=True, save_states=True).states
+    flat, out2 = x.view(b * n, d), torch.empty_like(h)
+    res = r(10, b * n, d)
+    big, bk = r(11, 1, 2, 16385), r(12, 2, 16385, std=0.01)      # several passes
+    few, fk, fdy = r(13, 9, 2, 300), r(14, 2, 300, std=0.05), r(15, 9, 2, 300)
+    last = r(16, b, 300, d).transpose(1, 2)                      # channel-last
+    lk, pos = r(17, d, 300, std=0.05), torch.full((b,), n - 1, dtype=torch.int32, device="cuda")
+    hist, hk, x1, z1 = r(18, b, d, n), r(19, d, n), x[:, 0].contiguous(), z[:, 0].contiguous()
+    nxt = torch.empty_like(cs)
+    k = dict(delta_softplus=True)
+    return [
+        ("conv", x, lambda s: sq.causal_conv1d(x, w, initial_state=cs, return_final_state=True, stream=s)),
+        ("conv gradient", dy, lambda s: sq.causal_conv1d_backward(dy, x, w, nw, stream=s)),
+        ("conv step", x1, lambda s: (sq.causal_conv1d_step(x1, cs, w, next_state=nxt, stream=s), nxt)),
+        ("scan", x, lambda s: sq.selective_scan(x, z, A, B, C, stream=s, save_states=True, **k)),
+        ("scan gradient", dy, lambda s: sq.selective_scan_backward(dy, x, z, A, B, C, st, stream=s, **k)),
+        ("scan step", x1, lambda s: (sq.selective_scan_step(
+            x1, z1, A, B[:, 0], C[:, 0], h, next_state=out2, stream=s, **k), out2)),
+        ("norm before", flat, lambda s: sq.norm_before(flat, nw, residual=res, scale=nw, stream=s)),
+        ("norm before gradient", flat, lambda s: sq.norm_before_backward(
+            res, flat, nw, nw, x=res, scale=nw, stream=s)),
+        ("norm after", flat, lambda s: (sq.norm_after(flat, nw, gate=res, groups=2, stream=s),)),
+        ("norm after gradient", flat, lambda s: sq.norm_after_backward(
+            res, flat, nw, nw, gate=res, scale=nw, stream=s)),
+        ("long conv, by definition", hist, lambda s: (sq.long_conv(hist[:, :, :50], hk[:, :50].contiguous(), nw, stream=s),)),
+        ("long conv, channel-last", last, lambda s: (sq.long_conv(last, lk, nw, stream=s),)),
+        ("long conv, several passes", big, lambda s: (sq.long_conv(big, bk, stream=s),)),
+        ("long conv gradient", few, lambda s: sq.long_conv_backward(fdy, few, fk, stream=s)),
+        ("long conv gradient, several passes", big, lambda s: sq.long_conv_backward(big, big, bk, stream=s)),
+        ("long step", x1, lambda s: (sq.long_conv_step(x1, hist, pos, hk, stream=s),)),
+    ]
+
+
+@pytest.mark.parametrize("i", range(16))
+def test_calls_run_on_the_given_stream(i):
+    """An input changes on the stream, behind a delay; only a call on that same
+    stream sees it, with all its passes and workspaces."""
+    name, t, call = stream_calls()[i]
+    old = [v.clone() for v in call(None) if v is not None]
+    new = rnd(300, *t.shape)
+    keep = t.clone()
+    t.copy_(new)
+    want = [v.clone() for v in call(None) if v is not None]
+    assert not all(torch.equal(p, q) for p, q in zip(old, want))
+    t.copy_(keep)
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        torch.cuda._sleep(20_000_000)           # some 10 ms
+        t.copy_(new)
+    got = call(s)
+    s.synchronize()
+    for p, q in zip((v for v in got if v is not None), want):
+        assert torch.equal(p, q), name
