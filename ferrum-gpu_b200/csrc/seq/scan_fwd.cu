@@ -432,19 +432,29 @@ ferrum_status scan_fwd(ferrum_device* dev, const ferrum_scan_args* a, cudaStream
   if (guard.status() != cudaSuccess) return cuda_error(guard.status(), "cudaSetDevice");
   // Lanes per channel: few keep the shuffles short. Where a batch has too few
   // channels to fill the GPU that way, a channel gets more lanes, then several
-  // warps that share its states. Measured (us, 16 states, bf16) for lanes x
-  // warps, the choice marked:
-  //                    4 x 1   8 x 1   16 x 1   16 x 2   16 x 4   8 x 4
-  //   8 x 2048 x 2048   382*    377     416      531      754     567
-  //   4 x 4096 x 2048   519     418*    424      547      752     586
-  //   2 x 8192 x 2048   883     574     471*     604      770     649
-  //   1 x 8192 x 2048   883     501     330      307*     436     332
-  //   1 x 4096 x 512    444     254     145      115       80*    125
-  // (13 x 777 x 1000 in float32: 137 and 152 with 4 x 1 and 8 x 1.)
+  // warps that share its states. Measured (us, bf16, lanes x warps; the choice
+  // marked):
+  //                             4 x 1   8 x 1   16 x 1   16 x 2   16 x 4
+  //   8 x 2048 x 2048, 16       390*    380     431      549      744
+  //   4 x 4096 x 2048, 16       515     422*    437      568      741
+  //   2 x 8192 x 2048, 16       851     568     484*     625      758
+  //   1 x 8192 x 2048, 16       850     482     338      318*     431
+  //   1 x 4096 x 512, 16        427     246     144      120       78*
+  //   13 x 777 x 1000, 16, f32  140*    152     184      212      252
+  //   8 x 2048 x 2048, 8        266*    258     285      352
+  //   2 x 8192 x 2048, 8        613     390     317*     396
+  //   1 x 8192 x 2048, 8        613     334     226      204*
+  //   2 x 8192 x 2048, 32      1348     935*   1135      936     1196
+  //   1 x 8192 x 2048, 32      1348     764     580      475*     671
+  //   8 x 2048 x 2048, 64      1153*   1335    3035     1956     2565
+  //   2 x 8192 x 2048, 64      2342    1678*   3399     2199     2538
+  //   1 x 8192 x 2048, 64      2341    1380    1714     1111*    1450
+  // (16 x 1 loses above 16 states: pieces of 128 steps of B and C leave room for
+  // three blocks an SM with 32 states, for one with 64.)
   const int64_t rows = s.batch * s.channels;
   const int level = rows >= 12288 || s.length <= 32  ? 0
                     : rows >= 6000 || s.length <= 64 ? 1
-                    : rows >= 3000                   ? 2
+                    : rows >= 3000                   ? (s.states > 16 ? 1 : 2)
                     : rows >= 1000                   ? 3 : 4;
   return with_dtype(a->dtype, [&](auto tag) {
     using T = decltype(tag);
@@ -452,7 +462,8 @@ ferrum_status scan_fwd(ferrum_device* dev, const ferrum_scan_args* a, cudaStream
       constexpr int NP = decltype(np)::value;
       if (level == 0) return run_fwd<T, 4, 1, NP>(a, s, stream, what);
       if (level == 1) return run_fwd<T, 8, 1, NP>(a, s, stream, what);
-      if (level == 2) return run_fwd<T, 16, 1, NP>(a, s, stream, what);
+      if constexpr (NP <= 16)
+        if (level == 2) return run_fwd<T, 16, 1, NP>(a, s, stream, what);
       if (level == 3 || NP == 8) return run_fwd<T, 16, 2, NP>(a, s, stream, what);
       if constexpr (NP > 8) return run_fwd<T, 16, 4, NP>(a, s, stream, what);
       return FERRUM_OK;
