@@ -132,9 +132,9 @@ const Tensor& writable(const Tensor& t, const char* what) {
 class Overlap {
  public:
   static bool of(const Tensor& a, const Tensor& b) {
+    const int64_t gap = (const char*)b.const_data_ptr() - (const char*)a.const_data_ptr();
+    if (gap >= 0 ? gap >= bytes(a) : -gap >= bytes(b)) return false;
     if (a.numel() == 0 || b.numel() == 0) return false;
-    const int64_t gap = (const char*)b.data_ptr() - (const char*)a.data_ptr();
-    if (gap >= bytes(a) || -gap >= bytes(b)) return false;
     Overlap o;
     o.add(a, 1), o.add(b, -1);
     std::sort(o.terms_.begin(), o.terms_.end(),
@@ -148,8 +148,10 @@ class Overlap {
   };
   static constexpr int kTries = 1 << 16;
   static int64_t bytes(const Tensor& t) {    // from its start to its end
+    if (t.is_contiguous()) return t.nbytes();
+    const auto size = t.sizes(), stride = t.strides();
     int64_t n = 1;
-    for (int64_t i = 0; i < t.dim(); ++i) n += (t.size(i) - 1) * t.stride(i);
+    for (size_t i = 0; i < size.size(); ++i) n += (size[i] - 1) * stride[i];
     return n * (int64_t)t.element_size();
   }
   void add(const Tensor& t, int sign) {
