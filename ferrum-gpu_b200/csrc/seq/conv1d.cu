@@ -7,8 +7,8 @@
 // them (4 in the gradient). Bytes in flight decide: 8 x 2048 x 4096, 4 taps,
 // bf16 took 75 us with 4 channels, 4 rows ahead and 24 warps an SM, 92 with 8
 // channels and 16 warps, 70 with 2 channels, 8 rows and 32 warps; the
-// gradient 142 with 24 warps and 129 with 32 (float32, whose windows spill
-// there, 162 and 181). That is 3.9 and 3.1 TB/s of the 6.5 of a copy, bound by
+// gradient 142 with 24 warps and 131 with 32 (float32, whose windows spill
+// there, 162 and 181; forward 95). That is 3.9 and 3.1 TB/s of the 6.5 of a copy, bound by
 // issue slots (61 and 72 %) and, forward, the SiLU's two special functions a
 // value (53 %). Runs are long (64 steps) where the batch fills the GPU
 // and shorter where it does not.

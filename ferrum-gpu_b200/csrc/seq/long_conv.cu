@@ -75,7 +75,10 @@ direct_dk_kernel(Rows<T> x, Rows<T> dy, float* __restrict__ dk, float* __restric
 }
 
 // One token: x goes into the history at its sequence's position, and the
-// history up to there, reversed, meets the filter. One block per (b, d).
+// history up to there, reversed, meets the filter. One block per (b, d), each
+// thread one value at a time: waits on loads bound it (8 x 1024 x 8192, bf16:
+// 127 us, where history and filter once would take 26; 1 x 1024 x 1024 10 us, of
+// which a launch is most).
 template <class T>
 __global__ void __launch_bounds__(kThreads)
 long_step_kernel(Rows<T> x, Rows<T> y, Rows<T> hist, const int32_t* __restrict__ positions,
@@ -170,7 +173,9 @@ struct LongCfg {
   // Blocks an SM that the registers must allow for. The kernels wait on loads
   // (the factors, mostly), so warps count more than registers: rows_kernel at
   // 8 x 1024 x 4096 took 340, 328, 281 and 312 us with 2, 3, 4 and 5 blocks;
-  // with 32 values a thread (M = 8192), 1362 us with 1 and 934 with 2. The
+  // with 32 values a thread (M = 8192), 1362 us with 1 and 934 with 2. Shorter
+  // rows alike: 2, 3, 4, 5 blocks at M = 128 193, 160, 144, 199 us, at 512 252, 215,
+  // 197, 230, at 2048 287, 258, 240, 289 (33.5 M values in all). The
   // dkernel's sums take 32 or 64 registers more: 2 blocks up to M = 2048, 3 at
   // 4096 (forward + gradient 722 -> 689 us), 1 at 8192.
   static constexpr int ROW_BLOCKS = LOGM >= 13 ? 2 : 4;
@@ -178,7 +183,8 @@ struct LongCfg {
   // its time where each is loaded when it is needed (8 x 1024 x 4096 without
   // any loads: 211 us). What shared memory is left beside ROW_BLOCKS blocks
   // takes the first STAGED of a thread's P of them, copied while the first
-  // transform runs: 281 -> 271 us, M = 8192 934 -> 840.
+  // transform runs: 281 -> 271 us, M = 8192 934 -> 840. (0, 5 and 8 staged at
+  // M = 128 164, 144, 170 us; at 512 201, 197, 225; at 2048 246, 240, 264.)
   static constexpr int STAGED = LOGM >= 13 ? 10 : 5;
   static constexpr size_t ROW_BYTES = BYTES + sizeof(float4) * (size_t)(STAGED * THREADS);
   static constexpr int DK_BLOCKS = LOGM >= 13 ? 1 : (LOGM == 12 ? 3 : 2);

@@ -16,9 +16,12 @@
 // no second pass over the arrays is needed; their few hundred partial sums
 // are added in a fixed order.
 // Measured, bf16, of the 6.5 TB/s of a copy: norm_before with a float32 residual,
-// 16384 x 2048, 68 us (91 %), its gradient 138 us (67 %; waits on loads at 32
-// warps an SM); norm_after, 8191 x 4096 in 8 groups, 68 us (61 %) and 109 us
-// (47 %): issue slots (58 and 68 %) and the gate's two special functions.
+// 16384 x 2048, 69 us (90 %), its gradient 139 us (66 %; waits on loads at 32
+// warps an SM); norm_after, 8191 x 4096 in 8 groups, 69 us (60 %) and 111 us
+// (46 %): issue slots (58 and 68 %) and the gate's two special functions. In one
+// group (512 threads a row) 78 and 166 us: barriers, and in the gradient the
+// column sums' spills, which above 8192 values cost most of the time
+// (4000 x 12000: 141 and 658 us; norm_before's gradient 350).
 #include <algorithm>
 
 #include "seq_common.cuh"
@@ -86,8 +89,10 @@ struct Unit {
 };
 
 // Warps an SM that the registers must allow for, so that enough loads are in
-// flight: 32; in norm_after's gradient, which spills more than it gains there
-// (16384 x 2048: 111 us against 125), 24 for blocks of up to 256 threads.
+// flight: 32; in norm_after's gradient, which spills more than it gains there,
+// 24 for blocks of up to 256 threads (us with 24 and 32: 16384 x 2048 in 8 groups
+// 111, 123, in one 138, 156; 65536 x 512 121, 140; 200000 x 128 170, 191). Wider
+// blocks lose by it (8191 x 4096 in one group 178, 166).
 constexpr int kWarps = 32, kAfterBwdWarps = 24;
 constexpr int min_blocks(int tpr, int values, int warps) {
   return values > 8 ? 1 : (tpr == 32 ? warps / 8 : std::max(1, warps * 32 / tpr));

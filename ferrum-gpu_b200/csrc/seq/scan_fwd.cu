@@ -22,9 +22,9 @@
 // channels, are converted to float32 once per piece. States go in fours: 4
 // chains in flight, 16-byte reads of B and C, and the two-wide FP32
 // instructions over pairs of states.
-// Measured, 16 states, bf16: 8 x 2048 x 2048 in 384 us, 1.4e12 exponentials a
-// second (39 % of the special-function unit, issue slots 56 %, shared memory
-// 64 %; HBM would take 41 us); 1 x 8192 x 2048 in 307 us. What is
+// Measured, 16 states, bf16: 8 x 2048 x 2048 in 390 us, 1.4e12 exponentials a
+// second (38 % of the special-function unit, issue slots 55 %, shared memory
+// 63 %; HBM would take 41 us); 1 x 8192 x 2048 in 318 us. What is
 // left is latency at 13 warps an SM: steps are a chain within a channel.
 // Giving each thread a share of a channel's states over all steps instead (no
 // compositions, 30 % fewer instructions) took 350 us at 8 x 2048 x 2048, but
