@@ -242,6 +242,26 @@ def test_scan_of_slow_states_errs_like_a_float32_loop(b, d):
     assert off(state, ref[0]) <= 2 * off(ref[1], ref[0])
 
 
+@pytest.mark.parametrize("b,d", SPLITS)
+def test_scan_states_of_rate_zero_stay(b, d):
+    """A = 0: the factor is 1 to the last bit, at every step and past the end, so
+    a state without input keeps its bits."""
+    n, N = 500, 16
+    u, B = torch.zeros(b, n, d, device="cuda"), rnd(1, b, n, N)
+    delta, A, h0 = rnd(2, b, n, d), full(0.0, d, N), rnd(3, b, d, N)
+    for softplus in (True, False):
+        r = sq.selective_scan(u, delta, A, B, B, delta_softplus=softplus, initial_state=h0,
+                              save_states=True)
+        assert torch.equal(r.final_state, h0)
+        assert all(torch.equal(r.states[:, i], h0) for i in range(r.states.shape[1]))
+    state = h0.clone()
+    sq.selective_scan_step(u[:, 0], delta[:, 0], A, B[:, 0], B[:, 0], state, delta_softplus=True)
+    assert torch.equal(state, h0)
+    dfin = rnd(4, b, d, N)
+    g = sq.selective_scan_backward(u, u, delta, A, B, B, r.states, dfinal_state=dfin)
+    assert torch.equal(g.dinitial_state, dfin)
+
+
 # ---------------------------------------------------------------- sizes
 
 def test_lengths_that_wrap_around_are_refused():
