@@ -83,6 +83,21 @@ def test_scan_of_growing_states(b, d, N, n, rate):
         assert ((r.states[:, at] - mid).abs() <= tol * mid).all()
 
 
+@pytest.mark.parametrize("b,d", SPLITS)
+def test_scan_of_states_that_grow_by_negative_steps(b, d):
+    """dt A and dt u are the same for -dt, -A, -u: so are the results, to the bit."""
+    n, N, rate = 112, 16, 1.45
+    B, C, h0 = rnd(1, b, n, N), rnd(2, b, n, N), rnd(3, b, d, N, std=1e-37)
+    u, dt = rnd(4, b, n, d, std=1e-37), full(1.0, b, n, d)
+    dt[:, ::7] = -0.5                                # some factors below 1 too
+    A = full(rate, d, N)
+    p = sq.selective_scan(u, dt, A, B, C, initial_state=h0, save_states=True)
+    q = sq.selective_scan(-u, -dt, -A, B, C, initial_state=h0, save_states=True)
+    assert bool(torch.isfinite(p.final_state).all())
+    for x, y in zip(p, q):
+        assert torch.equal(x, y)
+
+
 @pytest.mark.parametrize("n", [5, 64, 150])
 @pytest.mark.parametrize("b,d", SPLITS)
 def test_scan_states_that_forget_at_once(b, d, n):
