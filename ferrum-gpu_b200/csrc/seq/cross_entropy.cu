@@ -1,0 +1,81 @@
+// Softmax cross entropy of hidden rows against a vocabulary matrix: C entries.
+#include "cross_entropy.cuh"
+
+namespace ferrum {
+namespace seq {
+namespace {
+
+ferrum_status check_loss(const ferrum_device* dev, const ferrum_cross_entropy_args* a,
+                         const char* what, bool bwd) {
+  if (ferrum_status s = check_args(dev, a, what)) return s;
+  if (a->width < 1) return invalid(what, "width must be at least 1");
+  if (a->vocab < 1) return invalid(what, "vocab must be at least 1");
+  // (rows are numbered by 32 bits in the tensor copies)
+  if (a->tokens > 0x7fffff00 || a->vocab > 0x7fffff00 || a->width > 0x7fffff00)
+    return invalid(what, "tokens, vocab and width must be below 2^31 - 256");
+  if (bounded_product({a->tokens, a->width}) < 0 || bounded_product({a->vocab, a->width}) < 0)
+    return invalid(what, "tokens * width or vocab * width is too large");
+  const size_t e = dtype_size(a->dtype);
+  const bool none = a->tokens == 0;
+  struct {
+    const void* p;
+    size_t align;
+    bool optional;
+    const char* name;
+  } const arrays[] = {
+      {a->x, e, none, "x"},
+      {a->weight, e, false, "weight"},
+      {a->targets, 8, none, "targets"},
+      {a->loss, 4, bwd || none, "loss"},
+      {a->lse, 4, none, "lse"},
+      {a->dloss, 4, true, "dloss"},
+      {a->dlse, 4, true, "dlse"},
+      {a->dx, e, !bwd || none, "dx"},
+      {a->dweight, e, !bwd, "dweight"},
+  };
+  for (const auto& v : arrays)
+    if (ferrum_status s = check_ptr(v.p, v.align, v.optional, what, v.name)) return s;
+  return FERRUM_OK;
+}
+
+}  // namespace
+}  // namespace seq
+}  // namespace ferrum
+
+using namespace ferrum;
+using namespace ferrum::seq;
+
+extern "C" {
+
+ferrum_status ferrum_linear_cross_entropy(ferrum_device* dev, const ferrum_cross_entropy_args* a,
+                                          void* stream) {
+  const char* what = "linear_cross_entropy";
+  return guarded(what, [&]() -> ferrum_status {
+    if (ferrum_status s = check_loss(dev, a, what, false)) return s;
+    if (a->tokens == 0) return FERRUM_OK;
+    DeviceGuard guard(dev->ordinal);
+    if (guard.status() != cudaSuccess) return cuda_error(guard.status(), "cudaSetDevice");
+    launch_detail::clear_stale_error();
+    return loss_fwd_f32(dev, a, (cudaStream_t)stream, what);
+  });
+}
+
+ferrum_status ferrum_linear_cross_entropy_bwd(ferrum_device* dev,
+                                              const ferrum_cross_entropy_args* a, void* stream) {
+  const char* what = "linear_cross_entropy_bwd";
+  return guarded(what, [&]() -> ferrum_status {
+    if (ferrum_status s = check_loss(dev, a, what, true)) return s;
+    DeviceGuard guard(dev->ordinal);
+    if (guard.status() != cudaSuccess) return cuda_error(guard.status(), "cudaSetDevice");
+    cudaStream_t st = (cudaStream_t)stream;
+    if (a->tokens == 0) {      // no gradient of the weights
+      cudaError_t e = cudaMemset2DAsync(a->dweight, (size_t)a->dweight_stride * dtype_size(a->dtype), 0,
+                                        a->width * dtype_size(a->dtype), a->vocab, st);
+      return e == cudaSuccess ? FERRUM_OK : cuda_error(e, what);
+    }
+    launch_detail::clear_stale_error();
+    return loss_bwd_f32(dev, a, st, what);
+  });
+}
+
+}  // extern "C"

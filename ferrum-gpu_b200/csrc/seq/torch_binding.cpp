@@ -9,6 +9,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <pybind11/pybind11.h>
 #include <pybind11/stl.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <algorithm>
@@ -41,6 +42,9 @@ std::string type_name(at::ScalarType t) {
     case at::kFloat: return "float32";
     case at::kHalf: return "float16";
     case at::kBFloat16: return "bfloat16";
+    case at::kDouble: return "float64";
+    case at::kInt: return "int32";
+    case at::kLong: return "int64";
     default: return c10::toString(t);
   }
 }
@@ -700,6 +704,225 @@ Tensor long_conv_step(const Opt& xo, const Opt& history, const Opt& positions, c
   return y;
 }
 
+// ---------------------------------------------------------------- gated recurrence
+
+ferrum_recurrence_args recurrence_args(const Tensor& x, const Opt& ig, const Opt& rg,
+                                       const Opt& decay, const Opt& state, const Opt& lengths,
+                                       const char* state_name) {
+  const bool step = x.dim() == 2;
+  const int64_t b = x.size(0), n = step ? 1 : x.size(1), d = x.size(-1);
+  ferrum_recurrence_args a = {};
+  a.dtype = dtype_of(x), a.batch = b, a.length = n, a.channels = d;
+  a.x = rows(x);
+  a.input_gate = rows(like(ig, x, x.sizes(), "input_gate"));
+  a.recurrence_gate = rows(like(rg, x, x.sizes(), "recurrence_gate"));
+  required(decay, "decay");
+  a.decay = param(decay, x, {d}, "decay");
+  a.initial_state = param(state, x, {b, d}, state_name);
+  a.lengths = param<int32_t>(lengths, x, {b}, "lengths", at::kInt);
+  return a;
+}
+
+int64_t saves(const ferrum_recurrence_args& a) {
+  return ((int64_t)a.length + FERRUM_RECURRENCE_SAVE_STEPS - 1) / FERRUM_RECURRENCE_SAVE_STEPS;
+}
+
+py::tuple gated_recurrence(const Opt& xo, const Opt& ig, const Opt& rg, const Opt& decay,
+                           const Opt& state, const Opt& lengths, bool save, const Opt& out,
+                           const py::object& device, const py::object& stream) {
+  const Tensor& x = activation(xo, "x", 3);
+  auto a = recurrence_args(x, ig, rg, decay, state, lengths, "initial_state");
+  Call c(x, device, stream);
+  Tensor y = output(c, out, x, {{"x", &xo}, {"input_gate", &ig}, {"recurrence_gate", &rg},
+                                {"decay", &decay}, {"initial_state", &state}, {"lengths", &lengths}});
+  const int64_t b = x.size(0), d = x.size(2);
+  Tensor fin = c.empty({b, d}, at::kFloat), saved;
+  if (save) saved = c.empty({b, saves(a), d}, at::kFloat);
+  a.out = rows(y), a.final_state = ptr(fin), a.saved_states = ptr(saved);
+  c.run(ferrum_gated_recurrence, a, {&xo, &ig, &rg, &decay, &state, &lengths, &out});
+  return py::make_tuple(y, fin, to_py(saved));
+}
+
+py::tuple gated_recurrence_backward(const Opt& douto, const Opt& xo, const Opt& ig, const Opt& rg,
+                                    const Opt& decay, const Opt& states, const Opt& lengths,
+                                    const Opt& dfinal, const py::object& device,
+                                    const py::object& stream) {
+  const Tensor& x = activation(xo, "x", 3);
+  auto a = recurrence_args(x, ig, rg, decay, std::nullopt, lengths, "");
+  const Tensor& dout = like(douto, x, x.sizes(), "dout");
+  required(states, "states");
+  const int64_t b = x.size(0), d = x.size(2);
+  a.saved_states = param(states, x, {b, saves(a), d}, "states");
+  a.dfinal_state = param(dfinal, x, {b, d}, "dfinal_state");
+  Call c(x, device, stream);
+  Tensor dx = c.empty_like(x), di = c.empty_like(x), dr = c.empty_like(x);
+  Tensor dd = c.empty({d}, at::kFloat), dinit = c.empty({b, d}, at::kFloat);
+  a.dout = rows(dout), a.dx = rows(dx), a.dinput_gate = rows(di), a.drecurrence_gate = rows(dr);
+  a.ddecay = ptr(dd), a.dinitial_state = ptr(dinit);
+  c.run(ferrum_gated_recurrence_bwd, a,
+        {&douto, &xo, &ig, &rg, &decay, &states, &lengths, &dfinal});
+  return py::make_tuple(dx, di, dr, dd, dinit);
+}
+
+Tensor gated_recurrence_step(const Opt& xo, const Opt& ig, const Opt& rg, const Opt& decay,
+                             const Opt& state, const Opt& next, const Opt& out,
+                             const py::object& device, const py::object& stream) {
+  const Tensor& x = activation(xo, "x", 2);
+  required(state, "state");
+  auto a = recurrence_args(x, ig, rg, decay, state, std::nullopt, "state");
+  a.final_state = given(next) ? param(next, x, {x.size(0), x.size(1)}, "next_state")
+                              : (float*)a.initial_state;
+  apart_states(state, next, {{"x", &xo}, {"input_gate", &ig}, {"recurrence_gate", &rg},
+                             {"decay", &decay}});
+  Call c(x, device, stream);
+  Tensor y = output(c, out, x, {{"x", &xo}, {"input_gate", &ig}, {"recurrence_gate", &rg},
+                                {"decay", &decay}, {"state", &state}, {"next_state", &next}});
+  a.out = rows(y);
+  c.run(ferrum_gated_recurrence_step, a, {&xo, &ig, &rg, &decay, &state, &next, &out});
+  return y;
+}
+
+// ---------------------------------------------------------------- dropout
+
+// Chance, seed (an integer, or one int64 on the device) and offset. `held` keeps
+// a seed tensor for the call's list of what it uses.
+ferrum_dropout_args dropout_args(const Tensor& x, double p, const py::object& seed, int64_t offset,
+                                 Opt& held) {
+  if (!(p >= 0.0 && p <= 1.0)) bad("p must be in [0, 1], got " + std::to_string(p));
+  ferrum_dropout_args a = {};
+  a.p = p, a.offset = (uint64_t)offset;
+  const int64_t d = x.size(-1);
+  a.rows = d ? x.numel() / d : 0, a.channels = d;
+  if (THPVariable_Check(seed.ptr())) {
+    held = THPVariable_Unpack(seed.ptr());
+    const Tensor& t = required(held, "seed");
+    if (t.numel() != 1)
+      bad("seed must be an integer or a tensor of one value, got shape " + dims(t.sizes()));
+    if (t.scalar_type() != at::kLong)
+      bad("seed must be int64, got " + type_name(t.scalar_type()));
+    if (t.device() != x.device())
+      bad("seed is on " + t.device().str() + ", expected " + x.device().str());
+    a.seed_ptr = (const uint64_t*)t.const_data_ptr();
+  } else {
+    PyObject* n = PyNumber_Index(seed.ptr());   // TypeError for what is no integer
+    if (n == nullptr) throw py::error_already_set();
+    a.seed = PyLong_AsUnsignedLongLongMask(n);
+    Py_DECREF(n);
+    if (PyErr_Occurred()) throw py::error_already_set();
+  }
+  return a;
+}
+
+Tensor dropout(const Opt& xo, double p, const py::object& seed, int64_t offset, const Opt& residual,
+               const Opt& out, const py::object& device, const py::object& stream) {
+  const Tensor& x = activation(xo, "x", 0);
+  Opt held;
+  auto a = dropout_args(x, p, seed, offset, held);
+  at::ScalarType rt = x.scalar_type();
+  if (given(residual)) rt = residual_like(residual, x, "residual").scalar_type();
+  a.dtype = dtype_of(x), a.residual_dtype = rt == at::kFloat ? FERRUM_F32 : a.dtype;
+  a.x = x.data_ptr(), a.x_stride = matrix(x, "x").stride;
+  if (given(residual)) {
+    a.residual = residual->data_ptr(), a.residual_stride = matrix(*residual, "residual").stride;
+  }
+  Call c(x, device, stream);
+  Tensor y;
+  if (given(out)) {
+    if (out->scalar_type() != rt)
+      bad("out must be " + type_name(rt) + ", got " + type_name(out->scalar_type()));
+    required(out, "out"), place(*out, x, x.sizes(), "out");
+    y = writable(*out, "out");
+    apart(y, "out", {{"x", &xo}, {"residual", &residual}, {"seed", &held}});
+  } else {
+    y = c.empty(x.sizes(), rt);
+  }
+  a.y = y.data_ptr(), a.y_stride = matrix(y, "out").stride;
+  c.run(ferrum_dropout, a, {&xo, &residual, &held, &out});
+  return y;
+}
+
+Tensor dropout_backward(const Opt& dyo, double p, const py::object& seed, int64_t offset,
+                        const std::optional<at::ScalarType>& dtype, const py::object& device,
+                        const py::object& stream) {
+  const Tensor& dy = activation(dyo, "dy", 0);
+  Opt held;
+  auto a = dropout_args(dy, p, seed, offset, held);
+  const at::ScalarType xt = dtype ? *dtype : dy.scalar_type();
+  if (dy.scalar_type() != at::kFloat && xt != dy.scalar_type())
+    bad("dtype must be " + type_name(dy.scalar_type()) + " (dy's), got " + type_name(xt));
+  a.residual_dtype = dtype_of(dy);
+  a.dtype = xt == at::kFloat ? FERRUM_F32 : xt == at::kHalf ? FERRUM_F16 : FERRUM_BF16;
+  if (xt != at::kFloat && xt != at::kHalf && xt != at::kBFloat16)
+    bad("dtype must be float32, float16 or bfloat16, got " + type_name(xt));
+  Call c(dy, device, stream);
+  Tensor dx = c.empty(dy.sizes(), xt);
+  a.dy = dy.data_ptr(), a.dy_stride = matrix(dy, "dy").stride;
+  a.dx = dx.data_ptr(), a.dx_stride = dy.size(-1);
+  c.run(ferrum_dropout_bwd, a, {&dyo, &held});
+  return dx;
+}
+
+// ---------------------------------------------------------------- loss
+
+ferrum_cross_entropy_args loss_args(const Tensor& x, const Opt& weight, const Opt& targets) {
+  const int64_t d = x.size(-1);
+  const Tensor& w = required(weight, "weight");
+  if (w.dim() != 2 || w.size(0) < 1 || w.size(1) != d || d < 1)
+    bad("weight must be (vocabulary, width) with the width of x, got shapes " + dims(w.sizes()) +
+        " and " + dims(x.sizes()));
+  like(weight, x, w.sizes(), "weight");
+  const Tensor& t = required(targets, "targets");
+  if (t.scalar_type() != at::kLong)
+    bad("targets must be int64, got " + type_name(t.scalar_type()));
+  place(t, x, x.sizes().slice(0, x.dim() - 1), "targets");
+  if (!t.is_contiguous()) bad("targets must be contiguous");
+  ferrum_cross_entropy_args a = {};
+  a.dtype = dtype_of(x), a.tokens = x.numel() / d, a.width = d, a.vocab = w.size(0);
+  a.x = x.data_ptr(), a.x_stride = matrix(x, "x").stride;
+  a.weight = w.data_ptr(), a.weight_stride = matrix(w, "weight").stride;
+  a.targets = t.const_data_ptr<int64_t>();
+  return a;
+}
+
+// float32 of one value a token, contiguous; its pointer
+const float* per_token(const Opt& t, const Tensor& x, const char* what) {
+  if (!given(t)) return nullptr;
+  required(t, what);
+  if (t->scalar_type() != at::kFloat)
+    bad(std::string(what) + " must be float32, got " + type_name(t->scalar_type()));
+  place(*t, x, x.sizes().slice(0, x.dim() - 1), what);
+  if (!t->is_contiguous()) bad(std::string(what) + " must be contiguous");
+  return (const float*)t->const_data_ptr();
+}
+
+py::tuple linear_cross_entropy(const Opt& xo, const Opt& weight, const Opt& targets,
+                               const py::object& device, const py::object& stream) {
+  const Tensor& x = activation(xo, "x", 0);
+  auto a = loss_args(x, weight, targets);
+  Call c(x, device, stream);
+  const auto shape = x.sizes().slice(0, x.dim() - 1);
+  Tensor loss = c.empty(shape, at::kFloat), lse = c.empty(shape, at::kFloat);
+  a.loss = ptr(loss), a.lse = ptr(lse);
+  c.run(ferrum_linear_cross_entropy, a, {&xo, &weight, &targets});
+  return py::make_tuple(loss, lse);
+}
+
+py::tuple linear_cross_entropy_backward(const Opt& dloss, const Opt& xo, const Opt& weight,
+                                        const Opt& targets, const Opt& lse, const Opt& dlse,
+                                        const py::object& device, const py::object& stream) {
+  const Tensor& x = activation(xo, "x", 0);
+  auto a = loss_args(x, weight, targets);
+  required(lse, "lse");
+  a.lse = (float*)per_token(lse, x, "lse");
+  a.dloss = per_token(dloss, x, "dloss"), a.dlse = per_token(dlse, x, "dlse");
+  Call c(x, device, stream);
+  Tensor dx = c.empty_like(x), dw = c.empty_like(*weight);
+  a.dx = dx.data_ptr(), a.dx_stride = x.size(-1);
+  a.dweight = dw.data_ptr(), a.dweight_stride = x.size(-1);
+  c.run(ferrum_linear_cross_entropy_bwd, a, {&dloss, &xo, &weight, &targets, &lse, &dlse});
+  return py::make_tuple(dx, dw);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_sequence, m) {
@@ -716,5 +939,12 @@ PYBIND11_MODULE(_sequence, m) {
   m.def("long_conv", &long_conv);
   m.def("long_conv_backward", &long_conv_backward);
   m.def("long_conv_step", &long_conv_step);
+  m.def("gated_recurrence", &gated_recurrence);
+  m.def("gated_recurrence_backward", &gated_recurrence_backward);
+  m.def("gated_recurrence_step", &gated_recurrence_step);
+  m.def("dropout", &dropout);
+  m.def("dropout_backward", &dropout_backward);
+  m.def("linear_cross_entropy", &linear_cross_entropy);
+  m.def("linear_cross_entropy_backward", &linear_cross_entropy_backward);
   m.def("_shares_memory", &Overlap::of);
 }

@@ -86,7 +86,8 @@ class Rows(ctypes.Structure):
 
 def _fields(spec: str):
     """Struct fields from "type name name; type name" text."""
-    kinds = {"size": _sz, "int": _i, "i64": ctypes.c_int64, "ptr": _vp, "rows": Rows, "float": ctypes.c_float}
+    kinds = {"size": _sz, "int": _i, "i64": ctypes.c_int64, "ptr": _vp, "rows": Rows, "float": ctypes.c_float,
+             "double": ctypes.c_double, "u64": ctypes.c_uint64}
     out = []
     for part in spec.split(";"):
         words = part.split()
@@ -125,6 +126,26 @@ class LongArgs(ctypes.Structure):
                        "i64 dy_step dx_step; ptr dkernel dskip; rows history; ptr positions")
 
 
+class RecurrenceArgs(ctypes.Structure):
+    _fields_ = _fields("size struct_size; int dtype; size batch length channels;"
+                       "rows x input_gate recurrence_gate out;"
+                       "ptr decay initial_state final_state lengths saved_states;"
+                       "rows dout dx dinput_gate drecurrence_gate;"
+                       "ptr dfinal_state ddecay dinitial_state")
+
+
+class DropoutArgs(ctypes.Structure):
+    _fields_ = _fields("size struct_size; int dtype residual_dtype; size rows channels; double p;"
+                       "u64 seed offset; ptr seed_ptr x residual y;"
+                       "i64 x_stride residual_stride y_stride; ptr dy dx; i64 dy_stride dx_stride")
+
+
+class CrossEntropyArgs(ctypes.Structure):
+    _fields_ = _fields("size struct_size; int dtype; size tokens width vocab; ptr x weight;"
+                       "i64 x_stride weight_stride; ptr targets loss lse dloss dlse dx dweight;"
+                       "i64 dx_stride dweight_stride")
+
+
 # Sequence operators: entry point -> argument block; each is called with the
 # device handle, a pointer to its block and the stream.
 SEQ_SIGNATURES = {
@@ -141,6 +162,13 @@ SEQ_SIGNATURES = {
     "ferrum_long_conv": LongArgs,
     "ferrum_long_conv_bwd": LongArgs,
     "ferrum_long_conv_step": LongArgs,
+    "ferrum_gated_recurrence": RecurrenceArgs,
+    "ferrum_gated_recurrence_bwd": RecurrenceArgs,
+    "ferrum_gated_recurrence_step": RecurrenceArgs,
+    "ferrum_dropout": DropoutArgs,
+    "ferrum_dropout_bwd": DropoutArgs,
+    "ferrum_linear_cross_entropy": CrossEntropyArgs,
+    "ferrum_linear_cross_entropy_bwd": CrossEntropyArgs,
 }
 
 

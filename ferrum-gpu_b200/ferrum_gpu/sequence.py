@@ -1,4 +1,5 @@
-"""Sequence operators on torch CUDA tensors: causal filters and block norms.
+"""Sequence operators on torch CUDA tensors: causal filters, block norms, dropout
+and the loss.
 
 What a sequence model runs next to the FFT, without a counterpart in the
 reference:
@@ -6,8 +7,11 @@ reference:
 ``causal_conv1d``   short depthwise convolution (1 to 8 taps), bias, SiLU
 ``selective_scan``  input-dependent linear recurrence (state space scan)
 ``long_conv``       convolution with a filter as long as the sequence, by FFT
+``gated_recurrence``      linear recurrence of one state a channel, by gates
 ``norm_before``     residual update and norm in front of a block
 ``norm_after``      gated norm behind a block, scaled onto the residual
+``dropout``         onto the residual, from a counter-based generator
+``linear_cross_entropy``  softmax loss against a vocabulary, logits never kept
 
 The calls are not recorded by autograd: a result does not require a gradient,
 whatever its arguments do. Each operator has a ``*_backward`` instead, to be
@@ -72,6 +76,11 @@ _OTHERS = {
     "kind": ("a string", lambda v: isinstance(v, str)),
     "eps": ("a number", lambda v: hasattr(v, "__float__") and not isinstance(v, str)),
     "groups": ("an integer", lambda v: hasattr(v, "__index__")),
+    "p": ("a number", lambda v: hasattr(v, "__float__") and not isinstance(v, str)),
+    "seed": ("an integer or an int64 CUDA tensor",
+             lambda v: hasattr(v, "__index__") or hasattr(v, "__dlpack_device__")),
+    "offset": ("an integer", lambda v: hasattr(v, "__index__")),
+    "dtype": ("a torch.dtype", lambda v: v is None or isinstance(v, torch.dtype)),
     "device": ("a ferrum_gpu.cuda.Device", lambda v: True),      # looked at by the call
     "stream": ("a stream", lambda v: True),
     **{name: ("a truth value", lambda v: hasattr(v, "__bool__"))
@@ -310,8 +319,123 @@ def long_conv_step(x, history, positions, kernel, skip=None, *, out=None, device
     return _call(_sequence.long_conv_step, x, history, positions, kernel, skip, out, device, stream)
 
 
+# ---------------------------------------------------------------- gated recurrence
+
+class RecurrenceResult(NamedTuple):
+    out: torch.Tensor
+    final_state: torch.Tensor
+    states: Optional[torch.Tensor]
+
+
+class RecurrenceGrads(NamedTuple):
+    dx: torch.Tensor
+    dinput_gate: torch.Tensor
+    drecurrence_gate: torch.Tensor
+    ddecay: torch.Tensor
+    dinitial_state: torch.Tensor
+
+
+def gated_recurrence(x, input_gate, recurrence_gate, decay, *, initial_state=None, lengths=None,
+                     save_states=False, out=None, device=None, stream=None) -> RecurrenceResult:
+    """A linear recurrence of one state per channel, with gates from their logits:
+
+        a = exp(-decay sigmoid(recurrence_gate))
+        h = a h + sqrt(1 - a^2) sigmoid(input_gate) x,   out = h
+
+    x, input_gate, recurrence_gate: (batch, length, channels). decay:
+    (channels), not negative: a channel forgets at most by exp(-decay) a step.
+    initial_state: (batch, channels) float32. With ``save_states`` the result
+    carries what the backward needs. Where 1 - a^2 is not above 0, the root and
+    the gradient through it are 0.
+    """
+    return RecurrenceResult(*_call(
+        _sequence.gated_recurrence, x, input_gate, recurrence_gate, decay, initial_state, lengths,
+        save_states, out, device, stream))
+
+
+def gated_recurrence_backward(dout, x, input_gate, recurrence_gate, decay, states, *, lengths=None,
+                              dfinal_state=None, device=None, stream=None) -> RecurrenceGrads:
+    """Gradients of ``gated_recurrence`` for its output's gradient ``dout`` (and
+    that of its final state). ``states`` comes from the forward call with
+    ``save_states``."""
+    return RecurrenceGrads(*_call(
+        _sequence.gated_recurrence_backward, dout, x, input_gate, recurrence_gate, decay, states,
+        lengths, dfinal_state, device, stream))
+
+
+def gated_recurrence_step(x, input_gate, recurrence_gate, decay, state, *, next_state=None,
+                          out=None, device=None, stream=None):
+    """One step of every sequence. x, input_gate, recurrence_gate: (batch,
+    channels); state: (batch, channels) float32, updated in place unless
+    ``next_state`` takes the state after the step. Returns out (batch,
+    channels)."""
+    return _call(
+        _sequence.gated_recurrence_step, x, input_gate, recurrence_gate, decay, state, next_state,
+        out, device, stream)
+
+
+# ---------------------------------------------------------------- dropout
+
+def dropout(x, p, seed, *, offset=0, residual=None, out=None, device=None, stream=None):
+    """residual + (keep ? x / (1 - p) : 0), of residual's type (x's without one).
+
+    x: (..., channels); residual: same shape, float32 or x's type. p in [0,
+    1] is the chance that a value is dropped. The mask is a function of
+    ``seed``, ``offset`` and an element's index in x's shape (whatever the
+    strides), drawn from Philox4x32-10 and never stored. ``seed`` is an integer
+    or an int64 CUDA tensor of one value, read when the call runs: a captured
+    graph draws another mask once that value changes. Calls that share a seed
+    draw other masks by another ``offset``.
+    """
+    return _call(_sequence.dropout, x, p, seed, offset, residual, out, device, stream)
+
+
+def dropout_backward(dy, p, seed, *, offset=0, dtype=None, device=None, stream=None):
+    """The gradient of ``dropout``'s x, for the same p, seed and offset. dy may
+    be float32 and ``dtype`` (dy's if None) that of x. The gradient of residual
+    is dy."""
+    return _call(_sequence.dropout_backward, dy, p, seed, offset, dtype, device, stream)
+
+
+# ---------------------------------------------------------------- loss
+
+class CrossEntropyResult(NamedTuple):
+    loss: torch.Tensor
+    lse: torch.Tensor
+
+
+class CrossEntropyGrads(NamedTuple):
+    dx: torch.Tensor
+    dweight: torch.Tensor
+
+
+def linear_cross_entropy(x, weight, targets, *, device=None, stream=None) -> CrossEntropyResult:
+    """lse[t] = log sum_v exp(x[t] . weight[v]);  loss[t] = lse[t] - x[t] . weight[target[t]].
+
+    x: (..., width); weight: (vocabulary, width) of x's type; targets: int64 of
+    x's leading shape. loss and lse are float32 of that shape. The logits are
+    never kept: a piece at a time lives on chip. A row whose target lies outside
+    the vocabulary (-100, say) has no loss: its loss, lse and gradients are 0,
+    whatever its values.
+    """
+    return CrossEntropyResult(*_call(_sequence.linear_cross_entropy, x, weight, targets, device, stream))
+
+
+def linear_cross_entropy_backward(dloss, x, weight, targets, lse, *, dlse=None, device=None,
+                                  stream=None) -> CrossEntropyGrads:
+    """Gradients of ``linear_cross_entropy`` for those of loss (``dloss``) and
+    of lse (``dlse``), float32. ``lse`` is the forward's. The logits are computed
+    again, a piece of the vocabulary at a time. dx and dweight have x's type."""
+    return CrossEntropyGrads(*_call(
+        _sequence.linear_cross_entropy_backward, dloss, x, weight, targets, lse, dlse, device,
+        stream))
+
+
 __all__ = ["causal_conv1d", "causal_conv1d_backward", "causal_conv1d_step", "selective_scan",
            "selective_scan_backward", "selective_scan_step", "norm_before", "norm_before_backward",
            "norm_after", "norm_after_backward", "long_conv", "long_conv_backward",
            "long_conv_step", "ConvGrads", "ScanResult", "ScanGrads", "NormBeforeGrads",
-           "NormAfterGrads", "LongGrads"]
+           "NormAfterGrads", "LongGrads", "gated_recurrence", "gated_recurrence_backward",
+           "gated_recurrence_step", "dropout", "dropout_backward", "linear_cross_entropy",
+           "linear_cross_entropy_backward", "RecurrenceResult", "RecurrenceGrads",
+           "CrossEntropyResult", "CrossEntropyGrads"]

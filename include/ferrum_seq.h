@@ -1,8 +1,9 @@
 /*
  * ferrum_seq.h — C ABI of the sequence operators: causal filters along a
  * sequence (short convolution, long convolution through the FFT, selective
- * state space scan) and the norms around a sequence block. They have no
- * counterpart in the reference; they follow the conventions of ferrum_fft.h:
+ * state space scan, gated recurrence), the norms around a sequence block,
+ * dropout, and the loss against a vocabulary. They have no counterpart in
+ * the reference; they follow the conventions of ferrum_fft.h:
  * plain pointers and sizes, a status code, ferrum_last_error() for the
  * message, device memory on the handle's device, calls asynchronous on
  * `stream`, workspaces from the device's stream-ordered pool.
@@ -39,6 +40,8 @@ enum { FERRUM_NORM_RMS = 0, FERRUM_NORM_LAYER = 1 };
 #define FERRUM_SCAN_MAX_STATES 64
 /* Steps between the states the scan saves for its gradient. */
 #define FERRUM_SCAN_SAVE_STEPS 16
+/* Steps between the states the recurrence saves for its gradient. */
+#define FERRUM_RECURRENCE_SAVE_STEPS 16
 /* Longest sequence of the long convolution. */
 #define FERRUM_LONG_CONV_MAX_LENGTH (1 << 25)
 
@@ -194,6 +197,99 @@ ferrum_status ferrum_long_conv_bwd(ferrum_device *dev, const ferrum_long_conv_ar
                                    void *stream);
 ferrum_status ferrum_long_conv_step(ferrum_device *dev, const ferrum_long_conv_args *args,
                                     void *stream);
+
+/* ---------------------------------------------------------------------------
+ * Gated linear recurrence, one state per channel:
+ *   a = exp(-decay[d] * sigmoid(recurrence_gate[b,t,d]))
+ *   h = a * h + sqrt(1 - a^2) * sigmoid(input_gate[b,t,d]) * x[b,t,d];  out = h
+ * decay is not negative; where 1 - a^2 is not above 0 (or below 2^-126), the
+ * root and the gradient through it are 0.
+ */
+typedef struct {
+  size_t struct_size;
+  int dtype;
+  size_t batch, length, channels;
+  ferrum_rows x, input_gate, recurrence_gate, out;
+  const float *decay;                       /* (channels) */
+  const float *initial_state;               /* (batch, channels), optional (zeros) */
+  float *final_state;                       /* (batch, channels), optional */
+  const int32_t *lengths;
+  /* (batch, ceil(length / 16), channels): the state in front of every 16th
+   * step. Optional output of the recurrence, needed by its gradient. */
+  float *saved_states;
+  /* gradients (ferrum_gated_recurrence_bwd) */
+  ferrum_rows dout, dx, dinput_gate, drecurrence_gate;
+  const float *dfinal_state;                /* optional */
+  float *ddecay;
+  float *dinitial_state;                    /* optional */
+} ferrum_recurrence_args;
+
+ferrum_status ferrum_gated_recurrence(ferrum_device *dev, const ferrum_recurrence_args *args,
+                                      void *stream);
+ferrum_status ferrum_gated_recurrence_bwd(ferrum_device *dev, const ferrum_recurrence_args *args,
+                                          void *stream);
+/* One step of every sequence (length 1, no lengths): initial_state (required)
+ * before, final_state (required, may be the same array) after. */
+ferrum_status ferrum_gated_recurrence_step(ferrum_device *dev, const ferrum_recurrence_args *args,
+                                           void *stream);
+
+/* ---------------------------------------------------------------------------
+ * Dropout, over rows of `channels` values (strides in elements, values
+ * contiguous):
+ *   y = residual + (keep ? x / (1 - p) : 0)     (residual optional)
+ * Element i = row * channels + channel is kept where word i % 4 of
+ * Philox4x32-10 (Salmon et al., "Parallel random numbers: as easy as 1, 2,
+ * 3", SC 2011), with the counter (i / 4, offset) and the key seed, each 64 bits
+ * in two words, low word first, is not below p * 2^32. No mask is stored: the
+ * gradient draws the same words. y and residual have type residual_dtype
+ * (float32 or dtype).
+ */
+typedef struct {
+  size_t struct_size;
+  int dtype, residual_dtype;
+  size_t rows, channels;
+  double p;                             /* in [0, 1]; 1 keeps nothing */
+  uint64_t seed, offset;
+  const uint64_t *seed_ptr;             /* on the device, instead of seed; optional */
+  const void *x, *residual;
+  void *y;
+  int64_t x_stride, residual_stride, y_stride;
+  /* gradients: dx (type dtype) from dy (type residual_dtype) */
+  const void *dy;
+  void *dx;
+  int64_t dy_stride, dx_stride;
+} ferrum_dropout_args;
+
+ferrum_status ferrum_dropout(ferrum_device *dev, const ferrum_dropout_args *args, void *stream);
+/* The gradient of x; that of residual is dy. */
+ferrum_status ferrum_dropout_bwd(ferrum_device *dev, const ferrum_dropout_args *args, void *stream);
+
+/* ---------------------------------------------------------------------------
+ * Softmax cross entropy of rows against a vocabulary matrix:
+ *   l[t,v] = sum_d x[t,d] * weight[v,d]
+ *   lse[t] = log(sum_v exp(l[t,v]));  loss[t] = lse[t] - l[t, target[t]]
+ * x, weight, dx and dweight have type `dtype`. The logits are never stored as
+ * a whole. A row whose target lies outside [0, vocab) has no loss: its loss, lse
+ * and gradients are 0, whatever its values.
+ */
+typedef struct {
+  size_t struct_size;
+  int dtype;
+  size_t tokens, width, vocab;
+  const void *x, *weight;               /* (tokens, width), (vocab, width) */
+  int64_t x_stride, weight_stride;      /* of rows, in elements */
+  const int64_t *targets;               /* (tokens) */
+  float *loss, *lse;                    /* (tokens); lse is an input of the gradient */
+  /* gradients */
+  const float *dloss, *dlse;            /* (tokens); each optional */
+  void *dx, *dweight;
+  int64_t dx_stride, dweight_stride;
+} ferrum_cross_entropy_args;
+
+ferrum_status ferrum_linear_cross_entropy(ferrum_device *dev, const ferrum_cross_entropy_args *args,
+                                          void *stream);
+ferrum_status ferrum_linear_cross_entropy_bwd(ferrum_device *dev,
+                                              const ferrum_cross_entropy_args *args, void *stream);
 
 #ifdef __cplusplus
 }
