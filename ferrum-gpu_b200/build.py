@@ -48,7 +48,7 @@ CU_SOURCES = ["launch_rows.cu", "launch_pass.cu", "launch_misc.cu", "launch_tile
 # Sequence operators (include/ferrum_seq.h).
 SEQ_SOURCES = ["seq_common.cu", "conv1d.cu", "scan_fwd.cu", "scan_bwd.cu", "norm.cu",
                "long_conv.cu", "recurrence.cu", "dropout.cu", "cross_entropy.cu",
-               "cross_entropy_f32.cu"]
+               "cross_entropy_f32.cu", "cross_entropy_tc.cu"]
 LIB = os.path.join(PKG, "libferrum_fft.so")
 EXT = os.path.join(PKG, "_native" + sysconfig.get_config_var("EXT_SUFFIX"))
 SEQ_EXT = os.path.join(PKG, "_sequence" + sysconfig.get_config_var("EXT_SUFFIX"))

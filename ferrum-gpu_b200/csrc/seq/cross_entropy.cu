@@ -56,7 +56,8 @@ ferrum_status ferrum_linear_cross_entropy(ferrum_device* dev, const ferrum_cross
     DeviceGuard guard(dev->ordinal);
     if (guard.status() != cudaSuccess) return cuda_error(guard.status(), "cudaSetDevice");
     launch_detail::clear_stale_error();
-    return loss_fwd_f32(dev, a, (cudaStream_t)stream, what);
+    return a->dtype == FERRUM_F32 ? loss_fwd_f32(dev, a, (cudaStream_t)stream, what)
+                                  : loss_fwd_tc(dev, a, (cudaStream_t)stream, what);
   });
 }
 
@@ -74,7 +75,7 @@ ferrum_status ferrum_linear_cross_entropy_bwd(ferrum_device* dev,
       return e == cudaSuccess ? FERRUM_OK : cuda_error(e, what);
     }
     launch_detail::clear_stale_error();
-    return loss_bwd_f32(dev, a, st, what);
+    return a->dtype == FERRUM_F32 ? loss_bwd_f32(dev, a, st, what) : loss_bwd_tc(dev, a, st, what);
   });
 }
 

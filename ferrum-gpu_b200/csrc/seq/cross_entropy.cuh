@@ -37,6 +37,10 @@ ferrum_status loss_fwd_f32(ferrum_device* dev, const ferrum_cross_entropy_args* 
                            cudaStream_t stream, const char* what);
 ferrum_status loss_bwd_f32(ferrum_device* dev, const ferrum_cross_entropy_args* a,
                            cudaStream_t stream, const char* what);
+ferrum_status loss_fwd_tc(ferrum_device* dev, const ferrum_cross_entropy_args* a,
+                          cudaStream_t stream, const char* what);
+ferrum_status loss_bwd_tc(ferrum_device* dev, const ferrum_cross_entropy_args* a,
+                          cudaStream_t stream, const char* what);
 
 }  // namespace seq
 }  // namespace ferrum
