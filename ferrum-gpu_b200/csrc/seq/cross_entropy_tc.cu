@@ -1,7 +1,7 @@
 // The loss against a vocabulary on the tensor cores, for 16-bit types.
 //
-// Four products share one kernel, which differ in where their operands lie and
-// in what becomes of a finished tile (T tokens, D width, V vocabulary):
+// Four products share one kernel; they differ in where their operands lie and in
+// what becomes of a finished tile (T tokens, D width, V vocabulary):
 //   stats   x W^T  (T x V over D):  each row's largest logit and sum of exponentials
 //                                   over the tile's columns, and its target's logit
 //   grads   x W^T again:            G = (dloss + dlse) softmax - dloss onehot, to 16 bits
@@ -16,8 +16,9 @@
 // A pair of CTAs computes a tile of 256 x 256: each stages 128 rows of A and of B
 // (32 KiB a step of 64) by TMA, one thread of the leader issues 256 x 256 x 16
 // products whose accumulators lie in both CTAs' TMEM, 128 rows each. There are two
-// sets of accumulators (all 512 columns), so that four warps finish one tile while
-// the next is computed. 74 pairs walk the tiles.
+// sets of accumulators (all 512 columns), so that eight warps finish one tile while
+// the next is computed. 74 pairs walk the tiles; dx and dW of a piece share a launch,
+// so that the last wave of one is filled by the other.
 #include <cudaTypedefs.h>
 
 #include <algorithm>
@@ -67,11 +68,14 @@ namespace {
 constexpr int kTile = 256, kHalf = 128, kDepth = 64, kStages = 6;
 constexpr int kOperandBytes = kHalf * kDepth * 2;             // of one CTA and step
 constexpr int kStageBytes = 2 * kOperandBytes;
-constexpr int kThreads = 256, kEpilogueWarp = 4;
-constexpr int kSmemBytes = kStages * kStageBytes + 1024;      // and room to align
+constexpr int kEpilogueWarp = 4, kEpilogueWarps = 8;
+constexpr int kThreads = 32 * (kEpilogueWarp + kEpilogueWarps);
+constexpr int kSlotBytes = 32 * 128;                          // a warp's rows on their way out
+// and 1024 bytes of room to align
+constexpr int kSmemBytes = kStages * kStageBytes + kEpilogueWarps * kSlotBytes + 1024;
 constexpr int kGroup = 16;                                    // tiles of M that share a tile of N
 
-enum Kind { kStats, kGrads, kDx, kDw };
+enum Kind { kStats, kGrads, kWeights };
 
 // What a row needs to turn its logits into G: scaled gradients of its logits'
 // sum and of its loss, lse in units of ln 2, and its target (-1 without a loss).
@@ -80,30 +84,49 @@ struct RowCoef {
   int target;
 };
 
+// One product A B^T of the extents m x n over `steps` steps of depth.
 struct Product {
-  int64_t m, n;              // extents of the result
+  int64_t m, n;
   int tiles_m, tiles_n, splits, steps, steps_per_split;
+  bool a_mn, b_mn;           // operands whose rows run along the depth
+  bool sums;                 // the result: float32 sums, a slab per split (else 16 bits)
+  bool load, store_map;      // sums of earlier pieces come on top; `out` has a tensor map
+  void* out;
+  float* partial;            // float32 sums, rows of partial_ld
+  int64_t ld, partial_ld;
+};
+
+struct Work {
+  Product p[2];              // one after the other
+  int count;
   int* err_flag;
   // stats
   const int64_t* targets;
-  RowStat* stats;            // (tile of N, m)
+  RowStat* stats;            // (half tile of N, m)
   float* at_target;
   // grads
   const RowCoef* rows;
   int64_t first;             // the piece's first word
-  // grads: G; dx: the float32 sums (a slab per split); dW: dweight
-  void* out;
-  int64_t ld;
-  bool add;
   const float* scale;        // {2^s, 2^-s}
 };
 
-struct Place {
-  int tm, tn, split;
+struct Maps {
+  CUtensorMap a, b, out;
 };
-__device__ __forceinline__ Place place_of(const Product& p, int64_t t) {
-  const int64_t per = (int64_t)p.tiles_m * p.tiles_n;
+
+struct Place {
+  int product, tm, tn, split;
+};
+__device__ __forceinline__ int64_t tiles_of(const Product& p) {
+  return (int64_t)p.tiles_m * p.tiles_n * p.splits;
+}
+template <int KIND>
+__device__ __forceinline__ Place place_of(const Work& w, int64_t t) {
   Place q;
+  q.product = 0;
+  if (KIND == kWeights && t >= tiles_of(w.p[0])) q.product = 1, t -= tiles_of(w.p[0]);
+  const Product& p = w.p[q.product];
+  const int64_t per = (int64_t)p.tiles_m * p.tiles_n;
   q.split = (int)(t / per);
   t %= per;
   const int64_t group = t / ((int64_t)kGroup * p.tiles_n);
@@ -136,17 +159,18 @@ __device__ __forceinline__ bool wait(Shared* sh, uint64_t* bar, uint32_t phase, 
 }
 
 // ---------------------------------------------------------------- epilogues
-// One warp: rows m0 + lane, columns n0 .. n0 + 255 of a tile at TMEM address `acc`.
+// One warp: row m (its lane's), 128 columns from n0 on, at TMEM address `acc`.
 
-__device__ void finish_stats(const Product& p, uint32_t acc, int64_t m, int64_t n0, int tn) {
+__device__ void finish_stats(const Work& w, uint32_t acc, int64_t m, int64_t n0) {
+  const Product& p = w.p[0];
   const bool row = m < p.m;
-  const int64_t target = row ? p.targets[m] : -1;
-  const int at = target >= n0 && target < n0 + kTile && target < p.n ? (int)(target - n0) : -1;
-  const int cols = p.n - n0 < kTile ? (int)(p.n - n0) : kTile;
+  const int64_t target = row ? w.targets[m] : -1;
+  const int at = target >= n0 && target < n0 + kHalf && target < p.n ? (int)(target - n0) : -1;
+  const int cols = p.n - n0 < kHalf ? (int)(p.n - n0) : kHalf;      // (may be below 0)
   RowStat s = {-INFINITY, 0.f};
   float hit = 0.f;
 #pragma unroll 1
-  for (int c = 0; c < kTile; c += 32) {
+  for (int c = 0; c < kHalf; c += 32) {
     if (c >= cols) break;
     float v[32];
     tmem_load32(acc + c, v);
@@ -160,124 +184,147 @@ __device__ void finish_stats(const Product& p, uint32_t acc, int64_t m, int64_t 
 #pragma unroll
       for (int i = 0; i < 32; ++i) hit += at - c == i ? v[i] : 0.f;
     }
-    float top = v[0];
+    float t4[4] = {s.top, s.top, s.top, s.top};
 #pragma unroll
-    for (int i = 1; i < 32; ++i) top = fmaxf(top, v[i]);
-    top = fmaxf(top, s.top);
+    for (int i = 0; i < 32; ++i) t4[i % 4] = fmaxf(t4[i % 4], v[i]);
+    const float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
     const float k = shift_of(top) * kLog2e;
-    float sum = s.top == -INFINITY ? s.sum : s.sum * ex2(fmaf(shift_of(s.top), kLog2e, -k));
+    float s4[4] = {s.top == -INFINITY ? s.sum : s.sum * ex2(fmaf(shift_of(s.top), kLog2e, -k)), 0.f,
+                   0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < 32; ++i) sum += ex2(fmaf(v[i], kLog2e, -k));
-    s.top = top, s.sum = sum;
+    for (int i = 0; i < 32; ++i) s4[i % 4] += ex2(fmaf(v[i], kLog2e, -k));
+    s.top = top, s.sum = (s4[0] + s4[1]) + (s4[2] + s4[3]);
   }
-  if (!row) return;
-  p.stats[(int64_t)tn * p.m + m] = s;
-  if (at >= 0) p.at_target[m] = hit;
+  if (!row || cols <= 0) return;
+  w.stats[n0 / kHalf * p.m + m] = s;
+  if (at >= 0) w.at_target[m] = hit;
+}
+
+// A warp's 32 rows of 64 values, on their way out through its slot of shared
+// memory: rows of 128 bytes, swizzled as the tensor map has them, or single values
+// where the array has no map.
+template <class T>
+__device__ __forceinline__ void put_rows(const Product& p, const CUtensorMap* map, uint8_t* slot,
+                                         const float (&v)[2][32], int64_t m0, int64_t n0, int lane) {
+  // the store that read the slot before is done with it
+  if (lane == 0) bulk_wait_read_all();
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    uint4 q;
+    const float* u = &v[j / 4][j % 4 * 8];
+    q.x = pack_pair<T>(u[0], u[1]), q.y = pack_pair<T>(u[2], u[3]);
+    q.z = pack_pair<T>(u[4], u[5]), q.w = pack_pair<T>(u[6], u[7]);
+    *(uint4*)(slot + lane * 128 + ((j ^ (lane & 7)) * 16)) = q;
+  }
+  if (p.store_map) {
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0 && m0 < p.m && n0 < p.n) {
+      tma_store_tile2d(map, (int32_t)n0, (int32_t)m0, slot);
+      bulk_commit();
+    }
+  } else {
+    __syncwarp();
+    for (int r = 0; r < 32 && m0 + r < p.m; ++r) {
+      T* out = (T*)p.out + (m0 + r) * p.ld + n0;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int c = h * 32 + lane;
+        if (n0 + c < p.n) out[c] = *(const T*)(slot + r * 128 + (((c / 8) ^ (r & 7)) * 16) + c % 8 * 2);
+      }
+    }
+    __syncwarp();
+  }
 }
 
 template <class T>
-__device__ void finish_grads(const Product& p, uint32_t acc, int64_t m, int64_t n0) {
-  const bool row = m < p.m;
+__device__ void finish_grads(const Work& w, const CUtensorMap* map, uint8_t* slot, uint32_t acc,
+                             int64_t m0, int64_t n0, int lane) {
+  const Product& p = w.p[0];
   RowCoef q = {0.f, 0.f, 0.f, -1};
-  if (row) q = p.rows[m];
-  const int64_t at64 = (int64_t)q.target - p.first - n0;
-  const int at = q.target >= 0 && at64 >= 0 && at64 < kTile ? (int)at64 : -1;
-  T* out = (T*)p.out + m * p.ld + n0;
+  if (m0 + lane < p.m) q = w.rows[m0 + lane];
+  const int64_t at64 = (int64_t)q.target - w.first - n0;
+  const int at = q.target >= 0 && at64 >= 0 && at64 < kHalf ? (int)at64 : -1;
 #pragma unroll 1
-  for (int c = 0; c < kTile; c += 32) {
-    if (n0 + c >= p.ld) break;          // (ld is a multiple of 32)
-    float v[32];
-    tmem_load32(acc + c, v);
-    tmem_load_wait();
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = q.target < 0 ? 0.f : ex2(fmaf(v[i], kLog2e, -q.lse2)) * q.all;
-    if (at >= c && at < c + 32) {
-#pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] -= at - c == i ? q.one : 0.f;
-    }
-    if (row) {
-#pragma unroll
-      for (int i = 0; i < 32; i += 8) {
-        float w[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) w[j] = v[i + j];
-        store_vec<T, 8>(out + c + i, w);
-      }
-    }
-  }
-}
-
-__device__ void finish_dx(const Product& p, uint32_t acc, int64_t m, int64_t n0, int split) {
-  float* out = (float*)p.out + ((int64_t)split * p.m + m) * p.ld + n0;
-#pragma unroll 1
-  for (int c = 0; c < kTile; c += 32) {
-    float v[32];
-    tmem_load32(acc + c, v);
-    tmem_load_wait();
-    if (m >= p.m) continue;
-#pragma unroll
-    for (int i = 0; i < 32; i += 4) {
-      if (n0 + c + i >= p.ld) continue;    // (ld is a multiple of 8)
-      float4* o = (float4*)(out + c + i);
-      float4 w = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-      if (p.add) {
-        const float4 b = *o;
-        w.x += b.x, w.y += b.y, w.z += b.z, w.w += b.w;
-      }
-      *o = w;
-    }
-  }
-}
-
-template <class T>
-__device__ void finish_dw(const Product& p, uint32_t acc, int64_t m, int64_t n0) {
-  const float inv = p.scale[1];
-  T* out = (T*)p.out + m * p.ld + n0;
-  const bool wide = p.ld % 8 == 0 && (uintptr_t)p.out % 16 == 0;
-#pragma unroll 1
-  for (int c = 0; c < kTile; c += 32) {
+  for (int c = 0; c < kHalf; c += 64) {
     if (n0 + c >= p.n) break;
-    float v[32];
-    tmem_load32(acc + c, v);
+    float v[2][32];
+    tmem_load32(acc + c, v[0]);
+    tmem_load32(acc + c + 32, v[1]);
     tmem_load_wait();
-    if (m >= p.m) continue;
 #pragma unroll
-    for (int i = 0; i < 32; i += 8) {
-      float w[8];
+    for (int h = 0; h < 2; ++h) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = v[i + j] * inv;
-      const int64_t left = p.n - (n0 + c + i);
-      if (wide && left >= 8) {
-        store_vec<T, 8>(out + c + i, w);
-      } else {
+      for (int i = 0; i < 32; ++i)
+        v[h][i] = q.target < 0 ? 0.f : ex2(fmaf(v[h][i], kLog2e, -q.lse2)) * q.all;
+      if (at >= c + h * 32 && at < c + h * 32 + 32) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (j < left) out[c + i + j] = from_f<T>(w[j]);
+        for (int i = 0; i < 32; ++i) v[h][i] -= at - c - h * 32 == i ? q.one : 0.f;
       }
+    }
+    put_rows<T>(p, map, slot, v, m0, n0 + c, lane);
+  }
+}
+
+// Sums into `partial`, or with them, scaled back, to 16 bits.
+template <class T>
+__device__ void finish_weights(const Work& w, const Product& p, const CUtensorMap* map, uint8_t* slot,
+                               uint32_t acc, int64_t m0, int64_t n0, int split, int lane) {
+  const float inv = w.scale[1];
+  const int64_t m = m0 + lane;
+  float* part = p.partial ? p.partial + ((int64_t)split * p.m + m) * p.partial_ld + n0 : nullptr;
+#pragma unroll 1
+  for (int c = 0; c < kHalf; c += 64) {
+    if (n0 + c >= p.n) break;
+    float v[2][32];
+    tmem_load32(acc + c, v[0]);
+    tmem_load32(acc + c + 32, v[1]);
+    tmem_load_wait();
+    if (p.load && m < p.m) {
+#pragma unroll
+      for (int i = 0; i < 64; i += 4) {
+        if (n0 + c + i >= p.partial_ld) continue;    // (a multiple of 8)
+        const float4 b = *(const float4*)(part + c + i);
+        float* u = &v[i / 32][i % 32];
+        u[0] += b.x, u[1] += b.y, u[2] += b.z, u[3] += b.w;
+      }
+    }
+    if (p.sums) {
+      if (m >= p.m) continue;
+#pragma unroll
+      for (int i = 0; i < 64; i += 4) {
+        if (n0 + c + i >= p.partial_ld) continue;
+        const float* u = &v[i / 32][i % 32];
+        *(float4*)(part + c + i) = make_float4(u[0], u[1], u[2], u[3]);
+      }
+    } else {
+      // (a row without a loss has a zero in G, but W may hold infinities)
+      const bool keep = p.a_mn || (m < p.m && w.rows[m].target >= 0);
+#pragma unroll
+      for (int i = 0; i < 64; ++i) v[i / 32][i % 32] = keep ? v[i / 32][i % 32] * inv : 0.f;
+      put_rows<T>(p, map, slot, v, m0, n0 + c, lane);
     }
   }
 }
 
 // ---------------------------------------------------------------- the kernel
-// A is K-major (rows of the depth) in all products but dW's; B in stats and grads.
 template <class T, int KIND>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-loss_product_kernel(const __grid_constant__ CUtensorMap map_a,
-                    const __grid_constant__ CUtensorMap map_b, Product p) {
-  constexpr bool A_MN = KIND == kDw, B_MN = KIND == kDx || KIND == kDw;
-  constexpr uint32_t kIdesc = instruction_desc<T, A_MN, B_MN>(kTile, kTile);
-  constexpr uint32_t kBlock = 64 * kDepth * 2;     // bytes between 64-value blocks of MN-major rows
+loss_product_kernel(const __grid_constant__ Maps maps0, const __grid_constant__ Maps maps1,
+                    const __grid_constant__ Work w) {
   extern __shared__ uint8_t raw[];
   uint8_t* stages = (uint8_t*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
   __shared__ Shared sh;
+  constexpr uint32_t kBlock = 64 * kDepth * 2;     // bytes between 64-value blocks of MN-major rows
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const uint32_t rank = cluster_rank();
-  const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n * p.splits;
+  const int64_t tiles = tiles_of(w.p[0]) + (KIND == kWeights && w.count > 1 ? tiles_of(w.p[1]) : 0);
   const int64_t pair = blockIdx.x / 2, pairs = gridDim.x / 2;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) mbar_init(&sh.full[i], 1), mbar_init(&sh.empty[i], 1);
-    for (int i = 0; i < 2; ++i) mbar_init(&sh.done[i], 1), mbar_init(&sh.drained[i], 8);
+    for (int i = 0; i < 2; ++i) mbar_init(&sh.done[i], 1), mbar_init(&sh.drained[i], 2 * kEpilogueWarps);
     sh.dead = 0;
     fence_barrier_init();
   }
@@ -293,34 +340,37 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a,
     uint32_t phase = 0;
     bool ok = true;
     for (int64_t t = pair; ok && t < tiles; t += pairs) {
-      const Place q = place_of(p, t);
+      const Place q = place_of<KIND>(w, t);
+      const Product& p = w.p[q.product];
+      const Maps& maps = q.product ? maps1 : maps0;
+      const bool a_mn = KIND == kWeights && p.a_mn, b_mn = KIND == kWeights && p.b_mn;
       const int m0 = q.tm * kTile + (int)rank * kHalf, n0 = q.tn * kTile + (int)rank * kHalf;
       const int k0 = q.split * p.steps_per_split;
       const int k1 = k0 + p.steps_per_split < p.steps ? k0 + p.steps_per_split : p.steps;
       for (int k = k0; k < k1; ++k) {
-        if (!(ok = wait(&sh, &sh.empty[stage], phase ^ 1, p.err_flag))) break;
+        if (!(ok = wait(&sh, &sh.empty[stage], phase ^ 1, w.err_flag))) break;
         if (rank == 0) mbar_arrive_expect_tx(&sh.full[stage], 2 * kStageBytes);
         const uint32_t bar = map_to_rank(&sh.full[stage], 0);
         uint8_t* a = stages + stage * kStageBytes;
         uint8_t* b = a + kOperandBytes;
-        if constexpr (A_MN) {
-          pair_load(a, &map_a, m0, k * kDepth, bar);
-          pair_load(a + kBlock, &map_a, m0 + 64, k * kDepth, bar);
+        if (a_mn) {
+          pair_load(a, &maps.a, m0, k * kDepth, bar);
+          pair_load(a + kBlock, &maps.a, m0 + 64, k * kDepth, bar);
         } else {
-          pair_load(a, &map_a, k * kDepth, m0, bar);
+          pair_load(a, &maps.a, k * kDepth, m0, bar);
         }
-        if constexpr (B_MN) {
-          pair_load(b, &map_b, n0, k * kDepth, bar);
-          pair_load(b + kBlock, &map_b, n0 + 64, k * kDepth, bar);
+        if (b_mn) {
+          pair_load(b, &maps.b, n0, k * kDepth, bar);
+          pair_load(b + kBlock, &maps.b, n0 + 64, k * kDepth, bar);
         } else {
-          pair_load(b, &map_b, k * kDepth, n0, bar);
+          pair_load(b, &maps.b, k * kDepth, n0, bar);
         }
         if (++stage == kStages) stage = 0, phase ^= 1;
       }
     }
     // every stage's last release has arrived before this CTA may end
     for (int i = 0; ok && i < kStages; ++i) {
-      ok = wait(&sh, &sh.empty[stage], phase ^ 1, p.err_flag);
+      ok = wait(&sh, &sh.empty[stage], phase ^ 1, w.err_flag);
       if (++stage == kStages) stage = 0, phase ^= 1;
     }
   } else if (warp == 1 && lane == 0 && rank == 0) {   // products
@@ -328,22 +378,24 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a,
     uint32_t phase = 0, buf_phase = 0;
     bool ok = true;
     for (int64_t t = pair; ok && t < tiles; t += pairs) {
-      const Place q = place_of(p, t);
+      const Place q = place_of<KIND>(w, t);
+      const Product& p = w.p[q.product];
+      const bool a_mn = KIND == kWeights && p.a_mn, b_mn = KIND == kWeights && p.b_mn;
+      const uint32_t idesc = instruction_desc<T>(kTile, kTile, a_mn, b_mn);
+      // 16 steps of depth: 32 bytes along a K-major row, two atoms MN-major
+      const uint32_t a_step = a_mn ? 2048 : 32, b_step = b_mn ? 2048 : 32;
       const int k0 = q.split * p.steps_per_split;
       const int k1 = k0 + p.steps_per_split < p.steps ? k0 + p.steps_per_split : p.steps;
-      if (!(ok = wait(&sh, &sh.drained[buf], buf_phase ^ 1, p.err_flag))) break;
+      if (!(ok = wait(&sh, &sh.drained[buf], buf_phase ^ 1, w.err_flag))) break;
       tc_fence_after();
       for (int k = k0; k < k1; ++k) {
-        if (!(ok = wait(&sh, &sh.full[stage], phase, p.err_flag))) break;
+        if (!(ok = wait(&sh, &sh.full[stage], phase, w.err_flag))) break;
         tc_fence_after();
         const uint32_t a = smem_u32(stages + stage * kStageBytes), b = a + kOperandBytes;
 #pragma unroll
-        for (int i = 0; i < kDepth / 16; ++i) {
-          // 16 steps of depth: 32 bytes along a K-major row, two atoms MN-major
-          const uint64_t da = operand_desc(a + i * (A_MN ? 2048 : 32), A_MN ? kBlock : 16);
-          const uint64_t db = operand_desc(b + i * (B_MN ? 2048 : 32), B_MN ? kBlock : 16);
-          mma_pair(tmem + buf * kTile, da, db, kIdesc, k > k0 || i > 0);
-        }
+        for (int i = 0; i < kDepth / 16; ++i)
+          mma_pair(tmem + buf * kTile, operand_desc(a + i * a_step, kBlock),
+                   operand_desc(b + i * b_step, kBlock), idesc, k > k0 || i > 0);
         commit_pair(&sh.empty[stage]);
         if (++stage == kStages) stage = 0, phase ^= 1;
       }
@@ -354,25 +406,29 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a,
   } else if (warp >= kEpilogueWarp) {              // finished tiles
     int buf = 0;
     uint32_t buf_phase = 0;
-    const uint32_t lanes = (uint32_t)(warp - kEpilogueWarp) * 32;
+    // a warp reads the 32 lanes of TMEM that its number's last two bits name
+    const uint32_t lanes = (uint32_t)(warp % 4) * 32, half = (uint32_t)(warp - kEpilogueWarp) / 4;
+    uint8_t* slot = stages + kStages * kStageBytes + (warp - kEpilogueWarp) * kSlotBytes;
     for (int64_t t = pair; t < tiles; t += pairs) {
-      const Place q = place_of(p, t);
-      bool ok = lane != 0 || wait(&sh, &sh.done[buf], buf_phase, p.err_flag);
+      const Place q = place_of<KIND>(w, t);
+      bool ok = lane != 0 || wait(&sh, &sh.done[buf], buf_phase, w.err_flag);
       ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
       if (!ok) break;
       tc_fence_after();
-      const uint32_t acc = tmem + (lanes << 16) + buf * kTile;
-      const int64_t m = (int64_t)q.tm * kTile + rank * kHalf + lanes + lane;
-      const int64_t n0 = (int64_t)q.tn * kTile;
-      if constexpr (KIND == kStats) finish_stats(p, acc, m, n0, q.tn);
-      if constexpr (KIND == kGrads) finish_grads<T>(p, acc, m, n0);
-      if constexpr (KIND == kDx) finish_dx(p, acc, m, n0, q.split);
-      if constexpr (KIND == kDw) finish_dw<T>(p, acc, m, n0);
+      const uint32_t acc = tmem + (lanes << 16) + buf * kTile + half * kHalf;
+      const int64_t m0 = (int64_t)q.tm * kTile + rank * kHalf + lanes;
+      const int64_t n0 = (int64_t)q.tn * kTile + half * kHalf;
+      const CUtensorMap* out = q.product ? &maps1.out : &maps0.out;
+      if constexpr (KIND == kStats) finish_stats(w, acc, m0 + lane, n0);
+      if constexpr (KIND == kGrads) finish_grads<T>(w, out, slot, acc, m0, n0, lane);
+      if constexpr (KIND == kWeights)
+        finish_weights<T>(w, w.p[q.product], out, slot, acc, m0, n0, q.split, lane);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) arrive_at(map_to_rank(&sh.drained[buf], 0));
       if (++buf == 2) buf = 0, buf_phase ^= 1;
     }
+    if (lane == 0) bulk_wait_all();
   }
   __syncthreads();
   if (sh.dead) {     // let copies and products in flight land before their memory goes
@@ -388,89 +444,144 @@ loss_product_kernel(const __grid_constant__ CUtensorMap map_a,
 
 // ---------------------------------------------------------------- small kernels
 
-// A row's loss from its tiles' statistics: 32 rows by 8 strands of tiles a block,
+// A row's loss from its tiles' statistics: 32 rows by 32 strands of tiles a block,
 // joined in a fixed order.
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(1024)
 finish_loss_kernel(const RowStat* __restrict__ stats, int tiles, int64_t tokens, int64_t vocab,
                    const int64_t* __restrict__ targets, const float* __restrict__ at_target,
                    float* __restrict__ loss, float* __restrict__ lse) {
-  __shared__ RowStat part[8][32];
+  __shared__ RowStat part[32][33];
   const int x = threadIdx.x % 32, y = threadIdx.x / 32;
   const int64_t t = (int64_t)blockIdx.x * 32 + x;
   RowStat s = {-INFINITY, 0.f};
   if (t < tokens) {
 #pragma unroll 4
-    for (int i = y; i < tiles; i += 8) s = join(s, stats[(int64_t)i * tokens + t]);
+    for (int i = y; i < tiles; i += 32) s = join(s, stats[(int64_t)i * tokens + t]);
   }
   part[y][x] = s;
   __syncthreads();
-  if (y != 0 || t >= tokens) return;
-  for (int i = 1; i < 8; ++i) s = join(s, part[i][x]);
-  const bool counts = has_loss(targets[t], vocab);
+  s = part[x][y];                     // row y, strand x
+#pragma unroll
+  for (int o = 16; o > 0; o /= 2) {
+    RowStat q;
+    q.top = __shfl_down_sync(0xffffffffu, s.top, o), q.sum = __shfl_down_sync(0xffffffffu, s.sum, o);
+    s = join(s, q);
+  }
+  const int64_t r = (int64_t)blockIdx.x * 32 + y;
+  if (x != 0 || r >= tokens) return;
+  const bool counts = has_loss(targets[r], vocab);
   const float v = lse_of(s);
-  lse[t] = counts ? v : 0.f;
-  loss[t] = counts ? v - at_target[t] : 0.f;
+  lse[r] = counts ? v : 0.f;
+  loss[r] = counts ? v - at_target[r] : 0.f;
 }
 
-// Scale of G and every row's coefficients, in one block.
+// 8 values of a row into a 16-byte aligned place, zeros behind `width`.
+template <class T>
+__device__ __forceinline__ void copy8(const T* in, int64_t left, bool wide, bool keep, T* out) {
+  uint4 q = make_uint4(0, 0, 0, 0);
+  if (keep) {
+    if (wide && left >= 8) {
+      q = *(const uint4*)in;
+    } else {
+      T* e = (T*)&q;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (j < left) e[j] = in[j];
+    }
+  }
+  *(uint4*)out = q;
+}
+
+// Rows into 16-byte aligned ones of `ld` values, padded with zeros; rows without a
+// loss (where targets are given) become zero. A thread copies 8 values.
+template <class T>
+__device__ void copy_rows(const T* __restrict__ in, int64_t in_ld, int64_t width, T* __restrict__ out,
+                          int64_t ld, int64_t rows, const int64_t* __restrict__ targets, int64_t vocab,
+                          int64_t first, int64_t stride) {
+  const int64_t per = ld / 8;
+  const bool wide = in_ld % 8 == 0 && (uintptr_t)in % 16 == 0;
+  for (int64_t i = first; i < rows * per; i += stride) {
+    int64_t r, c;
+    if (rows * per <= 0xffffffffll) {
+      r = (uint32_t)i / (uint32_t)per, c = (uint32_t)i % (uint32_t)per * 8;
+    } else {
+      r = i / per, c = i % per * 8;
+    }
+    const bool keep = targets == nullptr || has_loss(targets[r], vocab);
+    copy8(in + r * in_ld + c, width - c, wide, keep, out + r * ld + c);
+  }
+}
+
+template <class T>
+__global__ void __launch_bounds__(256)
+copy_rows_kernel(const T* in, int64_t in_ld, int64_t width, T* out, int64_t ld, int64_t rows) {
+  copy_rows<T>(in, in_ld, width, out, ld, rows, nullptr, 0, (int64_t)blockIdx.x * 256 + threadIdx.x,
+               (int64_t)gridDim.x * 256);
+}
+
+// The gradient's start. The first block: scale of G and every row's coefficients;
+// the others: x with rows without a loss as zeros, so that nothing of theirs
+// reaches dW.
+template <class T>
 __global__ void __launch_bounds__(1024)
-row_coefs_kernel(int64_t tokens, int64_t vocab, const int64_t* __restrict__ targets,
-                 const float* __restrict__ lse, const float* __restrict__ dloss,
-                 const float* __restrict__ dlse, RowCoef* __restrict__ rows, float* scale) {
+prepare_kernel(const T* x, int64_t x_ld, int64_t width, T* out, int64_t ld, int64_t tokens,
+               int64_t vocab, const int64_t* __restrict__ targets, const float* __restrict__ lse,
+               const float* __restrict__ dloss, const float* __restrict__ dlse,
+               RowCoef* __restrict__ rows, float* scale) {
+  if (blockIdx.x > 0) {
+    copy_rows<T>(x, x_ld, width, out, ld, tokens, targets, vocab,
+                 (int64_t)(blockIdx.x - 1) * 1024 + threadIdx.x, (int64_t)(gridDim.x - 1) * 1024);
+    return;
+  }
   __shared__ float part[32];
   float top = 0.f;
+#pragma unroll 4
   for (int64_t t = threadIdx.x; t < tokens; t += 1024) {
-    if (!has_loss(targets[t], vocab)) continue;
     const float one = dloss ? dloss[t] : 0.f, all = one + (dlse ? dlse[t] : 0.f);
-    top = fmaxf(top, fmaxf(fabsf(one), fabsf(all)));
+    if (has_loss(targets[t], vocab)) top = fmaxf(top, fmaxf(fabsf(one), fabsf(all)));
   }
 #pragma unroll
   for (int o = 16; o > 0; o /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = top;
   __syncthreads();
   for (int i = 0; i < 32; ++i) top = fmaxf(top, part[i]);
-  // 2^13 over the largest, both rounded down to powers of two; 1 for 0 and infinity
+  // 2^13 over the largest, rounded down to a power of two; 1 for 0 and infinity
   const int e = (__float_as_int(top) >> 23) - 127;
   const int s = e == -127 || e == 128 ? 0 : (13 - e > 126 ? 126 : (13 - e < -126 ? -126 : 13 - e));
   const float up = __int_as_float((127 + s) << 23), down = __int_as_float((127 - s) << 23);
   if (threadIdx.x == 0) scale[0] = up, scale[1] = down;
+#pragma unroll 4
   for (int64_t t = threadIdx.x; t < tokens; t += 1024) {
     const int64_t at = targets[t];
-    RowCoef q = {0.f, 0.f, 0.f, -1};
-    if (has_loss(at, vocab)) {
-      const float one = dloss ? dloss[t] : 0.f, all = one + (dlse ? dlse[t] : 0.f);
-      q = {all * up, one * up, lse[t] * kLog2e, (int)at};
-    }
-    rows[t] = q;
+    const float one = dloss ? dloss[t] : 0.f, all = one + (dlse ? dlse[t] : 0.f);
+    const float norm = lse[t] * kLog2e;
+    const bool counts = has_loss(at, vocab);
+    rows[t] = {counts ? all * up : 0.f, counts ? one * up : 0.f, counts ? norm : 0.f,
+               counts ? (int)at : -1};
   }
 }
 
-// Rows into 16-byte aligned ones, padded with zeros to `ld`; rows without a loss
-// (where targets are given) become zero.
-template <class T>
-__global__ void __launch_bounds__(256)
-copy_rows_kernel(const T* __restrict__ in, int64_t in_ld, int64_t width, T* __restrict__ out,
-                 int64_t ld, int64_t rows, const int64_t* __restrict__ targets, int64_t vocab) {
-  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-    const bool keep = targets == nullptr || has_loss(targets[r], vocab);
-    for (int64_t c = threadIdx.x; c < ld; c += 256)
-      out[r * ld + c] = keep && c < width ? in[r * in_ld + c] : from_f<T>(0.f);
-  }
-}
-
+// dx from the slabs of its sums, in their order; 4 values a thread.
 template <class T>
 __global__ void __launch_bounds__(256)
 finish_dx_kernel(const float* __restrict__ sums, int splits, int64_t ld, int64_t tokens,
                  int64_t width, const RowCoef* __restrict__ rows, const float* __restrict__ scale,
                  T* __restrict__ dx, int64_t dx_ld) {
   const float inv = scale[1];
-  for (int64_t r = blockIdx.x; r < tokens; r += gridDim.x) {
+  const int64_t per = ld / 4;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < tokens * per; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / per, c = i % per * 4;
     const bool keep = rows[r].target >= 0;
-    for (int64_t c = threadIdx.x; c < width; c += 256) {
-      float v = 0.f;
-      for (int s = 0; s < splits; ++s) v += sums[((int64_t)s * tokens + r) * ld + c];
-      dx[r * dx_ld + c] = from_f<T>(keep ? v * inv : 0.f);
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int s = 0; s < splits; ++s) {
+      const float4 u = *(const float4*)(sums + ((int64_t)s * tokens + r) * ld + c);
+      v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
     }
+    const float o[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (c + j < width) dx[r * dx_ld + c + j] = from_f<T>(keep ? o[j] * inv : 0.f);
   }
 }
 
@@ -483,21 +594,29 @@ int pair_count() {
   return sms / 2;
 }
 
+Product product_of(int64_t m, int64_t n, int64_t depth, int splits = 1) {
+  Product p = {};
+  p.m = m, p.n = n;
+  p.tiles_m = (int)ceil_div(m, kTile), p.tiles_n = (int)ceil_div(n, kTile);
+  p.steps = (int)ceil_div(depth, kDepth);
+  p.steps_per_split = (int)ceil_div(p.steps, splits);
+  p.splits = (int)ceil_div(p.steps, p.steps_per_split);      // no empty one
+  return p;
+}
+
 template <class T, int KIND>
-ferrum_status run(const CUtensorMap& a, const CUtensorMap& b, Product p, int64_t depth, int splits,
-                  cudaStream_t stream, const char* what) {
+ferrum_status run(const Maps& m0, const Maps& m1, const Work& w, cudaStream_t stream,
+                  const char* what) {
   static std::atomic<uint64_t> smem_done{0};
   auto kernel = loss_product_kernel<T, KIND>;
   cudaError_t e = launch_detail::ensure_smem(kernel, kSmemBytes, smem_done);
   if (e != cudaSuccess) return cuda_error(e, what);
-  p.tiles_m = (int)ceil_div(p.m, kTile), p.tiles_n = (int)ceil_div(p.n, kTile);
-  p.steps = (int)ceil_div(depth, kDepth);
-  p.steps_per_split = (int)ceil_div(p.steps, splits);
-  p.splits = (int)ceil_div(p.steps, p.steps_per_split);      // no empty one
-  const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n * p.splits;
+  int64_t tiles = 0;
+  for (int i = 0; i < w.count; ++i)
+    tiles += (int64_t)w.p[i].tiles_m * w.p[i].tiles_n * w.p[i].splits;
   const int grid = 2 * (int)std::min<int64_t>(tiles, pair_count());
   launch_detail::clear_stale_error();
-  kernel<<<grid, kThreads, kSmemBytes, stream>>>(a, b, p);
+  kernel<<<grid, kThreads, kSmemBytes, stream>>>(m0, m1, w);
   return launched(what);
 }
 
@@ -510,12 +629,14 @@ struct Matrix {
 int64_t padded(int64_t n) { return ceil_div(n, 8) * 8; }
 
 template <class T>
-ferrum_status copy_rows(const void* in, int64_t in_ld, int64_t width, int64_t rows, T* out,
-                        const int64_t* targets, int64_t vocab, cudaStream_t stream,
-                        const char* what) {
+ferrum_status copied(Matrix<T>& m, int64_t width, int64_t rows, uint8_t*& at, cudaStream_t stream,
+                     const char* what) {
+  const int64_t ld = padded(width);
   launch_detail::clear_stale_error();
-  copy_rows_kernel<T><<<(unsigned)std::min<int64_t>(rows, 148 * 64), 256, 0, stream>>>(
-      (const T*)in, in_ld, width, out, padded(width), rows, targets, vocab);
+  copy_rows_kernel<T><<<(unsigned)std::min<int64_t>(ceil_div(rows * ld / 8, 256), 148 * 32), 256, 0, stream>>>(
+      m.p, m.ld, width, (T*)at, ld, rows);
+  m = {(const T*)at, ld};
+  at += rows * ld * 2;
   return launched(what);
 }
 
@@ -527,37 +648,36 @@ ferrum_status fwd(ferrum_device* dev, const ferrum_cross_entropy_args* a, cudaSt
                   const char* what) {
   const int64_t n = (int64_t)a->tokens, d = (int64_t)a->width, v = (int64_t)a->vocab;
   const bool copy_x = !mappable(a->x, a->x_stride, d), copy_w = !mappable(a->weight, a->weight_stride, d);
-  const int64_t ld = padded(d), tiles = ceil_div(v, kTile);
-  const size_t x_bytes = copy_x ? (size_t)(n * ld) * 2 : 0, w_bytes = copy_w ? (size_t)(v * ld) * 2 : 0;
-  PoolBuffer ws(dev, x_bytes + w_bytes + (size_t)(tiles * n) * sizeof(RowStat) + (size_t)n * 4, stream);
+  const int64_t ld = padded(d), halves = ceil_div(v, kHalf);
+  const size_t copies = (size_t)((copy_x ? n : 0) + (copy_w ? v : 0)) * ld * 2;
+  PoolBuffer ws(dev, copies + (size_t)(halves * n) * sizeof(RowStat) + (size_t)n * 4, stream);
   if (ws.status() != cudaSuccess) return cuda_error(ws.status(), "workspace");
   uint8_t* at = ws.as<uint8_t>();
-  Matrix<T> x = {(const T*)a->x, a->x_stride}, w = {(const T*)a->weight, a->weight_stride};
+  Matrix<T> x = {(const T*)a->x, a->x_stride}, wt = {(const T*)a->weight, a->weight_stride};
   if (copy_x) {
-    if (ferrum_status s = copy_rows<T>(a->x, a->x_stride, d, n, (T*)at, nullptr, 0, stream, what)) return s;
-    x = {(const T*)at, ld}, at += x_bytes;
+    if (ferrum_status s = copied(x, d, n, at, stream, what)) return s;
   }
   if (copy_w) {
-    if (ferrum_status s = copy_rows<T>(a->weight, a->weight_stride, d, v, (T*)at, nullptr, 0, stream, what)) return s;
-    w = {(const T*)at, ld}, at += w_bytes;
+    if (ferrum_status s = copied(wt, d, v, at, stream, what)) return s;
   }
-  CUtensorMap ma, mb;
-  cudaError_t e = tensor_map(&ma, is_bf16<T>(), x.p, d, n, x.ld, kHalf);
-  if (e == cudaSuccess) e = tensor_map(&mb, is_bf16<T>(), w.p, d, v, w.ld, kHalf);
+  Maps m = {};
+  cudaError_t e = tensor_map(&m.a, is_bf16<T>(), x.p, d, n, x.ld, kHalf);
+  if (e == cudaSuccess) e = tensor_map(&m.b, is_bf16<T>(), wt.p, d, v, wt.ld, kHalf);
   if (e != cudaSuccess) return cuda_error(e, "tensor map");
-  Product p = {};
-  p.m = n, p.n = v, p.err_flag = dev->err_flag, p.targets = a->targets;
-  p.stats = (RowStat*)at, p.at_target = (float*)(p.stats + tiles * n);
-  if (ferrum_status s = run<T, kStats>(ma, mb, p, d, 1, stream, what)) return s;
-  finish_loss_kernel<<<(unsigned)ceil_div(n, 32), 256, 0, stream>>>(
-      p.stats, (int)tiles, n, v, a->targets, p.at_target, a->loss, a->lse);
+  Work w = {};
+  w.p[0] = product_of(n, v, d), w.count = 1;
+  w.err_flag = dev->err_flag, w.targets = a->targets;
+  w.stats = (RowStat*)at, w.at_target = (float*)(w.stats + halves * n);
+  if (ferrum_status s = run<T, kStats>(m, m, w, stream, what)) return s;
+  finish_loss_kernel<<<(unsigned)ceil_div(n, 32), 1024, 0, stream>>>(
+      w.stats, (int)halves, n, v, a->targets, w.at_target, a->loss, a->lse);
   return launched(what);
 }
 
-// Words of a piece of the vocabulary: 128 MiB of G, but no fewer than 4096.
+// Words of a piece of the vocabulary: 256 MiB of G, but no fewer than 4096.
 int64_t piece_of(int64_t tokens, int64_t vocab) {
-  const int64_t n = std::max<int64_t>(((int64_t)1 << 26) / tokens / kTile * kTile, 4096);
-  return std::min(n, ceil_div(vocab, 32) * 32);
+  const int64_t n = std::max<int64_t>(((int64_t)1 << 27) / tokens / kTile * kTile, 4096);
+  return std::min(n, ceil_div(vocab, 64) * 64);
 }
 
 template <class T>
@@ -566,62 +686,80 @@ ferrum_status bwd(ferrum_device* dev, const ferrum_cross_entropy_args* a, cudaSt
   const int64_t n = (int64_t)a->tokens, d = (int64_t)a->width, v = (int64_t)a->vocab;
   const bool copy_w = !mappable(a->weight, a->weight_stride, d);
   const int64_t ld = padded(d), piece = piece_of(n, v);
+  const bool one_piece = piece >= v;
   // Few tokens make few tiles of dx: its depth is split so that all pairs work.
   const int64_t dx_tiles = ceil_div(n, kTile) * ceil_div(d, kTile);
-  const int splits = (int)std::max<int64_t>(
-      1, std::min<int64_t>(pair_count() / dx_tiles, ceil_div(piece, 4 * kDepth)));
-  auto round = [](size_t b) { return (b + 255) / 256 * 256; };
-  const size_t x_bytes = round((size_t)(n * ld) * 2), w_bytes = copy_w ? round((size_t)(v * ld) * 2) : 0;
-  const size_t g_bytes = round((size_t)(n * piece) * 2), dx_bytes = round((size_t)(splits * n * ld) * 4);
-  PoolBuffer ws(dev, x_bytes + w_bytes + g_bytes + dx_bytes + (size_t)n * sizeof(RowCoef) + 256, stream);
+  const int want = (int)std::max<int64_t>(
+      1, std::min<int64_t>(pair_count() / dx_tiles, ceil_div(std::min(piece, v), 4 * kDepth)));
+  const int splits = product_of(n, d, std::min(piece, v), want).splits;
+  const bool need_sums = splits > 1 || !one_piece;
+  auto round = [](int64_t b) { return (size_t)((b + 255) / 256 * 256); };
+  const size_t x_bytes = round(n * ld * 2), w_bytes = copy_w ? round(v * ld * 2) : 0;
+  const size_t g_bytes = round(n * piece * 2), sum_bytes = need_sums ? round(splits * n * ld * 4) : 0;
+  PoolBuffer ws(dev, x_bytes + w_bytes + g_bytes + sum_bytes + (size_t)n * sizeof(RowCoef) + 256, stream);
   if (ws.status() != cudaSuccess) return cuda_error(ws.status(), "workspace");
   uint8_t* at = ws.as<uint8_t>();
-  T* x = (T*)at;
-  at += x_bytes;
-  Matrix<T> w = {(const T*)a->weight, a->weight_stride};
-  // rows without a loss as zeros, so that nothing of theirs reaches dW
-  if (ferrum_status s = copy_rows<T>(a->x, a->x_stride, d, n, x, a->targets, v, stream, what)) return s;
-  if (copy_w) {
-    if (ferrum_status s = copy_rows<T>(a->weight, a->weight_stride, d, v, (T*)at, nullptr, 0, stream, what)) return s;
-    w = {(const T*)at, ld}, at += w_bytes;
-  }
-  T* g = (T*)at;
-  at += g_bytes;
-  float* sums = (float*)at;
-  at += dx_bytes;
   float* scale = (float*)at;
   RowCoef* rows = (RowCoef*)(at + 256);
-  row_coefs_kernel<<<1, 1024, 0, stream>>>(n, v, a->targets, a->lse, a->dloss, a->dlse, rows, scale);
+  at += 256 + n * sizeof(RowCoef);
+  at = (uint8_t*)(((uintptr_t)at + 15) & ~(uintptr_t)15);
+  T* x = (T*)at;
+  at += x_bytes;
+  T* g = (T*)at;
+  at += g_bytes;
+  float* sums = need_sums ? (float*)at : nullptr;
+  at += sum_bytes;
+  Matrix<T> wt = {(const T*)a->weight, a->weight_stride};
+  const int64_t copiers = std::min<int64_t>(ceil_div(n * ld / 8, 1024), 148 * 4);
+  prepare_kernel<T><<<(unsigned)copiers + 1, 1024, 0, stream>>>(
+      (const T*)a->x, a->x_stride, d, x, ld, n, v, a->targets, a->lse, a->dloss, a->dlse, rows, scale);
   if (ferrum_status s = launched(what)) return s;
+  if (copy_w) {
+    if (ferrum_status s = copied(wt, d, v, at, stream, what)) return s;
+  }
 
-  int used = 1;
+  const bool dx_map = mappable(a->dx, a->dx_stride, d), dw_map = mappable(a->dweight, a->dweight_stride, d);
   for (int64_t first = 0; first < v; first += piece) {
     const int64_t words = std::min(piece, v - first);
-    const T* wp = w.p + first * w.ld;
-    CUtensorMap x_k, w_k, g_k, w_mn, g_mn, x_mn;
-    cudaError_t e = tensor_map(&x_k, is_bf16<T>(), x, d, n, ld, kHalf);
-    if (e == cudaSuccess) e = tensor_map(&w_k, is_bf16<T>(), wp, d, words, w.ld, kHalf);
-    if (e == cudaSuccess) e = tensor_map(&g_k, is_bf16<T>(), g, words, n, piece, kHalf);
-    if (e == cudaSuccess) e = tensor_map(&w_mn, is_bf16<T>(), wp, d, words, w.ld, kDepth);
-    if (e == cudaSuccess) e = tensor_map(&g_mn, is_bf16<T>(), g, words, n, piece, kDepth);
-    if (e == cudaSuccess) e = tensor_map(&x_mn, is_bf16<T>(), x, d, n, ld, kDepth);
+    const bool last = first + words == v;
+    const T* wp = wt.p + first * wt.ld;
+    T* dw = (T*)a->dweight + first * a->dweight_stride;
+    Maps logits = {}, mx = {}, mw = {};
+    cudaError_t e = cudaSuccess;
+    auto map = [&](CUtensorMap& m, const void* p, int64_t cols, int64_t rows, int64_t pitch, int box) {
+      if (e == cudaSuccess) e = tensor_map(&m, is_bf16<T>(), p, cols, rows, pitch, box);
+    };
+    map(logits.a, x, d, n, ld, kHalf), map(logits.b, wp, d, words, wt.ld, kHalf);
+    map(logits.out, g, words, n, piece, 32);
+    map(mx.a, g, words, n, piece, kHalf), map(mx.b, wp, d, words, wt.ld, kDepth);
+    if (dx_map) map(mx.out, a->dx, d, n, a->dx_stride, 32);
+    map(mw.a, g, words, n, piece, kDepth), map(mw.b, x, d, n, ld, kDepth);
+    if (dw_map) map(mw.out, dw, d, words, a->dweight_stride, 32);
     if (e != cudaSuccess) return cuda_error(e, "tensor map");
-    Product p = {};
-    p.err_flag = dev->err_flag, p.rows = rows, p.scale = scale, p.first = first;
-    p.m = n, p.n = words, p.out = g, p.ld = piece;
-    if (ferrum_status s = run<T, kGrads>(x_k, w_k, p, d, 1, stream, what)) return s;
-    p.n = d, p.out = sums, p.ld = ld, p.add = first > 0;
-    if (first == 0) {
-      const int steps = (int)ceil_div(words, kDepth);
-      used = (int)ceil_div(steps, ceil_div(steps, splits));
-    }
-    if (ferrum_status s = run<T, kDx>(g_k, w_mn, p, words, used, stream, what)) return s;
-    p.m = words, p.out = (T*)a->dweight + first * a->dweight_stride, p.ld = a->dweight_stride;
-    if (ferrum_status s = run<T, kDw>(g_mn, x_mn, p, n, 1, stream, what)) return s;
+    Work w = {};
+    w.err_flag = dev->err_flag, w.rows = rows, w.scale = scale, w.first = first;
+    w.p[0] = product_of(n, words, d), w.count = 1;
+    w.p[0].store_map = true;
+    if (ferrum_status s = run<T, kGrads>(logits, logits, w, stream, what)) return s;
+
+    Product px = product_of(n, d, words, splits), pw = product_of(words, d, n);
+    px.b_mn = true;
+    px.partial = sums, px.partial_ld = ld;
+    px.load = first > 0, px.sums = splits > 1 || !last;
+    px.out = a->dx, px.ld = a->dx_stride, px.store_map = dx_map;
+    pw.a_mn = pw.b_mn = true;
+    pw.out = dw, pw.ld = a->dweight_stride, pw.store_map = dw_map;
+    // the product of the longer tiles first, so that the last ones are short
+    const bool x_first = px.steps_per_split >= pw.steps_per_split;
+    w.p[0] = x_first ? px : pw, w.p[1] = x_first ? pw : px, w.count = 2;
+    if (ferrum_status s = run<T, kWeights>(x_first ? mx : mw, x_first ? mw : mx, w, stream, what)) return s;
   }
-  finish_dx_kernel<T><<<(unsigned)std::min<int64_t>(n, 148 * 64), 256, 0, stream>>>(
-      sums, used, ld, n, d, rows, scale, (T*)a->dx, a->dx_stride);
-  return launched(what);
+  if (splits > 1) {
+    finish_dx_kernel<T><<<(unsigned)std::min<int64_t>(ceil_div(n * ld / 4, 256), 148 * 16), 256, 0, stream>>>(
+        sums, splits, ld, n, d, rows, scale, (T*)a->dx, a->dx_stride);
+    return launched(what);
+  }
+  return FERRUM_OK;
 }
 
 }  // namespace

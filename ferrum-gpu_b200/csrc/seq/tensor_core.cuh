@@ -24,10 +24,10 @@ __device__ __forceinline__ uint64_t operand_desc(uint32_t addr, uint32_t block) 
 }
 
 // Instruction: float32 accumulators, A and B of one 16-bit type, M x N.
-template <class T, bool A_MN, bool B_MN>
-constexpr uint32_t instruction_desc(int m, int n) {
+template <class T>
+__device__ __forceinline__ uint32_t instruction_desc(int m, int n, bool a_mn, bool b_mn) {
   const uint32_t type = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
-  return (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)A_MN << 15) | ((uint32_t)B_MN << 16) |
+  return (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
          ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 

@@ -878,8 +878,9 @@ ferrum_cross_entropy_args loss_args(const Tensor& x, const Opt& weight, const Op
   if (!t.is_contiguous()) bad("targets must be contiguous");
   ferrum_cross_entropy_args a = {};
   a.dtype = dtype_of(x), a.tokens = x.numel() / d, a.width = d, a.vocab = w.size(0);
-  a.x = x.data_ptr(), a.x_stride = matrix(x, "x").stride;
-  a.weight = w.data_ptr(), a.weight_stride = matrix(w, "weight").stride;
+  // (a single row's stride says nothing)
+  a.x = x.data_ptr(), a.x_stride = a.tokens > 1 ? matrix(x, "x").stride : d;
+  a.weight = w.data_ptr(), a.weight_stride = a.vocab > 1 ? matrix(w, "weight").stride : d;
   a.targets = t.const_data_ptr<int64_t>();
   return a;
 }
