@@ -73,7 +73,7 @@ constexpr int kThreads = 32 * (kEpilogueWarp + kEpilogueWarps);
 constexpr int kSlotBytes = 32 * 128;                          // a warp's rows on their way out
 // and 1024 bytes of room to align
 constexpr int kSmemBytes = kStages * kStageBytes + kEpilogueWarps * kSlotBytes + 1024;
-constexpr int kGroup = 16;                                    // tiles of M that share a tile of N
+constexpr uint32_t kGroup = 16;                                   // tiles of M that share a tile of N
 
 enum Kind { kStats, kGrads, kWeights };
 
@@ -88,7 +88,7 @@ struct RowCoef {
 struct Product {
   int64_t m, n;
   int tiles_m, tiles_n, splits, steps, steps_per_split;
-  bool a_mn, b_mn;           // operands whose rows run along the depth
+  bool a_mn;                 // A's rows run along the depth (as all of B's in kWeights)
   bool sums;                 // the result: float32 sums, a slab per split (else 16 bits)
   bool load, store_map;      // sums of earlier pieces come on top; `out` has a tensor map
   void* out;
@@ -114,26 +114,29 @@ struct Maps {
   CUtensorMap a, b, out;
 };
 
+// Tiles are numbered by 32 bits (the host checks): a division by 64 bits takes the
+// issuing thread longer than a step of the product.
 struct Place {
   int product, tm, tn, split;
 };
-__device__ __forceinline__ int64_t tiles_of(const Product& p) {
-  return (int64_t)p.tiles_m * p.tiles_n * p.splits;
+__host__ __device__ __forceinline__ uint32_t tiles_of(const Product& p) {
+  return (uint32_t)p.tiles_m * (uint32_t)p.tiles_n * (uint32_t)p.splits;
 }
 template <int KIND>
-__device__ __forceinline__ Place place_of(const Work& w, int64_t t) {
+__device__ __forceinline__ Place place_of(const Work& w, uint32_t t) {
   Place q;
   q.product = 0;
   if (KIND == kWeights && t >= tiles_of(w.p[0])) q.product = 1, t -= tiles_of(w.p[0]);
   const Product& p = w.p[q.product];
-  const int64_t per = (int64_t)p.tiles_m * p.tiles_n;
-  q.split = (int)(t / per);
-  t %= per;
-  const int64_t group = t / ((int64_t)kGroup * p.tiles_n);
-  const int first = (int)group * kGroup;
-  const int wide = p.tiles_m - first < kGroup ? p.tiles_m - first : kGroup;
-  t -= group * kGroup * p.tiles_n;
-  q.tm = first + (int)(t % wide), q.tn = (int)(t / wide);
+  q.split = 0;
+  if (KIND == kWeights && p.splits > 1) {
+    const uint32_t per = (uint32_t)p.tiles_m * (uint32_t)p.tiles_n;
+    q.split = (int)(t / per), t %= per;
+  }
+  const uint32_t group = t / ((uint32_t)kGroup * p.tiles_n), first = group * kGroup;
+  const uint32_t wide = p.tiles_m - first < kGroup ? p.tiles_m - first : kGroup;
+  t -= first * p.tiles_n;
+  q.tm = (int)(first + t % wide), q.tn = (int)(t / wide);
   return q;
 }
 
@@ -160,44 +163,63 @@ __device__ __forceinline__ bool wait(Shared* sh, uint64_t* bar, uint32_t phase, 
 
 // ---------------------------------------------------------------- epilogues
 // One warp: row m (its lane's), 128 columns from n0 on, at TMEM address `acc`.
+// `release` says that the accumulators have been read; it comes before the tile's
+// results are stored, whose completion it would otherwise wait for.
 
-__device__ void finish_stats(const Work& w, uint32_t acc, int64_t m, int64_t n0) {
-  const Product& p = w.p[0];
-  const bool row = m < p.m;
-  const int64_t target = row ? w.targets[m] : -1;
-  const int at = target >= n0 && target < n0 + kHalf && target < p.n ? (int)(target - n0) : -1;
-  const int cols = p.n - n0 < kHalf ? (int)(p.n - n0) : kHalf;      // (may be below 0)
-  RowStat s = {-INFINITY, 0.f};
-  float hit = 0.f;
-#pragma unroll 1
-  for (int c = 0; c < kHalf; c += 32) {
-    if (c >= cols) break;
-    float v[32];
-    tmem_load32(acc + c, v);
-    tmem_load_wait();
-    if (c + 32 > cols) {
-#pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (c + i >= cols) v[i] = -INFINITY;
+// What an epilogue reads of its row, a tile ahead of using it.
+template <int KIND>
+__device__ __forceinline__ RowCoef row_ahead(const Work& w, const Place& q, int64_t m) {
+  RowCoef r = {0.f, 0.f, 0.f, -1};
+  if constexpr (KIND == kStats) {
+    if (m < w.p[0].m) {
+      const int64_t at = w.targets[m];
+      r.target = has_loss(at, w.p[0].n) ? (int)at : -1;
     }
-    if (at >= c && at < c + 32) {
-#pragma unroll
-      for (int i = 0; i < 32; ++i) hit += at - c == i ? v[i] : 0.f;
-    }
-    float t4[4] = {s.top, s.top, s.top, s.top};
-#pragma unroll
-    for (int i = 0; i < 32; ++i) t4[i % 4] = fmaxf(t4[i % 4], v[i]);
-    const float top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
-    const float k = shift_of(top) * kLog2e;
-    float s4[4] = {s.top == -INFINITY ? s.sum : s.sum * ex2(fmaf(shift_of(s.top), kLog2e, -k)), 0.f,
-                   0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < 32; ++i) s4[i % 4] += ex2(fmaf(v[i], kLog2e, -k));
-    s.top = top, s.sum = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+  } else if constexpr (KIND == kGrads) {
+    if (m < w.p[0].m) r = w.rows[m];
+  } else {
+    const Product& p = w.p[q.product];
+    if (!p.a_mn && m < p.m) r.target = w.rows[m].target;
   }
-  if (!row || cols <= 0) return;
+  return r;
+}
+
+template <class F>
+__device__ void finish_stats(const Work& w, uint32_t acc, const RowCoef& row, int64_t m, int64_t n0,
+                             F release) {
+  const Product& p = w.p[0];
+  const int at = row.target - (int)n0;
+  const int cols = p.n - n0 < kHalf ? (int)(p.n - n0) : kHalf;      // (may be below 0)
+  if (cols <= 0) {
+    release();
+    return;
+  }
+  float v[4][32], hit = 0.f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) tmem_load32(acc + j * 32, v[j]);
+  tmem_load_wait();
+  release();
+  if (cols < kHalf) {
+#pragma unroll
+    for (int i = 0; i < kHalf; ++i)
+      if (i >= cols) v[i / 32][i % 32] = -INFINITY;
+  }
+  if (at >= 0 && at < kHalf) {
+#pragma unroll
+    for (int i = 0; i < kHalf; ++i) hit += at == i ? v[i / 32][i % 32] : 0.f;
+  }
+  float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, s4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < kHalf; ++i) t4[i % 4] = fmaxf(t4[i % 4], v[i / 32][i % 32]);
+  RowStat s;
+  s.top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
+  const float k = shift_of(s.top) * kLog2e;
+#pragma unroll
+  for (int i = 0; i < kHalf; ++i) s4[i % 4] += ex2(fmaf(v[i / 32][i % 32], kLog2e, -k));
+  s.sum = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+  if (m >= p.m) return;
   w.stats[n0 / kHalf * p.m + m] = s;
-  if (at >= 0) w.at_target[m] = hit;
+  if (row.target >= 0 && at >= 0 && at < kHalf) w.at_target[m] = hit;
 }
 
 // A warp's 32 rows of 64 values, on their way out through its slot of shared
@@ -238,14 +260,14 @@ __device__ __forceinline__ void put_rows(const Product& p, const CUtensorMap* ma
   }
 }
 
-template <class T>
+template <class T, class F>
 __device__ void finish_grads(const Work& w, const CUtensorMap* map, uint8_t* slot, uint32_t acc,
-                             int64_t m0, int64_t n0, int lane) {
+                             const RowCoef& q, int64_t m0, int64_t n0, int lane, F release) {
   const Product& p = w.p[0];
-  RowCoef q = {0.f, 0.f, 0.f, -1};
-  if (m0 + lane < p.m) q = w.rows[m0 + lane];
+  // (a target in front of the piece is below 0, whatever is taken from it)
   const int64_t at64 = (int64_t)q.target - w.first - n0;
   const int at = q.target >= 0 && at64 >= 0 && at64 < kHalf ? (int)at64 : -1;
+  if (n0 >= p.n) release();
 #pragma unroll 1
   for (int c = 0; c < kHalf; c += 64) {
     if (n0 + c >= p.n) break;
@@ -253,6 +275,7 @@ __device__ void finish_grads(const Work& w, const CUtensorMap* map, uint8_t* slo
     tmem_load32(acc + c, v[0]);
     tmem_load32(acc + c + 32, v[1]);
     tmem_load_wait();
+    if (c + 64 >= kHalf || n0 + c + 64 >= p.n) release();
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
 #pragma unroll
@@ -268,12 +291,14 @@ __device__ void finish_grads(const Work& w, const CUtensorMap* map, uint8_t* slo
 }
 
 // Sums into `partial`, or with them, scaled back, to 16 bits.
-template <class T>
+template <class T, class F>
 __device__ void finish_weights(const Work& w, const Product& p, const CUtensorMap* map, uint8_t* slot,
-                               uint32_t acc, int64_t m0, int64_t n0, int split, int lane) {
+                               uint32_t acc, const RowCoef& row, int64_t m0, int64_t n0, int split,
+                               int lane, F release) {
   const float inv = w.scale[1];
   const int64_t m = m0 + lane;
   float* part = p.partial ? p.partial + ((int64_t)split * p.m + m) * p.partial_ld + n0 : nullptr;
+  if (n0 >= p.n) release();
 #pragma unroll 1
   for (int c = 0; c < kHalf; c += 64) {
     if (n0 + c >= p.n) break;
@@ -281,6 +306,7 @@ __device__ void finish_weights(const Work& w, const Product& p, const CUtensorMa
     tmem_load32(acc + c, v[0]);
     tmem_load32(acc + c + 32, v[1]);
     tmem_load_wait();
+    if (c + 64 >= kHalf || n0 + c + 64 >= p.n) release();
     if (p.load && m < p.m) {
 #pragma unroll
       for (int i = 0; i < 64; i += 4) {
@@ -299,8 +325,8 @@ __device__ void finish_weights(const Work& w, const Product& p, const CUtensorMa
         *(float4*)(part + c + i) = make_float4(u[0], u[1], u[2], u[3]);
       }
     } else {
-      // (a row without a loss has a zero in G, but W may hold infinities)
-      const bool keep = p.a_mn || (m < p.m && w.rows[m].target >= 0);
+      // (a row without a loss has zeros in G, but W may hold infinities)
+      const bool keep = p.a_mn || row.target >= 0;
 #pragma unroll
       for (int i = 0; i < 64; ++i) v[i / 32][i % 32] = keep ? v[i / 32][i % 32] * inv : 0.f;
       put_rows<T>(p, map, slot, v, m0, n0 + c, lane);
@@ -319,8 +345,8 @@ loss_product_kernel(const __grid_constant__ Maps maps0, const __grid_constant__ 
   constexpr uint32_t kBlock = 64 * kDepth * 2;     // bytes between 64-value blocks of MN-major rows
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const uint32_t rank = cluster_rank();
-  const int64_t tiles = tiles_of(w.p[0]) + (KIND == kWeights && w.count > 1 ? tiles_of(w.p[1]) : 0);
-  const int64_t pair = blockIdx.x / 2, pairs = gridDim.x / 2;
+  const uint32_t tiles = tiles_of(w.p[0]) + (KIND == kWeights && w.count > 1 ? tiles_of(w.p[1]) : 0);
+  const uint32_t pair = blockIdx.x / 2, pairs = gridDim.x / 2;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) mbar_init(&sh.full[i], 1), mbar_init(&sh.empty[i], 1);
@@ -339,34 +365,42 @@ loss_product_kernel(const __grid_constant__ Maps maps0, const __grid_constant__ 
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
-    for (int64_t t = pair; ok && t < tiles; t += pairs) {
-      const Place q = place_of<KIND>(w, t);
+    const uint32_t bars = map_to_rank(&sh.full[0], 0);
+    auto tile = [&](auto a_mn, const Place& q) {
+      constexpr bool A_MN = decltype(a_mn)::value, B_MN = KIND == kWeights;
       const Product& p = w.p[q.product];
-      const Maps& maps = q.product ? maps1 : maps0;
-      const bool a_mn = KIND == kWeights && p.a_mn, b_mn = KIND == kWeights && p.b_mn;
+      const CUtensorMap* map_a = q.product ? &maps1.a : &maps0.a;
+      const CUtensorMap* map_b = q.product ? &maps1.b : &maps0.b;
       const int m0 = q.tm * kTile + (int)rank * kHalf, n0 = q.tn * kTile + (int)rank * kHalf;
       const int k0 = q.split * p.steps_per_split;
       const int k1 = k0 + p.steps_per_split < p.steps ? k0 + p.steps_per_split : p.steps;
       for (int k = k0; k < k1; ++k) {
-        if (!(ok = wait(&sh, &sh.empty[stage], phase ^ 1, w.err_flag))) break;
+        if (!(ok = wait(&sh, &sh.empty[stage], phase ^ 1, w.err_flag))) return;
         if (rank == 0) mbar_arrive_expect_tx(&sh.full[stage], 2 * kStageBytes);
-        const uint32_t bar = map_to_rank(&sh.full[stage], 0);
+        const uint32_t bar = bars + stage * 8;
         uint8_t* a = stages + stage * kStageBytes;
         uint8_t* b = a + kOperandBytes;
-        if (a_mn) {
-          pair_load(a, &maps.a, m0, k * kDepth, bar);
-          pair_load(a + kBlock, &maps.a, m0 + 64, k * kDepth, bar);
+        if constexpr (A_MN) {
+          pair_load(a, map_a, m0, k * kDepth, bar);
+          pair_load(a + kBlock, map_a, m0 + 64, k * kDepth, bar);
         } else {
-          pair_load(a, &maps.a, k * kDepth, m0, bar);
+          pair_load(a, map_a, k * kDepth, m0, bar);
         }
-        if (b_mn) {
-          pair_load(b, &maps.b, n0, k * kDepth, bar);
-          pair_load(b + kBlock, &maps.b, n0 + 64, k * kDepth, bar);
+        if constexpr (B_MN) {
+          pair_load(b, map_b, n0, k * kDepth, bar);
+          pair_load(b + kBlock, map_b, n0 + 64, k * kDepth, bar);
         } else {
-          pair_load(b, &maps.b, k * kDepth, n0, bar);
+          pair_load(b, map_b, k * kDepth, n0, bar);
         }
         if (++stage == kStages) stage = 0, phase ^= 1;
       }
+    };
+    for (uint32_t t = pair; ok && t < tiles; t += pairs) {
+      const Place q = place_of<KIND>(w, t);
+      if (KIND == kWeights && w.p[q.product].a_mn)
+        tile(std::true_type(), q);
+      else
+        tile(std::false_type(), q);
     }
     // every stage's last release has arrived before this CTA may end
     for (int i = 0; ok && i < kStages; ++i) {
@@ -374,34 +408,43 @@ loss_product_kernel(const __grid_constant__ Maps maps0, const __grid_constant__ 
       if (++stage == kStages) stage = 0, phase ^= 1;
     }
   } else if (warp == 1 && lane == 0 && rank == 0) {   // products
+    // One thread issues four instructions a step of 512 cycles, so what it computes
+    // per step is little: descriptors move by sums.
     int stage = 0, buf = 0;
     uint32_t phase = 0, buf_phase = 0;
     bool ok = true;
-    for (int64_t t = pair; ok && t < tiles; t += pairs) {
-      const Place q = place_of<KIND>(w, t);
-      const Product& p = w.p[q.product];
-      const bool a_mn = KIND == kWeights && p.a_mn, b_mn = KIND == kWeights && p.b_mn;
-      const uint32_t idesc = instruction_desc<T>(kTile, kTile, a_mn, b_mn);
+    const uint64_t first_a = operand_desc(smem_u32(stages), kBlock);
+    const uint64_t first_b = operand_desc(smem_u32(stages) + kOperandBytes, kBlock);
+    auto tile = [&](auto a_mn, const Place& q) {
+      constexpr bool A_MN = decltype(a_mn)::value, B_MN = KIND == kWeights;
+      constexpr uint32_t kIdesc = instruction_desc<T>(kTile, kTile, A_MN, B_MN);
       // 16 steps of depth: 32 bytes along a K-major row, two atoms MN-major
-      const uint32_t a_step = a_mn ? 2048 : 32, b_step = b_mn ? 2048 : 32;
+      constexpr uint32_t kStepA = (A_MN ? 2048 : 32) / 16, kStepB = (B_MN ? 2048 : 32) / 16;
+      const Product& p = w.p[q.product];
       const int k0 = q.split * p.steps_per_split;
       const int k1 = k0 + p.steps_per_split < p.steps ? k0 + p.steps_per_split : p.steps;
-      if (!(ok = wait(&sh, &sh.drained[buf], buf_phase ^ 1, w.err_flag))) break;
+      if (!(ok = wait(&sh, &sh.drained[buf], buf_phase ^ 1, w.err_flag))) return;
       tc_fence_after();
+      const uint32_t acc = tmem + buf * kTile;
       for (int k = k0; k < k1; ++k) {
-        if (!(ok = wait(&sh, &sh.full[stage], phase, w.err_flag))) break;
+        if (!(ok = wait(&sh, &sh.full[stage], phase, w.err_flag))) return;
         tc_fence_after();
-        const uint32_t a = smem_u32(stages + stage * kStageBytes), b = a + kOperandBytes;
+        const uint64_t a = first_a + stage * (kStageBytes / 16), b = first_b + stage * (kStageBytes / 16);
 #pragma unroll
         for (int i = 0; i < kDepth / 16; ++i)
-          mma_pair(tmem + buf * kTile, operand_desc(a + i * a_step, kBlock),
-                   operand_desc(b + i * b_step, kBlock), idesc, k > k0 || i > 0);
+          mma_pair(acc, a + i * kStepA, b + i * kStepB, kIdesc, k > k0 || i > 0);
         commit_pair(&sh.empty[stage]);
         if (++stage == kStages) stage = 0, phase ^= 1;
       }
-      if (!ok) break;
       commit_pair(&sh.done[buf]);
       if (++buf == 2) buf = 0, buf_phase ^= 1;
+    };
+    for (uint32_t t = pair; ok && t < tiles; t += pairs) {
+      const Place q = place_of<KIND>(w, t);
+      if (KIND == kWeights && w.p[q.product].a_mn)
+        tile(std::true_type(), q);
+      else
+        tile(std::false_type(), q);
     }
   } else if (warp >= kEpilogueWarp) {              // finished tiles
     int buf = 0;
@@ -409,23 +452,36 @@ loss_product_kernel(const __grid_constant__ Maps maps0, const __grid_constant__ 
     // a warp reads the 32 lanes of TMEM that its number's last two bits name
     const uint32_t lanes = (uint32_t)(warp % 4) * 32, half = (uint32_t)(warp - kEpilogueWarp) / 4;
     uint8_t* slot = stages + kStages * kStageBytes + (warp - kEpilogueWarp) * kSlotBytes;
-    for (int64_t t = pair; t < tiles; t += pairs) {
-      const Place q = place_of<KIND>(w, t);
+    const uint32_t drained = map_to_rank(&sh.drained[0], 0);
+    Place next = {};
+    RowCoef row_next = {};
+    auto look_ahead = [&](uint32_t t) {
+      if (t >= tiles) return;
+      next = place_of<KIND>(w, t);
+      row_next = row_ahead<KIND>(w, next, (int64_t)next.tm * kTile + rank * kHalf + lanes + lane);
+    };
+    look_ahead(pair);
+    for (uint32_t t = pair; t < tiles; t += pairs) {
       bool ok = lane != 0 || wait(&sh, &sh.done[buf], buf_phase, w.err_flag);
       ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
       if (!ok) break;
       tc_fence_after();
+      const Place q = next;
+      const RowCoef row = row_next;
+      look_ahead(t + pairs);
       const uint32_t acc = tmem + (lanes << 16) + buf * kTile + half * kHalf;
       const int64_t m0 = (int64_t)q.tm * kTile + rank * kHalf + lanes;
       const int64_t n0 = (int64_t)q.tn * kTile + half * kHalf;
       const CUtensorMap* out = q.product ? &maps1.out : &maps0.out;
-      if constexpr (KIND == kStats) finish_stats(w, acc, m0 + lane, n0);
-      if constexpr (KIND == kGrads) finish_grads<T>(w, out, slot, acc, m0, n0, lane);
+      auto release = [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_at(drained + buf * 8);
+      };
+      if constexpr (KIND == kStats) finish_stats(w, acc, row, m0 + lane, n0, release);
+      if constexpr (KIND == kGrads) finish_grads<T>(w, out, slot, acc, row, m0, n0, lane, release);
       if constexpr (KIND == kWeights)
-        finish_weights<T>(w, w.p[q.product], out, slot, acc, m0, n0, q.split, lane);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) arrive_at(map_to_rank(&sh.drained[buf], 0));
+        finish_weights<T>(w, w.p[q.product], out, slot, acc, row, m0, n0, q.split, lane, release);
       if (++buf == 2) buf = 0, buf_phase ^= 1;
     }
     if (lane == 0) bulk_wait_all();
@@ -614,6 +670,7 @@ ferrum_status run(const Maps& m0, const Maps& m1, const Work& w, cudaStream_t st
   int64_t tiles = 0;
   for (int i = 0; i < w.count; ++i)
     tiles += (int64_t)w.p[i].tiles_m * w.p[i].tiles_n * w.p[i].splits;
+  if (tiles > 0x7fffffff) return invalid(what, "too many tiles for one launch");
   const int grid = 2 * (int)std::min<int64_t>(tiles, pair_count());
   launch_detail::clear_stale_error();
   kernel<<<grid, kThreads, kSmemBytes, stream>>>(m0, m1, w);
@@ -743,11 +800,10 @@ ferrum_status bwd(ferrum_device* dev, const ferrum_cross_entropy_args* a, cudaSt
     if (ferrum_status s = run<T, kGrads>(logits, logits, w, stream, what)) return s;
 
     Product px = product_of(n, d, words, splits), pw = product_of(words, d, n);
-    px.b_mn = true;
     px.partial = sums, px.partial_ld = ld;
     px.load = first > 0, px.sums = splits > 1 || !last;
     px.out = a->dx, px.ld = a->dx_stride, px.store_map = dx_map;
-    pw.a_mn = pw.b_mn = true;
+    pw.a_mn = true;
     pw.out = dw, pw.ld = a->dweight_stride, pw.store_map = dw_map;
     // the product of the longer tiles first, so that the last ones are short
     const bool x_first = px.steps_per_split >= pw.steps_per_split;

@@ -25,7 +25,7 @@ __device__ __forceinline__ uint64_t operand_desc(uint32_t addr, uint32_t block) 
 
 // Instruction: float32 accumulators, A and B of one 16-bit type, M x N.
 template <class T>
-__device__ __forceinline__ uint32_t instruction_desc(int m, int n, bool a_mn, bool b_mn) {
+constexpr uint32_t instruction_desc(int m, int n, bool a_mn, bool b_mn) {
   const uint32_t type = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
   return (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
          ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
@@ -50,8 +50,11 @@ __device__ __forceinline__ uint32_t map_to_rank(const void* p, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
   return a;
 }
+// Arrives on a barrier of either CTA. It orders no memory: what it announces are
+// reads of TMEM, complete and fenced before it. (Released, it would wait for the
+// warp's stores: 2 of 9 stalls an issue.)
 __device__ __forceinline__ void arrive_at(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 // Box (x, y) of a tensor map into this CTA's shared memory, its bytes counted by
