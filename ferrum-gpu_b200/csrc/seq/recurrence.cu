@@ -1,18 +1,30 @@
 // Gated linear recurrence over (batch, length, channels), one state a channel
-// (recurrence.cuh has a step's arithmetic). A thread owns a channel of a
-// sequence and walks its steps.
+// (recurrence.cuh has a step's arithmetic).
 //
-// Gradient, with G the gradient of the state:  G_t = dout_t + a_{t+1} G_{t+1}.
-// It walks backwards over pieces of 16 steps, whose states it computes again
-// from the one the forward saved in front of them.
+// A warp owns 16 steps of a row of channels (64 forward in 16-bit types, else 32).
+// It copies them to shared memory a turn ahead, turns them into factors and inputs
+// in registers, and sums them up as one map h -> A h + Q, with A from the sum of
+// the logarithms. The maps of a turn's warps (8 a block, 1 to 8 blocks of a
+// cluster, joined over distributed shared memory) give each warp the state it
+// starts from; it then walks its 16 steps and stores them. One pass over the
+// data, no block waits for another that might not run. What bounds it: see the
+// figures at the launch.
+//
+// Gradient, with G the gradient of the state:  G_t = dout_t + a_{t+1} G_{t+1}. The
+// same backwards over time; the states come from those the forward saved in front
+// of every 16 steps.
+#include <algorithm>
+#include <atomic>
+
 #include "recurrence.cuh"
 
 namespace ferrum {
 namespace seq {
 namespace {
 
-constexpr int kThreads = 128;
-constexpr int kSave = FERRUM_RECURRENCE_SAVE_STEPS;
+constexpr int kSteps = FERRUM_RECURRENCE_SAVE_STEPS;    // of a warp and turn
+constexpr int kMaxWarps = 8, kMaxCluster = 8;
+constexpr int kStepThreads = 128;
 
 template <class T>
 struct RecArrays {
@@ -25,7 +37,8 @@ struct RecArrays {
   float* saved;
   const float* dfinal;
   float* dinitial;
-  int64_t batch, length, channels;
+  float* part;                 // (batch * cluster, channels): sums of ddecay
+  int64_t batch, length, channels, groups;
 };
 
 __device__ __forceinline__ int64_t valid_length(const int32_t* lengths, int64_t b, int64_t length) {
@@ -34,75 +47,364 @@ __device__ __forceinline__ int64_t valid_length(const int32_t* lengths, int64_t 
   return n < 0 ? 0 : (n > length ? length : n);
 }
 
-template <class T>
-__global__ void __launch_bounds__(kThreads) recurrence_fwd_kernel(RecArrays<T> p) {
-  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (i >= p.batch * p.channels) return;
-  const int64_t b = i / p.channels, d = i % p.channels;
-  const int64_t len = valid_length(p.lengths, b, p.length);
-  const int64_t saves = (p.length + kSave - 1) / kSave;
-  const float decay = p.decay[d];
-  float h = p.initial ? p.initial[i] : 0.f;
-  for (int64_t t = 0; t < p.length; ++t) {
-    if (p.saved && t % kSave == 0) p.saved[(b * saves + t / kSave) * p.channels + d] = h;
-    if (t < len) {
-      const Decay a = decay_of(decay, gate_of(to_f(p.rg.at(b, t)[d])).on);
-      const float u = gate_of(to_f(p.ig.at(b, t)[d])).on * to_f(p.x.at(b, t)[d]);
-      h += fmaf(a.m, h, a.root * u);
-    }
-    p.out.at(b, t)[d] = from_f<T>(t < len ? h : 0.f);
-  }
-  if (p.final) p.final[i] = h;
+__device__ __forceinline__ void cp_async_wait_older() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
+
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// Stores to this CTA's shared variable in CTA `rank` of the cluster.
+__device__ __forceinline__ void store_at_rank(float2* p, uint32_t rank, float2 v) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+               : "=r"(a)
+               : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(a), "f"(v.x), "f"(v.y) : "memory");
 }
 
-template <class T>
-__global__ void __launch_bounds__(kThreads) recurrence_bwd_kernel(RecArrays<T> p, float* part) {
-  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (i >= p.batch * p.channels) return;
-  const int64_t b = i / p.channels, d = i % p.channels;
+// A warp's rows of one array in shared memory: 16 steps of 32 * VL channels.
+// ALIGNED: rows begin at multiples of 16 bytes. Otherwise a row's copy begins at the
+// 16-byte unit that holds its first value, so up to 14 bytes in front of it come
+// along, from the same unit; behind its last value nothing is read.
+template <class T, int VL, bool ALIGNED>
+struct Stage {
+  static constexpr int kRow = 32 * VL * (int)sizeof(T), kPitch = kRow + (ALIGNED ? 0 : 16);
+  static constexpr int kUnits = kPitch / 16, kBytes = kSteps * kPitch;
+  // Steps [0, n) from `p` on, `st` values apart, `channels` of them.
+  static __device__ __forceinline__ void fill(uint8_t* s, const T* p, int64_t st, int n, int channels,
+                                              int lane) {
+#pragma unroll
+    for (int i = 0; i < (kSteps * kUnits + 31) / 32; ++i) {
+      const int e = i * 32 + lane, step = e / kUnits, unit = e % kUnits;
+      if (kSteps * kUnits % 32 != 0 && step >= kSteps) break;
+      const uint8_t* row = (const uint8_t*)(p + (step < n ? step : 0) * st);
+      const uint8_t* src = (ALIGNED ? row : (const uint8_t*)((uintptr_t)row & ~(uintptr_t)15)) + unit * 16;
+      const int left = (int)(row - src) + channels * (int)sizeof(T);
+      const int bytes = step >= n || left <= 0 ? 0 : (left < 16 ? left : 16);
+      cp_async<16>(s + step * kPitch + unit * 16, bytes ? src : row - ((uintptr_t)row & 15), bytes);
+    }
+  }
+  // Channels 2 * lane and the next one (aligned, 16 bits), else lane and lane + 32.
+  static constexpr bool kPairs = ALIGNED && VL == 2;
+  static __device__ __forceinline__ int channel(int lane, int e) {
+    return kPairs ? 2 * lane + e : lane + 32 * e;
+  }
+  static __device__ __forceinline__ void load(const uint8_t* s, const T* p, int64_t st, int step, int lane,
+                                              float (&v)[VL]) {
+    const uint8_t* row = s + step * kPitch;
+    if constexpr (!ALIGNED) row += (uintptr_t)(p + step * st) & 15;
+    if constexpr (kPairs) {
+      load_vec<T, 2>((const T*)row + 2 * lane, v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < VL; ++e) v[e] = to_f(((const T*)row)[lane + 32 * e]);
+    }
+  }
+  static __device__ __forceinline__ void store(T* row, int lane, int channels, const float (&v)[VL]) {
+    if constexpr (kPairs) {
+      if (2 * lane < channels) store_vec<T, 2>(row + 2 * lane, v);   // (channels is even)
+    } else {
+#pragma unroll
+      for (int e = 0; e < VL; ++e)
+        if (lane + 32 * e < channels) row[lane + 32 * e] = from_f<T>(v[e]);
+    }
+  }
+};
+
+// Maps of a turn's warps, and of its blocks, by parity of the turn: a warp is never
+// two turns ahead of another.
+template <int VL>
+struct Exchange {
+  float2 warp[2][kMaxWarps][32 * VL];            // factor's code, Q
+  // (only clusters of several blocks have what follows)
+  float log_a[kMaxWarps][32 * VL];
+  float2 block[2][kMaxCluster][32 * VL];
+  static constexpr size_t kAlone = sizeof(float2) * 2 * kMaxWarps * 32 * VL;
+};
+
+// The state in front of this warp's part of the turn, in the order that `first`
+// and `dir` give (0 and 1 forwards, the last and -1 backwards); `carry` moves on to
+// the state behind the turn.
+template <int VL>
+__device__ __forceinline__ void exchange(Exchange<VL>& x, int parity, int warp, int warps, uint32_t rank,
+                                         uint32_t size, bool back, int lane, const Factor (&a)[VL],
+                                         const float (&log_a)[VL], const float (&q)[VL],
+                                         float (&carry)[VL], float (&h)[VL]) {
+#pragma unroll
+  for (int e = 0; e < VL; ++e) {
+    x.warp[parity][warp][lane + 32 * e] = make_float2(a[e].code, q[e]);
+    if (size > 1) x.log_a[warp][lane + 32 * e] = log_a[e];
+  }
+  __syncthreads();
+  const int at = back ? warps - 1 - warp : warp;         // place in the walk
+  if (size > 1) {
+    if (warp < VL) {          // warp e sums up the block for its 32 channels
+      const int c = lane + 32 * warp;
+      float sum = 0.f, q2 = 0.f;
+      for (int i = 0; i < warps; ++i) {
+        const int w = back ? warps - 1 - i : i;
+        const float2 m = x.warp[parity][w][c];
+        sum += x.log_a[w][c];
+        q2 = Factor{m.x}.step(q2, m.y);
+      }
+      const float2 m = make_float2(factor_of(sum).code, q2);
+      for (uint32_t r = 0; r < size; ++r) store_at_rank(&x.block[parity][rank][c], r, m);
+    }
+    cluster_sync();
+#pragma unroll
+    for (int e = 0; e < VL; ++e) {
+      for (uint32_t i = 0; i < size; ++i) {
+        const uint32_t r = back ? size - 1 - i : i;
+        if (r == rank) h[e] = carry[e];
+        const float2 m = x.block[parity][r][lane + 32 * e];
+        carry[e] = Factor{m.x}.step(carry[e], m.y);
+      }
+      for (int i = 0; i < at; ++i) {
+        const float2 m = x.warp[parity][back ? warps - 1 - i : i][lane + 32 * e];
+        h[e] = Factor{m.x}.step(h[e], m.y);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < VL; ++e) {
+      for (int i = 0; i < warps; ++i) {
+        if (i == at) h[e] = carry[e];
+        const float2 m = x.warp[parity][back ? warps - 1 - i : i][lane + 32 * e];
+        carry[e] = Factor{m.x}.step(carry[e], m.y);
+      }
+    }
+  }
+}
+
+template <class T, int VL, bool ALIGNED>
+__global__ void __launch_bounds__(32 * kMaxWarps, 2) recurrence_fwd_kernel(RecArrays<T> p) {
+  using S = Stage<T, VL, ALIGNED>;
+  extern __shared__ __align__(16) uint8_t raw[];
+  Exchange<VL>& ex = *(Exchange<VL>*)raw;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32;
+  const uint32_t rank = cluster_rank(), size = cluster_size();
+  uint8_t* stage = raw + (size > 1 ? sizeof(Exchange<VL>) : Exchange<VL>::kAlone) + warp * 6 * S::kBytes;
+  const int64_t part = blockIdx.x / size, b = part / p.groups, d0 = part % p.groups * 32 * VL;
+  const int channels = p.channels - d0 < 32 * VL ? (int)(p.channels - d0) : 32 * VL;
   const int64_t len = valid_length(p.lengths, b, p.length);
-  const int64_t saves = (p.length + kSave - 1) / kSave;
-  const float decay = p.decay[d];
-  float later = p.dfinal ? p.dfinal[i] : 0.f, sum = 0.f;
-  for (int64_t t = len; t < p.length; ++t)
-    p.dx.at(b, t)[d] = p.dig.at(b, t)[d] = p.drg.at(b, t)[d] = from_f<T>(0.f);
-  for (int64_t s = (len + kSave - 1) / kSave - 1; s >= 0; --s) {
-    const int64_t t0 = s * kSave;
-    const int n = (int)(len - t0 < kSave ? len - t0 : kSave);
-    float before[kSave];
-    float h = p.saved[(b * saves + s) * p.channels + d];
-    for (int j = 0; j < n; ++j) {
+  const int64_t chunk = (int64_t)size * warps * kSteps, turns = (p.length + chunk - 1) / chunk;
+  const int64_t saves = (p.length + kSteps - 1) / kSteps;
+  int64_t t0 = ((int64_t)rank * warps + warp) * kSteps;
+  float decay[VL], carry[VL];
+#pragma unroll
+  for (int e = 0; e < VL; ++e) {
+    const int c = S::channel(lane, e);
+    decay[e] = c < channels ? p.decay[d0 + c] : 0.f;
+    carry[e] = c < channels && p.initial ? p.initial[b * p.channels + d0 + c] : 0.f;
+  }
+  auto valid = [&](int64_t t) {
+    return (int)(len - t < 0 ? 0 : (len - t < kSteps ? len - t : kSteps));
+  };
+  auto fill = [&](int64_t t, int buf) {
+    const int n = valid(t);
+    if (n > 0) {
+      uint8_t* s = stage + buf * 3 * S::kBytes;
+      S::fill(s, p.x.at(b, t) + d0, p.x.st, n, channels, lane);
+      S::fill(s + S::kBytes, p.ig.at(b, t) + d0, p.ig.st, n, channels, lane);
+      S::fill(s + 2 * S::kBytes, p.rg.at(b, t) + d0, p.rg.st, n, channels, lane);
+    }
+    cp_async_commit();
+  };
+  fill(t0, 0);
+  for (int64_t turn = 0; turn < turns; ++turn, t0 += chunk) {
+    const int parity = (int)(turn & 1), n = valid(t0);
+    __syncwarp();
+    if (turn + 1 < turns)
+      fill(t0 + chunk, parity ^ 1);
+    else
+      cp_async_commit();
+    cp_async_wait_older();
+    __syncwarp();
+    const uint8_t* s = stage + parity * 3 * S::kBytes;
+    const T *px = p.x.at(b, t0) + d0, *pi = p.ig.at(b, t0) + d0, *pr = p.rg.at(b, t0) + d0;
+    Factor a[kSteps][VL], all[VL];
+    float in[kSteps][VL], sum[VL], q[VL], h[VL];
+#pragma unroll
+    for (int e = 0; e < VL; ++e) sum[e] = q[e] = 0.f;
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) {
+      float x[VL], ig[VL], rg[VL];
+      S::load(s, px, p.x.st, j, lane, x);
+      S::load(s + S::kBytes, pi, p.ig.st, j, lane, ig);
+      S::load(s + 2 * S::kBytes, pr, p.rg.st, j, lane, rg);
+#pragma unroll
+      for (int e = 0; e < VL; ++e) {
+        const float r = gate_of(rg[e]).on();
+        const Decay d = decay_of(decay[e], r);
+        a[j][e].code = j < n ? d.a.code : kKeep;
+        in[j][e] = j < n ? d.root() * (gate_of(ig[e]).on() * x[e]) : 0.f;
+        sum[e] += j < n ? r : 0.f;
+        q[e] = a[j][e].step(q[e], in[j][e]);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < VL; ++e) {
+      sum[e] *= -decay[e];
+      all[e] = factor_of(sum[e]);
+    }
+    exchange<VL>(ex, parity, warp, warps, rank, size, false, lane, all, sum, q, carry, h);
+    if (t0 < p.length) {
+      if (p.saved) {
+#pragma unroll
+        for (int e = 0; e < VL; ++e) {
+          const int c = S::channel(lane, e);
+          if (c < channels) p.saved[(b * saves + t0 / kSteps) * p.channels + d0 + c] = h[e];
+        }
+      }
+      T* po = p.out.at(b, t0) + d0;
+      const int rows = p.length - t0 < kSteps ? (int)(p.length - t0) : kSteps;
+#pragma unroll
+      for (int j = 0; j < kSteps; ++j) {
+        if (j >= rows) break;
+        float o[VL];
+#pragma unroll
+        for (int e = 0; e < VL; ++e) {
+          h[e] = a[j][e].step(h[e], in[j][e]);
+          o[e] = j < n ? h[e] : 0.f;
+        }
+        S::store(po, lane, channels, o);
+        po += p.out.st;
+      }
+    }
+  }
+  if (p.final && warp == 0 && rank == 0) {
+#pragma unroll
+    for (int e = 0; e < VL; ++e) {
+      const int c = S::channel(lane, e);
+      if (c < channels) p.final[b * p.channels + d0 + c] = carry[e];
+    }
+  }
+  if (size > 1) cluster_sync();       // no block ends while another may store to it
+}
+
+template <class T, bool ALIGNED, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) recurrence_bwd_kernel(RecArrays<T> p) {
+  using S = Stage<T, 1, ALIGNED>;
+  extern __shared__ __align__(16) uint8_t raw[];
+  Exchange<1>& ex = *(Exchange<1>*)raw;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32;
+  const uint32_t rank = cluster_rank(), size = cluster_size();
+  uint8_t* stage = raw + (size > 1 ? sizeof(Exchange<1>) : Exchange<1>::kAlone) + warp * 8 * S::kBytes;
+  const int64_t part = blockIdx.x / size, b = part / p.groups, d0 = part % p.groups * 32;
+  const int channels = p.channels - d0 < 32 ? (int)(p.channels - d0) : 32;
+  const bool mine = lane < channels;
+  const int64_t len = valid_length(p.lengths, b, p.length), at = b * p.channels + d0 + lane;
+  const int64_t chunk = (int64_t)size * warps * kSteps, turns = (p.length + chunk - 1) / chunk;
+  const int64_t saves = (p.length + kSteps - 1) / kSteps;
+  int64_t t0 = (turns - 1) * chunk + ((int64_t)rank * warps + warp) * kSteps;
+  const float decay = mine ? p.decay[d0 + lane] : 0.f;
+  float carry[1] = {mine && p.dfinal ? p.dfinal[at] : 0.f}, total = 0.f;
+  auto valid = [&](int64_t t) {
+    return (int)(len - t < 0 ? 0 : (len - t < kSteps ? len - t : kSteps));
+  };
+  auto fill = [&](int64_t t, int buf) {
+    const int n = valid(t);
+    if (n > 0) {
+      uint8_t* s = stage + buf * 4 * S::kBytes;
+      S::fill(s, p.x.at(b, t) + d0, p.x.st, n, channels, lane);
+      S::fill(s + S::kBytes, p.ig.at(b, t) + d0, p.ig.st, n, channels, lane);
+      S::fill(s + 2 * S::kBytes, p.rg.at(b, t) + d0, p.rg.st, n, channels, lane);
+      S::fill(s + 3 * S::kBytes, p.dout.at(b, t) + d0, p.dout.st, n, channels, lane);
+    }
+    cp_async_commit();
+  };
+  if (turns > 0) fill(t0, (int)(turns - 1) & 1);
+  for (int64_t turn = turns - 1; turn >= 0; --turn, t0 -= chunk) {
+    const int parity = (int)(turn & 1), n = valid(t0);
+    __syncwarp();
+    if (turn > 0)
+      fill(t0 - chunk, parity ^ 1);
+    else
+      cp_async_commit();
+    float h = n > 0 && mine ? p.saved[(b * saves + t0 / kSteps) * p.channels + d0 + lane] : 0.f;
+    cp_async_wait_older();
+    __syncwarp();
+    const uint8_t* s = stage + parity * 4 * S::kBytes;
+    const T *px = p.x.at(b, t0) + d0, *pi = p.ig.at(b, t0) + d0, *pr = p.rg.at(b, t0) + d0;
+    const T* pg = p.dout.at(b, t0) + d0;
+    Gate i[kSteps], r[kSteps];
+    Decay dec[kSteps];
+    float before[kSteps], sum[1] = {0.f}, q[1] = {0.f}, later[1];
+#pragma unroll
+    for (int j = 0; j < kSteps; ++j) {
+      float x[1], ig[1], rg[1];
+      S::load(s, px, p.x.st, j, lane, x);
+      S::load(s + S::kBytes, pi, p.ig.st, j, lane, ig);
+      S::load(s + 2 * S::kBytes, pr, p.rg.st, j, lane, rg);
+      i[j] = gate_of(ig[0]), r[j] = gate_of(rg[0]);
+      dec[j] = decay_of(decay, r[j].on());
+      if (j >= n) dec[j].a.code = kKeep;
+      sum[0] += j < n ? r[j].on() : 0.f;
       before[j] = h;
-      const Decay a = decay_of(decay, gate_of(to_f(p.rg.at(b, t0 + j)[d])).on);
-      const float u = gate_of(to_f(p.ig.at(b, t0 + j)[d])).on * to_f(p.x.at(b, t0 + j)[d]);
-      h += fmaf(a.m, h, a.root * u);
+      h = dec[j].a.step(h, dec[j].root() * (i[j].on() * x[0]));
     }
-    for (int j = n - 1; j >= 0; --j) {
-      const int64_t t = t0 + j;
-      const Gate r = gate_of(to_f(p.rg.at(b, t)[d])), ig = gate_of(to_f(p.ig.at(b, t)[d]));
-      const Decay a = decay_of(decay, r.on);
-      const float g = to_f(p.dout.at(b, t)[d]) + later;
-      const StepGrads q = step_grads(g, before[j], to_f(p.x.at(b, t)[d]), ig, r, a, decay);
-      p.dx.at(b, t)[d] = from_f<T>(q.dx);
-      p.dig.at(b, t)[d] = from_f<T>(q.dig);
-      p.drg.at(b, t)[d] = from_f<T>(q.drg);
-      sum += q.ddecay;
-      later = fmaf(a.m, g, g);
+#pragma unroll
+    for (int j = kSteps - 1; j >= 0; --j) {
+      float g[1];
+      S::load(s + 3 * S::kBytes, pg, p.dout.st, j, lane, g);
+      q[0] = dec[j].a.times((j < n ? g[0] : 0.f) + q[0]);
+    }
+    sum[0] *= -decay;
+    const Factor all[1] = {factor_of(sum[0])};
+    exchange<1>(ex, parity, warp, warps, rank, size, true, lane, all, sum, q, carry, later);
+    if (t0 < p.length) {
+      const int rows = p.length - t0 < kSteps ? (int)(p.length - t0) : kSteps;
+#pragma unroll
+      for (int j = kSteps - 1; j >= 0; --j) {
+        if (j >= rows) continue;
+        StepGrads o = {0.f, 0.f, 0.f, 0.f};
+        if (j < n) {
+          float x[1], g[1];
+          S::load(s, px, p.x.st, j, lane, x);
+          S::load(s + 3 * S::kBytes, pg, p.dout.st, j, lane, g);
+          g[0] += later[0];
+          o = step_grads(g[0], before[j], x[0], i[j], r[j], dec[j], decay);
+          total += o.ddecay;
+          later[0] = dec[j].a.times(g[0]);
+        }
+        if (mine) {
+          p.dx.at(b, t0 + j)[d0 + lane] = from_f<T>(o.dx);
+          p.dig.at(b, t0 + j)[d0 + lane] = from_f<T>(o.dig);
+          p.drg.at(b, t0 + j)[d0 + lane] = from_f<T>(o.drg);
+        }
+      }
     }
   }
-  part[i] = sum;
-  if (p.dinitial) p.dinitial[i] = later;
+  if (p.dinitial && mine && warp == 0 && rank == 0) p.dinitial[at] = carry[0];
+  // the block's sum of ddecay, warp by warp
+  __syncthreads();
+  ex.warp[0][warp][lane].x = total;
+  __syncthreads();
+  if (warp == 0 && mine) {
+    float v = 0.f;
+    for (int w = 0; w < warps; ++w) v += ex.warp[0][w][lane].x;
+    p.part[(b * size + rank) * p.channels + d0 + lane] = v;
+  }
+  if (size > 1) cluster_sync();
 }
 
 template <class T>
-__global__ void __launch_bounds__(kThreads) recurrence_step_kernel(RecArrays<T> p) {
-  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+__global__ void __launch_bounds__(kStepThreads) recurrence_step_kernel(RecArrays<T> p) {
+  const int64_t i = (int64_t)blockIdx.x * kStepThreads + threadIdx.x;
   if (i >= p.batch * p.channels) return;
   const int64_t b = i / p.channels, d = i % p.channels;
-  const Decay a = decay_of(p.decay[d], gate_of(to_f(p.rg.at(b, 0)[d])).on);
-  const float u = gate_of(to_f(p.ig.at(b, 0)[d])).on * to_f(p.x.at(b, 0)[d]);
-  const float h0 = p.initial[i];
-  const float h = h0 + fmaf(a.m, h0, a.root * u);
+  const Decay a = decay_of(p.decay[d], gate_of(to_f(p.rg.at(b, 0)[d])).on());
+  const float u = gate_of(to_f(p.ig.at(b, 0)[d])).on() * to_f(p.x.at(b, 0)[d]);
+  const float h = a.a.step(p.initial[i], a.root() * u);
   p.out.at(b, 0)[d] = from_f<T>(h);
   p.final[i] = h;
 }
@@ -115,7 +417,7 @@ RecArrays<T> arrays_of(const ferrum_recurrence_args* a) {
   p.dig = rows_of<T>(a->dinput_gate), p.drg = rows_of<T>(a->drecurrence_gate);
   p.decay = a->decay, p.initial = a->initial_state, p.final = a->final_state;
   p.lengths = a->lengths, p.saved = a->saved_states, p.dfinal = a->dfinal_state;
-  p.dinitial = a->dinitial_state;
+  p.dinitial = a->dinitial_state, p.part = nullptr, p.groups = 0;
   p.batch = (int64_t)a->batch, p.length = (int64_t)a->length, p.channels = (int64_t)a->channels;
   return p;
 }
@@ -155,6 +457,89 @@ ferrum_status check_recurrence(const ferrum_device* dev, const ferrum_recurrence
   return FERRUM_OK;
 }
 
+// Blocks of a cluster: more of them where there are few rows of channels, as long
+// as each has steps to walk.
+int cluster_of(int64_t parts, int64_t length, int warps) {
+  int c = 1;
+  while (c < kMaxCluster && parts * c * 2 <= 148 * 2 && (int64_t)c * warps * kSteps < length) c *= 2;
+  return c;
+}
+
+// Warps of a block, 16 steps each: no more than the steps need, nor than let two
+// blocks share an SM's 228 KiB.
+struct Shape {
+  int cluster, warps;
+  size_t smem;
+};
+template <class X>
+Shape shape_of(int64_t parts, int64_t length, int most, size_t per_warp) {
+  auto fit = [&](size_t fixed) {
+    const int64_t room = (int64_t)((113 * 1024 - fixed) / per_warp);
+    return (int)std::max<int64_t>(1, std::min<int64_t>({most, room, ceil_div(length, kSteps)}));
+  };
+  Shape s;
+  s.warps = fit(X::kAlone);
+  s.cluster = cluster_of(parts, length, s.warps);
+  if (s.cluster > 1) s.warps = fit(sizeof(X));
+  s.smem = (s.cluster > 1 ? sizeof(X) : X::kAlone) + s.warps * per_warp;
+  return s;
+}
+
+bool rows_aligned(std::initializer_list<const ferrum_rows*> arrays, size_t e) {
+  for (const ferrum_rows* r : arrays)
+    if (!aligned(r->ptr, 16) || r->batch_stride * (int64_t)e % 16 != 0 ||
+        r->row_stride * (int64_t)e % 16 != 0)
+      return false;
+  return true;
+}
+
+template <class K, class T>
+ferrum_status launch(K kernel, std::atomic<uint64_t>& smem_done, const RecArrays<T>& p, const Shape& s,
+                     cudaStream_t stream, const char* what) {
+  const int64_t blocks = p.batch * p.groups * s.cluster;
+  if (blocks > 0x7fffffff) return invalid(what, "too many blocks for one launch");
+  cudaError_t e = launch_detail::ensure_smem(kernel, 113 * 1024, smem_done);
+  if (e != cudaSuccess) return cuda_error(e, what);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)s.cluster, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)blocks), cfg.blockDim = dim3(32 * s.warps);
+  cfg.dynamicSmemBytes = s.smem, cfg.stream = stream, cfg.attrs = attr, cfg.numAttrs = 1;
+  launch_detail::clear_stale_error();
+  e = cudaLaunchKernelEx(&cfg, kernel, p);
+  return e == cudaSuccess ? FERRUM_OK : cuda_error(e, what);
+}
+
+template <class T, int VL, bool ALIGNED>
+ferrum_status run_fwd(RecArrays<T> p, cudaStream_t stream, const char* what) {
+  static std::atomic<uint64_t> smem_done{0};
+  p.groups = ceil_div(p.channels, 32 * VL);
+  const Shape s = shape_of<Exchange<VL>>(p.batch * p.groups, p.length, kMaxWarps,
+                                         6 * Stage<T, VL, ALIGNED>::kBytes);
+  return launch(recurrence_fwd_kernel<T, VL, ALIGNED>, smem_done, p, s, stream, what);
+}
+
+template <class T, bool ALIGNED>
+ferrum_status run_bwd(ferrum_device* dev, RecArrays<T> p, float* ddecay, cudaStream_t stream,
+                      const char* what) {
+  static std::atomic<uint64_t> smem_done{0};
+  constexpr int kWarps = sizeof(T) == 4 ? 4 : 8;
+  p.groups = ceil_div(p.channels, 32);
+  const Shape s = shape_of<Exchange<1>>(p.batch * p.groups, p.length, kWarps,
+                                        8 * Stage<T, 1, ALIGNED>::kBytes);
+  const int64_t sums = p.batch * s.cluster;
+  PoolBuffer ws(dev, (size_t)(sums * p.channels) * 4 + 4, stream);
+  if (ws.status() != cudaSuccess) return cuda_error(ws.status(), "workspace");
+  p.part = ws.as<float>();
+  if (p.batch > 0) {
+    if (ferrum_status f = launch(recurrence_bwd_kernel<T, ALIGNED, kWarps>, smem_done, p, s, stream, what))
+      return f;
+  }
+  cudaError_t e = launch_sum_rows(p.part, sums, p.channels, p.channels, ddecay, nullptr, stream);
+  return e == cudaSuccess ? FERRUM_OK : cuda_error(e, what);
+}
+
 }  // namespace
 }  // namespace seq
 }  // namespace ferrum
@@ -175,10 +560,12 @@ ferrum_status ferrum_gated_recurrence(ferrum_device* dev, const ferrum_recurrenc
     if (guard.status() != cudaSuccess) return cuda_error(guard.status(), "cudaSetDevice");
     return with_dtype(a->dtype, [&](auto tag) {
       using T = decltype(tag);
-      launch_detail::clear_stale_error();
-      recurrence_fwd_kernel<T><<<(unsigned)ceil_div(n, kThreads), kThreads, 0, (cudaStream_t)stream>>>(
-          arrays_of<T>(a));
-      return launched(what);
+      constexpr int VL = sizeof(T) == 2 ? 2 : 1;
+      const bool wide = rows_aligned({&a->x, &a->input_gate, &a->recurrence_gate, &a->out}, sizeof(T)) &&
+                        a->channels % VL == 0;
+      const RecArrays<T> p = arrays_of<T>(a);
+      return wide ? run_fwd<T, VL, true>(p, (cudaStream_t)stream, what)
+                  : run_fwd<T, VL, false>(p, (cudaStream_t)stream, what);
     });
   });
 }
@@ -189,23 +576,16 @@ ferrum_status ferrum_gated_recurrence_bwd(ferrum_device* dev, const ferrum_recur
   return guarded(what, [&]() -> ferrum_status {
     if (ferrum_status s = check_recurrence(dev, a, what, true)) return s;
     if (a->channels == 0) return FERRUM_OK;
-    const int64_t n = (int64_t)a->batch * (int64_t)a->channels;
     cudaStream_t st = (cudaStream_t)stream;
     DeviceGuard guard(dev->ordinal);
     if (guard.status() != cudaSuccess) return cuda_error(guard.status(), "cudaSetDevice");
-    return with_dtype(a->dtype, [&](auto tag) -> ferrum_status {
+    return with_dtype(a->dtype, [&](auto tag) {
       using T = decltype(tag);
-      PoolBuffer ws(dev, (size_t)n * 4 + 4, st);
-      if (ws.status() != cudaSuccess) return cuda_error(ws.status(), "workspace");
-      if (n > 0) {
-        launch_detail::clear_stale_error();
-        recurrence_bwd_kernel<T><<<(unsigned)ceil_div(n, kThreads), kThreads, 0, st>>>(
-            arrays_of<T>(a), ws.as<float>());
-        if (ferrum_status s = launched(what)) return s;
-      }
-      cudaError_t e = launch_sum_rows(ws.as<float>(), (int64_t)a->batch, (int64_t)a->channels,
-                                      (int64_t)a->channels, a->ddecay, nullptr, st);
-      return e == cudaSuccess ? FERRUM_OK : cuda_error(e, what);
+      const bool wide =
+          rows_aligned({&a->x, &a->input_gate, &a->recurrence_gate, &a->dout}, sizeof(T));
+      const RecArrays<T> p = arrays_of<T>(a);
+      return wide ? run_bwd<T, true>(dev, p, a->ddecay, st, what)
+                  : run_bwd<T, false>(dev, p, a->ddecay, st, what);
     });
   });
 }
@@ -226,7 +606,7 @@ ferrum_status ferrum_gated_recurrence_step(ferrum_device* dev, const ferrum_recu
     return with_dtype(a->dtype, [&](auto tag) {
       using T = decltype(tag);
       launch_detail::clear_stale_error();
-      recurrence_step_kernel<T><<<(unsigned)ceil_div(n, kThreads), kThreads, 0,
+      recurrence_step_kernel<T><<<(unsigned)ceil_div(n, kStepThreads), kStepThreads, 0,
                                   (cudaStream_t)stream>>>(arrays_of<T>(a));
       return launched(what);
     });
