@@ -71,37 +71,55 @@ __device__ __forceinline__ void store_at_rank(float2* p, uint32_t rank, float2 v
   asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(a), "f"(v.x), "f"(v.y) : "memory");
 }
 
-// A warp's rows of one array in shared memory: 16 steps of 32 * VL channels.
-// ALIGNED: rows begin at multiples of 16 bytes. Otherwise a row's copy begins at the
-// 16-byte unit that holds its first value, so up to 14 bytes in front of it come
-// along, from the same unit; behind its last value nothing is read.
-template <class T, int VL, bool ALIGNED>
+// How the rows of a call lie: at multiples of 16 bytes, of 4 bytes with an even
+// number of channels (16-bit types), or of an element.
+enum Lie { kWhole, kPaired, kSingle };
+
+// A warp's rows of one array in shared memory: 16 steps of 32 * VL channels. Where
+// rows do not begin at multiples of 16 bytes, a row's copy begins at the 16-byte
+// unit that holds its first value, so up to 14 bytes in front of it come along, from
+// the same unit; behind its last value nothing is read.
+template <class T, int VL, int LIE>
 struct Stage {
-  static constexpr int kRow = 32 * VL * (int)sizeof(T), kPitch = kRow + (ALIGNED ? 0 : 16);
+  static constexpr int kRow = 32 * VL * (int)sizeof(T), kPitch = kRow + (LIE == kWhole ? 0 : 16);
   static constexpr int kUnits = kPitch / 16, kBytes = kSteps * kPitch;
   // Steps [0, n) from `p` on, `st` values apart, `channels` of them.
   static __device__ __forceinline__ void fill(uint8_t* s, const T* p, int64_t st, int n, int channels,
                                               int lane) {
+    if constexpr (LIE == kWhole) {
+      // 32 / kUnits rows at a time: a lane keeps its place in the row
+      constexpr int kAtOnce = 32 / kUnits;
+      const int step = lane / kUnits, unit = lane % kUnits;
+      const int left = channels * (int)sizeof(T) - unit * 16, bytes = left < 0 ? 0 : (left < 16 ? left : 16);
+      const T* src = p + step * st + (bytes ? unit * (16 / (int)sizeof(T)) : 0);
+      uint8_t* dst = s + step * kPitch + unit * 16;
 #pragma unroll
-    for (int i = 0; i < (kSteps * kUnits + 31) / 32; ++i) {
-      const int e = i * 32 + lane, step = e / kUnits, unit = e % kUnits;
-      if (kSteps * kUnits % 32 != 0 && step >= kSteps) break;
-      const uint8_t* row = (const uint8_t*)(p + (step < n ? step : 0) * st);
-      const uint8_t* src = (ALIGNED ? row : (const uint8_t*)((uintptr_t)row & ~(uintptr_t)15)) + unit * 16;
-      const int left = (int)(row - src) + channels * (int)sizeof(T);
-      const int bytes = step >= n || left <= 0 ? 0 : (left < 16 ? left : 16);
-      cp_async<16>(s + step * kPitch + unit * 16, bytes ? src : row - ((uintptr_t)row & 15), bytes);
+      for (int i = 0; i < kSteps / kAtOnce; ++i)
+        if (i * kAtOnce < n - step) cp_async<16>(dst + i * kAtOnce * kPitch, src + i * kAtOnce * st, bytes);
+    } else {
+#pragma unroll
+      for (int i = 0; i < (kSteps * kUnits + 31) / 32; ++i) {
+        const int e = i * 32 + lane, step = e / kUnits, unit = e % kUnits;
+        if (step >= n) break;
+        const uint8_t* row = (const uint8_t*)(p + step * st);
+        const int in_front = (int)((uintptr_t)row & 15);
+        const int left = in_front + channels * (int)sizeof(T) - unit * 16;
+        const int bytes = left < 0 ? 0 : (left < 16 ? left : 16);
+        cp_async<16>(s + step * kPitch + unit * 16, row - in_front + (bytes ? unit * 16 : 0), bytes);
+      }
     }
   }
-  // Channels 2 * lane and the next one (aligned, 16 bits), else lane and lane + 32.
-  static constexpr bool kPairs = ALIGNED && VL == 2;
+  // Channels 2 * lane and the next one, else lane and lane + 32.
+  static constexpr bool kPairs = LIE != kSingle && VL == 2;
   static __device__ __forceinline__ int channel(int lane, int e) {
     return kPairs ? 2 * lane + e : lane + 32 * e;
   }
   static __device__ __forceinline__ void load(const uint8_t* s, const T* p, int64_t st, int step, int lane,
                                               float (&v)[VL]) {
     const uint8_t* row = s + step * kPitch;
-    if constexpr (!ALIGNED) row += (uintptr_t)(p + step * st) & 15;
+    // (the low bits of the row's address)
+    if constexpr (LIE != kWhole)
+      row += ((uint32_t)(uintptr_t)p + (uint32_t)step * (uint32_t)st * (uint32_t)sizeof(T)) & 15;
     if constexpr (kPairs) {
       load_vec<T, 2>((const T*)row + 2 * lane, v);
     } else {
@@ -185,9 +203,9 @@ __device__ __forceinline__ void exchange(Exchange<VL>& x, int parity, int warp, 
   }
 }
 
-template <class T, int VL, bool ALIGNED>
+template <class T, int VL, int LIE>
 __global__ void __launch_bounds__(32 * kMaxWarps, 2) recurrence_fwd_kernel(RecArrays<T> p) {
-  using S = Stage<T, VL, ALIGNED>;
+  using S = Stage<T, VL, LIE>;
   extern __shared__ __align__(16) uint8_t raw[];
   Exchange<VL>& ex = *(Exchange<VL>*)raw;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32;
@@ -206,6 +224,10 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 2) recurrence_fwd_kernel(RecAr
     decay[e] = c < channels ? p.decay[d0 + c] : 0.f;
     carry[e] = c < channels && p.initial ? p.initial[b * p.channels + d0 + c] : 0.f;
   }
+  bool mild = true;
+#pragma unroll
+  for (int e = 0; e < VL; ++e) mild = mild && decay[e] >= 0.f && decay[e] <= kShortDecay;
+  mild = __all_sync(0xffffffffu, mild);
   auto valid = [&](int64_t t) {
     return (int)(len - t < 0 ? 0 : (len - t < kSteps ? len - t : kSteps));
   };
@@ -231,33 +253,37 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 2) recurrence_fwd_kernel(RecAr
     __syncwarp();
     const uint8_t* s = stage + parity * 3 * S::kBytes;
     const T *px = p.x.at(b, t0) + d0, *pi = p.ig.at(b, t0) + d0, *pr = p.rg.at(b, t0) + d0;
-    Factor a[kSteps][VL], all[VL];
-    float in[kSteps][VL], sum[VL], q[VL], h[VL];
+    // SHORT: all steps inside the sequence, all decays in expm1_short's range
+    auto walk = [&](auto is_short) {
+      constexpr bool SHORT = decltype(is_short)::value;
+      Factor a[kSteps][VL], all[VL];
+      float in[kSteps][VL], sum[VL], q[VL], h[VL];
 #pragma unroll
-    for (int e = 0; e < VL; ++e) sum[e] = q[e] = 0.f;
+      for (int e = 0; e < VL; ++e) sum[e] = q[e] = 0.f;
 #pragma unroll
-    for (int j = 0; j < kSteps; ++j) {
-      float x[VL], ig[VL], rg[VL];
-      S::load(s, px, p.x.st, j, lane, x);
-      S::load(s + S::kBytes, pi, p.ig.st, j, lane, ig);
-      S::load(s + 2 * S::kBytes, pr, p.rg.st, j, lane, rg);
+      for (int j = 0; j < kSteps; ++j) {
+        float x[VL], ig[VL], rg[VL];
+        S::load(s, px, p.x.st, j, lane, x);
+        S::load(s + S::kBytes, pi, p.ig.st, j, lane, ig);
+        S::load(s + 2 * S::kBytes, pr, p.rg.st, j, lane, rg);
+#pragma unroll
+        for (int e = 0; e < VL; ++e) {
+          const float r = sigmoid_f(rg[e]);
+          float w;
+          a[j][e] = step_factor<SHORT>(decay[e], r, w);
+          in[j][e] = root_of(w) * (sigmoid_f(ig[e]) * x[e]);
+          if (SHORT || j < n) sum[e] += r;
+          if (!SHORT && j >= n) a[j][e].code = kKeep, in[j][e] = 0.f;
+          q[e] = step_on<SHORT>(a[j][e], q[e], in[j][e]);
+        }
+      }
 #pragma unroll
       for (int e = 0; e < VL; ++e) {
-        const float r = gate_of(rg[e]).on();
-        const Decay d = decay_of(decay[e], r);
-        a[j][e].code = j < n ? d.a.code : kKeep;
-        in[j][e] = j < n ? d.root() * (gate_of(ig[e]).on() * x[e]) : 0.f;
-        sum[e] += j < n ? r : 0.f;
-        q[e] = a[j][e].step(q[e], in[j][e]);
+        sum[e] *= -decay[e];
+        all[e] = factor_of(sum[e]);
       }
-    }
-#pragma unroll
-    for (int e = 0; e < VL; ++e) {
-      sum[e] *= -decay[e];
-      all[e] = factor_of(sum[e]);
-    }
-    exchange<VL>(ex, parity, warp, warps, rank, size, false, lane, all, sum, q, carry, h);
-    if (t0 < p.length) {
+      exchange<VL>(ex, parity, warp, warps, rank, size, false, lane, all, sum, q, carry, h);
+      if (t0 >= p.length) return;
       if (p.saved) {
 #pragma unroll
         for (int e = 0; e < VL; ++e) {
@@ -269,17 +295,21 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 2) recurrence_fwd_kernel(RecAr
       const int rows = p.length - t0 < kSteps ? (int)(p.length - t0) : kSteps;
 #pragma unroll
       for (int j = 0; j < kSteps; ++j) {
-        if (j >= rows) break;
+        if (!SHORT && j >= rows) break;
         float o[VL];
 #pragma unroll
         for (int e = 0; e < VL; ++e) {
-          h[e] = a[j][e].step(h[e], in[j][e]);
-          o[e] = j < n ? h[e] : 0.f;
+          h[e] = step_on<SHORT>(a[j][e], h[e], in[j][e]);
+          o[e] = SHORT || j < n ? h[e] : 0.f;
         }
         S::store(po, lane, channels, o);
         po += p.out.st;
       }
-    }
+    };
+    if (n == kSteps && mild)
+      walk(std::true_type());
+    else
+      walk(std::false_type());
   }
   if (p.final && warp == 0 && rank == 0) {
 #pragma unroll
@@ -291,9 +321,9 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 2) recurrence_fwd_kernel(RecAr
   if (size > 1) cluster_sync();       // no block ends while another may store to it
 }
 
-template <class T, bool ALIGNED, int WARPS>
+template <class T, int LIE, int WARPS>
 __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) recurrence_bwd_kernel(RecArrays<T> p) {
-  using S = Stage<T, 1, ALIGNED>;
+  using S = Stage<T, 1, LIE>;
   extern __shared__ __align__(16) uint8_t raw[];
   Exchange<1>& ex = *(Exchange<1>*)raw;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32;
@@ -307,6 +337,7 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) recurrence_bwd_kernel(
   const int64_t saves = (p.length + kSteps - 1) / kSteps;
   int64_t t0 = (turns - 1) * chunk + ((int64_t)rank * warps + warp) * kSteps;
   const float decay = mine ? p.decay[d0 + lane] : 0.f;
+  const bool mild = __all_sync(0xffffffffu, decay >= 0.f && decay <= kShortDecay);
   float carry[1] = {mine && p.dfinal ? p.dfinal[at] : 0.f}, total = 0.f;
   auto valid = [&](int64_t t) {
     return (int)(len - t < 0 ? 0 : (len - t < kSteps ? len - t : kSteps));
@@ -336,53 +367,66 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) recurrence_bwd_kernel(
     const uint8_t* s = stage + parity * 4 * S::kBytes;
     const T *px = p.x.at(b, t0) + d0, *pi = p.ig.at(b, t0) + d0, *pr = p.rg.at(b, t0) + d0;
     const T* pg = p.dout.at(b, t0) + d0;
-    Gate i[kSteps], r[kSteps];
-    Decay dec[kSteps];
-    float before[kSteps], sum[1] = {0.f}, q[1] = {0.f}, later[1];
+    // Every gradient of a step is its state's gradient g times a number that the
+    // walk forwards computes: dx = g root i, dig = dx x (1 - i),
+    // ddecay = -g r a (h - a / root i x), drg = ddecay decay (1 - r).
+    auto walk = [&](auto is_short) {
+      constexpr bool SHORT = decltype(is_short)::value;
+      Factor a[kSteps];
+      float fx[kSteps], fi[kSteps], fr[kSteps], fd[kSteps];
+      float sum[1] = {0.f}, q[1] = {0.f}, later[1];
 #pragma unroll
-    for (int j = 0; j < kSteps; ++j) {
-      float x[1], ig[1], rg[1];
-      S::load(s, px, p.x.st, j, lane, x);
-      S::load(s + S::kBytes, pi, p.ig.st, j, lane, ig);
-      S::load(s + 2 * S::kBytes, pr, p.rg.st, j, lane, rg);
-      i[j] = gate_of(ig[0]), r[j] = gate_of(rg[0]);
-      dec[j] = decay_of(decay, r[j].on());
-      if (j >= n) dec[j].a.code = kKeep;
-      sum[0] += j < n ? r[j].on() : 0.f;
-      before[j] = h;
-      h = dec[j].a.step(h, dec[j].root() * (i[j].on() * x[0]));
-    }
-#pragma unroll
-    for (int j = kSteps - 1; j >= 0; --j) {
-      float g[1];
-      S::load(s + 3 * S::kBytes, pg, p.dout.st, j, lane, g);
-      q[0] = dec[j].a.times((j < n ? g[0] : 0.f) + q[0]);
-    }
-    sum[0] *= -decay;
-    const Factor all[1] = {factor_of(sum[0])};
-    exchange<1>(ex, parity, warp, warps, rank, size, true, lane, all, sum, q, carry, later);
-    if (t0 < p.length) {
-      const int rows = p.length - t0 < kSteps ? (int)(p.length - t0) : kSteps;
+      for (int j = 0; j < kSteps; ++j) {
+        float x[1], ig[1], rg[1], w;
+        S::load(s, px, p.x.st, j, lane, x);
+        S::load(s + S::kBytes, pi, p.ig.st, j, lane, ig);
+        S::load(s + 2 * S::kBytes, pr, p.rg.st, j, lane, rg);
+        const Gate i = gate_of(ig[0]), r = gate_of(rg[0]);
+        a[j] = step_factor<SHORT>(decay, r.on, w);
+        const float inv = inverse_root_of(w), factor = SHORT ? 1.f + a[j].code : a[j].value();
+        fx[j] = w * inv * i.on;
+        const float in = fx[j] * x[0];
+        fi[j] = in * i.off;
+        fd[j] = -r.on * factor * fmaf(-factor * inv, i.on * x[0], h);
+        fr[j] = fd[j] * decay * r.off;
+        if (SHORT || j < n) sum[0] += r.on;
+        if (!SHORT && j >= n) a[j].code = kKeep;
+        h = step_on<SHORT>(a[j], h, in);
+      }
 #pragma unroll
       for (int j = kSteps - 1; j >= 0; --j) {
-        if (j >= rows) continue;
-        StepGrads o = {0.f, 0.f, 0.f, 0.f};
-        if (j < n) {
-          float x[1], g[1];
-          S::load(s, px, p.x.st, j, lane, x);
-          S::load(s + 3 * S::kBytes, pg, p.dout.st, j, lane, g);
-          g[0] += later[0];
-          o = step_grads(g[0], before[j], x[0], i[j], r[j], dec[j], decay);
-          total += o.ddecay;
-          later[0] = dec[j].a.times(g[0]);
-        }
-        if (mine) {
-          p.dx.at(b, t0 + j)[d0 + lane] = from_f<T>(o.dx);
-          p.dig.at(b, t0 + j)[d0 + lane] = from_f<T>(o.dig);
-          p.drg.at(b, t0 + j)[d0 + lane] = from_f<T>(o.drg);
-        }
+        float g[1];
+        S::load(s + 3 * S::kBytes, pg, p.dout.st, j, lane, g);
+        q[0] = step_times<SHORT>(a[j], (SHORT || j < n ? g[0] : 0.f) + q[0]);
       }
-    }
+      sum[0] *= -decay;
+      const Factor all[1] = {factor_of(sum[0])};
+      exchange<1>(ex, parity, warp, warps, rank, size, true, lane, all, sum, q, carry, later);
+      if (t0 >= p.length) return;
+      const int rows = p.length - t0 < kSteps ? (int)(p.length - t0) : kSteps;
+      T* ox = p.dx.at(b, t0 + rows - 1) + d0 + lane;
+      T* oi = p.dig.at(b, t0 + rows - 1) + d0 + lane;
+      T* orr = p.drg.at(b, t0 + rows - 1) + d0 + lane;
+#pragma unroll
+      for (int j = kSteps - 1; j >= 0; --j) {
+        if (!SHORT && j >= rows) continue;
+        float g[1];
+        S::load(s + 3 * S::kBytes, pg, p.dout.st, j, lane, g);
+        const bool on = SHORT || j < n;
+        g[0] += later[0];
+        if (on) total = fmaf(g[0], fd[j], total), later[0] = step_times<SHORT>(a[j], g[0]);
+        if (mine) {
+          *ox = from_f<T>(on ? g[0] * fx[j] : 0.f);
+          *oi = from_f<T>(on ? g[0] * fi[j] : 0.f);
+          *orr = from_f<T>(on ? g[0] * fr[j] : 0.f);
+        }
+        ox -= p.dx.st, oi -= p.dig.st, orr -= p.drg.st;
+      }
+    };
+    if (n == kSteps && mild)
+      walk(std::true_type());
+    else
+      walk(std::false_type());
   }
   if (p.dinitial && mine && warp == 0 && rank == 0) p.dinitial[at] = carry[0];
   // the block's sum of ddecay, warp by warp
@@ -397,16 +441,27 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) recurrence_bwd_kernel(
   if (size > 1) cluster_sync();
 }
 
-template <class T>
+// One step of every sequence, VL channels a thread, each read before it is written.
+template <class T, int VL>
 __global__ void __launch_bounds__(kStepThreads) recurrence_step_kernel(RecArrays<T> p) {
+  const uint32_t per = (uint32_t)(p.channels / VL);
   const int64_t i = (int64_t)blockIdx.x * kStepThreads + threadIdx.x;
-  if (i >= p.batch * p.channels) return;
-  const int64_t b = i / p.channels, d = i % p.channels;
-  const Decay a = decay_of(p.decay[d], gate_of(to_f(p.rg.at(b, 0)[d])).on());
-  const float u = gate_of(to_f(p.ig.at(b, 0)[d])).on() * to_f(p.x.at(b, 0)[d]);
-  const float h = a.a.step(p.initial[i], a.root() * u);
-  p.out.at(b, 0)[d] = from_f<T>(h);
-  p.final[i] = h;
+  if (i >= p.batch * per) return;
+  const int64_t b = i <= 0xffffffffll ? (uint32_t)i / per : i / per, d = (i - b * per) * VL;
+  float x[VL], ig[VL], rg[VL], decay[VL], h[VL];
+  load_vec<T, VL>(p.x.at(b, 0) + d, x);
+  load_vec<T, VL>(p.ig.at(b, 0) + d, ig);
+  load_vec<T, VL>(p.rg.at(b, 0) + d, rg);
+  load_vec<float, VL>(p.decay + d, decay);
+  load_vec<float, VL>(p.initial + b * p.channels + d, h);
+#pragma unroll
+  for (int e = 0; e < VL; ++e) {
+    float w;
+    const Factor a = factor_of(-decay[e] * sigmoid_f(rg[e]), &w);
+    h[e] = a.step(h[e], root_of(w) * (sigmoid_f(ig[e]) * x[e]));
+  }
+  store_vec<T, VL>(p.out.at(b, 0) + d, h);
+  store_vec<float, VL>(p.final + b * p.channels + d, h);
 }
 
 template <class T>
@@ -485,10 +540,10 @@ Shape shape_of(int64_t parts, int64_t length, int most, size_t per_warp) {
   return s;
 }
 
-bool rows_aligned(std::initializer_list<const ferrum_rows*> arrays, size_t e) {
+bool rows_aligned(std::initializer_list<const ferrum_rows*> arrays, size_t e, int64_t bytes) {
   for (const ferrum_rows* r : arrays)
-    if (!aligned(r->ptr, 16) || r->batch_stride * (int64_t)e % 16 != 0 ||
-        r->row_stride * (int64_t)e % 16 != 0)
+    if (!aligned(r->ptr, (size_t)bytes) || r->batch_stride * (int64_t)e % bytes != 0 ||
+        r->row_stride * (int64_t)e % bytes != 0)
       return false;
   return true;
 }
@@ -511,29 +566,29 @@ ferrum_status launch(K kernel, std::atomic<uint64_t>& smem_done, const RecArrays
   return e == cudaSuccess ? FERRUM_OK : cuda_error(e, what);
 }
 
-template <class T, int VL, bool ALIGNED>
+template <class T, int VL, int LIE>
 ferrum_status run_fwd(RecArrays<T> p, cudaStream_t stream, const char* what) {
   static std::atomic<uint64_t> smem_done{0};
   p.groups = ceil_div(p.channels, 32 * VL);
   const Shape s = shape_of<Exchange<VL>>(p.batch * p.groups, p.length, kMaxWarps,
-                                         6 * Stage<T, VL, ALIGNED>::kBytes);
-  return launch(recurrence_fwd_kernel<T, VL, ALIGNED>, smem_done, p, s, stream, what);
+                                         6 * Stage<T, VL, LIE>::kBytes);
+  return launch(recurrence_fwd_kernel<T, VL, LIE>, smem_done, p, s, stream, what);
 }
 
-template <class T, bool ALIGNED>
+template <class T, int LIE>
 ferrum_status run_bwd(ferrum_device* dev, RecArrays<T> p, float* ddecay, cudaStream_t stream,
                       const char* what) {
   static std::atomic<uint64_t> smem_done{0};
   constexpr int kWarps = sizeof(T) == 4 ? 4 : 8;
   p.groups = ceil_div(p.channels, 32);
   const Shape s = shape_of<Exchange<1>>(p.batch * p.groups, p.length, kWarps,
-                                        8 * Stage<T, 1, ALIGNED>::kBytes);
+                                        8 * Stage<T, 1, LIE>::kBytes);
   const int64_t sums = p.batch * s.cluster;
   PoolBuffer ws(dev, (size_t)(sums * p.channels) * 4 + 4, stream);
   if (ws.status() != cudaSuccess) return cuda_error(ws.status(), "workspace");
   p.part = ws.as<float>();
   if (p.batch > 0) {
-    if (ferrum_status f = launch(recurrence_bwd_kernel<T, ALIGNED, kWarps>, smem_done, p, s, stream, what))
+    if (ferrum_status f = launch(recurrence_bwd_kernel<T, LIE, kWarps>, smem_done, p, s, stream, what))
       return f;
   }
   cudaError_t e = launch_sum_rows(p.part, sums, p.channels, p.channels, ddecay, nullptr, stream);
@@ -561,11 +616,17 @@ ferrum_status ferrum_gated_recurrence(ferrum_device* dev, const ferrum_recurrenc
     return with_dtype(a->dtype, [&](auto tag) {
       using T = decltype(tag);
       constexpr int VL = sizeof(T) == 2 ? 2 : 1;
-      const bool wide = rows_aligned({&a->x, &a->input_gate, &a->recurrence_gate, &a->out}, sizeof(T)) &&
-                        a->channels % VL == 0;
+      cudaStream_t st = (cudaStream_t)stream;
       const RecArrays<T> p = arrays_of<T>(a);
-      return wide ? run_fwd<T, VL, true>(p, (cudaStream_t)stream, what)
-                  : run_fwd<T, VL, false>(p, (cudaStream_t)stream, what);
+      auto lie = [&](int64_t bytes) {
+        return rows_aligned({&a->x, &a->input_gate, &a->recurrence_gate, &a->out}, sizeof(T), bytes);
+      };
+      const bool even = a->channels % VL == 0;
+      if (even && lie(16)) return run_fwd<T, VL, kWhole>(p, st, what);
+      if constexpr (VL == 2) {
+        if (even && lie(4)) return run_fwd<T, VL, kPaired>(p, st, what);
+      }
+      return run_fwd<T, VL, kSingle>(p, st, what);
     });
   });
 }
@@ -582,10 +643,10 @@ ferrum_status ferrum_gated_recurrence_bwd(ferrum_device* dev, const ferrum_recur
     return with_dtype(a->dtype, [&](auto tag) {
       using T = decltype(tag);
       const bool wide =
-          rows_aligned({&a->x, &a->input_gate, &a->recurrence_gate, &a->dout}, sizeof(T));
+          rows_aligned({&a->x, &a->input_gate, &a->recurrence_gate, &a->dout}, sizeof(T), 16);
       const RecArrays<T> p = arrays_of<T>(a);
-      return wide ? run_bwd<T, true>(dev, p, a->ddecay, st, what)
-                  : run_bwd<T, false>(dev, p, a->ddecay, st, what);
+      return wide ? run_bwd<T, kWhole>(dev, p, a->ddecay, st, what)
+                  : run_bwd<T, kSingle>(dev, p, a->ddecay, st, what);
     });
   });
 }
@@ -603,11 +664,21 @@ ferrum_status ferrum_gated_recurrence_step(ferrum_device* dev, const ferrum_recu
     if (n == 0) return FERRUM_OK;
     DeviceGuard guard(dev->ordinal);
     if (guard.status() != cudaSuccess) return cuda_error(guard.status(), "cudaSetDevice");
-    return with_dtype(a->dtype, [&](auto tag) {
+    return with_dtype(a->dtype, [&](auto tag) -> ferrum_status {
       using T = decltype(tag);
+      const RecArrays<T> p = arrays_of<T>(a);
+      cudaStream_t st = (cudaStream_t)stream;
+      const bool wide = a->channels % 4 == 0 && aligned(a->decay, 16) && aligned(a->initial_state, 16) &&
+                        aligned(a->final_state, 16) &&
+                        rows_aligned({&a->x, &a->input_gate, &a->recurrence_gate, &a->out}, sizeof(T),
+                                     4 * sizeof(T));
+      const int64_t blocks = ceil_div(wide ? n / 4 : n, kStepThreads);
+      if (blocks > 0x7fffffff || a->channels > 0xffffffffull) return invalid(what, "too many values for one launch");
       launch_detail::clear_stale_error();
-      recurrence_step_kernel<T><<<(unsigned)ceil_div(n, kStepThreads), kStepThreads, 0,
-                                  (cudaStream_t)stream>>>(arrays_of<T>(a));
+      if (wide)
+        recurrence_step_kernel<T, 4><<<(unsigned)blocks, kStepThreads, 0, st>>>(p);
+      else
+        recurrence_step_kernel<T, 1><<<(unsigned)blocks, kStepThreads, 0, st>>>(p);
       return launched(what);
     });
   });
