@@ -89,6 +89,7 @@ struct Product {
   int64_t m, n;
   int tiles_m, tiles_n, splits, steps, steps_per_split;
   bool a_mn;                 // A's rows run along the depth (as all of B's in kWeights)
+  bool tokens;               // its rows are tokens (dx)
   bool sums;                 // the result: float32 sums, a slab per split (else 16 bits)
   bool load, store_map;      // sums of earlier pieces come on top; `out` has a tensor map
   void* out;
@@ -147,7 +148,8 @@ struct Shared {
 };
 
 // A bounded wait; once one has run out, all others of the CTA end too.
-__device__ __forceinline__ bool wait(Shared* sh, uint64_t* bar, uint32_t phase, int* err_flag) {
+template <class S>
+__device__ __forceinline__ bool wait(S* sh, uint64_t* bar, uint32_t phase, int* err_flag) {
   if (mbar_try_wait(bar, phase)) return true;
   const uint64_t t0 = global_ns();
   while (!mbar_try_wait(bar, phase)) {
@@ -179,7 +181,7 @@ __device__ __forceinline__ RowCoef row_ahead(const Work& w, const Place& q, int6
     if (m < w.p[0].m) r = w.rows[m];
   } else {
     const Product& p = w.p[q.product];
-    if (!p.a_mn && m < p.m) r.target = w.rows[m].target;
+    if (p.tokens && m < p.m) r.target = w.rows[m].target;
   }
   return r;
 }
@@ -326,7 +328,7 @@ __device__ void finish_weights(const Work& w, const Product& p, const CUtensorMa
       }
     } else {
       // (a row without a loss has zeros in G, but W may hold infinities)
-      const bool keep = p.a_mn || row.target >= 0;
+      const bool keep = !p.tokens || row.target >= 0;
 #pragma unroll
       for (int i = 0; i < 64; ++i) v[i / 32][i % 32] = keep ? v[i / 32][i % 32] * inv : 0.f;
       put_rows<T>(p, map, slot, v, m0, n0 + c, lane);
@@ -355,11 +357,16 @@ loss_product_kernel(const __grid_constant__ Maps maps0, const __grid_constant__ 
     fence_barrier_init();
   }
   if (warp == 2) tmem_alloc_pair(&sh.tmem);
+  if (warp == 3 && lane == 0) {
+    map_prefetch(&maps0.a), map_prefetch(&maps0.b);
+    if (KIND == kWeights) map_prefetch(&maps1.a), map_prefetch(&maps1.b);
+  }
   tc_fence_before();
   __syncthreads();
   cluster_sync();
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
+  start_next(), await_previous();
 
   if (warp == 0 && lane == 0) {                    // copies
     int stage = 0;
@@ -498,7 +505,239 @@ loss_product_kernel(const __grid_constant__ Maps maps0, const __grid_constant__ 
   if (warp == 2) tmem_free_pair(tmem);
 }
 
+// ---------------------------------------------------------------- few tokens
+// With few tokens the products' time is W's way from HBM, and tiles of 256 tokens are
+// mostly empty. So the sides change: 128 words are the rows of a product, the tokens
+// its NT columns (32 or 64), one CTA a tile, and what shared memory is left holds
+// copies of W under way (8 or 10 steps of 16 KiB). CTAs take words by units of 32, so that
+// all have work of nearly one size. A warp's 32 lanes are words; values of a token
+// are joined across them by exchanges that halve the columns each time, which leaves
+// lane l with column l: 31 shuffles for 32 columns.
+constexpr int kFewRows = 128, kUnit = 32;
+constexpr int kFewThreads = 256, kFewEpilogueWarps = 4;
+
+template <int NT>
+struct FewShape {
+  static constexpr int kBytesA = kFewRows * kDepth * 2, kBytesB = NT * kDepth * 2;
+  static constexpr int kStage = kBytesA + kBytesB;
+  static constexpr int kCount = 208 * 1024 / kStage < 12 ? 208 * 1024 / kStage : 12;
+  static constexpr int kSmem = kCount * kStage + 1024;
+  static constexpr int kChunks = NT / 32;
+};
+
+struct FewWork {
+  int64_t tokens, vocab;
+  int steps, units, units_each;      // of depth; of words, and at most of one CTA
+  int* err_flag;
+  const int64_t* targets;            // stats
+  RowStat* stats;                    // (CTA, token)
+  float* at_target;
+  const RowCoef* rows;               // grads
+  void* out;                         // G transposed: (vocab, ld), tokens behind the last as zeros
+  int64_t ld;
+};
+
+template <int NT>
+struct FewShared {
+  uint64_t full[FewShape<NT>::kCount], empty[FewShape<NT>::kCount], done[2], drained[2];
+  uint32_t tmem;
+  int dead;
+  RowCoef rows[NT];
+  RowStat stats[kFewEpilogueWarps][NT];
+};
+
+template <class F>
+__device__ __forceinline__ float spread(float (&v)[32], int lane, F op) {
+#pragma unroll
+  for (int o = 16; o > 0; o /= 2) {
+    const bool up = (lane & o) != 0;
+#pragma unroll
+    for (int i = 0; i < o; ++i) {
+      const float keep = up ? v[i + o] : v[i], send = up ? v[i] : v[i + o];
+      v[i] = op(keep, __shfl_xor_sync(0xffffffffu, send, o));
+    }
+  }
+  return v[0];
+}
+
+template <class T, int NT, bool GRADS>
+__global__ void __launch_bounds__(kFewThreads, 1)
+loss_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
+                const __grid_constant__ FewWork w) {
+  using S = FewShape<NT>;
+  extern __shared__ uint8_t raw[];
+  uint8_t* stages = (uint8_t*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+  __shared__ FewShared<NT> sh;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int unit0 = (int)blockIdx.x * w.units_each;
+  const int unit1 = unit0 + w.units_each < w.units ? unit0 + w.units_each : w.units;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S::kCount; ++i) mbar_init(&sh.full[i], 1), mbar_init(&sh.empty[i], 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&sh.done[i], 1), mbar_init(&sh.drained[i], kFewEpilogueWarps);
+    sh.dead = 0;
+    fence_barrier_init();
+  }
+  if (warp == 2) tmem_alloc<2 * NT>(&sh.tmem);
+  if (warp == 3 && lane == 0) map_prefetch(&map_w), map_prefetch(&map_x);
+  start_next(), await_previous();
+  if (threadIdx.x < NT) {
+    RowCoef q = {0.f, 0.f, 0.f, -1};
+    if (threadIdx.x < w.tokens) {
+      if constexpr (GRADS) {
+        q = w.rows[threadIdx.x];
+      } else {
+        const int64_t at = w.targets[threadIdx.x];
+        if (has_loss(at, w.vocab)) q.target = (int)at;
+      }
+    }
+    sh.rows[threadIdx.x] = q;
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+
+  if (warp == 0 && lane == 0) {                       // copies
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int u = unit0; ok && u < unit1; u += kFewRows / kUnit) {
+      const int boxes = unit1 - u < kFewRows / kUnit ? unit1 - u : kFewRows / kUnit;
+      for (int k = 0; k < w.steps; ++k) {
+        if (!(ok = wait(&sh, &sh.empty[stage], phase ^ 1, w.err_flag))) break;
+        uint8_t* a = stages + stage * S::kStage;
+        mbar_arrive_expect_tx(&sh.full[stage], (uint32_t)(boxes * (S::kBytesA / 4) + S::kBytesB));
+        for (int i = 0; i < boxes; ++i)
+          tma_load_tile2d(a + i * (S::kBytesA / 4), &map_w, k * kDepth, (u + i) * kUnit, &sh.full[stage]);
+        tma_load_tile2d(a + S::kBytesA, &map_x, k * kDepth, 0, &sh.full[stage]);
+        if (++stage == S::kCount) stage = 0, phase ^= 1;
+      }
+    }
+    for (int i = 0; ok && i < S::kCount; ++i) {
+      ok = wait(&sh, &sh.empty[stage], phase ^ 1, w.err_flag);
+      if (++stage == S::kCount) stage = 0, phase ^= 1;
+    }
+  } else if (warp == 1 && lane == 0) {                // products
+    constexpr uint32_t kIdesc = instruction_desc<T>(kFewRows, NT, false, false);
+    int stage = 0, buf = 0;
+    uint32_t phase = 0, buf_phase = 0;
+    bool ok = true;
+    const uint64_t first = operand_desc(smem_u32(stages), 16);
+    for (int u = unit0; ok && u < unit1; u += kFewRows / kUnit) {
+      if (!(ok = wait(&sh, &sh.drained[buf], buf_phase ^ 1, w.err_flag))) break;
+      tc_fence_after();
+      for (int k = 0; k < w.steps; ++k) {
+        if (!(ok = wait(&sh, &sh.full[stage], phase, w.err_flag))) break;
+        tc_fence_after();
+        const uint64_t a = first + stage * (S::kStage / 16), b = a + S::kBytesA / 16;
+#pragma unroll
+        for (int i = 0; i < kDepth / 16; ++i)
+          mma_one(tmem + buf * NT, a + i * 2, b + i * 2, kIdesc, k > 0 || i > 0);
+        commit_one(&sh.empty[stage]);
+        if (++stage == S::kCount) stage = 0, phase ^= 1;
+      }
+      if (!ok) break;
+      commit_one(&sh.done[buf]);
+      if (++buf == 2) buf = 0, buf_phase ^= 1;
+    }
+  } else if (warp >= 4) {                             // finished tiles
+    int buf = 0;
+    uint32_t buf_phase = 0;
+    const int part = warp - 4;
+    RowStat run[S::kChunks];
+#pragma unroll
+    for (int c = 0; c < S::kChunks; ++c) run[c] = {-INFINITY, 0.f};
+    for (int u = unit0; u < unit1; u += kFewRows / kUnit) {
+      bool ok = lane != 0 || wait(&sh, &sh.done[buf], buf_phase, w.err_flag);
+      ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t acc = tmem + ((uint32_t)part * 32 << 16) + buf * NT;
+      // (a part without words of this CTA's holds what an earlier tile left)
+      const int64_t word = (int64_t)(u + part) * kUnit + lane;
+      const bool mine = u + part < unit1 && word < w.vocab;
+#pragma unroll
+      for (int c = 0; c < S::kChunks; ++c) {
+        float v[32];
+        tmem_load32(acc + c * 32, v);
+        tmem_load_wait();
+        if (c == S::kChunks - 1) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sh.drained[buf]);
+        }
+        if constexpr (GRADS) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const RowCoef q = sh.rows[c * 32 + i];
+            const float g = ex2(fmaf(v[i], kLog2e, -q.lse2)) * q.all - (q.target == word ? q.one : 0.f);
+            v[i] = q.target < 0 ? 0.f : g;
+          }
+          if (mine) {
+            T* out = (T*)w.out + word * w.ld + c * 32;
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+              float o[8];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) o[j] = v[i + j];
+              store_vec<T, 8>(out + i, o);
+            }
+            if (NT == 32) {          // (rows are of 64 values at least)
+              const float zero[8] = {};
+#pragma unroll
+              for (int i = 32; i < 64; i += 8) store_vec<T, 8>(out + i, zero);
+            }
+          }
+        } else {
+          if (!mine) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] = -INFINITY;
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (sh.rows[c * 32 + i].target == word) w.at_target[c * 32 + i] = v[i];
+          }
+          float m[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) m[i] = v[i];
+          const float top = spread(m, lane, [](float a, float b) { return fmaxf(a, b); });
+          const float shift = shift_of(top) * kLog2e;
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            v[i] = ex2(fmaf(v[i], kLog2e, -__shfl_sync(0xffffffffu, shift, i)));
+          const float sum = spread(v, lane, [](float a, float b) { return a + b; });
+          run[c] = join(run[c], {top, sum});
+        }
+      }
+      if (++buf == 2) buf = 0, buf_phase ^= 1;
+    }
+    if constexpr (!GRADS) {
+#pragma unroll
+      for (int c = 0; c < S::kChunks; ++c) sh.stats[part][c * 32 + lane] = run[c];
+    }
+  }
+  __syncthreads();
+  if (!GRADS && threadIdx.x < NT && threadIdx.x < w.tokens) {
+    RowStat s = sh.stats[0][threadIdx.x];
+    for (int i = 1; i < kFewEpilogueWarps; ++i) s = join(s, sh.stats[i][threadIdx.x]);
+    w.stats[(int64_t)blockIdx.x * w.tokens + threadIdx.x] = s;
+  }
+  if (sh.dead) {     // let copies and products in flight land before their memory goes
+    const uint64_t t0 = global_ns();
+    while (global_ns() - t0 < 20000000ull) {
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 2) tmem_free<2 * NT>(tmem);
+}
+
 // ---------------------------------------------------------------- small kernels
+// Each kernel of a call starts while the one in front of it ends (its barriers,
+// TMEM and tensor maps are then set up already) and waits before it reads or
+// writes what that one has to do with.
 
 // A row's loss from its tiles' statistics: 32 rows by 32 strands of tiles a block,
 // joined in a fixed order.
@@ -507,6 +746,7 @@ finish_loss_kernel(const RowStat* __restrict__ stats, int tiles, int64_t tokens,
                    const int64_t* __restrict__ targets, const float* __restrict__ at_target,
                    float* __restrict__ loss, float* __restrict__ lse) {
   __shared__ RowStat part[32][33];
+  await_previous();
   const int x = threadIdx.x % 32, y = threadIdx.x / 32;
   const int64_t t = (int64_t)blockIdx.x * 32 + x;
   RowStat s = {-INFINITY, 0.f};
@@ -571,6 +811,7 @@ __device__ void copy_rows(const T* __restrict__ in, int64_t in_ld, int64_t width
 template <class T>
 __global__ void __launch_bounds__(256)
 copy_rows_kernel(const T* in, int64_t in_ld, int64_t width, T* out, int64_t ld, int64_t rows) {
+  start_next(), await_previous();
   copy_rows<T>(in, in_ld, width, out, ld, rows, nullptr, 0, (int64_t)blockIdx.x * 256 + threadIdx.x,
                (int64_t)gridDim.x * 256);
 }
@@ -584,6 +825,7 @@ prepare_kernel(const T* x, int64_t x_ld, int64_t width, T* out, int64_t ld, int6
                int64_t vocab, const int64_t* __restrict__ targets, const float* __restrict__ lse,
                const float* __restrict__ dloss, const float* __restrict__ dlse,
                RowCoef* __restrict__ rows, float* scale) {
+  start_next(), await_previous();
   if (blockIdx.x > 0) {
     copy_rows<T>(x, x_ld, width, out, ld, tokens, targets, vocab,
                  (int64_t)(blockIdx.x - 1) * 1024 + threadIdx.x, (int64_t)(gridDim.x - 1) * 1024);
@@ -623,6 +865,7 @@ __global__ void __launch_bounds__(256)
 finish_dx_kernel(const float* __restrict__ sums, int splits, int64_t ld, int64_t tokens,
                  int64_t width, const RowCoef* __restrict__ rows, const float* __restrict__ scale,
                  T* __restrict__ dx, int64_t dx_ld) {
+  await_previous();
   const float inv = scale[1];
   const int64_t per = ld / 4;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < tokens * per; i += (int64_t)gridDim.x * 256) {
@@ -642,6 +885,22 @@ finish_dx_kernel(const float* __restrict__ sums, int splits, int64_t ld, int64_t
 }
 
 // ---------------------------------------------------------------- host
+// A launch that may start while the call's one in front of it ends (`first`: one that
+// may not).
+template <class... P, class... A>
+ferrum_status start(const char* what, bool first, void (*kernel)(P...), int64_t grid, int block,
+                    size_t smem, cudaStream_t stream, A... args) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid), cfg.blockDim = dim3((unsigned)block);
+  cfg.dynamicSmemBytes = smem, cfg.stream = stream, cfg.attrs = attr, cfg.numAttrs = first ? 0 : 1;
+  launch_detail::clear_stale_error();
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  return e == cudaSuccess ? FERRUM_OK : cuda_error(e, what);
+}
+
 int pair_count() {
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) != cudaSuccess ||
@@ -661,7 +920,7 @@ Product product_of(int64_t m, int64_t n, int64_t depth, int splits = 1) {
 }
 
 template <class T, int KIND>
-ferrum_status run(const Maps& m0, const Maps& m1, const Work& w, cudaStream_t stream,
+ferrum_status run(const Maps& m0, const Maps& m1, const Work& w, bool first, cudaStream_t stream,
                   const char* what) {
   static std::atomic<uint64_t> smem_done{0};
   auto kernel = loss_product_kernel<T, KIND>;
@@ -672,9 +931,7 @@ ferrum_status run(const Maps& m0, const Maps& m1, const Work& w, cudaStream_t st
     tiles += (int64_t)w.p[i].tiles_m * w.p[i].tiles_n * w.p[i].splits;
   if (tiles > 0x7fffffff) return invalid(what, "too many tiles for one launch");
   const int grid = 2 * (int)std::min<int64_t>(tiles, pair_count());
-  launch_detail::clear_stale_error();
-  kernel<<<grid, kThreads, kSmemBytes, stream>>>(m0, m1, w);
-  return launched(what);
+  return start(what, first, kernel, grid, kThreads, kSmemBytes, stream, m0, m1, w);
 }
 
 // An operand as the products need it: the caller's array, or a copy in 16-byte rows.
@@ -686,49 +943,88 @@ struct Matrix {
 int64_t padded(int64_t n) { return ceil_div(n, 8) * 8; }
 
 template <class T>
-ferrum_status copied(Matrix<T>& m, int64_t width, int64_t rows, uint8_t*& at, cudaStream_t stream,
-                     const char* what) {
+ferrum_status copied(Matrix<T>& m, int64_t width, int64_t rows, uint8_t*& at, bool first,
+                     cudaStream_t stream, const char* what) {
   const int64_t ld = padded(width);
-  launch_detail::clear_stale_error();
-  copy_rows_kernel<T><<<(unsigned)std::min<int64_t>(ceil_div(rows * ld / 8, 256), 148 * 32), 256, 0, stream>>>(
-      m.p, m.ld, width, (T*)at, ld, rows);
+  const ferrum_status s =
+      start(what, first, copy_rows_kernel<T>, std::min<int64_t>(ceil_div(rows * ld / 8, 256), 148 * 32),
+            256, 0, stream, m.p, m.ld, width, (T*)at, ld, rows);
   m = {(const T*)at, ld};
   at += rows * ld * 2;
-  return launched(what);
+  return s;
 }
 
 template <class T>
 constexpr bool is_bf16() { return std::is_same<T, __nv_bfloat16>::value; }
+
+// Up to so many tokens the sides change. Forward and gradient, us, with tiles of 256
+// tokens and with the sides changed: 8 x 4096 x 131072 221, 637 and 196, 616;
+// 64 x 256 x 2000 14.7, 30.6 and 12.7, 25.0; 64 x 2048 x 32000 37.6, 109 and 39.3, 105;
+// 100 x 2048 x 32000 37.4, 113 and 43.0, 111.
+constexpr int64_t kFewTokens = 64;
+
+// Launches the kernel for few tokens; `ctas` (of the statistics) is set.
+template <class T, bool GRADS>
+ferrum_status run_few(const Matrix<T>& wt, const Matrix<T>& x, int64_t width, FewWork w, int& ctas,
+                      bool first, cudaStream_t stream, const char* what) {
+  w.steps = (int)ceil_div(width, kDepth), w.units = (int)ceil_div(w.vocab, kUnit);
+  w.units_each = (int)ceil_div(w.units, 2 * pair_count());
+  ctas = (int)ceil_div(w.units, w.units_each);
+  auto go = [&](auto n) -> ferrum_status {
+    constexpr int NT = decltype(n)::value;
+    static std::atomic<uint64_t> smem_done{0};
+    CUtensorMap mw, mx;
+    cudaError_t e = tensor_map(&mw, is_bf16<T>(), wt.p, width, w.vocab, wt.ld, kUnit);
+    if (e == cudaSuccess) e = tensor_map(&mx, is_bf16<T>(), x.p, width, w.tokens, x.ld, NT);
+    if (e != cudaSuccess) return cuda_error(e, "tensor map");
+    auto kernel = loss_few_kernel<T, NT, GRADS>;
+    e = launch_detail::ensure_smem(kernel, FewShape<NT>::kSmem, smem_done);
+    if (e != cudaSuccess) return cuda_error(e, what);
+    return start(what, first, kernel, ctas, kFewThreads, FewShape<NT>::kSmem, stream, mw, mx, w);
+  };
+  return w.tokens <= 32 ? go(std::integral_constant<int, 32>()) : go(std::integral_constant<int, 64>());
+}
 
 template <class T>
 ferrum_status fwd(ferrum_device* dev, const ferrum_cross_entropy_args* a, cudaStream_t stream,
                   const char* what) {
   const int64_t n = (int64_t)a->tokens, d = (int64_t)a->width, v = (int64_t)a->vocab;
   const bool copy_x = !mappable(a->x, a->x_stride, d), copy_w = !mappable(a->weight, a->weight_stride, d);
-  const int64_t ld = padded(d), halves = ceil_div(v, kHalf);
+  const bool few = n <= kFewTokens;
+  const int64_t ld = padded(d);
+  int parts = few ? 2 * pair_count() : (int)ceil_div(v, kHalf);      // of each row's statistics
   const size_t copies = (size_t)((copy_x ? n : 0) + (copy_w ? v : 0)) * ld * 2;
-  PoolBuffer ws(dev, copies + (size_t)(halves * n) * sizeof(RowStat) + (size_t)n * 4, stream);
+  PoolBuffer ws(dev, copies + (size_t)(parts * n) * sizeof(RowStat) + (size_t)n * 4, stream);
   if (ws.status() != cudaSuccess) return cuda_error(ws.status(), "workspace");
   uint8_t* at = ws.as<uint8_t>();
   Matrix<T> x = {(const T*)a->x, a->x_stride}, wt = {(const T*)a->weight, a->weight_stride};
   if (copy_x) {
-    if (ferrum_status s = copied(x, d, n, at, stream, what)) return s;
+    if (ferrum_status s = copied(x, d, n, at, true, stream, what)) return s;
   }
   if (copy_w) {
-    if (ferrum_status s = copied(wt, d, v, at, stream, what)) return s;
+    if (ferrum_status s = copied(wt, d, v, at, !copy_x, stream, what)) return s;
   }
-  Maps m = {};
-  cudaError_t e = tensor_map(&m.a, is_bf16<T>(), x.p, d, n, x.ld, kHalf);
-  if (e == cudaSuccess) e = tensor_map(&m.b, is_bf16<T>(), wt.p, d, v, wt.ld, kHalf);
-  if (e != cudaSuccess) return cuda_error(e, "tensor map");
-  Work w = {};
-  w.p[0] = product_of(n, v, d), w.count = 1;
-  w.err_flag = dev->err_flag, w.targets = a->targets;
-  w.stats = (RowStat*)at, w.at_target = (float*)(w.stats + halves * n);
-  if (ferrum_status s = run<T, kStats>(m, m, w, stream, what)) return s;
-  finish_loss_kernel<<<(unsigned)ceil_div(n, 32), 1024, 0, stream>>>(
-      w.stats, (int)halves, n, v, a->targets, w.at_target, a->loss, a->lse);
-  return launched(what);
+  const bool first = !copy_x && !copy_w;
+  RowStat* stats = (RowStat*)at;
+  float* at_target = (float*)(stats + parts * n);
+  if (few) {
+    FewWork w = {};
+    w.tokens = n, w.vocab = v, w.err_flag = dev->err_flag, w.targets = a->targets;
+    w.stats = stats, w.at_target = at_target;
+    if (ferrum_status s = run_few<T, false>(wt, x, d, w, parts, first, stream, what)) return s;
+  } else {
+    Maps m = {};
+    cudaError_t e = tensor_map(&m.a, is_bf16<T>(), x.p, d, n, x.ld, kHalf);
+    if (e == cudaSuccess) e = tensor_map(&m.b, is_bf16<T>(), wt.p, d, v, wt.ld, kHalf);
+    if (e != cudaSuccess) return cuda_error(e, "tensor map");
+    Work w = {};
+    w.p[0] = product_of(n, v, d), w.count = 1;
+    w.err_flag = dev->err_flag, w.targets = a->targets;
+    w.stats = stats, w.at_target = at_target;
+    if (ferrum_status s = run<T, kStats>(m, m, w, first, stream, what)) return s;
+  }
+  return start(what, false, finish_loss_kernel, ceil_div(n, 32), 1024, 0, stream, (const RowStat*)stats,
+               parts, n, v, a->targets, (const float*)at_target, a->loss, a->lse);
 }
 
 // Words of a piece of the vocabulary: 256 MiB of G, but no fewer than 4096.
@@ -742,7 +1038,9 @@ ferrum_status bwd(ferrum_device* dev, const ferrum_cross_entropy_args* a, cudaSt
                   const char* what) {
   const int64_t n = (int64_t)a->tokens, d = (int64_t)a->width, v = (int64_t)a->vocab;
   const bool copy_w = !mappable(a->weight, a->weight_stride, d);
-  const int64_t ld = padded(d), piece = piece_of(n, v);
+  // With few tokens G lies the other way: (vocabulary, 64 tokens).
+  const bool few = n <= kFewTokens;
+  const int64_t ld = padded(d), piece = few ? v : piece_of(n, v), g_ld = few ? kDepth : piece;
   const bool one_piece = piece >= v;
   // Few tokens make few tiles of dx: its depth is split so that all pairs work.
   const int64_t dx_tiles = ceil_div(n, kTile) * ceil_div(d, kTile);
@@ -752,7 +1050,7 @@ ferrum_status bwd(ferrum_device* dev, const ferrum_cross_entropy_args* a, cudaSt
   const bool need_sums = splits > 1 || !one_piece;
   auto round = [](int64_t b) { return (size_t)((b + 255) / 256 * 256); };
   const size_t x_bytes = round(n * ld * 2), w_bytes = copy_w ? round(v * ld * 2) : 0;
-  const size_t g_bytes = round(n * piece * 2), sum_bytes = need_sums ? round(splits * n * ld * 4) : 0;
+  const size_t g_bytes = round((few ? v : n) * g_ld * 2), sum_bytes = need_sums ? round(splits * n * ld * 4) : 0;
   PoolBuffer ws(dev, x_bytes + w_bytes + g_bytes + sum_bytes + (size_t)n * sizeof(RowCoef) + 256, stream);
   if (ws.status() != cudaSuccess) return cuda_error(ws.status(), "workspace");
   uint8_t* at = ws.as<uint8_t>();
@@ -768,11 +1066,12 @@ ferrum_status bwd(ferrum_device* dev, const ferrum_cross_entropy_args* a, cudaSt
   at += sum_bytes;
   Matrix<T> wt = {(const T*)a->weight, a->weight_stride};
   const int64_t copiers = std::min<int64_t>(ceil_div(n * ld / 8, 1024), 148 * 4);
-  prepare_kernel<T><<<(unsigned)copiers + 1, 1024, 0, stream>>>(
-      (const T*)a->x, a->x_stride, d, x, ld, n, v, a->targets, a->lse, a->dloss, a->dlse, rows, scale);
-  if (ferrum_status s = launched(what)) return s;
+  if (ferrum_status s = start(what, true, prepare_kernel<T>, copiers + 1, 1024, 0, stream,
+                              (const T*)a->x, a->x_stride, d, x, ld, n, v, a->targets,
+                              (const float*)a->lse, a->dloss, a->dlse, rows, scale))
+    return s;
   if (copy_w) {
-    if (ferrum_status s = copied(wt, d, v, at, stream, what)) return s;
+    if (ferrum_status s = copied(wt, d, v, at, false, stream, what)) return s;
   }
 
   const bool dx_map = mappable(a->dx, a->dx_stride, d), dw_map = mappable(a->dweight, a->dweight_stride, d);
@@ -786,35 +1085,47 @@ ferrum_status bwd(ferrum_device* dev, const ferrum_cross_entropy_args* a, cudaSt
     auto map = [&](CUtensorMap& m, const void* p, int64_t cols, int64_t rows, int64_t pitch, int box) {
       if (e == cudaSuccess) e = tensor_map(&m, is_bf16<T>(), p, cols, rows, pitch, box);
     };
-    map(logits.a, x, d, n, ld, kHalf), map(logits.b, wp, d, words, wt.ld, kHalf);
-    map(logits.out, g, words, n, piece, 32);
-    map(mx.a, g, words, n, piece, kHalf), map(mx.b, wp, d, words, wt.ld, kDepth);
+    if (!few) {
+      map(logits.a, x, d, n, ld, kHalf), map(logits.b, wp, d, words, wt.ld, kHalf);
+      map(logits.out, g, words, n, g_ld, 32);
+    }
+    if (few)
+      map(mx.a, g, g_ld, words, g_ld, kDepth), map(mw.a, g, g_ld, words, g_ld, kHalf);
+    else
+      map(mx.a, g, words, n, g_ld, kHalf), map(mw.a, g, words, n, g_ld, kDepth);
+    map(mx.b, wp, d, words, wt.ld, kDepth), map(mw.b, x, d, n, ld, kDepth);
     if (dx_map) map(mx.out, a->dx, d, n, a->dx_stride, 32);
-    map(mw.a, g, words, n, piece, kDepth), map(mw.b, x, d, n, ld, kDepth);
     if (dw_map) map(mw.out, dw, d, words, a->dweight_stride, 32);
     if (e != cudaSuccess) return cuda_error(e, "tensor map");
     Work w = {};
     w.err_flag = dev->err_flag, w.rows = rows, w.scale = scale, w.first = first;
-    w.p[0] = product_of(n, words, d), w.count = 1;
-    w.p[0].store_map = true;
-    if (ferrum_status s = run<T, kGrads>(logits, logits, w, stream, what)) return s;
+    if (few) {
+      FewWork f = {};
+      int ctas = 0;
+      f.tokens = n, f.vocab = v, f.err_flag = dev->err_flag, f.rows = rows, f.out = g, f.ld = g_ld;
+      if (ferrum_status s = run_few<T, true>(wt, Matrix<T>{x, ld}, d, f, ctas, false, stream, what)) return s;
+    } else {
+      w.p[0] = product_of(n, words, d), w.count = 1;
+      w.p[0].store_map = true;
+      if (ferrum_status s = run<T, kGrads>(logits, logits, w, false, stream, what)) return s;
+    }
 
-    Product px = product_of(n, d, words, splits), pw = product_of(words, d, n);
+    Product px = product_of(n, d, words, splits), pw = product_of(words, d, few ? g_ld : n);
+    px.tokens = true;
     px.partial = sums, px.partial_ld = ld;
     px.load = first > 0, px.sums = splits > 1 || !last;
     px.out = a->dx, px.ld = a->dx_stride, px.store_map = dx_map;
-    pw.a_mn = true;
+    (few ? px : pw).a_mn = true;
     pw.out = dw, pw.ld = a->dweight_stride, pw.store_map = dw_map;
     // the product of the longer tiles first, so that the last ones are short
     const bool x_first = px.steps_per_split >= pw.steps_per_split;
     w.p[0] = x_first ? px : pw, w.p[1] = x_first ? pw : px, w.count = 2;
-    if (ferrum_status s = run<T, kWeights>(x_first ? mx : mw, x_first ? mw : mx, w, stream, what)) return s;
+    if (ferrum_status s = run<T, kWeights>(x_first ? mx : mw, x_first ? mw : mx, w, false, stream, what)) return s;
   }
-  if (splits > 1) {
-    finish_dx_kernel<T><<<(unsigned)std::min<int64_t>(ceil_div(n * ld / 4, 256), 148 * 16), 256, 0, stream>>>(
-        sums, splits, ld, n, d, rows, scale, (T*)a->dx, a->dx_stride);
-    return launched(what);
-  }
+  if (splits > 1)
+    return start(what, false, finish_dx_kernel<T>, std::min<int64_t>(ceil_div(n * ld / 4, 256), 148 * 16),
+                 256, 0, stream, (const float*)sums, splits, ld, n, d, (const RowCoef*)rows,
+                 (const float*)scale, (T*)a->dx, a->dx_stride);
   return FERRUM_OK;
 }
 

@@ -68,6 +68,16 @@ __device__ __forceinline__ void pair_load(void* dst, const CUtensorMap* map, int
       : "memory");
 }
 
+__device__ __forceinline__ void map_prefetch(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
+// Lets the stream's next kernel start (where its launch allows that), and waits for
+// the end of the one in front (at once where this launch did not).
+__device__ __forceinline__ void start_next() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void await_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---------------------------------------------------------------- TMEM
 // All 512 columns of both CTAs; called by one whole warp of each.
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t* at) {
@@ -102,6 +112,34 @@ __device__ __forceinline__ void commit_pair(uint64_t* bar) {
       "h"((uint16_t)3)
       : "memory");
 }
+// The same for one CTA alone: `COLS` columns of TMEM, a power of two from 32 on.
+template <int COLS>
+__device__ __forceinline__ void tmem_alloc(uint32_t* at) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(at)),
+               "n"(COLS)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+}
+template <int COLS>
+__device__ __forceinline__ void tmem_free(uint32_t base) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "n"(COLS));
+}
+__device__ __forceinline__ void mma_one(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+      : "memory");
+}
+__device__ __forceinline__ void commit_one(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+                   smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
 // 32 columns from `at` on of this warp's 32 lanes, a lane a row. The warp is
 // brought together first.
 __device__ __forceinline__ void tmem_load32(uint32_t at, float (&v)[32]) {
