@@ -5,6 +5,38 @@ namespace ferrum {
 namespace seq {
 namespace {
 
+// A row's loss from its tiles' statistics: 32 rows by 32 strands of tiles a block,
+// joined in a fixed order.
+__global__ void __launch_bounds__(1024)
+finish_loss_kernel(const RowStat* __restrict__ stats, int tiles, int64_t tokens, int64_t vocab,
+                   const int64_t* __restrict__ targets, const float* __restrict__ at_target,
+                   float* __restrict__ loss, float* __restrict__ lse) {
+  __shared__ RowStat part[32][33];
+  await_previous();
+  const int x = threadIdx.x % 32, y = threadIdx.x / 32;
+  const int64_t t = (int64_t)blockIdx.x * 32 + x;
+  RowStat s = {-INFINITY, 0.f};
+  if (t < tokens) {
+#pragma unroll 4
+    for (int i = y; i < tiles; i += 32) s = join(s, stats[(int64_t)i * tokens + t]);
+  }
+  part[y][x] = s;
+  __syncthreads();
+  s = part[x][y];                     // row y, strand x
+#pragma unroll
+  for (int o = 16; o > 0; o /= 2) {
+    RowStat q;
+    q.top = __shfl_down_sync(0xffffffffu, s.top, o), q.sum = __shfl_down_sync(0xffffffffu, s.sum, o);
+    s = join(s, q);
+  }
+  const int64_t r = (int64_t)blockIdx.x * 32 + y;
+  if (x != 0 || r >= tokens) return;
+  const bool counts = has_loss(targets[r], vocab);
+  const float v = lse_of(s);
+  lse[r] = counts ? v : 0.f;
+  loss[r] = counts ? v - at_target[r] : 0.f;
+}
+
 ferrum_status check_loss(const ferrum_device* dev, const ferrum_cross_entropy_args* a,
                          const char* what, bool bwd) {
   if (ferrum_status s = check_args(dev, a, what)) return s;
@@ -39,6 +71,14 @@ ferrum_status check_loss(const ferrum_device* dev, const ferrum_cross_entropy_ar
 }
 
 }  // namespace
+
+ferrum_status finish_loss(const RowStat* stats, int parts, const float* at_target,
+                          const ferrum_cross_entropy_args* a, cudaStream_t stream, const char* what) {
+  const int64_t n = (int64_t)a->tokens;
+  return start(what, false, finish_loss_kernel, ceil_div(n, 32), 1024, 0, stream, stats, parts, n,
+               (int64_t)a->vocab, a->targets, at_target, a->loss, a->lse);
+}
+
 }  // namespace seq
 }  // namespace ferrum
 

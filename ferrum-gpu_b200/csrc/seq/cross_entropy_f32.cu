@@ -1,5 +1,13 @@
-// The loss against a vocabulary with its products on the FMA pipe: pieces of
-// the vocabulary, whose logits live in a workspace until the next piece.
+// The loss against a vocabulary in float32: the products on the FMA pipe, as the
+// tensor cores have no product of that precision, with the same epilogues and order of
+// kernels as in 16 bits (cross_entropy_tc.cu).
+//
+// A block of 256 threads computes a tile of 128 x 128, 8 x 8 a thread, two values of a
+// row at a time (fma.rn.f32x2), from steps of 16 that it copies to shared memory
+// through registers a step ahead. 64 multiply-adds a thread take 4 reads of 16 bytes:
+// bound by the FMA pipe (72 TFLOP/s). The depth of dx, the vocabulary, is split so that
+// there are tiles for all SMs; its slabs are added in order, which also halves the
+// error of one long sum.
 #include <algorithm>
 
 #include "cross_entropy.cuh"
@@ -8,214 +16,313 @@ namespace ferrum {
 namespace seq {
 namespace {
 
-constexpr int kTile = 128, kStep = 16, kThreads = 256;
+constexpr int kTile = 128, kStep = 16, kThreads = 256, kPitch = kTile + 4;
 
-// One operand of a product: element (row, k) is at p[row * row_stride + k * k_stride].
-// With `targets`, k counts tokens, and those without a loss read as zero.
-template <class T>
+enum Kind { kStats, kGrads, kWeights };
+
+// One operand: rows by depth, one of them contiguous, 16-byte rows.
 struct Operand {
-  const T* p;
-  int64_t row_stride, k_stride, rows;
-  const int64_t* targets;
+  const float* p;
+  int64_t ld, rows;
+  bool along;                // its rows of memory run along the depth's steps (MN-major)
+};
+struct Product {
+  Operand a, b;
+  int64_t depth, depth_per_split;
+  int tiles_m, tiles_n, splits;
+  float* out;                // sums: slabs of a.rows rows
+  int64_t ld;
+  bool sums, load;           // onto those of earlier pieces
+};
+struct Work {
+  Product p[2];
+  int count;
+  const int64_t* targets;    // stats
+  RowStat* stats;            // (tile of N, token)
+  float* at_target;
   int64_t vocab;
+  const RowCoef* rows;       // grads
+  int64_t first;
+  const float* scale;
 };
 
-// C[m, n] = alpha sum_k A(m, k) B(n, k) (+ C), a tile of 128 x 128 a block,
-// 8 x 8 a thread.
-template <class TA, class TB, class TC>
-__global__ void __launch_bounds__(kThreads)
-product_kernel(Operand<TA> A, Operand<TB> B, TC* C, int64_t ldc, int64_t depth, int64_t col_tiles,
-               bool add) {
-  __shared__ float sa[kStep][kTile + 4], sb[kStep][kTile + 4];
-  const int64_t m0 = blockIdx.x / col_tiles * kTile, n0 = blockIdx.x % col_tiles * kTile;
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  float acc[8][8] = {};
-  auto stage = [&](auto& op, float (*s)[kTile + 4], int64_t r0, int64_t k0) {
-#pragma unroll
-    for (int j = 0; j < kTile * kStep / kThreads; ++j) {
-      const int e = j * kThreads + threadIdx.x;
-      // neighbouring threads along the axis that is contiguous
-      const int k = op.k_stride == 1 ? e % kStep : e / kTile;
-      const int r = op.k_stride == 1 ? e / kStep : e % kTile;
-      float v = 0.f;
-      if (r0 + r < op.rows && k0 + k < depth &&
-          (op.targets == nullptr || has_loss(op.targets[k0 + k], op.vocab)))
-        v = to_f(op.p[(r0 + r) * op.row_stride + (k0 + k) * op.k_stride]);
-      s[k][r] = v;
+__device__ __forceinline__ void fma2(float2& d, float2 a, float2 b) {
+  uint64_t& r = *(uint64_t*)&d;
+  asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(r) : "l"(*(const uint64_t*)&a), "l"(*(const uint64_t*)&b));
+}
+
+// This thread's 8 of a step's 128 x 16 values of an operand, on their way to shared
+// memory as [depth][row]: two units of 4.
+struct Piece {
+  const float* p;            // the first unit; the second lies `next` values on
+  int64_t next, step;        // and those of the next step of depth `step`
+  int rows;                  // units: of the first unit's row or rows, those that exist
+  bool along, second;        // (not along: the second unit's row exists)
+  float4 v[2];
+
+  __device__ __forceinline__ Piece(const Operand& o, int64_t r0, int64_t k0) : along(o.along) {
+    const int t = threadIdx.x;
+    if (along) {             // 32 threads a step of depth
+      const int64_t r = r0 + t % 32 * 4;
+      p = o.p + (k0 + t / 32) * o.ld + r, next = 8 * o.ld, step = kStep * o.ld;
+      rows = (int)(o.rows - r < 4 ? o.rows - r : 4), second = true;
+    } else {                 // 4 threads a row
+      const int64_t r = r0 + t / 4;
+      p = o.p + r * o.ld + k0 + t % 4 * 4, next = 64 * o.ld, step = kStep;
+      rows = r < o.rows ? 4 : 0, second = r + 64 < o.rows;
     }
-  };
-  for (int64_t k0 = 0; k0 < depth; k0 += kStep) {
-    stage(A, sa, m0, k0);
-    stage(B, sb, n0, k0);
-    __syncthreads();
+  }
+  // The next step, `left` of whose steps of depth exist.
+  __device__ __forceinline__ void load(int left) {
+    const int t = threadIdx.x;
 #pragma unroll
-    for (int k = 0; k < kStep; ++k) {
-      float a[8], b[8];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        a[i] = sa[k][ty * 4 + i], a[4 + i] = sa[k][64 + ty * 4 + i];
-        b[i] = sb[k][tx * 4 + i], b[4 + i] = sb[k][64 + tx * 4 + i];
+    for (int i = 0; i < 2; ++i) {
+      int n;
+      if (along)
+        n = t / 32 + 8 * i < left ? rows : 0;
+      else
+        n = (i == 0 ? rows > 0 : second) ? left - t % 4 * 4 : 0;
+      const float* q = p + i * next;
+      v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (n >= 4) {
+        v[i] = *(const float4*)q;
+      } else {
+        if (n > 0) v[i].x = q[0];
+        if (n > 1) v[i].y = q[1];
+        if (n > 2) v[i].z = q[2];
       }
+    }
+    p += step;
+  }
+  __device__ __forceinline__ void store(float (*s)[kPitch]) const {
+    const int t = threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (along) {
+        *(float4*)&s[t / 32 + 8 * i][t % 32 * 4] = v[i];
+      } else {
+        const int r = t / 4 + 64 * i, k = t % 4 * 4;
+        s[k][r] = v[i].x, s[k + 1][r] = v[i].y, s[k + 2][r] = v[i].z, s[k + 3][r] = v[i].w;
+      }
+    }
+  }
+};
+
+template <int KIND>
+__global__ void __launch_bounds__(kThreads, 2) loss_f32_kernel(const __grid_constant__ Work w) {
+  __shared__ __align__(16) float sa[2][kStep][kPitch], sb[2][kStep][kPitch];
+  start_next(), await_previous();
+  int t = blockIdx.x;
+  const int first = w.p[0].tiles_m * w.p[0].tiles_n * w.p[0].splits;
+  const bool second = KIND == kWeights && t >= first;
+  if (second) t -= first;
+  const Product& p = w.p[second];
+  const int split = t / (p.tiles_m * p.tiles_n);
+  t %= p.tiles_m * p.tiles_n;
+  const int64_t m0 = (int64_t)(t % p.tiles_m) * kTile, n0 = (int64_t)(t / p.tiles_m) * kTile;
+  const int64_t k0 = split * p.depth_per_split;
+  const int depth = (int)(p.depth - k0 < p.depth_per_split ? p.depth - k0 : p.depth_per_split);
+  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+  float2 acc[8][4];
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = make_float2(0.f, 0.f);
+  Piece a(p.a, m0, k0), b(p.b, n0, k0);
+  a.load(depth), b.load(depth);
+  a.store(sa[0]), b.store(sb[0]);
+  __syncthreads();
+  int buf = 0;
+#pragma unroll 1
+  for (int k = kStep; k < depth + kStep; k += kStep, buf ^= 1) {
+    const bool more = k < depth;
+    if (more) a.load(depth - k), b.load(depth - k);
+#pragma unroll
+    for (int q = 0; q < kStep; ++q) {
+      float x[8];
+      float2 y[4];
+      *(float4*)&x[0] = *(const float4*)&sa[buf][q][ty * 4];
+      *(float4*)&x[4] = *(const float4*)&sa[buf][q][64 + ty * 4];
+      *(float4*)&y[0] = *(const float4*)&sb[buf][q][tx * 4];
+      *(float4*)&y[2] = *(const float4*)&sb[buf][q][64 + tx * 4];
 #pragma unroll
       for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc[i][j] = fmaf(a[i], b[j], acc[i][j]);
+        for (int j = 0; j < 4; ++j) fma2(acc[i][j], make_float2(x[i], x[i]), y[j]);
     }
+    if (more) a.store(sa[buf ^ 1]), b.store(sb[buf ^ 1]);
     __syncthreads();
   }
+  // row i of the thread is m0 + i / 4 * 64 + ty * 4 + i % 4; its values j < 4 are
+  // columns n0 + tx * 4 + j, the others 64 further
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int64_t m = m0 + (i / 4) * 64 + ty * 4 + i % 4;
-    if (m >= A.rows) continue;
+    const int64_t m = m0 + i / 4 * 64 + ty * 4 + i % 4;
+    const bool row = m < p.a.rows;
+    float v[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int64_t n = n0 + (j / 4) * 64 + tx * 4 + j % 4;
-      if (n >= B.rows) continue;
-      TC* c = C + m * ldc + n;
-      *c = from_f<TC>(add ? to_f(*c) + acc[i][j] : acc[i][j]);
+    for (int j = 0; j < 8; ++j) v[j] = j % 2 ? acc[i][j / 2].y : acc[i][j / 2].x;
+    auto column = [&](int j) { return n0 + j / 4 * 64 + tx * 4 + j % 4; };
+    if constexpr (KIND == kStats) {
+      const int64_t target = row ? w.targets[m] : -1;
+      float top = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (column(j) >= p.b.rows) v[j] = -INFINITY;
+        else if (column(j) == target) w.at_target[m] = v[j];
+        top = fmaxf(top, v[j]);
+      }
+#pragma unroll
+      for (int o = 8; o > 0; o /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const float k = shift_of(top) * kLog2e;
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum += ex2(fmaf(v[j], kLog2e, -k));
+#pragma unroll
+      for (int o = 8; o > 0; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (row && tx == 0) w.stats[n0 / kTile * p.a.rows + m] = {top, sum};
+      continue;
+    }
+    if (!row) continue;
+    float* out = p.out + (p.sums ? split * p.a.rows : 0) * p.ld + m * p.ld;
+    if constexpr (KIND == kGrads) {
+      const RowCoef q = w.rows[m];
+      const int64_t at = (int64_t)q.target - w.first;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float g = ex2(fmaf(v[j], kLog2e, -q.lse2)) * q.all - (column(j) == at ? q.one : 0.f);
+        v[j] = q.target < 0 ? 0.f : g;
+      }
+    } else {
+      const float inv = p.sums ? 1.f : w.scale[1];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        v[j] *= inv;
+        if (p.load && column(j) < p.b.rows) v[j] += out[column(j)];
+      }
+    }
+    const bool wide = p.ld % 4 == 0 && (uintptr_t)p.out % 16 == 0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int64_t n = column(4 * h);
+      if (wide && n + 4 <= p.b.rows) {
+        *(float4*)(out + n) = make_float4(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (n + j < p.b.rows) out[n + j] = v[4 * h + j];
+      }
     }
   }
 }
 
-template <class TA, class TB, class TC>
-ferrum_status product(const Operand<TA>& A, const Operand<TB>& B, TC* C, int64_t ldc, int64_t depth,
-                      bool add, cudaStream_t stream, const char* what) {
-  const int64_t cols = ceil_div(B.rows, kTile), blocks = cols * ceil_div(A.rows, kTile);
-  if (blocks > 0x7fffffff) return invalid(what, "too many blocks for one launch");
-  launch_detail::clear_stale_error();
-  product_kernel<<<(unsigned)blocks, kThreads, 0, stream>>>(A, B, C, ldc, depth, cols, add);
-  return launched(what);
+int sm_count() {
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    sms = 148;
+  return sms;
 }
 
-__device__ RowStat block_join(RowStat s) {
-  __shared__ RowStat sh[kThreads];
-  sh[threadIdx.x] = s;
-  __syncthreads();
-  for (int o = kThreads / 2; o > 0; o /= 2) {
-    if ((int)threadIdx.x < o) sh[threadIdx.x] = join(sh[threadIdx.x], sh[threadIdx.x + o]);
-    __syncthreads();
-  }
-  return sh[0];
+Product product_of(const Operand& a, const Operand& b, int64_t depth, int splits = 1) {
+  Product p = {};
+  p.a = a, p.b = b, p.depth = depth;
+  p.tiles_m = (int)ceil_div(a.rows, kTile), p.tiles_n = (int)ceil_div(b.rows, kTile);
+  p.depth_per_split = ceil_div(ceil_div(depth, kStep), splits) * kStep;
+  p.splits = (int)ceil_div(depth, p.depth_per_split);
+  return p;
 }
 
-// A row's statistics, a block a row, joined with those of the pieces before;
-// after the last piece its loss.
-__global__ void __launch_bounds__(kThreads)
-piece_stats_kernel(const float* __restrict__ logits, int64_t n, int64_t first, LossSizes z,
-                   const int64_t* __restrict__ targets, RowStat* stats, float* at_target,
-                   float* loss, float* lse) {
-  const int64_t t = blockIdx.x;
-  const float* l = logits + t * n;
-  RowStat s = {-INFINITY, 0.f};
-  for (int64_t v = threadIdx.x; v < n; v += kThreads)
-    s = join(s, {l[v], fabsf(l[v]) == INFINITY ? ex2(l[v]) : 1.f + (l[v] - l[v])});
-  s = block_join(s);
-  if (threadIdx.x != 0) return;
-  const int64_t at = targets[t] - first;
-  const bool counts = has_loss(targets[t], z.vocab);
-  if (counts && at >= 0 && at < n) at_target[t] = l[at];
-  if (first > 0) s = join(stats[t], s);
-  stats[t] = s;
-  if (first + n == z.vocab) {
-    lse[t] = counts ? lse_of(s) : 0.f;
-    loss[t] = counts ? lse_of(s) - at_target[t] : 0.f;
-  }
+template <int KIND>
+ferrum_status run(const Work& w, bool first, cudaStream_t stream, const char* what) {
+  int64_t blocks = 0;
+  for (int i = 0; i < w.count; ++i) blocks += (int64_t)w.p[i].tiles_m * w.p[i].tiles_n * w.p[i].splits;
+  if (blocks > 0x7fffffff) return invalid(what, "too many tiles for one launch");
+  return start(what, first, loss_f32_kernel<KIND>, blocks, kThreads, 0, stream, w);
 }
 
-// The gradient of a piece's logits, in their place.
-__global__ void __launch_bounds__(kThreads)
-piece_grads_kernel(float* __restrict__ logits, int64_t n, int64_t first, LossSizes z,
-                   const int64_t* __restrict__ targets, const float* __restrict__ lse,
-                   const float* __restrict__ dloss, const float* __restrict__ dlse) {
-  const int64_t t = blockIdx.x, at = targets[t] - first;
-  float* l = logits + t * n;
-  const bool counts = has_loss(targets[t], z.vocab);
-  const float one = dloss ? dloss[t] : 0.f, all = one + (dlse ? dlse[t] : 0.f), norm = lse[t];
-  for (int64_t v = threadIdx.x; v < n; v += kThreads)
-    l[v] = counts ? expf(l[v] - norm) * all - (v == at ? one : 0.f) : 0.f;
-}
-
-// Columns of a piece: 64 MiB of logits, but no fewer than 1024.
-int64_t piece_of(const LossSizes& z) {
-  const int64_t n = ((int64_t)1 << 24) / std::max<int64_t>(z.tokens, 1) / 128 * 128;
-  return std::min(z.vocab, std::max<int64_t>(n, 1024));
-}
-
-LossSizes sizes_of(const ferrum_cross_entropy_args* a) {
-  return {(int64_t)a->tokens, (int64_t)a->width, (int64_t)a->vocab};
-}
-
-template <class T>
-ferrum_status fwd(ferrum_device* dev, const ferrum_cross_entropy_args* a, cudaStream_t stream,
-                  const char* what) {
-  const LossSizes z = sizes_of(a);
-  const int64_t piece = piece_of(z);
-  PoolBuffer ws(dev, (size_t)(z.tokens * piece) * 4 + (size_t)z.tokens * 12, stream);
-  if (ws.status() != cudaSuccess) return cuda_error(ws.status(), "workspace");
-  RowStat* stats = ws.as<RowStat>();
-  float* at_target = (float*)(stats + z.tokens);
-  float* logits = at_target + z.tokens;
-  for (int64_t v = 0; v < z.vocab; v += piece) {
-    const int64_t n = std::min(piece, z.vocab - v);
-    const Operand<T> x = {(const T*)a->x, a->x_stride, 1, z.tokens, nullptr, 0};
-    const Operand<T> w = {(const T*)a->weight + v * a->weight_stride, a->weight_stride, 1, n, nullptr, 0};
-    if (ferrum_status s = product(x, w, logits, n, z.width, false, stream, what)) return s;
-    piece_stats_kernel<<<(unsigned)z.tokens, kThreads, 0, stream>>>(
-        logits, n, v, z, a->targets, stats, at_target, a->loss, a->lse);
-    if (ferrum_status s = launched(what)) return s;
-  }
-  return FERRUM_OK;
-}
-
-template <class T>
-__global__ void __launch_bounds__(kThreads)
-round_rows_kernel(const float* __restrict__ in, T* out, int64_t ld, int64_t width) {
-  for (int64_t d = threadIdx.x; d < width; d += kThreads)
-    out[blockIdx.x * ld + d] = from_f<T>(in[blockIdx.x * width + d]);
-}
-
-template <class T>
-ferrum_status bwd(ferrum_device* dev, const ferrum_cross_entropy_args* a, cudaStream_t stream,
-                  const char* what) {
-  const LossSizes z = sizes_of(a);
-  const int64_t piece = piece_of(z);
-  PoolBuffer ws(dev, (size_t)(z.tokens * (piece + z.width)) * 4, stream);
-  if (ws.status() != cudaSuccess) return cuda_error(ws.status(), "workspace");
-  float* logits = ws.as<float>();
-  float* sum = logits + z.tokens * piece;
-  T* dw = (T*)a->dweight;
-  for (int64_t v = 0; v < z.vocab; v += piece) {
-    const int64_t n = std::min(piece, z.vocab - v);
-    const T* wp = (const T*)a->weight + v * a->weight_stride;
-    const Operand<T> x = {(const T*)a->x, a->x_stride, 1, z.tokens, nullptr, 0};
-    const Operand<T> w = {wp, a->weight_stride, 1, n, nullptr, 0};
-    if (ferrum_status s = product(x, w, logits, n, z.width, false, stream, what)) return s;
-    piece_grads_kernel<<<(unsigned)z.tokens, kThreads, 0, stream>>>(
-        logits, n, v, z, a->targets, a->lse, a->dloss, a->dlse);
-    if (ferrum_status s = launched(what)) return s;
-    const Operand<float> g = {logits, n, 1, z.tokens, nullptr, 0};
-    const Operand<T> wt = {wp, 1, a->weight_stride, z.width, nullptr, 0};
-    if (ferrum_status s = product(g, wt, sum, z.width, n, v > 0, stream, what)) return s;
-    const Operand<float> gt = {logits, 1, n, n, nullptr, 0};
-    const Operand<T> xt = {(const T*)a->x, 1, a->x_stride, z.width, a->targets, z.vocab};
-    if (ferrum_status s = product(gt, xt, dw + v * a->dweight_stride, a->dweight_stride, z.tokens,
-                                  false, stream, what))
-      return s;
-  }
-  round_rows_kernel<<<(unsigned)z.tokens, kThreads, 0, stream>>>(sum, (T*)a->dx, a->dx_stride, z.width);
-  return launched(what);
+bool whole_rows(const void* p, int64_t ld, int64_t cols) {
+  return aligned(p, 16) && ld % 4 == 0 && ld >= cols;
 }
 
 }  // namespace
 
 ferrum_status loss_fwd_f32(ferrum_device* dev, const ferrum_cross_entropy_args* a,
                            cudaStream_t stream, const char* what) {
-  return with_dtype(a->dtype, [&](auto tag) { return fwd<decltype(tag)>(dev, a, stream, what); });
+  const int64_t n = (int64_t)a->tokens, d = (int64_t)a->width, v = (int64_t)a->vocab;
+  const bool copy_x = !whole_rows(a->x, a->x_stride, d), copy_w = !whole_rows(a->weight, a->weight_stride, d);
+  const int64_t ld = padded(d), parts = ceil_div(v, kTile);
+  PoolBuffer ws(dev, (size_t)((copy_x ? n : 0) + (copy_w ? v : 0)) * ld * 4 +
+                         (size_t)(parts * n) * sizeof(RowStat) + (size_t)n * 4, stream);
+  if (ws.status() != cudaSuccess) return cuda_error(ws.status(), "workspace");
+  uint8_t* at = ws.as<uint8_t>();
+  Matrix<float> x = {(const float*)a->x, a->x_stride}, wt = {(const float*)a->weight, a->weight_stride};
+  if (copy_x) {
+    if (ferrum_status s = copied(x, d, n, at, true, stream, what)) return s;
+  }
+  if (copy_w) {
+    if (ferrum_status s = copied(wt, d, v, at, !copy_x, stream, what)) return s;
+  }
+  Work w = {};
+  w.p[0] = product_of({x.p, x.ld, n, false}, {wt.p, wt.ld, v, false}, d), w.count = 1;
+  w.targets = a->targets, w.vocab = v;
+  w.stats = (RowStat*)at, w.at_target = (float*)(w.stats + parts * n);
+  if (ferrum_status s = run<kStats>(w, !copy_x && !copy_w, stream, what)) return s;
+  return finish_loss(w.stats, (int)parts, w.at_target, a, stream, what);
 }
 
 ferrum_status loss_bwd_f32(ferrum_device* dev, const ferrum_cross_entropy_args* a,
                            cudaStream_t stream, const char* what) {
-  return with_dtype(a->dtype, [&](auto tag) { return bwd<decltype(tag)>(dev, a, stream, what); });
+  const int64_t n = (int64_t)a->tokens, d = (int64_t)a->width, v = (int64_t)a->vocab;
+  const bool copy_w = !whole_rows(a->weight, a->weight_stride, d);
+  // Words of a piece: 256 MiB of G, but no fewer than 4096.
+  const int64_t ld = padded(d);
+  const int64_t piece = std::min<int64_t>(
+      padded(v), std::max<int64_t>(((int64_t)1 << 26) / n / kTile * kTile, 4096));
+  // dx: tiles for two blocks an SM, of 256 words at least
+  const int64_t dx_tiles = ceil_div(n, kTile) * ceil_div(d, kTile);
+  const int want = (int)std::max<int64_t>(
+      1, std::min<int64_t>(2 * sm_count() / dx_tiles, ceil_div(std::min(piece, v), 256)));
+  const int splits = product_of({nullptr, 0, n, false}, {nullptr, 0, d, false}, std::min(piece, v), want).splits;
+  auto round = [](int64_t b) { return (size_t)((b + 255) / 256 * 256); };
+  const size_t x_bytes = round(n * ld * 4), w_bytes = copy_w ? round(v * ld * 4) : 0;
+  const size_t g_bytes = round(n * piece * 4), sum_bytes = round(splits * n * ld * 4);
+  PoolBuffer ws(dev, x_bytes + w_bytes + g_bytes + sum_bytes + (size_t)n * sizeof(RowCoef) + 256, stream);
+  if (ws.status() != cudaSuccess) return cuda_error(ws.status(), "workspace");
+  uint8_t* at = ws.as<uint8_t>();
+  float* x = (float*)at;
+  float* g = (float*)(at += x_bytes);
+  float* sums = (float*)(at += g_bytes);
+  at += sum_bytes;
+  Matrix<float> wt = {(const float*)a->weight, a->weight_stride};
+  float* scale = (float*)(at + w_bytes);
+  RowCoef* rows = (RowCoef*)(at + w_bytes + 256);
+  const int64_t copiers = std::min<int64_t>(ceil_div(n * ld / 4, 1024), 148 * 4);
+  if (ferrum_status s = start(what, true, prepare_kernel<float>, copiers + 1, 1024, 0, stream,
+                              (const float*)a->x, a->x_stride, d, x, ld, n, v, a->targets,
+                              (const float*)a->lse, a->dloss, a->dlse, rows, scale))
+    return s;
+  if (copy_w) {
+    if (ferrum_status s = copied(wt, d, v, at, false, stream, what)) return s;
+  }
+  for (int64_t first = 0; first < v; first += piece) {
+    const int64_t words = std::min(piece, v - first);
+    const float* wp = wt.p + first * wt.ld;
+    Work w = {};
+    w.rows = rows, w.scale = scale, w.first = first, w.count = 1;
+    w.p[0] = product_of({x, ld, n, false}, {wp, wt.ld, words, false}, d);
+    w.p[0].out = g, w.p[0].ld = piece;
+    if (ferrum_status s = run<kGrads>(w, false, stream, what)) return s;
+    w.p[0] = product_of({g, piece, n, false}, {wp, wt.ld, d, true}, words, splits);
+    w.p[0].out = sums, w.p[0].ld = ld, w.p[0].sums = true, w.p[0].load = first > 0;
+    w.p[1] = product_of({g, piece, words, true}, {x, ld, d, true}, n);
+    w.p[1].out = (float*)a->dweight + first * a->dweight_stride, w.p[1].ld = a->dweight_stride;
+    w.count = 2;
+    if (ferrum_status s = run<kWeights>(w, false, stream, what)) return s;
+  }
+  return start(what, false, finish_dx_kernel<float>, std::min<int64_t>(ceil_div(n * ld / 4, 256), 148 * 16),
+               256, 0, stream, (const float*)sums, splits, ld, n, d, (const RowCoef*)rows,
+               (const float*)scale, (float*)a->dx, a->dx_stride);
 }
 
 }  // namespace seq

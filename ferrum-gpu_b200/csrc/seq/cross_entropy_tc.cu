@@ -77,13 +77,6 @@ constexpr uint32_t kGroup = 16;                                   // tiles of M 
 
 enum Kind { kStats, kGrads, kWeights };
 
-// What a row needs to turn its logits into G: scaled gradients of its logits'
-// sum and of its loss, lse in units of ln 2, and its target (-1 without a loss).
-struct RowCoef {
-  float all, one, lse2;
-  int target;
-};
-
 // One product A B^T of the extents m x n over `steps` steps of depth.
 struct Product {
   int64_t m, n;
@@ -734,173 +727,7 @@ loss_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
   if (warp == 2) tmem_free<2 * NT>(tmem);
 }
 
-// ---------------------------------------------------------------- small kernels
-// Each kernel of a call starts while the one in front of it ends (its barriers,
-// TMEM and tensor maps are then set up already) and waits before it reads or
-// writes what that one has to do with.
-
-// A row's loss from its tiles' statistics: 32 rows by 32 strands of tiles a block,
-// joined in a fixed order.
-__global__ void __launch_bounds__(1024)
-finish_loss_kernel(const RowStat* __restrict__ stats, int tiles, int64_t tokens, int64_t vocab,
-                   const int64_t* __restrict__ targets, const float* __restrict__ at_target,
-                   float* __restrict__ loss, float* __restrict__ lse) {
-  __shared__ RowStat part[32][33];
-  await_previous();
-  const int x = threadIdx.x % 32, y = threadIdx.x / 32;
-  const int64_t t = (int64_t)blockIdx.x * 32 + x;
-  RowStat s = {-INFINITY, 0.f};
-  if (t < tokens) {
-#pragma unroll 4
-    for (int i = y; i < tiles; i += 32) s = join(s, stats[(int64_t)i * tokens + t]);
-  }
-  part[y][x] = s;
-  __syncthreads();
-  s = part[x][y];                     // row y, strand x
-#pragma unroll
-  for (int o = 16; o > 0; o /= 2) {
-    RowStat q;
-    q.top = __shfl_down_sync(0xffffffffu, s.top, o), q.sum = __shfl_down_sync(0xffffffffu, s.sum, o);
-    s = join(s, q);
-  }
-  const int64_t r = (int64_t)blockIdx.x * 32 + y;
-  if (x != 0 || r >= tokens) return;
-  const bool counts = has_loss(targets[r], vocab);
-  const float v = lse_of(s);
-  lse[r] = counts ? v : 0.f;
-  loss[r] = counts ? v - at_target[r] : 0.f;
-}
-
-// 8 values of a row into a 16-byte aligned place, zeros behind `width`.
-template <class T>
-__device__ __forceinline__ void copy8(const T* in, int64_t left, bool wide, bool keep, T* out) {
-  uint4 q = make_uint4(0, 0, 0, 0);
-  if (keep) {
-    if (wide && left >= 8) {
-      q = *(const uint4*)in;
-    } else {
-      T* e = (T*)&q;
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (j < left) e[j] = in[j];
-    }
-  }
-  *(uint4*)out = q;
-}
-
-// Rows into 16-byte aligned ones of `ld` values, padded with zeros; rows without a
-// loss (where targets are given) become zero. A thread copies 8 values.
-template <class T>
-__device__ void copy_rows(const T* __restrict__ in, int64_t in_ld, int64_t width, T* __restrict__ out,
-                          int64_t ld, int64_t rows, const int64_t* __restrict__ targets, int64_t vocab,
-                          int64_t first, int64_t stride) {
-  const int64_t per = ld / 8;
-  const bool wide = in_ld % 8 == 0 && (uintptr_t)in % 16 == 0;
-  for (int64_t i = first; i < rows * per; i += stride) {
-    int64_t r, c;
-    if (rows * per <= 0xffffffffll) {
-      r = (uint32_t)i / (uint32_t)per, c = (uint32_t)i % (uint32_t)per * 8;
-    } else {
-      r = i / per, c = i % per * 8;
-    }
-    const bool keep = targets == nullptr || has_loss(targets[r], vocab);
-    copy8(in + r * in_ld + c, width - c, wide, keep, out + r * ld + c);
-  }
-}
-
-template <class T>
-__global__ void __launch_bounds__(256)
-copy_rows_kernel(const T* in, int64_t in_ld, int64_t width, T* out, int64_t ld, int64_t rows) {
-  start_next(), await_previous();
-  copy_rows<T>(in, in_ld, width, out, ld, rows, nullptr, 0, (int64_t)blockIdx.x * 256 + threadIdx.x,
-               (int64_t)gridDim.x * 256);
-}
-
-// The gradient's start. The first block: scale of G and every row's coefficients;
-// the others: x with rows without a loss as zeros, so that nothing of theirs
-// reaches dW.
-template <class T>
-__global__ void __launch_bounds__(1024)
-prepare_kernel(const T* x, int64_t x_ld, int64_t width, T* out, int64_t ld, int64_t tokens,
-               int64_t vocab, const int64_t* __restrict__ targets, const float* __restrict__ lse,
-               const float* __restrict__ dloss, const float* __restrict__ dlse,
-               RowCoef* __restrict__ rows, float* scale) {
-  start_next(), await_previous();
-  if (blockIdx.x > 0) {
-    copy_rows<T>(x, x_ld, width, out, ld, tokens, targets, vocab,
-                 (int64_t)(blockIdx.x - 1) * 1024 + threadIdx.x, (int64_t)(gridDim.x - 1) * 1024);
-    return;
-  }
-  __shared__ float part[32];
-  float top = 0.f;
-#pragma unroll 4
-  for (int64_t t = threadIdx.x; t < tokens; t += 1024) {
-    const float one = dloss ? dloss[t] : 0.f, all = one + (dlse ? dlse[t] : 0.f);
-    if (has_loss(targets[t], vocab)) top = fmaxf(top, fmaxf(fabsf(one), fabsf(all)));
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = top;
-  __syncthreads();
-  for (int i = 0; i < 32; ++i) top = fmaxf(top, part[i]);
-  // 2^13 over the largest, rounded down to a power of two; 1 for 0 and infinity
-  const int e = (__float_as_int(top) >> 23) - 127;
-  const int s = e == -127 || e == 128 ? 0 : (13 - e > 126 ? 126 : (13 - e < -126 ? -126 : 13 - e));
-  const float up = __int_as_float((127 + s) << 23), down = __int_as_float((127 - s) << 23);
-  if (threadIdx.x == 0) scale[0] = up, scale[1] = down;
-#pragma unroll 4
-  for (int64_t t = threadIdx.x; t < tokens; t += 1024) {
-    const int64_t at = targets[t];
-    const float one = dloss ? dloss[t] : 0.f, all = one + (dlse ? dlse[t] : 0.f);
-    const float norm = lse[t] * kLog2e;
-    const bool counts = has_loss(at, vocab);
-    rows[t] = {counts ? all * up : 0.f, counts ? one * up : 0.f, counts ? norm : 0.f,
-               counts ? (int)at : -1};
-  }
-}
-
-// dx from the slabs of its sums, in their order; 4 values a thread.
-template <class T>
-__global__ void __launch_bounds__(256)
-finish_dx_kernel(const float* __restrict__ sums, int splits, int64_t ld, int64_t tokens,
-                 int64_t width, const RowCoef* __restrict__ rows, const float* __restrict__ scale,
-                 T* __restrict__ dx, int64_t dx_ld) {
-  await_previous();
-  const float inv = scale[1];
-  const int64_t per = ld / 4;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < tokens * per; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / per, c = i % per * 4;
-    const bool keep = rows[r].target >= 0;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-    for (int s = 0; s < splits; ++s) {
-      const float4 u = *(const float4*)(sums + ((int64_t)s * tokens + r) * ld + c);
-      v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
-    }
-    const float o[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (c + j < width) dx[r * dx_ld + c + j] = from_f<T>(keep ? o[j] * inv : 0.f);
-  }
-}
-
 // ---------------------------------------------------------------- host
-// A launch that may start while the call's one in front of it ends (`first`: one that
-// may not).
-template <class... P, class... A>
-ferrum_status start(const char* what, bool first, void (*kernel)(P...), int64_t grid, int block,
-                    size_t smem, cudaStream_t stream, A... args) {
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)grid), cfg.blockDim = dim3((unsigned)block);
-  cfg.dynamicSmemBytes = smem, cfg.stream = stream, cfg.attrs = attr, cfg.numAttrs = first ? 0 : 1;
-  launch_detail::clear_stale_error();
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
-  return e == cudaSuccess ? FERRUM_OK : cuda_error(e, what);
-}
-
 int pair_count() {
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) != cudaSuccess ||
@@ -932,26 +759,6 @@ ferrum_status run(const Maps& m0, const Maps& m1, const Work& w, bool first, cud
   if (tiles > 0x7fffffff) return invalid(what, "too many tiles for one launch");
   const int grid = 2 * (int)std::min<int64_t>(tiles, pair_count());
   return start(what, first, kernel, grid, kThreads, kSmemBytes, stream, m0, m1, w);
-}
-
-// An operand as the products need it: the caller's array, or a copy in 16-byte rows.
-template <class T>
-struct Matrix {
-  const T* p;
-  int64_t ld;
-};
-int64_t padded(int64_t n) { return ceil_div(n, 8) * 8; }
-
-template <class T>
-ferrum_status copied(Matrix<T>& m, int64_t width, int64_t rows, uint8_t*& at, bool first,
-                     cudaStream_t stream, const char* what) {
-  const int64_t ld = padded(width);
-  const ferrum_status s =
-      start(what, first, copy_rows_kernel<T>, std::min<int64_t>(ceil_div(rows * ld / 8, 256), 148 * 32),
-            256, 0, stream, m.p, m.ld, width, (T*)at, ld, rows);
-  m = {(const T*)at, ld};
-  at += rows * ld * 2;
-  return s;
 }
 
 template <class T>
@@ -1023,8 +830,7 @@ ferrum_status fwd(ferrum_device* dev, const ferrum_cross_entropy_args* a, cudaSt
     w.stats = stats, w.at_target = at_target;
     if (ferrum_status s = run<T, kStats>(m, m, w, first, stream, what)) return s;
   }
-  return start(what, false, finish_loss_kernel, ceil_div(n, 32), 1024, 0, stream, (const RowStat*)stats,
-               parts, n, v, a->targets, (const float*)at_target, a->loss, a->lse);
+  return finish_loss(stats, parts, at_target, a, stream, what);
 }
 
 // Words of a piece of the vocabulary: 256 MiB of G, but no fewer than 4096.

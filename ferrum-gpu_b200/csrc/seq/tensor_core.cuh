@@ -6,7 +6,7 @@
 #include <cuda.h>
 
 #include "../tma_util.cuh"
-#include "seq_common.cuh"
+#include "cross_entropy.cuh"
 
 namespace ferrum {
 namespace seq {
@@ -71,12 +71,6 @@ __device__ __forceinline__ void pair_load(void* dst, const CUtensorMap* map, int
 __device__ __forceinline__ void map_prefetch(const CUtensorMap* map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
-// Lets the stream's next kernel start (where its launch allows that), and waits for
-// the end of the one in front (at once where this launch did not).
-__device__ __forceinline__ void start_next() {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-}
-__device__ __forceinline__ void await_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // ---------------------------------------------------------------- TMEM
 // All 512 columns of both CTAs; called by one whole warp of each.
