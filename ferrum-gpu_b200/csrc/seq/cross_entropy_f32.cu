@@ -2,10 +2,11 @@
 // tensor cores have no product of that precision, with the same epilogues and order of
 // kernels as in 16 bits (cross_entropy_tc.cu).
 //
-// A block of 256 threads computes a tile of 128 x 128, 8 x 8 a thread, two values of a
-// row at a time (fma.rn.f32x2), from steps of 16 that it copies to shared memory
-// through registers a step ahead. 64 multiply-adds a thread take 4 reads of 16 bytes:
-// bound by the FMA pipe (72 TFLOP/s). The depth of dx, the vocabulary, is split so that
+// A block of 256 threads computes a tile of 128 x 128 (or of 64 or 32 rows, where there
+// are few tiles or tokens), 8 x 8 a thread, two values of a row at a time
+// (fma.rn.f32x2), from steps of 16 that it copies to shared memory through registers a
+// step ahead. 64 multiply-adds a thread take 4 reads of 16 bytes: bound by the FMA
+// pipe (72 TFLOP/s). The depth of dx, the vocabulary, is split so that
 // there are tiles for all SMs; its slabs are added in order, which also halves the
 // error of one long sum.
 #include <algorithm>
@@ -16,7 +17,7 @@ namespace ferrum {
 namespace seq {
 namespace {
 
-constexpr int kTile = 128, kStep = 16, kThreads = 256, kPitch = kTile + 4;
+constexpr int kTile = 128, kStep = 16, kThreads = 256;
 
 enum Kind { kStats, kGrads, kWeights };
 
@@ -51,35 +52,39 @@ __device__ __forceinline__ void fma2(float2& d, float2 a, float2 b) {
   asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(r) : "l"(*(const uint64_t*)&a), "l"(*(const uint64_t*)&b));
 }
 
-// This thread's 8 of a step's 128 x 16 values of an operand, on their way to shared
-// memory as [depth][row]: two units of 4.
+// This thread's part of a step's ROWS x 16 values of an operand, on their way to
+// shared memory as [depth][row]: units of 4 values.
+template <int ROWS>
 struct Piece {
+  static constexpr int kUnits = ROWS < 64 ? 1 : ROWS / 64, kPitch = ROWS + 4;
+  static constexpr int kAcross = ROWS / 4;      // threads across the rows of one step of depth
   const float* p;            // the first unit; the second lies `next` values on
   int64_t next, step;        // and those of the next step of depth `step`
-  int rows;                  // units: of the first unit's row or rows, those that exist
+  int rows;                  // of the first unit's row or rows, those that exist
   bool along, second;        // (not along: the second unit's row exists)
-  float4 v[2];
+  float4 v[kUnits];
 
   __device__ __forceinline__ Piece(const Operand& o, int64_t r0, int64_t k0) : along(o.along) {
     const int t = threadIdx.x;
-    if (along) {             // 32 threads a step of depth
-      const int64_t r = r0 + t % 32 * 4;
-      p = o.p + (k0 + t / 32) * o.ld + r, next = 8 * o.ld, step = kStep * o.ld;
+    if (along) {
+      const int64_t r = r0 + t % kAcross * 4;
+      p = o.p + (k0 + t / kAcross) * o.ld + r, next = kThreads / kAcross * o.ld, step = kStep * o.ld;
       rows = (int)(o.rows - r < 4 ? o.rows - r : 4), second = true;
     } else {                 // 4 threads a row
       const int64_t r = r0 + t / 4;
       p = o.p + r * o.ld + k0 + t % 4 * 4, next = 64 * o.ld, step = kStep;
       rows = r < o.rows ? 4 : 0, second = r + 64 < o.rows;
     }
+    if (ROWS < 64 && t >= ROWS * 4) rows = 0;
   }
   // The next step, `left` of whose steps of depth exist.
   __device__ __forceinline__ void load(int left) {
     const int t = threadIdx.x;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kUnits; ++i) {
       int n;
       if (along)
-        n = t / 32 + 8 * i < left ? rows : 0;
+        n = t / kAcross + kThreads / kAcross * i < left ? rows : 0;
       else
         n = (i == 0 ? rows > 0 : second) ? left - t % 4 * 4 : 0;
       const float* q = p + i * next;
@@ -96,10 +101,11 @@ struct Piece {
   }
   __device__ __forceinline__ void store(float (*s)[kPitch]) const {
     const int t = threadIdx.x;
+    if (ROWS < 64 && t >= ROWS * 4) return;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kUnits; ++i) {
       if (along) {
-        *(float4*)&s[t / 32 + 8 * i][t % 32 * 4] = v[i];
+        *(float4*)&s[t / kAcross + kThreads / kAcross * i][t % kAcross * 4] = v[i];
       } else {
         const int r = t / 4 + 64 * i, k = t % 4 * 4;
         s[k][r] = v[i].x, s[k + 1][r] = v[i].y, s[k + 2][r] = v[i].z, s[k + 3][r] = v[i].w;
@@ -108,9 +114,10 @@ struct Piece {
   }
 };
 
-template <int KIND>
+template <int KIND, int ROWS>
 __global__ void __launch_bounds__(kThreads, 2) loss_f32_kernel(const __grid_constant__ Work w) {
-  __shared__ __align__(16) float sa[2][kStep][kPitch], sb[2][kStep][kPitch];
+  constexpr int kMine = ROWS / 16;        // rows of a thread
+  __shared__ __align__(16) float sa[2][kStep][ROWS + 4], sb[2][kStep][kTile + 4];
   start_next(), await_previous();
   int t = blockIdx.x;
   const int first = w.p[0].tiles_m * w.p[0].tiles_n * w.p[0].splits;
@@ -119,16 +126,17 @@ __global__ void __launch_bounds__(kThreads, 2) loss_f32_kernel(const __grid_cons
   const Product& p = w.p[second];
   const int split = t / (p.tiles_m * p.tiles_n);
   t %= p.tiles_m * p.tiles_n;
-  const int64_t m0 = (int64_t)(t % p.tiles_m) * kTile, n0 = (int64_t)(t / p.tiles_m) * kTile;
+  const int64_t m0 = (int64_t)(t % p.tiles_m) * ROWS, n0 = (int64_t)(t / p.tiles_m) * kTile;
   const int64_t k0 = split * p.depth_per_split;
   const int depth = (int)(p.depth - k0 < p.depth_per_split ? p.depth - k0 : p.depth_per_split);
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  float2 acc[8][4];
+  float2 acc[kMine][4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
+  for (int i = 0; i < kMine; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = make_float2(0.f, 0.f);
-  Piece a(p.a, m0, k0), b(p.b, n0, k0);
+  Piece<ROWS> a(p.a, m0, k0);
+  Piece<kTile> b(p.b, n0, k0);
   a.load(depth), b.load(depth);
   a.store(sa[0]), b.store(sb[0]);
   __syncthreads();
@@ -139,25 +147,28 @@ __global__ void __launch_bounds__(kThreads, 2) loss_f32_kernel(const __grid_cons
     if (more) a.load(depth - k), b.load(depth - k);
 #pragma unroll
     for (int q = 0; q < kStep; ++q) {
-      float x[8];
+      float x[kMine];
       float2 y[4];
-      *(float4*)&x[0] = *(const float4*)&sa[buf][q][ty * 4];
-      *(float4*)&x[4] = *(const float4*)&sa[buf][q][64 + ty * 4];
+      if constexpr (kMine == 2) {
+        *(float2*)&x[0] = *(const float2*)&sa[buf][q][ty * 2];
+      } else {
+        *(float4*)&x[0] = *(const float4*)&sa[buf][q][ty * 4];
+        if constexpr (kMine == 8) *(float4*)&x[4] = *(const float4*)&sa[buf][q][64 + ty * 4];
+      }
       *(float4*)&y[0] = *(const float4*)&sb[buf][q][tx * 4];
       *(float4*)&y[2] = *(const float4*)&sb[buf][q][64 + tx * 4];
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+      for (int i = 0; i < kMine; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) fma2(acc[i][j], make_float2(x[i], x[i]), y[j]);
     }
     if (more) a.store(sa[buf ^ 1]), b.store(sb[buf ^ 1]);
     __syncthreads();
   }
-  // row i of the thread is m0 + i / 4 * 64 + ty * 4 + i % 4; its values j < 4 are
-  // columns n0 + tx * 4 + j, the others 64 further
+  // of a row's values, j < 4 are columns n0 + tx * 4 + j, the others 64 further
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int64_t m = m0 + i / 4 * 64 + ty * 4 + i % 4;
+  for (int i = 0; i < kMine; ++i) {
+    const int64_t m = m0 + (kMine == 2 ? ty * 2 + i : i / 4 * 64 + ty * 4 + i % 4);
     const bool row = m < p.a.rows;
     float v[8];
 #pragma unroll
@@ -224,21 +235,30 @@ int sm_count() {
   return sms;
 }
 
-Product product_of(const Operand& a, const Operand& b, int64_t depth, int splits = 1) {
+Product product_of(int tile_rows, const Operand& a, const Operand& b, int64_t depth, int splits = 1) {
   Product p = {};
   p.a = a, p.b = b, p.depth = depth;
-  p.tiles_m = (int)ceil_div(a.rows, kTile), p.tiles_n = (int)ceil_div(b.rows, kTile);
+  p.tiles_m = (int)ceil_div(a.rows, tile_rows), p.tiles_n = (int)ceil_div(b.rows, kTile);
   p.depth_per_split = ceil_div(ceil_div(depth, kStep), splits) * kStep;
   p.splits = (int)ceil_div(depth, p.depth_per_split);
   return p;
 }
 
+// Rows of a tile of m x n: fewer where there are few tokens, and where tiles of more
+// leave SMs without work.
+int rows_of(int64_t m, int64_t n) {
+  if (m <= 32) return 32;
+  return ceil_div(m, 128) * ceil_div(n, kTile) < 4 * sm_count() ? 64 : 128;
+}
+
 template <int KIND>
-ferrum_status run(const Work& w, bool first, cudaStream_t stream, const char* what) {
+ferrum_status run(const Work& w, int tile_rows, bool first, cudaStream_t stream, const char* what) {
   int64_t blocks = 0;
   for (int i = 0; i < w.count; ++i) blocks += (int64_t)w.p[i].tiles_m * w.p[i].tiles_n * w.p[i].splits;
   if (blocks > 0x7fffffff) return invalid(what, "too many tiles for one launch");
-  return start(what, first, loss_f32_kernel<KIND>, blocks, kThreads, 0, stream, w);
+  if (tile_rows == 32) return start(what, first, loss_f32_kernel<KIND, 32>, blocks, kThreads, 0, stream, w);
+  if (tile_rows == 64) return start(what, first, loss_f32_kernel<KIND, 64>, blocks, kThreads, 0, stream, w);
+  return start(what, first, loss_f32_kernel<KIND, 128>, blocks, kThreads, 0, stream, w);
 }
 
 bool whole_rows(const void* p, int64_t ld, int64_t cols) {
@@ -264,10 +284,11 @@ ferrum_status loss_fwd_f32(ferrum_device* dev, const ferrum_cross_entropy_args* 
     if (ferrum_status s = copied(wt, d, v, at, !copy_x, stream, what)) return s;
   }
   Work w = {};
-  w.p[0] = product_of({x.p, x.ld, n, false}, {wt.p, wt.ld, v, false}, d), w.count = 1;
+  const int tile = rows_of(n, v);
+  w.p[0] = product_of(tile, {x.p, x.ld, n, false}, {wt.p, wt.ld, v, false}, d), w.count = 1;
   w.targets = a->targets, w.vocab = v;
   w.stats = (RowStat*)at, w.at_target = (float*)(w.stats + parts * n);
-  if (ferrum_status s = run<kStats>(w, !copy_x && !copy_w, stream, what)) return s;
+  if (ferrum_status s = run<kStats>(w, tile, !copy_x && !copy_w, stream, what)) return s;
   return finish_loss(w.stats, (int)parts, w.at_target, a, stream, what);
 }
 
@@ -280,10 +301,11 @@ ferrum_status loss_bwd_f32(ferrum_device* dev, const ferrum_cross_entropy_args* 
   const int64_t piece = std::min<int64_t>(
       padded(v), std::max<int64_t>(((int64_t)1 << 26) / n / kTile * kTile, 4096));
   // dx: tiles for two blocks an SM, of 256 words at least
-  const int64_t dx_tiles = ceil_div(n, kTile) * ceil_div(d, kTile);
+  const int g_tile = rows_of(n, std::min(piece, v)), tile = n <= 32 ? 32 : 64;
+  const int64_t dx_tiles = ceil_div(n, tile) * ceil_div(d, kTile);
   const int want = (int)std::max<int64_t>(
       1, std::min<int64_t>(2 * sm_count() / dx_tiles, ceil_div(std::min(piece, v), 256)));
-  const int splits = product_of({nullptr, 0, n, false}, {nullptr, 0, d, false}, std::min(piece, v), want).splits;
+  const int splits = product_of(tile, {nullptr, 0, n, false}, {nullptr, 0, d, false}, std::min(piece, v), want).splits;
   auto round = [](int64_t b) { return (size_t)((b + 255) / 256 * 256); };
   const size_t x_bytes = round(n * ld * 4), w_bytes = copy_w ? round(v * ld * 4) : 0;
   const size_t g_bytes = round(n * piece * 4), sum_bytes = round(splits * n * ld * 4);
@@ -310,15 +332,15 @@ ferrum_status loss_bwd_f32(ferrum_device* dev, const ferrum_cross_entropy_args* 
     const float* wp = wt.p + first * wt.ld;
     Work w = {};
     w.rows = rows, w.scale = scale, w.first = first, w.count = 1;
-    w.p[0] = product_of({x, ld, n, false}, {wp, wt.ld, words, false}, d);
+    w.p[0] = product_of(g_tile, {x, ld, n, false}, {wp, wt.ld, words, false}, d);
     w.p[0].out = g, w.p[0].ld = piece;
-    if (ferrum_status s = run<kGrads>(w, false, stream, what)) return s;
-    w.p[0] = product_of({g, piece, n, false}, {wp, wt.ld, d, true}, words, splits);
+    if (ferrum_status s = run<kGrads>(w, g_tile, false, stream, what)) return s;
+    w.p[0] = product_of(tile, {g, piece, n, false}, {wp, wt.ld, d, true}, words, splits);
     w.p[0].out = sums, w.p[0].ld = ld, w.p[0].sums = true, w.p[0].load = first > 0;
-    w.p[1] = product_of({g, piece, words, true}, {x, ld, d, true}, n);
+    w.p[1] = product_of(tile, {g, piece, words, true}, {x, ld, d, true}, n);
     w.p[1].out = (float*)a->dweight + first * a->dweight_stride, w.p[1].ld = a->dweight_stride;
     w.count = 2;
-    if (ferrum_status s = run<kWeights>(w, false, stream, what)) return s;
+    if (ferrum_status s = run<kWeights>(w, tile, false, stream, what)) return s;
   }
   return start(what, false, finish_dx_kernel<float>, std::min<int64_t>(ceil_div(n * ld / 4, 256), 148 * 16),
                256, 0, stream, (const float*)sums, splits, ld, n, d, (const RowCoef*)rows,
