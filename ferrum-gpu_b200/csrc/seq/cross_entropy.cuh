@@ -114,22 +114,34 @@ prepare_kernel(const T* x, int64_t x_ld, int64_t width, T* out, int64_t ld, int6
                  (int64_t)(blockIdx.x - 1) * 1024 + threadIdx.x, (int64_t)(gridDim.x - 1) * 1024);
     return;
   }
-  __shared__ float part[32];
-  float top = 0.f;
+  // the largest |dloss| and |dloss + dlse|
+  __shared__ float part[2][32];
+  float top[2] = {0.f, 0.f};
 #pragma unroll 4
   for (int64_t t = threadIdx.x; t < tokens; t += 1024) {
     const float one = dloss ? dloss[t] : 0.f, all = one + (dlse ? dlse[t] : 0.f);
-    if (has_loss(targets[t], vocab)) top = fmaxf(top, fmaxf(fabsf(one), fabsf(all)));
+    if (has_loss(targets[t], vocab)) top[0] = fmaxf(top[0], fabsf(one)), top[1] = fmaxf(top[1], fabsf(all));
   }
 #pragma unroll
-  for (int o = 16; o > 0; o /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = top;
+  for (int i = 0; i < 2; ++i) {
+#pragma unroll
+    for (int o = 16; o > 0; o /= 2) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
+    if (threadIdx.x % 32 == 0) part[i][threadIdx.x / 32] = top[i];
+  }
   __syncthreads();
-  for (int i = 0; i < 32; ++i) top = fmaxf(top, part[i]);
-  // 2^13 over the largest, rounded down to a power of two; 1 for 0 and infinity
-  const int e = (__float_as_int(top) >> 23) - 127;
-  const int s = e == -127 || e == 128 ? 0 : (13 - e > 126 ? 126 : (13 - e < -126 ? -126 : 13 - e));
-  const float up = __int_as_float((127 + s) << 23), down = __int_as_float((127 - s) << 23);
+  for (int i = 0; i < 32; ++i) top[0] = fmaxf(top[0], part[0][i]), top[1] = fmaxf(top[1], part[1][i]);
+  // That of the loss is scaled to 2^13, unless the other is so much larger that it
+  // would leave float16's range. A target's value is nearly -dloss: where all tokens
+  // weigh the same it then is nearly -2^13, which 16 bits hold without the error that
+  // they would all have alike. Out of the middle of the range, by a power of two;
+  // 0 and infinity, not at all.
+  const float unit = top[1] <= 4.f * top[0] ? top[0] : top[1];
+  float up = 8192.f / unit, down = unit / 8192.f;
+  if (!(unit > 0x1p-100f && unit < 0x1p100f)) {
+    const int e = (__float_as_int(unit) >> 23) - 127;
+    const int s = e == -127 || e == 128 ? 0 : (13 - e > 126 ? 126 : (13 - e < -126 ? -126 : 13 - e));
+    up = __int_as_float((127 + s) << 23), down = __int_as_float((127 - s) << 23);
+  }
   if (threadIdx.x == 0) scale[0] = up, scale[1] = down;
 #pragma unroll 4
   for (int64_t t = threadIdx.x; t < tokens; t += 1024) {

@@ -456,6 +456,26 @@ def test_loss_gradients_of_any_size(scale, dtype):
     check_loss(x, w, t, d)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("count", [1, 777, 1000])
+def test_loss_gradients_do_not_share_an_error(count, dtype):
+    """A mean over tokens: every target's value is nearly -1 / count, and a rounding
+    that all had alike would be a relative error of the whole, up to u. Rounding the
+    outputs alone leaves u sqrt(E[1 / m^2] / 3) = 0.425 u over mantissas m in [1, 2);
+    the softmax's part, below 0.2 of the whole here, adds as much of its own size:
+    0.425 u sqrt(1 + 0.2^2) < 0.5 u."""
+    x, w, t = loss_case(count, 256, 3000, dtype, 0.0)
+    scale = 1024.0 if dtype == torch.float16 else 1.0
+    d = torch.full((count,), scale / count, device="cuda")
+    r = sq.linear_cross_entropy(x, w, t)
+    g = sq.linear_cross_entropy_backward(d, x, w, t, r.lse)
+    p = torch.softmax(x.double() @ w.double().t(), 1)
+    p[torch.arange(count, device="cuda"), t] -= 1
+    p *= scale / count
+    for got, ref in ((g.dx, p @ w.double()), (g.dweight, p.t() @ x.double())):
+        assert ((got.double() - ref).norm() / ref.norm()).item() <= 0.5 * U[dtype]
+
+
 def test_loss_rows_without_a_target_are_not_read():
     for dtype in TYPES:
         x, w, t = loss_case(140, 64, 600, dtype, 0.4)
