@@ -244,13 +244,15 @@ __device__ __forceinline__ void put_rows(const Product& p, const CUtensorMap* ma
     }
   } else {
     __syncwarp();
-    for (int r = 0; r < 32 && m0 + r < p.m; ++r) {
-      T* out = (T*)p.out + (m0 + r) * p.ld + n0;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int c = h * 32 + lane;
-        if (n0 + c < p.n) out[c] = *(const T*)(slot + r * 128 + (((c / 8) ^ (r & 7)) * 16) + c % 8 * 2);
-      }
+    const int rows = p.m - m0 < 32 ? (int)(p.m - m0) : 32, cols = p.n - n0 < 64 ? (int)(p.n - n0) : 64;
+    T* out = (T*)p.out + m0 * p.ld + n0 + lane;
+#pragma unroll 8
+    for (int r = 0; r < rows; ++r, out += p.ld) {
+      const uint8_t* row = slot + r * 128 + lane % 8 * 2;
+      const T lo = *(const T*)(row + ((lane / 8) ^ (r & 7)) * 16);
+      const T hi = *(const T*)(row + ((lane / 8 + 4) ^ (r & 7)) * 16);
+      if (lane < cols) out[0] = lo;
+      if (lane + 32 < cols) out[32] = hi;
     }
     __syncwarp();
   }
