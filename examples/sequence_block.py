@@ -2,11 +2,13 @@
 
     python examples/sequence_block.py [--steps N]
 
-Two layers, each  norm_before -> mixer -> norm_after onto the residual stream:
+Three layers, each  norm_before -> mixer -> norm_after onto the residual stream:
 the first mixes along the sequence with causal_conv1d and selective_scan, the
-second with long_conv (through the FFT). Trains on a synthetic task (repeat the
-token seen LAG steps ago) and then answers token by token on kept state,
-checking that both forms agree. Needs a B200.
+second with long_conv (through the FFT), the third with gated_recurrence, and
+drops some of what it adds (dropout). The loss is linear_cross_entropy against the
+vocabulary. Trains on a synthetic task (repeat the token seen LAG steps ago) and
+then answers token by token on kept state, checking that both forms agree. Needs
+a B200.
 """
 
 from __future__ import annotations
@@ -23,7 +25,7 @@ sys.path.insert(0, os.path.join(os.path.dirname(os.path.abspath(__file__)), ".."
 
 from ferrum_gpu import sequence as sq  # noqa: E402
 
-VOCAB, WIDTH, STATES, TAPS, LAG = 16, 64, 16, 4, 5
+VOCAB, WIDTH, STATES, TAPS, LAG, DROP = 16, 64, 16, 4, 5, 0.05
 
 
 # Each operator with its gradient, as torch.autograd sees it.
@@ -66,6 +68,48 @@ class LongConv(torch.autograd.Function):
     def backward(ctx, dy):
         g = sq.long_conv_backward(dy, *ctx.saved_tensors)
         return g.dx, g.dkernel, g.dskip
+
+
+class Recurrence(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, input_gate, recurrence_gate, decay):
+        r = sq.gated_recurrence(x, input_gate, recurrence_gate, decay, save_states=True)
+        ctx.save_for_backward(x, input_gate, recurrence_gate, decay, r.states)
+        return r.out
+
+    @staticmethod
+    def backward(ctx, dout):
+        g = sq.gated_recurrence_backward(dout.contiguous(), *ctx.saved_tensors)
+        return g.dx, g.dinput_gate, g.drecurrence_gate, g.ddecay
+
+
+class Dropout(torch.autograd.Function):
+    """residual + dropout(x), the mask drawn again for the gradient."""
+
+    @staticmethod
+    def forward(ctx, x, residual, p, seed):
+        ctx.p, ctx.seed, ctx.dtype = p, seed, x.dtype
+        return sq.dropout(x, p, seed, residual=residual)
+
+    @staticmethod
+    def backward(ctx, dy):
+        dy = dy.contiguous()
+        return sq.dropout_backward(dy, ctx.p, ctx.seed, dtype=ctx.dtype), dy, None, None
+
+
+class Loss(torch.autograd.Function):
+    """Each token's loss against the vocabulary; targets outside it have none."""
+
+    @staticmethod
+    def forward(ctx, x, weight, targets):
+        r = sq.linear_cross_entropy(x, weight, targets)
+        ctx.save_for_backward(x, weight, targets, r.lse)
+        return r.loss
+
+    @staticmethod
+    def backward(ctx, dloss):
+        g = sq.linear_cross_entropy_backward(dloss.contiguous(), *ctx.saved_tensors)
+        return g.dx, g.dweight, None
 
 
 class NormBefore(torch.autograd.Function):
@@ -161,18 +205,56 @@ class LongLayer(nn.Module):
         return sq.norm_after(y, self.norm_out, gate=gate, residual=h, scale=self.scale)
 
 
+class RecurrenceLayer(nn.Module):
+    def __init__(self):
+        super().__init__()
+        self.norm_in, self.norm_out = nn.Parameter(torch.ones(WIDTH)), nn.Parameter(torch.ones(WIDTH))
+        self.scale = nn.Parameter(torch.full((WIDTH,), 0.5))
+        self.proj_in = nn.Linear(WIDTH, 4 * WIDTH, bias=False)     # x, both gates, gate
+        # at half open gates, memories of 2 to 200 steps
+        self.log_decay = nn.Parameter(torch.linspace(math.log(1e-2), 0.0, WIDTH))
+        # read when the mask is drawn: a captured step draws another mask once it changes
+        self.register_buffer("seed", torch.zeros(1, dtype=torch.int64))
+
+    def forward(self, h):
+        x, i, r, gate = self.proj_in(NormBefore.apply(h, self.norm_in)).split(WIDTH, -1)
+        y = Recurrence.apply(x, i, r, torch.exp(self.log_decay))
+        if not self.training:
+            return NormAfter.apply(y, self.norm_out, gate, h, self.scale)
+        self.seed += 1
+        y = NormAfter.apply(y, self.norm_out, gate, torch.zeros_like(h), self.scale)
+        return Dropout.apply(y, h, DROP, self.seed.clone())
+
+    def start(self, batch):
+        return {"state": torch.zeros(batch, WIDTH, device=self.scale.device)}
+
+    def step(self, h, s):
+        y, _ = sq.norm_before(h, self.norm_in)
+        x, i, r, gate = self.proj_in(y).split(WIDTH, -1)
+        y = sq.gated_recurrence_step(x, i, r, torch.exp(self.log_decay), s["state"])
+        return sq.norm_after(y, self.norm_out, gate=gate, residual=h, scale=self.scale)
+
+
 class Model(nn.Module):
     def __init__(self, length):
         super().__init__()
         self.embed = nn.Embedding(VOCAB, WIDTH)
-        self.layers = nn.ModuleList([ScanLayer(), LongLayer(length)])
+        self.layers = nn.ModuleList([ScanLayer(), LongLayer(length), RecurrenceLayer()])
         self.head = nn.Linear(WIDTH, VOCAB, bias=False)
 
-    def forward(self, tokens):
+    def hidden(self, tokens):
         h = self.embed(tokens)
         for layer in self.layers:
             h = layer(h)
-        return self.head(h)
+        return h
+
+    def forward(self, tokens):
+        return self.head(self.hidden(tokens))
+
+    def loss(self, tokens, targets):
+        """The mean over the tokens whose target lies in the vocabulary; no logits."""
+        losses = Loss.apply(self.hidden(tokens), self.head.weight, targets)
+        return losses.sum() / ((targets >= 0) & (targets < VOCAB)).sum()
 
     @torch.no_grad()
     def decode(self, tokens):
@@ -194,14 +276,15 @@ def main(steps: int = 200, batch: int = 16, length: int = 96):
     losses = []
     for _ in range(steps):
         tokens = torch.randint(VOCAB, (batch, length), device="cuda")
-        logits = model(tokens)
-        loss = nn.functional.cross_entropy(logits[:, LAG:].reshape(-1, VOCAB),
-                                           tokens[:, :-LAG].reshape(-1))
+        targets = torch.full_like(tokens, -100)
+        targets[:, LAG:] = tokens[:, :-LAG]
+        loss = model.loss(tokens, targets)
         opt.zero_grad()
         loss.backward()
         opt.step()
         losses.append(loss.detach())
     losses = torch.stack(losses).tolist()
+    model.eval()
     with torch.no_grad():
         prompt, stepped = model(tokens), model.decode(tokens)
     gap = ((prompt - stepped).abs().max() / prompt.abs().max()).item()

@@ -87,15 +87,14 @@ struct Stage {
   static __device__ __forceinline__ void fill(uint8_t* s, const T* p, int64_t st, int n, int channels,
                                               int lane) {
     if constexpr (LIE == kWhole) {
-      // 32 / kUnits rows at a time: a lane keeps its place in the row
-      constexpr int kAtOnce = 32 / kUnits;
-      const int step = lane / kUnits, unit = lane % kUnits;
-      const int left = channels * (int)sizeof(T) - unit * 16, bytes = left < 0 ? 0 : (left < 16 ? left : 16);
-      const T* src = p + step * st + (bytes ? unit * (16 / (int)sizeof(T)) : 0);
-      uint8_t* dst = s + step * kPitch + unit * 16;
 #pragma unroll
-      for (int i = 0; i < kSteps / kAtOnce; ++i)
-        if (i * kAtOnce < n - step) cp_async<16>(dst + i * kAtOnce * kPitch, src + i * kAtOnce * st, bytes);
+      for (int i = 0; i < kSteps * kUnits / 32; ++i) {
+        const int e = i * 32 + lane, step = e / kUnits, unit = e % kUnits;
+        const uint8_t* row = (const uint8_t*)(p + (step < n ? step : 0) * st);
+        const int left = channels * (int)sizeof(T) - unit * 16;
+        const int bytes = step >= n || left <= 0 ? 0 : (left < 16 ? left : 16);
+        cp_async<16>(s + step * kPitch + unit * 16, row + (bytes ? unit * 16 : 0), bytes);
+      }
     } else {
 #pragma unroll
       for (int i = 0; i < (kSteps * kUnits + 31) / 32; ++i) {
