@@ -240,6 +240,38 @@ def test_recurrence_long_memory_in_float32():
     assert err.max().item() <= 4 * n ** 0.5 * EPS
 
 
+def test_recurrence_empty():
+    d = torch.ones(8, device="cuda")
+    for b, n, c in ((2, 0, 8), (0, 5, 8), (2, 5, 0)):
+        x = torch.zeros(b, n, c, device="cuda")
+        h = rnd(1, b, c)
+        r = sq.gated_recurrence(x, x, x, d[:c].contiguous(), initial_state=h, save_states=True)
+        assert r.out.shape == x.shape and (b * c == 0 or n or torch.equal(r.final_state, h))
+        g = sq.gated_recurrence_backward(x, x, x, x, d[:c].contiguous(), r.states, dfinal_state=h)
+        assert g.dx.shape == x.shape and g.ddecay.shape == (c,)
+        assert not g.ddecay.any() and (n or torch.equal(g.dinitial_state, h))
+
+
+def test_recurrence_beyond_2_31_values():
+    """The end of an array of more than 2^31 values, against a short call on that end:
+    with memories of less than 40 steps (e^-0.45 a step and more), a start 400 steps
+    earlier from zero leaves e^-180 of a difference."""
+    n, d = 2 ** 21 + 100, 1040
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.empty(1, n, d, device="cuda", dtype=torch.bfloat16).normal_(generator=g)
+    gate = torch.zeros(1, 1, 1, device="cuda", dtype=torch.bfloat16).expand(1, n, d).contiguous()
+    decay = torch.full((d,), 0.9, device="cuda")
+    whole = sq.gated_recurrence(x, gate, gate, decay, save_states=True)
+    end = slice(n - 500, n)
+    part = sq.gated_recurrence(x[:, end], gate[:, end], gate[:, end], decay)
+    bound = 2 * (20 + 400) * EPS * 4.0
+    within(whole.out[:, -100:], part.out[:, -100:].double(), 2.0 ** -8 * part.out[:, -100:].double().abs() + bound)
+    within(whole.final_state, part.final_state.double(), bound)
+    back = sq.gated_recurrence_backward(x, x, gate, gate, decay, whole.states)
+    assert torch.isfinite(back.dx[:, -100:].float()).all() and bool(back.dx[:, -1].any())
+    assert bool(back.dx[:, 0].any()) and torch.isfinite(back.ddecay).all()
+
+
 # ---------------------------------------------------------------- dropout
 # y = res + x * scale: the rounding of scale and of the product, then the sum's,
 # which is the output's.
@@ -439,6 +471,15 @@ def test_loss(case, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens,width,vocab", [(40000, 16, 9000), (256, 64, 700000), (65, 40, 70000)])
+def test_loss_in_pieces_of_the_vocabulary(tokens, width, vocab, dtype):
+    """Many tokens in three pieces; many words in two, with dx in slabs besides."""
+    x, w, t = loss_case(tokens, width, vocab, dtype, 0.1)
+    d = torch.full((tokens,), 1.0 if dtype == torch.float16 else 1.0 / tokens, device="cuda")
+    check_loss(x, w, t, d)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_loss_normaliser_gradient(dtype):
     x, w, t = loss_case(150, 96, 700, dtype, 0.2)
     check_loss(x, w, t, rnd(9, 150), rnd(10, 150, std=0.1))
@@ -499,16 +540,22 @@ def test_loss_extreme_logits(dtype):
     x, w, t = loss_case(70, 64, 500, dtype, 0.0, scale=60.0)
     check_loss(x, w, t, torch.ones(70, device="cuda"))
     # infinite logits, of either sign
-    x = torch.ones(3, 8, device="cuda", dtype=dtype)
-    w = torch.zeros(300, 8, device="cuda", dtype=dtype)
-    w[7, 0] = float("-inf")
-    r = sq.linear_cross_entropy(x, w, torch.tensor([0, 299, 7], device="cuda"))
-    want = torch.tensor([299.0]).log().item()
-    assert torch.allclose(r.lse, torch.full_like(r.lse, want), rtol=1e-6, atol=0)
-    assert r.loss[2].item() == float("inf")
-    w[9, 0] = float("inf")
-    r = sq.linear_cross_entropy(x, w, torch.tensor([0, 299, 7], device="cuda"))
-    assert bool(torch.isinf(r.lse).all())
+    for tokens in (3, 70):
+        x = torch.ones(tokens, 8, device="cuda", dtype=dtype)
+        w = torch.zeros(300, 8, device="cuda", dtype=dtype)
+        w[7, 0] = float("-inf")
+        t = torch.tensor([0, 299, 7], device="cuda").repeat(24)[:tokens].contiguous()
+        r = sq.linear_cross_entropy(x, w, t)
+        want = torch.tensor([299.0]).log().item()
+        assert torch.allclose(r.lse, torch.full_like(r.lse, want), rtol=1e-6, atol=0)
+        assert r.loss[2].item() == float("inf")
+        w[9, 0] = float("inf")
+        r = sq.linear_cross_entropy(x, w, t)
+        assert bool(torch.isinf(r.lse).all())
+        x[1, 3] = float("nan")
+        w[7, 0] = w[9, 0] = 0.0
+        r = sq.linear_cross_entropy(x, w, t)      # a row keeps its NaN to itself
+        assert torch.isnan(r.loss).tolist() == [i == 1 for i in range(tokens)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
