@@ -52,84 +52,95 @@ namespace {
 // TMEM and tensor maps are then set up already) and waits before it reads or
 // writes what that one has to do with.
 
-// 16 bytes of a row into an aligned place, zeros behind `left` values.
+// 16 bytes of a row, zeros behind `left` values.
 template <class T>
-__device__ __forceinline__ void copy_unit(const T* in, int64_t left, bool wide, bool keep, T* out) {
+__device__ __forceinline__ uint4 row_unit(const T* in, int64_t left, bool wide) {
   constexpr int kUnit = 16 / sizeof(T);
+  if (wide && left >= kUnit) return *(const uint4*)in;
   uint4 q = make_uint4(0, 0, 0, 0);
-  if (keep) {
-    if (wide && left >= kUnit) {
-      q = *(const uint4*)in;
-    } else {
-      T* e = (T*)&q;
+  T* e = (T*)&q;
 #pragma unroll
-      for (int j = 0; j < kUnit; ++j)
-        if (j < left) e[j] = in[j];
-    }
-  }
-  *(uint4*)out = q;
+  for (int j = 0; j < kUnit; ++j)
+    if (j < left) e[j] = in[j];
+  return q;
 }
 
-// Rows into 16-byte aligned ones of `ld` values, padded with zeros; rows without a
-// loss (where targets are given) become zero. A thread copies 16 bytes.
+// Rows into 16-byte aligned ones of `ld` values, padded with zeros. A thread copies 16
+// bytes at a time.
 template <class T>
-__device__ void copy_rows(const T* __restrict__ in, int64_t in_ld, int64_t width, T* __restrict__ out,
-                          int64_t ld, int64_t rows, const int64_t* __restrict__ targets, int64_t vocab,
-                          int64_t first, int64_t stride) {
+__global__ void __launch_bounds__(256)
+copy_rows_kernel(const T* __restrict__ in, int64_t in_ld, int64_t width, T* __restrict__ out, int64_t ld,
+                 int64_t rows) {
+  start_next(), await_previous();
   constexpr int kUnit = 16 / sizeof(T);
   const int64_t per = ld / kUnit;
   const bool wide = in_ld % kUnit == 0 && (uintptr_t)in % 16 == 0;
-  for (int64_t i = first; i < rows * per; i += stride) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * per; i += (int64_t)gridDim.x * 256) {
     int64_t r, c;
     if (rows * per <= 0xffffffffll) {
       r = (uint32_t)i / (uint32_t)per, c = (int64_t)((uint32_t)i % (uint32_t)per) * kUnit;
     } else {
       r = i / per, c = i % per * kUnit;
     }
-    const bool keep = targets == nullptr || has_loss(targets[r], vocab);
-    copy_unit(in + r * in_ld + c, width - c, wide, keep, out + r * ld + c);
+    *(uint4*)(out + r * ld + c) = row_unit(in + r * in_ld + c, width - c, wide);
   }
 }
 
-template <class T>
-__global__ void __launch_bounds__(256)
-copy_rows_kernel(const T* in, int64_t in_ld, int64_t width, T* out, int64_t ld, int64_t rows) {
-  start_next(), await_previous();
-  copy_rows<T>(in, in_ld, width, out, ld, rows, nullptr, 0, (int64_t)blockIdx.x * 256 + threadIdx.x,
-               (int64_t)gridDim.x * 256);
-}
+// The gradient works on the tokens that have a loss, one after the other, as many as
+// there are rounded up to 64 (and 64 at least): the rows behind the last are zeros.
+constexpr int kTokenRound = 64;
 
-// The gradient's start. The first block: scale of G and every row's coefficients;
-// the others: x with rows without a loss as zeros, so that nothing of theirs
-// reaches dW.
+struct LiveTokens {
+  RowCoef* rows;             // coefficients
+  int* index;                // their place among all tokens; -1 behind the last
+  int* count;                // with those behind the last
+  float* scale;              // of G, and its inverse
+};
+
+// The gradient's start: the tokens with a loss moved together (x into 16-byte rows of
+// `ld` values), scale of G and every row's coefficients, dx of the others zeroed. Each
+// block counts the tokens in front of its own.
 template <class T>
 __global__ void __launch_bounds__(1024)
-prepare_kernel(const T* x, int64_t x_ld, int64_t width, T* out, int64_t ld, int64_t tokens,
-               int64_t vocab, const int64_t* __restrict__ targets, const float* __restrict__ lse,
-               const float* __restrict__ dloss, const float* __restrict__ dlse,
-               RowCoef* __restrict__ rows, float* scale) {
-  start_next(), await_previous();
-  if (blockIdx.x > 0) {
-    copy_rows<T>(x, x_ld, width, out, ld, tokens, targets, vocab,
-                 (int64_t)(blockIdx.x - 1) * 1024 + threadIdx.x, (int64_t)(gridDim.x - 1) * 1024);
-    return;
-  }
-  // the largest |dloss| and |dloss + dlse|
+prepare_kernel(const T* __restrict__ x, int64_t x_ld, int64_t width, T* __restrict__ out, int64_t ld,
+               int64_t tokens, int64_t vocab, const int64_t* __restrict__ targets,
+               const float* __restrict__ lse, const float* __restrict__ dloss,
+               const float* __restrict__ dlse, LiveTokens live, T* __restrict__ dx, int64_t dx_ld) {
+  constexpr int kUnit = 16 / sizeof(T);
   __shared__ float part[2][32];
+  __shared__ int counts[2][32], place[1024];
+  start_next(), await_previous();
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int64_t each = (tokens + gridDim.x - 1) / gridDim.x, r0 = blockIdx.x * each;
+  const int64_t r1 = r0 + each < tokens ? r0 + each : tokens;
+  // the largest |dloss| and |dloss + dlse|, tokens in front of the block's, all tokens
   float top[2] = {0.f, 0.f};
+  int n[2] = {0, 0};
 #pragma unroll 4
   for (int64_t t = threadIdx.x; t < tokens; t += 1024) {
     const float one = dloss ? dloss[t] : 0.f, all = one + (dlse ? dlse[t] : 0.f);
-    if (has_loss(targets[t], vocab)) top[0] = fmaxf(top[0], fabsf(one)), top[1] = fmaxf(top[1], fabsf(all));
+    if (has_loss(targets[t], vocab)) {
+      top[0] = fmaxf(top[0], fabsf(one)), top[1] = fmaxf(top[1], fabsf(all));
+      n[0] += t < r0, n[1] += 1;
+    }
   }
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
 #pragma unroll
-    for (int o = 16; o > 0; o /= 2) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
-    if (threadIdx.x % 32 == 0) part[i][threadIdx.x / 32] = top[i];
+    for (int o = 16; o > 0; o /= 2) {
+      top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
+      n[i] += __shfl_xor_sync(0xffffffffu, n[i], o);
+    }
+    if (lane == 0) part[i][warp] = top[i], counts[i][warp] = n[i];
   }
   __syncthreads();
-  for (int i = 0; i < 32; ++i) top[0] = fmaxf(top[0], part[0][i]), top[1] = fmaxf(top[1], part[1][i]);
+  n[0] = n[1] = 0;
+  for (int i = 0; i < 32; ++i) {
+    top[0] = fmaxf(top[0], part[0][i]), top[1] = fmaxf(top[1], part[1][i]);
+    n[0] += counts[0][i], n[1] += counts[1][i];
+  }
+  const int total = n[1], padded_total = total > 0 ? (total + kTokenRound - 1) / kTokenRound * kTokenRound
+                                                   : kTokenRound;
   // That of the loss is scaled to 2^13, unless the other is so much larger that it
   // would leave float16's range. A target's value is nearly -dloss: where all tokens
   // weigh the same it then is nearly -2^13, which 16 bits hold without the error that
@@ -142,40 +153,91 @@ prepare_kernel(const T* x, int64_t x_ld, int64_t width, T* out, int64_t ld, int6
     const int s = e == -127 || e == 128 ? 0 : (13 - e > 126 ? 126 : (13 - e < -126 ? -126 : 13 - e));
     up = __int_as_float((127 + s) << 23), down = __int_as_float((127 - s) << 23);
   }
-  if (threadIdx.x == 0) scale[0] = up, scale[1] = down;
-#pragma unroll 4
-  for (int64_t t = threadIdx.x; t < tokens; t += 1024) {
-    const int64_t at = targets[t];
-    const float one = dloss ? dloss[t] : 0.f, all = one + (dlse ? dlse[t] : 0.f);
-    const float norm = lse[t] * kLog2e;
-    const bool counts = has_loss(at, vocab);
-    rows[t] = {counts ? all * up : 0.f, counts ? one * up : 0.f, counts ? norm : 0.f,
-               counts ? (int)at : -1};
+  if (blockIdx.x == 0 && threadIdx.x == 0) live.scale[0] = up, live.scale[1] = down, *live.count = padded_total;
+  const int64_t per = ld / kUnit;
+  const bool wide = x_ld % kUnit == 0 && (uintptr_t)x % 16 == 0;
+  const bool wide_dx = dx_ld % kUnit == 0 && (uintptr_t)dx % 16 == 0;
+  int next = n[0];                       // place of the next token with a loss
+  for (int64_t base = r0; base < r1; base += 1024) {
+    const int64_t t = base + threadIdx.x;
+    const int64_t at = t < r1 ? targets[t] : -1;
+    const bool counts_for = t < r1 && has_loss(at, vocab);
+    const uint32_t mask = __ballot_sync(0xffffffffu, counts_for);
+    __syncthreads();                     // (what the turn before read)
+    if (lane == 0) counts[0][warp] = __popc(mask);
+    __syncthreads();
+    int mine = next + __popc(mask & ((1u << lane) - 1));
+    for (int i = 0; i < 32; ++i) {
+      if (i < warp) mine += counts[0][i];
+      next += counts[0][i];
+    }
+    place[threadIdx.x] = counts_for ? mine : -1;
+    if (counts_for) {
+      const float one = dloss ? dloss[t] : 0.f, all = one + (dlse ? dlse[t] : 0.f);
+      live.rows[mine] = {all * up, one * up, lse[t] * kLog2e, (int)at};
+      live.index[mine] = (int)t;
+    }
+    __syncthreads();
+    const int rows = r1 - base < 1024 ? (int)(r1 - base) : 1024;
+    // a warp a row, four loads of a lane under way at once
+    for (int r = warp; r < rows; r += 32) {
+      const int to = place[r];
+      if (to >= 0) {
+        const T* from = x + (base + r) * x_ld;
+        for (int64_t u = lane; u < per; u += 128) {
+          uint4 q[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (u + 32 * j < per) q[j] = row_unit(from + (u + 32 * j) * kUnit, width - (u + 32 * j) * kUnit, wide);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (u + 32 * j < per) *(uint4*)(out + to * ld + (u + 32 * j) * kUnit) = q[j];
+        }
+      } else {
+        T* zero = dx + (base + r) * dx_ld;
+        for (int64_t c = lane * kUnit; c < width; c += 32 * kUnit) {
+          if (wide_dx && c + kUnit <= width) {
+            *(uint4*)(zero + c) = make_uint4(0, 0, 0, 0);
+          } else {
+            for (int j = 0; j < kUnit && c + j < width; ++j) zero[c + j] = from_f<T>(0.f);
+          }
+        }
+      }
+    }
+  }
+  if (blockIdx.x == gridDim.x - 1) {
+    const int behind = padded_total - total;
+    if ((int)threadIdx.x < behind) {
+      live.rows[total + threadIdx.x] = {0.f, 0.f, 0.f, -1};
+      live.index[total + threadIdx.x] = -1;
+    }
+    for (int64_t i = threadIdx.x; i < behind * per; i += 1024)
+      *(uint4*)(out + total * ld + i * kUnit) = make_uint4(0, 0, 0, 0);
   }
 }
 
-// dx from the slabs of its sums, in their order; 4 values a thread.
+// dx from the slabs of its sums, of `rows` rows each, in their order; 4 values a thread.
 template <class T>
 __global__ void __launch_bounds__(256)
-finish_dx_kernel(const float* __restrict__ sums, int splits, int64_t ld, int64_t tokens,
-                 int64_t width, const RowCoef* __restrict__ rows, const float* __restrict__ scale,
-                 T* __restrict__ dx, int64_t dx_ld) {
+finish_dx_kernel(const float* __restrict__ sums, int splits, int64_t ld, int64_t rows, int64_t width,
+                 LiveTokens live, T* __restrict__ dx, int64_t dx_ld) {
   await_previous();
-  const float inv = scale[1];
-  const int64_t per = ld / 4;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < tokens * per; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / per, c = i % per * 4;
-    const bool keep = rows[r].target >= 0;
+  const float inv = live.scale[1];
+  const int64_t per = ld / 4, all = *live.count * per;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = all <= 0xffffffffll ? (uint32_t)i / (uint32_t)per : i / per, c = (i - r * per) * 4;
+    const int at = live.index[r];
+    if (at < 0) continue;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
     for (int s = 0; s < splits; ++s) {
-      const float4 u = *(const float4*)(sums + ((int64_t)s * tokens + r) * ld + c);
+      const float4 u = *(const float4*)(sums + ((int64_t)s * rows + r) * ld + c);
       v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
     }
     const float o[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (c + j < width) dx[r * dx_ld + c + j] = from_f<T>(keep ? o[j] * inv : 0.f);
+      if (c + j < width) dx[at * dx_ld + c + j] = from_f<T>(o[j] * inv);
   }
 }
 
@@ -201,6 +263,10 @@ struct Matrix {
   const T* p;
   int64_t ld;
 };
+// Blocks of the gradient's start, no fewer than a token and 16 KiB of x each, and one an SM.
+inline int64_t blocks_to_prepare(int64_t tokens, int64_t bytes) {
+  return std::max<int64_t>(1, std::min({ceil_div(tokens * bytes, 16 * 1024), tokens, (int64_t)148 * 4}));
+}
 inline int64_t padded(int64_t n) { return ceil_div(n, 8) * 8; }
 
 template <class T>

@@ -34,6 +34,7 @@ struct Product {
   float* out;                // sums: slabs of a.rows rows
   int64_t ld;
   bool sums, load;           // onto those of earlier pieces
+  bool live_rows, live_depth;  // of A; the number of tokens with a loss
 };
 struct Work {
   Product p[2];
@@ -42,9 +43,8 @@ struct Work {
   RowStat* stats;            // (tile of N, token)
   float* at_target;
   int64_t vocab;
-  const RowCoef* rows;       // grads
+  LiveTokens live;           // gradients
   int64_t first;
-  const float* scale;
 };
 
 __device__ __forceinline__ void fma2(float2& d, float2 a, float2 b) {
@@ -127,15 +127,20 @@ __global__ void __launch_bounds__(kThreads, 2) loss_f32_kernel(const __grid_cons
   const int split = t / (p.tiles_m * p.tiles_n);
   t %= p.tiles_m * p.tiles_n;
   const int64_t m0 = (int64_t)(t % p.tiles_m) * ROWS, n0 = (int64_t)(t / p.tiles_m) * kTile;
+  const int live = KIND == kStats ? 0 : *w.live.count;
+  Operand oa = p.a;
+  if (p.live_rows) oa.rows = live;
+  if (m0 >= oa.rows) return;
   const int64_t k0 = split * p.depth_per_split;
-  const int depth = (int)(p.depth - k0 < p.depth_per_split ? p.depth - k0 : p.depth_per_split);
+  const int depth = p.live_depth ? live
+                                 : (int)(p.depth - k0 < p.depth_per_split ? p.depth - k0 : p.depth_per_split);
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
   float2 acc[kMine][4];
 #pragma unroll
   for (int i = 0; i < kMine; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = make_float2(0.f, 0.f);
-  Piece<ROWS> a(p.a, m0, k0);
+  Piece<ROWS> a(oa, m0, k0);
   Piece<kTile> b(p.b, n0, k0);
   a.load(depth), b.load(depth);
   a.store(sa[0]), b.store(sb[0]);
@@ -169,7 +174,7 @@ __global__ void __launch_bounds__(kThreads, 2) loss_f32_kernel(const __grid_cons
 #pragma unroll
   for (int i = 0; i < kMine; ++i) {
     const int64_t m = m0 + (kMine == 2 ? ty * 2 + i : i / 4 * 64 + ty * 4 + i % 4);
-    const bool row = m < p.a.rows;
+    const bool row = m < oa.rows;
     float v[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = j % 2 ? acc[i][j / 2].y : acc[i][j / 2].x;
@@ -197,7 +202,7 @@ __global__ void __launch_bounds__(kThreads, 2) loss_f32_kernel(const __grid_cons
     if (!row) continue;
     float* out = p.out + (p.sums ? split * p.a.rows : 0) * p.ld + m * p.ld;
     if constexpr (KIND == kGrads) {
-      const RowCoef q = w.rows[m];
+      const RowCoef q = w.live.rows[m];
       const int64_t at = (int64_t)q.target - w.first;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -205,7 +210,7 @@ __global__ void __launch_bounds__(kThreads, 2) loss_f32_kernel(const __grid_cons
         v[j] = q.target < 0 ? 0.f : g;
       }
     } else {
-      const float inv = p.sums ? 1.f : w.scale[1];
+      const float inv = p.sums ? 1.f : w.live.scale[1];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         v[j] *= inv;
@@ -306,23 +311,25 @@ ferrum_status loss_bwd_f32(ferrum_device* dev, const ferrum_cross_entropy_args* 
   const int want = (int)std::max<int64_t>(
       1, std::min<int64_t>(2 * sm_count() / dx_tiles, ceil_div(std::min(piece, v), 256)));
   const int splits = product_of(tile, {nullptr, 0, n, false}, {nullptr, 0, d, false}, std::min(piece, v), want).splits;
+  const int64_t rows = ceil_div(n, kTokenRound) * kTokenRound;    // room for all tokens
   auto round = [](int64_t b) { return (size_t)((b + 255) / 256 * 256); };
-  const size_t x_bytes = round(n * ld * 4), w_bytes = copy_w ? round(v * ld * 4) : 0;
-  const size_t g_bytes = round(n * piece * 4), sum_bytes = round(splits * n * ld * 4);
-  PoolBuffer ws(dev, x_bytes + w_bytes + g_bytes + sum_bytes + (size_t)n * sizeof(RowCoef) + 256, stream);
+  const size_t x_bytes = round(rows * ld * 4), w_bytes = copy_w ? round(v * ld * 4) : 0;
+  const size_t g_bytes = round(rows * piece * 4), sum_bytes = round(splits * rows * ld * 4);
+  const size_t row_bytes = round(rows * sizeof(RowCoef)), index_bytes = round(rows * 4);
+  PoolBuffer ws(dev, x_bytes + w_bytes + g_bytes + sum_bytes + row_bytes + index_bytes + 256, stream);
   if (ws.status() != cudaSuccess) return cuda_error(ws.status(), "workspace");
   uint8_t* at = ws.as<uint8_t>();
-  float* x = (float*)at;
+  LiveTokens live;
+  live.scale = (float*)at, live.count = (int*)(at + 16);
+  live.rows = (RowCoef*)(at += 256), live.index = (int*)(at += row_bytes);
+  float* x = (float*)(at += index_bytes);
   float* g = (float*)(at += x_bytes);
   float* sums = (float*)(at += g_bytes);
   at += sum_bytes;
   Matrix<float> wt = {(const float*)a->weight, a->weight_stride};
-  float* scale = (float*)(at + w_bytes);
-  RowCoef* rows = (RowCoef*)(at + w_bytes + 256);
-  const int64_t copiers = std::min<int64_t>(ceil_div(n * ld / 4, 1024), 148 * 4);
-  if (ferrum_status s = start(what, true, prepare_kernel<float>, copiers + 1, 1024, 0, stream,
-                              (const float*)a->x, a->x_stride, d, x, ld, n, v, a->targets,
-                              (const float*)a->lse, a->dloss, a->dlse, rows, scale))
+  if (ferrum_status s = start(what, true, prepare_kernel<float>, blocks_to_prepare(n, ld * 4), 1024, 0,
+                              stream, (const float*)a->x, a->x_stride, d, x, ld, n, v, a->targets,
+                              (const float*)a->lse, a->dloss, a->dlse, live, (float*)a->dx, a->dx_stride))
     return s;
   if (copy_w) {
     if (ferrum_status s = copied(wt, d, v, at, false, stream, what)) return s;
@@ -331,20 +338,21 @@ ferrum_status loss_bwd_f32(ferrum_device* dev, const ferrum_cross_entropy_args* 
     const int64_t words = std::min(piece, v - first);
     const float* wp = wt.p + first * wt.ld;
     Work w = {};
-    w.rows = rows, w.scale = scale, w.first = first, w.count = 1;
-    w.p[0] = product_of(g_tile, {x, ld, n, false}, {wp, wt.ld, words, false}, d);
-    w.p[0].out = g, w.p[0].ld = piece;
+    w.live = live, w.first = first, w.count = 1;
+    w.p[0] = product_of(g_tile, {x, ld, rows, false}, {wp, wt.ld, words, false}, d);
+    w.p[0].out = g, w.p[0].ld = piece, w.p[0].live_rows = true;
     if (ferrum_status s = run<kGrads>(w, g_tile, false, stream, what)) return s;
-    w.p[0] = product_of(tile, {g, piece, n, false}, {wp, wt.ld, d, true}, words, splits);
-    w.p[0].out = sums, w.p[0].ld = ld, w.p[0].sums = true, w.p[0].load = first > 0;
-    w.p[1] = product_of(tile, {g, piece, words, true}, {x, ld, d, true}, n);
+    w.p[0] = product_of(tile, {g, piece, rows, false}, {wp, wt.ld, d, true}, words, splits);
+    w.p[0].out = sums, w.p[0].ld = ld, w.p[0].sums = w.p[0].live_rows = true,
+     w.p[0].load = first > 0;
+    w.p[1] = product_of(tile, {g, piece, words, true}, {x, ld, d, true}, rows);
     w.p[1].out = (float*)a->dweight + first * a->dweight_stride, w.p[1].ld = a->dweight_stride;
+    w.p[1].live_depth = true;
     w.count = 2;
     if (ferrum_status s = run<kWeights>(w, tile, false, stream, what)) return s;
   }
   return start(what, false, finish_dx_kernel<float>, std::min<int64_t>(ceil_div(n * ld / 4, 256), 148 * 16),
-               256, 0, stream, (const float*)sums, splits, ld, n, d, (const RowCoef*)rows,
-               (const float*)scale, (float*)a->dx, a->dx_stride);
+               256, 0, stream, (const float*)sums, splits, ld, rows, d, live, (float*)a->dx, a->dx_stride);
 }
 
 }  // namespace seq

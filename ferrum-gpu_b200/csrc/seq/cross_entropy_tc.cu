@@ -83,7 +83,8 @@ struct Product {
   int64_t m, n;
   int tiles_m, tiles_n, splits, steps, steps_per_split;
   bool a_mn;                 // A's rows run along the depth (as all of B's in kWeights)
-  bool tokens;               // its rows are tokens (dx)
+  bool live_rows, live_depth;  // m or the depth is the number of tokens with a loss
+  bool dx;                   // rows go to the tokens' places
   bool sums;                 // the result: float32 sums, a slab per split (else 16 bits)
   bool load, store_map;      // sums of earlier pieces come on top; `out` has a tensor map
   void* out;
@@ -99,10 +100,10 @@ struct Work {
   const int64_t* targets;
   RowStat* stats;            // (half tile of N, m)
   float* at_target;
-  // grads
-  const RowCoef* rows;
+  // gradients
+  LiveTokens live;
+  int known;                 // how many tokens have a loss (with those behind), if the host knows
   int64_t first;             // the piece's first word
-  const float* scale;        // {2^s, 2^-s}
 };
 
 struct Maps {
@@ -114,22 +115,40 @@ struct Maps {
 struct Place {
   int product, tm, tn, split;
 };
-__host__ __device__ __forceinline__ uint32_t tiles_of(const Product& p) {
-  return (uint32_t)p.tiles_m * (uint32_t)p.tiles_n * (uint32_t)p.splits;
+// Extents that depend on the number `live` of tokens with a loss.
+__device__ __forceinline__ int64_t rows_of(const Product& p, int live) { return p.live_rows ? live : p.m; }
+__device__ __forceinline__ uint32_t tiles_m_of(const Product& p, int live) {
+  return p.live_rows ? (uint32_t)(live + kTile - 1) / kTile : p.tiles_m;
+}
+__device__ __forceinline__ uint32_t tiles_of(const Product& p, int live) {
+  return tiles_m_of(p, live) * (uint32_t)p.tiles_n * (uint32_t)p.splits;
+}
+// A tile's steps of depth, from k0 up to k1.
+struct Depth {
+  int k0, k1;
+};
+__device__ __forceinline__ Depth depth_of(const Product& p, int split, int live) {
+  if (p.live_depth) return {0, live / kDepth};
+  const int k0 = split * p.steps_per_split, k1 = k0 + p.steps_per_split;
+  return {k0, k1 < p.steps ? k1 : p.steps};
 }
 template <int KIND>
-__device__ __forceinline__ Place place_of(const Work& w, uint32_t t) {
+__device__ __forceinline__ Place place_of(const Work& w, uint32_t t, int live) {
   Place q;
   q.product = 0;
-  if (KIND == kWeights && t >= tiles_of(w.p[0])) q.product = 1, t -= tiles_of(w.p[0]);
+  if (KIND == kWeights) {
+    const uint32_t first = tiles_of(w.p[0], live);
+    if (t >= first) q.product = 1, t -= first;
+  }
   const Product& p = w.p[q.product];
+  const uint32_t tiles_m = tiles_m_of(p, live);
   q.split = 0;
   if (KIND == kWeights && p.splits > 1) {
-    const uint32_t per = (uint32_t)p.tiles_m * (uint32_t)p.tiles_n;
+    const uint32_t per = tiles_m * (uint32_t)p.tiles_n;
     q.split = (int)(t / per), t %= per;
   }
   const uint32_t group = t / ((uint32_t)kGroup * p.tiles_n), first = group * kGroup;
-  const uint32_t wide = p.tiles_m - first < kGroup ? p.tiles_m - first : kGroup;
+  const uint32_t wide = tiles_m - first < kGroup ? tiles_m - first : kGroup;
   t -= first * p.tiles_n;
   q.tm = (int)(first + t % wide), q.tn = (int)(t / wide);
   return q;
@@ -164,7 +183,7 @@ __device__ __forceinline__ bool wait(S* sh, uint64_t* bar, uint32_t phase, int* 
 
 // What an epilogue reads of its row, a tile ahead of using it.
 template <int KIND>
-__device__ __forceinline__ RowCoef row_ahead(const Work& w, const Place& q, int64_t m) {
+__device__ __forceinline__ RowCoef row_ahead(const Work& w, const Place& q, int64_t m, int live) {
   RowCoef r = {0.f, 0.f, 0.f, -1};
   if constexpr (KIND == kStats) {
     if (m < w.p[0].m) {
@@ -172,10 +191,9 @@ __device__ __forceinline__ RowCoef row_ahead(const Work& w, const Place& q, int6
       r.target = has_loss(at, w.p[0].n) ? (int)at : -1;
     }
   } else if constexpr (KIND == kGrads) {
-    if (m < w.p[0].m) r = w.rows[m];
+    if (m < live) r = w.live.rows[m];
   } else {
-    const Product& p = w.p[q.product];
-    if (p.tokens && m < p.m) r.target = w.rows[m].target;
+    if (w.p[q.product].dx && m < live) r.target = w.live.index[m];   // (where the row goes)
   }
   return r;
 }
@@ -218,12 +236,14 @@ __device__ void finish_stats(const Work& w, uint32_t acc, const RowCoef& row, in
   if (row.target >= 0 && at >= 0 && at < kHalf) w.at_target[m] = hit;
 }
 
-// A warp's 32 rows of 64 values, on their way out through its slot of shared
-// memory: rows of 128 bytes, swizzled as the tensor map has them, or single values
-// where the array has no map.
+// A warp's 32 rows of 64 values, on their way out through its slot of shared memory:
+// rows of 128 bytes, swizzled as the tensor map has them, or single values where the
+// array has no map or rows go to places of their own (`place`, the lane's row's; -1 for
+// none). `rows`: those of the product.
 template <class T>
 __device__ __forceinline__ void put_rows(const Product& p, const CUtensorMap* map, uint8_t* slot,
-                                         const float (&v)[2][32], int64_t m0, int64_t n0, int lane) {
+                                         const float (&v)[2][32], int64_t rows, int64_t m0, int64_t n0,
+                                         int place, int lane) {
   // the store that read the slot before is done with it
   if (lane == 0) bulk_wait_read_all();
   __syncwarp();
@@ -238,21 +258,23 @@ __device__ __forceinline__ void put_rows(const Product& p, const CUtensorMap* ma
   if (p.store_map) {
     fence_proxy_async_smem();
     __syncwarp();
-    if (lane == 0 && m0 < p.m && n0 < p.n) {
+    if (lane == 0 && m0 < rows && n0 < p.n) {
       tma_store_tile2d(map, (int32_t)n0, (int32_t)m0, slot);
       bulk_commit();
     }
   } else {
     __syncwarp();
-    const int rows = p.m - m0 < 32 ? (int)(p.m - m0) : 32, cols = p.n - n0 < 64 ? (int)(p.n - n0) : 64;
-    T* out = (T*)p.out + m0 * p.ld + n0 + lane;
+    const int cols = p.n - n0 < 64 ? (int)(p.n - n0) : 64;
+    if (!p.dx) place = m0 + lane < rows ? (int)(m0 + lane) : -1;
+    T* out = (T*)p.out + n0 + lane;
 #pragma unroll 8
-    for (int r = 0; r < rows; ++r, out += p.ld) {
+    for (int r = 0; r < 32; ++r) {
+      const int to = __shfl_sync(0xffffffffu, place, r);
       const uint8_t* row = slot + r * 128 + lane % 8 * 2;
       const T lo = *(const T*)(row + ((lane / 8) ^ (r & 7)) * 16);
       const T hi = *(const T*)(row + ((lane / 8 + 4) ^ (r & 7)) * 16);
-      if (lane < cols) out[0] = lo;
-      if (lane + 32 < cols) out[32] = hi;
+      if (to >= 0 && lane < cols) out[to * p.ld] = lo;
+      if (to >= 0 && lane + 32 < cols) out[to * p.ld + 32] = hi;
     }
     __syncwarp();
   }
@@ -260,7 +282,8 @@ __device__ __forceinline__ void put_rows(const Product& p, const CUtensorMap* ma
 
 template <class T, class F>
 __device__ void finish_grads(const Work& w, const CUtensorMap* map, uint8_t* slot, uint32_t acc,
-                             const RowCoef& q, int64_t m0, int64_t n0, int lane, F release) {
+                             const RowCoef& q, int64_t rows, int64_t m0, int64_t n0, int lane,
+                             F release) {
   const Product& p = w.p[0];
   // (a target in front of the piece is below 0, whatever is taken from it)
   const int64_t at64 = (int64_t)q.target - w.first - n0;
@@ -284,16 +307,16 @@ __device__ void finish_grads(const Work& w, const CUtensorMap* map, uint8_t* slo
         for (int i = 0; i < 32; ++i) v[h][i] -= at - c - h * 32 == i ? q.one : 0.f;
       }
     }
-    put_rows<T>(p, map, slot, v, m0, n0 + c, lane);
+    put_rows<T>(p, map, slot, v, rows, m0, n0 + c, -1, lane);
   }
 }
 
 // Sums into `partial`, or with them, scaled back, to 16 bits.
 template <class T, class F>
 __device__ void finish_weights(const Work& w, const Product& p, const CUtensorMap* map, uint8_t* slot,
-                               uint32_t acc, const RowCoef& row, int64_t m0, int64_t n0, int split,
-                               int lane, F release) {
-  const float inv = w.scale[1];
+                               uint32_t acc, const RowCoef& row, int64_t rows, int64_t m0, int64_t n0,
+                               int split, int lane, F release) {
+  const float inv = w.live.scale[1];
   const int64_t m = m0 + lane;
   float* part = p.partial ? p.partial + ((int64_t)split * p.m + m) * p.partial_ld + n0 : nullptr;
   if (n0 >= p.n) release();
@@ -305,7 +328,7 @@ __device__ void finish_weights(const Work& w, const Product& p, const CUtensorMa
     tmem_load32(acc + c + 32, v[1]);
     tmem_load_wait();
     if (c + 64 >= kHalf || n0 + c + 64 >= p.n) release();
-    if (p.load && m < p.m) {
+    if (p.load && m < rows) {
 #pragma unroll
       for (int i = 0; i < 64; i += 4) {
         if (n0 + c + i >= p.partial_ld) continue;    // (a multiple of 8)
@@ -315,7 +338,7 @@ __device__ void finish_weights(const Work& w, const Product& p, const CUtensorMa
       }
     }
     if (p.sums) {
-      if (m >= p.m) continue;
+      if (m >= rows) continue;
 #pragma unroll
       for (int i = 0; i < 64; i += 4) {
         if (n0 + c + i >= p.partial_ld) continue;
@@ -323,11 +346,9 @@ __device__ void finish_weights(const Work& w, const Product& p, const CUtensorMa
         *(float4*)(part + c + i) = make_float4(u[0], u[1], u[2], u[3]);
       }
     } else {
-      // (a row without a loss has zeros in G, but W may hold infinities)
-      const bool keep = !p.tokens || row.target >= 0;
 #pragma unroll
-      for (int i = 0; i < 64; ++i) v[i / 32][i % 32] = keep ? v[i / 32][i % 32] * inv : 0.f;
-      put_rows<T>(p, map, slot, v, m0, n0 + c, lane);
+      for (int i = 0; i < 64; ++i) v[i / 32][i % 32] *= inv;
+      put_rows<T>(p, map, slot, v, rows, m0, n0 + c, row.target, lane);
     }
   }
 }
@@ -343,7 +364,6 @@ loss_product_kernel(const __grid_constant__ Maps maps0, const __grid_constant__ 
   constexpr uint32_t kBlock = 64 * kDepth * 2;     // bytes between 64-value blocks of MN-major rows
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const uint32_t rank = cluster_rank();
-  const uint32_t tiles = tiles_of(w.p[0]) + (KIND == kWeights && w.count > 1 ? tiles_of(w.p[1]) : 0);
   const uint32_t pair = blockIdx.x / 2, pairs = gridDim.x / 2;
 
   if (threadIdx.x == 0) {
@@ -363,6 +383,8 @@ loss_product_kernel(const __grid_constant__ Maps maps0, const __grid_constant__ 
   tc_fence_after();
   const uint32_t tmem = sh.tmem;
   start_next(), await_previous();
+  const int live = KIND == kStats ? 0 : (w.known ? w.known : *w.live.count);
+  const uint32_t tiles = tiles_of(w.p[0], live) + (KIND == kWeights ? tiles_of(w.p[1], live) : 0);
 
   if (warp == 0 && lane == 0) {                    // copies
     int stage = 0;
@@ -375,8 +397,7 @@ loss_product_kernel(const __grid_constant__ Maps maps0, const __grid_constant__ 
       const CUtensorMap* map_a = q.product ? &maps1.a : &maps0.a;
       const CUtensorMap* map_b = q.product ? &maps1.b : &maps0.b;
       const int m0 = q.tm * kTile + (int)rank * kHalf, n0 = q.tn * kTile + (int)rank * kHalf;
-      const int k0 = q.split * p.steps_per_split;
-      const int k1 = k0 + p.steps_per_split < p.steps ? k0 + p.steps_per_split : p.steps;
+      const int k0 = depth_of(p, q.split, live).k0, k1 = depth_of(p, q.split, live).k1;
       for (int k = k0; k < k1; ++k) {
         if (!(ok = wait(&sh, &sh.empty[stage], phase ^ 1, w.err_flag))) return;
         if (rank == 0) mbar_arrive_expect_tx(&sh.full[stage], 2 * kStageBytes);
@@ -399,7 +420,7 @@ loss_product_kernel(const __grid_constant__ Maps maps0, const __grid_constant__ 
       }
     };
     for (uint32_t t = pair; ok && t < tiles; t += pairs) {
-      const Place q = place_of<KIND>(w, t);
+      const Place q = place_of<KIND>(w, t, live);
       if (KIND == kWeights && w.p[q.product].a_mn)
         tile(std::true_type(), q);
       else
@@ -424,8 +445,7 @@ loss_product_kernel(const __grid_constant__ Maps maps0, const __grid_constant__ 
       // 16 steps of depth: 32 bytes along a K-major row, two atoms MN-major
       constexpr uint32_t kStepA = (A_MN ? 2048 : 32) / 16, kStepB = (B_MN ? 2048 : 32) / 16;
       const Product& p = w.p[q.product];
-      const int k0 = q.split * p.steps_per_split;
-      const int k1 = k0 + p.steps_per_split < p.steps ? k0 + p.steps_per_split : p.steps;
+      const int k0 = depth_of(p, q.split, live).k0, k1 = depth_of(p, q.split, live).k1;
       if (!(ok = wait(&sh, &sh.drained[buf], buf_phase ^ 1, w.err_flag))) return;
       tc_fence_after();
       const uint32_t acc = tmem + buf * kTile;
@@ -443,7 +463,7 @@ loss_product_kernel(const __grid_constant__ Maps maps0, const __grid_constant__ 
       if (++buf == 2) buf = 0, buf_phase ^= 1;
     };
     for (uint32_t t = pair; ok && t < tiles; t += pairs) {
-      const Place q = place_of<KIND>(w, t);
+      const Place q = place_of<KIND>(w, t, live);
       if (KIND == kWeights && w.p[q.product].a_mn)
         tile(std::true_type(), q);
       else
@@ -460,8 +480,8 @@ loss_product_kernel(const __grid_constant__ Maps maps0, const __grid_constant__ 
     RowCoef row_next = {};
     auto look_ahead = [&](uint32_t t) {
       if (t >= tiles) return;
-      next = place_of<KIND>(w, t);
-      row_next = row_ahead<KIND>(w, next, (int64_t)next.tm * kTile + rank * kHalf + lanes + lane);
+      next = place_of<KIND>(w, t, live);
+      row_next = row_ahead<KIND>(w, next, (int64_t)next.tm * kTile + rank * kHalf + lanes + lane, live);
     };
     look_ahead(pair);
     for (uint32_t t = pair; t < tiles; t += pairs) {
@@ -482,9 +502,10 @@ loss_product_kernel(const __grid_constant__ Maps maps0, const __grid_constant__ 
         if (lane == 0) arrive_at(drained + buf * 8);
       };
       if constexpr (KIND == kStats) finish_stats(w, acc, row, m0 + lane, n0, release);
-      if constexpr (KIND == kGrads) finish_grads<T>(w, out, slot, acc, row, m0, n0, lane, release);
+      if constexpr (KIND == kGrads) finish_grads<T>(w, out, slot, acc, row, live, m0, n0, lane, release);
       if constexpr (KIND == kWeights)
-        finish_weights<T>(w, w.p[q.product], out, slot, acc, row, m0, n0, q.split, lane, release);
+        finish_weights<T>(w, w.p[q.product], out, slot, acc, row, rows_of(w.p[q.product], live), m0, n0,
+                          q.split, lane, release);
       if (++buf == 2) buf = 0, buf_phase ^= 1;
     }
     if (lane == 0) bulk_wait_all();
@@ -856,17 +877,20 @@ ferrum_status bwd(ferrum_device* dev, const ferrum_cross_entropy_args* a, cudaSt
   const int want = (int)std::max<int64_t>(
       1, std::min<int64_t>(pair_count() / dx_tiles, ceil_div(std::min(piece, v), 4 * kDepth)));
   const int splits = product_of(n, d, std::min(piece, v), want).splits;
+  const int64_t rows = ceil_div(n, kTokenRound) * kTokenRound;    // room for all tokens
   const bool need_sums = splits > 1 || !one_piece;
   auto round = [](int64_t b) { return (size_t)((b + 255) / 256 * 256); };
-  const size_t x_bytes = round(n * ld * 2), w_bytes = copy_w ? round(v * ld * 2) : 0;
-  const size_t g_bytes = round((few ? v : n) * g_ld * 2), sum_bytes = need_sums ? round(splits * n * ld * 4) : 0;
-  PoolBuffer ws(dev, x_bytes + w_bytes + g_bytes + sum_bytes + (size_t)n * sizeof(RowCoef) + 256, stream);
+  const size_t x_bytes = round(rows * ld * 2), w_bytes = copy_w ? round(v * ld * 2) : 0;
+  const size_t g_bytes = round((few ? v : rows) * g_ld * 2);
+  const size_t sum_bytes = need_sums ? round(splits * rows * ld * 4) : 0;
+  const size_t row_bytes = round(rows * sizeof(RowCoef)), index_bytes = round(rows * 4);
+  PoolBuffer ws(dev, x_bytes + w_bytes + g_bytes + sum_bytes + row_bytes + index_bytes + 256, stream);
   if (ws.status() != cudaSuccess) return cuda_error(ws.status(), "workspace");
   uint8_t* at = ws.as<uint8_t>();
-  float* scale = (float*)at;
-  RowCoef* rows = (RowCoef*)(at + 256);
-  at += 256 + n * sizeof(RowCoef);
-  at = (uint8_t*)(((uintptr_t)at + 15) & ~(uintptr_t)15);
+  LiveTokens live;
+  live.scale = (float*)at, live.count = (int*)(at + 16);
+  live.rows = (RowCoef*)(at += 256), live.index = (int*)(at += row_bytes);
+  at += index_bytes;
   T* x = (T*)at;
   at += x_bytes;
   T* g = (T*)at;
@@ -874,16 +898,15 @@ ferrum_status bwd(ferrum_device* dev, const ferrum_cross_entropy_args* a, cudaSt
   float* sums = need_sums ? (float*)at : nullptr;
   at += sum_bytes;
   Matrix<T> wt = {(const T*)a->weight, a->weight_stride};
-  const int64_t copiers = std::min<int64_t>(ceil_div(n * ld / 8, 1024), 148 * 4);
-  if (ferrum_status s = start(what, true, prepare_kernel<T>, copiers + 1, 1024, 0, stream,
+  if (ferrum_status s = start(what, true, prepare_kernel<T>, blocks_to_prepare(n, ld * 2), 1024, 0, stream,
                               (const T*)a->x, a->x_stride, d, x, ld, n, v, a->targets,
-                              (const float*)a->lse, a->dloss, a->dlse, rows, scale))
+                              (const float*)a->lse, a->dloss, a->dlse, live, (T*)a->dx, a->dx_stride))
     return s;
   if (copy_w) {
     if (ferrum_status s = copied(wt, d, v, at, false, stream, what)) return s;
   }
 
-  const bool dx_map = mappable(a->dx, a->dx_stride, d), dw_map = mappable(a->dweight, a->dweight_stride, d);
+  const bool dw_map = mappable(a->dweight, a->dweight_stride, d);
   for (int64_t first = 0; first < v; first += piece) {
     const int64_t words = std::min(piece, v - first);
     const bool last = first + words == v;
@@ -895,35 +918,36 @@ ferrum_status bwd(ferrum_device* dev, const ferrum_cross_entropy_args* a, cudaSt
       if (e == cudaSuccess) e = tensor_map(&m, is_bf16<T>(), p, cols, rows, pitch, box);
     };
     if (!few) {
-      map(logits.a, x, d, n, ld, kHalf), map(logits.b, wp, d, words, wt.ld, kHalf);
-      map(logits.out, g, words, n, g_ld, 32);
+      map(logits.a, x, d, rows, ld, kHalf), map(logits.b, wp, d, words, wt.ld, kHalf);
+      map(logits.out, g, words, rows, g_ld, 32);
     }
     if (few)
       map(mx.a, g, g_ld, words, g_ld, kDepth), map(mw.a, g, g_ld, words, g_ld, kHalf);
     else
-      map(mx.a, g, words, n, g_ld, kHalf), map(mw.a, g, words, n, g_ld, kDepth);
-    map(mx.b, wp, d, words, wt.ld, kDepth), map(mw.b, x, d, n, ld, kDepth);
-    if (dx_map) map(mx.out, a->dx, d, n, a->dx_stride, 32);
+      map(mx.a, g, words, rows, g_ld, kHalf), map(mw.a, g, words, rows, g_ld, kDepth);
+    map(mx.b, wp, d, words, wt.ld, kDepth), map(mw.b, x, d, rows, ld, kDepth);
     if (dw_map) map(mw.out, dw, d, words, a->dweight_stride, 32);
     if (e != cudaSuccess) return cuda_error(e, "tensor map");
     Work w = {};
-    w.err_flag = dev->err_flag, w.rows = rows, w.scale = scale, w.first = first;
+    w.err_flag = dev->err_flag, w.live = live, w.first = first;
+    w.known = rows == kTokenRound ? kTokenRound : 0;
     if (few) {
       FewWork f = {};
       int ctas = 0;
-      f.tokens = n, f.vocab = v, f.err_flag = dev->err_flag, f.rows = rows, f.out = g, f.ld = g_ld;
+      f.tokens = n, f.vocab = v, f.err_flag = dev->err_flag, f.rows = live.rows, f.out = g, f.ld = g_ld;
       if (ferrum_status s = run_few<T, true>(wt, Matrix<T>{x, ld}, d, f, ctas, false, stream, what)) return s;
     } else {
-      w.p[0] = product_of(n, words, d), w.count = 1;
-      w.p[0].store_map = true;
+      w.p[0] = product_of(rows, words, d), w.count = 1;
+      w.p[0].store_map = w.p[0].live_rows = true;
+      w.p[0].out = g;
       if (ferrum_status s = run<T, kGrads>(logits, logits, w, false, stream, what)) return s;
     }
 
-    Product px = product_of(n, d, words, splits), pw = product_of(words, d, few ? g_ld : n);
-    px.tokens = true;
+    Product px = product_of(rows, d, words, splits), pw = product_of(words, d, few ? g_ld : rows);
+    px.live_rows = px.dx = true, pw.live_depth = !few;
     px.partial = sums, px.partial_ld = ld;
     px.load = first > 0, px.sums = splits > 1 || !last;
-    px.out = a->dx, px.ld = a->dx_stride, px.store_map = dx_map;
+    px.out = a->dx, px.ld = a->dx_stride;
     (few ? px : pw).a_mn = true;
     pw.out = dw, pw.ld = a->dweight_stride, pw.store_map = dw_map;
     // the product of the longer tiles first, so that the last ones are short
@@ -933,8 +957,7 @@ ferrum_status bwd(ferrum_device* dev, const ferrum_cross_entropy_args* a, cudaSt
   }
   if (splits > 1)
     return start(what, false, finish_dx_kernel<T>, std::min<int64_t>(ceil_div(n * ld / 4, 256), 148 * 16),
-                 256, 0, stream, (const float*)sums, splits, ld, n, d, (const RowCoef*)rows,
-                 (const float*)scale, (T*)a->dx, a->dx_stride);
+                 256, 0, stream, (const float*)sums, splits, ld, rows, d, live, (T*)a->dx, a->dx_stride);
   return FERRUM_OK;
 }
 
