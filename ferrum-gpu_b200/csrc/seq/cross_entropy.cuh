@@ -87,14 +87,14 @@ copy_rows_kernel(const T* __restrict__ in, int64_t in_ld, int64_t width, T* __re
 }
 
 // The gradient works on the tokens that have a loss, one after the other, as many as
-// there are rounded up to 64 (and 64 at least): the rows behind the last are zeros.
-constexpr int kTokenRound = 64;
-
+// there are rounded up to `round` (and that many at least), whole steps of a product's
+// depth: the rows behind the last are zeros.
 struct LiveTokens {
   RowCoef* rows;             // coefficients
   int* index;                // their place among all tokens; -1 behind the last
   int* count;                // with those behind the last
   float* scale;              // of G, and its inverse
+  int round;                 // 64 at most
 };
 
 // The gradient's start: the tokens with a loss moved together (x into 16-byte rows of
@@ -139,8 +139,8 @@ prepare_kernel(const T* __restrict__ x, int64_t x_ld, int64_t width, T* __restri
     top[0] = fmaxf(top[0], part[0][i]), top[1] = fmaxf(top[1], part[1][i]);
     n[0] += counts[0][i], n[1] += counts[1][i];
   }
-  const int total = n[1], padded_total = total > 0 ? (total + kTokenRound - 1) / kTokenRound * kTokenRound
-                                                   : kTokenRound;
+  const int total = n[1];
+  const int padded_total = total > 0 ? (total + live.round - 1) / live.round * live.round : live.round;
   // That of the loss is scaled to 2^13, unless the other is so much larger that it
   // would leave float16's range. A target's value is nearly -dloss: where all tokens
   // weigh the same it then is nearly -2^13, which 16 bits hold without the error that

@@ -311,7 +311,7 @@ ferrum_status loss_bwd_f32(ferrum_device* dev, const ferrum_cross_entropy_args* 
   const int want = (int)std::max<int64_t>(
       1, std::min<int64_t>(2 * sm_count() / dx_tiles, ceil_div(std::min(piece, v), 256)));
   const int splits = product_of(tile, {nullptr, 0, n, false}, {nullptr, 0, d, false}, std::min(piece, v), want).splits;
-  const int64_t rows = ceil_div(n, kTokenRound) * kTokenRound;    // room for all tokens
+  const int64_t rows = ceil_div(n, kStep) * kStep;    // room for all tokens
   auto round = [](int64_t b) { return (size_t)((b + 255) / 256 * 256); };
   const size_t x_bytes = round(rows * ld * 4), w_bytes = copy_w ? round(v * ld * 4) : 0;
   const size_t g_bytes = round(rows * piece * 4), sum_bytes = round(splits * rows * ld * 4);
@@ -320,7 +320,7 @@ ferrum_status loss_bwd_f32(ferrum_device* dev, const ferrum_cross_entropy_args* 
   if (ws.status() != cudaSuccess) return cuda_error(ws.status(), "workspace");
   uint8_t* at = ws.as<uint8_t>();
   LiveTokens live;
-  live.scale = (float*)at, live.count = (int*)(at + 16);
+  live.round = kStep, live.scale = (float*)at, live.count = (int*)(at + 16);
   live.rows = (RowCoef*)(at += 256), live.index = (int*)(at += row_bytes);
   float* x = (float*)(at += index_bytes);
   float* g = (float*)(at += x_bytes);

@@ -877,7 +877,7 @@ ferrum_status bwd(ferrum_device* dev, const ferrum_cross_entropy_args* a, cudaSt
   const int want = (int)std::max<int64_t>(
       1, std::min<int64_t>(pair_count() / dx_tiles, ceil_div(std::min(piece, v), 4 * kDepth)));
   const int splits = product_of(n, d, std::min(piece, v), want).splits;
-  const int64_t rows = ceil_div(n, kTokenRound) * kTokenRound;    // room for all tokens
+  const int64_t rows = ceil_div(n, kDepth) * kDepth;    // room for all tokens
   const bool need_sums = splits > 1 || !one_piece;
   auto round = [](int64_t b) { return (size_t)((b + 255) / 256 * 256); };
   const size_t x_bytes = round(rows * ld * 2), w_bytes = copy_w ? round(v * ld * 2) : 0;
@@ -888,7 +888,7 @@ ferrum_status bwd(ferrum_device* dev, const ferrum_cross_entropy_args* a, cudaSt
   if (ws.status() != cudaSuccess) return cuda_error(ws.status(), "workspace");
   uint8_t* at = ws.as<uint8_t>();
   LiveTokens live;
-  live.scale = (float*)at, live.count = (int*)(at + 16);
+  live.round = kDepth, live.scale = (float*)at, live.count = (int*)(at + 16);
   live.rows = (RowCoef*)(at += 256), live.index = (int*)(at += row_bytes);
   at += index_bytes;
   T* x = (T*)at;
@@ -930,7 +930,7 @@ ferrum_status bwd(ferrum_device* dev, const ferrum_cross_entropy_args* a, cudaSt
     if (e != cudaSuccess) return cuda_error(e, "tensor map");
     Work w = {};
     w.err_flag = dev->err_flag, w.live = live, w.first = first;
-    w.known = rows == kTokenRound ? kTokenRound : 0;
+    w.known = rows == kDepth ? kDepth : 0;
     if (few) {
       FewWork f = {};
       int ctas = 0;
