@@ -95,6 +95,7 @@ struct LiveTokens {
   int* count;                // with those behind the last
   float* scale;              // of G, and its inverse
   int round;                 // 64 at most
+  int64_t x_rows;            // rows of x that exist: none behind them is read
 };
 
 // The gradient's start: the tokens with a loss moved together (x into 16-byte rows of
@@ -134,10 +135,14 @@ prepare_kernel(const T* __restrict__ x, int64_t x_ld, int64_t width, T* __restri
     if (lane == 0) part[i][warp] = top[i], counts[i][warp] = n[i];
   }
   __syncthreads();
-  n[0] = n[1] = 0;
-  for (int i = 0; i < 32; ++i) {
-    top[0] = fmaxf(top[0], part[0][i]), top[1] = fmaxf(top[1], part[1][i]);
-    n[0] += counts[0][i], n[1] += counts[1][i];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    top[i] = part[i][lane], n[i] = counts[i][lane];
+#pragma unroll
+    for (int o = 16; o > 0; o /= 2) {
+      top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], o));
+      n[i] += __shfl_xor_sync(0xffffffffu, n[i], o);
+    }
   }
   const int total = n[1];
   const int padded_total = total > 0 ? (total + live.round - 1) / live.round * live.round : live.round;
@@ -166,11 +171,14 @@ prepare_kernel(const T* __restrict__ x, int64_t x_ld, int64_t width, T* __restri
     __syncthreads();                     // (what the turn before read)
     if (lane == 0) counts[0][warp] = __popc(mask);
     __syncthreads();
-    int mine = next + __popc(mask & ((1u << lane) - 1));
-    for (int i = 0; i < 32; ++i) {
-      if (i < warp) mine += counts[0][i];
-      next += counts[0][i];
+    int in_front = lane < warp ? counts[0][lane] : 0, group = counts[0][lane];
+#pragma unroll
+    for (int o = 16; o > 0; o /= 2) {
+      in_front += __shfl_xor_sync(0xffffffffu, in_front, o);
+      group += __shfl_xor_sync(0xffffffffu, group, o);
     }
+    const int mine = next + in_front + __popc(mask & ((1u << lane) - 1));
+    next += group;
     place[threadIdx.x] = counts_for ? mine : -1;
     if (counts_for) {
       const float one = dloss ? dloss[t] : 0.f, all = one + (dlse ? dlse[t] : 0.f);
@@ -211,7 +219,8 @@ prepare_kernel(const T* __restrict__ x, int64_t x_ld, int64_t width, T* __restri
       live.rows[total + threadIdx.x] = {0.f, 0.f, 0.f, -1};
       live.index[total + threadIdx.x] = -1;
     }
-    for (int64_t i = threadIdx.x; i < behind * per; i += 1024)
+    const int64_t zeros = (padded_total < live.x_rows ? padded_total : live.x_rows) - total;
+    for (int64_t i = threadIdx.x; i < zeros * per; i += 1024)
       *(uint4*)(out + total * ld + i * kUnit) = make_uint4(0, 0, 0, 0);
   }
 }

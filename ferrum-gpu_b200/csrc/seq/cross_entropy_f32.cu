@@ -320,7 +320,7 @@ ferrum_status loss_bwd_f32(ferrum_device* dev, const ferrum_cross_entropy_args* 
   if (ws.status() != cudaSuccess) return cuda_error(ws.status(), "workspace");
   uint8_t* at = ws.as<uint8_t>();
   LiveTokens live;
-  live.round = kStep, live.scale = (float*)at, live.count = (int*)(at + 16);
+  live.round = kStep, live.x_rows = rows, live.scale = (float*)at, live.count = (int*)(at + 16);
   live.rows = (RowCoef*)(at += 256), live.index = (int*)(at += row_bytes);
   float* x = (float*)(at += index_bytes);
   float* g = (float*)(at += x_bytes);

@@ -880,7 +880,7 @@ ferrum_status bwd(ferrum_device* dev, const ferrum_cross_entropy_args* a, cudaSt
   const int64_t rows = ceil_div(n, kDepth) * kDepth;    // room for all tokens
   const bool need_sums = splits > 1 || !one_piece;
   auto round = [](int64_t b) { return (size_t)((b + 255) / 256 * 256); };
-  const size_t x_bytes = round(rows * ld * 2), w_bytes = copy_w ? round(v * ld * 2) : 0;
+  const size_t x_bytes = round(n * ld * 2), w_bytes = copy_w ? round(v * ld * 2) : 0;
   const size_t g_bytes = round((few ? v : rows) * g_ld * 2);
   const size_t sum_bytes = need_sums ? round(splits * rows * ld * 4) : 0;
   const size_t row_bytes = round(rows * sizeof(RowCoef)), index_bytes = round(rows * 4);
@@ -888,7 +888,8 @@ ferrum_status bwd(ferrum_device* dev, const ferrum_cross_entropy_args* a, cudaSt
   if (ws.status() != cudaSuccess) return cuda_error(ws.status(), "workspace");
   uint8_t* at = ws.as<uint8_t>();
   LiveTokens live;
-  live.round = kDepth, live.scale = (float*)at, live.count = (int*)(at + 16);
+  live.round = kDepth, live.x_rows = n;      // (the tensor maps end there)
+  live.scale = (float*)at, live.count = (int*)(at + 16);
   live.rows = (RowCoef*)(at += 256), live.index = (int*)(at += row_bytes);
   at += index_bytes;
   T* x = (T*)at;
@@ -918,14 +919,14 @@ ferrum_status bwd(ferrum_device* dev, const ferrum_cross_entropy_args* a, cudaSt
       if (e == cudaSuccess) e = tensor_map(&m, is_bf16<T>(), p, cols, rows, pitch, box);
     };
     if (!few) {
-      map(logits.a, x, d, rows, ld, kHalf), map(logits.b, wp, d, words, wt.ld, kHalf);
+      map(logits.a, x, d, n, ld, kHalf), map(logits.b, wp, d, words, wt.ld, kHalf);
       map(logits.out, g, words, rows, g_ld, 32);
     }
     if (few)
       map(mx.a, g, g_ld, words, g_ld, kDepth), map(mw.a, g, g_ld, words, g_ld, kHalf);
     else
       map(mx.a, g, words, rows, g_ld, kHalf), map(mw.a, g, words, rows, g_ld, kDepth);
-    map(mx.b, wp, d, words, wt.ld, kDepth), map(mw.b, x, d, rows, ld, kDepth);
+    map(mx.b, wp, d, words, wt.ld, kDepth), map(mw.b, x, d, n, ld, kDepth);
     if (dw_map) map(mw.out, dw, d, words, a->dweight_stride, 32);
     if (e != cudaSuccess) return cuda_error(e, "tensor map");
     Work w = {};
