@@ -20,6 +20,15 @@
 // sets of accumulators (all 512 columns), so that eight warps finish one tile while
 // the next is computed. 74 pairs walk the tiles; dx and dW of a piece share a launch,
 // so that the last wave of one is filled by the other.
+//
+// 8192 x 2048 x 32768 bf16: 715 us forward (1.54 PFLOP/s; cuBLAS takes 702 for the
+// logits alone), 2390 for the gradient (1.38 PFLOP/s over its three products, at the
+// power limit; a library product sustains 1.39). The tensor pipe is busy for 90 to
+// 95 % of the cycles. What it took: one thread issues the products, so descriptors move
+// by sums and tiles are numbered by 32 bits (gradient 2755 -> 2350 us); accumulators
+// are read at once and released before anything is stored (16384 x 512 x 32768:
+// 575 -> 386 us); an arrival that orders no memory, since one that does waits for the
+// warp's stores.
 #include <cudaTypedefs.h>
 
 #include <algorithm>
@@ -857,7 +866,9 @@ ferrum_status fwd(ferrum_device* dev, const ferrum_cross_entropy_args* a, cudaSt
   return finish_loss(stats, parts, at_target, a, stream, what);
 }
 
-// Words of a piece of the vocabulary: 256 MiB of G, but no fewer than 4096.
+// Words of a piece of the vocabulary: 256 MiB of G, but no fewer than 4096 (gradient of
+// 8192 x 2048 x 32768 with 128 and 256 MiB: 2466 and 2350 us; every piece but the first
+// reads dx's sums again).
 int64_t piece_of(int64_t tokens, int64_t vocab) {
   const int64_t n = std::max<int64_t>(((int64_t)1 << 27) / tokens / kTile * kTile, 4096);
   return std::min(n, ceil_div(vocab, 64) * 64);

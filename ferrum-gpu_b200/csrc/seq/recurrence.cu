@@ -7,8 +7,13 @@
 // the logarithms. The maps of a turn's warps (8 a block, 1 to 8 blocks of a
 // cluster, joined over distributed shared memory) give each warp the state it
 // starts from; it then walks its 16 steps and stores them. One pass over the
-// data, no block waits for another that might not run. What bounds it: see the
-// figures at the launch.
+// data, no block waits for another that might not run.
+//
+// 8 x 2048 x 4096 bf16: 160 us forward, 3.3 TB/s of the 6.5 of a copy (57
+// instructions a value, issue slots 70 % busy, special functions 52 %: five a value
+// are 75 us); its gradient 290 us, 3.2 TB/s (114 instructions, 75 %). float32: 172 us,
+// 6.2 TB/s, and 395, 4.8 TB/s. 1 x 8191 x 2048 bf16: 66 and 104 us, 10 and 32 turns
+// one after the other. 128 registers and 14 to 15 warps an SM in both.
 //
 // Gradient, with G the gradient of the state:  G_t = dout_t + a_{t+1} G_{t+1}. The
 // same backwards over time; the states come from those the forward saved in front
@@ -72,7 +77,8 @@ __device__ __forceinline__ void store_at_rank(float2* p, uint32_t rank, float2 v
 }
 
 // How the rows of a call lie: at multiples of 16 bytes, of 4 bytes with an even
-// number of channels (16-bit types), or of an element.
+// number of channels (16-bit types), or of an element (8 x 2048 x 4095: 226 us where
+// 4096 channels take 160).
 enum Lie { kWhole, kPaired, kSingle };
 
 // A warp's rows of one array in shared memory: 16 steps of 32 * VL channels. Where
@@ -512,7 +518,9 @@ ferrum_status check_recurrence(const ferrum_device* dev, const ferrum_recurrence
 }
 
 // Blocks of a cluster: more of them where there are few rows of channels, as long
-// as each has steps to walk.
+// as each has steps to walk. With 1, 2, 4 and 8 blocks, us: 1 x 8191 x 2048 bf16
+// forward 224, 156, 86, 66, gradient (twice the rows) 238, 159, 110, 114;
+// 8 x 2048 x 4096 164, 209, 230, 311 and 310, 367, 395, 453.
 int cluster_of(int64_t parts, int64_t length, int warps) {
   int c = 1;
   while (c < kMaxCluster && parts * c * 2 <= 148 * 2 && (int64_t)c * warps * kSteps < length) c *= 2;
