@@ -67,6 +67,9 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
+// The block's barrier for warps that come to it from different places of the code (as
+// __syncthreads() is not meant for).
+__device__ __forceinline__ void block_sync() { asm volatile("bar.sync 0;" ::: "memory"); }
 // Stores to this CTA's shared variable in CTA `rank` of the cluster.
 __device__ __forceinline__ void store_at_rank(float2* p, uint32_t rank, float2 v) {
   uint32_t a;
@@ -167,7 +170,7 @@ __device__ __forceinline__ void exchange(Exchange<VL>& x, int parity, int warp, 
     x.warp[parity][warp][lane + 32 * e] = make_float2(a[e].code, q[e]);
     if (size > 1) x.log_a[warp][lane + 32 * e] = log_a[e];
   }
-  __syncthreads();
+  block_sync();
   const int at = back ? warps - 1 - warp : warp;         // place in the walk
   if (size > 1) {
     if (warp < VL) {          // warp e sums up the block for its 32 channels

@@ -23,7 +23,8 @@ every sequence on kept state. They call the C ABI of ``include/ferrum_seq.h``
 Activations are float32, float16 or bfloat16 tensors, all of one type, shaped
 (batch, length, channels) with contiguous channels and any other strides
 (``long_conv``: (batch, channels, length), any strides). Parameters, scan
-states and parameter gradients are float32. Arithmetic runs in float32; an
+states and parameter gradients are float32 (but a vocabulary matrix and its
+gradient, which have x's type). Arithmetic runs in float32; an
 output is rounded once to its type. Results do not depend on scheduling.
 
 ``lengths`` (int32, one per sequence) are the valid lengths of a padded batch:
@@ -424,8 +425,9 @@ def linear_cross_entropy(x, weight, targets, *, device=None, stream=None) -> Cro
 def linear_cross_entropy_backward(dloss, x, weight, targets, lse, *, dlse=None, device=None,
                                   stream=None) -> CrossEntropyGrads:
     """Gradients of ``linear_cross_entropy`` for those of loss (``dloss``) and
-    of lse (``dlse``), float32. ``lse`` is the forward's. The logits are computed
-    again, a piece of the vocabulary at a time. dx and dweight have x's type."""
+    of lse (``dlse``), float32; either may be None. ``lse`` is the forward's. The
+    logits are computed again, a piece of the vocabulary at a time, for the tokens
+    that have a loss. dx and dweight have x's type."""
     return CrossEntropyGrads(*_call(
         _sequence.linear_cross_entropy_backward, dloss, x, weight, targets, lse, dlse, device,
         stream))

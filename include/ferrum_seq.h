@@ -11,7 +11,8 @@
  * Each call takes a pointer to an argument block. `struct_size` is
  * sizeof(the block); zero the block, then set what the call uses. Strides are
  * in elements. NULL marks an absent optional array. Activations ("data") have
- * type `dtype`; parameters, scan states and parameter gradients are float32.
+ * type `dtype`; parameters, scan states and parameter gradients are float32 (but
+ * a vocabulary matrix and its gradient, of type `dtype`).
  * Sums, recurrences and statistics run in float32; each output is rounded
  * once to its type. No result depends on the order in which blocks run.
  * An array that a call writes shares no memory with its other arrays, except

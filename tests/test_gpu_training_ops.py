@@ -457,6 +457,7 @@ LOSS = [  # tokens, width, vocab, masked
     (300, 512, 4099, 0.1),
     (700, 200, 9000, 0.1),
     (5, 2048, 3001, 0.2),
+    (70, 24, 3, 0.2),
     (100, 320, 5000, 0.1),
     (64, 136, 20011, 0.1),
 ]
