@@ -314,10 +314,32 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 2) recurrence_fwd_kernel(RecAr
         po += p.out.st;
       }
     };
+    // Behind the sequence's end the state stands still (8 sequences of 0 to 2048 steps x
+    // 4096 bf16: 187 us where warps walk their padding, 121 where they do not; the
+    // gradient 353 and 209).
+    auto stand = [&] {
+      Factor all[VL];
+      float none[VL], h[VL];
+#pragma unroll
+      for (int e = 0; e < VL; ++e) all[e].code = kKeep, none[e] = 0.f;
+      exchange<VL>(ex, parity, warp, warps, rank, size, false, lane, all, none, none, carry, h);
+      if (t0 >= p.length) return;
+      if (p.saved) {
+#pragma unroll
+        for (int e = 0; e < VL; ++e) {
+          const int c = S::channel(lane, e);
+          if (c < channels) p.saved[(b * saves + t0 / kSteps) * p.channels + d0 + c] = h[e];
+        }
+      }
+      const int rows = p.length - t0 < kSteps ? (int)(p.length - t0) : kSteps;
+      for (int j = 0; j < rows; ++j) S::store(p.out.at(b, t0 + j) + d0, lane, channels, none);
+    };
     if (n == kSteps && mild)
       walk(std::true_type());
-    else
+    else if (n > 0)
       walk(std::false_type());
+    else
+      stand();
   }
   if (p.final && warp == 0 && rank == 0) {
 #pragma unroll
@@ -329,8 +351,9 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 2) recurrence_fwd_kernel(RecAr
   if (size > 1) cluster_sync();       // no block ends while another may store to it
 }
 
+// (Blocks an SM by their shared memory: two of 8 warps, three of 4.)
 template <class T, int LIE, int WARPS>
-__global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) recurrence_bwd_kernel(RecArrays<T> p) {
+__global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 2 : 3) recurrence_bwd_kernel(RecArrays<T> p) {
   using S = Stage<T, 1, LIE>;
   extern __shared__ __align__(16) uint8_t raw[];
   Exchange<1>& ex = *(Exchange<1>*)raw;
@@ -431,10 +454,25 @@ __global__ void __launch_bounds__(32 * WARPS, 16 / WARPS) recurrence_bwd_kernel(
         ox -= p.dx.st, oi -= p.dig.st, orr -= p.drg.st;
       }
     };
+    auto stand = [&] {
+      const Factor all[1] = {{kKeep}};
+      const float none[1] = {0.f};
+      float later[1];
+      exchange<1>(ex, parity, warp, warps, rank, size, true, lane, all, none, none, carry, later);
+      if (t0 >= p.length || !mine) return;
+      const int rows = p.length - t0 < kSteps ? (int)(p.length - t0) : kSteps;
+      for (int j = 0; j < rows; ++j) {
+        p.dx.at(b, t0 + j)[d0 + lane] = from_f<T>(0.f);
+        p.dig.at(b, t0 + j)[d0 + lane] = from_f<T>(0.f);
+        p.drg.at(b, t0 + j)[d0 + lane] = from_f<T>(0.f);
+      }
+    };
     if (n == kSteps && mild)
       walk(std::true_type());
-    else
+    else if (n > 0)
       walk(std::false_type());
+    else
+      stand();
   }
   if (p.dinitial && mine && warp == 0 && rank == 0) p.dinitial[at] = carry[0];
   // the block's sum of ddecay, warp by warp
