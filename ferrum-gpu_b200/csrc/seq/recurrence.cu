@@ -11,8 +11,8 @@
 //
 // 8 x 2048 x 4096 bf16: 160 us forward, 3.3 TB/s of the 6.5 of a copy (57
 // instructions a value, issue slots 70 % busy, special functions 52 %: five a value
-// are 75 us); its gradient 290 us, 3.2 TB/s (114 instructions, 75 %). float32: 172 us,
-// 6.2 TB/s, and 395, 4.8 TB/s. 1 x 8191 x 2048 bf16: 66 and 104 us, 10 and 32 turns
+// are 75 us); its gradient 294 us, 3.2 TB/s (114 instructions, 75 %). float32: 173 us,
+// 6.2 TB/s, and 406, 4.6 TB/s. 1 x 8191 x 2048 bf16: 66 and 104 us, 10 and 32 turns
 // one after the other. 128 registers and 14 to 15 warps an SM in both.
 //
 // Gradient, with G the gradient of the state:  G_t = dout_t + a_{t+1} G_{t+1}. The
