@@ -347,7 +347,8 @@ def gated_recurrence(x, input_gate, recurrence_gate, decay, *, initial_state=Non
     (channels), not negative: a channel forgets at most by exp(-decay) a step.
     initial_state: (batch, channels) float32. With ``save_states`` the result
     carries what the backward needs. Where 1 - a^2 is not above 0, the root and
-    the gradient through it are 0.
+    the gradient through it are 0. A state that is infinite is NaN a step later (h
+    moves by (a - 1) h where a is close to 1).
     """
     return RecurrenceResult(*_call(
         _sequence.gated_recurrence, x, input_gate, recurrence_gate, decay, initial_state, lengths,
