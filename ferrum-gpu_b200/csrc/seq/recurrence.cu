@@ -64,13 +64,15 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
-}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+__device__ __forceinline__ void cluster_sync() { cluster_arrive(), cluster_wait(); }
 // The block's barrier for warps that come to it from different places of the code (as
 // __syncthreads() is not meant for).
 __device__ __forceinline__ void block_sync() { asm volatile("bar.sync 0;" ::: "memory"); }
-// Stores to this CTA's shared variable in CTA `rank` of the cluster.
+// Stores to this CTA's shared variable in CTA `rank` of the cluster, which has started (the
+// kernels arrive at the cluster's barrier first thing and wait there in front of their
+// first turn, behind its copies).
 __device__ __forceinline__ void store_at_rank(float2* p, uint32_t rank, float2 v) {
   uint32_t a;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
@@ -218,6 +220,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 2) recurrence_fwd_kernel(RecAr
   Exchange<VL>& ex = *(Exchange<VL>*)raw;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32;
   const uint32_t rank = cluster_rank(), size = cluster_size();
+  if (size > 1) cluster_arrive();     // waited for in front of the first store to another block
   uint8_t* stage = raw + (size > 1 ? sizeof(Exchange<VL>) : Exchange<VL>::kAlone) + warp * 6 * S::kBytes;
   const int64_t part = blockIdx.x / size, b = part / p.groups, d0 = part % p.groups * 32 * VL;
   const int channels = p.channels - d0 < 32 * VL ? (int)(p.channels - d0) : 32 * VL;
@@ -250,6 +253,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 2) recurrence_fwd_kernel(RecAr
     cp_async_commit();
   };
   fill(t0, 0);
+  if (size > 1) cluster_wait();
   for (int64_t turn = 0; turn < turns; ++turn, t0 += chunk) {
     const int parity = (int)(turn & 1), n = valid(t0);
     __syncwarp();
@@ -359,6 +363,7 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 2 : 3) recurrence_bwd
   Exchange<1>& ex = *(Exchange<1>*)raw;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32;
   const uint32_t rank = cluster_rank(), size = cluster_size();
+  if (size > 1) cluster_arrive();     // waited for in front of the first store to another block
   uint8_t* stage = raw + (size > 1 ? sizeof(Exchange<1>) : Exchange<1>::kAlone) + warp * 8 * S::kBytes;
   const int64_t part = blockIdx.x / size, b = part / p.groups, d0 = part % p.groups * 32;
   const int channels = p.channels - d0 < 32 ? (int)(p.channels - d0) : 32;
@@ -385,6 +390,7 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 2 : 3) recurrence_bwd
     cp_async_commit();
   };
   if (turns > 0) fill(t0, (int)(turns - 1) & 1);
+  if (size > 1) cluster_wait();
   for (int64_t turn = turns - 1; turn >= 0; --turn, t0 -= chunk) {
     const int parity = (int)(turn & 1), n = valid(t0);
     __syncwarp();
