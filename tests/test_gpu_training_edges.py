@@ -67,3 +67,91 @@ def test_clusters_with_empty_sequences(b, kind, dtype):
     assert torch.equal(g.dinitial_state[none], dfin[none])
     for v in (r.out, g.dx, g.dinput_gate, g.drecurrence_gate):
         assert not v[none].any()
+
+
+# ---------------------------------------------------------------- decays
+
+def decays(kind, d):
+    """`mild` channels take the recurrence's short form, `strong` ones the general one, a
+    warp with both of them the general one for all; log-uniform up to 20."""
+    u = torch.rand(d, generator=torch.Generator().manual_seed(d)).cuda()
+    mild, strong = 0.01 * 100 ** u, 1.001 * 20 ** u
+    if kind == "mild":
+        return mild
+    if kind == "strong":
+        return strong
+    if kind == "groups":         # 64 channels of one kind, then 64 of the other
+        return torch.where(torch.arange(d, device="cuda") // 64 % 2 == 0, mild, strong)
+    return torch.where(torch.arange(d, device="cuda") % 5 == 3, strong, mild)
+
+
+def check_recurrence(x, ig, rg, decay, h, ln, dout, dfin, memory):
+    """All outputs and gradients against 64 bits. A step adds 10 units of 2^-24 and its
+    input 20, which live on for `memory` steps; gradients are sums of the same kind
+    over the state's gradient: four times that (test_gpu_training_ops.py has the
+    derivation). drg is ddecay's term times decay (1 - r), ddecay the sum of its terms."""
+    b, n, d = x.shape
+    leaves = [clean(v, ln).requires_grad_() for v in (x, ig, rg)]
+    leaves += [decay.double().requires_grad_(), h.double().requires_grad_()]
+    out_ref, fin_ref = ref_recurrence(*leaves, ln)
+    want = torch.autograd.grad((out_ref * clean(dout, ln)).sum() + (fin_ref * dfin.double()).sum(), leaves)
+    r = sq.gated_recurrence(x, ig, rg, decay, initial_state=h, lengths=ln, save_states=True)
+    got = sq.gated_recurrence_backward(dout, x, ig, rg, decay, r.states, lengths=ln, dfinal_state=dfin)
+    c = (20 + 10 * min(n, memory)) * EPS
+    top = max(out_ref.detach().abs().max().item(), h.abs().max().item())
+    within(r.out, out_ref, c * top, "out")
+    within(r.final_state, fin_ref, c * top, "final state")
+    for g, w, what in zip(got, want, got._fields):
+        if what == "ddecay":
+            per = want[2].abs() / (decay.double() * (1 - torch.sigmoid(leaves[2].detach())))
+            assert ((g.double() - w).abs() <= 4 * c * per.sum((0, 1)).clamp(min=top) + U[F32] * w.abs()).all(), what
+        else:
+            within(g, w, 4 * c * max(w.abs().max().item(), top), what)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("kind", ["mild", "strong", "groups", "mixed"])
+@pytest.mark.parametrize("b,n,d", [(3, 1300, 200), (7, 700, 198), (15, 300, 200), (60, 200, 130), (2, 40, 77)])
+def test_recurrence_decays(b, n, d, kind, ragged, dtype):
+    """Full warps of the short and the general form, over several turns, in clusters of
+    8, 4, 2 and 1 blocks, whole and ragged."""
+    x, ig, rg, dout = (rnd(k, b, n, d, dtype=dtype) for k in range(4))
+    ln = lengths_of(b, n, "mixed") if ragged else None
+    if ragged:
+        pad = torch.arange(n, device="cuda")[None] >= ln[:, None].long()
+        for v in (x, ig, rg, dout):
+            v[pad] = float("nan")
+    # decays from 0.01 on, at gates whose mean over 200 steps is above 0.45
+    check_recurrence(x, ig, rg, decays(kind, d), rnd(6, b, d), ln, dout, rnd(7, b, d), 222)
+
+
+def test_recurrence_extreme_gates_have_gradients():
+    """Shut and open gates and a decay that forgets at once: where the root is not 0 the
+    gradients are the formula's, where it is 0 (a = 1) the gradient through it is 0."""
+    n = 40
+    x, dout = rnd(1, 1, n, 6), rnd(3, 1, n, 6)
+    ig = torch.zeros(1, n, 6, device="cuda")
+    rg = torch.tensor([-20.0, 0.0, 20.0, 0.0, -200.0, 0.0], device="cuda").expand(1, n, 6).contiguous()
+    decay = torch.tensor([1.0, 200.0, 1.0, 80.0, 1.0, 0.0], device="cuda")
+    h = rnd(2, 1, 6)
+    r = sq.gated_recurrence(x, ig, rg, decay, initial_state=h, save_states=True)
+    g = sq.gated_recurrence_backward(dout, x, ig, rg, decay, r.states)
+    wide = [v[..., :4].double().requires_grad_() for v in (x, ig, rg, decay, h)]
+    out, _ = ref_recurrence(*wide, None)
+    want = torch.autograd.grad((out * dout[..., :4].double()).sum(), wide)
+    # sigmoid(-20)'s exponential: its argument's rounding is 20 units more; the root of
+    # its 1 - a^2 divides what the state's gradients, sums of n terms, are off by
+    c = 4 * (20 + 20 + 10 * n) * EPS
+    for v, w, what in zip(g, want, g._fields):
+        err, size = (v[..., :4].double() - w).abs(), w.abs()
+        assert (err.flatten(0, -2).amax(0) <= c * size.flatten(0, -2).amax(0).clamp(min=1e-30)).all() \
+            if what != "ddecay" else (err <= c * size + c).all(), what
+    # a = 1: nothing goes in, the state's gradient passes on as it is
+    back = dout[0, :, 4:].double().flip(0).cumsum(0).flip(0)
+    assert not g.dx[..., 4:].any() and not g.dinput_gate[..., 4:].any() and not g.drecurrence_gate[..., 4:].any()
+    within(g.dinitial_state[:, 4:], back[:1], n * EPS * dout.double().abs().sum(1)[:, 4:])
+    # ddecay = -sum r h G: r is 0, or 1/2 of a state that stands still
+    assert g.ddecay[4].item() == 0
+    term = back[:, 1] * h[0, 5].double() / 2
+    assert abs(g.ddecay[5].item() + term.sum().item()) <= 2 * n * EPS * term.abs().sum().item()
