@@ -174,6 +174,9 @@ __device__ __forceinline__ void exchange(Exchange<VL>& x, int parity, int warp, 
   }
   block_sync();
   const int at = back ? warps - 1 - warp : warp;         // place in the walk
+  float start[VL];
+#pragma unroll
+  for (int e = 0; e < VL; ++e) start[e] = carry[e];
   if (size > 1) {
     if (warp < VL) {          // warp e sums up the block for its 32 channels
       const int c = lane + 32 * warp;
@@ -183,6 +186,14 @@ __device__ __forceinline__ void exchange(Exchange<VL>& x, int parity, int warp, 
         const float2 m = x.warp[parity][w][c];
         sum += x.log_a[w][c];
         q2 = Factor{m.x}.step(q2, m.y);
+      }
+      if (isnan(q2)) {
+        q2 = 0.f;
+#pragma unroll 1
+        for (int i = 0; i < warps; ++i) {
+          const float2 m = x.warp[parity][back ? warps - 1 - i : i][c];
+          q2 = Factor{m.x}.step<true>(q2, m.y);
+        }
       }
       const float2 m = make_float2(factor_of(sum).code, q2);
       for (uint32_t r = 0; r < size; ++r) store_at_rank(&x.block[parity][rank][c], r, m);
@@ -209,6 +220,24 @@ __device__ __forceinline__ void exchange(Exchange<VL>& x, int parity, int warp, 
         const float2 m = x.warp[parity][back ? warps - 1 - i : i][lane + 32 * e];
         carry[e] = Factor{m.x}.step(carry[e], m.y);
       }
+    }
+  }
+  // Walks that keep infinities cost more: only where these ended in NaN.
+#pragma unroll
+  for (int e = 0; e < VL; ++e) {
+    if (!isnan(carry[e]) && !isnan(h[e])) continue;
+    carry[e] = start[e];
+#pragma unroll 1
+    for (int i = 0; i < (int)(size > 1 ? size : warps); ++i) {
+      const int r = back ? (int)(size > 1 ? size : warps) - 1 - i : i;
+      if (size > 1 ? r == (int)rank : i == at) h[e] = carry[e];
+      const float2 m = size > 1 ? x.block[parity][r][lane + 32 * e] : x.warp[parity][r][lane + 32 * e];
+      carry[e] = Factor{m.x}.step<true>(carry[e], m.y);
+    }
+#pragma unroll 1
+    for (int i = 0; size > 1 && i < at; ++i) {
+      const float2 m = x.warp[parity][back ? warps - 1 - i : i][lane + 32 * e];
+      h[e] = Factor{m.x}.step<true>(h[e], m.y);
     }
   }
 }
@@ -291,6 +320,14 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 2) recurrence_fwd_kernel(RecAr
       }
 #pragma unroll
       for (int e = 0; e < VL; ++e) {
+        if (isnan(q[e])) {              // (as in exchange())
+          q[e] = 0.f;
+#pragma unroll
+          for (int j = 0; j < kSteps; ++j) q[e] = step_on<SHORT, true>(a[j][e], q[e], in[j][e]);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < VL; ++e) {
         sum[e] *= -decay[e];
         all[e] = factor_of(sum[e]);
       }
@@ -303,20 +340,30 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 2) recurrence_fwd_kernel(RecAr
           if (c < channels) p.saved[(b * saves + t0 / kSteps) * p.channels + d0 + c] = h[e];
         }
       }
-      T* po = p.out.at(b, t0) + d0;
       const int rows = p.length - t0 < kSteps ? (int)(p.length - t0) : kSteps;
+      float start[VL];
 #pragma unroll
-      for (int j = 0; j < kSteps; ++j) {
-        if (!SHORT && j >= rows) break;
-        float o[VL];
+      for (int e = 0; e < VL; ++e) start[e] = h[e];
+      auto show = [&](auto any) {
+        T* po = p.out.at(b, t0) + d0;
 #pragma unroll
-        for (int e = 0; e < VL; ++e) {
-          h[e] = step_on<SHORT>(a[j][e], h[e], in[j][e]);
-          o[e] = SHORT || j < n ? h[e] : 0.f;
+        for (int j = 0; j < kSteps; ++j) {
+          if (!SHORT && j >= rows) break;
+          float o[VL];
+#pragma unroll
+          for (int e = 0; e < VL; ++e) {
+            h[e] = step_on<SHORT, any.value>(a[j][e], h[e], in[j][e]);
+            o[e] = SHORT || j < n ? h[e] : 0.f;
+          }
+          S::store(po, lane, channels, o);
+          po += p.out.st;
         }
-        S::store(po, lane, channels, o);
-        po += p.out.st;
-      }
+      };
+      show(std::false_type());
+      bool lost = false;
+#pragma unroll
+      for (int e = 0; e < VL; ++e) lost = lost || isnan(h[e]), h[e] = start[e];
+      if (lost) show(std::true_type());
     };
     // Behind the sequence's end the state stands still (8 sequences of 0 to 2048 steps x
     // 4096 bf16: 187 us where warps walk their padding, 121 where they do not; the
@@ -510,7 +557,7 @@ __global__ void __launch_bounds__(kStepThreads) recurrence_step_kernel(RecArrays
   for (int e = 0; e < VL; ++e) {
     float w;
     const Factor a = factor_of(-decay[e] * sigmoid_f(rg[e]), &w);
-    h[e] = a.step(h[e], root_of(w) * (sigmoid_f(ig[e]) * x[e]));
+    h[e] = a.step<true>(h[e], root_of(w) * (sigmoid_f(ig[e]) * x[e]));
   }
   store_vec<T, VL>(p.out.at(b, 0) + d, h);
   store_vec<float, VL>(p.final + b * p.channels + d, h);

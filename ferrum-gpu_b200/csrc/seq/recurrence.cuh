@@ -33,9 +33,11 @@ struct Factor {
     return __float_as_int(code) < 0 ? 1.f + code : code;
   }
   __device__ __forceinline__ float times(float h) const { return fmaf(code, h, rest(h)); }
-  // a h + b, the sum of the small terms first
+  // a h + b, the sum of the small terms first. An infinite h comes out as NaN, which
+  // stays NaN in all steps to come; ANY keeps it infinite, as a > 0 does.
+  template <bool ANY = false>
   __device__ __forceinline__ float step(float h, float b) const {
-    return fmaf(code, h, b) + rest(h);
+    return ANY && fabsf(h) == INFINITY ? h + b : fmaf(code, h, b) + rest(h);
   }
 };
 constexpr float kKeep = -0.f;                   // the code of a = 1
@@ -110,9 +112,10 @@ template <bool SHORT>
 __device__ __forceinline__ float step_times(Factor a, float h) {
   return SHORT ? fmaf(a.code, h, h) : a.times(h);
 }
-template <bool SHORT>
+template <bool SHORT, bool ANY = false>
 __device__ __forceinline__ float step_on(Factor a, float h, float b) {
-  return SHORT ? fmaf(a.code, h, b) + h : a.step(h, b);
+  if (SHORT) return ANY && fabsf(h) == INFINITY ? h + b : fmaf(a.code, h, b) + h;
+  return a.step<ANY>(h, b);
 }
 
 }  // namespace seq

@@ -344,11 +344,11 @@ def gated_recurrence(x, input_gate, recurrence_gate, decay, *, initial_state=Non
         h = a h + sqrt(1 - a^2) sigmoid(input_gate) x,   out = h
 
     x, input_gate, recurrence_gate: (batch, length, channels). decay:
-    (channels), not negative: a channel forgets at most by exp(-decay) a step.
-    initial_state: (batch, channels) float32. With ``save_states`` the result
-    carries what the backward needs. Where 1 - a^2 is not above 0, the root and
-    the gradient through it are 0. A state that is infinite is NaN a step later (h
-    moves by (a - 1) h where a is close to 1).
+    (channels), not negative: a channel
+    forgets at most by exp(-decay) a step. initial_state: (batch, channels)
+    float32. With ``save_states`` the result carries what the backward needs.
+    Where 1 - a^2 is not above 0 (or below 2^-126), the root and the gradient
+    through it are 0. An infinite state stays infinite.
     """
     return RecurrenceResult(*_call(
         _sequence.gated_recurrence, x, input_gate, recurrence_gate, decay, initial_state, lengths,
@@ -359,7 +359,8 @@ def gated_recurrence_backward(dout, x, input_gate, recurrence_gate, decay, state
                               dfinal_state=None, device=None, stream=None) -> RecurrenceGrads:
     """Gradients of ``gated_recurrence`` for its output's gradient ``dout`` (and
     that of its final state). ``states`` comes from the forward call with
-    ``save_states``."""
+    ``save_states``. Gradients that an infinite state or an infinite ``dout`` reaches
+    are not finite: infinite or NaN."""
     return RecurrenceGrads(*_call(
         _sequence.gated_recurrence_backward, dout, x, input_gate, recurrence_gate, decay, states,
         lengths, dfinal_state, device, stream))

@@ -155,3 +155,50 @@ def test_recurrence_extreme_gates_have_gradients():
     assert g.ddecay[4].item() == 0
     term = back[:, 1] * h[0, 5].double() / 2
     assert abs(g.ddecay[5].item() + term.sum().item()) <= 2 * n * EPS * term.abs().sum().item()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("b,n,d", [(2, 1, 8), (3, 1300, 96), (7, 300, 130), (80, 90, 64)])
+def test_a_recurrence_keeps_infinities(b, n, d, dtype):
+    """a > 0, so an infinite state stays infinite, whatever the factors and however they
+    are joined; only infinities of both signs make NaN. Other channels do not see it."""
+    x, ig, rg = (rnd(k, b, n, d, dtype=dtype) for k in range(3))
+    decay, h = decays("mixed", d), rnd(6, b, d)
+    ln = lengths_of(b, n, "mixed")
+    plain = sq.gated_recurrence(x, ig, rg, decay, initial_state=h, lengths=ln, save_states=True)
+    inf, t = float("inf"), n // 3
+    x2, h2 = x.clone(), h.clone()
+    h2[:, 0], h2[:, 3], h2[:, 6] = inf, -inf, inf
+    x2[:, t, 1], x2[:, t, 2] = inf, -inf
+    x2[:, n // 2, 6] = -inf
+    r = sq.gated_recurrence(x2, ig, rg, decay, initial_state=h2, lengths=ln, save_states=True)
+    out, fin = ref_recurrence(*(v.double() for v in (x2, ig, rg, decay, h2)), ln)
+    hit = [0, 1, 2, 3, 6]
+    rest = [c for c in range(d) if c not in hit]
+    for got, want in ((r.out, out), (r.final_state, fin)):
+        off = ~torch.isfinite(want)
+        assert torch.equal(got[off].double().nan_to_num(7.0, 8.0, 9.0), want[off].nan_to_num(7.0, 8.0, 9.0))
+        within(got[~off], want[~off], (20 + 10 * min(n, 222)) * EPS * h.abs().max().clamp(min=out[~torch.isinf(out)].nan_to_num().abs().max()).item())
+    for u, v in ((r.out, plain.out), (r.final_state, plain.final_state), (r.states, plain.states)):
+        assert torch.equal(u[..., rest], v[..., rest])
+    # token by token
+    step = [v[:, 0].contiguous() for v in (x2, ig, rg)]
+    want, _ = ref_recurrence(*(v[:, None].double() for v in step), decay.double(), h2.double(), None)
+    y = sq.gated_recurrence_step(*step, decay, h2)
+    for got in (y, h2):
+        assert torch.equal(torch.isfinite(got), torch.isfinite(want[:, 0]))
+        off = torch.isinf(want[:, 0])
+        assert torch.equal(got[off].double(), want[:, 0][off])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_gradient_behind_the_end_passes_on_as_it_is(dtype):
+    """The final state's gradient is the initial one's where a sequence has no step."""
+    b, n, d = 5, 400, 40
+    x, ig, rg, dout = (rnd(k, b, n, d, dtype=dtype) for k in range(4))
+    decay, dfin = rnd(5, d).abs(), rnd(7, b, d)
+    dfin[:, 3], dfin[:, 5] = float("inf"), -float("inf")
+    ln = torch.zeros(b, dtype=torch.int32, device="cuda")
+    s = sq.gated_recurrence(x, ig, rg, decay, lengths=ln, save_states=True).states
+    g = sq.gated_recurrence_backward(dout, x, ig, rg, decay, s, lengths=ln, dfinal_state=dfin)
+    assert torch.equal(g.dinitial_state, dfin)
