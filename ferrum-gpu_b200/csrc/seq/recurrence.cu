@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 2) recurrence_fwd_kernel(RecAr
 #pragma unroll
   for (int e = 0; e < VL; ++e) {
     const int c = S::channel(lane, e);
-    decay[e] = c < channels ? p.decay[d0 + c] : 0.f;
+    decay[e] = c < channels ? checked_decay(p.decay[d0 + c]) : 0.f;
     carry[e] = c < channels && p.initial ? p.initial[b * p.channels + d0 + c] : 0.f;
   }
   bool mild = true;
@@ -419,7 +419,7 @@ __global__ void __launch_bounds__(32 * WARPS, WARPS == 8 ? 2 : 3) recurrence_bwd
   const int64_t chunk = (int64_t)size * warps * kSteps, turns = (p.length + chunk - 1) / chunk;
   const int64_t saves = (p.length + kSteps - 1) / kSteps;
   int64_t t0 = (turns - 1) * chunk + ((int64_t)rank * warps + warp) * kSteps;
-  const float decay = mine ? p.decay[d0 + lane] : 0.f;
+  const float decay = mine ? checked_decay(p.decay[d0 + lane]) : 0.f;
   const bool mild = __all_sync(0xffffffffu, decay >= 0.f && decay <= kShortDecay);
   float carry[1] = {mine && p.dfinal ? p.dfinal[at] : 0.f}, total = 0.f;
   auto valid = [&](int64_t t) {
@@ -556,7 +556,7 @@ __global__ void __launch_bounds__(kStepThreads) recurrence_step_kernel(RecArrays
 #pragma unroll
   for (int e = 0; e < VL; ++e) {
     float w;
-    const Factor a = factor_of(-decay[e] * sigmoid_f(rg[e]), &w);
+    const Factor a = factor_of(-checked_decay(decay[e]) * sigmoid_f(rg[e]), &w);
     h[e] = a.step<true>(h[e], root_of(w) * (sigmoid_f(ig[e]) * x[e]));
   }
   store_vec<T, VL>(p.out.at(b, 0) + d, h);

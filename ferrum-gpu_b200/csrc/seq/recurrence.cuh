@@ -42,15 +42,17 @@ struct Factor {
 };
 constexpr float kKeep = -0.f;                   // the code of a = 1
 
-// e^x for x <= 88: x = k ln 2 + r with |r| <= ln 2 / 2; (e^r - 1 - r) / r^2 by a
+// A negative decay has no root: NaN.
+__device__ __forceinline__ float checked_decay(float decay) { return decay < 0.f ? NAN : decay; }
+
+// e^x for x <= 0: x = k ln 2 + r with |r| <= ln 2 / 2; (e^r - 1 - r) / r^2 by a
 // polynomial of degree 4, fitted for the relative error of e^r - 1 (largest 0.23
 // units of 2^-24). One rounded ln 2 is enough: k of it shifts e^r by k 2e-9, of an
 // a that is 2^k. Below -87 the factor is 0; NaN stays NaN.
-// `w`: 1 - a^2 with its relative accuracy, not below 0.
+// `w`: 1 - a^2 with its relative accuracy.
 __device__ __forceinline__ Factor factor_of(float x, float* w = nullptr) {
   const float magic = 12582912.f;                    // 1.5 * 2^23: rounds to an integer
-  float v = x < -87.f ? -87.f : x;
-  v = v > 88.f ? 88.f : v;
+  const float v = x < -87.f ? -87.f : x;
   const float kf = fmaf(v, kLog2e, magic);
   const float k = kf - magic;
   const float two_k = __int_as_float((__float_as_int(kf) << 23) + 0x3f800000);
@@ -62,11 +64,8 @@ __device__ __forceinline__ Factor factor_of(float x, float* w = nullptr) {
   p = fmaf(p, r, 0.5f);
   const float q = fmaf(r * r, p, r);                 // e^r - 1
   const float a = x < -87.f ? 0.f : fmaf(two_k, q, two_k);
-  const bool near = k == 0.f && v <= 0.f;
-  if (w) {
-    const float far = fmaf(-a, a, 1.f);      // (below 0 where the state grows)
-    *w = near ? -q * (2.f + q) : (far < 0.f ? 0.f : far);
-  }
+  const bool near = k == 0.f;
+  if (w) *w = near ? -q * (2.f + q) : fmaf(-a, a, 1.f);
   return {near ? -fabsf(q) : a};
 }
 

@@ -344,7 +344,7 @@ def gated_recurrence(x, input_gate, recurrence_gate, decay, *, initial_state=Non
         h = a h + sqrt(1 - a^2) sigmoid(input_gate) x,   out = h
 
     x, input_gate, recurrence_gate: (batch, length, channels). decay:
-    (channels), not negative: a channel
+    (channels), not negative (a negative one makes its channel NaN): a channel
     forgets at most by exp(-decay) a step. initial_state: (batch, channels)
     float32. With ``save_states`` the result carries what the backward needs.
     Where 1 - a^2 is not above 0 (or below 2^-126), the root and the gradient

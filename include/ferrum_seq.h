@@ -203,7 +203,7 @@ ferrum_status ferrum_long_conv_step(ferrum_device *dev, const ferrum_long_conv_a
  * Gated linear recurrence, one state per channel:
  *   a = exp(-decay[d] * sigmoid(recurrence_gate[b,t,d]))
  *   h = a * h + sqrt(1 - a^2) * sigmoid(input_gate[b,t,d]) * x[b,t,d];  out = h
- * decay is not negative; where 1 - a^2 is
+ * decay is not negative (a negative one makes its channel NaN); where 1 - a^2 is
  * not above 0 (or below 2^-126), the root and the gradient through it are 0. An
  * infinite state stays infinite; gradients that it or an infinite dout reaches are
  * infinite or NaN.

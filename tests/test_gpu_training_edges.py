@@ -202,3 +202,28 @@ def test_a_gradient_behind_the_end_passes_on_as_it_is(dtype):
     s = sq.gated_recurrence(x, ig, rg, decay, lengths=ln, save_states=True).states
     g = sq.gated_recurrence_backward(dout, x, ig, rg, decay, s, lengths=ln, dfinal_state=dfin)
     assert torch.equal(g.dinitial_state, dfin)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_negative_decay_is_nan(dtype):
+    """sqrt(1 - a^2) of a factor above 1 does not exist: its channel is NaN, no other."""
+    b, n, d = 3, 100, 40
+    x, ig, rg, dout = (rnd(k, b, n, d, dtype=dtype) for k in range(4))
+    decay, h = rnd(5, d).abs() + 0.01, rnd(6, b, d)
+    bad = decay.clone()
+    bad[7], bad[20] = -0.5, -float("inf")
+    ln = torch.tensor([n, 40, 0], dtype=torch.int32, device="cuda")
+    r = [sq.gated_recurrence(x, ig, rg, v, initial_state=h, lengths=ln, save_states=True) for v in (decay, bad)]
+    g = [sq.gated_recurrence_backward(dout, x, ig, rg, v, q.states, lengths=ln) for v, q in zip((decay, bad), r)]
+    rest = [c for c in range(d) if c not in (7, 20)]
+    for u, v in zip((*r[0], *g[0]), (*r[1], *g[1])):
+        within(v[..., rest], u[..., rest].double(), 2 * (20 + 10 * n) * EPS * u.abs().max().item())
+    for c in (7, 20):
+        for v in (r[1].out, g[1].dx, g[1].dinput_gate, g[1].drecurrence_gate):
+            assert torch.isnan(v[0, :, c]).all() and torch.isnan(v[1, :40, c]).all()
+            assert not v[1, 40:, c].any() and not v[2, :, c].any()
+        assert torch.isnan(r[1].final_state[:2, c]).all() and r[1].final_state[2, c] == h[2, c]
+        assert torch.isnan(g[1].ddecay[c])
+    step = [v[:, 0].contiguous() for v in (x, ig, rg)]
+    y = sq.gated_recurrence_step(*step, bad, h.clone())
+    assert torch.isnan(y).any(0).tolist() == [c in (7, 20) for c in range(d)]
