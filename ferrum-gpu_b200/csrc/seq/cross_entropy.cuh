@@ -29,14 +29,23 @@ __device__ __forceinline__ RowStat join(RowStat a, RowStat b) {
   return r;
 }
 
+// |value| from which on its multiple by log2 e may leave float32's range: the difference is
+// taken first then.
+constexpr float kFar = 2e38f;
+
 __device__ __forceinline__ float lse_of(RowStat r) { return shift_of(r.top) + logf(r.sum); }
 
 // What a row needs to turn its logits into G: scaled gradients of its logits'
-// sum and of its loss, lse in units of ln 2, and its target (-1 without a loss).
+// sum and of its loss, lse, and its target (-1 without a loss).
 struct RowCoef {
-  float all, one, lse2;
+  float all, one, lse;
   int target;
 };
+// softmax = 2^(logit scale - lse scale). Where lse is finite and beyond kFar, logits are 2^104
+// and more apart, or equal: any scale serves that keeps the products finite.
+__device__ __forceinline__ float softmax_scale(float lse) {
+  return fabsf(lse) > kFar && fabsf(lse) < INFINITY ? 0x1p-30f : kLog2e;
+}
 
 // Lets the stream's next kernel start (where its launch allows that), and waits for
 // the end of the one in front (at once where this launch did not).
@@ -182,7 +191,7 @@ prepare_kernel(const T* __restrict__ x, int64_t x_ld, int64_t width, T* __restri
     place[threadIdx.x] = counts_for ? mine : -1;
     if (counts_for) {
       const float one = dloss ? dloss[t] : 0.f, all = one + (dlse ? dlse[t] : 0.f);
-      live.rows[mine] = {all * up, one * up, lse[t] * kLog2e, (int)at};
+      live.rows[mine] = {all * up, one * up, lse[t], (int)at};
       live.index[mine] = (int)t;
     }
     __syncthreads();

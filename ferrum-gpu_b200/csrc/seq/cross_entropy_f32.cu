@@ -190,10 +190,11 @@ __global__ void __launch_bounds__(kThreads, 2) loss_f32_kernel(const __grid_cons
       }
 #pragma unroll
       for (int o = 8; o > 0; o /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const float k = shift_of(top) * kLog2e;
+      const float shift = shift_of(top), k = shift * kLog2e;
       float sum = 0.f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sum += ex2(fmaf(v[j], kLog2e, -k));
+      for (int j = 0; j < 8; ++j)
+        sum += ex2(fabsf(shift) > kFar ? (v[j] - shift) * kLog2e : fmaf(v[j], kLog2e, -k));
 #pragma unroll
       for (int o = 8; o > 0; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       if (row && tx == 0) w.stats[n0 / kTile * p.a.rows + m] = {top, sum};
@@ -204,9 +205,10 @@ __global__ void __launch_bounds__(kThreads, 2) loss_f32_kernel(const __grid_cons
     if constexpr (KIND == kGrads) {
       const RowCoef q = w.live.rows[m];
       const int64_t at = (int64_t)q.target - w.first;
+      const float scale = softmax_scale(q.lse), lse = q.lse * scale;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float g = ex2(fmaf(v[j], kLog2e, -q.lse2)) * q.all - (column(j) == at ? q.one : 0.f);
+        const float g = ex2(fmaf(v[j], scale, -lse)) * q.all - (column(j) == at ? q.one : 0.f);
         v[j] = q.target < 0 ? 0.f : g;
       }
     } else {

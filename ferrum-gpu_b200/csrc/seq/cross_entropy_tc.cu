@@ -239,6 +239,11 @@ __device__ void finish_stats(const Work& w, uint32_t acc, const RowCoef& row, in
   const float k = shift_of(s.top) * kLog2e;
 #pragma unroll
   for (int i = 0; i < kHalf; ++i) s4[i % 4] += ex2(fmaf(v[i / 32][i % 32], kLog2e, -k));
+  if (fabsf(s.top) > kFar && fabsf(s.top) < INFINITY) {
+    s4[0] = s4[1] = s4[2] = s4[3] = 0.f;
+#pragma unroll
+    for (int i = 0; i < kHalf; ++i) s4[i % 4] += ex2((v[i / 32][i % 32] - s.top) * kLog2e);
+  }
   s.sum = (s4[0] + s4[1]) + (s4[2] + s4[3]);
   if (m >= p.m) return;
   w.stats[n0 / kHalf * p.m + m] = s;
@@ -297,6 +302,7 @@ __device__ void finish_grads(const Work& w, const CUtensorMap* map, uint8_t* slo
   // (a target in front of the piece is below 0, whatever is taken from it)
   const int64_t at64 = (int64_t)q.target - w.first - n0;
   const int at = q.target >= 0 && at64 >= 0 && at64 < kHalf ? (int)at64 : -1;
+  const float scale = softmax_scale(q.lse), lse = q.lse * scale;
   if (n0 >= p.n) release();
 #pragma unroll 1
   for (int c = 0; c < kHalf; c += 64) {
@@ -310,7 +316,7 @@ __device__ void finish_grads(const Work& w, const CUtensorMap* map, uint8_t* slo
     for (int h = 0; h < 2; ++h) {
 #pragma unroll
       for (int i = 0; i < 32; ++i)
-        v[h][i] = q.target < 0 ? 0.f : ex2(fmaf(v[h][i], kLog2e, -q.lse2)) * q.all;
+        v[h][i] = q.target < 0 ? 0.f : ex2(fmaf(v[h][i], scale, -lse)) * q.all;
       if (at >= c + h * 32 && at < c + h * 32 + 32) {
 #pragma unroll
         for (int i = 0; i < 32; ++i) v[h][i] -= at - c - h * 32 == i ? q.one : 0.f;
@@ -568,7 +574,8 @@ struct FewShared {
   uint64_t full[FewShape<NT>::kCount], empty[FewShape<NT>::kCount], done[2], drained[2];
   uint32_t tmem;
   int dead;
-  RowCoef rows[NT];
+  RowCoef rows[NT];          // (lse times `scale`)
+  float scale[NT];
   RowStat stats[kFewEpilogueWarps][NT];
 };
 
@@ -617,7 +624,9 @@ loss_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
         if (has_loss(at, w.vocab)) q.target = (int)at;
       }
     }
-    sh.rows[threadIdx.x] = q;
+    const float scale = softmax_scale(q.lse);
+    q.lse *= scale;
+    sh.rows[threadIdx.x] = q, sh.scale[threadIdx.x] = scale;
   }
   tc_fence_before();
   __syncthreads();
@@ -697,7 +706,7 @@ loss_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
             const RowCoef q = sh.rows[c * 32 + i];
-            const float g = ex2(fmaf(v[i], kLog2e, -q.lse2)) * q.all - (q.target == word ? q.one : 0.f);
+            const float g = ex2(fmaf(v[i], sh.scale[c * 32 + i], -q.lse)) * q.all - (q.target == word ? q.one : 0.f);
             v[i] = q.target < 0 ? 0.f : g;
           }
           if (mine) {
@@ -728,10 +737,15 @@ loss_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
 #pragma unroll
           for (int i = 0; i < 32; ++i) m[i] = v[i];
           const float top = spread(m, lane, [](float a, float b) { return fmaxf(a, b); });
-          const float shift = shift_of(top) * kLog2e;
+          const float shift = shift_of(top), shift2 = shift * kLog2e;
+          if (__any_sync(0xffffffffu, fabsf(shift) > kFar)) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            v[i] = ex2(fmaf(v[i], kLog2e, -__shfl_sync(0xffffffffu, shift, i)));
+            for (int i = 0; i < 32; ++i) v[i] = ex2((v[i] - __shfl_sync(0xffffffffu, shift, i)) * kLog2e);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              v[i] = ex2(fmaf(v[i], kLog2e, -__shfl_sync(0xffffffffu, shift2, i)));
+          }
           const float sum = spread(v, lane, [](float a, float b) { return a + b; });
           run[c] = join(run[c], {top, sum});
         }

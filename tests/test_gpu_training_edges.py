@@ -227,3 +227,45 @@ def test_a_negative_decay_is_nan(dtype):
     step = [v[:, 0].contiguous() for v in (x, ig, rg)]
     y = sq.gated_recurrence_step(*step, bad, h.clone())
     assert torch.isnan(y).any(0).tolist() == [c in (7, 20) for c in range(d)]
+
+
+# ---------------------------------------------------------------- logits near float32's ends
+
+@pytest.mark.parametrize("dtype", [F32, torch.bfloat16])
+@pytest.mark.parametrize("tokens", [3, 40, 300])
+def test_loss_of_logits_near_the_largest(tokens, dtype):
+    """Logits of 3e38 are finite, their multiples by log2 e are not. A row's lse is its
+    largest logit then (its spacing in float32 is 2^104), the softmax 1 there."""
+    big = 2.0 ** 64
+    x = torch.zeros(tokens, 16, device="cuda", dtype=dtype)
+    w = torch.zeros(700, 16, device="cuda", dtype=dtype)
+    kind = torch.arange(tokens, device="cuda") % 3
+    t = (torch.arange(tokens, device="cuda") * 37 + 1) % 700
+    x[kind == 0, 0] = big            # word 5 is far above all others
+    w[5, 0] = 0.75 * big
+    x[kind == 1, 1] = big            # all words near the lowest, word 9 a little less so
+    w[:, 1] = -0.875 * big
+    w[9, 1] = -0.75 * big
+    x[kind == 2, 2] = 1.0            # an ordinary row among them
+    w[:, 2] = torch.arange(700, device="cuda").to(dtype) / 256
+    logits = x.double() @ w.double().t()
+    lse = torch.logsumexp(logits, 1)
+    at = torch.arange(tokens, device="cuda")
+    loss = lse - logits[at, t]
+    for targets in (t, logits.argmax(1)):
+        loss = lse - logits[at, targets]
+        r = sq.linear_cross_entropy(x, w, targets)
+        within(r.lse, lse, 32 * EPS * lse.abs(), "lse")
+        within(r.loss, loss, 64 * EPS * (1 + lse.abs()) * (kind == 2).double(), "loss")
+        d = torch.ones(tokens, device="cuda")
+        g = sq.linear_cross_entropy_backward(d, x, w, targets, r.lse)
+        p = torch.softmax(logits, 1)
+        size = p.clone()
+        size[at, targets] += 1
+        p[at, targets] -= 1
+        # G is rounded to 16 bits for 16-bit types, its exponentials' arguments to lse's spacing
+        u = U[dtype] + 64 * EPS * (1 + logits.abs().amax(1)[kind == 2].max())
+        err = u * size + 2.0 ** -126
+        for got, ref, e in ((g.dx, p @ w.double(), err @ w.double().abs()),
+                            (g.dweight, p.t() @ x.double(), err.t() @ x.double().abs())):
+            within(got, ref, 2 * e)
