@@ -6,9 +6,11 @@
 // are few tiles or tokens), 8 x 8 a thread, two values of a row at a time
 // (fma.rn.f32x2), from steps of 16 that it copies to shared memory through registers a
 // step ahead. 64 multiply-adds a thread take 4 reads of 16 bytes: bound by the FMA
-// pipe (72 TFLOP/s). The depth of dx, the vocabulary, is split so that
-// there are tiles for all SMs; its slabs are added in order, which also halves the
-// error of one long sum. 4096 x 1024 x 4096: 51 TFLOP/s forward, 46 for the gradient.
+// pipe (72 TFLOP/s). The depths of dx, the vocabulary, and of dW, the tokens, are split so
+// that there are tiles for all SMs; slabs are added in order. No sum is a chain of more
+// than 1024 terms (of one as long as a row is wide where logits are made). 4096 x 1024 x
+// 4096: 682 us forward (50 TFLOP/s), 2350 for the gradient (44); 16384 x 64 x 256: its
+// gradient 114 us, 1125 with dW's depth in one piece.
 #include <algorithm>
 
 #include "cross_entropy.cuh"
@@ -18,6 +20,10 @@ namespace seq {
 namespace {
 
 constexpr int kTile = 128, kStep = 16, kThreads = 256;
+// Depth after which the weights' products put their sums down and begin anew: a sum of n terms
+// of either sign, one after the other, is off by about 0.4 sqrt(n / 2) units of 2^-24 (dW of
+// 65536 x 64 x 256: 3.9e-6 in one chain, the plain form 4.1e-7).
+constexpr int kChain = 1024;
 
 enum Kind { kStats, kGrads, kWeights };
 
@@ -34,7 +40,7 @@ struct Product {
   float* out;                // sums: slabs of a.rows rows
   int64_t ld;
   bool sums, load;           // onto those of earlier pieces
-  bool live_rows, live_depth;  // of A; the number of tokens with a loss
+  bool live_rows, live_depth;  // of A; the number of tokens with a loss, shared out to the splits
 };
 struct Work {
   Product p[2];
@@ -114,6 +120,11 @@ struct Piece {
   }
 };
 
+// Tokens of each split of a product whose depth they are; splits behind the last have none.
+__host__ __device__ inline int64_t live_each(int64_t live, int splits) {
+  return ((live + kStep - 1) / kStep + splits - 1) / splits * kStep;
+}
+
 template <int KIND, int ROWS>
 __global__ void __launch_bounds__(kThreads, 2) loss_f32_kernel(const __grid_constant__ Work w) {
   constexpr int kMine = ROWS / 16;        // rows of a thread
@@ -131,9 +142,10 @@ __global__ void __launch_bounds__(kThreads, 2) loss_f32_kernel(const __grid_cons
   Operand oa = p.a;
   if (p.live_rows) oa.rows = live;
   if (m0 >= oa.rows) return;
-  const int64_t k0 = split * p.depth_per_split;
-  const int depth = p.live_depth ? live
-                                 : (int)(p.depth - k0 < p.depth_per_split ? p.depth - k0 : p.depth_per_split);
+  const int64_t each = p.live_depth ? live_each(live, p.splits) : p.depth_per_split;
+  const int64_t k0 = split * each, left = (p.live_depth ? live : p.depth) - k0;
+  const int depth = (int)(left < each ? left : each);
+  if (depth <= 0) return;
   const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
   float2 acc[kMine][4];
 #pragma unroll
@@ -145,92 +157,125 @@ __global__ void __launch_bounds__(kThreads, 2) loss_f32_kernel(const __grid_cons
   a.load(depth), b.load(depth);
   a.store(sa[0]), b.store(sb[0]);
   __syncthreads();
-  int buf = 0;
+  int buf = 0, k = kStep, done = 0;
+  do {                       // (a chain of sums; one alone but in kWeights)
+    const int stop = KIND != kWeights || depth - done <= kChain ? depth : done + kChain;
 #pragma unroll 1
-  for (int k = kStep; k < depth + kStep; k += kStep, buf ^= 1) {
-    const bool more = k < depth;
-    if (more) a.load(depth - k), b.load(depth - k);
+    for (; k < stop + kStep; k += kStep, buf ^= 1) {
+      const bool more = k < depth;
+      if (more) a.load(depth - k), b.load(depth - k);
 #pragma unroll
-    for (int q = 0; q < kStep; ++q) {
-      float x[kMine];
-      float2 y[4];
-      if constexpr (kMine == 2) {
-        *(float2*)&x[0] = *(const float2*)&sa[buf][q][ty * 2];
-      } else {
-        *(float4*)&x[0] = *(const float4*)&sa[buf][q][ty * 4];
-        if constexpr (kMine == 8) *(float4*)&x[4] = *(const float4*)&sa[buf][q][64 + ty * 4];
+      for (int q = 0; q < kStep; ++q) {
+        float x[kMine];
+        float2 y[4];
+        if constexpr (kMine == 2) {
+          *(float2*)&x[0] = *(const float2*)&sa[buf][q][ty * 2];
+        } else {
+          *(float4*)&x[0] = *(const float4*)&sa[buf][q][ty * 4];
+          if constexpr (kMine == 8) *(float4*)&x[4] = *(const float4*)&sa[buf][q][64 + ty * 4];
+        }
+        *(float4*)&y[0] = *(const float4*)&sb[buf][q][tx * 4];
+        *(float4*)&y[2] = *(const float4*)&sb[buf][q][64 + tx * 4];
+#pragma unroll
+        for (int i = 0; i < kMine; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) fma2(acc[i][j], make_float2(x[i], x[i]), y[j]);
       }
-      *(float4*)&y[0] = *(const float4*)&sb[buf][q][tx * 4];
-      *(float4*)&y[2] = *(const float4*)&sb[buf][q][64 + tx * 4];
+      if (more) a.store(sa[buf ^ 1]), b.store(sb[buf ^ 1]);
+      __syncthreads();
+    }
+    // of a row's values, j < 4 are columns n0 + tx * 4 + j, the others 64 further
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int64_t m = m0 + (kMine == 2 ? ty * 2 + i : i / 4 * 64 + ty * 4 + i % 4);
+      const bool row = m < oa.rows;
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = j % 2 ? acc[i][j / 2].y : acc[i][j / 2].x;
+      auto column = [&](int j) { return n0 + j / 4 * 64 + tx * 4 + j % 4; };
+      if constexpr (KIND == kStats) {
+        const int64_t target = row ? w.targets[m] : -1;
+        float top = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (column(j) >= p.b.rows) v[j] = -INFINITY;
+          else if (column(j) == target) w.at_target[m] = v[j];
+          top = fmaxf(top, v[j]);
+        }
+#pragma unroll
+        for (int o = 8; o > 0; o /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float shift = shift_of(top), shift2 = shift * kLog2e;
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          sum += ex2(fabsf(shift) > kFar ? (v[j] - shift) * kLog2e : fmaf(v[j], kLog2e, -shift2));
+#pragma unroll
+        for (int o = 8; o > 0; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (row && tx == 0) w.stats[n0 / kTile * p.a.rows + m] = {top, sum};
+        continue;
+      }
+      if (!row) continue;
+      float* out = p.out + (p.sums ? split * p.a.rows : 0) * p.ld + m * p.ld;
+      if constexpr (KIND == kGrads) {
+        const RowCoef q = w.live.rows[m];
+        const int64_t at = (int64_t)q.target - w.first;
+        const float scale = softmax_scale(q.lse), lse = q.lse * scale;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float g = ex2(fmaf(v[j], scale, -lse)) * q.all - (column(j) == at ? q.one : 0.f);
+          v[j] = q.target < 0 ? 0.f : g;
+        }
+      } else {
+        const bool load = p.load || done > 0;
+        const float inv = p.sums || stop < depth ? 1.f : w.live.scale[1];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if (load && column(j) < p.b.rows) v[j] += out[column(j)];
+          v[j] *= inv;
+        }
+      }
+      const bool wide = p.ld % 4 == 0 && (uintptr_t)p.out % 16 == 0;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int64_t n = column(4 * h);
+        if (wide && n + 4 <= p.b.rows) {
+          *(float4*)(out + n) = make_float4(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (n + j < p.b.rows) out[n + j] = v[4 * h + j];
+        }
+      }
+    }
+    if constexpr (KIND == kWeights) {
 #pragma unroll
       for (int i = 0; i < kMine; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) fma2(acc[i][j], make_float2(x[i], x[i]), y[j]);
+        for (int j = 0; j < 4; ++j) acc[i][j] = make_float2(0.f, 0.f);
     }
-    if (more) a.store(sa[buf ^ 1]), b.store(sb[buf ^ 1]);
-    __syncthreads();
-  }
-  // of a row's values, j < 4 are columns n0 + tx * 4 + j, the others 64 further
-#pragma unroll
-  for (int i = 0; i < kMine; ++i) {
-    const int64_t m = m0 + (kMine == 2 ? ty * 2 + i : i / 4 * 64 + ty * 4 + i % 4);
-    const bool row = m < oa.rows;
-    float v[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = j % 2 ? acc[i][j / 2].y : acc[i][j / 2].x;
-    auto column = [&](int j) { return n0 + j / 4 * 64 + tx * 4 + j % 4; };
-    if constexpr (KIND == kStats) {
-      const int64_t target = row ? w.targets[m] : -1;
-      float top = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (column(j) >= p.b.rows) v[j] = -INFINITY;
-        else if (column(j) == target) w.at_target[m] = v[j];
-        top = fmaxf(top, v[j]);
-      }
-#pragma unroll
-      for (int o = 8; o > 0; o /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const float shift = shift_of(top), k = shift * kLog2e;
-      float sum = 0.f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        sum += ex2(fabsf(shift) > kFar ? (v[j] - shift) * kLog2e : fmaf(v[j], kLog2e, -k));
-#pragma unroll
-      for (int o = 8; o > 0; o /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (row && tx == 0) w.stats[n0 / kTile * p.a.rows + m] = {top, sum};
-      continue;
+  } while (KIND == kWeights && (done += kChain) < depth);
+}
+
+// dW from the slabs of its sums, of `words` rows each, in their order; 4 values a thread.
+__global__ void __launch_bounds__(256)
+finish_dw_kernel(const float* __restrict__ sums, int splits, int64_t ld, int64_t words, int64_t width,
+                 LiveTokens live, float* __restrict__ dw, int64_t dw_ld) {
+  await_previous();
+  const float inv = live.scale[1];
+  const int64_t each = live_each(*live.count, splits), per = ld / 4, all = words * per;
+  const int used = (int)((*live.count + each - 1) / each);
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = all <= 0xffffffffll ? (uint32_t)i / (uint32_t)per : i / per, c = (i - r * per) * 4;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int s = 0; s < used; ++s) {
+      const float4 u = *(const float4*)(sums + ((int64_t)s * words + r) * ld + c);
+      v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
     }
-    if (!row) continue;
-    float* out = p.out + (p.sums ? split * p.a.rows : 0) * p.ld + m * p.ld;
-    if constexpr (KIND == kGrads) {
-      const RowCoef q = w.live.rows[m];
-      const int64_t at = (int64_t)q.target - w.first;
-      const float scale = softmax_scale(q.lse), lse = q.lse * scale;
+    const float o[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float g = ex2(fmaf(v[j], scale, -lse)) * q.all - (column(j) == at ? q.one : 0.f);
-        v[j] = q.target < 0 ? 0.f : g;
-      }
-    } else {
-      const float inv = p.sums ? 1.f : w.live.scale[1];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        v[j] *= inv;
-        if (p.load && column(j) < p.b.rows) v[j] += out[column(j)];
-      }
-    }
-    const bool wide = p.ld % 4 == 0 && (uintptr_t)p.out % 16 == 0;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int64_t n = column(4 * h);
-      if (wide && n + 4 <= p.b.rows) {
-        *(float4*)(out + n) = make_float4(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (n + j < p.b.rows) out[n + j] = v[4 * h + j];
-      }
-    }
+    for (int j = 0; j < 4; ++j)
+      if (c + j < width) dw[r * dw_ld + c + j] = o[j] * inv;
   }
 }
 
@@ -315,11 +360,15 @@ ferrum_status loss_bwd_f32(ferrum_device* dev, const ferrum_cross_entropy_args* 
       1, std::min<int64_t>(2 * sm_count() / dx_tiles, ceil_div(std::min(piece, v), 256)));
   const int splits = product_of(tile, {nullptr, 0, n, false}, {nullptr, 0, d, false}, std::min(piece, v), want).splits;
   const int64_t rows = ceil_div(n, kStep) * kStep;    // room for all tokens
+  // dW: the same, of 256 tokens at least
+  const int64_t dw_tiles = ceil_div(std::min(piece, v), tile) * ceil_div(d, kTile);
+  const int dw_splits = (int)std::max<int64_t>(1, std::min<int64_t>(2 * sm_count() / dw_tiles, ceil_div(n, 256)));
   auto round = [](int64_t b) { return (size_t)((b + 255) / 256 * 256); };
   const size_t x_bytes = round(rows * ld * 4), w_bytes = copy_w ? round(v * ld * 4) : 0;
   const size_t g_bytes = round(rows * piece * 4), sum_bytes = round(splits * rows * ld * 4);
+  const size_t dw_bytes = dw_splits > 1 ? round(dw_splits * std::min(piece, v) * ld * 4) : 0;
   const size_t row_bytes = round(rows * sizeof(RowCoef)), index_bytes = round(rows * 4);
-  PoolBuffer ws(dev, x_bytes + w_bytes + g_bytes + sum_bytes + row_bytes + index_bytes + 256, stream);
+  PoolBuffer ws(dev, x_bytes + w_bytes + g_bytes + sum_bytes + dw_bytes + row_bytes + index_bytes + 256, stream);
   if (ws.status() != cudaSuccess) return cuda_error(ws.status(), "workspace");
   uint8_t* at = ws.as<uint8_t>();
   LiveTokens live;
@@ -328,7 +377,8 @@ ferrum_status loss_bwd_f32(ferrum_device* dev, const ferrum_cross_entropy_args* 
   float* x = (float*)(at += index_bytes);
   float* g = (float*)(at += x_bytes);
   float* sums = (float*)(at += g_bytes);
-  at += sum_bytes;
+  float* dw_sums = (float*)(at += sum_bytes);
+  at += dw_bytes;
   Matrix<float> wt = {(const float*)a->weight, a->weight_stride};
   if (ferrum_status s = start(what, true, prepare_kernel<float>, blocks_to_prepare(n, ld * 4), 1024, 0,
                               stream, (const float*)a->x, a->x_stride, d, x, ld, n, v, a->targets,
@@ -349,10 +399,18 @@ ferrum_status loss_bwd_f32(ferrum_device* dev, const ferrum_cross_entropy_args* 
     w.p[0].out = sums, w.p[0].ld = ld, w.p[0].sums = w.p[0].live_rows = true,
      w.p[0].load = first > 0;
     w.p[1] = product_of(tile, {g, piece, words, true}, {x, ld, d, true}, rows);
-    w.p[1].out = (float*)a->dweight + first * a->dweight_stride, w.p[1].ld = a->dweight_stride;
+    float* dw = (float*)a->dweight + first * a->dweight_stride;
+    w.p[1].out = dw, w.p[1].ld = a->dweight_stride;
     w.p[1].live_depth = true;
+    if (dw_splits > 1) w.p[1].splits = dw_splits, w.p[1].out = dw_sums, w.p[1].ld = ld, w.p[1].sums = true;
     w.count = 2;
     if (ferrum_status s = run<kWeights>(w, tile, false, stream, what)) return s;
+    if (dw_splits > 1) {
+      const int64_t grid = std::min<int64_t>(ceil_div(words * ld / 4, 256), sm_count() * 16);
+      if (ferrum_status s = start(what, false, finish_dw_kernel, grid, 256, 0, stream, (const float*)dw_sums,
+                                  dw_splits, ld, words, d, live, dw, a->dweight_stride))
+        return s;
+    }
   }
   return start(what, false, finish_dx_kernel<float>, std::min<int64_t>(ceil_div(n * ld / 4, 256), 148 * 16),
                256, 0, stream, (const float*)sums, splits, ld, rows, d, live, (float*)a->dx, a->dx_stride);

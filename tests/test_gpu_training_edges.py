@@ -269,3 +269,35 @@ def test_loss_of_logits_near_the_largest(tokens, dtype):
         for got, ref, e in ((g.dx, p @ w.double(), err @ w.double().abs()),
                             (g.dweight, p.t() @ x.double(), err.t() @ x.double().abs())):
             within(got, ref, 2 * e)
+
+
+# ---------------------------------------------------------------- long sums
+
+@pytest.mark.parametrize("tokens,width,vocab,masked", [(65536, 64, 256, 0.0), (50001, 40, 77, 0.4),
+                                                       (20000, 256, 9600, 0.0), (12345, 30, 1001, 1.0)])
+def test_weights_gradient_over_many_tokens(tokens, width, vocab, masked):
+    """In float32 dW is a sum over tokens, of either sign: n of them one after the other
+    are off by 0.6 sqrt(n / 2) units of 2^-24 at random (each addition rounds a partial
+    sum of sqrt(k) terms by 0.3 units of its size at most, twice that for the spread of
+    sizes). No chain is longer than 1024, whose sums are added; 8 units for the terms."""
+    x, w = rnd(1, tokens, width), rnd(2, vocab, width, std=1.5 / width ** 0.5)
+    g = torch.Generator().manual_seed(3)
+    t = torch.randint(vocab, (tokens,), generator=g)
+    t[torch.rand(tokens, generator=g) < masked] = -100
+    t = t.cuda()
+    d = torch.full((tokens,), 1.0 / tokens, device="cuda")
+    r = sq.linear_cross_entropy(x, w, t)
+    got = sq.linear_cross_entropy_backward(d, x, w, t, r.lse)
+    want = torch.zeros(vocab, width, dtype=torch.float64, device="cuda")
+    for i in range(0, tokens, 4096):
+        xs, ts = x[i:i + 4096][t[i:i + 4096] >= 0].double(), t[i:i + 4096][t[i:i + 4096] >= 0]
+        p = torch.softmax(xs @ w.double().t(), 1)
+        p[torch.arange(len(ts), device="cuda"), ts] -= 1
+        want += p.t() @ xs / tokens
+    if masked == 1.0:
+        assert not got.dweight.any() and not got.dx.any()
+        return
+    units = 0.6 * (1024 / 2) ** 0.5 + 0.6 * (tokens / 1024 / 2) ** 0.5 + 8
+    assert ((got.dweight.double() - want).norm() / want.norm()).item() <= units * EPS
+    again = sq.linear_cross_entropy_backward(d, x, w, t, r.lse)
+    assert torch.equal(again.dweight, got.dweight) and torch.equal(again.dx, got.dx)
