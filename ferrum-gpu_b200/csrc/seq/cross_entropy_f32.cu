@@ -311,7 +311,10 @@ ferrum_status run(const Work& w, int tile_rows, bool first, cudaStream_t stream,
   if (blocks > 0x7fffffff) return invalid(what, "too many tiles for one launch");
   if (tile_rows == 32) return start(what, first, loss_f32_kernel<KIND, 32>, blocks, kThreads, 0, stream, w);
   if (tile_rows == 64) return start(what, first, loss_f32_kernel<KIND, 64>, blocks, kThreads, 0, stream, w);
-  return start(what, first, loss_f32_kernel<KIND, 128>, blocks, kThreads, 0, stream, w);
+  if constexpr (KIND == kWeights)
+    return invalid(what, "no tile of 128 rows");      // (the gradient asks for 64 or 32)
+  else
+    return start(what, first, loss_f32_kernel<KIND, 128>, blocks, kThreads, 0, stream, w);
 }
 
 bool whole_rows(const void* p, int64_t ld, int64_t cols) {
