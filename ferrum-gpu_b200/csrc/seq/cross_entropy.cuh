@@ -281,9 +281,18 @@ struct Matrix {
   const T* p;
   int64_t ld;
 };
-// Blocks of the gradient's start, no fewer than a token and 16 KiB of x each, and one an SM.
+// SMs of the current device.
+inline int sm_count() {
+  int dev = 0, sms = 148;
+  if (cudaGetDevice(&dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    sms = 148;
+  return sms;
+}
+// Blocks of the gradient's start: a token and 16 KiB of x each at least, and no more than run at
+// once, since each looks through all targets for those in front of its own.
 inline int64_t blocks_to_prepare(int64_t tokens, int64_t bytes) {
-  return std::max<int64_t>(1, std::min({ceil_div(tokens * bytes, 16 * 1024), tokens, (int64_t)148 * 4}));
+  return std::max<int64_t>(1, std::min({ceil_div(tokens * bytes, 16 * 1024), tokens, (int64_t)sm_count() * 2}));
 }
 inline int64_t padded(int64_t n) { return ceil_div(n, 8) * 8; }
 
@@ -292,7 +301,7 @@ ferrum_status copied(Matrix<T>& m, int64_t width, int64_t rows, uint8_t*& at, bo
                      cudaStream_t stream, const char* what) {
   const int64_t ld = padded(width);
   const ferrum_status s =
-      start(what, first, copy_rows_kernel<T>, std::min<int64_t>(ceil_div(rows * ld / 8, 256), 148 * 32),
+      start(what, first, copy_rows_kernel<T>, std::min<int64_t>(ceil_div(rows * ld / 8, 256), sm_count() * 32),
             256, 0, stream, m.p, m.ld, width, (T*)at, ld, rows);
   m = {(const T*)at, ld};
   at += rows * ld * (int64_t)sizeof(T);

@@ -279,14 +279,6 @@ finish_dw_kernel(const float* __restrict__ sums, int splits, int64_t ld, int64_t
   }
 }
 
-int sm_count() {
-  int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    sms = 148;
-  return sms;
-}
-
 Product product_of(int tile_rows, const Operand& a, const Operand& b, int64_t depth, int splits = 1) {
   Product p = {};
   p.a = a, p.b = b, p.depth = depth;
@@ -415,7 +407,7 @@ ferrum_status loss_bwd_f32(ferrum_device* dev, const ferrum_cross_entropy_args* 
         return s;
     }
   }
-  return start(what, false, finish_dx_kernel<float>, std::min<int64_t>(ceil_div(n * ld / 4, 256), 148 * 16),
+  return start(what, false, finish_dx_kernel<float>, std::min<int64_t>(ceil_div(n * ld / 4, 256), sm_count() * 16),
                256, 0, stream, (const float*)sums, splits, ld, rows, d, live, (float*)a->dx, a->dx_stride);
 }
 

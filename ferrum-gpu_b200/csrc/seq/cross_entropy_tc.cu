@@ -775,13 +775,7 @@ loss_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
 }
 
 // ---------------------------------------------------------------- host
-int pair_count() {
-  int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    sms = 148;
-  return sms / 2;
-}
+int pair_count() { return sm_count() / 2; }
 
 Product product_of(int64_t m, int64_t n, int64_t depth, int splits = 1) {
   Product p = {};
@@ -982,7 +976,7 @@ ferrum_status bwd(ferrum_device* dev, const ferrum_cross_entropy_args* a, cudaSt
     if (ferrum_status s = run<T, kWeights>(x_first ? mx : mw, x_first ? mw : mx, w, false, stream, what)) return s;
   }
   if (splits > 1)
-    return start(what, false, finish_dx_kernel<T>, std::min<int64_t>(ceil_div(n * ld / 4, 256), 148 * 16),
+    return start(what, false, finish_dx_kernel<T>, std::min<int64_t>(ceil_div(n * ld / 4, 256), sm_count() * 16),
                  256, 0, stream, (const float*)sums, splits, ld, rows, d, live, (T*)a->dx, a->dx_stride);
   return FERRUM_OK;
 }
