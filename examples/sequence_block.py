@@ -87,14 +87,15 @@ class Dropout(torch.autograd.Function):
     """residual + dropout(x), the mask drawn again for the gradient."""
 
     @staticmethod
-    def forward(ctx, x, residual, p, seed):
-        ctx.p, ctx.seed, ctx.dtype = p, seed, x.dtype
-        return sq.dropout(x, p, seed, residual=residual)
+    def forward(ctx, x, residual, p, seed, offset=0):
+        ctx.p, ctx.seed, ctx.offset, ctx.dtype = p, seed, offset, x.dtype
+        return sq.dropout(x, p, seed, offset=offset, residual=residual)
 
     @staticmethod
     def backward(ctx, dy):
         dy = dy.contiguous()
-        return sq.dropout_backward(dy, ctx.p, ctx.seed, dtype=ctx.dtype), dy, None, None
+        dx = sq.dropout_backward(dy, ctx.p, ctx.seed, offset=ctx.offset, dtype=ctx.dtype)
+        return dx, dy, None, None, None
 
 
 class Loss(torch.autograd.Function):
@@ -206,8 +207,9 @@ class LongLayer(nn.Module):
 
 
 class RecurrenceLayer(nn.Module):
-    def __init__(self):
+    def __init__(self, index=0):
         super().__init__()
+        self.index = index        # layers count seeds alike: each draws masks of its own by it
         self.norm_in, self.norm_out = nn.Parameter(torch.ones(WIDTH)), nn.Parameter(torch.ones(WIDTH))
         self.scale = nn.Parameter(torch.full((WIDTH,), 0.5))
         self.proj_in = nn.Linear(WIDTH, 4 * WIDTH, bias=False)     # x, both gates, gate
@@ -223,7 +225,7 @@ class RecurrenceLayer(nn.Module):
             return NormAfter.apply(y, self.norm_out, gate, h, self.scale)
         self.seed += 1
         y = NormAfter.apply(y, self.norm_out, gate, torch.zeros_like(h), self.scale)
-        return Dropout.apply(y, h, DROP, self.seed.clone())
+        return Dropout.apply(y, h, DROP, self.seed.clone(), self.index)
 
     def start(self, batch):
         return {"state": torch.zeros(batch, WIDTH, device=self.scale.device)}
@@ -239,7 +241,7 @@ class Model(nn.Module):
     def __init__(self, length):
         super().__init__()
         self.embed = nn.Embedding(VOCAB, WIDTH)
-        self.layers = nn.ModuleList([ScanLayer(), LongLayer(length), RecurrenceLayer()])
+        self.layers = nn.ModuleList([ScanLayer(), LongLayer(length), RecurrenceLayer(2)])
         self.head = nn.Linear(WIDTH, VOCAB, bias=False)
 
     def hidden(self, tokens):
