@@ -8,11 +8,14 @@ test.
 
 from __future__ import annotations
 
+import threading
+
 import pytest
 import torch
 
 from conftest import gpu_available
-from test_gpu_training_ops import EPS, F32, TYPES, U, clean, ref_recurrence, rnd, within
+from test_gpu_training_ops import EPS, F32, TYPES, U, clean, loss_case, ref_recurrence, rnd, within
+from test_training_edges import words
 
 from ferrum_gpu import sequence as sq
 
@@ -301,3 +304,148 @@ def test_weights_gradient_over_many_tokens(tokens, width, vocab, masked):
     assert ((got.dweight.double() - want).norm() / want.norm()).item() <= units * EPS
     again = sq.linear_cross_entropy_backward(d, x, w, t, r.lse)
     assert torch.equal(again.dweight, got.dweight) and torch.equal(again.dx, got.dx)
+
+
+# ---------------------------------------------------------------- dropout's words
+
+@pytest.mark.parametrize("seed,offset", [
+    (0, 0), (2 ** 64 - 1, 2 ** 64 - 1), (0x299F31D0A4093822, 0x0370734413198A2E),
+    (1 << 32, 0), (0, 1 << 32), (0x80000000, 0x8000000080000000)])
+def test_dropout_follows_the_generator(seed, offset):
+    """All bits of seed and offset reach the words (test_training_edges.py pins these by
+    published vectors): masks of several chances bound each word from both sides."""
+    n = 4096
+    want = torch.tensor(words(0, n, seed, offset))
+    x = torch.ones(n, device="cuda")
+    signed = lambda v: v - 2 ** 64 if v >= 2 ** 63 else v
+    for p in (0.001, 0.1, 0.25, 0.5, 0.75, 0.999):
+        keep = want >= int(p * 2 ** 32)
+        for s in (seed, torch.tensor([signed(seed)], device="cuda")):
+            assert torch.equal((sq.dropout(x, p, s, offset=signed(offset)) != 0).cpu(), keep)
+            assert torch.equal((sq.dropout_backward(x, p, s, offset=signed(offset)) != 0).cpu(), keep)
+
+
+# ---------------------------------------------------------------- far and long recurrences
+
+def test_recurrence_gradients_beyond_2_31_values():
+    """The end of an array of more than 2^31 values: gradients flow from the end, so those
+    of the last 100 steps differ from a short call's by what its start does not know,
+    e^-0.45 a step over 400 of them."""
+    n, d = 2 ** 21 + 100, 1040
+    g = torch.Generator(device="cuda").manual_seed(1)
+    new = lambda: torch.empty(1, n, d, device="cuda", dtype=torch.bfloat16).normal_(generator=g)
+    x, ig, dout = new(), new(), new()
+    rg = torch.zeros(1, 1, 1, device="cuda", dtype=torch.bfloat16).expand(1, n, d).contiguous()
+    decay = torch.full((d,), 0.9, device="cuda")
+    s = sq.gated_recurrence(x, ig, rg, decay, save_states=True).states
+    whole = sq.gated_recurrence_backward(dout, x, ig, rg, decay, s)
+    end = slice(n - 500, n)
+    part = [v[:, end].contiguous() for v in (x, ig, rg)]
+    s = sq.gated_recurrence(*part, decay, save_states=True).states
+    tail = sq.gated_recurrence_backward(dout[:, end].contiguous(), *part, decay, s)
+    for name in ("dx", "dinput_gate", "drecurrence_gate"):
+        a, b = getattr(whole, name)[:, -100:], getattr(tail, name)[:, -100:].double()
+        # memories of 1 / (1 - e^-0.45) < 3 steps: 4 (20 + 10 * 3) units of the largest, and
+        # two roundings to bfloat16
+        within(a, b, 2.0 ** -8 * b.abs() + 4 * 50 * EPS * b.abs().max().item())
+    # ddecay: the other steps' part is missing from the short call's, n / 500 times as much
+    assert torch.isfinite(whole.ddecay).all()
+
+
+def test_recurrence_gradients_of_a_long_memory_in_float32():
+    """Factors up to 0.9999 over 4000 steps: neither states nor their gradients add up
+    errors in one direction. Each is off by sqrt(n) units at random, of which four times
+    are allowed, and what a gradient multiplies them with by 20 units."""
+    n, d = 4000, 64
+    x, ig, dout = rnd(1, 1, n, d), rnd(2, 1, n, d), rnd(4, 1, n, d)
+    rg = rnd(3, 1, n, d, std=0.1)
+    decay = torch.logspace(-3.7, -0.5, d, device="cuda")
+    wide = [v.double().requires_grad_() for v in (x, ig, rg, decay)]
+    out, _ = ref_recurrence(*wide, None, None)
+    want = torch.autograd.grad((out * dout.double()).sum(), wide)
+    s = sq.gated_recurrence(x, ig, rg, decay, save_states=True).states
+    got = sq.gated_recurrence_backward(dout, x, ig, rg, decay, s)
+    with torch.no_grad():
+        xd, i, r = x.double(), torch.sigmoid(ig.double()), torch.sigmoid(rg.double())
+        la = -decay.double() * r
+        a, root = torch.exp(la), torch.sqrt(-torch.expm1(2 * la))
+        grad, later = torch.empty_like(xd), torch.zeros(1, d, dtype=torch.float64, device="cuda")
+        for t in range(n - 1, -1, -1):
+            grad[:, t] = dout[:, t].double() + later
+            later = a[:, t] * grad[:, t]
+        top = grad.abs().amax(1)                      # of a channel
+        states = out.abs().amax(1)
+        off = (4 * n ** 0.5 + 20) * EPS
+        term = (r * a * (states + a / root * i * xd.abs())).amax(1)     # of ddecay, per G
+        size = {"dx": (root * i).amax(1), "dinput_gate": (root * xd.abs() * i * (1 - i)).amax(1),
+                "drecurrence_gate": 2 * term * decay.double() / 2}
+    for name, w in zip(("dx", "dinput_gate", "drecurrence_gate"), want):
+        err = (getattr(got, name).double() - w).abs().amax(1)
+        assert (err <= off * top * size[name] + U[F32] * w.abs().amax(1)).all(), name
+    # ddecay: n terms with both errors, those of neighbours alike for a memory's length
+    err = (got.ddecay.double() - want[3]).abs()
+    assert (err <= 2 * off * n * (top * term)[0]).all()
+
+
+# ---------------------------------------------------------------- the loss's rounding in 16 bits
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("tokens,width,vocab", [(777, 256, 3000), (4096, 64, 256), (40, 128, 1000), (900, 100, 70)])
+def test_loss_gradients_round_twice_in_16_bits(tokens, width, vocab, dtype):
+    """The logits' gradients are rounded to 16 bits between the products, with weights that
+    differ from token to token: a random relative error of u sqrt(E[1 / m^2] / 3) = 0.425 u
+    over mantissas m in [1, 2), as much as rounding the outputs leaves; both together
+    0.425 sqrt(2) u = 0.6 u, and 0.05 u for mantissas that do not spread evenly."""
+    x, w, t = loss_case(tokens, width, vocab, dtype, 0.0)
+    d = rnd(9, tokens).abs() + 0.1
+    r = sq.linear_cross_entropy(x, w, t)
+    g = sq.linear_cross_entropy_backward(d, x, w, t, r.lse)
+    p = torch.softmax(x.double() @ w.double().t(), 1)
+    p[torch.arange(tokens, device="cuda"), t] -= 1
+    p *= d.double()[:, None]
+    for got, ref in ((g.dx, p @ w.double()), (g.dweight, p.t() @ x.double())):
+        assert ((got.double() - ref).norm() / ref.norm()).item() <= 0.65 * U[dtype]
+
+
+# ---------------------------------------------------------------- two callers at once
+
+def test_two_threads_call_at_once():
+    """Calls of two host threads, each on a stream of its own, do not share workspaces."""
+    jobs = []
+    for seed in (0, 50):
+        x, ig, rg, dout = (rnd(seed + k, 2, 900, 96, dtype=torch.bfloat16) for k in range(4))
+        decay = rnd(seed + 4, 96).abs()
+        lx, lw, lt = loss_case(300, 100, 2001, torch.bfloat16, 0.2, seed=seed)
+        fx, fw, ft = loss_case(3000, 40, 77, F32, 0.2, seed=seed)
+
+        def job(stream=None, x=x, ig=ig, rg=rg, dout=dout, decay=decay, lx=lx, lw=lw, lt=lt, fx=fx, fw=fw, ft=ft):
+            k = {"stream": stream}
+            r = sq.gated_recurrence(x, ig, rg, decay, save_states=True, **k)
+            g = sq.gated_recurrence_backward(dout, x, ig, rg, decay, r.states, **k)
+            out = [*r, *g, sq.dropout(lx, 0.3, 5, **k)]
+            for a, b, t in ((lx, lw, lt), (fx, fw, ft)):
+                l = sq.linear_cross_entropy(a, b, t, **k)
+                out += [*l, *sq.linear_cross_entropy_backward(torch.ones_like(l.loss), a, b, t, l.lse, **k)]
+            return out
+
+        jobs.append(job)
+    want = [job() for job in jobs]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def work(i):
+        s = torch.cuda.Stream()
+        for _ in range(10):
+            got[i].append(jobs[i](stream=s))
+        s.synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    for i in range(2):
+        assert len(got[i]) == 10
+        for out in got[i]:
+            for a, b in zip(out, want[i]):
+                assert torch.equal(a, b)
