@@ -8,6 +8,7 @@ test.
 
 from __future__ import annotations
 
+import ctypes
 import threading
 
 import pytest
@@ -17,7 +18,7 @@ from conftest import gpu_available
 from test_gpu_training_ops import EPS, F32, TYPES, U, clean, loss_case, ref_recurrence, rnd, within
 from test_training_edges import words
 
-from ferrum_gpu import sequence as sq
+from ferrum_gpu import capi, sequence as sq
 
 pytestmark = pytest.mark.gpu
 
@@ -449,3 +450,29 @@ def test_two_threads_call_at_once():
         for out in got[i]:
             for a, b in zip(out, want[i]):
                 assert torch.equal(a, b)
+
+
+# ---------------------------------------------------------------- wide rows
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_loss_refuses_rows_too_wide_for_16_bits(dtype):
+    """Logits of 2^20 products are off by 2^16 additions cut off by half a unit of 2^-23 on
+    average, of a sum that grows to the logit: 0.004 of it, twice that allowed."""
+    n = 1 << 20
+    x, w = rnd(1, 3, n + 1, dtype=dtype), rnd(2, 5, n + 1, dtype=dtype, std=2.0 ** -10)
+    t = torch.tensor([0, 4, 2], device="cuda")
+    with pytest.raises(ValueError, match="width must be at most 2.20 in 16-bit types"):
+        sq.linear_cross_entropy(x, w, t)
+    with pytest.raises(ValueError, match="width must be at most 2.20 in 16-bit types"):
+        sq.linear_cross_entropy_backward(None, x, w, t, torch.zeros(3, device="cuda"))
+    r = sq.linear_cross_entropy(x[:, :n], w[:, :n], t)
+    logits = x[:, :n].double() @ w[:, :n].double().t()
+    off = 2 * 0.004 * logits.abs().amax(1)
+    within(r.lse, torch.logsumexp(logits, 1), off)
+    within(r.loss, torch.logsumexp(logits, 1) - logits[torch.arange(3, device="cuda"), t], 2 * off)
+    dev = capi.DeviceHandle(0)
+    for name in ("ferrum_linear_cross_entropy", "ferrum_linear_cross_entropy_bwd"):
+        block = capi.SEQ_SIGNATURES[name]
+        args = block(struct_size=ctypes.sizeof(block), dtype=1, tokens=1, width=n + 1, vocab=1)
+        assert getattr(capi.lib(), name)(dev.ptr, ctypes.byref(args), None) == capi.FERRUM_ERR_INVALID_ARG
+        assert "2^20" in capi.last_error()
