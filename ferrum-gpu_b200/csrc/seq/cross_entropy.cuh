@@ -259,6 +259,35 @@ finish_dx_kernel(const float* __restrict__ sums, int splits, int64_t ld, int64_t
   }
 }
 
+// Tokens of each split of dW's depth, whole steps of it; splits behind the last have none.
+__host__ __device__ inline int64_t live_each(int64_t live, int splits, int step) {
+  return ((live + step - 1) / step + splits - 1) / splits * step;
+}
+
+// dW from the slabs of its sums, of `words` rows each, in their order; 4 values a thread.
+template <class T>
+__global__ void __launch_bounds__(256)
+finish_dw_kernel(const float* __restrict__ sums, int splits, int step, int64_t ld, int64_t words,
+                 int64_t width, LiveTokens live, T* __restrict__ dw, int64_t dw_ld) {
+  await_previous();
+  const float inv = live.scale[1];
+  const int64_t each = live_each(*live.count, splits, step), per = ld / 4, all = words * per;
+  const int used = (int)((*live.count + each - 1) / each);
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = all <= 0xffffffffll ? (uint32_t)i / (uint32_t)per : i / per, c = (i - r * per) * 4;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int s = 0; s < used; ++s) {
+      const float4 u = *(const float4*)(sums + ((int64_t)s * words + r) * ld + c);
+      v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+    }
+    const float o[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (c + j < width) dw[r * dw_ld + c + j] = from_f<T>(o[j] * inv);
+  }
+}
+
 // A launch that may start while the call's one in front of it ends (`first`: one that
 // may not).
 template <class... P, class... A>

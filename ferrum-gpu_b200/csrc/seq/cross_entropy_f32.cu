@@ -120,11 +120,6 @@ struct Piece {
   }
 };
 
-// Tokens of each split of a product whose depth they are; splits behind the last have none.
-__host__ __device__ inline int64_t live_each(int64_t live, int splits) {
-  return ((live + kStep - 1) / kStep + splits - 1) / splits * kStep;
-}
-
 template <int KIND, int ROWS>
 __global__ void __launch_bounds__(kThreads, 2) loss_f32_kernel(const __grid_constant__ Work w) {
   constexpr int kMine = ROWS / 16;        // rows of a thread
@@ -142,7 +137,7 @@ __global__ void __launch_bounds__(kThreads, 2) loss_f32_kernel(const __grid_cons
   Operand oa = p.a;
   if (p.live_rows) oa.rows = live;
   if (m0 >= oa.rows) return;
-  const int64_t each = p.live_depth ? live_each(live, p.splits) : p.depth_per_split;
+  const int64_t each = p.live_depth ? live_each(live, p.splits, kStep) : p.depth_per_split;
   const int64_t k0 = split * each, left = (p.live_depth ? live : p.depth) - k0;
   const int depth = (int)(left < each ? left : each);
   if (depth <= 0) return;
@@ -254,29 +249,6 @@ __global__ void __launch_bounds__(kThreads, 2) loss_f32_kernel(const __grid_cons
         for (int j = 0; j < 4; ++j) acc[i][j] = make_float2(0.f, 0.f);
     }
   } while (KIND == kWeights && (done += kChain) < depth);
-}
-
-// dW from the slabs of its sums, of `words` rows each, in their order; 4 values a thread.
-__global__ void __launch_bounds__(256)
-finish_dw_kernel(const float* __restrict__ sums, int splits, int64_t ld, int64_t words, int64_t width,
-                 LiveTokens live, float* __restrict__ dw, int64_t dw_ld) {
-  await_previous();
-  const float inv = live.scale[1];
-  const int64_t each = live_each(*live.count, splits), per = ld / 4, all = words * per;
-  const int used = (int)((*live.count + each - 1) / each);
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = all <= 0xffffffffll ? (uint32_t)i / (uint32_t)per : i / per, c = (i - r * per) * 4;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-    for (int s = 0; s < used; ++s) {
-      const float4 u = *(const float4*)(sums + ((int64_t)s * words + r) * ld + c);
-      v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
-    }
-    const float o[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (c + j < width) dw[r * dw_ld + c + j] = o[j] * inv;
-  }
 }
 
 Product product_of(int tile_rows, const Operand& a, const Operand& b, int64_t depth, int splits = 1) {
@@ -402,8 +374,8 @@ ferrum_status loss_bwd_f32(ferrum_device* dev, const ferrum_cross_entropy_args* 
     if (ferrum_status s = run<kWeights>(w, tile, false, stream, what)) return s;
     if (dw_splits > 1) {
       const int64_t grid = std::min<int64_t>(ceil_div(words * ld / 4, 256), sm_count() * 16);
-      if (ferrum_status s = start(what, false, finish_dw_kernel, grid, 256, 0, stream, (const float*)dw_sums,
-                                  dw_splits, ld, words, d, live, dw, a->dweight_stride))
+      if (ferrum_status s = start(what, false, finish_dw_kernel<float>, grid, 256, 0, stream, (const float*)dw_sums,
+                                  dw_splits, kStep, ld, words, d, live, dw, a->dweight_stride))
         return s;
     }
   }

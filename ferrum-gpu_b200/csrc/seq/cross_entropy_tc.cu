@@ -83,6 +83,10 @@ constexpr int kThreads = 32 * (kEpilogueWarp + kEpilogueWarps);
 constexpr int kSlotBytes = 32 * 128;                          // a warp's rows on their way out
 // and 1024 bytes of room to align
 constexpr int kSmemBytes = kStages * kStageBytes + kEpilogueWarps * kSlotBytes + 1024;
+// Tokens that one chain of dW's sums takes at most. The tensor cores cut off each of its n / 16
+// additions, by half a unit of 2^-23 on average, of a sum that grows as sqrt(n): n / 24 units of
+// 2^-24 at its end, which is 0.17 of float16's rounding at 32768.
+constexpr int64_t kChain = 32768;
 constexpr uint32_t kGroup = 16;                                   // tiles of M that share a tile of N
 
 enum Kind { kStats, kGrads, kWeights };
@@ -92,7 +96,8 @@ struct Product {
   int64_t m, n;
   int tiles_m, tiles_n, splits, steps, steps_per_split;
   bool a_mn;                 // A's rows run along the depth (as all of B's in kWeights)
-  bool live_rows, live_depth;  // m or the depth is the number of tokens with a loss
+  bool live_rows, live_depth;  // m or the depth is the number of tokens with a loss (the
+                               // depth shared out to the splits)
   bool dx;                   // rows go to the tokens' places
   bool sums;                 // the result: float32 sums, a slab per split (else 16 bits)
   bool load, store_map;      // sums of earlier pieces come on top; `out` has a tensor map
@@ -129,17 +134,27 @@ __device__ __forceinline__ int64_t rows_of(const Product& p, int live) { return 
 __device__ __forceinline__ uint32_t tiles_m_of(const Product& p, int live) {
   return p.live_rows ? (uint32_t)(live + kTile - 1) / kTile : p.tiles_m;
 }
+__device__ __forceinline__ int steps_each(const Product& p, int live) {   // (as live_each())
+  if (!p.live_depth) return p.steps_per_split;
+  return p.splits > 1 ? (live / kDepth + p.splits - 1) / p.splits : live / kDepth;
+}
+// Splits that have a step of depth.
+__device__ __forceinline__ int splits_of(const Product& p, int live) {
+  if (!p.live_depth || p.splits == 1) return p.splits;
+  const int each = steps_each(p, live);
+  return (live / kDepth + each - 1) / each;
+}
 __device__ __forceinline__ uint32_t tiles_of(const Product& p, int live) {
-  return tiles_m_of(p, live) * (uint32_t)p.tiles_n * (uint32_t)p.splits;
+  return tiles_m_of(p, live) * (uint32_t)p.tiles_n * (uint32_t)splits_of(p, live);
 }
 // A tile's steps of depth, from k0 up to k1.
 struct Depth {
   int k0, k1;
 };
 __device__ __forceinline__ Depth depth_of(const Product& p, int split, int live) {
-  if (p.live_depth) return {0, live / kDepth};
-  const int k0 = split * p.steps_per_split, k1 = k0 + p.steps_per_split;
-  return {k0, k1 < p.steps ? k1 : p.steps};
+  const int each = steps_each(p, live), all = p.live_depth ? live / kDepth : p.steps;
+  const int k0 = split * each, k1 = k0 + each;
+  return {k0, k1 < all ? k1 : all};
 }
 template <int KIND>
 __device__ __forceinline__ Place place_of(const Work& w, uint32_t t, int live) {
@@ -897,13 +912,22 @@ ferrum_status bwd(ferrum_device* dev, const ferrum_cross_entropy_args* a, cudaSt
       1, std::min<int64_t>(pair_count() / dx_tiles, ceil_div(std::min(piece, v), 4 * kDepth)));
   const int splits = product_of(n, d, std::min(piece, v), want).splits;
   const int64_t rows = ceil_div(n, kDepth) * kDepth;    // room for all tokens
+  // So are the tokens of few tiles of dW, from 4096 on and 1024 at least in a split, since its
+  // sums take a launch to join (us without and with splits: 1500 x 256 x 500 32.5 and 37.6,
+  // 2500 x 256 x 500 37.6 and 40.2, 4096 x 1024 x 1000 68.7 and 57.5, 16384 x 64 x 256 96.6 and
+  // 43.5, with splits of 256 tokens 60), and those of a long chain.
+  const int64_t dw_tiles = ceil_div(std::min(piece, v), kTile) * ceil_div(d, kTile);
+  const int64_t dw_want = std::max(n < 4096 ? 1 : std::min<int64_t>(pair_count() / dw_tiles, n / 1024),
+                                   ceil_div(n, kChain));
+  const int dw_splits = few ? 1 : product_of(1, 1, rows, (int)dw_want).splits;
   const bool need_sums = splits > 1 || !one_piece;
   auto round = [](int64_t b) { return (size_t)((b + 255) / 256 * 256); };
   const size_t x_bytes = round(n * ld * 2), w_bytes = copy_w ? round(v * ld * 2) : 0;
   const size_t g_bytes = round((few ? v : rows) * g_ld * 2);
   const size_t sum_bytes = need_sums ? round(splits * rows * ld * 4) : 0;
+  const size_t dw_bytes = dw_splits > 1 ? round(dw_splits * std::min(piece, v) * ld * 4) : 0;
   const size_t row_bytes = round(rows * sizeof(RowCoef)), index_bytes = round(rows * 4);
-  PoolBuffer ws(dev, x_bytes + w_bytes + g_bytes + sum_bytes + row_bytes + index_bytes + 256, stream);
+  PoolBuffer ws(dev, x_bytes + w_bytes + g_bytes + sum_bytes + dw_bytes + row_bytes + index_bytes + 256, stream);
   if (ws.status() != cudaSuccess) return cuda_error(ws.status(), "workspace");
   uint8_t* at = ws.as<uint8_t>();
   LiveTokens live;
@@ -916,7 +940,8 @@ ferrum_status bwd(ferrum_device* dev, const ferrum_cross_entropy_args* a, cudaSt
   T* g = (T*)at;
   at += g_bytes;
   float* sums = need_sums ? (float*)at : nullptr;
-  at += sum_bytes;
+  float* dw_sums = (float*)(at += sum_bytes);
+  at += dw_bytes;
   Matrix<T> wt = {(const T*)a->weight, a->weight_stride};
   if (ferrum_status s = start(what, true, prepare_kernel<T>, blocks_to_prepare(n, ld * 2), 1024, 0, stream,
                               (const T*)a->x, a->x_stride, d, x, ld, n, v, a->targets,
@@ -963,17 +988,24 @@ ferrum_status bwd(ferrum_device* dev, const ferrum_cross_entropy_args* a, cudaSt
       if (ferrum_status s = run<T, kGrads>(logits, logits, w, false, stream, what)) return s;
     }
 
-    Product px = product_of(rows, d, words, splits), pw = product_of(words, d, few ? g_ld : rows);
+    Product px = product_of(rows, d, words, splits), pw = product_of(words, d, few ? g_ld : rows, dw_splits);
     px.live_rows = px.dx = true, pw.live_depth = !few;
     px.partial = sums, px.partial_ld = ld;
     px.load = first > 0, px.sums = splits > 1 || !last;
     px.out = a->dx, px.ld = a->dx_stride;
     (few ? px : pw).a_mn = true;
     pw.out = dw, pw.ld = a->dweight_stride, pw.store_map = dw_map;
+    if (dw_splits > 1) pw.sums = true, pw.partial = dw_sums, pw.partial_ld = ld;
     // the product of the longer tiles first, so that the last ones are short
     const bool x_first = px.steps_per_split >= pw.steps_per_split;
     w.p[0] = x_first ? px : pw, w.p[1] = x_first ? pw : px, w.count = 2;
     if (ferrum_status s = run<T, kWeights>(x_first ? mx : mw, x_first ? mw : mx, w, false, stream, what)) return s;
+    if (dw_splits > 1) {
+      const int64_t grid = std::min<int64_t>(ceil_div(words * ld / 4, 256), sm_count() * 16);
+      if (ferrum_status s = start(what, false, finish_dw_kernel<T>, grid, 256, 0, stream, (const float*)dw_sums,
+                                  dw_splits, kDepth, ld, words, d, live, dw, a->dweight_stride))
+        return s;
+    }
   }
   if (splits > 1)
     return start(what, false, finish_dx_kernel<T>, std::min<int64_t>(ceil_div(n * ld / 4, 256), sm_count() * 16),
