@@ -25,7 +25,8 @@ Activations are float32, float16 or bfloat16 tensors, all of one type, shaped
 (``long_conv``: (batch, channels, length), any strides). Parameters, scan
 states and parameter gradients are float32 (but a vocabulary matrix and its
 gradient, which have x's type). Arithmetic runs in float32; an
-output is rounded once to its type. Results do not depend on scheduling.
+output is rounded once to its type (``linear_cross_entropy_backward`` rounds
+once more in between). Results do not depend on scheduling.
 
 ``lengths`` (int32, one per sequence) are the valid lengths of a padded batch:
 steps past them are not read, and their outputs and gradients are zero.
@@ -419,7 +420,8 @@ def linear_cross_entropy(x, weight, targets, *, device=None, stream=None) -> Cro
     of x's type; targets: int64 of x's leading shape. loss and lse are float32 of that shape. The logits are
     never kept: a piece at a time lives on chip. A row whose target lies outside
     the vocabulary (-100, say) has no loss: its loss, lse and gradients are 0,
-    whatever its values.
+    whatever its values. Workspace: 8 bytes for each token and 128 words, and a
+    copy of x or weight whose rows do not begin at multiples of 16 bytes.
     """
     return CrossEntropyResult(*_call(_sequence.linear_cross_entropy, x, weight, targets, device, stream))
 
@@ -429,7 +431,16 @@ def linear_cross_entropy_backward(dloss, x, weight, targets, lse, *, dlse=None, 
     """Gradients of ``linear_cross_entropy`` for those of loss (``dloss``) and
     of lse (``dlse``), float32; either may be None. ``lse`` is the forward's. The
     logits are computed again, a piece of the vocabulary at a time, for the tokens
-    that have a loss. dx and dweight have x's type."""
+    that have a loss. dx and dweight have x's type.
+
+    In 16-bit types the logits' gradients are rounded to 16 bits between the
+    products, whose operands they are: dx and dweight are up to 1.4 times as far
+    from the exact ones as rounding the outputs leaves them (in float16, dx of
+    tokens whose weight is less than 2^-18 of the largest is farther). Workspace:
+    those gradients (256 MiB, or of 4096 words if that is more), a copy of x, one of
+    weight as above, and float32 sums of dx (tokens x width) and dweight where their
+    products are split.
+    """
     return CrossEntropyGrads(*_call(
         _sequence.linear_cross_entropy_backward, dloss, x, weight, targets, lse, dlse, device,
         stream))

@@ -14,7 +14,7 @@
  * type `dtype`; parameters, scan states and parameter gradients are float32 (but
  * a vocabulary matrix and its gradient, of type `dtype`).
  * Sums, recurrences and statistics run in float32; each output is rounded
- * once to its type. No result depends on the order in which blocks run.
+ * once to its type (the loss's gradient says what else it rounds). No result depends on the order in which blocks run.
  * An array that a call writes shares no memory with its other arrays, except
  * where a block says so; the C entries take the caller's word for it.
  *
@@ -274,8 +274,17 @@ ferrum_status ferrum_dropout_bwd(ferrum_device *dev, const ferrum_dropout_args *
  *   l[t,v] = sum_d x[t,d] * weight[v,d]
  *   lse[t] = log(sum_v exp(l[t,v]));  loss[t] = lse[t] - l[t, target[t]]
  * x, weight, dx and dweight have type `dtype`. 16-bit rows are at most
- * FERRUM_LOSS_MAX_WIDTH_16 wide. The logits are never stored as a whole. A row whose target lies outside [0, vocab) has no loss: its loss, lse
- * and gradients are 0, whatever its values.
+ * FERRUM_LOSS_MAX_WIDTH_16 wide. The logits are never stored as a whole. A row
+ * whose target lies outside [0, vocab) has no loss: its loss, lse and gradients
+ * are 0, whatever its values.
+ * In 16-bit types the gradient rounds the logits' gradients to 16 bits between
+ * its products: dx and dweight are up to 1.4 times as far from the exact ones as
+ * their own rounding leaves them.
+ * Workspace of the loss: 8 bytes for each token and 128 words, and a copy of x or
+ * weight whose rows do not begin at multiples of 16 bytes. Of the gradient: the
+ * logits' gradients of a piece of the vocabulary (256 MiB, or 4096 words if that
+ * is more), a copy of x, one of weight as above, and float32 sums of dx
+ * (tokens * width) and dweight where their products are split.
  */
 typedef struct {
   size_t struct_size;
