@@ -12,7 +12,8 @@
 // down to 2^-27 in full precision, dloss may be tiny, and a target's value, nearly
 // -dloss, is nearly -2^13 where all tokens weigh the same, so that its rounding to 16
 // bits is none. The others' roundings have random signs: 8192 x 2048 x 32768 bf16, dx
-// and dW are 0.00166 from 64 bits, of which rounding themselves is 0.00166.
+// and dW are 0.00166 from 64 bits, of which rounding themselves is 0.00166; 16384 x 64 x
+// 256, where the softmax is larger, 0.00195 and 0.00175 of 0.00165.
 //
 // A pair of CTAs computes a tile of 256 x 256: each stages 128 rows of A and of B
 // (32 KiB a step of 64) by TMA, one thread of the leader issues 256 x 256 x 16
@@ -821,8 +822,10 @@ template <class T>
 constexpr bool is_bf16() { return std::is_same<T, __nv_bfloat16>::value; }
 
 // Up to so many tokens the sides change. Forward and gradient, us, with tiles of 256
-// tokens and with the sides changed: 8 x 4096 x 131072 221, 637 and 196, 616;
-// 64 x 256 x 2000 14.7, 30.6 and 12.7, 25.0; 64 x 2048 x 32000 37.6, 109 and 39.3, 105;
+// tokens and with the sides changed: 8 x 4096 x 131072 267, 607 and 195, 587;
+// 40 x 2048 x 32000 40.8, 114 and 39.3, 103; 64 x 256 x 2000 13.9, 27 and 15.4, 23.5;
+// 64 x 512 x 8000 16.9, 49 and 14.8, 43; 64 x 2048 x 32000 40.8, 112 and 39.3, 103;
+// 64 x 4096 x 32000 61.4, 180 and 63.1, 172; 64 x 4096 x 131072 198, 610 and 200, 595.
 // 100 x 2048 x 32000 37.4, 113 and 43.0, 111.
 constexpr int64_t kFewTokens = 64;
 

@@ -14,7 +14,8 @@
 namespace ferrum {
 namespace seq {
 
-// sigmoid(x) and 1 - sigmoid(x), each with a relative error of a few units.
+// sigmoid(x) and 1 - sigmoid(x), each with a relative error of a few units; below -4 of |x|
+// / 2 units more, from rounding the exponential's argument.
 struct Gate {
   float on, off;
 };
@@ -46,8 +47,8 @@ constexpr float kKeep = -0.f;                   // the code of a = 1
 __device__ __forceinline__ float checked_decay(float decay) { return decay < 0.f ? NAN : decay; }
 
 // e^x for x <= 0: x = k ln 2 + r with |r| <= ln 2 / 2; (e^r - 1 - r) / r^2 by a
-// polynomial of degree 4, fitted for the relative error of e^r - 1 (largest 0.23
-// units of 2^-24). One rounded ln 2 is enough: k of it shifts e^r by k 2e-9, of an
+// polynomial of degree 4, fitted for the relative error of e^r - 1 (largest 0.30
+// units of 2^-24, at r = -0.30). One rounded ln 2 is enough: k of it shifts e^r by k 2e-9, of an
 // a that is 2^k. Below -87 the factor is 0; NaN stays NaN.
 // `w`: 1 - a^2 with its relative accuracy.
 __device__ __forceinline__ Factor factor_of(float x, float* w = nullptr) {
@@ -69,8 +70,8 @@ __device__ __forceinline__ Factor factor_of(float x, float* w = nullptr) {
   return {near ? -fabsf(q) : a};
 }
 
-// e^x - 1 for x in [-1, 0], a polynomial as above, of degree 5 (largest error 0.05
-// units before its own roundings): 8 instructions where factor_of takes 25.
+// e^x - 1 for x in [-1, 0], a polynomial as above, of degree 5 (largest relative error
+// 0.17 units of 2^-24 before its own roundings, at x = -0.95): 8 instructions where factor_of takes 25.
 constexpr float kShortDecay = 1.f;
 __device__ __forceinline__ float expm1_short(float x) {
   float p = 0.00012913093087263405f;
