@@ -45,11 +45,12 @@ ferrum_status check_loss(const ferrum_device* dev, const ferrum_cross_entropy_ar
   // (rows are numbered by 32 bits in the tensor copies)
   if (a->tokens > 0x7fffff00 || a->vocab > 0x7fffff00 || a->width > 0x7fffff00)
     return invalid(what, "tokens, vocab and width must be below 2^31 - 256");
-  // The tensor cores cut off each of a logit's width / 16 additions, by half a unit of 2^-23 on
-  // average: at 2^20 that is 0.0024 of the logit, as bfloat16's rounding of x and weight (at
-  // 2^26, 0.15 was measured, and a tile took 0.3 of the second that waits are given).
+  // The tensor cores cut off each of the width / 16 additions of a logit in the gradient, which
+  // shrinks it by 1.5e-8 of it each: at 2^16 that is 6e-5 of the logit, and the softmax of one of
+  // 2.5 off by a third of float16's rounding, in one direction. (At 2^26 a tile also takes 0.3 of
+  // the second that waits are given.)
   if (a->dtype != FERRUM_F32 && a->width > FERRUM_LOSS_MAX_WIDTH_16)
-    return invalid(what, "width must be at most 2^20 in 16-bit types");
+    return invalid(what, "width must be at most 2^16 in 16-bit types");
   if (bounded_product({a->tokens, a->width}) < 0 || bounded_product({a->vocab, a->width}) < 0)
     return invalid(what, "tokens * width or vocab * width is too large");
   const size_t e = dtype_size(a->dtype);

@@ -88,6 +88,12 @@ constexpr int kSmemBytes = kStages * kStageBytes + kEpilogueWarps * kSlotBytes +
 // additions, by half a unit of 2^-23 on average, of a sum that grows as sqrt(n): n / 24 units of
 // 2^-24 at its end, which is 0.17 of float16's rounding at 32768.
 constexpr int64_t kChain = 32768;
+// Steps of depth after which the logits of the loss are taken from TMEM and added up in
+// registers, which round: a chain of width / 16 additions that are cut off shrinks its sum by
+// 1.5e-8 of it each on average (1000 x 4096 x 256 bf16 in one chain: lse 1.3e-6 from 64 bits,
+// loss 1.6e-6; in four 3.0e-7 and 3.6e-7; 4096 x 2048 x 32768 355 and 362 us). The gradient
+// rounds to 16 bits what it makes of its logits.
+constexpr int kPartSteps = 16;
 constexpr uint32_t kGroup = 16;                                   // tiles of M that share a tile of N
 
 enum Kind { kStats, kGrads, kWeights };
@@ -115,6 +121,7 @@ struct Work {
   const int64_t* targets;
   RowStat* stats;            // (half tile of N, m)
   float* at_target;
+  int parts;                 // of the depth
   // gradients
   LiveTokens live;
   int known;                 // how many tokens have a loss (with those behind), if the host knows
@@ -223,14 +230,16 @@ __device__ __forceinline__ RowCoef row_ahead(const Work& w, const Place& q, int6
   return r;
 }
 
-template <class F>
+// `more(acc)`: another part of the depth, its accumulators at `acc`, if there is one.
+template <class F, class G>
 __device__ void finish_stats(const Work& w, uint32_t acc, const RowCoef& row, int64_t m, int64_t n0,
-                             F release) {
+                             F release, G more) {
   const Product& p = w.p[0];
   const int at = row.target - (int)n0;
   const int cols = p.n - n0 < kHalf ? (int)(p.n - n0) : kHalf;      // (may be below 0)
   if (cols <= 0) {
-    release();
+    do release();
+    while (more(acc));
     return;
   }
   float v[4][32], hit = 0.f;
@@ -238,6 +247,18 @@ __device__ void finish_stats(const Work& w, uint32_t acc, const RowCoef& row, in
   for (int j = 0; j < 4; ++j) tmem_load32(acc + j * 32, v[j]);
   tmem_load_wait();
   release();
+#pragma unroll 1
+  while (more(acc)) {
+#pragma unroll
+    for (int j = 0; j < kHalf / 16; ++j) {
+      float u[16];
+      tmem_load16(acc + j * 16, u);
+      tmem_load_wait();
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[j / 2][j % 2 * 16 + i] += u[i];
+    }
+    release();
+  }
   if (cols < kHalf) {
 #pragma unroll
     for (int i = 0; i < kHalf; ++i)
@@ -476,22 +497,26 @@ loss_product_kernel(const __grid_constant__ Maps maps0, const __grid_constant__ 
       // 16 steps of depth: 32 bytes along a K-major row, two atoms MN-major
       constexpr uint32_t kStepA = (A_MN ? 2048 : 32) / 16, kStepB = (B_MN ? 2048 : 32) / 16;
       const Product& p = w.p[q.product];
-      const int k0 = depth_of(p, q.split, live).k0, k1 = depth_of(p, q.split, live).k1;
-      if (!(ok = wait(&sh, &sh.drained[buf], buf_phase ^ 1, w.err_flag))) return;
-      tc_fence_after();
-      const uint32_t acc = tmem + buf * kTile;
-      for (int k = k0; k < k1; ++k) {
-        if (!(ok = wait(&sh, &sh.full[stage], phase, w.err_flag))) return;
+      const int end = depth_of(p, q.split, live).k1;
+      for (int k0 = depth_of(p, q.split, live).k0; k0 < end;) {
+        const int k1 = KIND == kStats && end - k0 > kPartSteps ? k0 + kPartSteps : end;
+        if (!(ok = wait(&sh, &sh.drained[buf], buf_phase ^ 1, w.err_flag))) return;
         tc_fence_after();
-        const uint64_t a = first_a + stage * (kStageBytes / 16), b = first_b + stage * (kStageBytes / 16);
+        const uint32_t acc = tmem + buf * kTile;
+        for (int k = k0; k < k1; ++k) {
+          if (!(ok = wait(&sh, &sh.full[stage], phase, w.err_flag))) return;
+          tc_fence_after();
+          const uint64_t a = first_a + stage * (kStageBytes / 16), b = first_b + stage * (kStageBytes / 16);
 #pragma unroll
-        for (int i = 0; i < kDepth / 16; ++i)
-          mma_pair(acc, a + i * kStepA, b + i * kStepB, kIdesc, k > k0 || i > 0);
-        commit_pair(&sh.empty[stage]);
-        if (++stage == kStages) stage = 0, phase ^= 1;
+          for (int i = 0; i < kDepth / 16; ++i)
+            mma_pair(acc, a + i * kStepA, b + i * kStepB, kIdesc, k > k0 || i > 0);
+          commit_pair(&sh.empty[stage]);
+          if (++stage == kStages) stage = 0, phase ^= 1;
+        }
+        commit_pair(&sh.done[buf]);
+        if (++buf == 2) buf = 0, buf_phase ^= 1;
+        k0 = k1;
       }
-      commit_pair(&sh.done[buf]);
-      if (++buf == 2) buf = 0, buf_phase ^= 1;
     };
     for (uint32_t t = pair; ok && t < tiles; t += pairs) {
       const Place q = place_of<KIND>(w, t, live);
@@ -515,24 +540,39 @@ loss_product_kernel(const __grid_constant__ Maps maps0, const __grid_constant__ 
       row_next = row_ahead<KIND>(w, next, (int64_t)next.tm * kTile + rank * kHalf + lanes + lane, live);
     };
     look_ahead(pair);
-    for (uint32_t t = pair; t < tiles; t += pairs) {
-      bool ok = lane != 0 || wait(&sh, &sh.done[buf], buf_phase, w.err_flag);
+    bool ok = true;
+    // the next accumulators' address, once they are done
+    auto await_done = [&]() -> uint32_t {
+      ok = lane != 0 || wait(&sh, &sh.done[buf], buf_phase, w.err_flag);
       ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
-      if (!ok) break;
       tc_fence_after();
+      return tmem + (lanes << 16) + buf * kTile + half * kHalf;
+    };
+    auto release = [&] {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_at(drained + buf * 8);
+    };
+    for (uint32_t t = pair; t < tiles; t += pairs) {
+      uint32_t acc = await_done();
+      if (!ok) break;
       const Place q = next;
       const RowCoef row = row_next;
       look_ahead(t + pairs);
-      const uint32_t acc = tmem + (lanes << 16) + buf * kTile + half * kHalf;
       const int64_t m0 = (int64_t)q.tm * kTile + rank * kHalf + lanes;
       const int64_t n0 = (int64_t)q.tn * kTile + half * kHalf;
       const CUtensorMap* out = q.product ? &maps1.out : &maps0.out;
-      auto release = [&] {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) arrive_at(drained + buf * 8);
-      };
-      if constexpr (KIND == kStats) finish_stats(w, acc, row, m0 + lane, n0, release);
+      if constexpr (KIND == kStats) {
+        int part = 0;
+        auto more = [&](uint32_t& at) {
+          if (++part >= w.parts) return false;
+          if (++buf == 2) buf = 0, buf_phase ^= 1;
+          at = await_done();
+          return ok;
+        };
+        finish_stats(w, acc, row, m0 + lane, n0, release, more);
+        if (!ok) break;
+      }
       if constexpr (KIND == kGrads) finish_grads<T>(w, out, slot, acc, row, live, m0, n0, lane, release);
       if constexpr (KIND == kWeights)
         finish_weights<T>(w, w.p[q.product], out, slot, acc, row, rows_of(w.p[q.product], live), m0, n0,
@@ -575,7 +615,8 @@ struct FewShape {
 
 struct FewWork {
   int64_t tokens, vocab;
-  int steps, units, units_each;      // of depth; of words, and at most of one CTA
+  int steps, part_steps;             // of depth, and of one of its parts
+  int units, units_each;             // of words, and at most of one CTA
   int* err_flag;
   const int64_t* targets;            // stats
   RowStat* stats;                    // (CTA, token)
@@ -676,21 +717,24 @@ loss_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
     bool ok = true;
     const uint64_t first = operand_desc(smem_u32(stages), 16);
     for (int u = unit0; ok && u < unit1; u += kFewRows / kUnit) {
-      if (!(ok = wait(&sh, &sh.drained[buf], buf_phase ^ 1, w.err_flag))) break;
-      tc_fence_after();
-      for (int k = 0; k < w.steps; ++k) {
-        if (!(ok = wait(&sh, &sh.full[stage], phase, w.err_flag))) break;
+      for (int k0 = 0; ok && k0 < w.steps; k0 += w.part_steps) {
+        const int k1 = w.steps - k0 > w.part_steps ? k0 + w.part_steps : w.steps;
+        if (!(ok = wait(&sh, &sh.drained[buf], buf_phase ^ 1, w.err_flag))) break;
         tc_fence_after();
-        const uint64_t a = first + stage * (S::kStage / 16), b = a + S::kBytesA / 16;
+        for (int k = k0; k < k1; ++k) {
+          if (!(ok = wait(&sh, &sh.full[stage], phase, w.err_flag))) break;
+          tc_fence_after();
+          const uint64_t a = first + stage * (S::kStage / 16), b = a + S::kBytesA / 16;
 #pragma unroll
-        for (int i = 0; i < kDepth / 16; ++i)
-          mma_one(tmem + buf * NT, a + i * 2, b + i * 2, kIdesc, k > 0 || i > 0);
-        commit_one(&sh.empty[stage]);
-        if (++stage == S::kCount) stage = 0, phase ^= 1;
+          for (int i = 0; i < kDepth / 16; ++i)
+            mma_one(tmem + buf * NT, a + i * 2, b + i * 2, kIdesc, k > k0 || i > 0);
+          commit_one(&sh.empty[stage]);
+          if (++stage == S::kCount) stage = 0, phase ^= 1;
+        }
+        if (!ok) break;
+        commit_one(&sh.done[buf]);
+        if (++buf == 2) buf = 0, buf_phase ^= 1;
       }
-      if (!ok) break;
-      commit_one(&sh.done[buf]);
-      if (++buf == 2) buf = 0, buf_phase ^= 1;
     }
   } else if (warp >= 4) {                             // finished tiles
     int buf = 0;
@@ -700,24 +744,34 @@ loss_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
 #pragma unroll
     for (int c = 0; c < S::kChunks; ++c) run[c] = {-INFINITY, 0.f};
     for (int u = unit0; u < unit1; u += kFewRows / kUnit) {
-      bool ok = lane != 0 || wait(&sh, &sh.done[buf], buf_phase, w.err_flag);
-      ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+      float sums[S::kChunks][32];
+      bool ok = true;
+      for (int k0 = 0; k0 < w.steps; k0 += w.part_steps) {
+        ok = lane != 0 || wait(&sh, &sh.done[buf], buf_phase, w.err_flag);
+        ok = __shfl_sync(0xffffffffu, (int)ok, 0) != 0;
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t acc = tmem + ((uint32_t)part * 32 << 16) + buf * NT;
+#pragma unroll
+        for (int c = 0; c < S::kChunks; ++c) {
+          float v[32];
+          tmem_load32(acc + c * 32, v);
+          tmem_load_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) sums[c][i] = k0 == 0 ? v[i] : sums[c][i] + v[i];
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sh.drained[buf]);
+        if (++buf == 2) buf = 0, buf_phase ^= 1;
+      }
       if (!ok) break;
-      tc_fence_after();
-      const uint32_t acc = tmem + ((uint32_t)part * 32 << 16) + buf * NT;
       // (a part without words of this CTA's holds what an earlier tile left)
       const int64_t word = (int64_t)(u + part) * kUnit + lane;
       const bool mine = u + part < unit1 && word < w.vocab;
 #pragma unroll
       for (int c = 0; c < S::kChunks; ++c) {
-        float v[32];
-        tmem_load32(acc + c * 32, v);
-        tmem_load_wait();
-        if (c == S::kChunks - 1) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sh.drained[buf]);
-        }
+        float (&v)[32] = sums[c];
         if constexpr (GRADS) {
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
@@ -766,7 +820,6 @@ loss_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
           run[c] = join(run[c], {top, sum});
         }
       }
-      if (++buf == 2) buf = 0, buf_phase ^= 1;
     }
     if constexpr (!GRADS) {
 #pragma unroll
@@ -834,6 +887,7 @@ template <class T, bool GRADS>
 ferrum_status run_few(const Matrix<T>& wt, const Matrix<T>& x, int64_t width, FewWork w, int& ctas,
                       bool first, cudaStream_t stream, const char* what) {
   w.steps = (int)ceil_div(width, kDepth), w.units = (int)ceil_div(w.vocab, kUnit);
+  w.part_steps = GRADS ? w.steps : kPartSteps;
   w.units_each = (int)ceil_div(w.units, 2 * pair_count());
   ctas = (int)ceil_div(w.units, w.units_each);
   auto go = [&](auto n) -> ferrum_status {
@@ -887,6 +941,7 @@ ferrum_status fwd(ferrum_device* dev, const ferrum_cross_entropy_args* a, cudaSt
     w.p[0] = product_of(n, v, d), w.count = 1;
     w.err_flag = dev->err_flag, w.targets = a->targets;
     w.stats = stats, w.at_target = at_target;
+    w.parts = (int)ceil_div(w.p[0].steps, kPartSteps);
     if (ferrum_status s = run<T, kStats>(m, m, w, first, stream, what)) return s;
   }
   return finish_loss(stats, parts, at_target, a, stream, what);

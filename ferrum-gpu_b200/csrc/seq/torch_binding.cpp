@@ -872,7 +872,7 @@ ferrum_cross_entropy_args loss_args(const Tensor& x, const Opt& weight, const Op
         " and " + dims(x.sizes()));
   like(weight, x, w.sizes(), "weight");
   if (x.scalar_type() != at::kFloat && d > FERRUM_LOSS_MAX_WIDTH_16)
-    bad("width must be at most 2^20 in 16-bit types, got " + std::to_string(d));
+    bad("width must be at most 2^16 in 16-bit types, got " + std::to_string(d));
   const Tensor& t = required(targets, "targets");
   if (t.scalar_type() != at::kLong)
     bad("targets must be int64, got " + type_name(t.scalar_type()));

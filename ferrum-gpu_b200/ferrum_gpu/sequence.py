@@ -416,7 +416,7 @@ class CrossEntropyGrads(NamedTuple):
 def linear_cross_entropy(x, weight, targets, *, device=None, stream=None) -> CrossEntropyResult:
     """lse[t] = log sum_v exp(x[t] . weight[v]);  loss[t] = lse[t] - x[t] . weight[target[t]].
 
-    x: (..., width), at most 2^20 wide in 16-bit types; weight: (vocabulary, width)
+    x: (..., width), at most 2^16 wide in 16-bit types; weight: (vocabulary, width)
     of x's type; targets: int64 of x's leading shape. loss and lse are float32 of that shape. The logits are
     never kept: a piece at a time lives on chip. A row whose target lies outside
     the vocabulary (-100, say) has no loss: its loss, lse and gradients are 0,

@@ -46,7 +46,7 @@ enum { FERRUM_NORM_RMS = 0, FERRUM_NORM_LAYER = 1 };
 /* Longest sequence of the long convolution. */
 #define FERRUM_LONG_CONV_MAX_LENGTH (1 << 25)
 /* Widest rows of the loss in 16-bit types. */
-#define FERRUM_LOSS_MAX_WIDTH_16 (1 << 20)
+#define FERRUM_LOSS_MAX_WIDTH_16 (1 << 16)
 
 /* A (batch, length, channels) array: element (b, t, d) is at
  * ptr[b * batch_stride + t * row_stride + d]. Single-token calls use
