@@ -22,10 +22,10 @@
 // the next is computed. 74 pairs walk the tiles; dx and dW of a piece share a launch,
 // so that the last wave of one is filled by the other.
 //
-// 8192 x 2048 x 32768 bf16: 715 us forward (1.54 PFLOP/s; cuBLAS takes 702 for the
-// logits alone), 2390 for the gradient (1.38 PFLOP/s over its three products, at the
-// power limit; a library product sustains 1.39). The tensor pipe is busy for 90 to
-// 95 % of the cycles. What it took: one thread issues the products, so descriptors move
+// 8192 x 2048 x 32768 bf16: 725 us forward (1.52 PFLOP/s; cuBLAS takes 702 for the
+// logits alone), 2400 to 2550 for the gradient (1.37 to 1.29 PFLOP/s over its three
+// products, at the power limit; a library product sustains 1.39). The tensor pipe is
+// busy for 87 to 94 % of the cycles. What it took: one thread issues the products, so descriptors move
 // by sums and tiles are numbered by 32 bits (gradient 2755 -> 2350 us); accumulators
 // are read at once and released before anything is stored (16384 x 512 x 32768:
 // 575 -> 386 us); an arrival that orders no memory, since one that does waits for the

@@ -10,10 +10,11 @@
 // data, no block waits for another that might not run.
 //
 // 8 x 2048 x 4096 bf16: 160 us forward, 3.3 TB/s of the 6.5 of a copy (57
-// instructions a value, issue slots 70 % busy, special functions 52 %: five a value
-// are 75 us); its gradient 294 us, 3.2 TB/s (114 instructions, 75 %). float32: 173 us,
-// 6.2 TB/s, and 406, 4.6 TB/s. 1 x 8191 x 2048 bf16: 66 and 104 us, 10 and 32 turns
-// one after the other. 128 registers and 14 to 15 warps an SM in both.
+// instructions a value, issue slots 71 % busy, special functions 52 %: five a value
+// are 75 us); its gradient 293 us, 3.2 TB/s (114 instructions, 74 %). float32: 175 us,
+// 6.1 TB/s, and 414, 4.5 TB/s. 1 x 8191 x 2048 bf16: 67 and 107 us, 10 and 16 turns
+// one after the other. Where a warp has a decay above 1 (recurrence.cuh): 213 and 394,
+// 209 and 462, 85 and 136. 128 registers and 14 to 15 warps an SM in both.
 //
 // Gradient, with G the gradient of the state:  G_t = dout_t + a_{t+1} G_{t+1}. The
 // same backwards over time; the states come from those the forward saved in front
@@ -366,8 +367,8 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 2) recurrence_fwd_kernel(RecAr
       if (lost) show(std::true_type());
     };
     // Behind the sequence's end the state stands still (8 sequences of 0 to 2048 steps x
-    // 4096 bf16: 187 us where warps walk their padding, 121 where they do not; the
-    // gradient 353 and 209).
+    // 4096 bf16: 187 us where warps walk their padding, 123 where they do not; the
+    // gradient 353 and 218).
     auto stand = [&] {
       Factor all[VL];
       float none[VL], h[VL];
