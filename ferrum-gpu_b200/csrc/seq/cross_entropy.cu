@@ -49,7 +49,7 @@ ferrum_status check_loss(const ferrum_device* dev, const ferrum_cross_entropy_ar
   // shrinks it by 1.5e-8 of it each: at 2^16 that is 6e-5 of the logit, and the softmax of one of
   // 2.5 off by a third of float16's rounding, in one direction. (At 2^26 a tile also takes 0.3 of
   // the second that waits are given.)
-  if (a->dtype != FERRUM_F32 && a->width > FERRUM_LOSS_MAX_WIDTH_16)
+  if (bwd && a->dtype != FERRUM_F32 && a->width > FERRUM_LOSS_BWD_MAX_WIDTH_16)
     return invalid(what, "width must be at most 2^16 in 16-bit types");
   if (bounded_product({a->tokens, a->width}) < 0 || bounded_product({a->vocab, a->width}) < 0)
     return invalid(what, "tokens * width or vocab * width is too large");

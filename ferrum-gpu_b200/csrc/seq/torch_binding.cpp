@@ -871,8 +871,6 @@ ferrum_cross_entropy_args loss_args(const Tensor& x, const Opt& weight, const Op
     bad("weight must be (vocabulary, width) with the width of x, got shapes " + dims(w.sizes()) +
         " and " + dims(x.sizes()));
   like(weight, x, w.sizes(), "weight");
-  if (x.scalar_type() != at::kFloat && d > FERRUM_LOSS_MAX_WIDTH_16)
-    bad("width must be at most 2^16 in 16-bit types, got " + std::to_string(d));
   const Tensor& t = required(targets, "targets");
   if (t.scalar_type() != at::kLong)
     bad("targets must be int64, got " + type_name(t.scalar_type()));
@@ -915,6 +913,8 @@ py::tuple linear_cross_entropy_backward(const Opt& dloss, const Opt& xo, const O
                                         const py::object& device, const py::object& stream) {
   const Tensor& x = activation(xo, "x", 0);
   auto a = loss_args(x, weight, targets);
+  if (x.scalar_type() != at::kFloat && x.size(-1) > FERRUM_LOSS_BWD_MAX_WIDTH_16)
+    bad("width must be at most 2^16 in 16-bit types, got " + std::to_string(x.size(-1)));
   required(lse, "lse");
   a.lse = (float*)per_token(lse, x, "lse");
   a.dloss = per_token(dloss, x, "dloss"), a.dlse = per_token(dlse, x, "dlse");

@@ -416,8 +416,8 @@ class CrossEntropyGrads(NamedTuple):
 def linear_cross_entropy(x, weight, targets, *, device=None, stream=None) -> CrossEntropyResult:
     """lse[t] = log sum_v exp(x[t] . weight[v]);  loss[t] = lse[t] - x[t] . weight[target[t]].
 
-    x: (..., width), at most 2^16 wide in 16-bit types; weight: (vocabulary, width)
-    of x's type; targets: int64 of x's leading shape. loss and lse are float32 of that shape. The logits are
+    x: (..., width); weight: (vocabulary, width) of x's type; targets: int64 of
+    x's leading shape. loss and lse are float32 of that shape. The logits are
     never kept: a piece at a time lives on chip. A row whose target lies outside
     the vocabulary (-100, say) has no loss: its loss, lse and gradients are 0,
     whatever its values. Workspace: 8 bytes for each token and 128 words, and a
@@ -433,7 +433,7 @@ def linear_cross_entropy_backward(dloss, x, weight, targets, lse, *, dlse=None, 
     logits are computed again, a piece of the vocabulary at a time, for the tokens
     that have a loss. dx and dweight have x's type.
 
-    In 16-bit types the logits' gradients are rounded to 16 bits between the
+    16-bit rows are at most 2^16 wide. In 16-bit types the logits' gradients are rounded to 16 bits between the
     products, whose operands they are: dx and dweight are up to 1.4 times as far
     from the exact ones as rounding the outputs leaves them (in float16, dx of
     tokens whose weight is less than 2^-18 of the largest is farther). Workspace:

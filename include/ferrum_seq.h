@@ -45,8 +45,8 @@ enum { FERRUM_NORM_RMS = 0, FERRUM_NORM_LAYER = 1 };
 #define FERRUM_RECURRENCE_SAVE_STEPS 16
 /* Longest sequence of the long convolution. */
 #define FERRUM_LONG_CONV_MAX_LENGTH (1 << 25)
-/* Widest rows of the loss in 16-bit types. */
-#define FERRUM_LOSS_MAX_WIDTH_16 (1 << 16)
+/* Widest rows of the loss's gradient in 16-bit types. */
+#define FERRUM_LOSS_BWD_MAX_WIDTH_16 (1 << 16)
 
 /* A (batch, length, channels) array: element (b, t, d) is at
  * ptr[b * batch_stride + t * row_stride + d]. Single-token calls use
@@ -273,12 +273,11 @@ ferrum_status ferrum_dropout_bwd(ferrum_device *dev, const ferrum_dropout_args *
  * Softmax cross entropy of rows against a vocabulary matrix:
  *   l[t,v] = sum_d x[t,d] * weight[v,d]
  *   lse[t] = log(sum_v exp(l[t,v]));  loss[t] = lse[t] - l[t, target[t]]
- * x, weight, dx and dweight have type `dtype`. 16-bit rows are at most
- * FERRUM_LOSS_MAX_WIDTH_16 wide. The logits are never stored as a whole. A row
- * whose target lies outside [0, vocab) has no loss: its loss, lse and gradients
- * are 0, whatever its values.
- * In 16-bit types the gradient rounds the logits' gradients to 16 bits between
- * its products: dx and dweight are up to 1.4 times as far from the exact ones as
+ * x, weight, dx and dweight have type `dtype`. The logits are never stored as a
+ * whole. A row whose target lies outside [0, vocab) has no loss: its loss, lse and
+ * gradients are 0, whatever its values.
+ * In 16-bit types the gradient takes rows of up to FERRUM_LOSS_BWD_MAX_WIDTH_16
+ * values and rounds the logits' gradients to 16 bits between its products: dx and dweight are up to 1.4 times as far from the exact ones as
  * their own rounding leaves them.
  * Workspace of the loss: 8 bytes for each token and 128 words, and a copy of x or
  * weight whose rows do not begin at multiples of 16 bytes. Of the gradient: the

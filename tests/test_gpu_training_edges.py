@@ -497,25 +497,23 @@ def test_loss_of_wide_rows_keeps_float32(tokens, width, vocab, dtype):
         assert ((got.double() - ref).norm() / ref.norm()).item() <= 1e-6
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
-def test_loss_refuses_rows_too_wide_for_16_bits(dtype):
-    """The widest rows, in 64 parts of 64 additions, each cut off by a unit of 2^-23 at most,
-    and 63 rounded sums: below 256 units of 2^-24 of the largest partial sum (within 4 times
-    the logits' size). One more value is refused."""
-    n = 1 << 16
-    x, w = rnd(1, 3, n + 1, dtype=dtype), rnd(2, 5, n + 1, dtype=dtype, std=2.0 ** -8)
+def test_loss_gradient_refuses_rows_too_wide_for_16_bits(dtype):
+    """Rows beyond 2^16 values: the loss in parts of 64 additions, each cut off by a unit of
+    2^-23 at most, and a rounded sum for each part: below 512 units of 2^-24 of the largest
+    partial sum (within 4 times the logits' size). The gradient does not take them."""
+    n = (1 << 16) + 8
+    x, w = rnd(1, 3, n, dtype=dtype), rnd(2, 5, n, dtype=dtype, std=2.0 ** -8)
     t = torch.tensor([0, 4, 2], device="cuda")
-    with pytest.raises(ValueError, match="width must be at most 2.16 in 16-bit types"):
-        sq.linear_cross_entropy(x, w, t)
-    with pytest.raises(ValueError, match="width must be at most 2.16 in 16-bit types"):
-        sq.linear_cross_entropy_backward(None, x, w, t, torch.zeros(3, device="cuda"))
-    r = sq.linear_cross_entropy(x[:, :n], w[:, :n], t)
-    logits = x[:, :n].double() @ w[:, :n].double().t()
-    off = 4 * 256 * EPS * logits.abs().amax(1)
+    r = sq.linear_cross_entropy(x, w, t)
+    logits = x.double() @ w.double().t()
+    off = 4 * 512 * EPS * logits.abs().amax(1)
     within(r.lse, torch.logsumexp(logits, 1), off)
     within(r.loss, torch.logsumexp(logits, 1) - logits[torch.arange(3, device="cuda"), t], 2 * off)
+    with pytest.raises(ValueError, match="width must be at most 2.16 in 16-bit types"):
+        sq.linear_cross_entropy_backward(torch.ones(3, device="cuda"), x, w, t, r.lse)
+    sq.linear_cross_entropy_backward(torch.ones(3, device="cuda"), x[:, :-8], w[:, :-8], t, r.lse)
     dev = capi.DeviceHandle(0)
-    for name in ("ferrum_linear_cross_entropy", "ferrum_linear_cross_entropy_bwd"):
-        block = capi.SEQ_SIGNATURES[name]
-        args = block(struct_size=ctypes.sizeof(block), dtype=1, tokens=1, width=n + 1, vocab=1)
-        assert getattr(capi.lib(), name)(dev.ptr, ctypes.byref(args), None) == capi.FERRUM_ERR_INVALID_ARG
-        assert "2^16" in capi.last_error()
+    block = capi.SEQ_SIGNATURES["ferrum_linear_cross_entropy_bwd"]
+    args = block(struct_size=ctypes.sizeof(block), dtype=1, tokens=1, width=n, vocab=1)
+    assert capi.lib().ferrum_linear_cross_entropy_bwd(dev.ptr, ctypes.byref(args), None) == capi.FERRUM_ERR_INVALID_ARG
+    assert "2^16" in capi.last_error()
