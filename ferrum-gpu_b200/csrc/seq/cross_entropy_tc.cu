@@ -810,7 +810,10 @@ loss_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant
           const float shift = shift_of(top), shift2 = shift * kLog2e;
           if (__any_sync(0xffffffffu, fabsf(shift) > kFar)) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = ex2((v[i] - __shfl_sync(0xffffffffu, shift, i)) * kLog2e);
+            for (int i = 0; i < 32; ++i) {         // (other tokens as below)
+              const float from = __shfl_sync(0xffffffffu, shift, i), from2 = __shfl_sync(0xffffffffu, shift2, i);
+              v[i] = ex2(fabsf(from) > kFar ? (v[i] - from) * kLog2e : fmaf(v[i], kLog2e, -from2));
+            }
           } else {
 #pragma unroll
             for (int i = 0; i < 32; ++i)

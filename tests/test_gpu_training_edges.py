@@ -275,6 +275,22 @@ def test_loss_of_logits_near_the_largest(tokens, dtype):
             within(got, ref, 2 * e)
 
 
+@pytest.mark.parametrize("dtype", [F32, torch.bfloat16])
+@pytest.mark.parametrize("tokens", [3, 40, 300])
+def test_far_logits_change_no_other_row(tokens, dtype):
+    """A row's loss does not depend on what lies in its neighbours."""
+    x, w, t = loss_case(tokens, 24, 500, dtype, 0.0)
+    w[:, 23] = 0
+    w[7, 23] = 2.0 ** 64
+    x[:, 23] = 0
+    want = sq.linear_cross_entropy(x, w, t)
+    far = torch.arange(tokens, device="cuda") % 3 == 1
+    x[far, 23] = 0.75 * 2.0 ** 64
+    got = sq.linear_cross_entropy(x, w, t)
+    assert (got.lse[far] > 2e38).all()
+    assert torch.equal(got.lse[~far], want.lse[~far]) and torch.equal(got.loss[~far], want.loss[~far])
+
+
 # ---------------------------------------------------------------- long sums
 
 @pytest.mark.parametrize("tokens,width,vocab,masked", [(65536, 64, 256, 0.0), (50001, 40, 77, 0.4),
