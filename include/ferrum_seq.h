@@ -277,8 +277,9 @@ ferrum_status ferrum_dropout_bwd(ferrum_device *dev, const ferrum_dropout_args *
  * whole. A row whose target lies outside [0, vocab) has no loss: its loss, lse and
  * gradients are 0, whatever its values.
  * In 16-bit types the gradient takes rows of up to FERRUM_LOSS_BWD_MAX_WIDTH_16
- * values and rounds the logits' gradients to 16 bits between its products: dx and dweight are up to 1.4 times as far from the exact ones as
- * their own rounding leaves them.
+ * values and rounds the logits' gradients to 16 bits between its products: dx and
+ * dweight are up to 1.4 times as far from the exact ones as their own rounding
+ * leaves them.
  * Workspace of the loss: 8 bytes for each token and 128 words, and a copy of x or
  * weight whose rows do not begin at multiples of 16 bytes. Of the gradient: the
  * logits' gradients of a piece of the vocabulary (256 MiB, or 4096 words if that
